@@ -452,6 +452,68 @@ int tq_decode_streams(const tq_decode_layer *layer, long long tokens, long long 
 int tq_decode_append(const tq_decode_layer *layer, const void *k_new, const void *v_new, long long k_new_stride, long long v_new_stride,
                      long long evict, long long put, long long packed_slot, void *stream);
 
+/*
+ * Attention of any number of query tokens per sequence over packed tokens and uncompressed ones, softmax(scale * q K^T) V, without
+ * de-quantising (the reference composes it from decompress_kv, compressors_v3.py:205-233, and the model's attention): verification of
+ * drafted tokens over a cache, cross attention to an encoder's compressed states.
+ *   queries     query head j, token i of sequence b at element b * q_batch + j * q_head + i * q_token, head_dim elements in a row; head j
+ *               reads kv head j / group.  out: dense [batch, heads * group, n_queries, head_dim], same element type
+ *   k_idx ...   packed tokens as tq_compress leaves them, packed_row_stride slots a (sequence, kv head), `tokens` of which count
+ *   window      uncompressed tokens behind them, seen like them; drafts: uncompressed tokens that belong to the queries
+ *               (k == v == NULL and tokens == 0 where there are none; at most 65536 of each)
+ *   lengths     NULL, or on the device: how many keys (packed, then window) of each sequence count (below zero: none; more than there are: all)
+ *   mask        NULL, or a truth value per key (packed, then window) of each sequence, mask_stride >= tokens + window.tokens apart
+ *   tree        NULL: query i sees drafts 0 ... i (then drafts.tokens == n_queries); otherwise [n_queries, drafts.tokens] truth values,
+ *               tree_batch apart for each sequence (0: one for all)
+ *   weights     NULL, or float32 [batch * heads, weights_stride]: to the value of every key (packed, then window) the weights that the
+ *               row's queries give it are added, in an order that does not change
+ * A query that sees no key gets zeros.  Infinities and NaN in masked or uncounted keys have no effect on the queries that do not see them.
+ * Element type dtype for queries, results, window and drafts; head_dim 8 ... 256; strides in elements, any alignment of the element type.
+ * tq_attend_many_scratch: float32 values of scratch (16-byte aligned, not shared by launches that can overlap in time), or an error.
+ */
+typedef struct tq_plain_tokens {
+    const void *k, *v;
+    long long k_batch, k_head, k_token, v_batch, v_head, v_token;
+    long long tokens;
+} tq_plain_tokens;
+typedef struct tq_attend_request {
+    const void *queries;
+    void *out;
+    const uint8_t *k_idx;
+    const uint16_t *k_norms;
+    const uint8_t *v_idx;
+    const uint16_t *v_norms;
+    const void *table_k, *table_v;
+    const int32_t *lengths;
+    const uint8_t *mask, *tree;
+    float *weights;
+    tq_plain_tokens window, drafts;
+    long long q_batch, q_head, q_token, mask_stride, tree_batch, weights_stride;
+    long long batch, heads, group, n_queries, tokens, packed_row_stride;
+    float scale;
+    int head_dim, dtype, bits_k, bits_v;
+} tq_attend_request;
+long long tq_attend_many_scratch(const tq_attend_request *request);
+int tq_attend_many(const tq_attend_request *request, float *scratch, long long scratch_floats, void *stream);
+
+/*
+ * Eviction: of the `tokens` packed tokens of every row the `keep` with the largest weights stay, in their order; of equal weights the
+ * first ones (NaN counts as larger than every number).  No counterpart in the reference, which keeps every token.
+ *   from, to    packed stores of packed_row_stride slots a row (0: dense, `tokens` and `keep`); they must not overlap
+ *   weights     [rows, weights_stride] float32: the packed tokens', then `rest` of tokens that all stay (at most 65536)
+ *   weights_out [rows, weights_out_stride]: the weights of what stays, keep + rest a row
+ *   kept        [rows, keep] slot in `from` of every slot of `to`, ascending
+ */
+typedef struct tq_packed_store {
+    uint8_t *k_idx;
+    uint16_t *k_norms;
+    uint8_t *v_idx;
+    uint16_t *v_norms;
+    long long packed_row_stride;
+} tq_packed_store;
+int tq_evict(const tq_packed_store *from, const tq_packed_store *to, const float *weights, long long weights_stride, float *weights_out,
+             long long weights_out_stride, long long rest, long long rows, long long tokens, long long keep, int head_dim, int bits_k, int bits_v, long long *kept, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,8 +27,8 @@ FAST_INTERFACE = 3                  # INTERFACE there: what init and the functio
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
-           "tq_qjl_scores.hip", "tq_decode.hip", "tq_wide.hip", "tq_host.cpp")
-HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", os.path.join("..", "..", "include", "tqamd.h"))
+           "tq_qjl_scores.hip", "tq_decode.hip", "tq_wide.hip", "tq_many.hip", "tq_evict.hip", "tq_host.cpp")
+HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", "tq_many.h", "tq_many_kernel.h", os.path.join("..", "..", "include", "tqamd.h"))
 GPU_ARCH = "gfx950"
 
 TQ_F32, TQ_F16, TQ_BF16 = 0, 1, 2
@@ -205,6 +205,23 @@ class TqDecodeLayer(ctypes.Structure):
     ]
 
 
+class TqPlainTokens(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [(n, ctypes.c_longlong) for n in (
+        "k_batch", "k_head", "k_token", "v_batch", "v_head", "v_token", "tokens")]
+
+
+class TqAttendRequest(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("queries", "out", "k_idx", "k_norms", "v_idx", "v_norms", "table_k", "table_v", "lengths", "mask", "tree", "weights")]
+                + [("window", TqPlainTokens), ("drafts", TqPlainTokens)]
+                + [(n, ctypes.c_longlong) for n in ("q_batch", "q_head", "q_token", "mask_stride", "tree_batch", "weights_stride",
+                                                    "batch", "heads", "group", "n_queries", "tokens", "packed_row_stride")]
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int) for n in ("head_dim", "dtype", "bits_k", "bits_v")])
+
+
+class TqPackedStore(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_idx", "k_norms", "v_idx", "v_norms")] + [("packed_row_stride", ctypes.c_longlong)]
+
+
 EXPORTS = (
     "tq_abi_version", "tq_status_string", "tq_device_count", "tq_bytes_per_vector",
     "tq_decision_thresholds", "tq_table_bytes", "tq_table_build", "tq_table_check", "tq_table_quantize_host",
@@ -215,6 +232,7 @@ EXPORTS = (
     "tq_attend_prepare", "tq_attend_merge", "tq_append_token", "tq_attend_step",
     "tq_decode_supported", "tq_decode_scratch_floats", "tq_decode_attend", "tq_decode_attend_spread", "tq_decode_attend_cached", "tq_decode_streams", "tq_decode_append",
     "tq_compress_layer", "tq_restore_layer",
+    "tq_attend_many_scratch", "tq_attend_many", "tq_evict",
 )
 
 _lib = None
@@ -277,8 +295,12 @@ def lib() -> ctypes.CDLL:
     L.tq_decode_append.argtypes = [vp, vp, vp, ll, ll, ll, ll, ll, vp]
     L.tq_compress_layer.argtypes = [vp, vp, ci, ll, ll, ll, ll, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, vp]
     L.tq_restore_layer.argtypes = [vp, vp, vp, vp, ll, ll, ll, ll, vp, vp, ci, ci, ci, vp, vp, ll, ll, ll, vp, vp, ci, vp, vp]
+    L.tq_attend_many_scratch.restype = ll
+    L.tq_attend_many_scratch.argtypes = [vp]
+    L.tq_attend_many.argtypes = [vp, vp, ll, vp]
+    L.tq_evict.argtypes = [vp, vp, vp, ll, vp, ll, ll, ll, ll, ll, ci, ci, ci, vp, vp]
     for name in EXPORTS:
-        if name not in ("tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
+        if name not in ("tq_attend_many_scratch", "tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
             getattr(L, name).restype = ci
     _lib = L
     return L
@@ -700,6 +722,178 @@ def restore_layer(packed_k, packed_v, tokens: int, table_k: torch.Tensor, table_
         _drop_workspace(dev, stream)
     check(rc, "tq_restore_layer")
     return full_k, full_v
+
+
+MANY_SCRATCH = 1 << 28          # float32 values of scratch (1 GiB) above which a call of attend_many takes its queries in parts
+
+
+def _plain_tokens(pair, D: int) -> TqPlainTokens:
+    """Uncompressed keys and values [B,H,n,D] as the library sees them."""
+    if pair is None or pair[0].shape[2] == 0:
+        return TqPlainTokens()
+    k, v = pair
+    return TqPlainTokens(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k.shape[2])
+
+
+def _packed_pairs(packed, B: int, H: int, tokens: int, D: int, bits):
+    """The pairs (idx_bytes, vec_norms) of keys and values with one row stride, or ValueError where they are not [B,H,tokens,...]."""
+    strides, out = [], []
+    for (idx, nrm), b in zip(packed, bits):
+        if tuple(idx.shape) != (B, H, tokens, _packed_width(D, b)) or tuple(nrm.shape) != (B, H, tokens) or idx.dtype != torch.uint8 or nrm.dtype != torch.float16:
+            raise ValueError(f"packed tokens {tuple(idx.shape)} {idx.dtype} / {tuple(nrm.shape)} {nrm.dtype} are not {tokens} vectors of {D} elements at {b} bits "
+                             f"for each of {B} x {H} heads")
+        out.append((idx, nrm))
+        strides.append(packed_row_stride(idx, nrm))
+    if None in strides or strides[0] != strides[1]:
+        out, strides = [(idx.contiguous(), nrm.contiguous()) for idx, nrm in out], [0, 0]
+    return out, strides[0]
+
+
+def _as_truth(mask: torch.Tensor, what: str) -> torch.Tensor:
+    if mask.dtype != torch.bool:
+        raise ValueError(f"{what} must be of truth values (torch.bool), got {mask.dtype}")
+    return mask.contiguous().view(torch.uint8)
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def attend_many(queries: torch.Tensor, packed, tokens: int, tables, bits, window=None, drafts=None, lengths: Optional[torch.Tensor] = None,
+                mask: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                scale: Optional[float] = None) -> torch.Tensor:
+    """tq_attend_many: softmax(scale q K^T) V of queries [B,Hq,T,D] over `tokens` packed tokens ((k idx_bytes, vec_norms), (v idx_bytes, vec_norms), each
+    [B,H,tokens,..], or None), the window (keys, values [B,H,n,D], or None) behind them and the drafts (the same) -> [B,Hq,T,D] of the queries' type.
+    lengths [B] and mask [B, tokens + n] (truth values) say which of packed tokens and window count, tree [T, drafts] or [B, T, drafts] which
+    drafts a query sees (None: draft j if j <= i); what a key receives is added to weights [B,H,tokens + n] (float32)."""
+    _require_gpu(queries, "queries")
+    B, Hq, T, D = queries.shape
+    dev, dtype = queries.device, queries.dtype
+    code = dtype_code(dtype)
+    sides = [s for s in (window, drafts) if s is not None]
+    if packed is None and not sides:
+        raise ValueError("attention over nothing: neither packed tokens nor uncompressed ones")
+    H = packed[0][0].shape[1] if packed is not None else sides[0][0].shape[1]
+    if H == 0 or Hq % H:
+        raise ValueError(f"{Hq} query heads do not divide over {H} kv heads")
+    for k, v in sides:
+        if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, H, D):
+            raise ValueError(f"uncompressed keys {tuple(k.shape)} and values {tuple(v.shape)} do not go with queries {tuple(queries.shape)} over {H} kv heads")
+        if k.shape[2] > 65536:
+            raise ValueError(f"{k.shape[2]} uncompressed tokens: at most 65536")
+    n_win, n_draft = (0 if s is None else s[0].shape[2] for s in (window, drafts))
+    total = tokens + n_win
+    for name, t in (("packed tokens", packed[0][0] if packed is not None else None), ("packed values", packed[1][0] if packed is not None else None),
+                    ("codec table", tables[0]), ("codec table", tables[1]), ("lengths", lengths), ("mask", mask), ("tree mask", tree), ("weights", weights),
+                    *(("uncompressed tokens", t) for s in sides for t in s)):
+        if t is not None and t.device != dev:
+            raise TqError(f"{name} on {t.device}, queries on {dev}")
+    for table, b in zip(tables, bits):
+        check_table(table, D, b)
+    if any(t.dtype != dtype for s in sides for t in s):      # one element type for all: the widest
+        wide = lambda s: None if s is None else tuple(t.float() for t in s)  # noqa: E731
+        return attend_many(queries.float(), packed, tokens, tables, bits, wide(window), wide(drafts), lengths, mask, tree, weights, scale).to(dtype)
+    keep = []           # what the launches read must live until they are queued
+    r = TqAttendRequest()
+    if packed is not None and tokens:
+        pairs, r.packed_row_stride = _packed_pairs(packed, B, H, tokens, D, bits)
+        keep.append(pairs)
+        (r.k_idx, r.k_norms), (r.v_idx, r.v_norms) = ((i.data_ptr(), n.data_ptr()) for i, n in pairs)
+    dense = lambda s: None if s is None else tuple(t if t.stride(3) == 1 or t.numel() == 0 else t.contiguous() for t in s)  # noqa: E731
+    window, drafts = dense(window), dense(drafts)
+    r.window, r.drafts = _plain_tokens(window, D), _plain_tokens(drafts, D)
+    if lengths is not None:
+        if tuple(lengths.shape) != (B,) or lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
+            raise ValueError(f"lengths must be one whole number per sequence, [{B}]; got {tuple(lengths.shape)} {lengths.dtype}")
+        lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, total).to(torch.int32)).contiguous()
+        r.lengths = lengths.data_ptr()
+    if mask is not None:
+        if tuple(mask.shape) != (B, total):
+            raise ValueError(f"mask must say for each of {total} keys of {B} sequences whether it counts; got {tuple(mask.shape)}")
+        mask = _as_truth(mask, "mask")
+        r.mask, r.mask_stride = mask.data_ptr(), total
+    if weights is not None:
+        if tuple(weights.shape) != (B, H, total) or weights.dtype != torch.float32 or not weights.is_cuda:
+            raise ValueError(f"weights must be float32 [{B}, {H}, {total}]; got {tuple(weights.shape)} {weights.dtype}")
+        sb, sh, ss = weights.stride()
+        if (total > 1 and ss != 1) or (B > 1 and H > 1 and sb != H * sh) or (B * H > 1 and (sh if H > 1 else sb) < total):
+            raise ValueError("weights must be rows of consecutive values, a fixed number apart (sums are added in place)")
+        r.weights, r.weights_stride = weights.data_ptr(), sh if H > 1 else sb
+    if tree is None:
+        if n_draft and n_draft != T:
+            raise ValueError(f"{n_draft} drafted tokens and {T} queries: a tree mask has to say who sees whom")
+    else:
+        if tuple(tree.shape) not in ((T, n_draft), (B, T, n_draft)):
+            raise ValueError(f"tree mask must be [{T}, {n_draft}] or [{B}, {T}, {n_draft}]; got {tuple(tree.shape)}")
+        tree = _as_truth(tree, "tree mask")
+    if not queries.is_contiguous() and queries.stride(3) != 1:
+        queries = queries.contiguous()
+    r.batch, r.heads, r.group, r.n_queries, r.tokens = B, H, Hq // H, T, tokens
+    r.q_batch, r.q_head, r.q_token = queries.stride()[:3]
+    r.table_k, r.table_v = (t.data_ptr() for t in tables)
+    r.scale = D ** -0.5 if scale is None else float(scale)
+    r.head_dim, r.dtype, (r.bits_k, r.bits_v) = D, code, bits
+    r.queries = queries.data_ptr()
+    if tree is not None:
+        r.tree, r.tree_batch = tree.data_ptr(), T * n_draft if tree.dim() == 3 else 0
+    floats = int(lib().tq_attend_many_scratch(ctypes.byref(r)))
+    if floats < 0:
+        check(floats, "tq_attend_many_scratch")
+    if floats > MANY_SCRATCH and T > 1:
+        part = max(1, T * MANY_SCRATCH // floats)
+        if n_draft and tree is None:
+            tree = torch.ones(T, n_draft, dtype=torch.bool, device=dev).tril_()
+        elif tree is not None:
+            tree = tree.view(torch.bool)
+        cut = lambda lo: None if tree is None else tree[..., lo:lo + part, :]  # noqa: E731
+        return torch.cat([attend_many(queries[:, :, lo:lo + part], packed, tokens, tables, bits, window, drafts, lengths,
+                                      None if mask is None else mask.view(torch.bool), cut(lo), weights, scale) for lo in range(0, T, part)], 2)
+    with _on(dev):
+        out = torch.empty((B, Hq, T, D), dtype=dtype, device=dev)
+        r.out = out.data_ptr()
+        if out.numel():
+            stream = _stream_handle(dev)
+            scratch = step_scratch(dev, stream, floats)
+            if scratch is None:
+                scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+            check(lib().tq_attend_many(ctypes.byref(r), scratch.data_ptr(), scratch.numel(), stream), "tq_attend_many")
+    return out
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def evict(packed, tokens: int, bits, D: int, weights: torch.Tensor, keep: int, into=None, weights_into: Optional[torch.Tensor] = None):
+    """tq_evict: ((k idx_bytes, vec_norms), (v ...)) of the `keep` of `tokens` packed tokens of every row with the largest weights, their weights (and those behind the
+    packed tokens', which stay) and their slots [B,H,keep].  into / weights_into: stores [B,H,capacity,..] to write the first slots of."""
+    (k_idx, k_nrm), (v_idx, v_nrm) = packed
+    B, H = k_idx.shape[:2]
+    dev = k_idx.device
+    _require_gpu(k_idx, "packed tokens")
+    if isinstance(keep, bool) or int(keep) != keep or not 0 <= keep <= tokens:
+        raise ValueError(f"keep must be a whole number from 0 to {tokens}, got {keep!r}")
+    keep = int(keep)
+    if weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H) or weights.shape[2] < tokens or weights.dtype != torch.float32:
+        raise ValueError(f"weights must be float32 [{B}, {H}, {tokens} or more]; got {tuple(weights.shape)} {weights.dtype}")
+    for t in (k_nrm, v_idx, v_nrm, weights):
+        if t.device != dev:
+            raise TqError(f"packed tokens and weights on {dev} and {t.device}")
+    pairs, prs = _packed_pairs(packed, B, H, tokens, D, bits)
+    rest = weights.shape[2] - tokens
+    if rest > 65536:
+        raise ValueError(f"{rest} tokens behind the packed ones: at most 65536")
+    sb, sh, ss = weights.stride()
+    if ss != 1 or (B > 1 and H > 1 and sb != H * sh) or (B * H > 1 and (sh if H > 1 else sb) < weights.shape[2]):
+        weights = weights.contiguous()
+        sb, sh, ss = weights.stride()
+    with _on(dev):
+        if into is None:
+            into = tuple((torch.empty((B, H, keep, i.shape[3]), dtype=torch.uint8, device=dev), torch.empty((B, H, keep), dtype=torch.float16, device=dev)) for i, _ in pairs)
+        if weights_into is None:
+            weights_into = torch.empty((B, H, keep + rest), dtype=torch.float32, device=dev)
+        kept = torch.empty((B, H, keep), dtype=torch.int64, device=dev)
+        store = lambda p, stride: TqPackedStore(p[0][0].data_ptr(), p[0][1].data_ptr(), p[1][0].data_ptr(), p[1][1].data_ptr(), stride)  # noqa: E731
+        source, target = store(pairs, prs), store(into, into[0][0].shape[2])
+        check(lib().tq_evict(ctypes.byref(source), ctypes.byref(target), weights.data_ptr(), sh if H > 1 else sb, weights_into.data_ptr(), weights_into.shape[2], rest,
+                             B * H, tokens, keep, D, *bits, kept.data_ptr(), _stream_handle(dev)), "tq_evict")
+    return into, weights_into, kept
 
 
 def compress_into(states: torch.Tensor, table: torch.Tensor, bits: int,

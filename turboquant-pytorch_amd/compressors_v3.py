@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import functools
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -336,6 +336,57 @@ class TurboQuantV3:
             return None
         return _native.restore_layer((ck["idx_bytes"], ck["vec_norms"]), (cv["idx_bytes"], cv["vec_norms"]), split_at, kc.table(device),
                                      vc.table(device), kc.bits, vc.bits, k_win, v_win, None, 0, (shape, ck["shape"]))
+
+    def _packed_pairs(self, compressed_k: dict, compressed_v: dict):
+        """The dictionaries of compress_kv as the attention kernels take them: packed pairs (None: nothing is packed), their number of tokens, the window."""
+        shape, split_at = tuple(compressed_k["shape"]), compressed_k["split_at"]
+        if tuple(compressed_v["shape"]) != shape or compressed_v["split_at"] != split_at or (compressed_k["compressed"] is None) != (compressed_v["compressed"] is None):
+            raise ValueError("the dictionaries are not keys and values of the same tokens")
+        if shape[3] != self.head_dim:
+            raise ValueError(f"compressed for head dimension {shape[3]}, this codec is for {self.head_dim}")
+        B, H, S, D = shape
+        window = (compressed_k["fp16"], compressed_v["fp16"])
+        if compressed_k["compressed"] is None:
+            return None, 0, window
+        pairs = []
+        for c, comp in ((compressed_k["compressed"], self.key_compressor), (compressed_v["compressed"], self.val_compressor)):
+            width = math.ceil(D / (8 // comp.bits))
+            pairs.append((c["idx_bytes"].reshape(B, H, split_at, width), c["vec_norms"].reshape(B, H, split_at)))
+        return tuple(pairs), split_at, None if S == split_at else window
+
+    def attend_kv(self, query_states: torch.Tensor, compressed_k: dict, compressed_v: dict, lengths: Optional[torch.Tensor] = None,
+                  mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(scale * q K^T) V of any number of query tokens, [B,Hq,T,D] -> [B,Hq,T,D] in the queries' dtype, over what compress_kv made of keys and
+        values [B,H,S,D] -- attention to `decompress_kv` of the two, read from the packed form.  Cross attention: an encoder's states are
+        compressed once and attended to by every decoder step.  Query head j uses kv head j // (Hq / H); every query sees every key that counts.
+        lengths [B] (whole numbers): the first so many keys of each sequence count; mask [B,S] (truth values): those that are true do.  A sequence
+        of which no key counts gets zeros, and what lies in keys that do not count has no effect.
+        weights [B,H,S] (float32): what every key receives, summed over the query heads and tokens that read it, is added in place.
+        scale: D ** -0.5 by default.  Not differentiable."""
+        kc, vc, device = self.key_compressor, self.val_compressor, query_states.device
+        packed, tokens, window = self._packed_pairs(compressed_k, compressed_v)
+        return _native.attend_many(query_states, packed, tokens, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), window, None, lengths, mask, None,
+                                   weights, scale)
+
+    def evict_kv(self, compressed_k: dict, compressed_v: dict, weights: torch.Tensor, keep: int) -> Tuple[dict, dict, torch.Tensor, torch.Tensor]:
+        """Thin out what compress_kv made: of the packed tokens of every (sequence, kv head) the `keep` with the largest weights stay, in their order, the
+        window stays whole.  weights [B,H,S] float32, for instance what `attend_kv(weights=)` has summed; of equal ones the first tokens
+        stay, NaN counts as larger than every number.  Returns new dictionaries, the weights [B,H,keep + window] of what stays, and the
+        packed slots it had [B,H,keep] (int64).  With no more than `keep` packed tokens everything stays."""
+        kc, vc = self.key_compressor, self.val_compressor
+        packed, tokens, _ = self._packed_pairs(compressed_k, compressed_v)
+        B, H, S, D = compressed_k["shape"]
+        if tuple(weights.shape) != (B, H, S):
+            raise ValueError(f"weights must be [{B}, {H}, {S}], got {tuple(weights.shape)}")
+        if packed is None:
+            return dict(compressed_k), dict(compressed_v), weights.clone(), torch.empty((B, H, 0), dtype=torch.int64, device=weights.device)
+        (k, v), left, kept = _native.evict(packed, tokens, (kc.bits, vc.bits), D, weights, min(keep, tokens) if keep >= 0 else keep)
+        keep = kept.shape[2]
+        out = []
+        for c, (idx, nrm) in ((compressed_k, k), (compressed_v, v)):
+            out.append({"compressed": {"idx_bytes": idx, "vec_norms": nrm, "shape": (B, H, keep, D), "idx_pad": c["compressed"]["idx_pad"]},
+                        "fp16": c["fp16"], "shape": (B, H, S - tokens + keep, D), "split_at": keep})
+        return out[0], out[1], left, kept
 
     def memory_bytes(self, B: int, H: int, S: int) -> dict:
         """Bytes stored including the uncompressed window (compressors_v3.py:235-265)."""

@@ -1,0 +1,169 @@
+// Attention of several query tokens over a packed history and uncompressed tokens (tq_many.hip): what its kernels and the
+// sources that instantiate them share.
+//
+// A row is a (sequence, kv head); its M = group * queries query vectors are worked on in tiles of 32, the columns of a 32 x 32 matrix
+// product.  With q' = Pi_k q, logit(t, m) = norm_t * sum_j level[code_tj] q'_mj, so the keys are never turned back: the product runs over
+// the levels themselves.  Values the same way: sum_t p_tm norm_t level[code_tj] is turned by Pi_v once per query, at the end.
+#pragma once
+#include "tq_device.h"
+
+struct TqManyPlain {                 // uncompressed tokens of a row: token t of head h of sequence b at b * batch + h * head + t * token elements
+    const uint8_t *k, *v;
+    long long k_batch, k_head, k_token, v_batch, v_head, v_token;
+    uint32_t n;
+};
+
+struct TqManyArgs {
+    const uint8_t *q;                // query head j, token i of sequence b at b * q_batch + j * q_head + i * q_token elements
+    uint8_t *out;                    // dense [batch, query heads, queries, D]
+    long long q_batch, q_head, q_token;
+    const uint8_t *k_idx, *v_idx;
+    const uint16_t *k_norms, *v_norms;
+    const uint8_t *table_k, *table_v;
+    TqManyPlain plain[2];            // behind the packed tokens: the window, and the drafted tokens
+    const int32_t *lengths;          // keys of sequence b that count (packed, then window), or null: all
+    const uint8_t *mask;             // [batch, mask_stride] truth value of every key (packed, then window), or null
+    const uint8_t *tree;             // drafted token j is seen by query i if tree[b * tree_batch + i * plain[1].n + j], or null: if j <= i
+    long long mask_stride, tree_batch;
+    float *weights;                  // [rows, w_stride] what every key (packed, then window) receives is added here; or null
+    long long w_stride;
+    uint8_t *q_op;                   // rotated queries as operands, see q_operand_bytes
+    float *q_scale;                  // [rows, tiles] what a tile's products are multiplied with
+    float *rec;                      // [rows, tiles, records][32 largest logits, 32 sums, 32 x DP value sums]: packed tokens' (value space of the codec)
+    float *plain_rec;                // the same of the uncompressed tokens (plain space)
+    float *stat;                     // [rows, tiles][32 largest logits, 32 reciprocal sums], written by the merge (only with weights)
+    float scale;
+    uint32_t rows, heads, group, queries, M, tiles, tokens, packed_row_stride, D, bits_k, bits_v, dtype;
+    uint32_t splits, chunk, records, plain_records;
+    uint32_t aligned;                // vectors of queries and uncompressed tokens can be read 16 bytes at a time
+};
+
+namespace {
+
+typedef float tq_f4 __attribute__((ext_vector_type(4)));
+
+constexpr float MANY_NONE = -3.0e38f;        // largest logit of no token at all
+constexpr int LEVEL_SHIFT = 6;               // levels enter the products times 2^6: their second fp16 term stays above the subnormals' grid
+constexpr int Q_TOP = 13;                    // a tile's largest rotated query lies in [2^13, 2^14)
+constexpr int P_TOP = 14;                    // weight * value norm, at most 2^15
+constexpr int PLAIN_WAVES = 4;
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// Rotated queries of a tile: per fp16 term (leading, rest) and step s of 16 coordinates 64 lanes x 16 bytes; lane (n = lane % 32, hk = lane / 32) has
+// query n, coordinates hk * DP / 2 + 8 s ... + 7 (a lane's share of a packed key is then one run of bytes).
+__host__ __device__ constexpr uint32_t q_operand_bytes(uint32_t dp) { return 2u * (dp / 16u) * 1024u; }
+__host__ __device__ constexpr uint32_t record_floats(uint32_t dp) { return 64u + 32u * dp; }
+
+// Row of a result register r of a 32 x 32 product in lane half h
+__device__ __forceinline__ constexpr uint32_t acc_row(int r, uint32_t h) { return 8u * (uint32_t)(r / 4) + 4u * h + (uint32_t)(r % 4); }
+
+// Order of this wave's LDS accesses among its lanes
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Over the two lanes that share a column
+__device__ __forceinline__ float halves_max(float x) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+}
+__device__ __forceinline__ float halves_add(float x) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(two[0]) + __uint_as_float(two[1]);
+}
+
+// float -> two fp16 terms, packed (leading | rest << 16): 22 bits while neither term falls below 2^-14.  Infinities and NaN have no rest.
+__device__ __forceinline__ uint32_t fp16_terms(float x) {
+    const _Float16 hi = (_Float16)x;
+    const float r = x - (float)hi;
+    const _Float16 lo = (_Float16)(r == r ? r : 0.f);
+    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
+}
+// eight of them -> two operands
+__device__ __forceinline__ void fp16_operands(const uint32_t (&t)[8], tq_u4 &hi, tq_u4 &lo) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        hi[d] = __builtin_amdgcn_perm(t[2 * d + 1], t[2 * d], 0x05040100u);
+        lo[d] = __builtin_amdgcn_perm(t[2 * d + 1], t[2 * d], 0x07060302u);
+    }
+}
+
+// Eight floats -> three bf16 terms that add up to them (an infinity or NaN has only its first).
+__device__ __forceinline__ void bf16_terms(const float (&x)[8], tq_u4 (&t)[3]) {
+    uint32_t a[8], b[8], c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a[i] = __float_as_uint(x[i]) & 0xffff0000u;
+        float r = x[i] - __uint_as_float(a[i]);
+        r = r == r ? r : 0.f;
+        b[i] = __float_as_uint(r) & 0xffff0000u;
+        c[i] = __float_as_uint(r - __uint_as_float(b[i]));
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        t[0][d] = __builtin_amdgcn_perm(a[2 * d + 1], a[2 * d], 0x07060302u);
+        t[1][d] = __builtin_amdgcn_perm(b[2 * d + 1], b[2 * d], 0x07060302u);
+        t[2][d] = __builtin_amdgcn_perm(c[2 * d + 1], c[2 * d], 0x07060302u);
+    }
+}
+
+__device__ __forceinline__ float plain_element(const uint8_t *p, uint32_t dtype) {
+    if (dtype == TQ_F32) return *reinterpret_cast<const TQ_GLOBAL float *>((const TQ_GLOBAL uint8_t *)p);
+    const uint16_t h = tq_gload2(reinterpret_cast<const uint16_t *>(p));
+    return dtype == TQ_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+}
+
+// Elements [first, first + 8) of a vector as NT bf16 terms that add up to them (bf16: 1, fp16: 2, float32: 3); those from D on are zero.
+template <int DT> constexpr int plain_terms() { return DT == TQ_BF16 ? 1 : DT == TQ_F16 ? 2 : 3; }
+template <int DT>
+__device__ __forceinline__ void load_plain8(const uint8_t *vec, uint32_t first, uint32_t D, bool aligned, tq_u4 (&t)[3]) {
+    constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
+    const uint8_t *p = vec + first * ES;
+    float x[8];
+    if (first >= D) {
+        t[0] = t[1] = t[2] = tq_u4{0u, 0u, 0u, 0u};
+        return;
+    }
+    if (aligned) {           // (D is a multiple of 8 then)
+        const tq_u4 a = tq_gload16(p);
+        if constexpr (DT == TQ_BF16) {
+            t[0] = a;
+            return;
+        } else if constexpr (DT == TQ_F16) {
+            const tq_half8 h = __builtin_bit_cast(tq_half8, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+        } else {
+            const tq_u4 b = tq_gload16(p + 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = __uint_as_float(a[i]); x[4 + i] = __uint_as_float(b[i]); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = first + i < D ? plain_element(p + i * ES, DT) : 0.f;
+    }
+    bf16_terms(x, t);
+}
+
+// Position of a row's query vector m: query head and token
+struct ManyQuery {
+    uint32_t g, t;
+    __device__ __forceinline__ ManyQuery(const TqManyArgs &a, uint32_t m) : g(m / a.queries), t(m - g * a.queries) {}
+};
+__device__ __forceinline__ const uint8_t *many_query(const TqManyArgs &a, uint32_t row, uint32_t m, uint32_t elem_bytes) {
+    const uint32_t b = row / a.heads, h = row - b * a.heads;
+    const ManyQuery q(a, m);
+    return a.q + ((long long)b * a.q_batch + (long long)(h * a.group + q.g) * a.q_head + (long long)q.t * a.q_token) * elem_bytes;
+}
+
+// Keys of sequence b (packed, then window) that can count
+__device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b) {
+    const uint32_t all = a.tokens + a.plain[0].n;
+    if (!a.lengths) return all;
+    const int32_t l = a.lengths[b];
+    return l < 0 ? 0u : min((uint32_t)l, all);
+}
+
+}  // namespace

@@ -1,0 +1,165 @@
+// softmax(scale q K^T) V of any number of query tokens per sequence over a packed history, the window behind it and tokens that are in no
+// cache (drafts), with lengths and masks: tq_attend_many.  Launches: queries into the codec's space; packed tokens, a block a split of
+// them; uncompressed tokens; merge; and where the caller keeps count, what every key has received.
+#include "tq_many_kernel.h"
+
+namespace {
+
+constexpr int MAX_SPLITS = 64;
+
+int padded(int D) { return TQ_PADDED_DIM(D); }
+
+struct Plan {
+    long long rows, tiles, splits, records, plain_records, floats;
+};
+
+long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 31) / 32 + (r->drafts.tokens + 31) / 32; }
+
+int plan(const tq_attend_request *r, Plan &p) {
+    p.rows = r->batch * r->heads;
+    p.tiles = (r->group * r->n_queries + 31) / 32;
+    const long long at = p.rows * p.tiles;
+    p.splits = 1;
+    if (at && r->tokens) {
+        int cus = 0;
+        if (tq_device_cus(cus)) cus = 256;
+        p.splits = (2 * cus + at - 1) / at;
+        const long long most = (r->tokens + 127) / 128;
+        if (p.splits > most) p.splits = most;
+        if (p.splits > MAX_SPLITS) p.splits = MAX_SPLITS;
+        if (p.splits < 1) p.splits = 1;
+    }
+    p.records = r->tokens ? p.splits * ANY_WAVES : 0;
+    p.plain_records = plain_tiles(r) ? PLAIN_WAVES : 0;
+    const long long dp = padded(r->head_dim);
+    p.floats = at * ((long long)q_operand_bytes((uint32_t)dp) / 4 + (p.records + p.plain_records) * record_floats((uint32_t)dp) + 64) + (at + 3) / 4 * 4;
+    return at * p.splits > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;
+}
+
+int check(const tq_attend_request *r) {
+    if (!r) return TQ_ERR_NULL;
+    if (r->dtype != TQ_F32 && r->dtype != TQ_F16 && r->dtype != TQ_BF16) return TQ_ERR_DTYPE;
+    if (r->bits_k < 1 || r->bits_k > 8 || r->bits_v < 1 || r->bits_v > 8) return TQ_ERR_BITS;
+    if (r->head_dim < TQ_ANYDIM_MIN || r->head_dim > TQ_ANYDIM_MAX) return TQ_ERR_HEAD_DIM;
+    const long long most = 0x7fffffff;
+    if (r->batch < 0 || r->heads < 0 || r->group < 0 || r->n_queries < 0 || r->tokens < 0 || r->window.tokens < 0 || r->drafts.tokens < 0) return TQ_ERR_SIZE;
+    if (r->batch > most || r->heads > most || r->group > most || r->n_queries > most || r->tokens > most - 65536 || r->window.tokens > 65536 || r->drafts.tokens > 65536)
+        return TQ_ERR_SIZE;
+    if (r->batch * r->heads > most || r->heads * r->group > most || r->group * r->n_queries > most / 2) return TQ_ERR_SIZE;
+    const long long rows = r->batch * r->heads, tiles = (r->group * r->n_queries + 31) / 32;
+    if (rows && tiles > most / rows) return TQ_ERR_SIZE;
+    if (r->packed_row_stride < 0 || r->packed_row_stride > most || (r->packed_row_stride && r->packed_row_stride < r->tokens)) return TQ_ERR_SIZE;
+    return TQ_OK;
+}
+
+bool aligned16(const tq_plain_tokens &t, long long es) {
+    return !(((uintptr_t)t.k | (uintptr_t)t.v) & 15u) && !((t.k_batch * es) & 15) && !((t.k_head * es) & 15) && !((t.k_token * es) & 15) && !((t.v_batch * es) & 15) &&
+           !((t.v_head * es) & 15) && !((t.v_token * es) & 15);
+}
+
+TqManyPlain plain_of(const tq_plain_tokens &t) {
+    return TqManyPlain{static_cast<const uint8_t *>(t.k), static_cast<const uint8_t *>(t.v), t.k_batch, t.k_head, t.k_token, t.v_batch, t.v_head, t.v_token, (uint32_t)t.tokens};
+}
+
+template <int DP>
+void launch_dim(const TqManyArgs &a, hipStream_t s) {
+    const uint32_t at = a.rows * a.tiles;
+    if (a.records) hipLaunchKernelGGL((tq_many_any_kernel<DP>), dim3(at * a.splits), dim3(64 * ANY_WAVES), 0, s, a);
+    if (a.plain_records) {
+        const dim3 g(at), t(64 * PLAIN_WAVES);
+        if (a.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F32>), g, t, 0, s, a);
+        else if (a.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F16>), g, t, 0, s, a);
+        else hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_BF16>), g, t, 0, s, a);
+    }
+    hipLaunchKernelGGL((tq_many_merge_kernel<DP>), dim3(at), dim3(2 * DP), 0, s, a);
+    if (!a.weights) return;
+    if (a.tokens) {
+        const uint32_t blocks = (a.tokens + 32u * ANY_WAVES - 1u) / (32u * ANY_WAVES);
+        hipLaunchKernelGGL((tq_many_any_weights_kernel<DP>), dim3(a.rows * blocks), dim3(64 * ANY_WAVES), 0, s, a, blocks);
+    }
+    if (a.plain[0].n) {
+        const dim3 g(a.rows * ((a.plain[0].n + 31u) / 32u));
+        if (a.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_plain_weights_kernel<TQ_F32>), g, dim3(64), 0, s, a, DP / 16u);
+        else if (a.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_plain_weights_kernel<TQ_F16>), g, dim3(64), 0, s, a, DP / 16u);
+        else hipLaunchKernelGGL((tq_many_plain_weights_kernel<TQ_BF16>), g, dim3(64), 0, s, a, DP / 16u);
+    }
+}
+
+}  // namespace
+
+extern "C" long long tq_attend_many_scratch(const tq_attend_request *request) {
+    const int rc = check(request);
+    if (rc) return rc;
+    Plan p;
+    const int bad = plan(request, p);
+    return bad ? bad : p.floats;
+}
+
+extern "C" int tq_attend_many(const tq_attend_request *request, float *scratch, long long scratch_floats, void *stream) {
+    int rc = check(request);
+    if (rc) return rc;
+    const tq_attend_request &r = *request;
+    Plan p;
+    rc = plan(request, p);
+    if (rc) return rc;
+    if (p.rows * p.tiles == 0) return TQ_OK;
+    if (!r.queries || !r.out || !r.table_k || !r.table_v || !scratch) return TQ_ERR_NULL;
+    if (r.tokens && (!r.k_idx || !r.k_norms || !r.v_idx || !r.v_norms)) return TQ_ERR_NULL;
+    if ((r.window.tokens && (!r.window.k || !r.window.v)) || (r.drafts.tokens && (!r.drafts.k || !r.drafts.v))) return TQ_ERR_NULL;
+    const long long total = r.tokens + r.window.tokens;
+    if (r.mask && r.batch > 1 && r.mask_stride < total) return TQ_ERR_SIZE;
+    if (r.weights && p.rows > 1 && r.weights_stride < total) return TQ_ERR_SIZE;
+    if (!r.tree && r.drafts.tokens && r.drafts.tokens != r.n_queries) return TQ_ERR_SIZE;
+    const long long es = r.dtype == TQ_F32 ? 4 : 2;
+    if (((uintptr_t)r.table_k & 15u) || ((uintptr_t)r.table_v & 15u) || ((uintptr_t)scratch & 15u) || ((uintptr_t)r.k_norms & 1u) || ((uintptr_t)r.v_norms & 1u) ||
+        ((uintptr_t)r.lengths & 3u) || ((uintptr_t)r.weights & 3u) || ((uintptr_t)r.queries & (es - 1)) || ((uintptr_t)r.out & (es - 1)))
+        return TQ_ERR_ALIGN;
+    if (scratch_floats < p.floats) return TQ_ERR_CAPACITY;
+    const uint32_t dp = (uint32_t)padded(r.head_dim);
+    const long long at = p.rows * p.tiles;
+    TqManyArgs a{};
+    a.q = static_cast<const uint8_t *>(r.queries);
+    a.out = static_cast<uint8_t *>(r.out);
+    a.q_batch = r.q_batch; a.q_head = r.q_head; a.q_token = r.q_token;
+    a.k_idx = r.k_idx; a.v_idx = r.v_idx; a.k_norms = r.k_norms; a.v_norms = r.v_norms;
+    a.table_k = static_cast<const uint8_t *>(r.table_k); a.table_v = static_cast<const uint8_t *>(r.table_v);
+    a.plain[0] = plain_of(r.window); a.plain[1] = plain_of(r.drafts);
+    a.lengths = r.lengths; a.mask = r.mask; a.tree = r.tree;
+    a.mask_stride = r.mask_stride; a.tree_batch = r.tree_batch;
+    a.weights = r.weights; a.w_stride = r.weights_stride;
+    // scratch: operands, records, uncompressed tokens' records, statistics, scales
+    float *f = scratch;
+    a.q_op = reinterpret_cast<uint8_t *>(f); f += at * (q_operand_bytes(dp) / 4);
+    a.rec = f; f += at * p.records * record_floats(dp);
+    a.plain_rec = f; f += at * p.plain_records * record_floats(dp);
+    if (r.weights) a.stat = f;
+    f += at * 64;
+    a.q_scale = f;
+    a.scale = r.scale;
+    a.rows = (uint32_t)p.rows; a.heads = (uint32_t)r.heads; a.group = (uint32_t)r.group; a.queries = (uint32_t)r.n_queries;
+    a.M = (uint32_t)(r.group * r.n_queries); a.tiles = (uint32_t)p.tiles; a.tokens = (uint32_t)r.tokens;
+    a.packed_row_stride = (uint32_t)(r.packed_row_stride ? r.packed_row_stride : r.tokens);
+    a.D = (uint32_t)r.head_dim; a.bits_k = (uint32_t)r.bits_k; a.bits_v = (uint32_t)r.bits_v; a.dtype = (uint32_t)r.dtype;
+    a.splits = (uint32_t)p.splits; a.records = (uint32_t)p.records; a.plain_records = (uint32_t)p.plain_records;
+    a.chunk = (uint32_t)(((r.tokens + p.splits - 1) / p.splits + 31) / 32 * 32);
+    a.aligned = !(r.head_dim & 7) && !((uintptr_t)r.queries & 15u) && !((r.q_batch * es) & 15) && !((r.q_head * es) & 15) && !((r.q_token * es) & 15) &&
+                (!r.window.tokens || aligned16(r.window, es)) && (!r.drafts.tokens || aligned16(r.drafts, es));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    {
+        const dim3 g((unsigned)at), t(2 * dp);
+        if (r.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F32>), g, t, 0, s, a);
+        else if (r.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F16>), g, t, 0, s, a);
+        else hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_BF16>), g, t, 0, s, a);
+    }
+    switch (dp) {
+        case 32: launch_dim<32>(a, s); break;
+        case 64: launch_dim<64>(a, s); break;
+        case 96: launch_dim<96>(a, s); break;
+        case 128: launch_dim<128>(a, s); break;
+        case 160: launch_dim<160>(a, s); break;
+        case 192: launch_dim<192>(a, s); break;
+        case 224: launch_dim<224>(a, s); break;
+        default: launch_dim<256>(a, s); break;
+    }
+    return (int)hipGetLastError();
+}

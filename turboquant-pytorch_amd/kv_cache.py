@@ -53,9 +53,11 @@ class _LayerStore:
 
     # over all layers of the cache on this device: packed bytes of one token, and bytes of the windows; 0: not known
     cache_slot_bytes = cache_window_bytes = 0
+    # [B, H, capacity + window]: the attention every stored token has received, packed tokens first, then the window; zero behind them
+    weights = None
 
     def __init__(self, comp: TurboQuantV3, B: int, H: int, D: int, dtype: torch.dtype, device: torch.device,
-                 capacity: int, window: int):
+                 capacity: int, window: int, track_weights: bool = False):
         self.comp = comp
         self.B, self.H, self.D = B, H, D
         self.dtype, self.device = dtype, device
@@ -76,6 +78,8 @@ class _LayerStore:
         self._record = None
         # decode steps of this layer take one launch each way (tq_decode_append, tq_decode_attend)
         self.one_launch = _native.decode_supported(D, dtype, comp.key_bits, comp.value_bits)
+        if track_weights:
+            self.weights = torch.zeros((B, H, window), dtype=torch.float32, device=device)
         self.reserve(capacity)
 
     def __getstate__(self):
@@ -122,6 +126,12 @@ class _LayerStore:
             if old is not None and self.n_compressed:
                 buf[:, :, :self.n_compressed].copy_(old[:, :, :self.n_compressed])
             new.append(buf)
+        if self.weights is not None:
+            # a token keeps its place in this order when it goes from the window into the packed store: nothing moves then
+            weights = torch.zeros((self.B, self.H, cap + self.window_tokens), dtype=torch.float32, device=self.device)
+            held = self.n_compressed + self.n_recent
+            weights[:, :, :held].copy_(self.weights[:, :, :held])
+            self.weights = weights
         self.k_idx, self.k_nrm, self.v_idx, self.v_nrm = new
         self.capacity = cap
         self._consts = None
@@ -215,6 +225,21 @@ class _LayerStore:
         vc.compress_into(values, self.v_idx[:, :, lo:hi], self.v_nrm[:, :, lo:hi])
         self.n_compressed = hi
 
+    def evict(self, keep: int) -> torch.Tensor:
+        """Packed tokens but the `keep` with the largest weights leave; slots [B,H,keep] of those that stay."""
+        n, held = self.n_compressed, self.n_compressed + self.n_recent
+        if n <= keep:
+            return torch.arange(n, device=self.device).expand(self.B, self.H, n)
+        kc, vc = self.comp.key_compressor, self.comp.val_compressor
+        packed = ((self.k_idx[:, :, :n], self.k_nrm[:, :, :n]), (self.v_idx[:, :, :n], self.v_nrm[:, :, :n]))
+        into = tuple(tuple(torch.empty_like(t) for t in pair) for pair in ((self.k_idx, self.k_nrm), (self.v_idx, self.v_nrm)))
+        weights = torch.zeros_like(self.weights)
+        _, _, kept = _native.evict(packed, n, (kc.bits, vc.bits), self.D, self.weights[:, :, :held], keep, into, weights)
+        (self.k_idx, self.k_nrm), (self.v_idx, self.v_nrm) = into
+        self.weights, self.n_compressed = weights, keep
+        self._consts = self._record = None
+        return kept
+
     def window(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """Views [B,H,n_recent,D] of the uncompressed keys and values, oldest first."""
         return (self.k_win[:, :, self.w0:self.w0 + self.n_recent], self.v_win[:, :, self.w0:self.w0 + self.n_recent])
@@ -237,16 +262,22 @@ class _LayerStore:
 
 
 class V3Cache:
-    """Streaming compressed KV cache; `update` follows generation_test_v2.py:80-153."""
+    """Streaming compressed KV cache; `update` follows generation_test_v2.py:80-153.
+    track_weights: `attend` keeps the sum of the attention weights that every cached token has received (`attention_weights`),
+    by which `evict` thins out the packed store."""
+
+    track_weights = False
 
     def __init__(self, key_bits: int = 4, value_bits: int = 2, residual_window: int = 128,
-                 protected_layers: int = 0, n_layers: int = 36, *, capacity: int = 0):
+                 protected_layers: int = 0, n_layers: int = 36, *, capacity: int = 0, track_weights: bool = False):
         self.key_bits = key_bits
         self.value_bits = value_bits
         self.residual_window = residual_window
         self.protected_layers = protected_layers
         self.n_layers = n_layers
         self.capacity = capacity          # expected compressed tokens per sequence (0: grow on demand)
+        if track_weights:
+            self.track_weights = True
         self._compressors: Dict[int, TurboQuantV3] = {}
         self._stores: Dict[int, _LayerStore] = {}
 
@@ -272,7 +303,7 @@ class V3Cache:
         comp = self._get_compressor(layer_idx, D, device)
         st = self._stores.get(layer_idx)
         if st is None:
-            st = _LayerStore(comp, B, H, D, key_states.dtype, device, self.capacity, self.residual_window)
+            st = _LayerStore(comp, B, H, D, key_states.dtype, device, self.capacity, self.residual_window, self.track_weights)
             self._stores[layer_idx] = st
             self._count_slots()
         elif (st.B, st.H, st.D) != (B, H, D):
@@ -351,11 +382,12 @@ class V3Cache:
         """softmax(scale * q K^T) V of one query token per sequence, [B,Hq,1,D] -> [B,Hq,1,D], over everything
         cached for the layer -- what the model computes from the tensors `update` returns -- read
         straight from the packed store.  Query head j uses kv head j // (Hq / H).
+        A cache that tracks weights adds what every token receives to its sums, whatever `fused`.
         fused (default: whenever at most 16 query heads share a kv head): one kernel pass over packed keys and
         values with an online softmax per split of the history; otherwise three steps (scores from the packed
         keys, softmax in float32, weighted sum of the packed values).  Window tokens are used as they are."""
         st = self._stores.get(layer_idx)
-        if st is not None and st.one_launch and st.total_seq and fused is not False and query_states.is_cuda and not torch.compiler.is_compiling():
+        if st is not None and st.one_launch and st.total_seq and fused is not False and st.weights is None and query_states.is_cuda and not torch.compiler.is_compiling():
             B, Hq, Sq, D = query_states.shape
             G = Hq // st.H
             if Sq == 1 and B == st.B and D == st.D and Hq == G * st.H and 1 <= G <= 16 and st.n_recent <= 512:
@@ -376,6 +408,8 @@ class V3Cache:
         G = Hq // st.H
         scale = D ** -0.5 if scale is None else scale
         n_c, n_w = st.n_compressed, st.n_recent
+        if st.weights is not None:
+            return self._attend_many(st, query_states, None, None, scale, st.weights[:, :, :n_c + n_w])
         kc, vc = st.comp.key_compressor, st.comp.val_compressor
         one_launch = st.one_launch and query_states.dtype == st.dtype and G <= 16 and n_w <= 512 and B * st.H <= 65535 and fused is not False
         if D != _native.HEAD_DIM and not one_launch:
@@ -436,6 +470,57 @@ class V3Cache:
         return out.to(query_states.dtype).reshape(B, Hq, 1, D)
 
     @staticmethod
+    def _attend_many(st: _LayerStore, query_states: torch.Tensor, drafts, tree_mask, scale: Optional[float], weights) -> torch.Tensor:
+        """tq_attend_many over everything the layer holds."""
+        n = st.n_compressed
+        kc, vc, device = st.comp.key_compressor, st.comp.val_compressor, st.k_win.device
+        packed = ((st.k_idx[:, :, :n], st.k_nrm[:, :, :n]), (st.v_idx[:, :, :n], st.v_nrm[:, :, :n])) if n else None
+        return _native.attend_many(query_states, packed, n, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), st.window(), drafts, None, None,
+                                   tree_mask, weights, scale)
+
+    def attend_tree(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
+                    tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """Attention of drafted tokens, [B,Hq,T,D] -> [B,Hq,T,D], before any of them is accepted: every one sees everything cached for the layer and,
+        of the drafted keys and values [B,H,T,D], those that tree_mask ([T,T] or [B,T,T], truth values; row i is what token i sees) names, its
+        ancestors in the draft and itself.  Without a mask the drafted tokens follow one another.  The cache stays as it is: `append` the
+        accepted tokens' keys and values afterwards.  Nothing has to be cached yet; a token that sees nothing gets zeros.
+        (Draft and queries may differ in number: the mask is then [T, drafted].)  A cache that tracks weights does not count drafts."""
+        st = self._stores.get(layer_idx)
+        B, _, _, D = query_states.shape
+        if st is not None and st.total_seq:
+            if (st.B, st.D) != (B, D) or key_states.shape[1] != st.H:
+                raise ValueError(f"layer {layer_idx}: drafted states {tuple(query_states.shape)} / {tuple(key_states.shape)} do not match the cached "
+                                 f"batch/head/dim {(st.B, st.H, st.D)}")
+            return self._attend_many(st, query_states, (key_states, value_states), tree_mask, scale, None)
+        _native._require_gpu(query_states, "queries")
+        comp, device = self._get_compressor(layer_idx, D, query_states.device), query_states.device
+        kc, vc = comp.key_compressor, comp.val_compressor
+        return _native.attend_many(query_states, None, 0, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), None, (key_states, value_states), None, None,
+                                   tree_mask, None, scale)
+
+    def attention_weights(self, layer_idx: int = 0) -> torch.Tensor:
+        """[B,H,n] float32: what every token held for the layer, packed tokens first, then the window, has received in the `attend` calls since
+        it came (summed over the query heads of its kv head).  The cache's own memory: it moves on with the next call."""
+        st = self._stores.get(layer_idx)
+        if st is None:
+            raise ValueError(f"attention_weights: nothing is cached for layer {layer_idx}")
+        if st.weights is None:
+            raise ValueError("attention_weights: the cache does not track them (track_weights=True)")
+        return st.weights[:, :, :st.n_compressed + st.n_recent]
+
+    def evict(self, keep: int, layer_idx: Optional[int] = None):
+        """Of the packed tokens of every (sequence, kv head) the `keep` that have received most attention stay, in their order (of equal ones the first);
+        the window stays whole.  Answers with the packed slots of what stayed, [B,H,min(keep, packed)] (int64); without a
+        layer all layers are thinned out, and the answer is a dictionary of them.  `get_seq_length` still counts every token seen, so that
+        positions go on; `update`, `append`, `attend` and `attend_tree` work on what is left."""
+        if isinstance(keep, bool) or int(keep) != keep or keep < 0:
+            raise ValueError(f"evict: keep must be a whole number, 0 or more; got {keep!r}")
+        if layer_idx is None:
+            return {i: self.evict(keep, i) for i in sorted(self._stores)}
+        self.attention_weights(layer_idx)          # (raises where there are none)
+        return self._stores[layer_idx].evict(int(keep))
+
+    @staticmethod
     def _attend_step(st: _LayerStore, query_states: torch.Tensor, G: int, scale: float) -> Optional[torch.Tensor]:
         """The fused path of `attend` in one library call (rotate + window, packed history, merge), with the
         scratch kept per stream.  None when the queries are not laid out for it."""
@@ -488,8 +573,9 @@ class V3Cache:
             return "no compression"
         st = self._stores.get(0)
         comp = st.n_compressed if st is not None else 0
+        recent = st.n_recent if st is not None else 0
         total = st.total_seq if st is not None else 0
-        return f"{comp} compressed, {total - comp} fp16, {total} total"
+        return f"{comp} compressed, {recent} fp16, {total} total"
 
     def save(self, path: str, include_codec: bool = True) -> None:
         """Write configuration, packed history and window of every layer to one safetensors file."""
@@ -566,8 +652,10 @@ def hf_cache_class():
             return V3Cache.get_seq_length(self, layer_idx)
 
         def get_mask_sizes(self, query_length, layer_idx=0):
-            # (length, offset) of the keys the next update() of this layer will return
-            return V3Cache.get_seq_length(self, layer_idx) + int(query_length), 0
+            # (length, offset) of the keys the next update() of this layer will return (after an eviction fewer than were seen)
+            st = self._stores.get(layer_idx)
+            held = st.n_compressed + st.n_recent if st is not None else 0
+            return held + int(query_length), V3Cache.get_seq_length(self, layer_idx) - held
 
     return HFV3Cache
 

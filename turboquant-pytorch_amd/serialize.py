@@ -11,7 +11,7 @@ File layout (metadata key "tqamd" holds the JSON header):
 
   kind "kv-cache"   a V3Cache: per layer  L{i}.k_idx u8 [B,H,n_c,Gk], L{i}.k_nrm f16 [B,H,n_c],
                     L{i}.v_idx, L{i}.v_nrm, L{i}.k_win / L{i}.v_win [B,H,n_w,D] (the uncompressed
-                    window, oldest token first), and optionally the codec itself
+                    window, oldest token first), of a cache that tracks them L{i}.weights f32 [B,H,n_c + n_w], and optionally the codec itself
                     (L{i}.k_pi, L{i}.k_centroids, L{i}.v_pi, L{i}.v_centroids);
   kind "kv-pair"    the two dicts TurboQuantV3.compress_kv returns: k.* / v.* tensors
                     (idx_bytes, vec_norms, fp16).
@@ -132,7 +132,7 @@ def save_cache(cache, path: str, include_codec: bool = True) -> None:
         "kind": "kv-cache",
         "config": {"key_bits": cache.key_bits, "value_bits": cache.value_bits,
                    "residual_window": cache.residual_window, "protected_layers": cache.protected_layers,
-                   "n_layers": cache.n_layers},
+                   "n_layers": cache.n_layers, **({"track_weights": True} if cache.track_weights else {})},
         "layers": {},
     }
     tensors: Dict[str, torch.Tensor] = {}
@@ -151,6 +151,8 @@ def save_cache(cache, path: str, include_codec: bool = True) -> None:
             tensors[p + "v_idx"], tensors[p + "v_nrm"] = st.v_idx[:, :, :n_c], st.v_nrm[:, :, :n_c]
         if st.n_recent:
             tensors[p + "k_win"], tensors[p + "v_win"] = st.window()
+        if st.weights is not None:
+            tensors[p + "weights"] = st.weights[:, :, :n_c + st.n_recent]
         if include_codec:
             tensors[p + "k_pi"], tensors[p + "k_centroids"] = kc.Pi, kc.centroids
             tensors[p + "v_pi"], tensors[p + "v_centroids"] = vc.Pi, vc.centroids
@@ -190,7 +192,7 @@ def load_cache(path: str, device="cuda", cls=None):
                 comp.value_bits = bits
         n_c, n_w = info["n_compressed"], info["n_recent"]
         st = _LayerStore(comp, info["batch"], info["heads"], info["head_dim"], _DTYPES[info["dtype"]], device,
-                         n_c, cache.residual_window)
+                         n_c, cache.residual_window, cache.track_weights)
         if n_c:
             for name in ("k_idx", "k_nrm", "v_idx", "v_nrm"):
                 src = f.get_tensor(p + name)
@@ -207,6 +209,11 @@ def load_cache(path: str, device="cuda", cls=None):
             if n_w > st.win_cap:                       # a file whose window outgrew 2 x residual_window cannot come from save_cache
                 raise FormatError(f"{path}: window of layer {idx} holds {n_w} tokens, more than the cache keeps")
             st.extend_window(kw, vw)
+        if st.weights is not None:
+            weights = f.get_tensor(p + "weights")
+            if tuple(weights.shape) != (info["batch"], info["heads"], n_c + n_w) or weights.dtype != torch.float32:
+                raise FormatError(f"{path}: {p}weights is {tuple(weights.shape)} {weights.dtype}, expected {(info['batch'], info['heads'], n_c + n_w)} float32")
+            st.weights[:, :, :n_c + n_w].copy_(weights)
         st.total_seq = info["total_seq"]
         cache._stores[idx] = st
     cache._count_slots()
