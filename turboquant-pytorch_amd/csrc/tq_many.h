@@ -167,3 +167,8 @@ __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b)
 }
 
 }  // namespace
+
+// Launches tq_many_fast_kernel for one head dimension; ipbk, ipbv = codes per byte (1, 2, 4), qt = tiles of 32 queries a block, kt = fp16 terms of queries and key levels
+int tq_many_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
+int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
+int tq_many_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);

@@ -10,8 +10,31 @@ constexpr int MAX_SPLITS = 64;
 int padded(int D) { return TQ_PADDED_DIM(D); }
 
 struct Plan {
-    long long rows, tiles, splits, records, plain_records, floats;
+    long long rows, tiles, groups, splits, records, plain_records, floats;
+    int qt, kt;                      // tiles a block and fp16 terms of the kernels for one head dimension; qt = 0: the one for all
 };
+
+// Whether a head dimension and its code widths have a kernel of their own.  float32 results want two terms of weights and value levels as well.
+bool fast(const tq_attend_request *r) {
+    const int ik = 8 / r->bits_k, iv = 8 / r->bits_v;
+    return (r->head_dim == 64 || r->head_dim == 128 || r->head_dim == 256) && ik <= 4 && iv <= 4 && r->dtype != TQ_F32 && r->tokens >= 32 &&
+           !((uintptr_t)r->k_idx & (tq_packed_alignment(r->head_dim, r->bits_k) - 1u)) && !((uintptr_t)r->v_idx & (tq_packed_alignment(r->head_dim, r->bits_v) - 1u));
+}
+
+// splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and what its start
+// and its end cost
+long long fast_splits(long long blocks, long long tokens) {
+    int cus = 0;
+    if (tq_device_cus(cus)) cus = 256;
+    long long most = (tokens + 255) / 256, best = 1, best_cost = 0;
+    if (most > MAX_SPLITS) most = MAX_SPLITS;
+    for (long long s = 1; s <= most; ++s) {
+        const long long rounds = (blocks * s + cus - 1) / cus, cost = rounds * ((tokens + s - 1) / s + 1500) + 30 * s;
+        if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
+        if (rounds > 16 && s > 1) break;
+    }
+    return best;
+}
 
 long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 31) / 32 + (r->drafts.tokens + 31) / 32; }
 
@@ -20,7 +43,14 @@ int plan(const tq_attend_request *r, Plan &p) {
     p.tiles = (r->group * r->n_queries + 31) / 32;
     const long long at = p.rows * p.tiles;
     p.splits = 1;
-    if (at && r->tokens) {
+    p.qt = p.kt = 0;
+    p.groups = p.tiles;
+    if (at && r->tokens && fast(r)) {
+        p.kt = r->dtype == TQ_BF16 && !r->weights ? 1 : 2;
+        p.qt = p.kt == 1 && r->head_dim != 256 && p.tiles > 1 ? 2 : 1;
+        p.groups = (p.tiles + p.qt - 1) / p.qt;
+        p.splits = fast_splits(p.rows * p.groups, r->tokens);
+    } else if (at && r->tokens) {
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
         p.splits = (2 * cus + at - 1) / at;
@@ -29,7 +59,7 @@ int plan(const tq_attend_request *r, Plan &p) {
         if (p.splits > MAX_SPLITS) p.splits = MAX_SPLITS;
         if (p.splits < 1) p.splits = 1;
     }
-    p.records = r->tokens ? p.splits * ANY_WAVES : 0;
+    p.records = r->tokens ? p.splits * (p.qt ? 1 : ANY_WAVES) : 0;
     p.plain_records = plain_tiles(r) ? PLAIN_WAVES : 0;
     const long long dp = padded(r->head_dim);
     p.floats = at * ((long long)q_operand_bytes((uint32_t)dp) / 4 + (p.records + p.plain_records) * record_floats((uint32_t)dp) + 64) + (at + 3) / 4 * 4;
@@ -62,9 +92,15 @@ TqManyPlain plain_of(const tq_plain_tokens &t) {
 }
 
 template <int DP>
-void launch_dim(const TqManyArgs &a, hipStream_t s) {
+void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     const uint32_t at = a.rows * a.tiles;
-    if (a.records) hipLaunchKernelGGL((tq_many_any_kernel<DP>), dim3(at * a.splits), dim3(64 * ANY_WAVES), 0, s, a);
+    if (a.records && plan.qt) {
+        const dim3 g((unsigned)(plan.rows * plan.groups * plan.splits));
+        const int ik = 8 / (int)a.bits_k, iv = 8 / (int)a.bits_v;
+        if constexpr (DP == 64) tq_many_launch_d64(ik, iv, g, s, a, plan.qt, plan.kt);
+        if constexpr (DP == 128) tq_many_launch_d128(ik, iv, g, s, a, plan.qt, plan.kt);
+        if constexpr (DP == 256) tq_many_launch_d256(ik, iv, g, s, a, plan.qt, plan.kt);
+    } else if (a.records) hipLaunchKernelGGL((tq_many_any_kernel<DP>), dim3(at * a.splits), dim3(64 * ANY_WAVES), 0, s, a);
     if (a.plain_records) {
         const dim3 g(at), t(64 * PLAIN_WAVES);
         if (a.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F32>), g, t, 0, s, a);
@@ -146,20 +182,20 @@ extern "C" int tq_attend_many(const tq_attend_request *request, float *scratch, 
                 (!r.window.tokens || aligned16(r.window, es)) && (!r.drafts.tokens || aligned16(r.drafts, es));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     {
-        const dim3 g((unsigned)at), t(2 * dp);
-        if (r.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F32>), g, t, 0, s, a);
-        else if (r.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F16>), g, t, 0, s, a);
-        else hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_BF16>), g, t, 0, s, a);
+        const dim3 g((unsigned)(p.rows * ((p.tiles + 1) / 2))), t((p.tiles > 1 ? 4 : 2) * dp);
+        if (r.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F32>), g, t, 0, s, a, dp / 32u);
+        else if (r.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F16>), g, t, 0, s, a, dp / 32u);
+        else hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_BF16>), g, t, 0, s, a, dp / 32u);
     }
     switch (dp) {
-        case 32: launch_dim<32>(a, s); break;
-        case 64: launch_dim<64>(a, s); break;
-        case 96: launch_dim<96>(a, s); break;
-        case 128: launch_dim<128>(a, s); break;
-        case 160: launch_dim<160>(a, s); break;
-        case 192: launch_dim<192>(a, s); break;
-        case 224: launch_dim<224>(a, s); break;
-        default: launch_dim<256>(a, s); break;
+        case 32: launch_dim<32>(a, p, s); break;
+        case 64: launch_dim<64>(a, p, s); break;
+        case 96: launch_dim<96>(a, p, s); break;
+        case 128: launch_dim<128>(a, p, s); break;
+        case 160: launch_dim<160>(a, p, s); break;
+        case 192: launch_dim<192>(a, p, s); break;
+        case 224: launch_dim<224>(a, p, s); break;
+        default: launch_dim<256>(a, p, s); break;
     }
     return (int)hipGetLastError();
 }

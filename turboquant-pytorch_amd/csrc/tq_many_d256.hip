@@ -1,0 +1,7 @@
+#include "tq_many_fast.h"
+
+int tq_many_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt) {
+    if (ipbk == 4) return launch_many_fast<256, 4>(ipbv, grid, s, a, qt, kt);
+    if (ipbk == 2) return launch_many_fast<256, 2>(ipbv, grid, s, a, qt, kt);
+    return launch_many_fast<256, 1>(ipbv, grid, s, a, qt, kt);
+}

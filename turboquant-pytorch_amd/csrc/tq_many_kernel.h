@@ -6,15 +6,16 @@
 namespace {
 
 // ---- queries into the codec's space -----------------------------------------------------------------------------------------
-// Block (row, tile): wave w has coordinates 32 w ... + 31 of 32 queries, q' = scale * log2(e) * Pi_k q from the operands of the key codec's
-// table (Pi as three bf16 terms) and the queries' own bf16 terms, all products down to 2^-24 of the largest.  A tile is then scaled by
+// Block (row, two tiles, one where a row has no more): a tile's wave w has coordinates 32 w ... + 31 of 32 queries, q' = scale * log2(e) * Pi_k q from the operands of the key codec's
+// table (Pi as three bf16 terms) and the queries' own bf16 terms, all products down to 2^-24 of the largest.  The tiles of a block are then scaled by
 // the power of two that puts its largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)), so that no query is too large or too small for the two fp16
-// terms it is stored as: 22 bits for queries down to 2^-16 of the tile's largest.
+// terms it is stored as: 22 bits for queries down to 2^-16 of the largest.
 template <int DT>
-__global__ __launch_bounds__(512) void tq_many_prepare_kernel(TqManyArgs a) {
-    __shared__ float lds_top[8];
-    const uint32_t row = blockIdx.x / a.tiles, tile = blockIdx.x - row * a.tiles;
-    const uint32_t lane = threadIdx.x & 63u, wave = tq_uniform32(threadIdx.x >> 6), waves = blockDim.x >> 6, DP = 32u * waves, steps = 2u * waves;
+__global__ __launch_bounds__(1024) void tq_many_prepare_kernel(TqManyArgs a, uint32_t waves) {
+    __shared__ float lds_top[16];
+    const uint32_t lane = threadIdx.x & 63u, all = blockDim.x >> 6, every = tq_uniform32(threadIdx.x >> 6), side = every / waves, wave = every - side * waves;
+    const uint32_t pairs = (a.tiles + 1u) / 2u, row = blockIdx.x / pairs, tile = 2u * (blockIdx.x - row * pairs) + side;
+    const uint32_t DP = 32u * waves, steps = 2u * waves;
     const uint32_t n = lane & 31u, hk = lane >> 5, m = tile * 32u + n;
     constexpr int NT = plain_terms<DT>();
     const uint8_t *q = many_query(a, row, min(m, a.M - 1u), DT == TQ_F32 ? 4u : 2u);
@@ -41,13 +42,15 @@ __global__ __launch_bounds__(512) void tq_many_prepare_kernel(TqManyArgs a) {
     }
 #pragma unroll
     for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-    if (lane == 0u) lds_top[wave] = top;
+    if (lane == 0u) lds_top[every] = top;
     __syncthreads();
-    for (uint32_t w = 0; w < waves; ++w) top = fmaxf(top, lds_top[w]);
+    for (uint32_t w = 0; w < all; ++w) top = fmaxf(top, lds_top[w]);
+    if (tile >= a.tiles) return;
+    const size_t at = (size_t)row * a.tiles + tile;
     const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
     const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-    if (threadIdx.x == 0) a.q_scale[blockIdx.x] = __uint_as_float((uint32_t)(127 - up - LEVEL_SHIFT) << 23);
-    uint8_t *dst = a.q_op + (size_t)blockIdx.x * q_operand_bytes(DP);
+    if (wave == 0u && lane == 0u) a.q_scale[at] = __uint_as_float((uint32_t)(127 - up - LEVEL_SHIFT) << 23);
+    uint8_t *dst = a.q_op + at * q_operand_bytes(DP);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         uint32_t t[8];
@@ -451,6 +454,7 @@ __global__ __launch_bounds__(2 * DP < 64 ? 64 : 2 * DP) void tq_many_merge_kerne
             tq_f4 sum = {0.f, 0.f, 0.f, 0.f};
             for (uint32_t r = 0; r < count; ++r) {
                 const float *p = src + (size_t)r * record_floats(DP);
+                if (p[n] == MANY_NONE) continue;           // (its sums need not have been written)
                 const float f = __builtin_amdgcn_exp2f(p[n] - lds_m[n]);
                 const tq_f4 o = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>((const TQ_GLOBAL float *)p + 64u + n * DP + d);
 #pragma unroll
