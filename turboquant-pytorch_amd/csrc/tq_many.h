@@ -35,6 +35,7 @@ struct TqManyArgs {
     float scale;
     uint32_t rows, heads, group, queries, M, tiles, tokens, packed_row_stride, D, bits_k, bits_v, dtype;
     uint32_t splits, chunk, records, plain_records;
+    uint32_t plain_blocks;           // blocks of a launch, its first ones, that work on the uncompressed tokens
     uint32_t aligned;                // vectors of queries and uncompressed tokens can be read 16 bytes at a time
 };
 
@@ -158,6 +159,15 @@ __device__ __forceinline__ const uint8_t *many_query(const TqManyArgs &a, uint32
     return a.q + ((long long)b * a.q_batch + (long long)(h * a.group + q.g) * a.q_head + (long long)q.t * a.q_token) * elem_bytes;
 }
 
+// Whether a query with token position `own` sees uncompressed token t (`which`: 0 window, 1 drafts)
+__device__ __forceinline__ bool plain_seen(const TqManyArgs &a, uint32_t which, uint32_t b, uint32_t own, uint32_t t, uint32_t length) {
+    if (which == 0u) {
+        const uint32_t at = a.tokens + t;
+        return at < length && (!a.mask || a.mask[(long long)b * a.mask_stride + at]);
+    }
+    return a.tree ? a.tree[(long long)b * a.tree_batch + (long long)own * a.plain[1].n + t] != 0 : t <= own;
+}
+
 // Keys of sequence b (packed, then window) that can count
 __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b) {
     const uint32_t all = a.tokens + a.plain[0].n;
@@ -172,3 +182,7 @@ __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b)
 int tq_many_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
 int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
 int tq_many_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
+// the same for tq_many_weights_kernel, `blocks` a row
+int tq_many_weights_launch_d64(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);
+int tq_many_weights_launch_d128(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);
+int tq_many_weights_launch_d256(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);

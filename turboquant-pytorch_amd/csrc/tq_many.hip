@@ -9,6 +9,8 @@ constexpr int MAX_SPLITS = 64;
 
 int padded(int D) { return TQ_PADDED_DIM(D); }
 
+long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 31) / 32 + (r->drafts.tokens + 31) / 32; }
+
 struct Plan {
     long long rows, tiles, groups, splits, records, plain_records, floats;
     int qt, kt;                      // tiles a block and fp16 terms of the kernels for one head dimension; qt = 0: the one for all
@@ -22,21 +24,20 @@ bool fast(const tq_attend_request *r) {
 }
 
 // splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and what its start
-// and its end cost
-long long fast_splits(long long blocks, long long tokens) {
+// and its end cost; `others`: blocks of uncompressed tokens in the same launch
+long long fast_splits(long long blocks, long long others, long long tokens) {
     int cus = 0;
     if (tq_device_cus(cus)) cus = 256;
     long long most = (tokens + 255) / 256, best = 1, best_cost = 0;
     if (most > MAX_SPLITS) most = MAX_SPLITS;
     for (long long s = 1; s <= most; ++s) {
-        const long long rounds = (blocks * s + cus - 1) / cus, cost = rounds * ((tokens + s - 1) / s + 1500) + 30 * s;
+        const long long rounds = (blocks * s + others + cus - 1) / cus, cost = rounds * ((tokens + s - 1) / s + 1500) + 30 * s;
         if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
         if (rounds > 16 && s > 1) break;
     }
     return best;
 }
 
-long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 31) / 32 + (r->drafts.tokens + 31) / 32; }
 
 int plan(const tq_attend_request *r, Plan &p) {
     p.rows = r->batch * r->heads;
@@ -49,7 +50,7 @@ int plan(const tq_attend_request *r, Plan &p) {
         p.kt = r->dtype == TQ_BF16 && !r->weights ? 1 : 2;
         p.qt = p.kt == 1 && r->head_dim != 256 && p.tiles > 1 ? 2 : 1;
         p.groups = (p.tiles + p.qt - 1) / p.qt;
-        p.splits = fast_splits(p.rows * p.groups, r->tokens);
+        p.splits = fast_splits(p.rows * p.groups, plain_tiles(r) ? p.rows * p.groups : 0, r->tokens);
     } else if (at && r->tokens) {
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
@@ -60,10 +61,10 @@ int plan(const tq_attend_request *r, Plan &p) {
         if (p.splits < 1) p.splits = 1;
     }
     p.records = r->tokens ? p.splits * (p.qt ? 1 : ANY_WAVES) : 0;
-    p.plain_records = plain_tiles(r) ? PLAIN_WAVES : 0;
+    p.plain_records = plain_tiles(r) ? (p.qt ? 1 : PLAIN_WAVES) : 0;
     const long long dp = padded(r->head_dim);
     p.floats = at * ((long long)q_operand_bytes((uint32_t)dp) / 4 + (p.records + p.plain_records) * record_floats((uint32_t)dp) + 64) + (at + 3) / 4 * 4;
-    return at * p.splits > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;
+    return at * (p.splits + 1) * 4 > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;
 }
 
 int check(const tq_attend_request *r) {
@@ -95,21 +96,33 @@ template <int DP>
 void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     const uint32_t at = a.rows * a.tiles;
     if (a.records && plan.qt) {
-        const dim3 g((unsigned)(plan.rows * plan.groups * plan.splits));
+        const dim3 g((unsigned)(plan.rows * plan.groups * plan.splits + a.plain_blocks));
         const int ik = 8 / (int)a.bits_k, iv = 8 / (int)a.bits_v;
         if constexpr (DP == 64) tq_many_launch_d64(ik, iv, g, s, a, plan.qt, plan.kt);
         if constexpr (DP == 128) tq_many_launch_d128(ik, iv, g, s, a, plan.qt, plan.kt);
         if constexpr (DP == 256) tq_many_launch_d256(ik, iv, g, s, a, plan.qt, plan.kt);
     } else if (a.records) hipLaunchKernelGGL((tq_many_any_kernel<DP>), dim3(at * a.splits), dim3(64 * ANY_WAVES), 0, s, a);
-    if (a.plain_records) {
+    if (a.plain_records && !plan.qt) {
         const dim3 g(at), t(64 * PLAIN_WAVES);
         if (a.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F32>), g, t, 0, s, a);
         else if (a.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F16>), g, t, 0, s, a);
         else hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_BF16>), g, t, 0, s, a);
     }
-    hipLaunchKernelGGL((tq_many_merge_kernel<DP>), dim3(at), dim3(2 * DP), 0, s, a);
+    if (at < 512u) hipLaunchKernelGGL((tq_many_merge_kernel<DP, 8>), dim3(at * 4u), dim3(2 * DP), 0, s, a);
+    else hipLaunchKernelGGL((tq_many_merge_kernel<DP, 32>), dim3(at), dim3(2 * DP), 0, s, a);
     if (!a.weights) return;
-    if (a.tokens) {
+    if (a.tokens && plan.qt) {
+        int cus = 0;
+        if (tq_device_cus(cus)) cus = 256;
+        const uint32_t most = (a.tokens + 32u * 8u - 1u) / (32u * 8u);
+        uint32_t blocks = ((uint32_t)cus + a.rows - 1u) / a.rows;
+        if (blocks > most) blocks = most;
+        const dim3 g(a.rows * blocks);
+        const int ik = 8 / (int)a.bits_k;
+        if constexpr (DP == 64) tq_many_weights_launch_d64(ik, g, s, a, blocks);
+        if constexpr (DP == 128) tq_many_weights_launch_d128(ik, g, s, a, blocks);
+        if constexpr (DP == 256) tq_many_weights_launch_d256(ik, g, s, a, blocks);
+    } else if (a.tokens) {
         const uint32_t blocks = (a.tokens + 32u * ANY_WAVES - 1u) / (32u * ANY_WAVES);
         hipLaunchKernelGGL((tq_many_any_weights_kernel<DP>), dim3(a.rows * blocks), dim3(64 * ANY_WAVES), 0, s, a, blocks);
     }
@@ -181,7 +194,8 @@ extern "C" int tq_attend_many(const tq_attend_request *request, float *scratch, 
     a.aligned = !(r.head_dim & 7) && !((uintptr_t)r.queries & 15u) && !((r.q_batch * es) & 15) && !((r.q_head * es) & 15) && !((r.q_token * es) & 15) &&
                 (!r.window.tokens || aligned16(r.window, es)) && (!r.drafts.tokens || aligned16(r.drafts, es));
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    {
+    a.plain_blocks = p.qt && p.plain_records ? (uint32_t)(p.rows * p.groups) : 0u;
+    if (!p.qt) {
         const dim3 g((unsigned)(p.rows * ((p.tiles + 1) / 2))), t((p.tiles > 1 ? 4 : 2) * dp);
         if (r.dtype == TQ_F32) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F32>), g, t, 0, s, a, dp / 32u);
         else if (r.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_prepare_kernel<TQ_F16>), g, t, 0, s, a, dp / 32u);

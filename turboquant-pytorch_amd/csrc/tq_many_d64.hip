@@ -5,3 +5,9 @@ int tq_many_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqMan
     if (ipbk == 2) return launch_many_fast<64, 2>(ipbv, grid, s, a, qt, kt);
     return launch_many_fast<64, 1>(ipbv, grid, s, a, qt, kt);
 }
+
+int tq_many_weights_launch_d64(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks) {
+    if (ipbk == 4) return launch_many_weights<64, 4>(grid, s, a, blocks);
+    if (ipbk == 2) return launch_many_weights<64, 2>(grid, s, a, blocks);
+    return launch_many_weights<64, 1>(grid, s, a, blocks);
+}

@@ -108,6 +108,286 @@ struct ValueBytes {
     }
 };
 
+// Eight 16-bit elements from any address
+__device__ __forceinline__ tq_u4 load_elements(const uint8_t *p, bool aligned) {
+    if (aligned) return tq_gload16(p);
+    tq_u4 v;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+        v[d] = (uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * d) | ((uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * d + 1) << 16);
+    return v;
+}
+
+// Queries of QT tiles into the codec's space, q' = scale * log2(e) * Pi_k q, as fp16 operands in LDS ([tile][term][step][lane], as q_operand_bytes says): wave (tile i, w)
+// has coordinates 32 w ... + 31.  Pi as three bf16 terms, or for fp16 queries two fp16 ones (22 bits).  All tiles are scaled by the power of two
+// that puts their largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)); returns what products with them are to be multiplied by.
+template <int D, int QT, int KT, bool BF>
+__device__ __forceinline__ float rotate_queries(const TqManyArgs &a, uint32_t row, uint32_t tile0, uint8_t *ops, float *lds_top, uint32_t wave, uint32_t lane) {
+    constexpr int NC = D / 32, STEPS = D / 16, CH = STEPS < 8 ? STEPS : 8, TERMS = BF ? 3 : 2;
+    const uint32_t n = lane & 31u, h = lane >> 5, i = wave / NC, w = wave % NC;
+    float y[16], top = 0.f;
+    if (i < (uint32_t)QT) {
+        const uint32_t m = (tile0 + i) * 32u + n;
+        const uint8_t *q = many_query(a, row, min(m, a.M - 1u), 2u) + 16u * h;
+        const uint8_t *pi = a.table_k + (BF ? TQ_OFF_A_BF16(D) : TQ_OFF_A_F16) + ((size_t)w * STEPS * 64u + lane) * 16u;
+        tq_f16v acc = tq_zero16();
+#pragma unroll 1
+        for (int s0 = 0; s0 < STEPS; s0 += CH) {
+            tq_u4 x[CH], p[TERMS][CH];
+#pragma unroll
+            for (int s = 0; s < CH; ++s) {
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) p[t][s] = tq_gload16(pi + (size_t)t * TQ_OPERAND_BYTES_FOR(D) + (size_t)(s0 + s) * 1024u);
+            }
+            if (a.aligned) {
+#pragma unroll
+                for (int s = 0; s < CH; ++s) x[s] = tq_gload16(q + 32u * (s0 + s));
+            } else {
+#pragma unroll
+                for (int s = 0; s < CH; ++s) x[s] = load_elements(q + 32u * (s0 + s), false);
+            }
+#pragma unroll
+            for (int s = 0; s < CH; ++s)
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) acc = BF ? mfma_bf16(p[t][s], x[s], acc) : mfma_f16(p[t][s], x[s], acc);
+        }
+        const float f = a.scale * (BF ? LOG2E : LOG2E / (float)(1 << TQ_F16_PI_SHIFT));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {       // (the table's rows: register r of half h is coordinate 32 w + 16 h + r)
+            y[r] = m < a.M ? acc[r] * f : 0.f;
+            const float v = fabsf(y[r]);
+            top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
+        }
+        top = reduce_wave(top, OpMax());
+    }
+    if (lane == 0u) lds_top[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < FAST_WAVES; ++k) top = fmaxf(top, lds_top[k]);
+    const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+    const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+    if (i < (uint32_t)QT) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = fp16_terms(y[8 * j + k] * f);
+            tq_u4 hi, lo;
+            fp16_operands(t, hi, lo);
+            const uint32_t d = 32u * w + 16u * h + 8u * j, half = d / (D / 2u), s = (d - half * (D / 2u)) / 8u;
+            uint8_t *p = ops + ((i * KT * STEPS + s) * 64u + half * 32u + n) * 16u;
+            *reinterpret_cast<tq_u4 *>(p) = hi;
+            if constexpr (KT == 2) *reinterpret_cast<tq_u4 *>(p + STEPS * 1024u) = lo;
+        }
+    }
+    return __uint_as_float((uint32_t)(127 - up - (KT == 2 ? LEVEL_SHIFT : 0)) << 23);
+}
+
+// 32 uncompressed tokens of a row (`which`: 0 the window, 1 the drafts; from t0 on) against a tile of queries: raw 16-bit products are exact, weights enter the value
+// product as three bf16 terms, or two fp16 ones.  Coordinates of the sums as in the packed loop: row r of acc[c] is coordinate NC r + c.  Infinite and NaN
+// values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); the answer says whether there were any.
+template <int D, bool BF>
+__device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, uint32_t t0, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t lane,
+                                           float &m_ref, float &l, tq_f16v (&acc)[D / 32]) {
+    constexpr int NC = D / 32, STEPS = D / 16, PT = BF ? 3 : 2, VT = NC == 8 ? 8 : 16;       // VT: tokens whose values are held at a time
+    const TqManyPlain &seg = a.plain[which];
+    const uint32_t n = lane & 31u, h = lane >> 5, kv = row - b * a.heads;
+    const uint8_t *k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 2 + 16u * h;
+    const uint8_t *v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 2 + 2u * NC * n;
+    constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
+    bool wild = false;
+    uint32_t vw[VT][NC / 2];
+    auto load_values = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < VT; ++j) {
+            const uint8_t *p = v + (long long)min(t0 + acc_row(j0 + j, h), seg.n - 1u) * seg.v_token * 2;
+            if (a.aligned) {
+                if constexpr (NC == 2) vw[j][0] = tq_gload4(p);
+                else if constexpr (NC == 4) { const tq_u2 x = tq_gload8(p); vw[j][0] = x[0]; vw[j][1] = x[1]; }
+                else { const tq_u4 x = tq_gload16(p); vw[j][0] = x[0]; vw[j][1] = x[1]; vw[j][NC / 2 - 2] = x[2]; vw[j][NC / 2 - 1] = x[3]; }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC / 2; ++c)
+                    vw[j][c] = (uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * c) | ((uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * c + 1) << 16);
+            }
+        }
+    };
+    auto tame_values = [&](int j0) __attribute__((always_inline)) {
+        uint32_t over = 0u;
+#pragma unroll
+        for (int j = 0; j < VT; ++j)
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) {
+                if (t0 + acc_row(j0 + j, h) >= seg.n) vw[j][c] = 0u;
+                over |= (vw[j][c] & EXPO) + ONE;         // (an exponent of ones carries into the sign's place)
+            }
+        if (__any((over & 0x80008000u) != 0u)) {
+            wild = true;
+#pragma unroll
+            for (int j = 0; j < VT; ++j)
+#pragma unroll
+                for (int c = 0; c < NC / 2; ++c) vw[j][c] &= ~(((((vw[j][c] & EXPO) + ONE) >> 15) & 0x00010001u) * 0xffffu);
+        }
+    };
+    if constexpr (VT == 16) load_values(0);
+    {
+        const uint32_t m = min(tile * 32u + n, a.M - 1u);
+        const uint8_t *q = many_query(a, row, m, 2u) + 16u * h;
+        tq_f16v s = tq_zero16();
+        if (a.aligned) {
+#pragma unroll 1
+            for (int s0 = 0; s0 < STEPS; s0 += 4) {
+                tq_u4 x[4], y[4];
+#pragma unroll
+                for (int st = 0; st < 4; ++st) { x[st] = tq_gload16(k + 32 * (s0 + st)); y[st] = tq_gload16(q + 32 * (s0 + st)); }
+#pragma unroll
+                for (int st = 0; st < 4; ++st) s = BF ? mfma_bf16(x[st], y[st], s) : mfma_f16(x[st], y[st], s);
+            }
+        } else {
+#pragma unroll 1
+            for (int st = 0; st < STEPS; ++st) {
+                const tq_u4 x = load_elements(k + 32 * st, false), y = load_elements(q + 32 * st, false);
+                s = BF ? mfma_bf16(x, y, s) : mfma_f16(x, y, s);
+            }
+        }
+        const uint32_t own = ManyQuery(a, m).t;
+        float x[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint32_t t = t0 + acc_row(r, h);
+            x[r] = t < seg.n && plain_seen(a, which, b, own, t, length) ? s[r] * (a.scale * LOG2E) : MANY_NONE;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+        top = fmaxf(halves_max(top), m_ref);
+        const float shrink = __builtin_amdgcn_exp2f(m_ref - top);
+        m_ref = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = x[r] == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(x[r] - top);
+            sum += x[r];
+        }
+        l = l * shrink + sum;          // (this lane's half)
+        if (__any(shrink != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[c] *= shrink;
+        }
+        if constexpr (VT == 16) {
+            tame_values(0);
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            if constexpr (VT == 8) {
+                load_values(8 * st);
+                tame_values(8 * st);
+            }
+            tq_u4 p[3];
+            float ps[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ps[j] = x[8 * st + j];
+            if constexpr (BF) bf16_terms(ps, p);
+            else {
+                uint32_t t[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = fp16_terms(ps[j]);
+                fp16_operands(t, p[0], p[1]);
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                tq_u4 o;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    o[d] = __builtin_amdgcn_perm(vw[(VT == 16 ? 8 * st : 0) + 2 * d + 1][c / 2], vw[(VT == 16 ? 8 * st : 0) + 2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int t = 0; t < PT; ++t) acc[c] = BF ? mfma_bf16(o, p[t], acc[c]) : mfma_f16(o, p[t], acc[c]);
+            }
+        }
+    }
+    return wild;
+}
+
+// Infinite and NaN values of a row's uncompressed tokens into the sums of the queries that see them, whatever their weight (it is not zero).
+template <int D>
+__device__ __forceinline__ void add_wild(const TqManyArgs &a, float *rec, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t tid) {
+    const uint32_t kv = row - b * a.heads, elem = a.dtype;
+    for (uint32_t e = tid; e < 32u * D; e += FAST_THREADS) {
+        const uint32_t col = e / D, d = e - col * D, m = tile * 32u + col;
+        if (m >= a.M) return;
+        const uint32_t own = ManyQuery(a, m).t;
+        float sum = 0.f;
+        for (uint32_t which = 0; which < 2u; ++which) {
+            const TqManyPlain &seg = a.plain[which];
+            for (uint32_t t = 0; t < seg.n; ++t) {
+                const float v = plain_element(seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head + (long long)t * seg.v_token + d) * 2, elem);
+                if (!(fabsf(v) < __builtin_inff()) && plain_seen(a, which, b, own, t, length)) sum += v;
+            }
+        }
+        if (sum != 0.f) rec[64u + e] += sum;
+    }
+}
+
+// The sums of a block's waves, QT tiles of queries, into the block's record of each tile (its first float: rec + i * tile_step).  unit: what this wave's value sums are
+// multiplied by; m_ref: MANY_NONE where a wave has seen no token of a query; l: this lane's half.
+template <int D, int QT>
+__device__ __forceinline__ void put_block(uint8_t *lds, float (*lds_m)[32 * QT], float (*lds_l)[32 * QT], float *rec, size_t tile_step, uint32_t tiles, float unit, const float (&m_ref)[QT],
+                                          const float (&l)[QT], const tq_f16v (&acc)[QT][D / 32], uint32_t tid) {
+    constexpr int NC = D / 32, TC = NC < 4 ? NC : 4, MROW = 32 * TC + 4;
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const float both = halves_add(l[i]);
+        if (h == 0u) {
+            lds_m[wave][32 * i + n] = m_ref[i];
+            lds_l[wave][32 * i + n] = both;
+        }
+    }
+    __syncthreads();
+    float *area = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        if ((uint32_t)i >= tiles) break;
+        float m = MANY_NONE;
+#pragma unroll
+        for (int w = 0; w < FAST_WAVES; ++w) m = fmaxf(m, lds_m[w][32 * i + n]);
+        float *dst_rec = rec + i * tile_step;
+        if (tid < 32u) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < FAST_WAVES; ++w) sum = fmaf(lds_l[w][32 * i + n], __builtin_amdgcn_exp2f(lds_m[w][32 * i + n] - m), sum);
+            dst_rec[n] = m;
+            dst_rec[32u + n] = sum;
+        }
+        const float f = unit * __builtin_amdgcn_exp2f(lds_m[wave][32 * i + n] - m);
+#pragma unroll
+        for (int c0 = 0; c0 < NC; c0 += TC) {
+            if (i || c0) __syncthreads();
+#pragma unroll
+            for (int c = 0; c < TC; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<tq_f4 *>(area + (wave * 32u + n) * MROW + 32 * c + 8 * k + 4 * h) =
+                        tq_f4{acc[i][c0 + c][4 * k] * f, acc[i][c0 + c][4 * k + 1] * f, acc[i][c0 + c][4 * k + 2] * f, acc[i][c0 + c][4 * k + 3] * f};
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t pair = tid + e * FAST_THREADS, col = pair / 32u, r = pair % 32u;       // coordinates NC r + c0 ... of query col
+                float sum[TC];
+#pragma unroll
+                for (int c = 0; c < TC; ++c) sum[c] = 0.f;
+#pragma unroll
+                for (int w = 0; w < FAST_WAVES; ++w)
+#pragma unroll
+                    for (int c = 0; c < TC; ++c) sum[c] += area[(w * 32 + col) * MROW + 32 * c + r];
+                TQ_GLOBAL float *dst = (TQ_GLOBAL float *)dst_rec + 64u + col * D + NC * r + c0;
+                if constexpr (TC == 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(dst) = tq_f4{sum[0], sum[1], sum[2], sum[3]};
+                else { dst[0] = sum[0]; dst[1] = sum[1]; }
+            }
+        }
+    }
+}
+
 // Block = (row, QT tiles of 32 queries, split): its waves take runs of 32 tokens in turn, each by itself, and their sums meet in LDS at the end.
 //   * scores transposed: A = keys, decoded from the lane's own bytes by table, B = queries; a lane then has 16 tokens of one query;
 //   * softmax in base 2 against a reference per query that moves only when a logit exceeds it by 2^FAST_SLACK: no exchange between lanes;
@@ -123,9 +403,10 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     using Values = ValueBytes<IPBV, NC>;
     constexpr int QW = KT * QT * STEPS * 4;                                        // registers of the queries' operands
     constexpr bool QREG = QW + QT * NC * 16 <= 136;
-    constexpr int TC = NC < 4 ? NC : 4, MROW = 32 * TC + 4;                        // sums of a wave on their way through LDS, 32 TC coordinates at a time
-    constexpr int LUT_BYTES = 65536, Q_BYTES = QREG ? 0 : KT * QT * STEPS * 1024, MERGE_BYTES = FAST_WAVES * 32 * MROW * 4;
+    constexpr int TC = NC < 4 ? NC : 4;
+    constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024, MERGE_BYTES = FAST_WAVES * 32 * (32 * TC + 4) * 4;
     constexpr int AREA = LUT_BYTES + Q_BYTES > MERGE_BYTES ? LUT_BYTES + Q_BYTES : MERGE_BYTES;
+    static_assert(QT * NC <= FAST_WAVES, "waves that rotate");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[FAST_WAVES][32];
     __shared__ __attribute__((aligned(16))) uint16_t lds_vn[FAST_WAVES][32];
@@ -133,10 +414,45 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const uint32_t groups = (a.tiles + QT - 1u) / QT;
-    const uint32_t split = blockIdx.x % a.splits, at = blockIdx.x / a.splits, row = at / groups, tile0 = (at - row * groups) * QT, b = row / a.heads;
+    const bool packed = blockIdx.x >= a.plain_blocks;
+    const uint32_t block = packed ? blockIdx.x - a.plain_blocks : blockIdx.x;
+    const uint32_t split = packed ? block % a.splits : 0u, at = packed ? block / a.splits : block, row = at / groups, tile0 = (at - row * groups) * QT, b = row / a.heads;
     const size_t first_tile = (size_t)row * a.tiles + tile0;
-    const bool both = QT == 1 || tile0 + 1u < a.tiles;
-    const uint8_t *q_op = a.q_op + first_tile * q_operand_bytes(D);
+    const uint32_t tiles = min((uint32_t)QT, a.tiles - tile0);
+    const uint32_t length = many_length(a, b);
+
+    if (!packed) {
+        // A block of uncompressed tokens, window first: few, and first in the launch, so that they are done while the others are at the packed ones
+        const uint32_t first = (a.plain[0].n + 31u) / 32u, all = first + (a.plain[1].n + 31u) / 32u;
+        // (a tile of queries at a time: its sums and its tokens' values share the registers)
+#pragma unroll 1
+        for (uint32_t i = 0; i < tiles; ++i) {
+            float m1[1] = {MANY_NONE}, l1[1] = {0.f};
+            tq_f16v acc1[1][NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc1[0][c] = tq_zero16();
+            bool wild = false;
+#pragma unroll 1
+            for (uint32_t w = wave; w < all; w += FAST_WAVES) {
+                const uint32_t which = w < first ? 0u : 1u, t0 = 32u * (which ? w - first : w);
+                if (a.dtype == TQ_BF16) wild |= plain_tile<D, true>(a, which, t0, row, b, tile0 + i, length, lane, m1[0], l1[0], acc1[0]);
+                else wild |= plain_tile<D, false>(a, which, t0, row, b, tile0 + i, length, lane, m1[0], l1[0], acc1[0]);
+            }
+            if (i) __syncthreads();           // (what the last tile's sums went through)
+            if (lane == 0u) lds_kn[0][wave] = wild ? 1.f : 0.f;
+            float *rec = a.plain_rec + (first_tile + i) * record_floats(D);
+            put_block<D, 1>(lds, reinterpret_cast<float (*)[32]>(&lds_m[0][0]), reinterpret_cast<float (*)[32]>(&lds_l[0][0]), rec, 0, 1u, 1.f, m1, l1, acc1, tid);
+            float any = 0.f;
+#pragma unroll
+            for (int w = 0; w < FAST_WAVES; ++w) any += lds_kn[0][w];
+            if (any != 0.f) {
+                __threadfence_block();
+                __syncthreads();              // (what put_block has stored)
+                add_wild<D>(a, rec, row, b, tile0 + i, length, tid);
+            }
+        }
+        return;
+    }
 
     if constexpr (KT == 1) {
         Lut<IPBK> table;
@@ -152,29 +468,26 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         table.load(a.table_v + TQ_OFF_LUT(D), tid);
         table.store(lds + 128, tid);
     }
+    uint8_t *ops = lds + LUT_BYTES;
+    const float q_scale = a.dtype == TQ_BF16 ? rotate_queries<D, QT, KT, true>(a, row, tile0, ops, lds_kn[0], wave, lane) : rotate_queries<D, QT, KT, false>(a, row, tile0, ops, lds_kn[0], wave, lane);
+    __syncthreads();
     tq_u4 q[QREG ? KT * QT * STEPS : 1];
-    // operands of a tile: [term][step][lane]; one term is all that KT = 1 reads
+    if constexpr (QREG) {
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const uint8_t *src = q_op + (i && both ? q_operand_bytes(D) : 0u);
-        if constexpr (QREG) {
-#pragma unroll
-            for (int s = 0; s < KT * STEPS; ++s) q[i * KT * STEPS + s] = tq_gload16(src + (size_t)s * 1024u + lane * 16u);
-        } else {
-            tq_copy_to_lds(lds + LUT_BYTES + i * KT * STEPS * 1024, src, KT * STEPS * 1024, tid, FAST_THREADS);
-        }
+        for (int s = 0; s < KT * QT * STEPS; ++s) q[s] = *reinterpret_cast<const tq_u4 *>(ops + s * 1024 + lane * 16u);
     }
     auto query = [&](int i, int term, int s) __attribute__((always_inline)) -> tq_u4 {
         if constexpr (QREG) return q[(i * KT + term) * STEPS + s];
-        else return *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + ((i * KT + term) * STEPS + s) * 1024 + lane * 16u);
+        else return *reinterpret_cast<const tq_u4 *>(ops + ((i * KT + term) * STEPS + s) * 1024 + lane * 16u);
     };
-    // (the levels of KT = 1 come without 2^LEVEL_SHIFT)
-    const float q_scale = a.q_scale[first_tile] * (KT == 1 ? (float)(1 << LEVEL_SHIFT) : 1.f);
+    if (a.weights && split == 0u) {          // (KT = 2: whole operands) for the launch that adds up what keys receive
+        for (uint32_t i = tid; i < Q_BYTES / 16u; i += FAST_THREADS) tq_gstore16(a.q_op + first_tile * q_operand_bytes(D) + i * 16u, *reinterpret_cast<const tq_u4 *>(ops + i * 16u));
+        if (tid == 0u) a.q_scale[first_tile] = q_scale;
+    }
     const uint32_t slot_k = KT == 1 ? RepLut<IPBK>::lane_offset(lane) : Lut2<IPBK>::lane_offset(lane);
     const uint32_t slot_v = 128u + (IPBV == 4 && NC == 2 ? (lane & 30u) / 2u * 8u + 4u * (lane & 1u) : RepLut<IPBV>::lane_offset(lane));
-    __syncthreads();
 
-    const uint32_t seen = min(a.tokens, many_length(a, b));
+    const uint32_t seen = min(a.tokens, length);
     const uint32_t chunk = a.lengths ? ((seen + a.splits - 1u) / a.splits + 31u) / 32u * 32u : a.chunk;       // (a short sequence keeps all its blocks busy)
     const uint32_t begin = min(seen, split * chunk), end = min(seen, begin + chunk);
     const size_t slot0 = (size_t)row * a.packed_row_stride;
@@ -354,61 +667,106 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         wave_sync();
     }
 
-    // ---- the waves' sums, and the block's record of each tile
+    // ---- the block's record of each tile
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        l[i] = halves_add(l[i]) * (1.0f / (float)(1 << FAST_P));
-        if (h == 0u) {
-            lds_m[wave][32 * i + n] = m_ref[i] == FAST_START ? MANY_NONE : m_ref[i];
-            lds_l[wave][32 * i + n] = l[i];
-        }
+        m_ref[i] = m_ref[i] == FAST_START ? MANY_NONE : m_ref[i];
+        l[i] *= 1.0f / (float)(1 << FAST_P);
     }
-    __syncthreads();
-    float *area = reinterpret_cast<float *>(lds);
     const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P) << 23);
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        float m = MANY_NONE;
-#pragma unroll
-        for (int w = 0; w < FAST_WAVES; ++w) m = fmaxf(m, lds_m[w][32 * i + n]);
-        const bool write = i == 0 || both;
-        float *rec = a.rec + ((first_tile + i) * a.records + split) * record_floats(D);
-        if (tid < 32u && write) {
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < FAST_WAVES; ++w) sum = fmaf(lds_l[w][32 * i + n], __builtin_amdgcn_exp2f(lds_m[w][32 * i + n] - m), sum);
-            rec[n] = m;
-            rec[32u + n] = sum;
-        }
-        const float f = unit * __builtin_amdgcn_exp2f(lds_m[wave][32 * i + n] - m);
-#pragma unroll
-        for (int c0 = 0; c0 < NC; c0 += TC) {
-            if (i || c0) __syncthreads();
-#pragma unroll
-            for (int c = 0; c < TC; ++c)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    *reinterpret_cast<tq_f4 *>(area + (wave * 32u + n) * MROW + 32 * c + 8 * k + 4 * h) =
-                        tq_f4{acc[i][c0 + c][4 * k] * f, acc[i][c0 + c][4 * k + 1] * f, acc[i][c0 + c][4 * k + 2] * f, acc[i][c0 + c][4 * k + 3] * f};
-            __syncthreads();
-            if (write) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t pair = tid + e * FAST_THREADS, col = pair / 32u, r = pair % 32u;       // coordinates NC r + c0 ... of query col
-                    float sum[TC];
-#pragma unroll
-                    for (int c = 0; c < TC; ++c) sum[c] = 0.f;
-#pragma unroll
-                    for (int w = 0; w < FAST_WAVES; ++w)
-#pragma unroll
-                        for (int c = 0; c < TC; ++c) sum[c] += area[(w * 32 + col) * MROW + 32 * c + r];
-                    TQ_GLOBAL float *dst = (TQ_GLOBAL float *)rec + 64u + col * D + NC * r + c0;
-                    if constexpr (TC == 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(dst) = tq_f4{sum[0], sum[1], sum[2], sum[3]};
-                    else { dst[0] = sum[0]; dst[1] = sum[1]; }
-                }
-            }
-        }
+    __syncthreads();
+    put_block<D, QT>(lds, lds_m, lds_l, a.rec + (first_tile * a.records + split) * record_floats(D), (size_t)a.records * record_floats(D), tiles, unit, m_ref, l, acc, tid);
+}
+
+// What the packed tokens receive: weight = 2^(logit - largest) / sum with the statistics of the merge, from the two-term products.  Rows of the product are queries
+// here, columns tokens, so that a token's sum is made in its lane; rows in which a tile has no query are left out eight at a time.  Block = part of
+// a row's tokens, a wave takes 32 at a time and all tiles of queries in order (the first one's operands lie in LDS, a decode step has no more).
+template <int D, int IPBK>
+__global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_kernel(TqManyArgs a, uint32_t blocks) {
+    constexpr int STEPS = D / 16, KB = D / 2 / IPBK, KW = KB / 4, GBK = D / IPBK, LUT_BYTES = 65536;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LUT_BYTES + 2 * STEPS * 1024];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
+    const uint32_t row = blockIdx.x / blocks, b = row / a.heads;
+    const size_t first_tile = (size_t)row * a.tiles;
+    const uint32_t seen = min(a.tokens, many_length(a, b));
+    {
+        Lut2<IPBK> table;
+        table.load(a.table_k, a.bits_k, D, tid);
+        table.store(lds, tid);
     }
+    tq_copy_to_lds(lds + LUT_BYTES, a.q_op + first_tile * q_operand_bytes(D), 2 * STEPS * 1024, tid, FAST_THREADS);
+    const uint32_t slot = Lut2<IPBK>::lane_offset(lane);
+    const float scale0 = a.q_scale[first_tile];
+    __syncthreads();
+    const size_t slot0 = (size_t)row * a.packed_row_stride;
+    const uint32_t last = a.tokens - 32u, step = 32u * FAST_WAVES * blocks;
+    for (uint32_t t_run = 32u * ((blockIdx.x - row * blocks) * FAST_WAVES + wave); t_run < seen; t_run += step) {
+        const uint32_t t0 = min(t_run, last), t = t0 + n;
+        uint32_t kraw[KW];
+        const uint8_t *p = a.k_idx + (slot0 + t) * GBK + h * KB;
+        if constexpr (KB % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < KB / 16; ++i) {
+                const tq_u4 v = tq_gload16(p + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) kraw[4 * i + j] = v[j];
+            }
+        } else {
+            const tq_u2 v = tq_gload8(p);
+            kraw[0] = v[0]; kraw[1] = v[1];
+        }
+        const float norm = (float)__builtin_bit_cast(_Float16, tq_gload2(a.k_norms + slot0 + t));
+        const bool counts = t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
+        float *dst = a.weights + (long long)row * a.w_stride + t;
+        const float before = h == 0u && counts ? *dst : 0.f;
+        float w = 0.f;
+        auto add = [&](const tq_f16v &s, uint32_t tile, float kn, uint32_t queries) __attribute__((always_inline)) {
+            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * 64u + 4u * h;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (8u * g >= queries) break;
+                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(fmaf(s[4 * g + r], kn, -m[r])), inv[r], w);
+            }
+        };
+        {
+            tq_f16v s = tq_zero16();
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                tq_u4 hi, lo;
+                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
+                const tq_u4 qh = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + st * 1024 + lane * 16u), ql = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + (STEPS + st) * 1024 + lane * 16u);
+                s = mfma_f16(qh, hi, s);
+                s = mfma_f16(ql, hi, s);
+                s = mfma_f16(qh, lo, s);
+            }
+            add(s, 0u, norm * scale0, a.M);
+        }
+#pragma unroll 1
+        for (uint32_t tile = 1; tile < a.tiles; ++tile) {
+            const uint8_t *ops = a.q_op + (first_tile + tile) * q_operand_bytes(D) + lane * 16u;
+            tq_f16v s = tq_zero16();
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                tq_u4 hi, lo;
+                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
+                const tq_u4 qh = tq_gload16(ops + st * 1024), ql = tq_gload16(ops + (STEPS + st) * 1024);
+                s = mfma_f16(qh, hi, s);
+                s = mfma_f16(ql, hi, s);
+                s = mfma_f16(qh, lo, s);
+            }
+            add(s, tile, norm * a.q_scale[first_tile + tile], a.M - 32u * tile);
+        }
+        w = halves_add(w);
+        if (h == 0u && counts) *dst = before + w;
+    }
+}
+
+template <int D, int IPBK>
+int launch_many_weights(dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks) {
+    hipLaunchKernelGGL((tq_many_weights_kernel<D, IPBK>), grid, dim3(FAST_THREADS), 0, s, a, blocks);
+    return 0;
 }
 
 // ipb: codes per byte

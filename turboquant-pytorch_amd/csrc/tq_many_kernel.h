@@ -127,13 +127,7 @@ __device__ __forceinline__ void plain_logits(const TqManyArgs &a, const TqManyPl
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const uint32_t t = t0 + acc_row(r, h);
-        bool seen = t < seg.n;
-        if (seen && which == 0u) {
-            const uint32_t at = a.tokens + t;
-            seen = at < length && (!a.mask || a.mask[(long long)b * a.mask_stride + at]);
-        } else if (seen) {
-            seen = a.tree ? a.tree[(long long)b * a.tree_batch + (long long)i * seg.n + t] != 0 : t <= i;
-        }
+        const bool seen = t < seg.n && plain_seen(a, which, b, i, t, length);
         x[r] = seen ? acc[r] * (a.scale * LOG2E) : MANY_NONE;
     }
 }
@@ -420,72 +414,103 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------------------
-// Block (row, tile), DP / 32 waves: the records' sums with their factors, the packed ones turned back by Pi_v (two fp16 terms each of Pi_v^T,
+// Block (row, tile, C of its 32 queries), DP / 32 waves: the records' sums with their factors, the packed ones turned back by Pi_v (two fp16 terms each of Pi_v^T,
 // from the value codec's table, and of the sums: 22 bits), the uncompressed ones added, everything divided by the sum of weights.
-// A query that sees nothing gets zeros.
-template <int DP>
-__global__ __launch_bounds__(2 * DP < 64 ? 64 : 2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
-    constexpr uint32_t NT = 2 * DP, ROW = DP + 4;
-    __shared__ __attribute__((aligned(16))) float lds_o[2][32 * ROW];       // packed, plain
-    __shared__ float lds_m[32], lds_inv[32], lds_up[32];
-    const uint32_t row = blockIdx.x / a.tiles, tile = blockIdx.x - row * a.tiles, b = row / a.heads, kv = row - b * a.heads;
+// A query that sees nothing gets zeros.  C = 8 where tiles are few: the records are then read by four times as many blocks.
+constexpr uint32_t MERGE_RECORDS = 260;
+template <int DP, int C>
+__global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
+    constexpr uint32_t NT = 2 * DP, ROW = DP + 4, PARTS = NT / C, UNITS = C * DP / 4;      // (NT is a multiple of 64)
+    __shared__ __attribute__((aligned(16))) float lds_o[2][C * ROW];        // packed, plain
+    __shared__ float lds_f[MERGE_RECORDS][C], lds_red[2][PARTS][C], lds_top[C];
+    const uint32_t group = blockIdx.x % (32u / C), at = blockIdx.x / (32u / C);
+    const uint32_t row = at / a.tiles, tile = at - row * a.tiles, b = row / a.heads, kv = row - b * a.heads, col0 = group * C;
+    if (tile * 32u + col0 >= a.M && !a.stat) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n32 = lane & 31u, h = lane >> 5;
-    const float *rec = a.rec + (size_t)blockIdx.x * a.records * record_floats(DP), *plain = a.plain_rec + (size_t)blockIdx.x * a.plain_records * record_floats(DP);
-    if (tid < 32u) {
-        float m = MANY_NONE, l = 0.f;
-        for (uint32_t i = 0; i < a.records; ++i) m = fmaxf(m, rec[(size_t)i * record_floats(DP) + tid]);
-        for (uint32_t i = 0; i < a.plain_records; ++i) m = fmaxf(m, plain[(size_t)i * record_floats(DP) + tid]);
-        for (uint32_t i = 0; i < a.records; ++i) l = fmaf(rec[(size_t)i * record_floats(DP) + 32u + tid], __builtin_amdgcn_exp2f(rec[(size_t)i * record_floats(DP) + tid] - m), l);
-        for (uint32_t i = 0; i < a.plain_records; ++i) l = fmaf(plain[(size_t)i * record_floats(DP) + 32u + tid], __builtin_amdgcn_exp2f(plain[(size_t)i * record_floats(DP) + tid] - m), l);
-        lds_m[tid] = m;
-        lds_inv[tid] = l == 0.f ? 0.f : 1.0f / l;
-        if (a.stat) {
-            a.stat[(size_t)blockIdx.x * 64u + tid] = m;
-            a.stat[(size_t)blockIdx.x * 64u + 32u + tid] = tile * 32u + tid < a.M ? lds_inv[tid] : 0.f;
-        }
+    const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + (size_t)at * a.records * record_floats(DP);
+    const TQ_GLOBAL float *plain = (const TQ_GLOBAL float *)a.plain_rec + (size_t)at * a.plain_records * record_floats(DP);
+    const uint32_t all = a.records + a.plain_records;
+    auto record = [&](uint32_t i) { return i < a.records ? rec + (size_t)i * record_floats(DP) : plain + (size_t)(i - a.records) * record_floats(DP); };
+    const uint32_t c = tid % C, part = tid / C;
+    float top = MANY_NONE;
+    for (uint32_t i = part; i < all; i += PARTS) {
+        const float v = record(i)[col0 + c];
+        lds_f[i][c] = v;
+        top = fmaxf(top, v);
     }
+    lds_red[0][part][c] = top;
     __syncthreads();
+    for (uint32_t k = 0; k < PARTS; ++k) top = fmaxf(top, lds_red[0][k][c]);
+    float sum = 0.f;
+    for (uint32_t i = part; i < all; i += PARTS) {
+        const float v = lds_f[i][c], f = v == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(v - top);
+        lds_f[i][c] = f;
+        sum = fmaf(record(i)[32u + col0 + c], f, sum);
+    }
+    lds_red[1][part][c] = sum;
+    __syncthreads();
+    // ---- sums
 #pragma unroll
     for (uint32_t which = 0; which < 2; ++which) {
-        const float *src = which ? plain : rec;
-        const uint32_t count = which ? a.plain_records : a.records;
-        for (uint32_t i = tid; i < 32u * DP / 4u; i += NT) {
-            const uint32_t n = i / (DP / 4u), d = (i - n * (DP / 4u)) * 4u;
-            tq_f4 sum = {0.f, 0.f, 0.f, 0.f};
-            for (uint32_t r = 0; r < count; ++r) {
-                const float *p = src + (size_t)r * record_floats(DP);
-                if (p[n] == MANY_NONE) continue;           // (its sums need not have been written)
-                const float f = __builtin_amdgcn_exp2f(p[n] - lds_m[n]);
-                const tq_f4 o = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>((const TQ_GLOBAL float *)p + 64u + n * DP + d);
+        const TQ_GLOBAL float *src = (which ? plain : rec) + 64u + col0 * DP;
+        const uint32_t count = which ? a.plain_records : a.records, first = which ? a.records : 0u;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = fmaf(o[k], f, sum[k]);
+        for (uint32_t u = tid; u < UNITS; u += NT) {
+            const uint32_t q = u / (DP / 4u), d = (u - q * (DP / 4u)) * 4u;
+            tq_f4 o = {0.f, 0.f, 0.f, 0.f};
+            const TQ_GLOBAL float *p = src + q * DP + d;
+            for (uint32_t r0 = 0; r0 < count; r0 += 8u) {
+                tq_f4 v[8];
+                float f[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    const uint32_t r = min(r0 + k, count - 1u);
+                    v[k] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(p + (size_t)r * record_floats(DP));
+                    f[k] = r0 + k < count ? lds_f[first + r][q] : 0.f;
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k)
+                    if (f[k] != 0.f)           // (a record of no token: its sums need not have been written)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = fmaf(v[k][e], f[k], o[e]);
             }
-            *reinterpret_cast<tq_f4 *>(&lds_o[which][n * ROW + d]) = sum;
+            *reinterpret_cast<tq_f4 *>(&lds_o[which][q * ROW + d]) = o;
+        }
+    }
+    if (tid < (uint32_t)C) {
+        float l = 0.f;
+        for (uint32_t k = 0; k < PARTS; ++k) l += lds_red[1][k][tid];
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        lds_top[tid] = inv;
+        if (a.stat) {          // (a query that is none, or sees nothing: weights of zero)
+            const bool some = tile * 32u + col0 + tid < a.M && inv != 0.f;
+            a.stat[(size_t)at * 64u + col0 + tid] = some ? top : -MANY_NONE;
+            a.stat[(size_t)at * 64u + 32u + col0 + tid] = some ? inv : 0.f;
         }
     }
     __syncthreads();
-    if (wave == 0u) {          // a query's sums into the range of two fp16 terms
-        float top = 0.f;
-        for (uint32_t d = 0; d < DP / 2u; ++d) {
-            const float v = fabsf(lds_o[0][n32 * ROW + h * (DP / 2u) + d]);
-            top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
-        }
-        top = halves_max(top);
-        const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
-        if (h == 0u) lds_up[n32] = (float)up;
+    // ---- back out of the codec's space; columns past C repeat the others
+    const uint32_t q = n32 % C;
+    float largest = 0.f;
+#pragma unroll
+    for (uint32_t d = 0; d < DP / 2u; d += 4u) {
+        const tq_f4 v = *reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + h * (DP / 2u) + d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
     }
-    __syncthreads();
-    const int up = (int)lds_up[n32];
+    largest = halves_max(largest);
+    const int up = largest > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(largest) >> 23) - 127))) : 0;
     const float f = __uint_as_float((uint32_t)(127 + up) << 23);
     // (128 wide the table's operands have an order of their own, see tq_table.h)
     const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(a.D) + ((size_t)wave * (DP / 16u) * 64u + lane) * 16u;
     const bool tuned = a.D == TQ_HEAD_DIM;
     tq_f16v acc = tq_zero16();
+#pragma unroll 4
     for (uint32_t s = 0; s < DP / 16u; ++s) {
         const uint32_t j = tuned ? 64u * h + 8u * s : 16u * s + 8u * h;
         uint32_t t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = fp16_terms(j + i < a.D ? lds_o[0][n32 * ROW + j + i] * f : 0.f);
+        for (int i = 0; i < 8; ++i) t[i] = fp16_terms(j + i < a.D ? lds_o[0][q * ROW + j + i] * f : 0.f);
         tq_u4 oh, ol;
         fp16_operands(t, oh, ol);
         const tq_u4 ph = tq_gload16(pi + (size_t)s * 1024u), pl = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(a.D) + (size_t)s * 1024u);
@@ -493,22 +518,35 @@ __global__ __launch_bounds__(2 * DP < 64 ? 64 : 2 * DP) void tq_many_merge_kerne
         acc = mfma_f16(ph, ol, acc);
         acc = mfma_f16(pl, oh, acc);
     }
-    const uint32_t m = tile * 32u + n32;
-    if (m >= a.M) return;
-    const float inv = lds_inv[n32], back = __uint_as_float((uint32_t)(127 - up) << 23);
+    const uint32_t m = tile * 32u + col0 + q;
+    if (m >= a.M || n32 >= (uint32_t)C) return;
+    const float inv = lds_top[q], back = __uint_as_float((uint32_t)(127 - up) << 23);
     const uint32_t d0 = tuned ? 64u * h + 16u * wave : 32u * wave + 16u * h;
-    const ManyQuery q(a, m);
-    const size_t first = (((size_t)b * a.heads * a.group + (size_t)kv * a.group + q.g) * a.queries + q.t) * a.D + d0;
+    const ManyQuery at_q(a, m);
+    const size_t first = (((size_t)b * a.heads * a.group + (size_t)kv * a.group + at_q.g) * a.queries + at_q.t) * a.D + d0;
+    float o[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[r] = inv == 0.f ? 0.f : fmaf(acc[r], back, lds_o[1][q * ROW + d0 + r]) * inv;
+    if (a.dtype != TQ_F32 && !(a.D & 31u) && !((uintptr_t)a.out & 15u)) {
+        uint32_t w[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            if (a.dtype == TQ_F16) w[d] = __builtin_bit_cast(uint32_t, tq_half2{(_Float16)o[2 * d], (_Float16)o[2 * d + 1]});
+            else w[d] = __builtin_bit_cast(uint32_t, tq_bf2{(__bf16)o[2 * d], (__bf16)o[2 * d + 1]});
+        }
+        tq_gstore16(a.out + first * 2u, tq_u4{w[0], w[1], w[2], w[3]});
+        tq_gstore16(a.out + first * 2u + 16u, tq_u4{w[4], w[5], w[6], w[7]});
+        return;
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const float o = inv == 0.f ? 0.f : fmaf(acc[r], back, lds_o[1][n32 * ROW + d0 + r]) * inv;
         if (d0 + r >= a.D) continue;
         if (a.dtype == TQ_F32) {
-            reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = o;
+            reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = o[r];
         } else {
             uint16_t e;
-            if (a.dtype == TQ_F16) e = __builtin_bit_cast(uint16_t, (_Float16)o);
-            else e = __builtin_bit_cast(uint16_t, (__bf16)o);
+            if (a.dtype == TQ_F16) e = __builtin_bit_cast(uint16_t, (_Float16)o[r]);
+            else e = __builtin_bit_cast(uint16_t, (__bf16)o[r]);
             reinterpret_cast<TQ_GLOBAL uint16_t *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = e;
         }
     }
