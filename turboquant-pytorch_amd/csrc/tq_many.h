@@ -168,6 +168,35 @@ __device__ __forceinline__ bool plain_seen(const TqManyArgs &a, uint32_t which, 
     return a.tree ? a.tree[(long long)b * a.tree_batch + (long long)own * a.plain[1].n + t] != 0 : t <= own;
 }
 
+// Coordinates d0 ... d0 + 15 of query vector m's result
+__device__ __forceinline__ void store_result(const TqManyArgs &a, uint32_t row, uint32_t m, uint32_t d0, const float (&o)[16]) {
+    const ManyQuery q(a, m);
+    const size_t first = (((size_t)row * a.group + q.g) * a.queries + q.t) * a.D + d0;
+    if (a.dtype != TQ_F32 && !(a.D & 31u) && !((uintptr_t)a.out & 15u)) {
+        uint32_t w[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            if (a.dtype == TQ_F16) w[d] = __builtin_bit_cast(uint32_t, tq_half2{(_Float16)o[2 * d], (_Float16)o[2 * d + 1]});
+            else w[d] = __builtin_bit_cast(uint32_t, tq_bf2{(__bf16)o[2 * d], (__bf16)o[2 * d + 1]});
+        }
+        tq_gstore16(a.out + first * 2u, tq_u4{w[0], w[1], w[2], w[3]});
+        tq_gstore16(a.out + first * 2u + 16u, tq_u4{w[4], w[5], w[6], w[7]});
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        if (d0 + r >= a.D) continue;
+        if (a.dtype == TQ_F32) {
+            reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = o[r];
+        } else {
+            uint16_t e;
+            if (a.dtype == TQ_F16) e = __builtin_bit_cast(uint16_t, (_Float16)o[r]);
+            else e = __builtin_bit_cast(uint16_t, (__bf16)o[r]);
+            reinterpret_cast<TQ_GLOBAL uint16_t *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = e;
+        }
+    }
+}
+
 // Keys of sequence b (packed, then window) that can count
 __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b) {
     const uint32_t all = a.tokens + a.plain[0].n;

@@ -31,7 +31,8 @@ long long fast_splits(long long blocks, long long others, long long tokens) {
     long long most = (tokens + 255) / 256, best = 1, best_cost = 0;
     if (most > MAX_SPLITS) most = MAX_SPLITS;
     for (long long s = 1; s <= most; ++s) {
-        const long long rounds = (blocks * s + others + cus - 1) / cus, cost = rounds * ((tokens + s - 1) / s + 1500) + 30 * s;
+        const long long rounds = (blocks * s + cus - 1) / cus, extra = s == 1 ? rounds * (others ? 1000 : 0) : blocks * s + others > rounds * cus ? (others + cus - 1) / cus * 1000 : 0;
+        const long long cost = rounds * ((tokens + s - 1) / s + 1500) + extra + (s > 1 ? 1000 : 0) + 30 * s;
         if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
         if (rounds > 16 && s > 1) break;
     }
@@ -60,8 +61,9 @@ int plan(const tq_attend_request *r, Plan &p) {
         if (p.splits > MAX_SPLITS) p.splits = MAX_SPLITS;
         if (p.splits < 1) p.splits = 1;
     }
-    p.records = r->tokens ? p.splits * (p.qt ? 1 : ANY_WAVES) : 0;
-    p.plain_records = plain_tiles(r) ? (p.qt ? 1 : PLAIN_WAVES) : 0;
+    const bool whole = p.qt && p.splits == 1;          // a block has all of its queries' tokens: no records, no merge
+    p.records = whole || !r->tokens ? 0 : p.splits * (p.qt ? 1 : ANY_WAVES);
+    p.plain_records = whole || !plain_tiles(r) ? 0 : (p.qt ? 1 : PLAIN_WAVES);
     const long long dp = padded(r->head_dim);
     p.floats = at * ((long long)q_operand_bytes((uint32_t)dp) / 4 + (p.records + p.plain_records) * record_floats((uint32_t)dp) + 64) + (at + 3) / 4 * 4;
     return at * (p.splits + 1) * 4 > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;
@@ -95,7 +97,7 @@ TqManyPlain plain_of(const tq_plain_tokens &t) {
 template <int DP>
 void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     const uint32_t at = a.rows * a.tiles;
-    if (a.records && plan.qt) {
+    if (plan.qt) {
         const dim3 g((unsigned)(plan.rows * plan.groups * plan.splits + a.plain_blocks));
         const int ik = 8 / (int)a.bits_k, iv = 8 / (int)a.bits_v;
         if constexpr (DP == 64) tq_many_launch_d64(ik, iv, g, s, a, plan.qt, plan.kt);
@@ -108,8 +110,10 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
         else if (a.dtype == TQ_F16) hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_F16>), g, t, 0, s, a);
         else hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_BF16>), g, t, 0, s, a);
     }
-    if (at < 512u) hipLaunchKernelGGL((tq_many_merge_kernel<DP, 8>), dim3(at * 4u), dim3(2 * DP), 0, s, a);
-    else hipLaunchKernelGGL((tq_many_merge_kernel<DP, 32>), dim3(at), dim3(2 * DP), 0, s, a);
+    if (a.records || a.plain_records) {
+        if (at < 512u) hipLaunchKernelGGL((tq_many_merge_kernel<DP, 8>), dim3(at * 4u), dim3(2 * DP), 0, s, a);
+        else hipLaunchKernelGGL((tq_many_merge_kernel<DP, 32>), dim3(at), dim3(2 * DP), 0, s, a);
+    }
     if (!a.weights) return;
     if (a.tokens && plan.qt) {
         int cus = 0;

@@ -185,19 +185,22 @@ __device__ __forceinline__ float rotate_queries(const TqManyArgs &a, uint32_t ro
 
 // 32 uncompressed tokens of a row (`which`: 0 the window, 1 the drafts; from t0 on) against a tile of queries: raw 16-bit products are exact, weights enter the value
 // product as three bf16 terms, or two fp16 ones.  Coordinates of the sums as in the packed loop: row r of acc[c] is coordinate NC r + c.  Infinite and NaN
-// values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); the answer says whether there were any.
+// values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); `wild` says whether there are any.
+// Up to 128 wide the tokens stay in registers from one tile of queries to the next (HELD), at 256 they are read as they are needed.
 template <int D, bool BF>
-__device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, uint32_t t0, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t lane,
-                                           float &m_ref, float &l, tq_f16v (&acc)[D / 32]) {
-    constexpr int NC = D / 32, STEPS = D / 16, PT = BF ? 3 : 2, VT = NC == 8 ? 8 : 16;       // VT: tokens whose values are held at a time
-    const TqManyPlain &seg = a.plain[which];
-    const uint32_t n = lane & 31u, h = lane >> 5, kv = row - b * a.heads;
-    const uint8_t *k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 2 + 16u * h;
-    const uint8_t *v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 2 + 2u * NC * n;
-    constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
-    bool wild = false;
+struct PlainTile {
+    static constexpr int NC = D / 32, STEPS = D / 16, PT = BF ? 3 : 2;
+    static constexpr bool HELD = D <= 128;
+    static constexpr int VT = HELD ? 16 : 8, KH = HELD ? STEPS : 1;       // VT: tokens whose values are held at a time
+    static constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
     uint32_t vw[VT][NC / 2];
-    auto load_values = [&](int j0) __attribute__((always_inline)) {
+    tq_u4 kx[KH];
+    const uint8_t *k, *v;
+    uint32_t which, t0;
+    bool wild;
+
+    __device__ __forceinline__ void load_values(const TqManyArgs &a, int j0, uint32_t h) {
+        const TqManyPlain &seg = a.plain[which];
 #pragma unroll
         for (int j = 0; j < VT; ++j) {
             const uint8_t *p = v + (long long)min(t0 + acc_row(j0 + j, h), seg.n - 1u) * seg.v_token * 2;
@@ -211,14 +214,14 @@ __device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, 
                     vw[j][c] = (uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * c) | ((uint32_t)tq_gload2(reinterpret_cast<const uint16_t *>(p) + 2 * c + 1) << 16);
             }
         }
-    };
-    auto tame_values = [&](int j0) __attribute__((always_inline)) {
+    }
+    __device__ __forceinline__ void tame_values(const TqManyArgs &a, int j0, uint32_t h) {
         uint32_t over = 0u;
 #pragma unroll
         for (int j = 0; j < VT; ++j)
 #pragma unroll
             for (int c = 0; c < NC / 2; ++c) {
-                if (t0 + acc_row(j0 + j, h) >= seg.n) vw[j][c] = 0u;
+                if (t0 + acc_row(j0 + j, h) >= a.plain[which].n) vw[j][c] = 0u;
                 over |= (vw[j][c] & EXPO) + ONE;         // (an exponent of ones carries into the sign's place)
             }
         if (__any((over & 0x80008000u) != 0u)) {
@@ -228,20 +231,47 @@ __device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, 
 #pragma unroll
                 for (int c = 0; c < NC / 2; ++c) vw[j][c] &= ~(((((vw[j][c] & EXPO) + ONE) >> 15) & 0x00010001u) * 0xffffu);
         }
-    };
-    if constexpr (VT == 16) load_values(0);
-    {
-        const uint32_t m = min(tile * 32u + n, a.M - 1u);
+    }
+    __device__ __forceinline__ void load(const TqManyArgs &a, uint32_t which_, uint32_t t0_, uint32_t row, uint32_t b, uint32_t lane) {
+        which = which_;
+        t0 = t0_;
+        const TqManyPlain &seg = a.plain[which];
+        const uint32_t n = lane & 31u, h = lane >> 5, kv = row - b * a.heads;
+        k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 2 + 16u * h;
+        v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 2 + 2u * NC * n;
+        if constexpr (HELD) {
+            if (a.aligned) {
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) kx[st] = tq_gload16(k + 32 * st);
+            } else {
+#pragma unroll 1
+                for (int st = 0; st < STEPS; ++st) {
+                    const tq_u4 x = load_elements(k + 32 * st, false);
+#pragma unroll
+                    for (int i = 0; i < STEPS; ++i) kx[i] = i == st ? x : kx[i];
+                }
+            }
+            load_values(a, 0, h);
+            tame_values(a, 0, h);
+        }
+    }
+    __device__ __forceinline__ void attend(const TqManyArgs &a, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t lane, float &m_ref, float &l, tq_f16v (&acc)[NC]) {
+        const TqManyPlain &seg = a.plain[which];
+        const uint32_t n = lane & 31u, h = lane >> 5, m = min(tile * 32u + n, a.M - 1u);
         const uint8_t *q = many_query(a, row, m, 2u) + 16u * h;
         tq_f16v s = tq_zero16();
         if (a.aligned) {
+            constexpr int CH = HELD ? STEPS : 4;
 #pragma unroll 1
-            for (int s0 = 0; s0 < STEPS; s0 += 4) {
-                tq_u4 x[4], y[4];
+            for (int s0 = 0; s0 < STEPS; s0 += CH) {
+                tq_u4 x[CH], y[CH];
 #pragma unroll
-                for (int st = 0; st < 4; ++st) { x[st] = tq_gload16(k + 32 * (s0 + st)); y[st] = tq_gload16(q + 32 * (s0 + st)); }
+                for (int st = 0; st < CH; ++st) {
+                    x[st] = HELD ? kx[HELD ? st : 0] : tq_gload16(k + 32 * (s0 + st));
+                    y[st] = tq_gload16(q + 32 * (s0 + st));
+                }
 #pragma unroll
-                for (int st = 0; st < 4; ++st) s = BF ? mfma_bf16(x[st], y[st], s) : mfma_f16(x[st], y[st], s);
+                for (int st = 0; st < CH; ++st) s = BF ? mfma_bf16(x[st], y[st], s) : mfma_f16(x[st], y[st], s);
             }
         } else {
 #pragma unroll 1
@@ -274,14 +304,11 @@ __device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, 
 #pragma unroll
             for (int c = 0; c < NC; ++c) acc[c] *= shrink;
         }
-        if constexpr (VT == 16) {
-            tame_values(0);
-        }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            if constexpr (VT == 8) {
-                load_values(8 * st);
-                tame_values(8 * st);
+            if constexpr (!HELD) {
+                load_values(a, 8 * st, h);
+                tame_values(a, 8 * st, h);
             }
             tq_u4 p[3];
             float ps[8];
@@ -299,93 +326,203 @@ __device__ __forceinline__ bool plain_tile(const TqManyArgs &a, uint32_t which, 
                 tq_u4 o;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                    o[d] = __builtin_amdgcn_perm(vw[(VT == 16 ? 8 * st : 0) + 2 * d + 1][c / 2], vw[(VT == 16 ? 8 * st : 0) + 2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                    o[d] = __builtin_amdgcn_perm(vw[(HELD ? 8 * st : 0) + 2 * d + 1][c / 2], vw[(HELD ? 8 * st : 0) + 2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                 for (int t = 0; t < PT; ++t) acc[c] = BF ? mfma_bf16(o, p[t], acc[c]) : mfma_f16(o, p[t], acc[c]);
             }
         }
     }
-    return wild;
+};
+
+// The sums of waves [w0, w0 + count) of a tile of queries into out[32][D + 4] and their largest logits and sums into out_m, out_l[32], all in LDS; every wave of the block
+// calls it, those with other w0 for another tile.  unit: what this wave's value sums are multiplied by; m_ref: MANY_NONE where it has seen no token of a
+// query; l: this lane's half.  area: [wave][32][64 + 4], two coordinates blocks of 32 at a time.
+template <int D>
+__device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], float (*lds_l)[32], float *out, float *out_m, float *out_l, uint32_t w0, uint32_t count, float unit, float m_ref,
+                                           float l, const tq_f16v (&acc)[D / 32], uint32_t tid) {
+    constexpr int NC = D / 32;
+    constexpr uint32_t MROW = 68u, ROW = D + 4;
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
+    const float both = halves_add(l);
+    if (h == 0u) {
+        lds_m[wave][n] = m_ref;
+        lds_l[wave][n] = both;
+    }
+    __syncthreads();
+    float m = MANY_NONE, sum = 0.f;
+    for (uint32_t w = w0; w < w0 + count; ++w) m = fmaxf(m, lds_m[w][n]);
+    for (uint32_t w = w0; w < w0 + count; ++w) sum = fmaf(lds_l[w][n], __builtin_amdgcn_exp2f(lds_m[w][n] - m), sum);
+    if (wave == w0 && h == 0u) {
+        out_m[n] = m;
+        out_l[n] = sum;
+    }
+    const float f = unit * __builtin_amdgcn_exp2f(m_ref - m);
+    const uint32_t mine = tid - w0 * 64u, threads = count * 64u;       // (a wave sums for its own tile)
+#pragma unroll
+    for (int c0 = 0; c0 < NC; c0 += 2) {
+        if (c0) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<tq_f4 *>(area + (wave * 32u + n) * MROW + 32 * c + 8 * k + 4 * h) =
+                    tq_f4{acc[c0 + c][4 * k] * f, acc[c0 + c][4 * k + 1] * f, acc[c0 + c][4 * k + 2] * f, acc[c0 + c][4 * k + 3] * f};
+        __syncthreads();
+        for (uint32_t pair = mine; pair < 1024u; pair += threads) {        // coordinates NC r + c0, + 1 of query col
+            const uint32_t col = pair / 32u, r = pair % 32u;
+            float x = 0.f, y = 0.f;
+            for (uint32_t w = w0; w < w0 + count; ++w) {
+                x += area[(w * 32u + col) * MROW + r];
+                y += area[(w * 32u + col) * MROW + 32u + r];
+            }
+            out[col * ROW + NC * r + c0] = x;
+            out[col * ROW + NC * r + c0 + 1] = y;
+        }
+    }
 }
 
-// Infinite and NaN values of a row's uncompressed tokens into the sums of the queries that see them, whatever their weight (it is not zero).
+// joined sums of a tile -> its record
 template <int D>
-__device__ __forceinline__ void add_wild(const TqManyArgs &a, float *rec, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t tid) {
+__device__ __forceinline__ void put_record(float *rec, const float *out, const float *out_m, const float *out_l, uint32_t tid) {
+    TQ_GLOBAL float *p = (TQ_GLOBAL float *)rec;
+    if (tid < 32u) { p[tid] = out_m[tid]; p[32u + tid] = out_l[tid]; }
+    for (uint32_t u = tid; u < 32u * D / 4u; u += FAST_THREADS) {
+        const uint32_t col = u / (D / 4u), d = (u - col * (D / 4u)) * 4u;
+        *reinterpret_cast<TQ_GLOBAL tq_f4 *>(p + 64u + col * D + d) = *reinterpret_cast<const tq_f4 *>(out + col * (D + 4u) + d);
+    }
+}
+
+// Infinite and NaN values of a row's uncompressed tokens into the joined sums of the queries that see them, whatever their weight (it is not zero).
+template <int D>
+__device__ __forceinline__ void add_wild(const TqManyArgs &a, float *out, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t tid) {
     const uint32_t kv = row - b * a.heads, elem = a.dtype;
+#pragma unroll 1
     for (uint32_t e = tid; e < 32u * D; e += FAST_THREADS) {
         const uint32_t col = e / D, d = e - col * D, m = tile * 32u + col;
         if (m >= a.M) return;
         const uint32_t own = ManyQuery(a, m).t;
         float sum = 0.f;
+#pragma unroll 1
         for (uint32_t which = 0; which < 2u; ++which) {
             const TqManyPlain &seg = a.plain[which];
+#pragma unroll 1
             for (uint32_t t = 0; t < seg.n; ++t) {
                 const float v = plain_element(seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head + (long long)t * seg.v_token + d) * 2, elem);
                 if (!(fabsf(v) < __builtin_inff()) && plain_seen(a, which, b, own, t, length)) sum += v;
             }
         }
-        if (sum != 0.f) rec[64u + e] += sum;
+        if (sum != 0.f) out[col * (D + 4u) + d] += sum;
     }
 }
 
-// The sums of a block's waves, QT tiles of queries, into the block's record of each tile (its first float: rec + i * tile_step).  unit: what this wave's value sums are
-// multiplied by; m_ref: MANY_NONE where a wave has seen no token of a query; l: this lane's half.
+// LDS once the packed tokens are done with: what waves join their sums through, and the joined sums of packed and uncompressed tokens of each tile
 template <int D, int QT>
-__device__ __forceinline__ void put_block(uint8_t *lds, float (*lds_m)[32 * QT], float (*lds_l)[32 * QT], float *rec, size_t tile_step, uint32_t tiles, float unit, const float (&m_ref)[QT],
-                                          const float (&l)[QT], const tq_f16v (&acc)[QT][D / 32], uint32_t tid) {
-    constexpr int NC = D / 32, TC = NC < 4 ? NC : 4, MROW = 32 * TC + 4;
-    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
+struct JoinArea {
+    static constexpr uint32_t TILE = 32u * (D + 4u) * 4u, JOIN = FAST_WAVES * 32u * 68u * 4u, PACKED = JOIN, PLAIN = PACKED + QT * TILE, STATS = PLAIN + QT * TILE, BYTES = STATS + 4u * QT * 128u;
+    static __device__ __forceinline__ float *sums(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + (plain ? PLAIN : PACKED) + i * TILE); }
+    static __device__ __forceinline__ float *largest(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + STATS + (2u * (plain * QT + i)) * 128u); }
+    static __device__ __forceinline__ float *total(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + STATS + (2u * (plain * QT + i) + 1u) * 128u); }
+};
+
+// A row's uncompressed tokens against the block's tiles of queries, joined sums into LDS.  Two tiles share the waves where four of them hold all tokens.
+template <int D, int QT, bool BF>
+__device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, float (*lds_m)[32], float (*lds_l)[32], float *lds_wild, uint32_t row, uint32_t b, uint32_t tile0, uint32_t tiles,
+                                            uint32_t length, uint32_t tid) {
+    constexpr int NC = D / 32;
+    using J = JoinArea<D, QT>;
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6);
+    const uint32_t first = (a.plain[0].n + 31u) / 32u, all = first + (a.plain[1].n + 31u) / 32u;
+    const bool share = QT == 2 && tiles == 2u && all <= FAST_WAVES / 2u;
+    const uint32_t count = share ? FAST_WAVES / 2u : FAST_WAVES, side = wave / count, w0 = side * count, rounds = share ? 1u : tiles;
+#pragma unroll 1
+    for (uint32_t i = 0; i < rounds; ++i) {
+        const uint32_t mine = share ? side : i;
+        float m = MANY_NONE, l = 0.f;
+        tq_f16v acc[NC];
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const float both = halves_add(l[i]);
-        if (h == 0u) {
-            lds_m[wave][32 * i + n] = m_ref[i];
-            lds_l[wave][32 * i + n] = both;
+        for (int c = 0; c < NC; ++c) acc[c] = tq_zero16();
+        bool wild = false;
+#pragma unroll 1
+        for (uint32_t w = wave - w0; w < all; w += count) {
+            PlainTile<D, BF> t;
+            t.wild = false;
+            t.load(a, w < first ? 0u : 1u, 32u * (w < first ? w : w - first), row, b, lane);
+            t.attend(a, row, b, tile0 + mine, length, lane, m, l, acc);
+            wild |= t.wild;
         }
-    }
-    __syncthreads();
-    float *area = reinterpret_cast<float *>(lds);
+        __syncthreads();             // (what the area held)
+        if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
+        join_waves<D>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, count, 1.f, m, l, acc, tid);
+        __syncthreads();
+        float any = 0.f;
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        if ((uint32_t)i >= tiles) break;
-        float m = MANY_NONE;
-#pragma unroll
-        for (int w = 0; w < FAST_WAVES; ++w) m = fmaxf(m, lds_m[w][32 * i + n]);
-        float *dst_rec = rec + i * tile_step;
-        if (tid < 32u) {
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < FAST_WAVES; ++w) sum = fmaf(lds_l[w][32 * i + n], __builtin_amdgcn_exp2f(lds_m[w][32 * i + n] - m), sum);
-            dst_rec[n] = m;
-            dst_rec[32u + n] = sum;
-        }
-        const float f = unit * __builtin_amdgcn_exp2f(lds_m[wave][32 * i + n] - m);
-#pragma unroll
-        for (int c0 = 0; c0 < NC; c0 += TC) {
-            if (i || c0) __syncthreads();
-#pragma unroll
-            for (int c = 0; c < TC; ++c)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    *reinterpret_cast<tq_f4 *>(area + (wave * 32u + n) * MROW + 32 * c + 8 * k + 4 * h) =
-                        tq_f4{acc[i][c0 + c][4 * k] * f, acc[i][c0 + c][4 * k + 1] * f, acc[i][c0 + c][4 * k + 2] * f, acc[i][c0 + c][4 * k + 3] * f};
+        for (int w = 0; w < FAST_WAVES; ++w) any += lds_wild[w];
+        if (any != 0.f) {
+            if (!share) add_wild<D>(a, J::sums(lds, 1u, i), row, b, tile0 + i, length, tid);
+            else
+                for (uint32_t k = 0; k < 2u; ++k) add_wild<D>(a, J::sums(lds, 1u, k), row, b, tile0 + k, length, tid);
             __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t pair = tid + e * FAST_THREADS, col = pair / 32u, r = pair % 32u;       // coordinates NC r + c0 ... of query col
-                float sum[TC];
-#pragma unroll
-                for (int c = 0; c < TC; ++c) sum[c] = 0.f;
-#pragma unroll
-                for (int w = 0; w < FAST_WAVES; ++w)
-#pragma unroll
-                    for (int c = 0; c < TC; ++c) sum[c] += area[(w * 32 + col) * MROW + 32 * c + r];
-                TQ_GLOBAL float *dst = (TQ_GLOBAL float *)dst_rec + 64u + col * D + NC * r + c0;
-                if constexpr (TC == 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(dst) = tq_f4{sum[0], sum[1], sum[2], sum[3]};
-                else { dst[0] = sum[0]; dst[1] = sum[1]; }
-            }
         }
     }
+}
+
+// Results of the block's tiles from the joined sums in LDS, where a row's tokens are in one split: packed sums turned back by Pi_v (two fp16 terms each, as the merge
+// does), the uncompressed ones added, divided by the sum of weights.
+template <int D, int QT>
+__device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, bool plain, uint32_t row, uint32_t tile0, uint32_t tiles, uint32_t tid) {
+    constexpr int NC = D / 32, STEPS = D / 16, CH = STEPS < 8 ? STEPS : 8;
+    using J = JoinArea<D, QT>;
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, i = wave / NC, w = wave % NC;
+    if (i >= tiles) return;
+    const float *o = J::sums(lds, 0u, i) + n * (D + 4u), *p = J::sums(lds, 1u, i) + n * (D + 4u);
+    const float m0 = J::largest(lds, 0u, i)[n], m1 = plain ? J::largest(lds, 1u, i)[n] : MANY_NONE, m = fmaxf(m0, m1);
+    const float f0 = m0 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m0 - m), f1 = m1 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+    const float l = J::total(lds, 0u, i)[n] * f0 + (plain ? J::total(lds, 1u, i)[n] * f1 : 0.f), inv = l == 0.f ? 0.f : 1.0f / l;
+    const uint32_t q = (tile0 + i) * 32u + n;
+    if (a.stat && w == 0u && h == 0u) {
+        float *stat = a.stat + ((size_t)row * a.tiles + tile0 + i) * 64u;
+        const bool some = q < a.M && inv != 0.f;
+        stat[n] = some ? m : -MANY_NONE;
+        stat[32u + n] = some ? inv : 0.f;
+    }
+    const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(D) + ((size_t)w * STEPS * 64u + lane) * 16u;
+    float largest = 0.f;
+#pragma unroll 8
+    for (uint32_t d = 0; d < D / 2u; d += 4u) {
+        const tq_f4 v = *reinterpret_cast<const tq_f4 *>(o + h * (D / 2u) + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
+    }
+    largest = halves_max(largest);
+    const int up = largest > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(largest) >> 23) - 127))) : 0;
+    const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+    tq_f16v acc = tq_zero16();
+#pragma unroll 1
+    for (int s0 = 0; s0 < STEPS; s0 += CH) {
+        tq_u4 ph[CH], pl[CH];
+#pragma unroll
+        for (int s = 0; s < CH; ++s) { ph[s] = tq_gload16(pi + (size_t)(s0 + s) * 1024u); pl[s] = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(D) + (size_t)(s0 + s) * 1024u); }
+#pragma unroll
+        for (int s = 0; s < CH; ++s) {
+            const uint32_t j = D == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
+            const tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + j), y = *reinterpret_cast<const tq_f4 *>(o + j + 4u);
+            uint32_t t[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { t[k] = fp16_terms(x[k] * f); t[4 + k] = fp16_terms(y[k] * f); }
+            tq_u4 oh, ol;
+            fp16_operands(t, oh, ol);
+            acc = mfma_f16(ph[s], oh, acc);
+            acc = mfma_f16(ph[s], ol, acc);
+            acc = mfma_f16(pl[s], oh, acc);
+        }
+    }
+    if (q >= a.M) return;
+    const float back = __uint_as_float((uint32_t)(127 - up) << 23) * f0;
+    const uint32_t d0 = D == TQ_HEAD_DIM ? 64u * h + 16u * w : 32u * w + 16u * h;
+    float out[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) out[r] = inv == 0.f ? 0.f : (acc[r] * back + (plain ? p[d0 + r] * f1 : 0.f)) * inv;
+    store_result(a, row, q, d0, out);
 }
 
 // Block = (row, QT tiles of 32 queries, split): its waves take runs of 32 tokens in turn, each by itself, and their sums meet in LDS at the end.
@@ -403,14 +540,14 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     using Values = ValueBytes<IPBV, NC>;
     constexpr int QW = KT * QT * STEPS * 4;                                        // registers of the queries' operands
     constexpr bool QREG = QW + QT * NC * 16 <= 136;
-    constexpr int TC = NC < 4 ? NC : 4;
-    constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024, MERGE_BYTES = FAST_WAVES * 32 * (32 * TC + 4) * 4;
-    constexpr int AREA = LUT_BYTES + Q_BYTES > MERGE_BYTES ? LUT_BYTES + Q_BYTES : MERGE_BYTES;
+    constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024;
+    using J = JoinArea<D, QT>;
+    constexpr int AREA = LUT_BYTES + Q_BYTES > (int)J::BYTES ? LUT_BYTES + Q_BYTES : (int)J::BYTES;
     static_assert(QT * NC <= FAST_WAVES, "waves that rotate");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[FAST_WAVES][32];
     __shared__ __attribute__((aligned(16))) uint16_t lds_vn[FAST_WAVES][32];
-    __shared__ float lds_m[FAST_WAVES][32 * QT], lds_l[FAST_WAVES][32 * QT];
+    __shared__ float lds_m[FAST_WAVES][32], lds_l[FAST_WAVES][32];
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const uint32_t groups = (a.tiles + QT - 1u) / QT;
@@ -421,39 +558,9 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     const uint32_t tiles = min((uint32_t)QT, a.tiles - tile0);
     const uint32_t length = many_length(a, b);
 
-    if (!packed) {
-        // A block of uncompressed tokens, window first: few, and first in the launch, so that they are done while the others are at the packed ones
-        const uint32_t first = (a.plain[0].n + 31u) / 32u, all = first + (a.plain[1].n + 31u) / 32u;
-        // (a tile of queries at a time: its sums and its tokens' values share the registers)
-#pragma unroll 1
-        for (uint32_t i = 0; i < tiles; ++i) {
-            float m1[1] = {MANY_NONE}, l1[1] = {0.f};
-            tq_f16v acc1[1][NC];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) acc1[0][c] = tq_zero16();
-            bool wild = false;
-#pragma unroll 1
-            for (uint32_t w = wave; w < all; w += FAST_WAVES) {
-                const uint32_t which = w < first ? 0u : 1u, t0 = 32u * (which ? w - first : w);
-                if (a.dtype == TQ_BF16) wild |= plain_tile<D, true>(a, which, t0, row, b, tile0 + i, length, lane, m1[0], l1[0], acc1[0]);
-                else wild |= plain_tile<D, false>(a, which, t0, row, b, tile0 + i, length, lane, m1[0], l1[0], acc1[0]);
-            }
-            if (i) __syncthreads();           // (what the last tile's sums went through)
-            if (lane == 0u) lds_kn[0][wave] = wild ? 1.f : 0.f;
-            float *rec = a.plain_rec + (first_tile + i) * record_floats(D);
-            put_block<D, 1>(lds, reinterpret_cast<float (*)[32]>(&lds_m[0][0]), reinterpret_cast<float (*)[32]>(&lds_l[0][0]), rec, 0, 1u, 1.f, m1, l1, acc1, tid);
-            float any = 0.f;
-#pragma unroll
-            for (int w = 0; w < FAST_WAVES; ++w) any += lds_kn[0][w];
-            if (any != 0.f) {
-                __threadfence_block();
-                __syncthreads();              // (what put_block has stored)
-                add_wild<D>(a, rec, row, b, tile0 + i, length, tid);
-            }
-        }
-        return;
-    }
-
+    // A row's uncompressed tokens: by the block that has its packed ones, where they are in one split, otherwise by blocks of their own, the first of
+    // the launch, so that they are done while the others are at the packed ones.
+    if (packed) {
     if constexpr (KT == 1) {
         Lut<IPBK> table;
         table.load(a.table_k + TQ_OFF_LUT(D), tid);
@@ -667,15 +774,29 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         wave_sync();
     }
 
-    // ---- the block's record of each tile
+    // ---- the waves' sums
+    const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        m_ref[i] = m_ref[i] == FAST_START ? MANY_NONE : m_ref[i];
-        l[i] *= 1.0f / (float)(1 << FAST_P);
+        __syncthreads();
+        join_waves<D>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, FAST_WAVES, unit,
+                      m_ref[i] == FAST_START ? MANY_NONE : m_ref[i], l[i] * (1.0f / (float)(1 << FAST_P)), acc[i], tid);
     }
-    const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P) << 23);
     __syncthreads();
-    put_block<D, QT>(lds, lds_m, lds_l, a.rec + (first_tile * a.records + split) * record_floats(D), (size_t)a.records * record_floats(D), tiles, unit, m_ref, l, acc, tid);
+    }
+    const bool whole = a.splits == 1u, plain = (a.plain[0].n | a.plain[1].n) != 0u;
+    if (plain && (whole || !packed)) {
+        if (a.dtype == TQ_BF16) plain_phase<D, QT, true>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
+        else plain_phase<D, QT, false>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
+    }
+    if (whole) {
+        finish_block<D, QT>(a, lds, plain, row, tile0, tiles, tid);
+        return;
+    }
+    for (uint32_t i = 0; i < tiles; ++i) {
+        float *rec = packed ? a.rec + ((first_tile + i) * a.records + split) * record_floats(D) : a.plain_rec + (first_tile + i) * record_floats(D);
+        put_record<D>(rec, J::sums(lds, packed ? 0u : 1u, i), J::largest(lds, packed ? 0u : 1u, i), J::total(lds, packed ? 0u : 1u, i), tid);
+    }
 }
 
 // What the packed tokens receive: weight = 2^(logit - largest) / sum with the statistics of the merge, from the two-term products.  Rows of the product are queries

@@ -424,7 +424,7 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     __shared__ __attribute__((aligned(16))) float lds_o[2][C * ROW];        // packed, plain
     __shared__ float lds_f[MERGE_RECORDS][C], lds_red[2][PARTS][C], lds_top[C];
     const uint32_t group = blockIdx.x % (32u / C), at = blockIdx.x / (32u / C);
-    const uint32_t row = at / a.tiles, tile = at - row * a.tiles, b = row / a.heads, kv = row - b * a.heads, col0 = group * C;
+    const uint32_t row = at / a.tiles, tile = at - row * a.tiles, b = row / a.heads, col0 = group * C;
     if (tile * 32u + col0 >= a.M && !a.stat) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n32 = lane & 31u, h = lane >> 5;
     const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + (size_t)at * a.records * record_floats(DP);
@@ -522,34 +522,10 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     if (m >= a.M || n32 >= (uint32_t)C) return;
     const float inv = lds_top[q], back = __uint_as_float((uint32_t)(127 - up) << 23);
     const uint32_t d0 = tuned ? 64u * h + 16u * wave : 32u * wave + 16u * h;
-    const ManyQuery at_q(a, m);
-    const size_t first = (((size_t)b * a.heads * a.group + (size_t)kv * a.group + at_q.g) * a.queries + at_q.t) * a.D + d0;
     float o[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[r] = inv == 0.f ? 0.f : fmaf(acc[r], back, lds_o[1][q * ROW + d0 + r]) * inv;
-    if (a.dtype != TQ_F32 && !(a.D & 31u) && !((uintptr_t)a.out & 15u)) {
-        uint32_t w[8];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-            if (a.dtype == TQ_F16) w[d] = __builtin_bit_cast(uint32_t, tq_half2{(_Float16)o[2 * d], (_Float16)o[2 * d + 1]});
-            else w[d] = __builtin_bit_cast(uint32_t, tq_bf2{(__bf16)o[2 * d], (__bf16)o[2 * d + 1]});
-        }
-        tq_gstore16(a.out + first * 2u, tq_u4{w[0], w[1], w[2], w[3]});
-        tq_gstore16(a.out + first * 2u + 16u, tq_u4{w[4], w[5], w[6], w[7]});
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        if (d0 + r >= a.D) continue;
-        if (a.dtype == TQ_F32) {
-            reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = o[r];
-        } else {
-            uint16_t e;
-            if (a.dtype == TQ_F16) e = __builtin_bit_cast(uint16_t, (_Float16)o[r]);
-            else e = __builtin_bit_cast(uint16_t, (__bf16)o[r]);
-            reinterpret_cast<TQ_GLOBAL uint16_t *>((TQ_GLOBAL uint8_t *)a.out)[first + r] = e;
-        }
-    }
+    for (int r = 0; r < 16; ++r) o[r] = inv == 0.f ? 0.f : fmaf(acc[r], back, d0 + r < DP ? lds_o[1][q * ROW + d0 + r] : 0.f) * inv;
+    store_result(a, row, m, d0, o);
 }
 
 }  // namespace
