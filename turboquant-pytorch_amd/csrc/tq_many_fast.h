@@ -86,6 +86,12 @@ struct ValueBytes {
         else if constexpr (VB == 4) raw[0] = tq_gload4(p);
         else { const tq_u2 v = tq_gload8(p); raw[0] = v[0]; raw[W - 1] = v[1]; }
     }
+    __device__ __forceinline__ void fetch(const uint8_t *p) {          // from LDS
+        if constexpr (VB == 1) raw[0] = *p;
+        else if constexpr (VB == 2) raw[0] = *reinterpret_cast<const uint16_t *>(p);
+        else if constexpr (VB == 4) raw[0] = *reinterpret_cast<const uint32_t *>(p);
+        else { const tq_u2 v = *reinterpret_cast<const tq_u2 *>(p); raw[0] = v[0]; raw[W - 1] = v[1]; }
+    }
     // fp16 pairs; slot: the lane's slot of entry 0 (64 wide, four codes a byte: of its half)
     __device__ __forceinline__ void decode(const uint8_t *lut, uint32_t slot, uint32_t (&out)[NC / 2]) const {
         if constexpr (IPB == 4 && NC == 2) out[0] = lut_entry<0, uint32_t>(lut, raw[0], slot);
@@ -529,7 +535,7 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 //   * scores transposed: A = keys, decoded from the lane's own bytes by table, B = queries; a lane then has 16 tokens of one query;
 //   * softmax in base 2 against a reference per query that moves only when a logit exceeds it by 2^FAST_SLACK: no exchange between lanes;
 //   * weights times value norms are, as they lie, the B operand of the value product (its contraction runs over the tokens in the order in which a lane
-//     has them); A = values, every lane reading its coordinates' bytes of the eight tokens straight from memory.
+//     has them); A = values, every lane decoding its coordinates' bytes of eight tokens.
 // KT = 1: queries and levels as one fp16 value each, for bfloat16: the 2^-12 roundings move logits of some ten by 1e-3, where a bfloat16 result is rounded by up to 4e-3.
 // KT = 2: two terms each (three products, 22 bits), for float16 and wherever sums of weights are kept.  Weights and value levels are one fp16 value each (the
 // reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's sum of weights is made of the rounded weights
@@ -541,8 +547,11 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     constexpr int QW = KT * QT * STEPS * 4;                                        // registers of the queries' operands
     constexpr bool QREG = QW + QT * NC * 16 <= 136;
     constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024;
+    constexpr int VPIECE = GBV / 2;                                                // bytes of a run's values that a lane stages
+    constexpr bool STAGE = GBV <= 128;
     using J = JoinArea<D, QT>;
-    constexpr int AREA = LUT_BYTES + Q_BYTES > (int)J::BYTES ? LUT_BYTES + Q_BYTES : (int)J::BYTES;
+    constexpr int LOOP_BYTES = LUT_BYTES + Q_BYTES + (STAGE ? FAST_WAVES * 32 * GBV : 0);
+    constexpr int AREA = LOOP_BYTES > (int)J::BYTES ? LOOP_BYTES : (int)J::BYTES;
     static_assert(QT * NC <= FAST_WAVES, "waves that rotate");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[FAST_WAVES][32];
@@ -599,9 +608,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     const uint32_t begin = min(seen, split * chunk), end = min(seen, begin + chunk);
     const size_t slot0 = (size_t)row * a.packed_row_stride;
     const uint8_t *mask = a.mask ? a.mask + (long long)b * a.mask_stride : nullptr;
-    const uint8_t *k_lane = a.k_idx + slot0 * GBK + n * GBK + h * KB;
-    const uint8_t *v_lane = a.v_idx + slot0 * GBV + 4u * h * GBV + (IPBV == 4 && NC == 2 ? n / 2u : n * Values::VB);
-    const uint16_t *n_lane = (h ? a.v_norms : a.k_norms) + slot0 + n;
+    const uint32_t k_lane = n * GBK + h * KB, v_lane = 4u * h * GBV + (IPBV == 4 && NC == 2 ? n / 2u : n * Values::VB);
 
     float m_ref[QT], l[QT];
     tq_f16v acc[QT][NC];
@@ -616,29 +623,42 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 
     // Loads of a run are issued while the one before it is worked on.  The last run of a row begins 32 tokens before the end: what the one before it
     // had already is hidden, and nothing past the row's tokens is read.
+    // Value bytes go through LDS on their way (a lane needs single bytes of sixteen tokens), but at 256 with a byte a code, where they are
+    // read from memory as they are needed.
     uint32_t kraw[KW];
+    tq_u4 vpiece[STAGE && VPIECE >= 16 ? VPIECE / 16 : 1];
     Values vraw[16];
-    uint16_t norm_raw = 0;
+    uint16_t kn_raw = 0, vn_raw = 0;
+    uint8_t *vstage = lds + LUT_BYTES + Q_BYTES + wave * (STAGE ? 32u * GBV : 0u);
     auto issue_keys = [&](uint32_t t) __attribute__((always_inline)) {
-        const uint8_t *p = k_lane + (size_t)t * GBK;
+        const uint8_t *p = a.k_idx + (slot0 + t) * GBK;
         if constexpr (KB % 16 == 0) {
 #pragma unroll
             for (int i = 0; i < KB / 16; ++i) {
-                const tq_u4 v = tq_gload16(p + 16 * i);
+                const tq_u4 v = tq_gload16(p + k_lane + 16 * i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) kraw[4 * i + j] = v[j];
             }
         } else {
             static_assert(KB == 8, "eight bytes");
-            const tq_u2 v = tq_gload8(p);
+            const tq_u2 v = tq_gload8(p + k_lane);
             kraw[0] = v[0]; kraw[1] = v[1];
         }
-        norm_raw = tq_gload2(n_lane + t);
+        kn_raw = tq_gload2(a.k_norms + slot0 + t + n);
+        vn_raw = tq_gload2(a.v_norms + slot0 + t + n);
     };
     auto issue_values = [&](uint32_t t) __attribute__((always_inline)) {
-        const uint8_t *p = v_lane + (size_t)t * GBV;
+        const uint8_t *p = a.v_idx + (slot0 + t) * GBV;
+        if constexpr (!STAGE) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) vraw[j].load(p + (8 * (j / 4) + j % 4) * GBV);
+            for (int j = 0; j < 16; ++j) vraw[j].load(p + v_lane + (8 * (j / 4) + j % 4) * GBV);
+        } else if constexpr (VPIECE == 8) {
+            const tq_u2 v = tq_gload8(p + lane * 8u);
+            vpiece[0][0] = v[0]; vpiece[0][1] = v[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPIECE / 16; ++i) vpiece[i] = tq_gload16(p + i * 1024 + lane * 16u);
+        }
     };
     const uint32_t last = a.tokens - 32u;    // (launched for 32 tokens at least)
     uint32_t t_next = begin + 32u * wave;
@@ -653,7 +673,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         uint32_t hidden = ~((count == 32u ? 0xffffffffu : (1u << count) - 1u) << (t_run - t0));
         if (mask) hidden |= ~(uint32_t)__ballot(mask[t0 + n] != 0);
         // ---- norms: keys' times the queries' scale, values' in the unit of the largest so far
-        float norm = (float)__builtin_bit_cast(_Float16, norm_raw);
+        float norm = (float)__builtin_bit_cast(_Float16, h ? vn_raw : kn_raw);
         if (hidden) norm = (hidden >> n) & 1u ? 0.f : norm;
         const int top = (int)((__float_as_uint(norm) >> 23) & 255u) - 127;
         if (__any(h && top > v_top)) {
@@ -671,6 +691,14 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         norm *= h ? __uint_as_float((uint32_t)(127 - v_top) << 23) : q_scale;
         if (h) lds_vn[wave][n] = __builtin_bit_cast(uint16_t, (_Float16)norm);
         else lds_kn[wave][n] = norm;
+        if constexpr (STAGE) {
+            if constexpr (VPIECE == 8) *reinterpret_cast<tq_u2 *>(vstage + lane * 8u) = tq_u2{vpiece[0][0], vpiece[0][1]};
+            else {
+#pragma unroll
+                for (int i = 0; i < VPIECE / 16; ++i) *reinterpret_cast<tq_u4 *>(vstage + i * 1024 + lane * 16u) = vpiece[i];
+            }
+            issue_values(t_after);
+        }
         wave_sync();
         // ---- scores
         tq_f16v s[QT];
@@ -717,9 +745,11 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 const float bias = (float)FAST_P - m_ref[i];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = fmaf(s[i][r], kn[r], bias);
-                if (hidden) {
+                if (hidden) {        // (opaque: in its branch, not ahead of it for every run)
+                    uint32_t bits = hidden >> (4u * h);
+                    asm volatile("" : "+v"(bits));
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] = (hidden >> acc_row(r, h)) & 1u ? -__builtin_inff() : x[r];
+                    for (int r = 0; r < 16; ++r) x[r] = (bits >> acc_row(r, 0u)) & 1u ? -__builtin_inff() : x[r];
                 }
             };
             logits();
@@ -728,8 +758,10 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
             for (int r = 1; r < 16; ++r) most = fmaxf(most, x[r]);
             if (__any(most > (float)(FAST_P + FAST_SLACK))) {
                 float now = -__builtin_inff();
+                uint32_t bits = hidden >> (4u * h);
+                asm volatile("" : "+v"(bits));
 #pragma unroll
-                for (int r = 0; r < 16; ++r) now = (hidden >> acc_row(r, h)) & 1u ? now : fmaxf(now, s[i][r] * kn[r]);
+                for (int r = 0; r < 16; ++r) now = (bits >> acc_row(r, 0u)) & 1u ? now : fmaxf(now, s[i][r] * kn[r]);
                 now = fmaxf(halves_max(now), m_ref[i]);
                 const float shrink = __builtin_amdgcn_exp2f(m_ref[i] - now);
                 m_ref[i] = now;
@@ -760,7 +792,13 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         for (int st = 0; st < 2; ++st) {
             uint32_t w[8][NC / 2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) vraw[8 * st + j].decode(lds, slot_v, w[j]);
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (STAGE) {
+                    Values v;
+                    v.fetch(vstage + v_lane + (16 * st + 8 * (j / 4) + j % 4) * GBV);
+                    v.decode(lds, slot_v, w[j]);
+                } else vraw[8 * st + j].decode(lds, slot_v, w[j]);
+            }
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 tq_u4 v;
@@ -770,7 +808,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 for (int i = 0; i < QT; ++i) acc[i][c] = mfma_f16(v, p[i][st], acc[i][c]);
             }
         }
-        issue_values(t_after);
+        if constexpr (!STAGE) issue_values(t_after);
         wave_sync();
     }
 
