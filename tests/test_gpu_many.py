@@ -323,6 +323,8 @@ def test_tracked_attention_sums(pkg):
     (1, 4, 333, 10, 33, 80, F32, 4, 4),
     (1, 2, 100, 3, 50, 33, F16, 2, 8),
     (3, 1, 40000, 5, 20001, 128, BF, 4, 2),
+    (1, 2, 1024, 0, 1023, 64, BF, 2, 2), (1, 1, 1, 0, 1, 64, BF, 2, 2), (2, 1, 4096, 1, 5, 64, BF, 2, 2), (1, 1, 16385, 0, 16000, 64, BF, 2, 2),
+    (1, 2, 65536, 3, 1030, 64, BF, 2, 2), (1, 2, 65537, 3, 40000, 64, BF, 2, 2), (1, 1, 200001, 0, 777, 64, BF, 2, 2),
 ])
 def test_evict_keeps_the_largest(pkg, B, H, n, w, keep, D, dtype, kb, vb):
     codec = pkg.TurboQuantV3(D, key_bits=kb, value_bits=vb, residual_window=w, layer_idx=8, device=DEV)

@@ -47,45 +47,188 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
     return before + x - v;
 }
 
-// Block = row.  The keep-th largest weight is found eight bits at a time from counts of the tokens that agree with it so far; the tokens above it
-// stay, and of those equal to it the first ones.
+// Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens; E = 0: of more, read again for every pass.
+// The keep-th largest weight lies in a range of whole numbers, at first all there are.  While more than 1024 tokens lie in it, it is cut into 2048 parts, the tokens of each are counted
+// in LDS, and the part with the keep-th one is the next range: a floating-point number's bits go with its logarithm, so that sums spread over the parts and few of the
+// counts' atomics meet (counting by the leading byte instead took 110 us for 8 x 32768 tokens; those at the lower end, zeros, are counted by ballots).
+// What is left is packed to one a thread and settled bit by bit, with ballots.  Tokens above the result stay, and of those equal to it the first ones; places come
+// from counts per wave and register, in the tokens' order.
+template <int E>
 __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t lds_count[256], lds_scan[SELECT_THREADS / 64], lds_found[2];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    const float *w = a.weights + (long long)row * a.w_stride;
-    uint32_t prefix = 0u, left = a.keep;          // left: how many of those that agree with the prefix stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256u) lds_count[tid] = 0u;
+    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048;
+    __shared__ uint32_t lds_part[PARTS], lds_few[SELECT_THREADS], lds_count[2][WAVES], lds_ends[2][WAVES], lds_place[E ? E * WAVES : 1], lds_found[3], lds_n;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6);
+    const TQ_GLOBAL float *w = (const TQ_GLOBAL float *)a.weights + (long long)row * a.w_stride;
+    uint32_t key[E ? E : 1], lo = 0xffffffffu, hi = 0u;           // a token that is none: 0, less than any number's
+    auto each = [&](auto f) __attribute__((always_inline)) {      // f(key) of all tokens, by all threads together
+        if constexpr (E) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(key[e]);
+        } else {
+            for (uint32_t i0 = 0; i0 < a.tokens; i0 += 8u * SELECT_THREADS) {
+                float v[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) v[k] = w[min(i0 + k * SELECT_THREADS + tid, a.tokens - 1u)];
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) f(i0 + k * SELECT_THREADS + tid < a.tokens ? order_of(v[k]) : 0u);
+            }
+        }
+    };
+    if constexpr (E) {
+        constexpr int CH = E < 8 ? E : 8;
+#pragma unroll
+        for (int e0 = 0; e0 < E; e0 += CH) {
+            float v[CH];
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v[e] = w[min((e0 + e) * SELECT_THREADS + tid, a.tokens - 1u)];
+#pragma unroll
+            for (int e = 0; e < CH; ++e) key[e0 + e] = (e0 + e) * SELECT_THREADS + tid < a.tokens ? order_of(v[e]) : 0u;
+        }
+    }
+    each([&](uint32_t k) {
+        hi = max(hi, k);
+        lo = min(lo, k - 1u);                             // (none: as large as can be)
+    });
+#pragma unroll
+    for (int i = 32; i; i >>= 1) { lo = min(lo, (uint32_t)__shfl_xor(lo, i)); hi = max(hi, (uint32_t)__shfl_xor(hi, i)); }
+    if (lane == 0u) { lds_ends[0][wave] = lo; lds_ends[1][wave] = hi; }
+    if (tid == 0u) lds_n = 0u;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < WAVES; ++k) { lo = min(lo, lds_ends[0][k]); hi = max(hi, lds_ends[1][k]); }
+    lo += 1u;                                             // (a row has a token at least)
+    uint32_t left = a.keep, agree = a.tokens;             // agree tokens in [lo, hi], of which the largest `left` stay; all above hi do
+    while (agree > SELECT_THREADS && lo < hi && left < agree) {
+        const uint32_t width = 32u - (uint32_t)__builtin_clz(hi - lo), shift = width > 11u ? width - 11u : 0u;
+#pragma unroll
+        for (uint32_t k = 0; k < PARTS / SELECT_THREADS; ++k) lds_part[tid + k * SELECT_THREADS] = 0u;
         __syncthreads();
-        for (uint32_t i = tid; i < a.tokens; i += SELECT_THREADS) {
-            const uint32_t u = order_of(w[i]);
-            if (shift == 24 || (u ^ prefix) >> (shift + 8) == 0u) atomicAdd(&lds_count[(u >> shift) & 255u], 1u);
+        uint32_t lowest = 0u;
+        each([&](uint32_t k) {
+            lowest += (uint32_t)__popcll(__ballot(k == lo));
+            if (k > lo && k <= hi) atomicAdd(&lds_part[(k - lo) >> shift], 1u);
+        });
+        if (lane == 0u && lowest) atomicAdd(&lds_part[0], lowest);
+        __syncthreads();
+        // from the upper end: two parts a thread
+        const uint32_t p1 = PARTS - 1u - 2u * tid, c1 = lds_part[p1], c0 = lds_part[p1 - 1u];
+        uint32_t all;
+        const uint32_t above = block_scan(c1 + c0, lds_count[0], all);
+        if (above < left && above + c1 + c0 >= left) {
+            const bool upper = above + c1 >= left;
+            lds_found[0] = upper ? p1 : p1 - 1u;
+            lds_found[1] = upper ? above : above + c1;
+            lds_found[2] = upper ? c1 : c0;
         }
         __syncthreads();
-        if (tid == 0u) {
-            uint32_t above = 0u, digit = 255u;
-            while (digit > 0u && above + lds_count[digit] < left) above += lds_count[digit--];
-            lds_found[0] = digit;
-            lds_found[1] = above;
-        }
-        __syncthreads();
-        prefix |= lds_found[0] << shift;
+        const uint32_t part = lds_found[0];
         left -= lds_found[1];
+        agree = lds_found[2];
+        lo += part << shift;
+        hi = min(hi, lo + ((1u << shift) - 1u));
         __syncthreads();
     }
-    long long *kept = a.kept + (long long)row * a.keep;
-    uint32_t out = 0u, equal = 0u;                // over the tokens before this round
-    for (uint32_t i0 = 0; i0 < a.tokens; i0 += SELECT_THREADS) {
-        const uint32_t i = i0 + tid;
-        const uint32_t u = i < a.tokens ? order_of(w[i]) : 0u;
-        const bool above = i < a.tokens && u > prefix, same = i < a.tokens && u == prefix;
+    uint32_t border = lo;                                  // with left == agree all from lo on stay, with lo == hi the first `left` of them
+    if (lo < hi && left < agree) {
+        each([&](uint32_t k) {
+            const bool in = k >= lo && k <= hi;
+            const unsigned long long mine = __ballot(in);
+            if (mine) {
+                uint32_t base = 0u;
+                if (lane == 0u) base = atomicAdd(&lds_n, (uint32_t)__popcll(mine));          // (in any order: they are only counted)
+                base = tq_uniform32(base);
+                if (in) lds_few[base + __builtin_amdgcn_mbcnt_hi((uint32_t)(mine >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mine, 0u))] = k;
+            }
+        });
+        __syncthreads();
+        const bool mine = tid < agree;
+        const uint32_t own = mine ? lds_few[tid] - lo : 0u, size = agree;
+        uint32_t found = 0u, turn = 0u;
+        auto count = [&](uint32_t from) {                  // of the packed ones, those at least `from` above lo
+            const uint32_t c = (uint32_t)__popcll(__ballot(mine && own >= from));
+            if (lane == 0u) lds_count[turn][wave] = c;
+            __syncthreads();
+            uint32_t v = 0u;
+#pragma unroll
+            for (uint32_t k = 0; k < WAVES; ++k) v += lds_count[turn][k];
+            turn ^= 1u;
+            return v;
+        };
+        uint32_t from_found = size;
+        for (int bit = 31 - __builtin_clz(hi - lo); bit >= 0; --bit) {
+            const uint32_t c = count(found | (1u << bit));
+            if (c >= left) { found |= 1u << bit; from_found = c; }
+        }
+        const uint32_t over = found == 0xffffffffu ? 0u : count(found + 1u);
+        border = lo + found;
+        left -= over;
+        agree = from_found - over;
+    }
+    // ---- places
+    TQ_GLOBAL long long *kept = (TQ_GLOBAL long long *)a.kept + (long long)row * a.keep;
+    auto before_lane = [&](unsigned long long m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
+    if constexpr (E == 0) {                                // eight tokens in a row a thread
+        uint32_t out = 0u, equal = 0u;                     // over the tokens before this round
+        for (uint32_t i0 = 0; i0 < a.tokens; i0 += 8u * SELECT_THREADS) {
+            uint32_t k8[8], same = 0u, more = 0u;
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                const uint32_t i = i0 + 8u * tid + k;
+                k8[k] = i < a.tokens ? order_of(w[i]) : 0u;
+                same += k8[k] == border ? 1u : 0u;
+            }
+            uint32_t all;
+            uint32_t rank = equal + block_scan(same, lds_count[0], all);
+            equal += all;
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                if (k8[k] == border && rank++ >= left && left < agree) k8[k] = 0u;
+                more += k8[k] >= border ? 1u : 0u;
+            }
+            uint32_t at = out + block_scan(more, lds_count[0], all);
+            out += all;
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k)
+                if (k8[k] >= border) kept[at++] = i0 + 8u * tid + k;
+        }
+        return;
+    } else {
+    auto scan = [&]() {                                    // lds_place, [register][wave]: counts -> sums of those before
+        __syncthreads();
         uint32_t all;
-        const uint32_t rank = equal + block_scan(same ? 1u : 0u, lds_scan, all);
-        equal += all;
-        const bool stays = above || (same && rank < left);
-        const uint32_t at = out + block_scan(stays ? 1u : 0u, lds_scan, all);
-        out += all;
-        if (stays) kept[at] = i;
+        const uint32_t v = tid < E * WAVES ? lds_place[tid] : 0u, x = block_scan(v, lds_count[0], all);
+        if (tid < E * WAVES) lds_place[tid] = x;
+        __syncthreads();
+    };
+    static_assert(E * WAVES <= SELECT_THREADS, "a count a thread");
+    if (left < agree) {                                    // of the tokens equal to the border only the first `left` stay: the others become none
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t c = (uint32_t)__popcll(__ballot(key[e] == border));
+            if (lane == 0u) lds_place[e * WAVES + wave] = c;
+        }
+        scan();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool same = key[e] == border;
+            const uint32_t rank = lds_place[e * WAVES + wave] + before_lane(__ballot(same));
+            if (same && rank >= left) key[e] = 0u;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t c = (uint32_t)__popcll(__ballot(key[e] >= border));
+        if (lane == 0u) lds_place[e * WAVES + wave] = c;
+    }
+    scan();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool stays = key[e] >= border;
+        const uint32_t at = lds_place[e * WAVES + wave] + before_lane(__ballot(stays));
+        if (stays) kept[at] = e * SELECT_THREADS + tid;
+    }
     }
 }
 
@@ -150,7 +293,14 @@ extern "C" int tq_evict(const tq_packed_store *from, const tq_packed_store *to, 
         a.unit[s] = !(low & 15u) ? 16u : !(low & 3u) ? 4u : 1u;
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (keep) hipLaunchKernelGGL(tq_evict_select_kernel, dim3((unsigned)rows), dim3(SELECT_THREADS), 0, st, a);
+    if (keep) {
+        const dim3 g((unsigned)rows), t(SELECT_THREADS);
+        if (tokens <= SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<1>), g, t, 0, st, a);
+        else if (tokens <= 4 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<4>), g, t, 0, st, a);
+        else if (tokens <= 16 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<16>), g, t, 0, st, a);
+        else if (tokens <= 32 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<32>), g, t, 0, st, a);
+        else hipLaunchKernelGGL((tq_evict_select_kernel<0>), g, t, 0, st, a);
+    }
     hipLaunchKernelGGL(tq_evict_move_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st, a, (uint32_t)blocks);
     return (int)hipGetLastError();
 }
