@@ -172,7 +172,8 @@ __device__ __forceinline__ bool plain_seen(const TqManyArgs &a, uint32_t which, 
 __device__ __forceinline__ void store_result(const TqManyArgs &a, uint32_t row, uint32_t m, uint32_t d0, const float (&o)[16]) {
     const ManyQuery q(a, m);
     const size_t first = (((size_t)row * a.group + q.g) * a.queries + q.t) * a.D + d0;
-    if (a.dtype != TQ_F32 && !(a.D & 31u) && !((uintptr_t)a.out & 15u)) {
+    if (d0 >= a.D) return;
+    if (a.dtype != TQ_F32 && !(a.D & 15u) && !((uintptr_t)a.out & 15u)) {
         uint32_t w[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -207,11 +208,13 @@ __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b)
 
 }  // namespace
 
-// Launches tq_many_fast_kernel for one head dimension; ipbk, ipbv = codes per byte (1, 2, 4), qt = tiles of 32 queries a block, kt = fp16 terms of queries and key levels
-int tq_many_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
-int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
-int tq_many_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt);
+// Launches tq_many_fast_kernel for one padded head dimension; ipbk, ipbv = codes per byte (1, 2, 4), qt = tiles of 32 queries a block, kt, vt = fp16 terms on the key and value side
+int tq_many_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt);
+int tq_many_launch_d96(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt);
+int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt);
+int tq_many_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt);
 // the same for tq_many_weights_kernel, `blocks` a row
 int tq_many_weights_launch_d64(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);
+int tq_many_weights_launch_d96(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);
 int tq_many_weights_launch_d128(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);
 int tq_many_weights_launch_d256(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks);

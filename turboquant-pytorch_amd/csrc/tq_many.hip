@@ -13,14 +13,17 @@ long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 3
 
 struct Plan {
     long long rows, tiles, groups, splits, records, plain_records, floats;
-    int qt, kt;                      // tiles a block and fp16 terms of the kernels for one head dimension; qt = 0: the one for all
+    int qt, kt, vt;                  // tiles a block and fp16 terms of the kernels for one padded head dimension; qt = 0: the one for all
 };
 
-// Whether a head dimension and its code widths have a kernel of their own.  float32 results want two terms of weights and value levels as well.
+// Whether a head dimension and its code widths have a kernel of their own.
 bool fast(const tq_attend_request *r) {
-    const int ik = 8 / r->bits_k, iv = 8 / r->bits_v;
-    return (r->head_dim == 64 || r->head_dim == 128 || r->head_dim == 256) && ik <= 4 && iv <= 4 && r->dtype != TQ_F32 && r->tokens >= 32 &&
-           !((uintptr_t)r->k_idx & (tq_packed_alignment(r->head_dim, r->bits_k) - 1u)) && !((uintptr_t)r->v_idx & (tq_packed_alignment(r->head_dim, r->bits_v) - 1u));
+    const int ik = 8 / r->bits_k, iv = 8 / r->bits_v, D = r->head_dim;
+    if (ik > 4 || iv > 4 || r->tokens < 32) return false;
+    if (D == 64 || D == 128 || D == 256)
+        return !((uintptr_t)r->k_idx & (tq_packed_alignment(D, r->bits_k) - 1u)) && !((uintptr_t)r->v_idx & (tq_packed_alignment(D, r->bits_v) - 1u));
+    // 65 to 96: whole groups of eight elements, and words of packed bytes
+    return D > 64 && D <= 96 && !(D & 7) && !(D / ik & 3) && !(D % ik) && !(D / iv & 3) && !(D % iv) && !(((uintptr_t)r->k_idx | (uintptr_t)r->v_idx) & 3u);
 }
 
 // splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and what its start
@@ -45,10 +48,11 @@ int plan(const tq_attend_request *r, Plan &p) {
     p.tiles = (r->group * r->n_queries + 31) / 32;
     const long long at = p.rows * p.tiles;
     p.splits = 1;
-    p.qt = p.kt = 0;
+    p.qt = p.kt = p.vt = 0;
     p.groups = p.tiles;
     if (at && r->tokens && fast(r)) {
         p.kt = r->dtype == TQ_BF16 && !r->weights ? 1 : 2;
+        p.vt = r->dtype == TQ_F32 ? 2 : 1;
         p.qt = p.kt == 1 && r->head_dim != 256 && p.tiles > 1 ? 2 : 1;
         p.groups = (p.tiles + p.qt - 1) / p.qt;
         p.splits = fast_splits(p.rows * p.groups, plain_tiles(r) ? p.rows * p.groups : 0, r->tokens);
@@ -100,9 +104,10 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     if (plan.qt) {
         const dim3 g((unsigned)(plan.rows * plan.groups * plan.splits + a.plain_blocks));
         const int ik = 8 / (int)a.bits_k, iv = 8 / (int)a.bits_v;
-        if constexpr (DP == 64) tq_many_launch_d64(ik, iv, g, s, a, plan.qt, plan.kt);
-        if constexpr (DP == 128) tq_many_launch_d128(ik, iv, g, s, a, plan.qt, plan.kt);
-        if constexpr (DP == 256) tq_many_launch_d256(ik, iv, g, s, a, plan.qt, plan.kt);
+        if constexpr (DP == 64) tq_many_launch_d64(ik, iv, g, s, a, plan.qt, plan.kt, plan.vt);
+        if constexpr (DP == 96) tq_many_launch_d96(ik, iv, g, s, a, plan.qt, plan.kt, plan.vt);
+        if constexpr (DP == 128) tq_many_launch_d128(ik, iv, g, s, a, plan.qt, plan.kt, plan.vt);
+        if constexpr (DP == 256) tq_many_launch_d256(ik, iv, g, s, a, plan.qt, plan.kt, plan.vt);
     } else if (a.records) hipLaunchKernelGGL((tq_many_any_kernel<DP>), dim3(at * a.splits), dim3(64 * ANY_WAVES), 0, s, a);
     if (a.plain_records && !plan.qt) {
         const dim3 g(at), t(64 * PLAIN_WAVES);
@@ -124,6 +129,7 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
         const dim3 g(a.rows * blocks);
         const int ik = 8 / (int)a.bits_k;
         if constexpr (DP == 64) tq_many_weights_launch_d64(ik, g, s, a, blocks);
+        if constexpr (DP == 96) tq_many_weights_launch_d96(ik, g, s, a, blocks);
         if constexpr (DP == 128) tq_many_weights_launch_d128(ik, g, s, a, blocks);
         if constexpr (DP == 256) tq_many_weights_launch_d256(ik, g, s, a, blocks);
     } else if (a.tokens) {

@@ -1,9 +1,9 @@
 #include "tq_many_fast.h"
 
-int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt) {
-    if (ipbk == 4) return launch_many_fast<128, 4>(ipbv, grid, s, a, qt, kt);
-    if (ipbk == 2) return launch_many_fast<128, 2>(ipbv, grid, s, a, qt, kt);
-    return launch_many_fast<128, 1>(ipbv, grid, s, a, qt, kt);
+int tq_many_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt) {
+    if (ipbk == 4) return launch_many_fast<128, 4>(ipbv, grid, s, a, qt, kt, vt);
+    if (ipbk == 2) return launch_many_fast<128, 2>(ipbv, grid, s, a, qt, kt, vt);
+    return launch_many_fast<128, 1>(ipbv, grid, s, a, qt, kt, vt);
 }
 
 int tq_many_weights_launch_d128(int ipbk, dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks) {

@@ -1,6 +1,8 @@
-// Attention of tiles of queries over packed tokens at head dimensions 64, 128 and 256, codes of one, two or four to a byte (tq_many.hip).
-// One source file per head dimension instantiates it.
+// Attention of tiles of queries over packed tokens at head dimensions 64, 65 to 96, 128 and 256, codes of one, two or four to a byte (tq_many.hip).
+// One source file per padded head dimension instantiates it.
 #pragma once
+#include <type_traits>
+
 #include "tq_many.h"
 #include "tq_lut.h"
 
@@ -13,7 +15,15 @@ constexpr int FAST_SLACK = 8;                // a column's reference moves when 
 constexpr int FAST_P = 14 - FAST_SLACK;      // weights enter the products times 2^FAST_P, at most 2^14; value norms below 2 in their unit
 constexpr float FAST_START = -1.0e30f;
 
-// The keys' table with two fp16 terms a level: an entry is the byte's leading terms, then the rests; spread over the banks as Lut does.
+// A head dimension as the kernels work on it: DP, the next multiple of 32.  64, 128 and 256 are taken as they are; for others (EVEN false, a.D below DP possible) packed
+// bytes go through LDS, where they may lie anywhere.  On the value side a lane has NC coordinates in a row, NC n ... NC n + NC - 1, of which the first LANES lanes' exist.
+template <int DP>
+struct Shape {
+    static constexpr bool EVEN = DP == 64 || DP == 128 || DP == 256;
+    static constexpr int NC = EVEN ? DP / 32 : DP <= 128 ? 4 : 8, LANES = DP / NC, TILES = DP / 32, STEPS = DP / 16;
+};
+
+// A table of two fp16 terms a level: an entry is the byte's leading terms, then the rests; spread over the banks as Lut does.
 template <int IPB>
 struct Lut2 {
     static constexpr int ROWS = 4;
@@ -114,6 +124,79 @@ struct ValueBytes {
     }
 };
 
+// The same from a table of two terms: leading terms and rests
+template <int IPB, int NC>
+__device__ __forceinline__ void decode_values2(const ValueBytes<IPB, NC> &v, const uint8_t *lut, uint32_t slot, uint32_t odd, uint32_t (&hi)[NC / 2], uint32_t (&lo)[NC / 2]) {
+    if constexpr (IPB == 1) {
+#pragma unroll
+        for (int i = 0; i < NC / 2; i += 2) {
+            const uint32_t r = v.raw[i / 2 < ValueBytes<IPB, NC>::W ? i / 2 : 0];
+            const uint32_t a = lut_entry<0, uint32_t>(lut, r, slot), b = lut_entry<1, uint32_t>(lut, r, slot);
+            hi[i] = __builtin_amdgcn_perm(b, a, 0x05040100u); lo[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            if constexpr (NC > 2) {
+                const uint32_t c = lut_entry<2, uint32_t>(lut, r, slot), d = lut_entry<3, uint32_t>(lut, r, slot);
+                hi[i + 1] = __builtin_amdgcn_perm(d, c, 0x05040100u); lo[i + 1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+            }
+        }
+    } else if constexpr (IPB == 2) {
+        tq_u2 e[NC / 2];
+        e[0] = lut_entry<0, tq_u2>(lut, v.raw[0], slot);
+        if constexpr (NC >= 4) e[NC / 2 > 1 ? 1 : 0] = lut_entry<1, tq_u2>(lut, v.raw[0], slot);
+        if constexpr (NC == 8) { e[2] = lut_entry<2, tq_u2>(lut, v.raw[0], slot); e[3] = lut_entry<3, tq_u2>(lut, v.raw[0], slot); }
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i) { hi[i] = e[i][0]; lo[i] = e[i][1]; }
+    } else {
+        const tq_u4 a = lut_entry<0, tq_u4>(lut, v.raw[0], slot);
+        if constexpr (NC == 2) { hi[0] = odd ? a[1] : a[0]; lo[0] = odd ? a[3] : a[2]; }
+        else {
+            hi[0] = a[0]; hi[1] = a[1]; lo[0] = a[2]; lo[1] = a[3];
+            if constexpr (NC == 8) { const tq_u4 b = lut_entry<1, tq_u4>(lut, v.raw[0], slot); hi[2] = b[0]; hi[3] = b[1]; lo[2] = b[2]; lo[3] = b[3]; }
+        }
+    }
+}
+
+// Packed keys of 32 tokens: a lane's share is half a token, D / 2 coordinates.  issue() asks for them; where the shape is not even, stage() puts the bytes into LDS and take() reads them
+// from there (what lies past a vector's end are codes of anything, against queries of zero).
+template <int DP, int IPB>
+struct KeyRun {
+    static constexpr bool EVEN = Shape<DP>::EVEN;
+    static constexpr int KB = DP / 2 / IPB, KW = KB / 4, GB = DP / IPB, PIECES = (GB + 7) / 8;      // (words of a run per lane)
+    uint32_t raw[KW], piece[EVEN ? 1 : PIECES];
+    __device__ __forceinline__ void issue(const uint8_t *run, uint32_t bytes, uint32_t lane) {          // bytes: of a token
+        const uint32_t n = lane & 31u, h = lane >> 5;
+        if constexpr (!EVEN) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) piece[i] = tq_gload4(run + 4u * min(64u * i + lane, 8u * bytes - 1u));
+        } else if constexpr (KB % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < KB / 16; ++i) {
+                const tq_u4 v = tq_gload16(run + (n * GB + h * KB) + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[4 * i + j] = v[j];
+            }
+        } else {
+            static_assert(KB % 16 == 0 || KB == 8 || !EVEN, "eight bytes");
+            const tq_u2 v = tq_gload8(run + (n * GB + h * KB));
+            raw[0] = v[0]; raw[KW > 1 ? 1 : 0] = v[1];
+        }
+    }
+    __device__ __forceinline__ void stage(uint8_t *lds, uint32_t lane) const {
+        if constexpr (!EVEN) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                if (64 * i + 64 <= 8 * GB || 64u * i + lane < 8u * GB) *reinterpret_cast<uint32_t *>(lds + 4u * (64u * i + lane)) = piece[i];
+        }
+    }
+    __device__ __forceinline__ void take(const uint8_t *lds, uint32_t bytes, uint32_t lane) {
+        if constexpr (!EVEN) {
+            const uint8_t *p = lds + (lane & 31u) * bytes + (lane >> 5) * KB;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) raw[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
+        }
+    }
+    static constexpr uint32_t BYTES = EVEN ? 0u : 32u * GB;
+};
+
 // Eight 16-bit elements from any address
 __device__ __forceinline__ tq_u4 load_elements(const uint8_t *p, bool aligned) {
     if (aligned) return tq_gload16(p);
@@ -126,77 +209,113 @@ __device__ __forceinline__ tq_u4 load_elements(const uint8_t *p, bool aligned) {
 
 // Queries of QT tiles into the codec's space, q' = scale * log2(e) * Pi_k q, as fp16 operands in LDS ([tile][term][step][lane], as q_operand_bytes says): wave (tile i, w)
 // has coordinates 32 w ... + 31.  Pi as three bf16 terms, or for fp16 queries two fp16 ones (22 bits).  All tiles are scaled by the power of two
-// that puts their largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)); returns what products with them are to be multiplied by.
-template <int D, int QT, int KT, bool BF>
-__device__ __forceinline__ float rotate_queries(const TqManyArgs &a, uint32_t row, uint32_t tile0, uint8_t *ops, float *lds_top, uint32_t wave, uint32_t lane) {
-    constexpr int NC = D / 32, STEPS = D / 16, CH = STEPS < 8 ? STEPS : 8, TERMS = BF ? 3 : 2;
-    const uint32_t n = lane & 31u, h = lane >> 5, i = wave / NC, w = wave % NC;
-    float y[16], top = 0.f;
-    if (i < (uint32_t)QT) {
-        const uint32_t m = (tile0 + i) * 32u + n;
-        const uint8_t *q = many_query(a, row, min(m, a.M - 1u), 2u) + 16u * h;
-        const uint8_t *pi = a.table_k + (BF ? TQ_OFF_A_BF16(D) : TQ_OFF_A_F16) + ((size_t)w * STEPS * 64u + lane) * 16u;
-        tq_f16v acc = tq_zero16();
-#pragma unroll 1
-        for (int s0 = 0; s0 < STEPS; s0 += CH) {
-            tq_u4 x[CH], p[TERMS][CH];
+// that puts their largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)); returns what products with them are to be multiplied by.  load() asks for everything, so that other loads
+// can be under way before finish() waits.
+template <int DP, int QT, int KT, int DT>
+struct Rotate {
+    static constexpr int TILES = Shape<DP>::TILES, STEPS = DP / 16, CH = DT == TQ_F32 ? 2 : STEPS < 8 ? STEPS : STEPS % 8 ? STEPS / 2 : 8, TERMS = DT == TQ_F16 ? 2 : 3, NT = DT == TQ_F32 ? 3 : 1;
+    static_assert(STEPS % CH == 0 && QT * TILES <= FAST_WAVES, "whole chunks, waves that rotate");
+    tq_u4 x[CH][NT], p[TERMS][CH];
+    const uint8_t *q, *pi;
+    uint32_t i, w, m;
+    __device__ __forceinline__ void fetch(const TqManyArgs &a, int s0, uint32_t h) {
+#pragma unroll
+        for (int s = 0; s < CH; ++s)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) p[t][s] = tq_gload16(pi + (size_t)t * TQ_OPERAND_BYTES_FOR(DP) + (size_t)(s0 + s) * 1024u);
+        if constexpr (DT == TQ_F32) {
 #pragma unroll
             for (int s = 0; s < CH; ++s) {
+                tq_u4 t[3];
+                load_plain8<TQ_F32>(q, 16u * (s0 + s) + 8u * h, a.D, a.aligned, t);
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t) p[t][s] = tq_gload16(pi + (size_t)t * TQ_OPERAND_BYTES_FOR(D) + (size_t)(s0 + s) * 1024u);
+                for (int k = 0; k < NT; ++k) x[s][k] = t[k];
             }
-            if (a.aligned) {
+        } else if (a.aligned) {
 #pragma unroll
-                for (int s = 0; s < CH; ++s) x[s] = tq_gload16(q + 32u * (s0 + s));
-            } else {
-#pragma unroll
-                for (int s = 0; s < CH; ++s) x[s] = load_elements(q + 32u * (s0 + s), false);
+            for (int s = 0; s < CH; ++s) {
+                const uint32_t d = 16u * (s0 + s) + 8u * h;
+                x[s][0] = tq_gload16(q + 2u * (Shape<DP>::EVEN ? d : min(d, a.D - 8u)));
+                if (!Shape<DP>::EVEN && d >= a.D) x[s][0] = tq_u4{0u, 0u, 0u, 0u};
             }
+        } else {
 #pragma unroll
-            for (int s = 0; s < CH; ++s)
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) acc = BF ? mfma_bf16(p[t][s], x[s], acc) : mfma_f16(p[t][s], x[s], acc);
-        }
-        const float f = a.scale * (BF ? LOG2E : LOG2E / (float)(1 << TQ_F16_PI_SHIFT));
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {       // (the table's rows: register r of half h is coordinate 32 w + 16 h + r)
-            y[r] = m < a.M ? acc[r] * f : 0.f;
-            const float v = fabsf(y[r]);
-            top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
-        }
-        top = reduce_wave(top, OpMax());
-    }
-    if (lane == 0u) lds_top[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < FAST_WAVES; ++k) top = fmaxf(top, lds_top[k]);
-    const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
-    const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-    if (i < (uint32_t)QT) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            uint32_t t[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = fp16_terms(y[8 * j + k] * f);
-            tq_u4 hi, lo;
-            fp16_operands(t, hi, lo);
-            const uint32_t d = 32u * w + 16u * h + 8u * j, half = d / (D / 2u), s = (d - half * (D / 2u)) / 8u;
-            uint8_t *p = ops + ((i * KT * STEPS + s) * 64u + half * 32u + n) * 16u;
-            *reinterpret_cast<tq_u4 *>(p) = hi;
-            if constexpr (KT == 2) *reinterpret_cast<tq_u4 *>(p + STEPS * 1024u) = lo;
+            for (int s = 0; s < CH; ++s) {
+                const uint32_t d = 16u * (s0 + s) + 8u * h;
+                x[s][0] = load_elements(q + 2u * (Shape<DP>::EVEN ? d : min(d, a.D - 8u)), false);
+                if (!Shape<DP>::EVEN && d >= a.D) x[s][0] = tq_u4{0u, 0u, 0u, 0u};
+            }
         }
     }
-    return __uint_as_float((uint32_t)(127 - up - (KT == 2 ? LEVEL_SHIFT : 0)) << 23);
-}
+    __device__ __forceinline__ void load(const TqManyArgs &a, uint32_t row, uint32_t tile0, uint32_t wave, uint32_t lane) {
+        i = wave / TILES;
+        w = wave % TILES;
+        m = (tile0 + i) * 32u + (lane & 31u);
+        if (i >= (uint32_t)QT) return;
+        q = many_query(a, row, min(m, a.M - 1u), DT == TQ_F32 ? 4u : 2u);
+        pi = a.table_k + (DT == TQ_F16 ? TQ_OFF_A_F16 : TQ_OFF_A_BF16(DP)) + ((size_t)w * STEPS * 64u + lane) * 16u;
+        fetch(a, 0, lane >> 5);
+    }
+    __device__ __forceinline__ float finish(const TqManyArgs &a, uint8_t *ops, float *lds_top, uint32_t wave, uint32_t lane) {
+        const uint32_t n = lane & 31u, h = lane >> 5;
+        float y[16], top = 0.f;
+        if (i < (uint32_t)QT) {
+            tq_f16v acc = tq_zero16();
+#pragma unroll 1
+            for (int s0 = 0;;) {
+#pragma unroll
+                for (int s = 0; s < CH; ++s)
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                        for (int k = 0; k < NT; ++k)
+                            if (t + k < 3) acc = DT == TQ_F16 ? mfma_f16(p[t][s], x[s][k], acc) : mfma_bf16(p[t][s], x[s][k], acc);
+                s0 += CH;
+                if (s0 >= STEPS) break;
+                fetch(a, s0, h);
+            }
+            const float f = a.scale * (DT == TQ_F16 ? LOG2E / (float)(1 << TQ_F16_PI_SHIFT) : LOG2E);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {       // (the table's rows: register r of half h is coordinate 32 w + 16 h + r)
+                y[r] = m < a.M ? acc[r] * f : 0.f;
+                const float v = fabsf(y[r]);
+                top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
+            }
+            top = reduce_wave(top, OpMax());
+        }
+        if (lane == 0u) lds_top[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < FAST_WAVES; ++k) top = fmaxf(top, lds_top[k]);
+        const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+        const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+        if (i < (uint32_t)QT) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t t[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) t[k] = fp16_terms(y[8 * j + k] * f);
+                tq_u4 hi, lo;
+                fp16_operands(t, hi, lo);
+                const uint32_t d = 32u * w + 16u * h + 8u * j, half = d / (DP / 2u), s = (d - half * (DP / 2u)) / 8u;
+                uint8_t *o = ops + ((i * KT * STEPS + s) * 64u + half * 32u + n) * 16u;
+                *reinterpret_cast<tq_u4 *>(o) = hi;
+                if constexpr (KT == 2) *reinterpret_cast<tq_u4 *>(o + STEPS * 1024u) = lo;
+            }
+        }
+        return __uint_as_float((uint32_t)(127 - up - (KT == 2 ? LEVEL_SHIFT : 0)) << 23);
+    }
+};
 
 // 32 uncompressed tokens of a row (`which`: 0 the window, 1 the drafts; from t0 on) against a tile of queries: raw 16-bit products are exact, weights enter the value
 // product as three bf16 terms, or two fp16 ones.  Coordinates of the sums as in the packed loop: row r of acc[c] is coordinate NC r + c.  Infinite and NaN
 // values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); `wild` says whether there are any.
 // Up to 128 wide the tokens stay in registers from one tile of queries to the next (HELD), at 256 they are read as they are needed.
-template <int D, bool BF>
+template <int DP, int DT>
 struct PlainTile {
-    static constexpr int NC = D / 32, STEPS = D / 16, PT = BF ? 3 : 2;
-    static constexpr bool HELD = D <= 128;
+    static constexpr bool BF = DT == TQ_BF16, EVEN = Shape<DP>::EVEN;
+    static constexpr int NC = Shape<DP>::NC, STEPS = DP / 16, PT = BF ? 3 : 2;
+    static constexpr bool HELD = DP <= 128;
     static constexpr int VT = HELD ? 16 : 8, KH = HELD ? STEPS : 1;       // VT: tokens whose values are held at a time
     static constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
     uint32_t vw[VT][NC / 2];
@@ -205,6 +324,12 @@ struct PlainTile {
     uint32_t which, t0;
     bool wild;
 
+    // elements 16 st + 8 h ... + 7 of a vector, zeros from D on (a multiple of 8)
+    static __device__ __forceinline__ tq_u4 half_step(const uint8_t *vec, int st, uint32_t h, uint32_t D, bool aligned) {
+        const uint32_t d = 16u * st + 8u * h;
+        const tq_u4 v = load_elements(vec + 2u * (EVEN ? d : min(d, D - 8u)), aligned);
+        return EVEN || d < D ? v : tq_u4{0u, 0u, 0u, 0u};
+    }
     __device__ __forceinline__ void load_values(const TqManyArgs &a, int j0, uint32_t h) {
         const TqManyPlain &seg = a.plain[which];
 #pragma unroll
@@ -243,16 +368,16 @@ struct PlainTile {
         t0 = t0_;
         const TqManyPlain &seg = a.plain[which];
         const uint32_t n = lane & 31u, h = lane >> 5, kv = row - b * a.heads;
-        k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 2 + 16u * h;
-        v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 2 + 2u * NC * n;
+        k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 2;
+        v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 2 + 2u * NC * (EVEN ? n : min(n, a.D / NC - 1u));
         if constexpr (HELD) {
             if (a.aligned) {
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) kx[st] = tq_gload16(k + 32 * st);
+                for (int st = 0; st < STEPS; ++st) kx[st] = half_step(k, st, h, a.D, true);
             } else {
 #pragma unroll 1
                 for (int st = 0; st < STEPS; ++st) {
-                    const tq_u4 x = load_elements(k + 32 * st, false);
+                    const tq_u4 x = half_step(k, st, h, a.D, false);
 #pragma unroll
                     for (int i = 0; i < STEPS; ++i) kx[i] = i == st ? x : kx[i];
                 }
@@ -264,7 +389,7 @@ struct PlainTile {
     __device__ __forceinline__ void attend(const TqManyArgs &a, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t lane, float &m_ref, float &l, tq_f16v (&acc)[NC]) {
         const TqManyPlain &seg = a.plain[which];
         const uint32_t n = lane & 31u, h = lane >> 5, m = min(tile * 32u + n, a.M - 1u);
-        const uint8_t *q = many_query(a, row, m, 2u) + 16u * h;
+        const uint8_t *q = many_query(a, row, m, 2u);
         tq_f16v s = tq_zero16();
         if (a.aligned) {
             constexpr int CH = HELD ? STEPS : 4;
@@ -273,8 +398,8 @@ struct PlainTile {
                 tq_u4 x[CH], y[CH];
 #pragma unroll
                 for (int st = 0; st < CH; ++st) {
-                    x[st] = HELD ? kx[HELD ? st : 0] : tq_gload16(k + 32 * (s0 + st));
-                    y[st] = tq_gload16(q + 32 * (s0 + st));
+                    x[st] = HELD ? kx[HELD ? st : 0] : half_step(k, s0 + st, h, a.D, true);
+                    y[st] = half_step(q, s0 + st, h, a.D, true);
                 }
 #pragma unroll
                 for (int st = 0; st < CH; ++st) s = BF ? mfma_bf16(x[st], y[st], s) : mfma_f16(x[st], y[st], s);
@@ -282,7 +407,7 @@ struct PlainTile {
         } else {
 #pragma unroll 1
             for (int st = 0; st < STEPS; ++st) {
-                const tq_u4 x = load_elements(k + 32 * st, false), y = load_elements(q + 32 * st, false);
+                const tq_u4 x = half_step(k, st, h, a.D, false), y = half_step(q, st, h, a.D, false);
                 s = BF ? mfma_bf16(x, y, s) : mfma_f16(x, y, s);
             }
         }
@@ -340,14 +465,102 @@ struct PlainTile {
     }
 };
 
+// The same for float32 elements: three bf16 terms of everything, products down to 2^-24 of the largest.
+template <int DP>
+struct PlainTile<DP, TQ_F32> {
+    static constexpr int NC = Shape<DP>::NC, STEPS = DP / 16;
+    const uint8_t *k, *v;
+    uint32_t which, t0;
+    bool wild;
+    __device__ __forceinline__ void load(const TqManyArgs &a, uint32_t which_, uint32_t t0_, uint32_t row, uint32_t b, uint32_t lane) {
+        which = which_;
+        t0 = t0_;
+        const TqManyPlain &seg = a.plain[which];
+        const uint32_t n = lane & 31u, kv = row - b * a.heads;
+        k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * 4;
+        v = seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head) * 4 + 4u * NC * min(n, a.D / NC - 1u);
+    }
+    __device__ __forceinline__ void attend(const TqManyArgs &a, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t lane, float &m_ref, float &l, tq_f16v (&acc)[NC]) {
+        const TqManyPlain &seg = a.plain[which];
+        const uint32_t n = lane & 31u, h = lane >> 5, m = min(tile * 32u + n, a.M - 1u);
+        const uint8_t *q = many_query(a, row, m, 4u);
+        tq_f16v s = tq_zero16();
+#pragma unroll 1
+        for (int st = 0; st < STEPS; ++st) {
+            tq_u4 kt[3], qt[3];
+            load_plain8<TQ_F32>(k, 16u * st + 8u * h, a.D, a.aligned, kt);
+            load_plain8<TQ_F32>(q, 16u * st + 8u * h, a.D, a.aligned, qt);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+                for (int j = 0; j < 3 - i; ++j) s = mfma_bf16(kt[i], qt[j], s);
+        }
+        const uint32_t own = ManyQuery(a, m).t;
+        float x[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint32_t t = t0 + acc_row(r, h);
+            x[r] = t < seg.n && plain_seen(a, which, b, own, t, length) ? s[r] * (a.scale * LOG2E) : MANY_NONE;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+        top = fmaxf(halves_max(top), m_ref);
+        const float shrink = __builtin_amdgcn_exp2f(m_ref - top);
+        m_ref = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = x[r] == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(x[r] - top);
+            sum += x[r];
+        }
+        l = l * shrink + sum;
+        if (__any(shrink != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[c] *= shrink;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            float ps[8], e[8][NC];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ps[j] = x[8 * st + j];
+                const uint32_t t = t0 + acc_row(8 * st + j, h);
+                const uint8_t *p = v + (long long)min(t, seg.n - 1u) * seg.v_token * 4;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const float value = t < seg.n ? plain_element(p + 4 * c, TQ_F32) : 0.f;
+                    const bool fine = fabsf(value) < __builtin_inff();
+                    wild = wild || !fine;
+                    e[j][c] = fine ? value : 0.f;
+                }
+            }
+            tq_u4 p[3];
+            bf16_terms(ps, p);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float own8[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) own8[j] = e[j][c];
+                tq_u4 vt[3];
+                bf16_terms(own8, vt);
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+#pragma unroll
+                    for (int j = 0; j < 3 - i; ++j) acc[c] = mfma_bf16(vt[i], p[j], acc[c]);
+            }
+        }
+    }
+};
+
 // The sums of waves [w0, w0 + count) of a tile of queries into out[32][D + 4] and their largest logits and sums into out_m, out_l[32], all in LDS; every wave of the block
 // calls it, those with other w0 for another tile.  unit: what this wave's value sums are multiplied by; m_ref: MANY_NONE where it has seen no token of a
 // query; l: this lane's half.  area: [wave][32][64 + 4], two coordinates blocks of 32 at a time.
-template <int D>
+template <int DP>
 __device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], float (*lds_l)[32], float *out, float *out_m, float *out_l, uint32_t w0, uint32_t count, float unit, float m_ref,
-                                           float l, const tq_f16v (&acc)[D / 32], uint32_t tid) {
-    constexpr int NC = D / 32;
-    constexpr uint32_t MROW = 68u, ROW = D + 4;
+                                           float l, const tq_f16v (&acc)[Shape<DP>::NC], uint32_t tid) {
+    constexpr int NC = Shape<DP>::NC;
+    constexpr uint32_t MROW = 68u, ROW = DP + 4;
     const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const float both = halves_add(l);
     if (h == 0u) {
@@ -376,6 +589,7 @@ __device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], floa
         __syncthreads();
         for (uint32_t pair = mine; pair < 1024u; pair += threads) {        // coordinates NC r + c0, + 1 of query col
             const uint32_t col = pair / 32u, r = pair % 32u;
+            if (Shape<DP>::LANES < 32 && r >= (uint32_t)Shape<DP>::LANES) continue;
             float x = 0.f, y = 0.f;
             for (uint32_t w = w0; w < w0 + count; ++w) {
                 x += area[(w * 32u + col) * MROW + r];
@@ -388,23 +602,23 @@ __device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], floa
 }
 
 // joined sums of a tile -> its record
-template <int D>
+template <int DP>
 __device__ __forceinline__ void put_record(float *rec, const float *out, const float *out_m, const float *out_l, uint32_t tid) {
     TQ_GLOBAL float *p = (TQ_GLOBAL float *)rec;
     if (tid < 32u) { p[tid] = out_m[tid]; p[32u + tid] = out_l[tid]; }
-    for (uint32_t u = tid; u < 32u * D / 4u; u += FAST_THREADS) {
-        const uint32_t col = u / (D / 4u), d = (u - col * (D / 4u)) * 4u;
-        *reinterpret_cast<TQ_GLOBAL tq_f4 *>(p + 64u + col * D + d) = *reinterpret_cast<const tq_f4 *>(out + col * (D + 4u) + d);
+    for (uint32_t u = tid; u < 32u * DP / 4u; u += FAST_THREADS) {
+        const uint32_t col = u / (DP / 4u), d = (u - col * (DP / 4u)) * 4u;
+        *reinterpret_cast<TQ_GLOBAL tq_f4 *>(p + 64u + col * DP + d) = *reinterpret_cast<const tq_f4 *>(out + col * (DP + 4u) + d);
     }
 }
 
 // Infinite and NaN values of a row's uncompressed tokens into the joined sums of the queries that see them, whatever their weight (it is not zero).
-template <int D>
+template <int DP>
 __device__ __forceinline__ void add_wild(const TqManyArgs &a, float *out, uint32_t row, uint32_t b, uint32_t tile, uint32_t length, uint32_t tid) {
     const uint32_t kv = row - b * a.heads, elem = a.dtype;
 #pragma unroll 1
-    for (uint32_t e = tid; e < 32u * D; e += FAST_THREADS) {
-        const uint32_t col = e / D, d = e - col * D, m = tile * 32u + col;
+    for (uint32_t e = tid; e < 32u * a.D; e += FAST_THREADS) {
+        const uint32_t col = e / a.D, d = e - col * a.D, m = tile * 32u + col;
         if (m >= a.M) return;
         const uint32_t own = ManyQuery(a, m).t;
         float sum = 0.f;
@@ -413,29 +627,29 @@ __device__ __forceinline__ void add_wild(const TqManyArgs &a, float *out, uint32
             const TqManyPlain &seg = a.plain[which];
 #pragma unroll 1
             for (uint32_t t = 0; t < seg.n; ++t) {
-                const float v = plain_element(seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head + (long long)t * seg.v_token + d) * 2, elem);
+                const float v = plain_element(seg.v + ((long long)b * seg.v_batch + (long long)kv * seg.v_head + (long long)t * seg.v_token + d) * (elem == TQ_F32 ? 4 : 2), elem);
                 if (!(fabsf(v) < __builtin_inff()) && plain_seen(a, which, b, own, t, length)) sum += v;
             }
         }
-        if (sum != 0.f) out[col * (D + 4u) + d] += sum;
+        if (sum != 0.f) out[col * (DP + 4u) + d] += sum;
     }
 }
 
 // LDS once the packed tokens are done with: what waves join their sums through, and the joined sums of packed and uncompressed tokens of each tile
-template <int D, int QT>
+template <int DP, int QT>
 struct JoinArea {
-    static constexpr uint32_t TILE = 32u * (D + 4u) * 4u, JOIN = FAST_WAVES * 32u * 68u * 4u, PACKED = JOIN, PLAIN = PACKED + QT * TILE, STATS = PLAIN + QT * TILE, BYTES = STATS + 4u * QT * 128u;
+    static constexpr uint32_t TILE = 32u * (DP + 4u) * 4u, JOIN = FAST_WAVES * 32u * 68u * 4u, PACKED = JOIN, PLAIN = PACKED + QT * TILE, STATS = PLAIN + QT * TILE, BYTES = STATS + 4u * QT * 128u;
     static __device__ __forceinline__ float *sums(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + (plain ? PLAIN : PACKED) + i * TILE); }
     static __device__ __forceinline__ float *largest(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + STATS + (2u * (plain * QT + i)) * 128u); }
     static __device__ __forceinline__ float *total(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + STATS + (2u * (plain * QT + i) + 1u) * 128u); }
 };
 
 // A row's uncompressed tokens against the block's tiles of queries, joined sums into LDS.  Two tiles share the waves where four of them hold all tokens.
-template <int D, int QT, bool BF>
+template <int DP, int QT, int DT>
 __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, float (*lds_m)[32], float (*lds_l)[32], float *lds_wild, uint32_t row, uint32_t b, uint32_t tile0, uint32_t tiles,
                                             uint32_t length, uint32_t tid) {
-    constexpr int NC = D / 32;
-    using J = JoinArea<D, QT>;
+    constexpr int NC = Shape<DP>::NC;
+    using J = JoinArea<DP, QT>;
     const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6);
     const uint32_t first = (a.plain[0].n + 31u) / 32u, all = first + (a.plain[1].n + 31u) / 32u;
     const bool share = QT == 2 && tiles == 2u && all <= FAST_WAVES / 2u;
@@ -450,7 +664,7 @@ __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, f
         bool wild = false;
 #pragma unroll 1
         for (uint32_t w = wave - w0; w < all; w += count) {
-            PlainTile<D, BF> t;
+            PlainTile<DP, DT> t;
             t.wild = false;
             t.load(a, w < first ? 0u : 1u, 32u * (w < first ? w : w - first), row, b, lane);
             t.attend(a, row, b, tile0 + mine, length, lane, m, l, acc);
@@ -458,15 +672,15 @@ __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, f
         }
         __syncthreads();             // (what the area held)
         if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
-        join_waves<D>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, count, 1.f, m, l, acc, tid);
+        join_waves<DP>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, count, 1.f, m, l, acc, tid);
         __syncthreads();
         float any = 0.f;
 #pragma unroll
         for (int w = 0; w < FAST_WAVES; ++w) any += lds_wild[w];
         if (any != 0.f) {
-            if (!share) add_wild<D>(a, J::sums(lds, 1u, i), row, b, tile0 + i, length, tid);
+            if (!share) add_wild<DP>(a, J::sums(lds, 1u, i), row, b, tile0 + i, length, tid);
             else
-                for (uint32_t k = 0; k < 2u; ++k) add_wild<D>(a, J::sums(lds, 1u, k), row, b, tile0 + k, length, tid);
+                for (uint32_t k = 0; k < 2u; ++k) add_wild<DP>(a, J::sums(lds, 1u, k), row, b, tile0 + k, length, tid);
             __syncthreads();
         }
     }
@@ -474,13 +688,13 @@ __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, f
 
 // Results of the block's tiles from the joined sums in LDS, where a row's tokens are in one split: packed sums turned back by Pi_v (two fp16 terms each, as the merge
 // does), the uncompressed ones added, divided by the sum of weights.
-template <int D, int QT>
+template <int DP, int QT>
 __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, bool plain, uint32_t row, uint32_t tile0, uint32_t tiles, uint32_t tid) {
-    constexpr int NC = D / 32, STEPS = D / 16, CH = STEPS < 8 ? STEPS : 8;
-    using J = JoinArea<D, QT>;
-    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, i = wave / NC, w = wave % NC;
+    constexpr int TILES = Shape<DP>::TILES, STEPS = DP / 16, CH = STEPS < 8 ? STEPS : 8;
+    using J = JoinArea<DP, QT>;
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, i = wave / TILES, w = wave % TILES;
     if (i >= tiles) return;
-    const float *o = J::sums(lds, 0u, i) + n * (D + 4u), *p = J::sums(lds, 1u, i) + n * (D + 4u);
+    const float *o = J::sums(lds, 0u, i) + n * (DP + 4u), *p = J::sums(lds, 1u, i) + n * (DP + 4u);
     const float m0 = J::largest(lds, 0u, i)[n], m1 = plain ? J::largest(lds, 1u, i)[n] : MANY_NONE, m = fmaxf(m0, m1);
     const float f0 = m0 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m0 - m), f1 = m1 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
     const float l = J::total(lds, 0u, i)[n] * f0 + (plain ? J::total(lds, 1u, i)[n] * f1 : 0.f), inv = l == 0.f ? 0.f : 1.0f / l;
@@ -491,11 +705,11 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
         stat[n] = some ? m : -MANY_NONE;
         stat[32u + n] = some ? inv : 0.f;
     }
-    const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(D) + ((size_t)w * STEPS * 64u + lane) * 16u;
+    const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(DP) + ((size_t)w * STEPS * 64u + lane) * 16u;
     float largest = 0.f;
 #pragma unroll 8
-    for (uint32_t d = 0; d < D / 2u; d += 4u) {
-        const tq_f4 v = *reinterpret_cast<const tq_f4 *>(o + h * (D / 2u) + d);
+    for (uint32_t d = 0; d < DP / 2u; d += 4u) {
+        const tq_f4 v = *reinterpret_cast<const tq_f4 *>(o + h * (DP / 2u) + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
     }
@@ -507,14 +721,17 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
     for (int s0 = 0; s0 < STEPS; s0 += CH) {
         tq_u4 ph[CH], pl[CH];
 #pragma unroll
-        for (int s = 0; s < CH; ++s) { ph[s] = tq_gload16(pi + (size_t)(s0 + s) * 1024u); pl[s] = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(D) + (size_t)(s0 + s) * 1024u); }
+        for (int s = 0; s < CH; ++s) { ph[s] = tq_gload16(pi + (size_t)(s0 + s) * 1024u); pl[s] = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(DP) + (size_t)(s0 + s) * 1024u); }
 #pragma unroll
         for (int s = 0; s < CH; ++s) {
-            const uint32_t j = D == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
+            const uint32_t j = DP == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
             const tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + j), y = *reinterpret_cast<const tq_f4 *>(o + j + 4u);
             uint32_t t[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { t[k] = fp16_terms(x[k] * f); t[4 + k] = fp16_terms(y[k] * f); }
+            for (int k = 0; k < 4; ++k) {
+                t[k] = Shape<DP>::EVEN || j + k < a.D ? fp16_terms(x[k] * f) : 0u;
+                t[4 + k] = Shape<DP>::EVEN || j + 4 + k < a.D ? fp16_terms(y[k] * f) : 0u;
+            }
             tq_u4 oh, ol;
             fp16_operands(t, oh, ol);
             acc = mfma_f16(ph[s], oh, acc);
@@ -524,7 +741,7 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
     }
     if (q >= a.M) return;
     const float back = __uint_as_float((uint32_t)(127 - up) << 23) * f0;
-    const uint32_t d0 = D == TQ_HEAD_DIM ? 64u * h + 16u * w : 32u * w + 16u * h;
+    const uint32_t d0 = DP == TQ_HEAD_DIM ? 64u * h + 16u * w : 32u * w + 16u * h;
     float out[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) out[r] = inv == 0.f ? 0.f : (acc[r] * back + (plain ? p[d0 + r] * f1 : 0.f)) * inv;
@@ -537,25 +754,27 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 //   * weights times value norms are, as they lie, the B operand of the value product (its contraction runs over the tokens in the order in which a lane
 //     has them); A = values, every lane decoding its coordinates' bytes of eight tokens.
 // KT = 1: queries and levels as one fp16 value each, for bfloat16: the 2^-12 roundings move logits of some ten by 1e-3, where a bfloat16 result is rounded by up to 4e-3.
-// KT = 2: two terms each (three products, 22 bits), for float16 and wherever sums of weights are kept.  Weights and value levels are one fp16 value each (the
+// KT = 2: two terms each (three products, 22 bits), for float16, float32 and wherever sums of weights are kept; VT = 2: of weights and value levels as well, for float32.  Weights and value levels are one fp16 value each (the
 // reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's sum of weights is made of the rounded weights
 // themselves, so that their rounding cancels in part.
-template <int D, int IPBK, int IPBV, int QT, int KT>
+template <int DP, int IPBK, int IPBV, int QT, int KT, int VT>
 __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_kernel(TqManyArgs a) {
-    constexpr int STEPS = D / 16, NC = D / 32, KB = D / 2 / IPBK, KW = KB / 4, GBK = D / IPBK, GBV = D / IPBV;
+    using S = Shape<DP>;
+    using Keys = KeyRun<DP, IPBK>;
+    constexpr int STEPS = S::STEPS, NC = S::NC, GBV_MAX = DP / IPBV;
     using Values = ValueBytes<IPBV, NC>;
     constexpr int QW = KT * QT * STEPS * 4;                                        // registers of the queries' operands
     constexpr bool QREG = QW + QT * NC * 16 <= 136;
     constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024;
-    constexpr int VPIECE = GBV / 2;                                                // bytes of a run's values that a lane stages
-    constexpr bool STAGE = GBV <= 128;
-    using J = JoinArea<D, QT>;
-    constexpr int LOOP_BYTES = LUT_BYTES + Q_BYTES + (STAGE ? FAST_WAVES * 32 * GBV : 0);
-    constexpr int AREA = LOOP_BYTES > (int)J::BYTES ? LOOP_BYTES : (int)J::BYTES;
-    static_assert(QT * NC <= FAST_WAVES, "waves that rotate");
+    constexpr bool STAGE = !S::EVEN || GBV_MAX <= 128;
+    constexpr int VPIECES = S::EVEN ? (GBV_MAX >= 32 ? GBV_MAX / 32 : 1) : (GBV_MAX + 31) / 32;        // 16 bytes of a run's values, that a lane stages
+    constexpr uint32_t WAVE_BYTES = Keys::BYTES + (STAGE ? 32u * GBV_MAX : 0u);
+    using J = JoinArea<DP, QT>;
+    constexpr uint32_t LOOP_BYTES = LUT_BYTES + Q_BYTES + FAST_WAVES * WAVE_BYTES + (S::EVEN ? 0u : 64u);       // (uneven: lanes past the last coordinate read on)
+    constexpr uint32_t AREA = LOOP_BYTES > J::BYTES ? LOOP_BYTES : J::BYTES;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[FAST_WAVES][32];
-    __shared__ __attribute__((aligned(16))) uint16_t lds_vn[FAST_WAVES][32];
+    __shared__ __attribute__((aligned(16))) std::conditional_t<VT == 2, float, uint16_t> lds_vn[FAST_WAVES][32];
     __shared__ float lds_m[FAST_WAVES][32], lds_l[FAST_WAVES][32];
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
@@ -570,45 +789,104 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     // A row's uncompressed tokens: by the block that has its packed ones, where they are in one split, otherwise by blocks of their own, the first of
     // the launch, so that they are done while the others are at the packed ones.
     if (packed) {
-    if constexpr (KT == 1) {
-        Lut<IPBK> table;
-        table.load(a.table_k + TQ_OFF_LUT(D), tid);
-        table.store(lds, tid);
-    } else {
-        Lut2<IPBK> table;
-        table.load(a.table_k, a.bits_k, D, tid);
-        table.store(lds, tid);
-    }
-    {
-        Lut<IPBV> table;
-        table.load(a.table_v + TQ_OFF_LUT(D), tid);
-        table.store(lds + 128, tid);
-    }
-    uint8_t *ops = lds + LUT_BYTES;
-    const float q_scale = a.dtype == TQ_BF16 ? rotate_queries<D, QT, KT, true>(a, row, tile0, ops, lds_kn[0], wave, lane) : rotate_queries<D, QT, KT, false>(a, row, tile0, ops, lds_kn[0], wave, lane);
-    __syncthreads();
-    tq_u4 q[QREG ? KT * QT * STEPS : 1];
-    if constexpr (QREG) {
-#pragma unroll
-        for (int s = 0; s < KT * QT * STEPS; ++s) q[s] = *reinterpret_cast<const tq_u4 *>(ops + s * 1024 + lane * 16u);
-    }
-    auto query = [&](int i, int term, int s) __attribute__((always_inline)) -> tq_u4 {
-        if constexpr (QREG) return q[(i * KT + term) * STEPS + s];
-        else return *reinterpret_cast<const tq_u4 *>(ops + ((i * KT + term) * STEPS + s) * 1024 + lane * 16u);
-    };
-    if (a.weights && split == 0u) {          // (KT = 2: whole operands) for the launch that adds up what keys receive
-        for (uint32_t i = tid; i < Q_BYTES / 16u; i += FAST_THREADS) tq_gstore16(a.q_op + first_tile * q_operand_bytes(D) + i * 16u, *reinterpret_cast<const tq_u4 *>(ops + i * 16u));
-        if (tid == 0u) a.q_scale[first_tile] = q_scale;
-    }
-    const uint32_t slot_k = KT == 1 ? RepLut<IPBK>::lane_offset(lane) : Lut2<IPBK>::lane_offset(lane);
-    const uint32_t slot_v = 128u + (IPBV == 4 && NC == 2 ? (lane & 30u) / 2u * 8u + 4u * (lane & 1u) : RepLut<IPBV>::lane_offset(lane));
-
+    const uint32_t GBK = S::EVEN ? DP / IPBK : (a.D + IPBK - 1u) / IPBK, GBV = S::EVEN ? DP / IPBV : (a.D + IPBV - 1u) / IPBV;
     const uint32_t seen = min(a.tokens, length);
     const uint32_t chunk = a.lengths ? ((seen + a.splits - 1u) / a.splits + 31u) / 32u * 32u : a.chunk;       // (a short sequence keeps all its blocks busy)
     const uint32_t begin = min(seen, split * chunk), end = min(seen, begin + chunk);
     const size_t slot0 = (size_t)row * a.packed_row_stride;
     const uint8_t *mask = a.mask ? a.mask + (long long)b * a.mask_stride : nullptr;
-    const uint32_t k_lane = n * GBK + h * KB, v_lane = 4u * h * GBV + (IPBV == 4 && NC == 2 ? n / 2u : n * Values::VB);
+    const uint32_t v_lane = 4u * h * GBV + (IPBV == 4 && NC == 2 ? n / 2u : n * Values::VB);
+
+    // Loads of a run are issued while the one before it is worked on.  The last run of a row begins 32 tokens before the end: what the one before it
+    // had already is hidden, and nothing past the row's tokens is read.
+    // Value bytes go through LDS on their way (a lane needs single bytes of sixteen tokens), but at 256 with a byte a code, where they are
+    // read from memory as they are needed.
+    Keys keys;
+    tq_u4 vpiece[VPIECES];
+    Values vraw[16];
+    uint16_t kn_raw = 0, vn_raw = 0;
+    uint8_t *kstage = lds + LUT_BYTES + Q_BYTES + wave * WAVE_BYTES, *vstage = kstage + Keys::BYTES;
+    auto issue_keys = [&](uint32_t t) __attribute__((always_inline)) {
+        keys.issue(a.k_idx + (slot0 + t) * GBK, GBK, lane);
+        kn_raw = tq_gload2(a.k_norms + slot0 + t + n);
+        vn_raw = tq_gload2(a.v_norms + slot0 + t + n);
+    };
+    auto issue_values = [&](uint32_t t) __attribute__((always_inline)) {
+        const uint8_t *p = a.v_idx + (slot0 + t) * GBV;
+        if constexpr (!STAGE) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) vraw[j].load(p + v_lane + (8 * (j / 4) + j % 4) * GBV);
+        } else if constexpr (!S::EVEN) {
+#pragma unroll
+            for (int i = 0; i < VPIECES; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) vpiece[i][k] = tq_gload4(p + 4u * min(256u * i + 64u * k + lane, 8u * GBV - 1u));
+        } else if constexpr (GBV_MAX == 16) {
+            const tq_u2 v = tq_gload8(p + lane * 8u);
+            vpiece[0][0] = v[0]; vpiece[0][1] = v[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPIECES; ++i) vpiece[i] = tq_gload16(p + i * 1024 + lane * 16u);
+        }
+    };
+    auto stage_values = [&]() __attribute__((always_inline)) {
+        if constexpr (!S::EVEN) {
+#pragma unroll
+            for (int i = 0; i < VPIECES; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (256u * i + 64u * k + lane < 8u * GBV_MAX) *reinterpret_cast<uint32_t *>(vstage + 4u * (256u * i + 64u * k + lane)) = vpiece[i][k];
+        } else if constexpr (GBV_MAX == 16) *reinterpret_cast<tq_u2 *>(vstage + lane * 8u) = tq_u2{vpiece[0][0], vpiece[0][1]};
+        else {
+#pragma unroll
+            for (int i = 0; i < VPIECES; ++i) *reinterpret_cast<tq_u4 *>(vstage + i * 1024 + lane * 16u) = vpiece[i];
+        }
+    };
+    const uint32_t last = a.tokens - 32u;    // (launched for 32 tokens at least)
+    uint32_t t_next = begin + 32u * wave;
+    // ---- start: tables, rotation and the first run are asked for before anything is waited for
+    uint8_t *ops = lds + LUT_BYTES;
+    std::conditional_t<KT == 1, Lut<IPBK>, Lut2<IPBK>> table_k;
+    std::conditional_t<VT == 1, Lut<IPBV>, Lut2<IPBV>> table_v;
+    if constexpr (KT == 1) table_k.load(a.table_k + TQ_OFF_LUT(DP), tid);
+    else table_k.load(a.table_k, a.bits_k, DP, tid);
+    if constexpr (VT == 1) table_v.load(a.table_v + TQ_OFF_LUT(DP), tid);
+    else table_v.load(a.table_v, a.bits_v, DP, tid);
+    float q_scale;
+    auto start = [&](auto dt_tag) __attribute__((always_inline)) {
+        Rotate<DP, QT, KT, decltype(dt_tag)::value> r;
+        r.load(a, row, tile0, wave, lane);
+        if (t_next < end) {
+            issue_keys(min(t_next, last));
+            issue_values(min(t_next, last));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        table_k.store(lds, tid);
+        table_v.store(lds + 128, tid);
+        q_scale = r.finish(a, ops, lds_kn[0], wave, lane);
+    };
+    if constexpr (VT == 2) start(std::integral_constant<int, TQ_F32>{});
+    else if (a.dtype == TQ_BF16) start(std::integral_constant<int, TQ_BF16>{});
+    else if constexpr (KT == 2) start(std::integral_constant<int, TQ_F16>{});
+    else __builtin_unreachable();            // (KT = 1 is launched for bfloat16 alone)
+    __syncthreads();
+    uint32_t ops_lane = LUT_BYTES + lane * 16u;
+    asm volatile("" : "+v"(ops_lane));        // (one base for all operands: the offsets then fit the instructions)
+    tq_u4 q[QREG ? KT * QT * STEPS : 1];
+    if constexpr (QREG) {
+#pragma unroll
+        for (int s = 0; s < KT * QT * STEPS; ++s) q[s] = *reinterpret_cast<const tq_u4 *>(lds + ops_lane + s * 1024);
+    }
+    auto query = [&](int i, int term, int s) __attribute__((always_inline)) -> tq_u4 {
+        if constexpr (QREG) return q[(i * KT + term) * STEPS + s];
+        else return *reinterpret_cast<const tq_u4 *>(lds + ops_lane + ((i * KT + term) * STEPS + s) * 1024);
+    };
+    if (a.weights && split == 0u) {          // (KT = 2: whole operands) for the launch that adds up what keys receive
+        for (uint32_t i = tid; i < Q_BYTES / 16u; i += FAST_THREADS) tq_gstore16(a.q_op + first_tile * q_operand_bytes(DP) + i * 16u, *reinterpret_cast<const tq_u4 *>(ops + i * 16u));
+        if (tid == 0u) a.q_scale[first_tile] = q_scale;
+    }
+    const uint32_t slot_k = KT == 1 ? RepLut<IPBK>::lane_offset(lane) : Lut2<IPBK>::lane_offset(lane);
+    const uint32_t slot_v = 128u + (VT == 2 ? Lut2<IPBV>::lane_offset(lane) : IPBV == 4 && NC == 2 ? (lane & 30u) / 2u * 8u + 4u * (lane & 1u) : RepLut<IPBV>::lane_offset(lane));
 
     float m_ref[QT], l[QT];
     tq_f16v acc[QT][NC];
@@ -620,52 +898,6 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         for (int c = 0; c < NC; ++c) acc[i][c] = tq_zero16();
     }
     int v_top = -100;                        // 2^v_top: unit of the value norms, their largest binary exponent so far
-
-    // Loads of a run are issued while the one before it is worked on.  The last run of a row begins 32 tokens before the end: what the one before it
-    // had already is hidden, and nothing past the row's tokens is read.
-    // Value bytes go through LDS on their way (a lane needs single bytes of sixteen tokens), but at 256 with a byte a code, where they are
-    // read from memory as they are needed.
-    uint32_t kraw[KW];
-    tq_u4 vpiece[STAGE && VPIECE >= 16 ? VPIECE / 16 : 1];
-    Values vraw[16];
-    uint16_t kn_raw = 0, vn_raw = 0;
-    uint8_t *vstage = lds + LUT_BYTES + Q_BYTES + wave * (STAGE ? 32u * GBV : 0u);
-    auto issue_keys = [&](uint32_t t) __attribute__((always_inline)) {
-        const uint8_t *p = a.k_idx + (slot0 + t) * GBK;
-        if constexpr (KB % 16 == 0) {
-#pragma unroll
-            for (int i = 0; i < KB / 16; ++i) {
-                const tq_u4 v = tq_gload16(p + k_lane + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) kraw[4 * i + j] = v[j];
-            }
-        } else {
-            static_assert(KB == 8, "eight bytes");
-            const tq_u2 v = tq_gload8(p + k_lane);
-            kraw[0] = v[0]; kraw[1] = v[1];
-        }
-        kn_raw = tq_gload2(a.k_norms + slot0 + t + n);
-        vn_raw = tq_gload2(a.v_norms + slot0 + t + n);
-    };
-    auto issue_values = [&](uint32_t t) __attribute__((always_inline)) {
-        const uint8_t *p = a.v_idx + (slot0 + t) * GBV;
-        if constexpr (!STAGE) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) vraw[j].load(p + v_lane + (8 * (j / 4) + j % 4) * GBV);
-        } else if constexpr (VPIECE == 8) {
-            const tq_u2 v = tq_gload8(p + lane * 8u);
-            vpiece[0][0] = v[0]; vpiece[0][1] = v[1];
-        } else {
-#pragma unroll
-            for (int i = 0; i < VPIECE / 16; ++i) vpiece[i] = tq_gload16(p + i * 1024 + lane * 16u);
-        }
-    };
-    const uint32_t last = a.tokens - 32u;    // (launched for 32 tokens at least)
-    uint32_t t_next = begin + 32u * wave;
-    if (t_next < end) {
-        issue_keys(min(t_next, last));
-        issue_values(min(t_next, last));
-    }
     while (t_next < end) {
         const uint32_t t_run = t_next, t0 = min(t_run, last), count = min(32u, end - t_run);
         t_next += 32u * FAST_WAVES;
@@ -689,30 +921,29 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 for (int c = 0; c < NC; ++c) acc[i][c] *= f;
         }
         norm *= h ? __uint_as_float((uint32_t)(127 - v_top) << 23) : q_scale;
-        if (h) lds_vn[wave][n] = __builtin_bit_cast(uint16_t, (_Float16)norm);
-        else lds_kn[wave][n] = norm;
+        if (!h) lds_kn[wave][n] = norm;
+        else if constexpr (VT == 2) lds_vn[wave][n] = norm;
+        else lds_vn[wave][n] = __builtin_bit_cast(uint16_t, (_Float16)norm);
+        keys.stage(kstage, lane);
         if constexpr (STAGE) {
-            if constexpr (VPIECE == 8) *reinterpret_cast<tq_u2 *>(vstage + lane * 8u) = tq_u2{vpiece[0][0], vpiece[0][1]};
-            else {
-#pragma unroll
-                for (int i = 0; i < VPIECE / 16; ++i) *reinterpret_cast<tq_u4 *>(vstage + i * 1024 + lane * 16u) = vpiece[i];
-            }
+            stage_values();
             issue_values(t_after);
         }
         wave_sync();
         // ---- scores
+        keys.take(kstage, GBK, lane);
         tq_f16v s[QT];
 #pragma unroll
         for (int i = 0; i < QT; ++i) s[i] = tq_zero16();
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
             if constexpr (KT == 1) {
-                const tq_u4 k = decode_keys<IPBK, KW>(kraw, st, lds, slot_k);
+                const tq_u4 k = decode_keys<IPBK, Keys::KW>(keys.raw, st, lds, slot_k);
 #pragma unroll
                 for (int i = 0; i < QT; ++i) s[i] = mfma_f16(k, query(i, 0, st), s[i]);
             } else {
                 tq_u4 hi, lo;
-                decode_keys2<IPBK, KW>(kraw, st, lds, slot_k, hi, lo);
+                decode_keys2<IPBK, Keys::KW>(keys.raw, st, lds, slot_k, hi, lo);
 #pragma unroll
                 for (int i = 0; i < QT; ++i) {
                     const tq_u4 qh = query(i, 0, st), ql = query(i, KT - 1, st);
@@ -724,7 +955,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         }
         issue_keys(t_after);
         // ---- weights
-        tq_u4 p[QT][2];
+        tq_u4 p[QT][2], p2[VT == 2 ? QT : 1][2];
         float kn[16];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -732,11 +963,17 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 #pragma unroll
             for (int j = 0; j < 4; ++j) kn[4 * k + j] = v[j];
         }
-        uint32_t vn[8];
+        uint32_t vn[VT == 2 ? 16 : 8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const tq_u2 v = *reinterpret_cast<const tq_u2 *>(&lds_vn[wave][8 * k + 4 * h]);
-            vn[2 * k] = v[0]; vn[2 * k + 1] = v[1];
+            if constexpr (VT == 2) {
+                const tq_u4 v = *reinterpret_cast<const tq_u4 *>(&lds_vn[wave][8 * k + 4 * h]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) vn[4 * k + j] = v[j];
+            } else {
+                const tq_u2 v = *reinterpret_cast<const tq_u2 *>(&lds_vn[wave][8 * k + 4 * h]);
+                vn[2 * k] = v[0]; vn[2 * k + 1] = v[1];
+            }
         }
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
@@ -776,36 +1013,58 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 for (int r = 0; r < 16; ++r) { x[r] = __builtin_amdgcn_exp2f(x[r]); sum += x[r]; }
                 l[i] += sum;
             }
+            if constexpr (VT == 2) {
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                tq_half2 w;
-                if constexpr (KT == 2) w = tq_half2{(_Float16)x[2 * d], (_Float16)x[2 * d + 1]};
-                else {
-                    w = tq_half2{(_Float16)__builtin_amdgcn_exp2f(x[2 * d]), (_Float16)__builtin_amdgcn_exp2f(x[2 * d + 1])};
-                    l[i] = __builtin_amdgcn_fdot2(w, tq_half2{(_Float16)1.f, (_Float16)1.f}, l[i], false);
+                for (int st = 0; st < 2; ++st) {
+                    uint32_t t[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[j] = fp16_terms(x[8 * st + j] * __uint_as_float(vn[8 * st + j]));
+                    fp16_operands(t, p[i][st], p2[i][st]);
                 }
-                p[i][d / 4][d % 4] = __builtin_bit_cast(uint32_t, w * __builtin_bit_cast(tq_half2, vn[d]));
+            } else {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    tq_half2 w;
+                    if constexpr (KT == 2) w = tq_half2{(_Float16)x[2 * d], (_Float16)x[2 * d + 1]};
+                    else {
+                        w = tq_half2{(_Float16)__builtin_amdgcn_exp2f(x[2 * d]), (_Float16)__builtin_amdgcn_exp2f(x[2 * d + 1])};
+                        l[i] = __builtin_amdgcn_fdot2(w, tq_half2{(_Float16)1.f, (_Float16)1.f}, l[i], false);
+                    }
+                    p[i][d / 4][d % 4] = __builtin_bit_cast(uint32_t, w * __builtin_bit_cast(tq_half2, vn[d]));
+                }
             }
         }
         // ---- values
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            uint32_t w[8][NC / 2];
+            uint32_t w[8][NC / 2], w2[VT == 2 ? 8 : 1][NC / 2];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (STAGE) {
-                    Values v;
-                    v.fetch(vstage + v_lane + (16 * st + 8 * (j / 4) + j % 4) * GBV);
-                    v.decode(lds, slot_v, w[j]);
-                } else vraw[8 * st + j].decode(lds, slot_v, w[j]);
+                Values v;
+                if constexpr (STAGE) v.fetch(vstage + v_lane + (16 * st + 8 * (j / 4) + j % 4) * GBV);
+                else v = vraw[8 * st + j];
+                if constexpr (VT == 2) decode_values2<IPBV, NC>(v, lds, slot_v, n & 1u, w[j], w2[j]);
+                else v.decode(lds, slot_v, w[j]);
             }
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                tq_u4 v;
+                auto operand = [&](const auto &x) __attribute__((always_inline)) {
+                    tq_u4 v;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) v[d] = __builtin_amdgcn_perm(w[2 * d + 1][c / 2], w[2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                    for (int d = 0; d < 4; ++d) v[d] = __builtin_amdgcn_perm(x[2 * d + 1][c / 2], x[2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                    return v;
+                };
+                const tq_u4 v = operand(w);
 #pragma unroll
                 for (int i = 0; i < QT; ++i) acc[i][c] = mfma_f16(v, p[i][st], acc[i][c]);
+                if constexpr (VT == 2) {
+                    const tq_u4 v2 = operand(w2);
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        acc[i][c] = mfma_f16(v, p2[i][st], acc[i][c]);
+                        acc[i][c] = mfma_f16(v2, p[i][st], acc[i][c]);
+                    }
+                }
             }
         }
         if constexpr (!STAGE) issue_values(t_after);
@@ -813,72 +1072,68 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     }
 
     // ---- the waves' sums
-    const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P) << 23);
+    const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P - (VT == 2 ? LEVEL_SHIFT : 0)) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
         __syncthreads();
-        join_waves<D>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, FAST_WAVES, unit,
+        join_waves<DP>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, FAST_WAVES, unit,
                       m_ref[i] == FAST_START ? MANY_NONE : m_ref[i], l[i] * (1.0f / (float)(1 << FAST_P)), acc[i], tid);
     }
     __syncthreads();
     }
     const bool whole = a.splits == 1u, plain = (a.plain[0].n | a.plain[1].n) != 0u;
     if (plain && (whole || !packed)) {
-        if (a.dtype == TQ_BF16) plain_phase<D, QT, true>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
-        else plain_phase<D, QT, false>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
+        if constexpr (VT == 2) plain_phase<DP, QT, TQ_F32>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
+        else if (a.dtype == TQ_BF16) plain_phase<DP, QT, TQ_BF16>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
+        else if constexpr (KT == 2) plain_phase<DP, QT, TQ_F16>(a, lds, lds_m, lds_l, lds_kn[0], row, b, tile0, tiles, length, tid);
     }
     if (whole) {
-        finish_block<D, QT>(a, lds, plain, row, tile0, tiles, tid);
+        finish_block<DP, QT>(a, lds, plain, row, tile0, tiles, tid);
         return;
     }
     for (uint32_t i = 0; i < tiles; ++i) {
-        float *rec = packed ? a.rec + ((first_tile + i) * a.records + split) * record_floats(D) : a.plain_rec + (first_tile + i) * record_floats(D);
-        put_record<D>(rec, J::sums(lds, packed ? 0u : 1u, i), J::largest(lds, packed ? 0u : 1u, i), J::total(lds, packed ? 0u : 1u, i), tid);
+        float *rec = packed ? a.rec + ((first_tile + i) * a.records + split) * record_floats(DP) : a.plain_rec + (first_tile + i) * record_floats(DP);
+        put_record<DP>(rec, J::sums(lds, packed ? 0u : 1u, i), J::largest(lds, packed ? 0u : 1u, i), J::total(lds, packed ? 0u : 1u, i), tid);
     }
 }
 
 // What the packed tokens receive: weight = 2^(logit - largest) / sum with the statistics of the merge, from the two-term products.  Rows of the product are queries
 // here, columns tokens, so that a token's sum is made in its lane; rows in which a tile has no query are left out eight at a time.  Block = part of
 // a row's tokens, a wave takes 32 at a time and all tiles of queries in order (the first one's operands lie in LDS, a decode step has no more).
-template <int D, int IPBK>
+template <int DP, int IPBK>
 __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_kernel(TqManyArgs a, uint32_t blocks) {
-    constexpr int STEPS = D / 16, KB = D / 2 / IPBK, KW = KB / 4, GBK = D / IPBK, LUT_BYTES = 65536;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[LUT_BYTES + 2 * STEPS * 1024];
+    using Keys = KeyRun<DP, IPBK>;
+    constexpr int STEPS = DP / 16, KW = Keys::KW, LUT_BYTES = 65536;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LUT_BYTES + 2 * STEPS * 1024 + FAST_WAVES * Keys::BYTES];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const uint32_t row = blockIdx.x / blocks, b = row / a.heads;
     const size_t first_tile = (size_t)row * a.tiles;
     const uint32_t seen = min(a.tokens, many_length(a, b));
     {
         Lut2<IPBK> table;
-        table.load(a.table_k, a.bits_k, D, tid);
+        table.load(a.table_k, a.bits_k, DP, tid);
         table.store(lds, tid);
     }
-    tq_copy_to_lds(lds + LUT_BYTES, a.q_op + first_tile * q_operand_bytes(D), 2 * STEPS * 1024, tid, FAST_THREADS);
+    tq_copy_to_lds(lds + LUT_BYTES, a.q_op + first_tile * q_operand_bytes(DP), 2 * STEPS * 1024, tid, FAST_THREADS);
     const uint32_t slot = Lut2<IPBK>::lane_offset(lane);
     const float scale0 = a.q_scale[first_tile];
     __syncthreads();
     const size_t slot0 = (size_t)row * a.packed_row_stride;
+    const uint32_t GBK = Shape<DP>::EVEN ? DP / IPBK : (a.D + IPBK - 1u) / IPBK;
+    uint8_t *kstage = lds + LUT_BYTES + 2 * STEPS * 1024 + wave * Keys::BYTES;
     const uint32_t last = a.tokens - 32u, step = 32u * FAST_WAVES * blocks;
     for (uint32_t t_run = 32u * ((blockIdx.x - row * blocks) * FAST_WAVES + wave); t_run < seen; t_run += step) {
         const uint32_t t0 = min(t_run, last), t = t0 + n;
-        uint32_t kraw[KW];
-        const uint8_t *p = a.k_idx + (slot0 + t) * GBK + h * KB;
-        if constexpr (KB % 16 == 0) {
-#pragma unroll
-            for (int i = 0; i < KB / 16; ++i) {
-                const tq_u4 v = tq_gload16(p + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) kraw[4 * i + j] = v[j];
-            }
-        } else {
-            const tq_u2 v = tq_gload8(p);
-            kraw[0] = v[0]; kraw[1] = v[1];
-        }
+        Keys keys;
+        keys.issue(a.k_idx + (slot0 + t0) * GBK, GBK, lane);
         const float norm = (float)__builtin_bit_cast(_Float16, tq_gload2(a.k_norms + slot0 + t));
         const bool counts = t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
         float *dst = a.weights + (long long)row * a.w_stride + t;
         const float before = h == 0u && counts ? *dst : 0.f;
         float w = 0.f;
+        keys.stage(kstage, lane);
+        wave_sync();
+        keys.take(kstage, GBK, lane);
         auto add = [&](const tq_f16v &s, uint32_t tile, float kn, uint32_t queries) __attribute__((always_inline)) {
             const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * 64u + 4u * h;
 #pragma unroll
@@ -894,7 +1149,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 tq_u4 hi, lo;
-                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
+                decode_keys2<IPBK, KW>(keys.raw, st, lds, slot, hi, lo);
                 const tq_u4 qh = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + st * 1024 + lane * 16u), ql = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + (STEPS + st) * 1024 + lane * 16u);
                 s = mfma_f16(qh, hi, s);
                 s = mfma_f16(ql, hi, s);
@@ -904,12 +1159,12 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
         }
 #pragma unroll 1
         for (uint32_t tile = 1; tile < a.tiles; ++tile) {
-            const uint8_t *ops = a.q_op + (first_tile + tile) * q_operand_bytes(D) + lane * 16u;
+            const uint8_t *ops = a.q_op + (first_tile + tile) * q_operand_bytes(DP) + lane * 16u;
             tq_f16v s = tq_zero16();
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 tq_u4 hi, lo;
-                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
+                decode_keys2<IPBK, KW>(keys.raw, st, lds, slot, hi, lo);
                 const tq_u4 qh = tq_gload16(ops + st * 1024), ql = tq_gload16(ops + (STEPS + st) * 1024);
                 s = mfma_f16(qh, hi, s);
                 s = mfma_f16(ql, hi, s);
@@ -919,28 +1174,30 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
         }
         w = halves_add(w);
         if (h == 0u && counts) *dst = before + w;
+        wave_sync();
     }
 }
 
-template <int D, int IPBK>
+template <int DP, int IPBK>
 int launch_many_weights(dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks) {
-    hipLaunchKernelGGL((tq_many_weights_kernel<D, IPBK>), grid, dim3(FAST_THREADS), 0, s, a, blocks);
+    hipLaunchKernelGGL((tq_many_weights_kernel<DP, IPBK>), grid, dim3(FAST_THREADS), 0, s, a, blocks);
     return 0;
 }
 
 // ipb: codes per byte
-template <int D, int IPBK, int IPBV>
-int launch_many_fast(dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt) {
-    if (kt == 2) hipLaunchKernelGGL((tq_many_fast_kernel<D, IPBK, IPBV, 1, 2>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if (D == 256 || qt == 1) hipLaunchKernelGGL((tq_many_fast_kernel<D, IPBK, IPBV, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if constexpr (D != 256) hipLaunchKernelGGL((tq_many_fast_kernel<D, IPBK, IPBV, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+template <int DP, int IPBK, int IPBV>
+int launch_many_fast(dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt) {
+    if (vt == 2) hipLaunchKernelGGL((tq_many_fast_kernel<DP, IPBK, IPBV, 1, 2, 2>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if (kt == 2) hipLaunchKernelGGL((tq_many_fast_kernel<DP, IPBK, IPBV, 1, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if (DP == 256 || qt == 1) hipLaunchKernelGGL((tq_many_fast_kernel<DP, IPBK, IPBV, 1, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if constexpr (DP != 256) hipLaunchKernelGGL((tq_many_fast_kernel<DP, IPBK, IPBV, 2, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
     return 0;
 }
-template <int D, int IPBK>
-int launch_many_fast(int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt) {
-    if (ipbv == 4) return launch_many_fast<D, IPBK, 4>(grid, s, a, qt, kt);
-    if (ipbv == 2) return launch_many_fast<D, IPBK, 2>(grid, s, a, qt, kt);
-    return launch_many_fast<D, IPBK, 1>(grid, s, a, qt, kt);
+template <int DP, int IPBK>
+int launch_many_fast(int ipbv, dim3 grid, hipStream_t s, const TqManyArgs &a, int qt, int kt, int vt) {
+    if (ipbv == 4) return launch_many_fast<DP, IPBK, 4>(grid, s, a, qt, kt, vt);
+    if (ipbv == 2) return launch_many_fast<DP, IPBK, 2>(grid, s, a, qt, kt, vt);
+    return launch_many_fast<DP, IPBK, 1>(grid, s, a, qt, kt, vt);
 }
 
 }  // namespace
