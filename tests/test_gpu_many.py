@@ -135,6 +135,14 @@ BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
     (1, 2, 4, 700, 128, 21, 128, BF, 8, 1),
     (1, 2, 4, 700, 128, 21, 64, BF, 2, 6),
     (1, 1, 4, 0, 20, 4, 128, BF, 4, 2),           # nothing packed yet
+    (1, 2, 2, 300, 20, 9, 72, F16, 4, 4),
+    (2, 1, 4, 200, 8, 40, 96, F32, 8, 2),
+    (1, 2, 3, 150, 16, 33, 88, BF, 4, 4),
+    (1, 1, 4, 1000, 64, 64, 96, BF, 4, 2),
+    (1, 2, 5, 600, 40, 17, 64, F32, 2, 2),
+    (1, 2, 4, 32, 0, 70, 80, BF, 2, 2),
+    (1, 1, 2, 517, 200, 11, 128, F32, 8, 8),
+    (1, 1, 2, 517, 200, 11, 72, BF, 2, 2),        # 18 bytes a vector
 ])
 def test_tree_against_float64(pkg, B, H, G, n, w, T, D, dtype, kb, vb):
     cache = make_cache(pkg, B, H, n, w, D, dtype, kb, vb, seed=n + T)

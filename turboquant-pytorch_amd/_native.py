@@ -23,7 +23,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libtqamd.so")
 FAST_NAME = "tqamd_fastcall"        # extension module: the eager calls from tensors to the library in one step each
 FAST_SOURCE = "tq_fastcall.cpp"
-FAST_INTERFACE = 3                  # INTERFACE there: what init and the functions take and answer
+FAST_INTERFACE = 4                  # INTERFACE there: what init and the functions take and answer
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
@@ -330,7 +330,8 @@ def fast():
             raise TqError(f"{path} was built for version {module.abi_version} of the library, this is {L.tq_abi_version()}: {how}")
         if getattr(module, "interface", None) != FAST_INTERFACE:       # (modules of before had none)
             raise TqError(f"{path} was built from another state of {FAST_SOURCE}: {how}")
-        entries = ("tq_compress", "tq_decompress", "tq_compress_layer", "tq_restore_layer", "tq_decode_append", "tq_decode_attend_cached", "tq_qjl_compress", "tq_qjl_query_scores")
+        entries = ("tq_compress", "tq_decompress", "tq_compress_layer", "tq_restore_layer", "tq_decode_append", "tq_decode_attend_cached", "tq_qjl_compress", "tq_qjl_query_scores",
+                   "tq_attend_many_scratch", "tq_attend_many", "tq_evict")
         module.init(tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in entries), _workspace, _drop_workspace, _step_scratch, _arrived, _TABLE_TAG)
         _fast = module
     return _fast
@@ -749,6 +750,20 @@ def _packed_pairs(packed, B: int, H: int, tokens: int, D: int, bits):
     return out, strides[0]
 
 
+def attend_many_store(queries: torch.Tensor, stores, tokens: int, tables, bits, windows, win_first: int, n_win: int, drafts, lengths, mask, tree, weights, scale) -> Optional[torch.Tensor]:
+    """attend_many on whole buffers, in one step: packed stores (k_idx, k_nrm, v_idx, v_nrm) [B,H,capacity,..] of which the first `tokens` slots count, windows (keys, values)
+    of which n_win tokens from win_first on do.  None where something is laid out otherwise, or is missing: the caller then goes by attend_many, which checks everything."""
+    if not tokens or not queries.is_cuda or torch.compiler.is_compiling():
+        return None
+    k_win, v_win = windows if windows is not None else (None, None)
+    k_new, v_new = drafts if drafts is not None else (None, None)
+    scale = queries.shape[-1] ** -0.5 if scale is None else float(scale)
+    out = fast().attend_many(queries, *stores, tokens, *tables, *bits, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale)
+    if type(out) is int:
+        check(out, "tq_attend_many")
+    return out
+
+
 def _as_truth(mask: torch.Tensor, what: str) -> torch.Tensor:
     if mask.dtype != torch.bool:
         raise ValueError(f"{what} must be of truth values (torch.bool), got {mask.dtype}")
@@ -870,6 +885,12 @@ def evict(packed, tokens: int, bits, D: int, weights: torch.Tensor, keep: int, i
     if isinstance(keep, bool) or int(keep) != keep or not 0 <= keep <= tokens:
         raise ValueError(f"keep must be a whole number from 0 to {tokens}, got {keep!r}")
     keep = int(keep)
+    if into is None and weights_into is None:
+        got = fast().evict(k_idx, k_nrm, v_idx, v_nrm, tokens, *bits, D, weights, keep)
+        if got is not None:
+            if type(got) is int:
+                check(got, "tq_evict")
+            return (got[:2], got[2:4]), got[4], got[5]
     if weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H) or weights.shape[2] < tokens or weights.dtype != torch.float32:
         raise ValueError(f"weights must be float32 [{B}, {H}, {tokens} or more]; got {tuple(weights.shape)} {weights.dtype}")
     for t in (k_nrm, v_idx, v_nrm, weights):

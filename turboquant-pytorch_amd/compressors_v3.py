@@ -364,6 +364,16 @@ class TurboQuantV3:
         weights [B,H,S] (float32): what every key receives, summed over the query heads and tokens that read it, is added in place.
         scale: D ** -0.5 by default.  Not differentiable."""
         kc, vc, device = self.key_compressor, self.val_compressor, query_states.device
+        ck, cv, shape = compressed_k["compressed"], compressed_v["compressed"], compressed_k["shape"]
+        if (ck is not None and cv is not None and device.type == "cuda" and compressed_v["shape"] == shape and compressed_v["split_at"] == compressed_k["split_at"]
+                and shape[3] == kc.head_dim == vc.head_dim and (weights is None or weights.shape[-1] == shape[2])):
+            tokens, windows = compressed_k["split_at"], (compressed_k["fp16"], compressed_v["fp16"])
+            stores = (ck["idx_bytes"], ck["vec_norms"], cv["idx_bytes"], cv["vec_norms"])
+            if stores[0].shape[2] == tokens and windows[0].shape[2] == windows[1].shape[2] == shape[2] - tokens:
+                out = _native.attend_many_store(query_states, stores, tokens, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), windows, 0, shape[2] - tokens,
+                                                None, lengths, mask, None, weights, scale)
+                if out is not None:
+                    return out
         packed, tokens, window = self._packed_pairs(compressed_k, compressed_v)
         return _native.attend_many(query_states, packed, tokens, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), window, None, lengths, mask, None,
                                    weights, scale)
@@ -380,7 +390,7 @@ class TurboQuantV3:
             raise ValueError(f"weights must be [{B}, {H}, {S}], got {tuple(weights.shape)}")
         if packed is None:
             return dict(compressed_k), dict(compressed_v), weights.clone(), torch.empty((B, H, 0), dtype=torch.int64, device=weights.device)
-        (k, v), left, kept = _native.evict(packed, tokens, (kc.bits, vc.bits), D, weights, min(keep, tokens) if keep >= 0 else keep)
+        (k, v), left, kept = _native.evict(packed, tokens, (kc.bits, vc.bits), D, weights, min(keep, tokens))
         keep = kept.shape[2]
         out = []
         for c, (idx, nrm) in ((compressed_k, k), (compressed_v, v)):

@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 3;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 4;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -36,6 +36,9 @@ struct Entries {
     decltype(&tq_decode_attend_cached) decode_attend;
     decltype(&tq_qjl_compress) qjl_compress;
     decltype(&tq_qjl_query_scores) qjl_query_scores;
+    decltype(&tq_attend_many_scratch) attend_many_scratch;
+    decltype(&tq_attend_many) attend_many;
+    decltype(&tq_evict) evict;
 } lib{};
 
 struct Raised {};        // a Python exception is set
@@ -440,6 +443,126 @@ PyObject *qjl_scores(PyObject *const *a) {
     return THPVariable_Wrap(out);
 }
 
+// The first `tokens` slots of packed stores [B,H,capacity,..], dense, as both calls below take them
+inline bool packed_store(const at::Tensor &ki, const at::Tensor &kn, const at::Tensor &vi, const at::Tensor &vn, long long tokens, long long D, long long bk, long long bv) {
+    if (ki.dim() != 4 || bk < 1 || bk > 8 || bv < 1 || bv > 8) return false;
+    const long long B = ki.size(0), H = ki.size(1), cap = ki.size(2);
+    for (const at::Tensor *t : {&ki, &kn, &vi, &vn})
+        if (!t->is_contiguous() || t->device() != ki.device()) return false;
+    return tokens >= 1 && tokens <= cap && shape_is(ki, {B, H, cap, packed_width(D, bk)}) && shape_is(vi, {B, H, cap, packed_width(D, bv)}) && shape_is(kn, {B, H, cap}) &&
+           shape_is(vn, {B, H, cap}) && ki.scalar_type() == at::kByte && vi.scalar_type() == at::kByte && kn.scalar_type() == at::kHalf && vn.scalar_type() == at::kHalf;
+}
+
+// tokens [first, first + n) of uncompressed keys and values [B,H,..,D] of the queries' type
+inline bool plain_tokens(PyObject *k_object, PyObject *v_object, long long first, long long n, const at::Tensor &q, long long H, tq_plain_tokens &out) {
+    out = tq_plain_tokens{};
+    if (n == 0) return true;
+    const at::Tensor *const k = tensor(k_object), *const v = tensor(v_object);
+    if (!k || !v || n < 0 || n > 65536 || first < 0) return false;
+    for (const at::Tensor *t : {k, v})
+        if (t->dim() != 4 || t->scalar_type() != q.scalar_type() || t->device() != q.device() || t->size(0) != q.size(0) || t->size(1) != H || t->size(2) < first + n ||
+            t->size(3) != q.size(3) || t->stride(3) != 1)
+            return false;
+    const long long elem = (long long)q.element_size();
+    out = {address(*k) + first * k->stride(2) * elem, address(*v) + first * v->stride(2) * elem, k->stride(0), k->stride(1), k->stride(2), v->stride(0), v->stride(1), v->stride(2), n};
+    return true;
+}
+
+// attend_many(queries, k_idx, k_norms, v_idx, v_norms, tokens, table_k, table_v, bits_k, bits_v, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale)
+// -> output: _native.attend_many where everything lies as the library takes it (packed stores dense, of which the first `tokens` slots count, window buffers of which
+// n_win tokens do; None where there is none).  Scratch of the stream as _native keeps it.
+PyObject *attend_many(PyObject *const *a) {
+    TENSOR(q, a[0]); TENSOR(ki, a[1]); TENSOR(kn, a[2]); TENSOR(vi, a[3]); TENSOR(vn, a[4]);
+    NEED(q.dim() == 4 && ki.dim() == 4 && q.stride(3) == 1 && q.device() == ki.device());
+    const int dt = dtype_code(q);
+    NEED(dt >= 0);
+    const long long tokens = integer(a[5]), bk = integer(a[8]), bv = integer(a[9]), B = q.size(0), Hq = q.size(1), T = q.size(2), D = q.size(3), H = ki.size(1), cap = ki.size(2);
+    NEED(ki.size(0) == B && B > 0 && H > 0 && T > 0 && Hq > 0 && Hq % H == 0 && packed_store(ki, kn, vi, vn, tokens, D, bk, bv));
+    TABLE(tk, a[6], q, D, bk); TABLE(tv, a[7], q, D, bv);
+    tq_attend_request r{};
+    const long long n_win = integer(a[13]), n_new = a[14] == Py_None ? 0 : T, total = tokens + n_win;
+    NEED(plain_tokens(a[10], a[11], integer(a[12]), n_win, q, H, r.window));
+    if (n_new) {
+        TENSOR(fresh, a[14]);
+        NEED(fresh.dim() == 4 && fresh.size(2) == T);
+    }
+    NEED(plain_tokens(a[14], a[15], 0, n_new, q, H, r.drafts));
+    if (a[16] != Py_None) {
+        TENSOR(lengths, a[16]);
+        NEED(lengths.scalar_type() == at::kInt && shape_is(lengths, {B}) && lengths.is_contiguous() && lengths.device() == q.device());
+        r.lengths = (const int32_t *)address(lengths);
+    }
+    if (a[17] != Py_None) {
+        TENSOR(mask, a[17]);
+        NEED(mask.scalar_type() == at::kBool && shape_is(mask, {B, total}) && mask.is_contiguous() && mask.device() == q.device());
+        r.mask = address(mask);
+        r.mask_stride = total;
+    }
+    if (a[18] != Py_None) {
+        TENSOR(tree, a[18]);
+        NEED(n_new && tree.scalar_type() == at::kBool && tree.is_contiguous() && tree.device() == q.device() && (shape_is(tree, {T, T}) || shape_is(tree, {B, T, T})));
+        r.tree = address(tree);
+        r.tree_batch = tree.dim() == 3 ? T * T : 0;
+    }
+    if (a[19] != Py_None) {
+        TENSOR(w, a[19]);
+        NEED(w.scalar_type() == at::kFloat && w.device() == q.device() && w.dim() == 3 && w.size(0) == B && w.size(1) == H && w.size(2) >= total && w.is_contiguous());
+        r.weights = (float *)address(w);
+        r.weights_stride = w.size(2);
+    }
+    const double scale = PyFloat_AsDouble(a[20]);
+    if (scale == -1.0 && PyErr_Occurred()) throw Raised{};
+    const Stream s(q);
+    NEED(s.ok);
+    NEED(!s.capturing());
+    r.queries = address(q);
+    r.k_idx = address(ki); r.k_norms = (const uint16_t *)address(kn); r.v_idx = address(vi); r.v_norms = (const uint16_t *)address(vn);
+    r.table_k = address(tk); r.table_v = address(tv);
+    r.q_batch = q.stride(0); r.q_head = q.stride(1); r.q_token = q.stride(2);
+    r.batch = B; r.heads = H; r.group = Hq / H; r.n_queries = T; r.tokens = tokens; r.packed_row_stride = cap;
+    r.scale = (float)scale;
+    r.head_dim = (int)D; r.dtype = dt; r.bits_k = (int)bk; r.bits_v = (int)bv;
+    const long long floats = lib.attend_many_scratch(&r);
+    NEED(floats >= 0);
+    PyObject *key = Py_BuildValue("(iK)", s.dev, s.handle);
+    if (!key) throw Raised{};
+    PyObject *scratch = PyDict_GetItem(g_scratch, key);      // borrowed; this frame keeps it through the call
+    Py_XINCREF(scratch);
+    Py_DECREF(key);
+    struct Held { PyObject *a; ~Held() { Py_XDECREF(a); } } held{scratch};
+    NEED(scratch);
+    TENSOR(buf, scratch);
+    NEED(buf.numel() >= floats);
+    at::Tensor out = empty({B, Hq, T, D}, q.scalar_type(), q);
+    r.out = address(out);
+    const int rc = launch(lib.attend_many, (const tq_attend_request *)&r, (float *)address(buf), (long long)buf.numel(), s.raw());
+    if (rc > 0) return PyLong_FromLong(rc);
+    NEED(rc == 0);           // (an argument the library refuses: nothing was launched)
+    return THPVariable_Wrap(out);
+}
+
+// evict(k_idx, k_norms, v_idx, v_norms, tokens, bits_k, bits_v, dim, weights, keep) -> (k_idx, k_norms, v_idx, v_norms, weights, kept): _native.evict on dense stores into new ones
+PyObject *evict(PyObject *const *a) {
+    TENSOR(ki, a[0]); TENSOR(kn, a[1]); TENSOR(vi, a[2]); TENSOR(vn, a[3]); TENSOR(w, a[8]);
+    const long long tokens = integer(a[4]), bk = integer(a[5]), bv = integer(a[6]), D = integer(a[7]);
+    NEED(PyLong_CheckExact(a[9]));
+    const long long keep = integer(a[9]);
+    NEED(packed_store(ki, kn, vi, vn, tokens, D, bk, bv) && keep >= 0 && keep <= tokens);
+    const long long B = ki.size(0), H = ki.size(1), cap = ki.size(2);
+    NEED(B * H > 0 && w.dim() == 3 && w.size(0) == B && w.size(1) == H && w.size(2) >= tokens && w.scalar_type() == at::kFloat && w.is_contiguous() && w.device() == ki.device());
+    const long long rest = w.size(2) - tokens;
+    const Stream s(ki);
+    NEED(s.ok);
+    at::Tensor ko = empty({B, H, keep, packed_width(D, bk)}, at::kByte, ki), kno = empty({B, H, keep}, at::kHalf, ki), vo = empty({B, H, keep, packed_width(D, bv)}, at::kByte, ki);
+    at::Tensor vno = empty({B, H, keep}, at::kHalf, ki), wo = empty({B, H, keep + rest}, at::kFloat, ki), kept = empty({B, H, keep}, at::kLong, ki);
+    const tq_packed_store from{address(ki), (uint16_t *)address(kn), address(vi), (uint16_t *)address(vn), cap}, to{address(ko), (uint16_t *)address(kno), address(vo), (uint16_t *)address(vno), keep};
+    const int rc = launch(lib.evict, (const tq_packed_store *)&from, (const tq_packed_store *)&to, (const float *)address(w), (long long)w.size(2), (float *)address(wo), keep + rest, rest, B * H, tokens, keep, (int)D, (int)bk, (int)bv,
+                          (long long *)address(kept), s.raw());
+    if (rc > 0) return PyLong_FromLong(rc);
+    NEED(rc == 0);
+    return wrapped({ko, kno, vo, vno, wo, kept});
+}
+
 // No exception leaves a function, and none records gradients.  Errors of torch's (no memory, a device error) become the Python exceptions
 // that its own functions raise.
 template <PyObject *(*F)(PyObject *const *), int N>
@@ -485,7 +608,7 @@ PyObject *init(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
-    TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8),
+    TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 21), TQ_ENTRY(evict, 10),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -474,6 +474,11 @@ class V3Cache:
         """tq_attend_many over everything the layer holds."""
         n = st.n_compressed
         kc, vc, device = st.comp.key_compressor, st.comp.val_compressor, st.k_win.device
+        if n:
+            out = _native.attend_many_store(query_states, (st.k_idx, st.k_nrm, st.v_idx, st.v_nrm), n, (kc.table(device), vc.table(device)), (kc.bits, vc.bits),
+                                            (st.k_win, st.v_win), st.w0, st.n_recent, drafts, None, None, tree_mask, None if weights is None else st.weights, scale)
+            if out is not None:
+                return out
         packed = ((st.k_idx[:, :, :n], st.k_nrm[:, :, :n]), (st.v_idx[:, :, :n], st.v_nrm[:, :, :n])) if n else None
         return _native.attend_many(query_states, packed, n, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), st.window(), drafts, None, None,
                                    tree_mask, weights, scale)
