@@ -553,11 +553,11 @@ struct PlainTile<DP, TQ_F32> {
     }
 };
 
-// The sums of waves [w0, w0 + count) of a tile of queries into out[32][D + 4] and their largest logits and sums into out_m, out_l[32], all in LDS; every wave of the block
+// The sums of waves [w0, w0 + COUNT) of a tile of queries into out[32][D + 4] and their largest logits and sums into out_m, out_l[32], all in LDS; every wave of the block
 // calls it, those with other w0 for another tile.  unit: what this wave's value sums are multiplied by; m_ref: MANY_NONE where it has seen no token of a
 // query; l: this lane's half.  area: [wave][32][64 + 4], two coordinates blocks of 32 at a time.
-template <int DP>
-__device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], float (*lds_l)[32], float *out, float *out_m, float *out_l, uint32_t w0, uint32_t count, float unit, float m_ref,
+template <int DP, int COUNT>
+__device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], float (*lds_l)[32], float *out, float *out_m, float *out_l, uint32_t w0, float unit, float m_ref,
                                            float l, const tq_f16v (&acc)[Shape<DP>::NC], uint32_t tid) {
     constexpr int NC = Shape<DP>::NC;
     constexpr uint32_t MROW = 68u, ROW = DP + 4;
@@ -569,14 +569,16 @@ __device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], floa
     }
     __syncthreads();
     float m = MANY_NONE, sum = 0.f;
-    for (uint32_t w = w0; w < w0 + count; ++w) m = fmaxf(m, lds_m[w][n]);
-    for (uint32_t w = w0; w < w0 + count; ++w) sum = fmaf(lds_l[w][n], __builtin_amdgcn_exp2f(lds_m[w][n] - m), sum);
+#pragma unroll
+    for (uint32_t w = 0; w < COUNT; ++w) m = fmaxf(m, lds_m[w0 + w][n]);
+#pragma unroll
+    for (uint32_t w = 0; w < COUNT; ++w) sum = fmaf(lds_l[w0 + w][n], __builtin_amdgcn_exp2f(lds_m[w0 + w][n] - m), sum);
     if (wave == w0 && h == 0u) {
         out_m[n] = m;
         out_l[n] = sum;
     }
     const float f = unit * __builtin_amdgcn_exp2f(m_ref - m);
-    const uint32_t mine = tid - w0 * 64u, threads = count * 64u;       // (a wave sums for its own tile)
+    const uint32_t mine = tid - w0 * 64u;       // (a wave sums for its own tile)
 #pragma unroll
     for (int c0 = 0; c0 < NC; c0 += 2) {
         if (c0) __syncthreads();
@@ -587,13 +589,15 @@ __device__ __forceinline__ void join_waves(float *area, float (*lds_m)[32], floa
                 *reinterpret_cast<tq_f4 *>(area + (wave * 32u + n) * MROW + 32 * c + 8 * k + 4 * h) =
                     tq_f4{acc[c0 + c][4 * k] * f, acc[c0 + c][4 * k + 1] * f, acc[c0 + c][4 * k + 2] * f, acc[c0 + c][4 * k + 3] * f};
         __syncthreads();
-        for (uint32_t pair = mine; pair < 1024u; pair += threads) {        // coordinates NC r + c0, + 1 of query col
-            const uint32_t col = pair / 32u, r = pair % 32u;
+#pragma unroll
+        for (uint32_t pair0 = 0; pair0 < 1024u; pair0 += COUNT * 64u) {        // coordinates NC r + c0, + 1 of query col
+            const uint32_t pair = pair0 + mine, col = pair / 32u, r = pair % 32u;
             if (Shape<DP>::LANES < 32 && r >= (uint32_t)Shape<DP>::LANES) continue;
             float x = 0.f, y = 0.f;
-            for (uint32_t w = w0; w < w0 + count; ++w) {
-                x += area[(w * 32u + col) * MROW + r];
-                y += area[(w * 32u + col) * MROW + 32u + r];
+#pragma unroll
+            for (uint32_t w = 0; w < COUNT; ++w) {
+                x += area[((w0 + w) * 32u + col) * MROW + r];
+                y += area[((w0 + w) * 32u + col) * MROW + 32u + r];
             }
             out[col * ROW + NC * r + c0] = x;
             out[col * ROW + NC * r + c0 + 1] = y;
@@ -672,7 +676,9 @@ __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, f
         }
         __syncthreads();             // (what the area held)
         if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
-        join_waves<DP>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, count, 1.f, m, l, acc, tid);
+        float *const area = reinterpret_cast<float *>(lds);
+        if (share) join_waves<DP, FAST_WAVES / 2>(area, lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, 1.f, m, l, acc, tid);
+        else join_waves<DP, FAST_WAVES>(area, lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), 0u, 1.f, m, l, acc, tid);
         __syncthreads();
         float any = 0.f;
 #pragma unroll
@@ -1076,7 +1082,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
         __syncthreads();
-        join_waves<DP>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, FAST_WAVES, unit,
+        join_waves<DP, FAST_WAVES>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, unit,
                       m_ref[i] == FAST_START ? MANY_NONE : m_ref[i], l[i] * (1.0f / (float)(1 << FAST_P)), acc[i], tid);
     }
     __syncthreads();

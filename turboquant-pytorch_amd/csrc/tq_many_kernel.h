@@ -417,14 +417,16 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
 // Block (row, tile, C of its 32 queries), DP / 32 waves: the records' sums with their factors, the packed ones turned back by Pi_v (two fp16 terms each of Pi_v^T,
 // from the value codec's table, and of the sums: 22 bits), the uncompressed ones added, everything divided by the sum of weights.
 // A query that sees nothing gets zeros.  C = 8 where tiles are few: the records are then read by four times as many blocks.
+// A launch of few blocks lasts as long as its chain of loads: what does not depend on anything (references, sums, the first records, Pi_v) is asked for at once.
 constexpr uint32_t MERGE_RECORDS = 260;
 template <int DP, int C>
 __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
-    constexpr uint32_t NT = 2 * DP, ROW = DP + 4, PARTS = NT / C, UNITS = C * DP / 4;      // (NT is a multiple of 64)
+    constexpr uint32_t NT = 2 * DP, ROW = DP + 4, PARTS = NT / C, UNITS = C * DP / 4, STEPS = DP / 16, CH = STEPS <= 8 ? STEPS : 8;      // (NT is a multiple of 64)
+    constexpr uint32_t UPT = (UNITS + NT - 1) / NT;                         // units of four coordinates a thread
     __shared__ __attribute__((aligned(16))) float lds_o[2][C * ROW];        // packed, plain
-    __shared__ float lds_f[MERGE_RECORDS][C], lds_red[2][PARTS][C], lds_top[C];
+    __shared__ float lds_f[MERGE_RECORDS][C], lds_red[2][PARTS][C], lds_inv[C];
     const uint32_t group = blockIdx.x % (32u / C), at = blockIdx.x / (32u / C);
-    const uint32_t row = at / a.tiles, tile = at - row * a.tiles, b = row / a.heads, col0 = group * C;
+    const uint32_t row = at / a.tiles, tile = at - row * a.tiles, col0 = group * C;
     if (tile * 32u + col0 >= a.M && !a.stat) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n32 = lane & 31u, h = lane >> 5;
     const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + (size_t)at * a.records * record_floats(DP);
@@ -432,61 +434,102 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     const uint32_t all = a.records + a.plain_records;
     auto record = [&](uint32_t i) { return i < a.records ? rec + (size_t)i * record_floats(DP) : plain + (size_t)(i - a.records) * record_floats(DP); };
     const uint32_t c = tid % C, part = tid / C;
-    float top = MANY_NONE;
-    for (uint32_t i = part; i < all; i += PARTS) {
-        const float v = record(i)[col0 + c];
-        lds_f[i][c] = v;
-        top = fmaxf(top, v);
+    // ---- references and sums, two records a thread at first
+    float ref[2], tot[2];
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t i = part + k * PARTS;
+        const TQ_GLOBAL float *p = record(min(i, all - 1u)) + col0 + c;
+        ref[k] = p[0];
+        tot[k] = p[32];
     }
+    // ---- a unit's first eight packed records and its first plain one
+    tq_f4 v[UPT == 1 ? 8 : 1], w[1];
+    const uint32_t q0 = tid / (DP / 4u), e0 = (tid - q0 * (DP / 4u)) * 4u;
+    if constexpr (UPT == 1) {
+        const uint32_t off = 64u + (col0 + q0) * DP + e0;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(record(min(k, all - 1u)) + off);
+        w[0] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(record(all - 1u) + off);
+    }
+    // ---- Pi_v (128 wide the table's operands have an order of their own, see tq_table.h)
+    const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(a.D) + ((size_t)wave * STEPS * 64u + lane) * 16u;
+    tq_u4 ph[CH], pl[CH];
+    auto load_pi = [&](uint32_t s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t s = 0; s < CH; ++s)
+            if (s0 + s < STEPS) { ph[s] = tq_gload16(pi + (size_t)(s0 + s) * 1024u); pl[s] = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(a.D) + (size_t)(s0 + s) * 1024u); }
+    };
+    load_pi(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- factors
+    float top = MANY_NONE;
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k)
+        if (part + k * PARTS < all) top = fmaxf(top, ref[k]);
+    for (uint32_t i = part + 2u * PARTS; i < all; i += PARTS) top = fmaxf(top, record(i)[col0 + c]);
     lds_red[0][part][c] = top;
     __syncthreads();
+#pragma unroll 8
     for (uint32_t k = 0; k < PARTS; ++k) top = fmaxf(top, lds_red[0][k][c]);
     float sum = 0.f;
-    for (uint32_t i = part; i < all; i += PARTS) {
-        const float v = lds_f[i][c], f = v == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(v - top);
+    auto factor = [&](uint32_t i, float r, float t) {          // (a record of no token: zero, its sums need not have been written)
+        const float f = r == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(r - top);
         lds_f[i][c] = f;
-        sum = fmaf(record(i)[32u + col0 + c], f, sum);
-    }
+        sum = f == 0.f ? sum : fmaf(t, f, sum);
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k)
+        if (part + k * PARTS < all) factor(part + k * PARTS, ref[k], tot[k]);
+    for (uint32_t i = part + 2u * PARTS; i < all; i += PARTS) factor(i, record(i)[col0 + c], record(i)[32u + col0 + c]);
     lds_red[1][part][c] = sum;
     __syncthreads();
-    // ---- sums
-#pragma unroll
-    for (uint32_t which = 0; which < 2; ++which) {
-        const TQ_GLOBAL float *src = (which ? plain : rec) + 64u + col0 * DP;
-        const uint32_t count = which ? a.plain_records : a.records, first = which ? a.records : 0u;
-#pragma unroll
-        for (uint32_t u = tid; u < UNITS; u += NT) {
-            const uint32_t q = u / (DP / 4u), d = (u - q * (DP / 4u)) * 4u;
-            tq_f4 o = {0.f, 0.f, 0.f, 0.f};
-            const TQ_GLOBAL float *p = src + q * DP + d;
-            for (uint32_t r0 = 0; r0 < count; r0 += 8u) {
-                tq_f4 v[8];
-                float f[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8u; ++k) {
-                    const uint32_t r = min(r0 + k, count - 1u);
-                    v[k] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(p + (size_t)r * record_floats(DP));
-                    f[k] = r0 + k < count ? lds_f[first + r][q] : 0.f;
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < 8u; ++k)
-                    if (f[k] != 0.f)           // (a record of no token: its sums need not have been written)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = fmaf(v[k][e], f[k], o[e]);
-            }
-            *reinterpret_cast<tq_f4 *>(&lds_o[which][q * ROW + d]) = o;
-        }
-    }
     if (tid < (uint32_t)C) {
         float l = 0.f;
+#pragma unroll 8
         for (uint32_t k = 0; k < PARTS; ++k) l += lds_red[1][k][tid];
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        lds_top[tid] = inv;
+        lds_inv[tid] = inv;
         if (a.stat) {          // (a query that is none, or sees nothing: weights of zero)
             const bool some = tile * 32u + col0 + tid < a.M && inv != 0.f;
             a.stat[(size_t)at * 64u + col0 + tid] = some ? top : -MANY_NONE;
             a.stat[(size_t)at * 64u + 32u + col0 + tid] = some ? inv : 0.f;
         }
+    }
+    // ---- sums
+    auto add = [&](tq_f4 &o, tq_f4 x, float f) __attribute__((always_inline)) {
+        if (f != 0.f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+    };
+#pragma unroll
+    for (uint32_t u0 = 0; u0 < UPT; ++u0) {
+        const uint32_t u = tid + u0 * NT;
+        if (UNITS % NT && u >= UNITS) break;
+        const uint32_t q = u / (DP / 4u), d = (u - q * (DP / 4u)) * 4u;
+        tq_f4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        const uint32_t off = 64u + (col0 + q) * DP + d;
+        uint32_t r0 = 0;
+        if constexpr (UPT == 1) {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k < a.records) add(o[0], v[k], lds_f[k][q]);
+            r0 = 8u;
+        }
+        for (; r0 < a.records; r0 += 8u) {
+            tq_f4 x[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(rec + (size_t)min(r0 + k, a.records - 1u) * record_floats(DP) + off);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (r0 + k < a.records) add(o[0], x[k], lds_f[r0 + k][q]);
+        }
+        if (UPT == 1 && a.plain_records == 1u) add(o[1], w[0], lds_f[all - 1u][q]);
+        else
+            for (uint32_t r = 0; r < a.plain_records; ++r)
+                add(o[1], *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(plain + (size_t)r * record_floats(DP) + off), lds_f[a.records + r][q]);
+        *reinterpret_cast<tq_f4 *>(&lds_o[0][q * ROW + d]) = o[0];
+        *reinterpret_cast<tq_f4 *>(&lds_o[1][q * ROW + d]) = o[1];
     }
     __syncthreads();
     // ---- back out of the codec's space; columns past C repeat the others
@@ -494,33 +537,37 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     float largest = 0.f;
 #pragma unroll
     for (uint32_t d = 0; d < DP / 2u; d += 4u) {
-        const tq_f4 v = *reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + h * (DP / 2u) + d]);
+        const tq_f4 x = *reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + h * (DP / 2u) + d]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
+        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(x[e]) < __builtin_inff() ? fabsf(x[e]) : 0.f);
     }
     largest = halves_max(largest);
     const int up = largest > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(largest) >> 23) - 127))) : 0;
     const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-    // (128 wide the table's operands have an order of their own, see tq_table.h)
-    const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(a.D) + ((size_t)wave * (DP / 16u) * 64u + lane) * 16u;
     const bool tuned = a.D == TQ_HEAD_DIM;
     tq_f16v acc = tq_zero16();
-#pragma unroll 4
-    for (uint32_t s = 0; s < DP / 16u; ++s) {
-        const uint32_t j = tuned ? 64u * h + 8u * s : 16u * s + 8u * h;
-        uint32_t t[8];
+#pragma unroll 1
+    for (uint32_t s0 = 0;;) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = fp16_terms(j + i < a.D ? lds_o[0][q * ROW + j + i] * f : 0.f);
-        tq_u4 oh, ol;
-        fp16_operands(t, oh, ol);
-        const tq_u4 ph = tq_gload16(pi + (size_t)s * 1024u), pl = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(a.D) + (size_t)s * 1024u);
-        acc = mfma_f16(ph, oh, acc);
-        acc = mfma_f16(ph, ol, acc);
-        acc = mfma_f16(pl, oh, acc);
+        for (uint32_t s = 0; s < CH; ++s) {
+            if (s0 + s >= STEPS) break;
+            const uint32_t j = tuned ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;
+            uint32_t t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = fp16_terms(j + i < a.D ? lds_o[0][q * ROW + j + i] * f : 0.f);
+            tq_u4 oh, ol;
+            fp16_operands(t, oh, ol);
+            acc = mfma_f16(ph[s], oh, acc);
+            acc = mfma_f16(ph[s], ol, acc);
+            acc = mfma_f16(pl[s], oh, acc);
+        }
+        s0 += CH;
+        if (s0 >= STEPS) break;
+        load_pi(s0);
     }
     const uint32_t m = tile * 32u + col0 + q;
     if (m >= a.M || n32 >= (uint32_t)C) return;
-    const float inv = lds_top[q], back = __uint_as_float((uint32_t)(127 - up) << 23);
+    const float inv = lds_inv[q], back = __uint_as_float((uint32_t)(127 - up) << 23);
     const uint32_t d0 = tuned ? 64u * h + 16u * wave : 32u * wave + 16u * h;
     float o[16];
 #pragma unroll
