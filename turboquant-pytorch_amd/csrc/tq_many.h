@@ -82,6 +82,17 @@ __device__ __forceinline__ uint32_t fp16_terms(float x) {
     const _Float16 lo = (_Float16)(r == r ? r : 0.f);
     return (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
 }
+// Eight floats, times f -> operands of both terms, in half the instructions (an infinity's rest is NaN: where everything turns into NaN anyway)
+__device__ __forceinline__ void fp16_split8(tq_f4 x, tq_f4 y, float f, tq_u4 &hi, tq_u4 &lo) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const float a = (d < 2 ? x[2 * d] : y[2 * d - 4]) * f, b = (d < 2 ? x[2 * d + 1] : y[2 * d - 3]) * f;
+        const tq_half2 h = {(_Float16)a, (_Float16)b};
+        const tq_half2 l = {(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])};
+        hi[d] = __builtin_bit_cast(uint32_t, h);
+        lo[d] = __builtin_bit_cast(uint32_t, l);
+    }
+}
 // eight of them -> two operands
 __device__ __forceinline__ void fp16_operands(const uint32_t (&t)[8], tq_u4 &hi, tq_u4 &lo) {
 #pragma unroll
@@ -204,6 +215,65 @@ __device__ __forceinline__ uint32_t many_length(const TqManyArgs &a, uint32_t b)
     if (!a.lengths) return all;
     const int32_t l = a.lengths[b];
     return l < 0 ? 0u : min((uint32_t)l, all);
+}
+
+// Base-2 logits of 32 uncompressed tokens x 32 queries, MANY_NONE where a token is not seen
+template <int DT>
+__device__ __forceinline__ void plain_logits(const TqManyArgs &a, const TqManyPlain &seg, uint32_t which, uint32_t row, uint32_t b, uint32_t kv, uint32_t t0, uint32_t m,
+                                             uint32_t lane, uint32_t length, uint32_t steps, float (&x)[16]) {
+    constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
+    constexpr int NT = plain_terms<DT>();
+    const uint32_t n = lane & 31u, h = lane >> 5;
+    const uint8_t *k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * ES;
+    const uint8_t *q = many_query(a, row, min(m, a.M - 1u), ES);
+    tq_f16v acc = tq_zero16();
+    for (uint32_t s = 0; s < steps; ++s) {
+        tq_u4 kt[3], qt[3];
+        load_plain8<DT>(k, 16u * s + 8u * h, a.D, a.aligned, kt);
+        load_plain8<DT>(q, 16u * s + 8u * h, a.D, a.aligned, qt);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (i + j < 3) acc = mfma_bf16(kt[i], qt[j], acc);
+    }
+    const uint32_t i = ManyQuery(a, min(m, a.M - 1u)).t;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const uint32_t t = t0 + acc_row(r, h);
+        const bool seen = t < seg.n && plain_seen(a, which, b, i, t, length);
+        x[r] = seen ? acc[r] * (a.scale * LOG2E) : MANY_NONE;
+    }
+}
+
+// What the window's tokens receive: wave = 32 tokens, all query tiles of the row in order.
+template <int DT>
+__device__ __forceinline__ void plain_weights(const TqManyArgs &a, uint32_t item, uint32_t steps, uint32_t lane) {
+    const TqManyPlain &seg = a.plain[0];
+    const uint32_t groups = (seg.n + 31u) / 32u;
+    const uint32_t row = item / groups, t0 = 32u * (item - row * groups), b = row / a.heads, kv = row - b * a.heads;
+    const uint32_t n = lane & 31u, h = lane >> 5, length = many_length(a, b);
+    float w[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = 0.f;
+    for (uint32_t tile = 0; tile < a.tiles; ++tile) {
+        float x[16];
+        plain_logits<DT>(a, seg, 0u, row, b, kv, t0, tile * 32u + n, lane, length, steps, x);
+        const float *stat = a.stat + ((size_t)row * a.tiles + tile) * 64u;
+        const float m = stat[n], inv = stat[32u + n];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(x[r] - m), inv, w[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) w[r] += __shfl_xor(w[r], i);
+    float own = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) own = n == (uint32_t)r ? w[r] : own;
+    const uint32_t t = t0 + acc_row((int)(n & 15u), h);
+    if (n < 16u && t < seg.n && a.tokens + t < length) a.weights[(long long)row * a.w_stride + a.tokens + t] += own;
 }
 
 }  // namespace

@@ -116,7 +116,7 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
         else hipLaunchKernelGGL((tq_many_plain_kernel<DP, TQ_BF16>), g, t, 0, s, a);
     }
     if (a.records || a.plain_records) {
-        if (at < 512u) hipLaunchKernelGGL((tq_many_merge_kernel<DP, 8>), dim3(at * 4u), dim3(2 * DP), 0, s, a);
+        if (at < 128u) hipLaunchKernelGGL((tq_many_merge_kernel<DP, 8>), dim3(at * 4u), dim3(2 * DP), 0, s, a);
         else hipLaunchKernelGGL((tq_many_merge_kernel<DP, 32>), dim3(at), dim3(2 * DP), 0, s, a);
     }
     if (!a.weights) return;
@@ -126,13 +126,16 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
         const uint32_t most = (a.tokens + 32u * 8u - 1u) / (32u * 8u);
         uint32_t blocks = ((uint32_t)cus + a.rows - 1u) / a.rows;
         if (blocks > most) blocks = most;
-        const dim3 g(a.rows * blocks);
+        const uint32_t window = a.rows * ((a.plain[0].n + 31u) / 32u);
+        const dim3 g(a.rows * blocks + (window + 7u) / 8u);
         const int ik = 8 / (int)a.bits_k;
         if constexpr (DP == 64) tq_many_weights_launch_d64(ik, g, s, a, blocks);
         if constexpr (DP == 96) tq_many_weights_launch_d96(ik, g, s, a, blocks);
         if constexpr (DP == 128) tq_many_weights_launch_d128(ik, g, s, a, blocks);
         if constexpr (DP == 256) tq_many_weights_launch_d256(ik, g, s, a, blocks);
-    } else if (a.tokens) {
+        return;
+    }
+    if (a.tokens) {
         const uint32_t blocks = (a.tokens + 32u * ANY_WAVES - 1u) / (32u * ANY_WAVES);
         hipLaunchKernelGGL((tq_many_any_weights_kernel<DP>), dim3(a.rows * blocks), dim3(64 * ANY_WAVES), 0, s, a, blocks);
     }

@@ -292,11 +292,8 @@ struct Rotate {
         if (i < (uint32_t)QT) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                uint32_t t[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) t[k] = fp16_terms(y[8 * j + k] * f);
                 tq_u4 hi, lo;
-                fp16_operands(t, hi, lo);
+                fp16_split8(tq_f4{y[8 * j], y[8 * j + 1], y[8 * j + 2], y[8 * j + 3]}, tq_f4{y[8 * j + 4], y[8 * j + 5], y[8 * j + 6], y[8 * j + 7]}, f, hi, lo);
                 const uint32_t d = 32u * w + 16u * h + 8u * j, half = d / (DP / 2u), s = (d - half * (DP / 2u)) / 8u;
                 uint8_t *o = ops + ((i * KT * STEPS + s) * 64u + half * 32u + n) * 16u;
                 *reinterpret_cast<tq_u4 *>(o) = hi;
@@ -731,15 +728,10 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 #pragma unroll
         for (int s = 0; s < CH; ++s) {
             const uint32_t j = DP == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
-            const tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + j), y = *reinterpret_cast<const tq_f4 *>(o + j + 4u);
-            uint32_t t[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                t[k] = Shape<DP>::EVEN || j + k < a.D ? fp16_terms(x[k] * f) : 0u;
-                t[4 + k] = Shape<DP>::EVEN || j + 4 + k < a.D ? fp16_terms(y[k] * f) : 0u;
-            }
+            tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + j), y = *reinterpret_cast<const tq_f4 *>(o + j + 4u);
+            if (!Shape<DP>::EVEN && j >= a.D) x = y = tq_f4{0.f, 0.f, 0.f, 0.f};        // (D a multiple of 8; what lies past it may be anything)
             tq_u4 oh, ol;
-            fp16_operands(t, oh, ol);
+            fp16_split8(x, y, f, oh, ol);
             acc = mfma_f16(ph[s], oh, acc);
             acc = mfma_f16(ph[s], ol, acc);
             acc = mfma_f16(pl[s], oh, acc);
@@ -1106,13 +1098,62 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 // What the packed tokens receive: weight = 2^(logit - largest) / sum with the statistics of the merge, from the two-term products.  Rows of the product are queries
 // here, columns tokens, so that a token's sum is made in its lane; rows in which a tile has no query are left out eight at a time.  Block = part of
 // a row's tokens, a wave takes 32 at a time and all tiles of queries in order (the first one's operands lie in LDS, a decode step has no more).
+// The first blocks are for the window's tokens: a wave 32 of them.
+template <int DP, int DT>
+__device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t item, uint32_t lane) {
+    if constexpr (DT == TQ_F32) plain_weights<TQ_F32>(a, item, DP / 16u, lane);
+    else {
+        using T = PlainTile<DP, DT>;
+        constexpr int STEPS = DP / 16, CH = DP <= 128 ? STEPS : 8;
+        const TqManyPlain &seg = a.plain[0];
+        const uint32_t groups = (seg.n + 31u) / 32u, row = item / groups, t0 = 32u * (item - row * groups), b = row / a.heads, kv = row - b * a.heads;
+        const uint32_t n = lane & 31u, h = lane >> 5, length = many_length(a, b), t = t0 + n, tc = min(t, seg.n - 1u);
+        const uint8_t *k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)tc * seg.k_token) * 2;
+        const bool seen = t < seg.n && plain_seen(a, 0u, b, 0u, tc, length);
+        float w = 0.f;
+#pragma unroll 1
+        for (uint32_t tile = 0; tile < a.tiles; ++tile) {             // rows of the product: queries, columns: tokens
+            const uint8_t *q = many_query(a, row, min(tile * 32u + n, a.M - 1u), 2u);
+            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + ((size_t)row * a.tiles + tile) * 64u + 4u * h;
+            tq_f16v s = tq_zero16();
+#pragma unroll 1
+            for (int s0 = 0; s0 < STEPS; s0 += CH) {
+                tq_u4 x[CH], y[CH];
+#pragma unroll
+                for (int st = 0; st < CH; ++st) { x[st] = T::half_step(k, s0 + st, h, a.D, a.aligned); y[st] = T::half_step(q, s0 + st, h, a.D, a.aligned); }
+#pragma unroll
+                for (int st = 0; st < CH; ++st) s = DT == TQ_BF16 ? mfma_bf16(y[st], x[st], s) : mfma_f16(y[st], x[st], s);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (inv[r] != 0.f) w = fmaf(__builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.scale * LOG2E, -m[r])), inv[r], w);
+            }
+        }
+        w = halves_add(w);
+        if (h == 0u && seen) a.weights[(long long)row * a.w_stride + a.tokens + t] += w;
+    }
+}
+
 template <int DP, int IPBK>
 __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_kernel(TqManyArgs a, uint32_t blocks) {
+    const uint32_t items = a.rows * ((a.plain[0].n + 31u) / 32u), first = (items + FAST_WAVES - 1u) / FAST_WAVES;
+    if (blockIdx.x < first) {
+        const uint32_t item = blockIdx.x * FAST_WAVES + tq_uniform32(threadIdx.x >> 6);
+        if (item >= items) return;
+        if (a.dtype == TQ_BF16) window_weights<DP, TQ_BF16>(a, item, threadIdx.x & 63u);
+        else if (a.dtype == TQ_F16) window_weights<DP, TQ_F16>(a, item, threadIdx.x & 63u);
+        else window_weights<DP, TQ_F32>(a, item, threadIdx.x & 63u);
+        return;
+    }
+    const uint32_t block = blockIdx.x - first;
     using Keys = KeyRun<DP, IPBK>;
     constexpr int STEPS = DP / 16, KW = Keys::KW, LUT_BYTES = 65536;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[LUT_BYTES + 2 * STEPS * 1024 + FAST_WAVES * Keys::BYTES];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
-    const uint32_t row = blockIdx.x / blocks, b = row / a.heads;
+    const uint32_t row = block / blocks, b = row / a.heads;
     const size_t first_tile = (size_t)row * a.tiles;
     const uint32_t seen = min(a.tokens, many_length(a, b));
     {
@@ -1128,7 +1169,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     const uint32_t GBK = Shape<DP>::EVEN ? DP / IPBK : (a.D + IPBK - 1u) / IPBK;
     uint8_t *kstage = lds + LUT_BYTES + 2 * STEPS * 1024 + wave * Keys::BYTES;
     const uint32_t last = a.tokens - 32u, step = 32u * FAST_WAVES * blocks;
-    for (uint32_t t_run = 32u * ((blockIdx.x - row * blocks) * FAST_WAVES + wave); t_run < seen; t_run += step) {
+    for (uint32_t t_run = 32u * ((block - row * blocks) * FAST_WAVES + wave); t_run < seen; t_run += step) {
         const uint32_t t0 = min(t_run, last), t = t0 + n;
         Keys keys;
         keys.issue(a.k_idx + (slot0 + t0) * GBK, GBK, lane);

@@ -104,34 +104,6 @@ __device__ __forceinline__ void put_sums(float *rec, uint32_t lane, float m, flo
 // and of the weights, down to 2^-24 of the largest: exact for 16-bit logits up to their summation.
 // WEIGHTS: instead of the sums, what every token of the window receives is added to a.weights; a.stat has the columns' statistics, and a block
 // goes through all tiles of its row, so that a token's sum is made by one wave in a fixed order.
-template <int DT>
-__device__ __forceinline__ void plain_logits(const TqManyArgs &a, const TqManyPlain &seg, uint32_t which, uint32_t row, uint32_t b, uint32_t kv, uint32_t t0, uint32_t m,
-                                             uint32_t lane, uint32_t length, uint32_t steps, float (&x)[16]) {
-    constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
-    constexpr int NT = plain_terms<DT>();
-    const uint32_t n = lane & 31u, h = lane >> 5;
-    const uint8_t *k = seg.k + ((long long)b * seg.k_batch + (long long)kv * seg.k_head + (long long)min(t0 + n, seg.n - 1u) * seg.k_token) * ES;
-    const uint8_t *q = many_query(a, row, min(m, a.M - 1u), ES);
-    tq_f16v acc = tq_zero16();
-    for (uint32_t s = 0; s < steps; ++s) {
-        tq_u4 kt[3], qt[3];
-        load_plain8<DT>(k, 16u * s + 8u * h, a.D, a.aligned, kt);
-        load_plain8<DT>(q, 16u * s + 8u * h, a.D, a.aligned, qt);
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                if (i + j < 3) acc = mfma_bf16(kt[i], qt[j], acc);
-    }
-    const uint32_t i = ManyQuery(a, min(m, a.M - 1u)).t;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const uint32_t t = t0 + acc_row(r, h);
-        const bool seen = t < seg.n && plain_seen(a, which, b, i, t, length);
-        x[r] = seen ? acc[r] * (a.scale * LOG2E) : MANY_NONE;
-    }
-}
-
 template <int DP, int DT>
 __global__ __launch_bounds__(64 * PLAIN_WAVES) void tq_many_plain_kernel(TqManyArgs a) {
     constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
@@ -207,34 +179,9 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void tq_many_plain_kernel(TqManyA
     put_sums<DP>(a.plain_rec + ((size_t)blockIdx.x * a.plain_records + wave) * record_floats(DP), lane, m, l, acc, 1.f);
 }
 
-// What the window's tokens receive: wave = 32 tokens, all query tiles of the row in order.
 template <int DT>
 __global__ __launch_bounds__(64) void tq_many_plain_weights_kernel(TqManyArgs a, uint32_t steps) {
-    const TqManyPlain &seg = a.plain[0];
-    const uint32_t groups = (seg.n + 31u) / 32u;
-    const uint32_t row = blockIdx.x / groups, t0 = 32u * (blockIdx.x - row * groups), b = row / a.heads, kv = row - b * a.heads;
-    const uint32_t lane = threadIdx.x, n = lane & 31u, h = lane >> 5, length = many_length(a, b);
-    float w[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) w[r] = 0.f;
-    for (uint32_t tile = 0; tile < a.tiles; ++tile) {
-        float x[16];
-        plain_logits<DT>(a, seg, 0u, row, b, kv, t0, tile * 32u + n, lane, length, steps, x);
-        const float *stat = a.stat + ((size_t)row * a.tiles + tile) * 64u;
-        const float m = stat[n], inv = stat[32u + n];
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(x[r] - m), inv, w[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int i = 1; i < 32; i <<= 1) w[r] += __shfl_xor(w[r], i);
-    float own = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) own = n == (uint32_t)r ? w[r] : own;
-    const uint32_t t = t0 + acc_row((int)(n & 15u), h);
-    if (n < 16u && t < seg.n && a.tokens + t < length) a.weights[(long long)row * a.w_stride + a.tokens + t] += own;
+    plain_weights<DT>(a, blockIdx.x, steps, threadIdx.x);
 }
 
 // ---- packed tokens, any head dimension ------------------------------------------------------------------------------------------
@@ -528,6 +475,9 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
         else
             for (uint32_t r = 0; r < a.plain_records; ++r)
                 add(o[1], *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(plain + (size_t)r * record_floats(DP) + off), lds_f[a.records + r][q]);
+        if (DP != a.D)               // (what lies past the last coordinate may be anything)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) o[0][e] = d + e < a.D ? o[0][e] : 0.f;
         *reinterpret_cast<tq_f4 *>(&lds_o[0][q * ROW + d]) = o[0];
         *reinterpret_cast<tq_f4 *>(&lds_o[1][q * ROW + d]) = o[1];
     }
@@ -535,7 +485,7 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     // ---- back out of the codec's space; columns past C repeat the others
     const uint32_t q = n32 % C;
     float largest = 0.f;
-#pragma unroll
+#pragma unroll 4
     for (uint32_t d = 0; d < DP / 2u; d += 4u) {
         const tq_f4 x = *reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + h * (DP / 2u) + d]);
 #pragma unroll
@@ -552,11 +502,8 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
         for (uint32_t s = 0; s < CH; ++s) {
             if (s0 + s >= STEPS) break;
             const uint32_t j = tuned ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;
-            uint32_t t[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = fp16_terms(j + i < a.D ? lds_o[0][q * ROW + j + i] * f : 0.f);
             tq_u4 oh, ol;
-            fp16_operands(t, oh, ol);
+            fp16_split8(*reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + j]), *reinterpret_cast<const tq_f4 *>(&lds_o[0][q * ROW + j + 4u]), f, oh, ol);
             acc = mfma_f16(ph[s], oh, acc);
             acc = mfma_f16(ph[s], ol, acc);
             acc = mfma_f16(pl[s], oh, acc);
