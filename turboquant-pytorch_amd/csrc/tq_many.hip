@@ -123,11 +123,11 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     if (a.tokens && plan.qt) {
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
-        const uint32_t most = (a.tokens + 32u * 8u - 1u) / (32u * 8u);
-        uint32_t blocks = ((uint32_t)cus + a.rows - 1u) / a.rows;
+        // one block is resident per compute unit; the window's come first
+        const uint32_t most = (a.tokens + 255u) / 256u, window = (a.rows * ((a.plain[0].n + 31u) / 32u) + 7u) / 8u;
+        uint32_t blocks = (uint32_t)cus > window + a.rows ? ((uint32_t)cus - window) / a.rows : 1u;
         if (blocks > most) blocks = most;
-        const uint32_t window = a.rows * ((a.plain[0].n + 31u) / 32u);
-        const dim3 g(a.rows * blocks + (window + 7u) / 8u);
+        const dim3 g(a.rows * blocks + window);
         const int ik = 8 / (int)a.bits_k;
         if constexpr (DP == 64) tq_many_weights_launch_d64(ik, g, s, a, blocks);
         if constexpr (DP == 96) tq_many_weights_launch_d96(ik, g, s, a, blocks);

@@ -1169,18 +1169,31 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     const uint32_t GBK = Shape<DP>::EVEN ? DP / IPBK : (a.D + IPBK - 1u) / IPBK;
     uint8_t *kstage = lds + LUT_BYTES + 2 * STEPS * 1024 + wave * Keys::BYTES;
     const uint32_t last = a.tokens - 32u, step = 32u * FAST_WAVES * blocks;
-    for (uint32_t t_run = 32u * ((block - row * blocks) * FAST_WAVES + wave); t_run < seen; t_run += step) {
-        const uint32_t t0 = min(t_run, last), t = t0 + n;
-        Keys keys;
-        keys.issue(a.k_idx + (slot0 + t0) * GBK, GBK, lane);
-        const float norm = (float)__builtin_bit_cast(_Float16, tq_gload2(a.k_norms + slot0 + t));
+    // (loads of a run are issued while the one before it is worked on)
+    Keys keys;
+    uint16_t norm_raw = 0;
+    float before_raw = 0.f;
+    float *const sums = a.weights + (long long)row * a.w_stride;
+    auto issue = [&](uint32_t t) __attribute__((always_inline)) {
+        keys.issue(a.k_idx + (slot0 + t) * GBK, GBK, lane);
+        norm_raw = tq_gload2(a.k_norms + slot0 + t + n);
+        before_raw = *((const TQ_GLOBAL float *)sums + t + n);
+    };
+    uint32_t t_next = 32u * ((block - row * blocks) * FAST_WAVES + wave);
+    if (t_next < seen) issue(min(t_next, last));
+    while (t_next < seen) {
+        const uint32_t t_run = t_next, t0 = min(t_run, last), t = t0 + n;
+        t_next += step;
+        const float norm = (float)__builtin_bit_cast(_Float16, norm_raw), before = before_raw;
         const bool counts = t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
-        float *dst = a.weights + (long long)row * a.w_stride + t;
-        const float before = h == 0u && counts ? *dst : 0.f;
         float w = 0.f;
         keys.stage(kstage, lane);
         wave_sync();
         keys.take(kstage, GBK, lane);
+        uint32_t kraw[KW];
+#pragma unroll
+        for (int i = 0; i < KW; ++i) kraw[i] = keys.raw[i];
+        if (t_next < seen) issue(min(t_next, last));
         auto add = [&](const tq_f16v &s, uint32_t tile, float kn, uint32_t queries) __attribute__((always_inline)) {
             const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * 64u + 4u * h;
 #pragma unroll
@@ -1196,7 +1209,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 tq_u4 hi, lo;
-                decode_keys2<IPBK, KW>(keys.raw, st, lds, slot, hi, lo);
+                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
                 const tq_u4 qh = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + st * 1024 + lane * 16u), ql = *reinterpret_cast<const tq_u4 *>(lds + LUT_BYTES + (STEPS + st) * 1024 + lane * 16u);
                 s = mfma_f16(qh, hi, s);
                 s = mfma_f16(ql, hi, s);
@@ -1211,7 +1224,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 tq_u4 hi, lo;
-                decode_keys2<IPBK, KW>(keys.raw, st, lds, slot, hi, lo);
+                decode_keys2<IPBK, KW>(kraw, st, lds, slot, hi, lo);
                 const tq_u4 qh = tq_gload16(ops + st * 1024), ql = tq_gload16(ops + (STEPS + st) * 1024);
                 s = mfma_f16(qh, hi, s);
                 s = mfma_f16(ql, hi, s);
@@ -1220,7 +1233,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
             add(s, tile, norm * a.q_scale[first_tile + tile], a.M - 32u * tile);
         }
         w = halves_add(w);
-        if (h == 0u && counts) *dst = before + w;
+        if (h == 0u && counts) *((TQ_GLOBAL float *)sums + t) = before + w;
         wave_sync();
     }
 }
