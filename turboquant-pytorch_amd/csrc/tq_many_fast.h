@@ -899,6 +899,9 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     while (t_next < end) {
         const uint32_t t_run = t_next, t0 = min(t_run, last), count = min(32u, end - t_run);
         t_next += 32u * FAST_WAVES;
+        // (the two waves of a SIMD go first in turn: left to itself the older one runs ahead, and the other then ends alone)
+        if (((t_run / (32u * FAST_WAVES)) ^ (wave >> 2)) & 1u) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         const uint32_t t_after = min(t_next < end ? t_next : t_run, last);
         uint32_t hidden = ~((count == 32u ? 0xffffffffu : (1u << count) - 1u) << (t_run - t0));
         if (mask) hidden |= ~(uint32_t)__ballot(mask[t0 + n] != 0);
@@ -1069,6 +1072,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         wave_sync();
     }
 
+    __builtin_amdgcn_s_setprio(0);
     // ---- the waves' sums
     const float unit = v_top == -100 ? 0.f : __uint_as_float((uint32_t)(127 + v_top - FAST_P - (VT == 2 ? LEVEL_SHIFT : 0)) << 23);
 #pragma unroll
@@ -1159,10 +1163,11 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     {
         Lut2<IPBK> table;
         table.load(a.table_k, a.bits_k, DP, tid);
-        table.store(lds, tid);
+        table.store(lds, tid);              // (alone, it takes the whole row)
+        table.store(lds + 128, tid);
     }
     tq_copy_to_lds(lds + LUT_BYTES, a.q_op + first_tile * q_operand_bytes(DP), 2 * STEPS * 1024, tid, FAST_THREADS);
-    const uint32_t slot = Lut2<IPBK>::lane_offset(lane);
+    const uint32_t slot = (lane & (64u / IPBK - 1u)) * 4u * IPBK;
     const float scale0 = a.q_scale[first_tile];
     __syncthreads();
     const size_t slot0 = (size_t)row * a.packed_row_stride;
@@ -1181,9 +1186,13 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     };
     uint32_t t_next = 32u * ((block - row * blocks) * FAST_WAVES + wave);
     if (t_next < seen) issue(min(t_next, last));
+    uint32_t first_of_two = wave >> 2;
     while (t_next < seen) {
         const uint32_t t_run = t_next, t0 = min(t_run, last), t = t0 + n;
         t_next += step;
+        first_of_two ^= 1u;                 // (as in the kernel above)
+        if (first_of_two) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         const float norm = (float)__builtin_bit_cast(_Float16, norm_raw), before = before_raw;
         const bool counts = t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
         float w = 0.f;
