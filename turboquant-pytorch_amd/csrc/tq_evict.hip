@@ -48,15 +48,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
 }
 
 // Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens; E = 0: of more, read again for every pass.
-// The keep-th largest weight lies in a range of whole numbers, at first all there are.  While more than 1024 tokens lie in it, it is cut into 2048 parts, the tokens of each are counted
+// The keep-th largest weight lies in a range of whole numbers, at first all there are.  While more than 256 tokens lie in it, it is cut into 2048 parts, the tokens of each are counted
 // in LDS, and the part with the keep-th one is the next range: a floating-point number's bits go with its logarithm, so that sums spread over the parts and few of the
 // counts' atomics meet (counting by the leading byte instead took 110 us for 8 x 32768 tokens; those at the lower end, zeros, are counted by ballots).
-// What is left is packed to one a thread and settled bit by bit, with ballots.  Tokens above the result stay, and of those equal to it the first ones; places come
+// What is left is packed, and four threads count those above each.  Tokens above the result stay, and of those equal to it the first ones; places come
 // from counts per wave and register, in the tokens' order.
 template <int E>
 __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictArgs a) {
-    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048;
-    __shared__ uint32_t lds_part[PARTS], lds_few[SELECT_THREADS], lds_count[2][WAVES], lds_ends[2][WAVES], lds_place[E ? E * WAVES : 1], lds_found[3], lds_n;
+    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048, FEW = 256;
+    __shared__ __attribute__((aligned(16))) uint32_t lds_few[FEW + 4];
+    __shared__ uint32_t lds_part[PARTS], lds_count[WAVES], lds_ends[2][WAVES], lds_place[E ? E * WAVES : 1], lds_found[3], lds_n;
     const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6);
     const TQ_GLOBAL float *w = (const TQ_GLOBAL float *)a.weights + (long long)row * a.w_stride;
     uint32_t key[E ? E : 1], lo = 0xffffffffu, hi = 0u;           // a token that is none: 0, less than any number's
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
         }
     };
     if constexpr (E) {
-        constexpr int CH = E < 8 ? E : 8;
+        constexpr int CH = E < 16 ? E : 16;
 #pragma unroll
         for (int e0 = 0; e0 < E; e0 += CH) {
             float v[CH];
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
     for (uint32_t k = 0; k < WAVES; ++k) { lo = min(lo, lds_ends[0][k]); hi = max(hi, lds_ends[1][k]); }
     lo += 1u;                                             // (a row has a token at least)
     uint32_t left = a.keep, agree = a.tokens;             // agree tokens in [lo, hi], of which the largest `left` stay; all above hi do
-    while (agree > SELECT_THREADS && lo < hi && left < agree) {
+    while (agree > FEW && lo < hi && left < agree) {
         const uint32_t width = 32u - (uint32_t)__builtin_clz(hi - lo), shift = width > 11u ? width - 11u : 0u;
 #pragma unroll
         for (uint32_t k = 0; k < PARTS / SELECT_THREADS; ++k) lds_part[tid + k * SELECT_THREADS] = 0u;
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
         // from the upper end: two parts a thread
         const uint32_t p1 = PARTS - 1u - 2u * tid, c1 = lds_part[p1], c0 = lds_part[p1 - 1u];
         uint32_t all;
-        const uint32_t above = block_scan(c1 + c0, lds_count[0], all);
+        const uint32_t above = block_scan(c1 + c0, lds_count, all);
         if (above < left && above + c1 + c0 >= left) {
             const bool upper = above + c1 >= left;
             lds_found[0] = upper ? p1 : p1 - 1u;
@@ -131,38 +132,26 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
     uint32_t border = lo;                                  // with left == agree all from lo on stay, with lo == hi the first `left` of them
     if (lo < hi && left < agree) {
         each([&](uint32_t k) {
-            const bool in = k >= lo && k <= hi;
-            const unsigned long long mine = __ballot(in);
-            if (mine) {
-                uint32_t base = 0u;
-                if (lane == 0u) base = atomicAdd(&lds_n, (uint32_t)__popcll(mine));          // (in any order: they are only counted)
-                base = tq_uniform32(base);
-                if (in) lds_few[base + __builtin_amdgcn_mbcnt_hi((uint32_t)(mine >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mine, 0u))] = k;
-            }
+            if (k >= lo && k <= hi) lds_few[atomicAdd(&lds_n, 1u)] = k;          // (in any order: they are only counted)
         });
+        if (tid < 4u) lds_few[agree + tid] = 0u;
         __syncthreads();
-        const bool mine = tid < agree;
-        const uint32_t own = mine ? lds_few[tid] - lo : 0u, size = agree;
-        uint32_t found = 0u, turn = 0u;
-        auto count = [&](uint32_t from) {                  // of the packed ones, those at least `from` above lo
-            const uint32_t c = (uint32_t)__popcll(__ballot(mine && own >= from));
-            if (lane == 0u) lds_count[turn][wave] = c;
-            __syncthreads();
-            uint32_t v = 0u;
+        static_assert(4u * FEW == SELECT_THREADS, "four threads a token");
+        const uint32_t own = lds_few[min(tid / 4u, agree)];
+        uint32_t over = 0u, same = 0u;
+#pragma unroll 4
+        for (uint32_t i = 4u * (tid & 3u); i < agree; i += 16u) {
+            const tq_u4 x = *reinterpret_cast<const tq_u4 *>(lds_few + i);
 #pragma unroll
-            for (uint32_t k = 0; k < WAVES; ++k) v += lds_count[turn][k];
-            turn ^= 1u;
-            return v;
-        };
-        uint32_t from_found = size;
-        for (int bit = 31 - __builtin_clz(hi - lo); bit >= 0; --bit) {
-            const uint32_t c = count(found | (1u << bit));
-            if (c >= left) { found |= 1u << bit; from_found = c; }
+            for (int k = 0; k < 4; ++k) { over += x[k] > own ? 1u : 0u; same += x[k] == own ? 1u : 0u; }
         }
-        const uint32_t over = found == 0xffffffffu ? 0u : count(found + 1u);
-        border = lo + found;
-        left -= over;
-        agree = from_found - over;
+#pragma unroll
+        for (int i = 1; i < 4; i <<= 1) { over += (uint32_t)__shfl_xor(over, i); same += (uint32_t)__shfl_xor(same, i); }
+        if (tid / 4u < agree && over < left && over + same >= left) { lds_found[0] = own; lds_found[1] = over; lds_found[2] = same; }        // (its equals say the same)
+        __syncthreads();
+        border = lds_found[0];
+        left -= lds_found[1];
+        agree = lds_found[2];
     }
     // ---- places
     TQ_GLOBAL long long *kept = (TQ_GLOBAL long long *)a.kept + (long long)row * a.keep;
@@ -178,14 +167,14 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
                 same += k8[k] == border ? 1u : 0u;
             }
             uint32_t all;
-            uint32_t rank = equal + block_scan(same, lds_count[0], all);
+            uint32_t rank = equal + block_scan(same, lds_count, all);
             equal += all;
 #pragma unroll
             for (uint32_t k = 0; k < 8u; ++k) {
                 if (k8[k] == border && rank++ >= left && left < agree) k8[k] = 0u;
                 more += k8[k] >= border ? 1u : 0u;
             }
-            uint32_t at = out + block_scan(more, lds_count[0], all);
+            uint32_t at = out + block_scan(more, lds_count, all);
             out += all;
 #pragma unroll
             for (uint32_t k = 0; k < 8u; ++k)
@@ -196,7 +185,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
     auto scan = [&]() {                                    // lds_place, [register][wave]: counts -> sums of those before
         __syncthreads();
         uint32_t all;
-        const uint32_t v = tid < E * WAVES ? lds_place[tid] : 0u, x = block_scan(v, lds_count[0], all);
+        const uint32_t v = tid < E * WAVES ? lds_place[tid] : 0u, x = block_scan(v, lds_count, all);
         if (tid < E * WAVES) lds_place[tid] = x;
         __syncthreads();
     };
