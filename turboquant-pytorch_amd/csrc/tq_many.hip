@@ -26,22 +26,23 @@ bool fast(const tq_attend_request *r) {
     return D > 64 && D <= 96 && !(D & 7) && !(D / ik & 3) && !(D % ik) && !(D / iv & 3) && !(D % iv) && !(((uintptr_t)r->k_idx | (uintptr_t)r->v_idx) & 3u);
 }
 
-// splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and what its start
-// and its end cost; `others`: blocks of uncompressed tokens in the same launch
-long long fast_splits(long long blocks, long long others, long long tokens) {
-    int cus = 0;
-    if (tq_device_cus(cus)) cus = 256;
+// Splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and, in tokens, what its start and its
+// end cost (1500) and its uncompressed tokens (1000; `others`: blocks of those in the same launch), and for the merge 1000 and 30 a split.  A token with two terms of
+// everything (float32) counts three times.  Measured (us) against all other numbers of splits, 8 key/value heads of 128: 2048 tokens x 32 query vectors 19.1 with 8 (1: 32.3,
+// 4: 20.1), 8192 x 32 22.3 with 16 (8: 23.6, 32: 31.4), 131072 x 32 50.5 with 31 (24: 49.9, 16: 62.5, 64: 67.6), 16 sequences of 8192 x 64 as below, 32 of 8192 x 4 with kept
+// sums 139 with 1 (2: 152); float32 rows of 1003 tokens, 80 wide, 21.7 with 4 (1: 24.8).
+long long fast_splits(int cus, long long blocks, long long others, long long tokens, int vt) {
+    const long long weight = vt == 2 ? 3 : 1;
     long long most = (tokens + 255) / 256, best = 1, best_cost = 0;
     if (most > MAX_SPLITS) most = MAX_SPLITS;
     for (long long s = 1; s <= most; ++s) {
         const long long rounds = (blocks * s + cus - 1) / cus, extra = s == 1 ? rounds * (others ? 1000 : 0) : blocks * s + others > rounds * cus ? (others + cus - 1) / cus * 1000 : 0;
-        const long long cost = rounds * ((tokens + s - 1) / s + 1500) + extra + (s > 1 ? 1000 : 0) + 30 * s;
+        const long long cost = rounds * ((tokens + s - 1) / s * weight + 1500) + extra + (s > 1 ? 1000 : 0) + 30 * s;
         if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
         if (rounds > 16 && s > 1) break;
     }
     return best;
 }
-
 
 int plan(const tq_attend_request *r, Plan &p) {
     p.rows = r->batch * r->heads;
@@ -53,9 +54,18 @@ int plan(const tq_attend_request *r, Plan &p) {
     if (at && r->tokens && fast(r)) {
         p.kt = r->dtype == TQ_BF16 && !r->weights ? 1 : 2;
         p.vt = r->dtype == TQ_F32 ? 2 : 1;
-        p.qt = p.kt == 1 && r->head_dim != 256 && p.tiles > 1 ? 2 : 1;
-        p.groups = (p.tiles + p.qt - 1) / p.qt;
-        p.splits = fast_splits(p.rows * p.groups, plain_tiles(r) ? p.rows * p.groups : 0, r->tokens);
+        // Two tiles of queries a block share what is read and decoded.  One, where that fills no more than a round of blocks without splitting a row: 16 sequences
+        // of 8192 tokens, 64 query vectors a head, 72 us against 84, 2 of 1024 x 512 28 against 39; but 8 of 4096 x 2048 408 against 536, 1 of 32768 x 256 75 against 78.
+        int cus = 0;
+        if (tq_device_cus(cus)) cus = 256;
+        const long long others = plain_tiles(r) ? at : 0;
+        p.qt = 1;
+        p.splits = fast_splits(cus, at, others, r->tokens, p.vt);
+        if (p.kt == 1 && r->head_dim != 256 && p.tiles > 1 && (p.splits > 1 || at > cus)) {
+            p.qt = 2;
+            p.groups = (p.tiles + 1) / 2;
+            p.splits = fast_splits(cus, p.rows * p.groups, others ? p.rows * p.groups : 0, r->tokens, p.vt);
+        }
     } else if (at && r->tokens) {
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
