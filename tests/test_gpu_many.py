@@ -367,6 +367,26 @@ def test_evict_keeps_the_largest(pkg, B, H, n, w, keep, D, dtype, kb, vb):
     assert torch.equal(everything[3], torch.arange(n, device=DEV).expand(B, H, n)) and torch.equal(everything[0]["compressed"]["idx_bytes"], ck["compressed"]["idx_bytes"])
 
 
+@pytest.mark.parametrize("n,keep", [(2000, 100), (3000, 1700), (40000, 300)])
+def test_evict_of_weights_that_lie_close(pkg, n, keep):
+    """More NaN than stay above numbers anywhere (the range of what is searched ends at the largest whole number), neighbours among float32, a few values many times."""
+    codec = pkg.TurboQuantV3(64, key_bits=2, value_bits=2, residual_window=0, layer_idx=8, device=DEV)
+    ck, cv = codec.compress_kv(rand((1, 2, n, 64), 1, BF), rand((1, 2, n, 64), 2, BF))
+    g = torch.Generator()
+    g.manual_seed(n)
+    places = torch.stack([torch.randperm(n, generator=g) for _ in range(2)]).unsqueeze(0)
+    neighbours = (places.int() + 0x3f8abcde).view(torch.float32)
+    many_nan = torch.where(places < 2 * keep, torch.full((), float("nan")), neighbours)
+    few_values = (places.int() % 3 + 0x3f8abcde).view(torch.float32)
+    steps = (places.int() // 700 * 5 + 0x3f8abcde).view(torch.float32)
+    far = torch.where(places < 300, torch.full((), float("inf")), neighbours * torch.tensor([1e-38, -1e30]).view(1, 2, 1))
+    for name, weights in {"neighbours": neighbours, "many NaN": many_nan, "few values": few_values, "steps": steps, "far": far}.items():
+        weights = weights.to(DEV)
+        kept = codec.evict_kv(ck, cv, weights, keep)[3]
+        want = torch.sort(torch.sort(weights, dim=-1, descending=True, stable=True).indices[:, :, :keep], dim=-1).values
+        assert torch.equal(kept, want), name
+
+
 @pytest.mark.parametrize("D,dtype", [(128, BF), (96, F16), (80, F32)])
 def test_generation_with_drafts_and_a_budget(pkg, D, dtype, tmp_path):
     """The operators as they are used together: verify a draft, append what is accepted, attend, thin out when over the budget, go on."""
@@ -505,3 +525,56 @@ def test_offsets_past_32_bits(pkg):
     weights = torch.rand(B, H, n, device=DEV)
     far, near = pkg._native.evict(packed, n, (4, 2), D, weights, 33), pkg._native.evict(dense, n, (4, 2), D, weights, 33)
     assert all(torch.equal(a, b) for x, y in zip(far[0], near[0]) for a, b in zip(x, y)) and torch.equal(far[2], near[2])
+
+
+def test_one_step_calls_answer_as_the_general_ones(pkg, monkeypatch):
+    """Eager calls go by one extension call where everything lies as the library takes it: the same bits as without it, window turned or not."""
+    cache = make_cache(pkg, 2, 2, 300, 16, 128, BF, track_weights=True)
+    k1, v1 = rand((2, 2, 5, 128), 7, BF), rand((2, 2, 5, 128), 8, BF)
+    for i in range(5):                                    # (the window is a ring of buffer slots: its first token moves)
+        cache.append(k1[:, :, i:i + 1], v1[:, :, i:i + 1], 1)
+    q, k, v, tree = rand((2, 8, 9, 128), 1, BF), rand((2, 2, 9, 128), 2, BF), rand((2, 2, 9, 128), 3, BF), random_tree(9, 1, 2)
+    codec = pkg.TurboQuantV3(128, key_bits=4, value_bits=2, residual_window=16, layer_idx=8, device=DEV)
+    ck, cv = codec.compress_kv(rand((2, 2, 200, 128), 4, BF), rand((2, 2, 200, 128), 5, BF))
+    lengths, mask = torch.tensor([150, 0], dtype=torch.int32, device=DEV), torch.rand(2, 200, device=DEV) < 0.5
+
+    def answers():
+        w = torch.zeros(2, 2, 200, device=DEV)
+        cache.attention_weights(1).zero_()
+        out = [cache.attend_tree(q, k, v, 1, tree), cache.attend_tree(q, k, v, 1), cache.attend(q[:, :, :1], 1), cache.attention_weights(1).clone(),
+               codec.attend_kv(q, ck, cv, lengths=lengths, mask=mask, weights=w, scale=0.1), w]
+        nk, nv, left, kept = codec.evict_kv(ck, cv, w, 33)
+        return out + [nk["compressed"]["idx_bytes"], nk["compressed"]["vec_norms"], nv["compressed"]["idx_bytes"], nv["compressed"]["vec_norms"], left, kept]
+    answers()                                             # (the scratch of the stream is there afterwards)
+    one_step = answers()
+    monkeypatch.setattr(pkg._native, "attend_many_store", lambda *a: None)
+
+    class Without:
+        evict = staticmethod(lambda *a: None)
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+    real = pkg._native.fast()
+    monkeypatch.setattr(pkg._native, "fast", lambda: Without())
+    for i, (a, b) in enumerate(zip(one_step, answers())):
+        assert torch.equal(a, b), i
+
+
+def test_eviction_from_the_cache_that_models_use(pkg):
+    """Positions go on after an eviction, masks are made for the keys that are left, and update answers with those and the new ones."""
+    cache = pkg.hf_cache_class()(key_bits=4, value_bits=2, residual_window=8, n_layers=4, track_weights=True)
+    k, v = rand((1, 2, 90, 128), 1, BF), rand((1, 2, 90, 128), 2, BF)
+    cache.update(k, v, 1)
+    for i in range(3):
+        cache.attend(rand((1, 4, 1, 128), 10 + i, BF), 1)
+    assert cache.get_mask_sizes(1, 1) == (91, 0)
+    kept = cache.evict(30, 1)
+    assert kept.shape == (1, 2, 30) and cache.get_seq_length(1) == 90 and cache.get_mask_sizes(5, 1) == (38 + 5, 52)
+    k1, v1 = rand((1, 2, 4, 128), 3, BF), rand((1, 2, 4, 128), 4, BF)
+    fk, fv = cache.update(k1, v1, 1)                      # (the window's oldest four tokens are packed by that)
+    K, V = contents(cache)
+    assert fk.shape == (1, 2, 42, 128) and torch.equal(fk[:, :, -4:], k1) and torch.equal(fv[:, :, -4:], v1)
+    assert (fk.double() - K).norm() <= 4e-3 * K.norm() and (fv.double() - V).norm() <= 4e-3 * V.norm() and cache.get_seq_length(1) == 94
+    q = rand((1, 4, 1, 128), 5, BF)
+    check(cache.attend(q, 1), q, K, V, torch.ones(42, dtype=torch.bool, device=DEV))
+    assert cache.evict(100, 1).shape == (1, 2, 34) and not cache.evict(0)[1].numel() and cache.get_mask_sizes(1, 1) == (9, 86)

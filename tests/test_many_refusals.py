@@ -1,8 +1,13 @@
 """What attention over several queries, kept sums and eviction refuse: found on the host, before anything is launched."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_entry_points_check_their_arguments(pkg):
@@ -115,3 +120,16 @@ def test_dictionaries_that_do_not_go_together(pkg):
     assert nk["split_at"] == 8 and kept.shape == (1, 2, 0) and left.shape == (1, 2, 8)
     with pytest.raises(ValueError, match="weights must be"):
         codec.evict_kv(ck, cv, torch.zeros(1, 2, 7), 3)
+
+
+def test_structures_match_the_header(pkg, tmp_path):
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler to read the header with")
+    pairs = ((pkg._native.TqPlainTokens, "tq_plain_tokens"), (pkg._native.TqAttendRequest, "tq_attend_request"), (pkg._native.TqPackedStore, "tq_packed_store"))
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "tqamd.h"\nint main(void) {\n'
+                   + "".join(f'  printf("%zu ", sizeof({c}));\n' + "".join(f'  printf("%zu ", offsetof({c}, {f[0]}));\n' for f in py._fields_) for py, c in pairs) + "  return 0;\n}\n")
+    subprocess.run([gcc, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert out == [x for py, _ in pairs for x in (ctypes.sizeof(py), *(getattr(py, f[0]).offset for f in py._fields_))]

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
         left -= lds_found[1];
         agree = lds_found[2];
         lo += part << shift;
-        hi = min(hi, lo + ((1u << shift) - 1u));
+        hi = lo + min(hi - lo, (1u << shift) - 1u);         // (the last part may reach past the largest number there is)
         __syncthreads();
     }
     uint32_t border = lo;                                  // with left == agree all from lo on stay, with lo == hi the first `left` of them
