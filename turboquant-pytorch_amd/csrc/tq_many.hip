@@ -1,6 +1,7 @@
 // softmax(scale q K^T) V of any number of query tokens per sequence over a packed history, the window behind it and tokens that are in no
-// cache (drafts), with lengths and masks: tq_attend_many.  Launches: queries into the codec's space; packed tokens, a block a split of
-// them; uncompressed tokens; merge; and where the caller keeps count, what every key has received.
+// cache (drafts), with lengths and masks: tq_attend_many.  Launches, where a kernel with tables is built (fast): packed and uncompressed tokens, a block a split of a row's
+// packed ones (tq_many_fast.h); merge, unless every row is in one split; and where the caller keeps count, what every key has received.  Otherwise one more
+// each for the queries into the codec's space and for the uncompressed tokens (tq_many_kernel.h).
 #include "tq_many_kernel.h"
 
 namespace {

@@ -645,7 +645,8 @@ struct JoinArea {
     static __device__ __forceinline__ float *total(uint8_t *lds, uint32_t plain, uint32_t i) { return reinterpret_cast<float *>(lds + STATS + (2u * (plain * QT + i) + 1u) * 128u); }
 };
 
-// A row's uncompressed tokens against the block's tiles of queries, joined sums into LDS.  Two tiles share the waves where four of them hold all tokens.
+// A row's uncompressed tokens against the block's tiles of queries, joined sums into LDS.  Two tiles share the waves where four of them hold all tokens (128 of a window,
+// 8 x 4096 x 2048: the call 418 us against 453).
 template <int DP, int QT, int DT>
 __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, float (*lds_m)[32], float (*lds_l)[32], float *lds_wild, uint32_t row, uint32_t b, uint32_t tile0, uint32_t tiles,
                                             uint32_t length, uint32_t tid) {
@@ -752,9 +753,14 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 //   * weights times value norms are, as they lie, the B operand of the value product (its contraction runs over the tokens in the order in which a lane
 //     has them); A = values, every lane decoding its coordinates' bytes of eight tokens.
 // KT = 1: queries and levels as one fp16 value each, for bfloat16: the 2^-12 roundings move logits of some ten by 1e-3, where a bfloat16 result is rounded by up to 4e-3.
-// KT = 2: two terms each (three products, 22 bits), for float16, float32 and wherever sums of weights are kept; VT = 2: of weights and value levels as well, for float32.  Weights and value levels are one fp16 value each (the
-// reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's sum of weights is made of the rounded weights
-// themselves, so that their rounding cancels in part.
+// KT = 2: two terms each (three products, 22 bits), for float16, float32 and wherever sums of weights are kept; VT = 2: of weights and value levels as well, for float32.
+// Weights and value levels are otherwise one fp16 value each (the reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's
+// sum of weights is made of the rounded weights themselves, so that their rounding cancels in part.  KT = 2 for bfloat16 too would take 93 us instead of 77 (below), 628 instead of 426.
+// What bounds it: a wave's vector instructions (some 300 for 32 tokens x 64 queries, the exponentials fourfold) and its products (32 of 32 cycles) hardly overlap with two waves a
+// SIMD; four would have 128 registers each, and spill a hundred.  128 wide, 4 and 2 bits, 8 kv heads, us of this launch: 1 x 2048 tokens x 32 query vectors 12 (start 5, run 2, join 3);
+// 1 x 32768 x 256 65 (530 TFLOP/s); 16 x 8192 x 64 77 (450 TFLOP/s, 1.5 TB/s); 32 x 8192 x 4 for sums 84 (2.5 TB/s); with 4 and 4 bits 8 x 4096 x 2048 391 to 440 (400 TFLOP/s), a third
+// of it outside the loop (start, join, uncompressed tokens, way back).
+// Query operands stay in registers where they fit beside the sums (QREG): 131 us against 136 for the call with 32 x 8192 x 4, with two tiles of 128 wide queries they would spill.
 template <int DP, int IPBK, int IPBV, int QT, int KT, int VT>
 __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_kernel(TqManyArgs a) {
     using S = Shape<DP>;
@@ -1103,6 +1109,8 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 // here, columns tokens, so that a token's sum is made in its lane; rows in which a tile has no query are left out eight at a time.  Block = part of
 // a row's tokens, a wave takes 32 at a time and all tiles of queries in order (the first one's operands lie in LDS, a decode step has no more).
 // The first blocks are for the window's tokens: a wave 32 of them.
+// 128 wide, 4 bits, 8 kv heads x 4 query vectors: 32768 tokens 11 us, 32 sequences of 8192 59 us (155 MB, 2.6 TB/s): the two-term entries' reads (LDS busy 39 % of the
+// time) and the products hardly overlap.  Loads two runs ahead instead of one changed nothing, none ahead took 14 instead of 11 us.
 template <int DP, int DT>
 __device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t item, uint32_t lane) {
     if constexpr (DT == TQ_F32) plain_weights<TQ_F32>(a, item, DP / 16u, lane);
