@@ -756,8 +756,8 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 // KT = 2: two terms each (three products, 22 bits), for float16, float32 and wherever sums of weights are kept; VT = 2: of weights and value levels as well, for float32.
 // Weights and value levels are otherwise one fp16 value each (the reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's
 // sum of weights is made of the rounded weights themselves, so that their rounding cancels in part.  KT = 2 for bfloat16 too would take 93 us instead of 77 (below), 628 instead of 426.
-// What bounds it: a wave's vector instructions (some 300 for 32 tokens x 64 queries, the exponentials fourfold) and its products (32 of 32 cycles) hardly overlap with two waves a
-// SIMD; four would have 128 registers each, and spill a hundred.  128 wide, 4 and 2 bits, 8 kv heads, us of this launch: 1 x 2048 tokens x 32 query vectors 12 (start 5, run 2, join 3);
+// What bounds it: vector instructions and products, which hardly overlap (16 x 8192 x 64: vector 52 % of the cycles, 280 a run of 32 tokens; matrix 24 %, LDS 40 %; 8 x 4096 x 2048: 51, 22
+// and 28 %). Waves are not what is missing: twelve with 168 registers took 84 us instead of 78 for the former, sixteen with 128 spill a hundred and took 178. 128 wide, 4 and 2 bits, 8 kv heads, us of this launch: 1 x 2048 tokens x 32 query vectors 12 (start 5, run 2, join 3);
 // 1 x 32768 x 256 65 (530 TFLOP/s); 16 x 8192 x 64 77 (450 TFLOP/s, 1.5 TB/s); 32 x 8192 x 4 for sums 84 (2.5 TB/s); with 4 and 4 bits 8 x 4096 x 2048 391 to 440 (400 TFLOP/s), a third
 // of it outside the loop (start, join, uncompressed tokens, way back).
 // Query operands stay in registers where they fit beside the sums (QREG): 131 us against 136 for the call with 32 x 8192 x 4, with two tiles of 128 wide queries they would spill.
