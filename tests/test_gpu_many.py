@@ -297,6 +297,27 @@ def test_values_of_any_size(pkg):
             check(codec.attend_kv(q, ck, cv, lengths=lengths), q, K, V, seen)
 
 
+@pytest.mark.parametrize("D,kb,dtype", [(64, 2, BF), (64, 4, F16), (64, 8, BF), (128, 2, F16), (128, 4, BF), (128, 6, BF), (256, 2, BF), (256, 4, F16), (256, 8, BF), (128, 4, F32), (96, 4, BF)])
+@pytest.mark.parametrize("G,T", [(1, 1), (3, 1), (4, 4), (5, 3), (17, 1), (4, 9)])
+def test_sums_of_few_and_many_queries(pkg, G, T, D, kb, dtype):
+    """Up to 16 query vectors a row have a launch of their own; tokens that are not whole runs, a masked sequence, a window.  The bound of test_cross_against_float64."""
+    B, H, S, w = 2, 3, 611, 37
+    codec = pkg.TurboQuantV3(D, key_bits=kb, value_bits=2, residual_window=w, layer_idx=8, device=DEV)
+    ck, cv = codec.compress_kv(outlier_kv((B, H, S, D), seed=G, dtype=dtype).to(DEV), outlier_kv((B, H, S, D), seed=T, dtype=dtype).to(DEV))
+    K, V = (torch.cat((dequantised(comp, (c["compressed"]["idx_bytes"], c["compressed"]["vec_norms"])), c["fp16"].double()), 2)
+            for c, comp in ((ck, codec.key_compressor), (cv, codec.val_compressor)))
+    q = rand((B, H * G, T, D), D, dtype)
+    seen = torch.ones(B, S, dtype=torch.bool, device=DEV)
+    seen[1, ::3], seen[1, 590:] = False, False
+    prior = torch.rand(B, H, S, device=DEV)
+    sums = prior.clone()
+    _, p = check(codec.attend_kv(q, ck, cv, mask=seen, weights=sums), q, K, V, seen.view(B, 1, 1, 1, S))
+    reach = (2.0 ** -20 + D * 2.0 ** -24) * D ** -0.5 * (q.double().norm(dim=-1).reshape(B, H, -1).amax(-1) * K.norm(dim=-1).amax(-1)).unsqueeze(-1)
+    got = p.sum((2, 3))
+    assert bool(((sums.double() - prior.double() - got).abs() <= got * torch.expm1(2 * reach) + got * (T * G + 8) * 2.0 ** -24 + (prior + got) * 2.0 ** -23).all())
+    assert torch.equal(sums[1, :, ::3], prior[1, :, ::3]) and torch.equal(sums[1, :, 590:], prior[1, :, 590:])
+
+
 def test_tracked_attention_sums(pkg):
     """Sums of several steps, tokens going from the window into the packed store in between."""
     B, H, G, D = 2, 2, 4, 128

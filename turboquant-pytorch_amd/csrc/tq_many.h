@@ -55,6 +55,10 @@ constexpr float LOG2E = 1.44269504088896340736f;
 __host__ __device__ constexpr uint32_t q_operand_bytes(uint32_t dp) { return 2u * (dp / 16u) * 1024u; }
 __host__ __device__ constexpr uint32_t record_floats(uint32_t dp) { return 64u + 32u * dp; }
 
+// Whether the kept sums' launch works on 16 columns instead of 32: no more query vectors a row, and a window of 16-bit elements (float32's in three terms would spill beside two
+// blocks a compute unit)
+__host__ __device__ inline bool many_few(const TqManyArgs &a, uint32_t dp) { return a.M <= 16u && a.dtype != TQ_F32 && (dp == 64u || dp == 128u || dp == 256u); }
+
 // Row of a result register r of a 32 x 32 product in lane half h
 __device__ __forceinline__ constexpr uint32_t acc_row(int r, uint32_t h) { return 8u * (uint32_t)(r / 4) + 4u * h + (uint32_t)(r % 4); }
 

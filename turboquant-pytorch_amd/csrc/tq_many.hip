@@ -134,9 +134,12 @@ void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     if (a.tokens && plan.qt) {
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
-        // one block is resident per compute unit; the window's come first
+        // one block is resident per compute unit, or two where it has no more than 16 query vectors; the window's come first
         const uint32_t most = (a.tokens + 255u) / 256u, window = (a.rows * ((a.plain[0].n + 31u) / 32u) + 7u) / 8u;
-        uint32_t blocks = (uint32_t)cus > window + a.rows ? ((uint32_t)cus - window) / a.rows : 1u;
+        const uint32_t places = (uint32_t)cus * (many_few(a, DP) && DP != 256 ? 2u : 1u);
+        // (their places are kept where that takes an eighth of the others' at most: 8 rows of 32768 tokens, 9.7 us with 63 blocks a row and 10.1 with 64; 256 of 8192, 45.5 with 1, 40.9 with 2)
+        const uint32_t every = max(places / a.rows, 1u), fewer = places > window ? (places - window) / a.rows : 0u;
+        uint32_t blocks = 8u * fewer >= 7u * every ? fewer : every;
         if (blocks > most) blocks = most;
         const dim3 g(a.rows * blocks + window);
         const int ik = 8 / (int)a.bits_k;

@@ -1109,7 +1109,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
 // here, columns tokens, so that a token's sum is made in its lane; rows in which a tile has no query are left out eight at a time.  Block = part of
 // a row's tokens, a wave takes 32 at a time and all tiles of queries in order (the first one's operands lie in LDS, a decode step has no more).
 // The first blocks are for the window's tokens: a wave 32 of them.
-// 128 wide, 4 bits, 8 kv heads x 4 query vectors: 32768 tokens 11 us, 32 sequences of 8192 59 us (155 MB, 2.6 TB/s): the two-term entries' reads (LDS busy 39 % of the
+// 128 wide, 4 bits, 8 kv heads x 4 query vectors (before those had the kernel below): 32768 tokens 11 us, 32 sequences of 8192 59 us (155 MB, 2.6 TB/s): the two-term entries' reads (LDS busy 39 % of the
 // time) and the products hardly overlap.  Loads two runs ahead instead of one changed nothing, none ahead took 14 instead of 11 us.
 template <int DP, int DT>
 __device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t item, uint32_t lane) {
@@ -1255,8 +1255,112 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     }
 }
 
+// The same for at most 16 query vectors a row (a decode step has no more): products of 16 x 16 with twice the contraction, so that half as many of their columns are empty, and
+// the queries' operands stay in registers.  Lane (n = lane % 16, kg = lane / 16) has coordinates kg * DP / 4 ... of query n and of tokens n and 16 + n of a run; the sums of a token
+// over the queries 4 kg ... + 3 lie in its four lanes.  Two blocks a compute unit, 256 wide (registers) one.
+// 128 wide, 4 bits, 8 kv heads x 4 query vectors: 32768 tokens 9.7 us (11.5 by the kernel above), 32 sequences of 8192 41 us (59), 155 MB at 3.8 TB/s.
+template <int DP, int IPBK>
+__global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) void tq_many_few_weights_kernel(TqManyArgs a, uint32_t blocks) {
+    const uint32_t items = a.rows * ((a.plain[0].n + 31u) / 32u), first = (items + FAST_WAVES - 1u) / FAST_WAVES;
+    if (blockIdx.x < first) {
+        const uint32_t item = blockIdx.x * FAST_WAVES + tq_uniform32(threadIdx.x >> 6);
+        if (item >= items) return;
+        if (a.dtype == TQ_BF16) window_weights<DP, TQ_BF16>(a, item, threadIdx.x & 63u);
+        else window_weights<DP, TQ_F16>(a, item, threadIdx.x & 63u);
+        return;
+    }
+    constexpr int STEPS = DP / 32, KW = DP / 16 / IPBK;                // steps of eight coordinates of a lane, words of its packed bytes a token
+    constexpr uint32_t GB = DP / IPBK;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[65536];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 15u, kg = lane >> 4;
+    const uint32_t block = blockIdx.x - first, row = block / blocks, b = row / a.heads;
+    const uint32_t seen = min(a.tokens, many_length(a, b));
+    {
+        Lut2<IPBK> table;
+        table.load(a.table_k, a.bits_k, DP, tid);
+        table.store(lds, tid);
+        table.store(lds + 128, tid);
+    }
+    tq_u4 q[2][STEPS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+            q[t][s] = tq_gload16(a.q_op + (size_t)row * q_operand_bytes(DP) + ((t * (DP / 16) + (kg & 1u) * STEPS + s) * 64u + (kg >> 1) * 32u + n) * 16u);
+    const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (size_t)row * 64u + 4u * kg;
+    tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (4u * kg + r >= a.M) { m[r] = -MANY_NONE; inv[r] = 0.f; }
+    const float q_scale = a.q_scale[row];
+    const uint32_t slot = (lane & (64u / IPBK - 1u)) * 4u * IPBK;
+    __syncthreads();
+    const size_t slot0 = (size_t)row * a.packed_row_stride;
+    const uint32_t last = a.tokens - 32u, step = 32u * FAST_WAVES * blocks;
+    float *const sums = a.weights + (long long)row * a.w_stride;
+    uint32_t raw[2][KW];
+    uint16_t norm_raw[2] = {0, 0};
+    float before_raw = 0.f;
+    auto issue = [&](uint32_t t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint8_t *p = a.k_idx + (slot0 + t + 16u * i + n) * GB + kg * (GB / 4u);
+            if constexpr (KW == 1) raw[i][0] = tq_gload4(p);
+            else if constexpr (KW == 2) { const tq_u2 v = tq_gload8(p); raw[i][0] = v[0]; raw[i][KW > 1 ? 1 : 0] = v[1]; }
+            else {
+#pragma unroll
+                for (int k = 0; k < KW / 4; ++k) {
+                    const tq_u4 v = tq_gload16(p + 16 * k);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) raw[i][4 * k + j] = v[j];
+                }
+            }
+            norm_raw[i] = tq_gload2(a.k_norms + slot0 + t + 16u * i + n);
+        }
+        before_raw = *((const TQ_GLOBAL float *)sums + t + (lane & 31u));
+    };
+    uint32_t t_next = 32u * ((block - row * blocks) * FAST_WAVES + wave);
+    if (t_next < seen) issue(min(t_next, last));
+    while (t_next < seen) {
+        const uint32_t t_run = t_next, t0 = min(t_run, last), t = t0 + (lane & 31u);
+        t_next += step;
+        const bool counts = lane < 32u && t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
+        const float before = before_raw, kn[2] = {(float)__builtin_bit_cast(_Float16, norm_raw[0]) * q_scale, (float)__builtin_bit_cast(_Float16, norm_raw[1]) * q_scale};
+        uint32_t now[2][KW];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < KW; ++k) now[i][k] = raw[i][k];
+        if (t_next < seen) issue(min(t_next, last));
+        float w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            tq_f4v s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                tq_u4 hi, lo;
+                decode_keys2<IPBK, KW>(now[i], st, lds, slot, hi, lo);
+                s = mfma16_f16(q[0][st], hi, s);
+                s = mfma16_f16(q[1][st], hi, s);
+                s = mfma16_f16(q[0][st], lo, s);
+            }
+            w[i] = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], kn[i], -m[r])), inv[r], w[i]);
+            w[i] = reduce_rows(w[i], OpAdd());
+        }
+        if (counts) *((TQ_GLOBAL float *)sums + t) = before + (lane & 16u ? w[1] : w[0]);
+    }
+}
+
 template <int DP, int IPBK>
 int launch_many_weights(dim3 grid, hipStream_t s, const TqManyArgs &a, uint32_t blocks) {
+    if constexpr (Shape<DP>::EVEN) {
+        if (many_few(a, DP)) {
+            hipLaunchKernelGGL((tq_many_few_weights_kernel<DP, IPBK>), grid, dim3(FAST_THREADS), 0, s, a, blocks);
+            return 0;
+        }
+    }
     hipLaunchKernelGGL((tq_many_weights_kernel<DP, IPBK>), grid, dim3(FAST_THREADS), 0, s, a, blocks);
     return 0;
 }
