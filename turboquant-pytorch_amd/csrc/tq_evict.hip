@@ -47,9 +47,9 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
     return before + x - v;
 }
 
-// Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens; E = 0: of more, read again for every pass (the call, 8 rows of 32768: 30 us
-// with E = 32, 54 with 0; 128 of 8191: 44 with 16, 48 with 32, 49 with 0; 8 of 1152: 18 with 4, 23 with 32).  Bound by its own steps one after the other: 10, 20 and 13 us for 4 KB,
-// 128 KB and 32 KB a row.
+// Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens; E = 0: of more, read again for every pass, 32 loads of a thread under way (the call,
+// 8 rows of 32768: 30 us with E = 32, 41 with 0; 128 of 8191: 45 with 16, 48 with 32, 58 with 0; 8 of 1152: 18 with 4, 24 with 32). Bound by its own steps one after the other: 10, 20 and
+// 13 us for 4 KB, 128 KB and 32 KB a row; E = 0 by the instructions of one compute unit a row: 8 rows of 131072 133 us, one of 2^20 794.
 // The keep-th largest weight lies in a range of whole numbers, at first all there are.  While more than 256 tokens lie in it, it is cut into 2048 parts, the tokens of each are counted
 // in LDS, and the part with the keep-th one is the next range: a floating-point number's bits go with its logarithm, so that sums spread over the parts and few of the
 // counts' atomics meet (counting by the leading byte instead took 110 us for 8 x 32768 tokens; those at the lower end, zeros, are counted by ballots).
@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
 // from counts per wave and register, in the tokens' order.
 template <int E>
 __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictArgs a) {
-    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048, FEW = 256;
+    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048, FEW = 256, AHEAD = 32;        // AHEAD: loads of a thread under way
     __shared__ __attribute__((aligned(16))) uint32_t lds_few[FEW + 4];
     __shared__ uint32_t lds_part[PARTS], lds_count[WAVES], lds_ends[2][WAVES], lds_place[E ? E * WAVES : 1], lds_found[3], lds_n;
     const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6);
@@ -68,12 +68,12 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
 #pragma unroll
             for (int e = 0; e < E; ++e) f(key[e]);
         } else {
-            for (uint32_t i0 = 0; i0 < a.tokens; i0 += 8u * SELECT_THREADS) {
-                float v[8];
+            for (uint32_t i0 = 0; i0 < a.tokens; i0 += AHEAD * SELECT_THREADS) {
+                float v[AHEAD];
 #pragma unroll
-                for (uint32_t k = 0; k < 8u; ++k) v[k] = w[min(i0 + k * SELECT_THREADS + tid, a.tokens - 1u)];
+                for (uint32_t k = 0; k < AHEAD; ++k) v[k] = w[min(i0 + k * SELECT_THREADS + tid, a.tokens - 1u)];
 #pragma unroll
-                for (uint32_t k = 0; k < 8u; ++k) f(i0 + k * SELECT_THREADS + tid < a.tokens ? order_of(v[k]) : 0u);
+                for (uint32_t k = 0; k < AHEAD; ++k) f(i0 + k * SELECT_THREADS + tid < a.tokens ? order_of(v[k]) : 0u);
             }
         }
     };
@@ -158,30 +158,38 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
     // ---- places
     TQ_GLOBAL long long *kept = (TQ_GLOBAL long long *)a.kept + (long long)row * a.keep;
     auto before_lane = [&](unsigned long long m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
-    if constexpr (E == 0) {                                // eight tokens in a row a thread
-        uint32_t out = 0u, equal = 0u;                     // over the tokens before this round
-        for (uint32_t i0 = 0; i0 < a.tokens; i0 += 8u * SELECT_THREADS) {
-            uint32_t k8[8], same = 0u, more = 0u;
+    if constexpr (E == 0) {                                // a sixteenth of the tokens a wave: counted, then written
+        const uint32_t part = (a.tokens + WAVES * 64u - 1u) / (WAVES * 64u) * 64u, begin = min(a.tokens, wave * part), end = min(a.tokens, begin + part);
+        const uint32_t limit = left < agree ? left : 0xffffffffu;               // of those equal to the border
+        auto tokens = [&](auto f) __attribute__((always_inline)) {               // f(token of this lane, key) of 64 at a time, in order
+            for (uint32_t i0 = begin; i0 < end; i0 += AHEAD * 64u) {
+                float v[AHEAD];
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k) {
-                const uint32_t i = i0 + 8u * tid + k;
-                k8[k] = i < a.tokens ? order_of(w[i]) : 0u;
-                same += k8[k] == border ? 1u : 0u;
+                for (uint32_t k = 0; k < AHEAD; ++k) v[k] = w[min(i0 + k * 64u + lane, a.tokens - 1u)];
+#pragma unroll
+                for (uint32_t k = 0; k < AHEAD; ++k) f(i0 + k * 64u + lane, i0 + k * 64u + lane < end ? order_of(v[k]) : 0u);
             }
-            uint32_t all;
-            uint32_t rank = equal + block_scan(same, lds_count, all);
-            equal += all;
+        };
+        uint32_t more = 0u, same = 0u;
+        tokens([&](uint32_t, uint32_t k) {
+            more += (uint32_t)__popcll(__ballot(k > border));
+            same += (uint32_t)__popcll(__ballot(k == border));
+        });
+        if (lane == 0u) { lds_ends[0][wave] = more; lds_ends[1][wave] = same; }
+        __syncthreads();
+        uint32_t out = 0u, equal = 0u;
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k) {
-                if (k8[k] == border && rank++ >= left && left < agree) k8[k] = 0u;
-                more += k8[k] >= border ? 1u : 0u;
-            }
-            uint32_t at = out + block_scan(more, lds_count, all);
-            out += all;
-#pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k)
-                if (k8[k] >= border) kept[at++] = i0 + 8u * tid + k;
-        }
+        for (uint32_t k = 0; k < WAVES; ++k)
+            if (k < wave) { out += lds_ends[0][k]; equal += lds_ends[1][k]; }
+        out += min(equal, limit);
+        tokens([&](uint32_t i, uint32_t k) {
+            const unsigned long long equals = __ballot(k == border);
+            const bool stays = k > border || (k == border && equal + before_lane(equals) < limit);
+            const unsigned long long staying = __ballot(stays);
+            if (stays) kept[out + before_lane(staying)] = i;
+            equal += (uint32_t)__popcll(equals);
+            out += (uint32_t)__popcll(staying);
+        });
         return;
     } else {
     auto scan = [&]() {                                    // lds_place, [register][wave]: counts -> sums of those before
