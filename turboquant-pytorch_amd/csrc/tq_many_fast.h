@@ -307,7 +307,7 @@ struct Rotate {
 // 32 uncompressed tokens of a row (`which`: 0 the window, 1 the drafts; from t0 on) against a tile of queries: raw 16-bit products are exact, weights enter the value
 // product as three bf16 terms, or two fp16 ones.  Coordinates of the sums as in the packed loop: row r of acc[c] is coordinate NC r + c.  Infinite and NaN
 // values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); `wild` says whether there are any.
-// Up to 128 wide the tokens stay in registers from one tile of queries to the next (HELD), at 256 they are read as they are needed.
+// Up to 128 wide all loads of the 32 tokens are under way at once (HELD), at 256 they would not fit into registers and are issued as they are needed.
 template <int DP, int DT>
 struct PlainTile {
     static constexpr bool BF = DT == TQ_BF16, EVEN = Shape<DP>::EVEN;
