@@ -503,6 +503,7 @@ int tq_attend_many(const tq_attend_request *request, float *scratch, long long s
  *   weights     [rows, weights_stride] float32: the packed tokens', then `rest` of tokens that all stay (at most 65536)
  *   weights_out [rows, weights_out_stride]: the weights of what stays, keep + rest a row
  *   kept        [rows, keep] slot in `from` of every slot of `to`, ascending
+ *   scratch     tq_evict_scratch(rows, tokens) words, none (NULL) up to 32768 tokens; not shared by launches that can overlap in time
  */
 typedef struct tq_packed_store {
     uint8_t *k_idx;
@@ -512,7 +513,9 @@ typedef struct tq_packed_store {
     long long packed_row_stride;
 } tq_packed_store;
 int tq_evict(const tq_packed_store *from, const tq_packed_store *to, const float *weights, long long weights_stride, float *weights_out,
-             long long weights_out_stride, long long rest, long long rows, long long tokens, long long keep, int head_dim, int bits_k, int bits_v, long long *kept, void *stream);
+             long long weights_out_stride, long long rest, long long rows, long long tokens, long long keep, int head_dim, int bits_k, int bits_v, long long *kept, uint32_t *scratch,
+             long long scratch_words, void *stream);
+long long tq_evict_scratch(long long rows, long long tokens);
 
 #ifdef __cplusplus
 }

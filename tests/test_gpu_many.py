@@ -388,7 +388,7 @@ def test_evict_keeps_the_largest(pkg, B, H, n, w, keep, D, dtype, kb, vb):
     assert torch.equal(everything[3], torch.arange(n, device=DEV).expand(B, H, n)) and torch.equal(everything[0]["compressed"]["idx_bytes"], ck["compressed"]["idx_bytes"])
 
 
-@pytest.mark.parametrize("n,keep", [(2000, 100), (3000, 1700), (40000, 300)])
+@pytest.mark.parametrize("n,keep", [(2000, 100), (3000, 1700), (40000, 300), (1100003, 400000)])
 def test_evict_of_weights_that_lie_close(pkg, n, keep):
     """More NaN than stay above numbers anywhere (the range of what is searched ends at the largest whole number), neighbours among float32, a few values many times."""
     codec = pkg.TurboQuantV3(64, key_bits=2, value_bits=2, residual_window=0, layer_idx=8, device=DEV)

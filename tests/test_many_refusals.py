@@ -64,8 +64,8 @@ def test_evict_entry_point_checks_its_arguments(pkg):
     native = pkg._native
     L = native.lib()
     full = native.TqPackedStore(4096, 4096, 4096, 4096, 0)
-    call = lambda frm=full, to=full, w=4096, ws=300, wo=4096, wos=300, rest=5, rows=2, tokens=100, keep=50, D=128, bk=4, bv=2, kept=4096: L.tq_evict(  # noqa: E731
-        ctypes.byref(frm) if frm is not None else None, ctypes.byref(to) if to is not None else None, w, ws, wo, wos, rest, rows, tokens, keep, D, bk, bv, kept, None)
+    call = lambda frm=full, to=full, w=4096, ws=300, wo=4096, wos=300, rest=5, rows=2, tokens=100, keep=50, D=128, bk=4, bv=2, kept=4096, scratch=None, words=0: L.tq_evict(  # noqa: E731
+        ctypes.byref(frm) if frm is not None else None, ctypes.byref(to) if to is not None else None, w, ws, wo, wos, rest, rows, tokens, keep, D, bk, bv, kept, scratch, words, None)
     assert call(frm=None) == -1 and call(to=None) == -1 and call(w=None) == -1 and call(wo=None) == -1 and call(kept=None) == -1
     assert call(bk=0) == -2 and call(bv=9) == -2 and call(D=7) == -3 and call(D=300) == -3
     for bad in ({"rows": -1}, {"tokens": -1}, {"keep": -1}, {"keep": 101}, {"rest": -1}, {"rest": 65537}, {"ws": 104}, {"wos": 54}, {"rows": 1 << 31},
@@ -75,6 +75,10 @@ def test_evict_entry_point_checks_its_arguments(pkg):
     assert call(w=4098) == -8 and call(wo=4098) == -8 and call(kept=4100) == -8 and call(frm=native.TqPackedStore(4096, 4097, 4096, 4096, 0)) == -8
     assert call(frm=native.TqPackedStore(4096, 4096, None, 4096, 0)) == -1 and call(to=native.TqPackedStore(None, 4096, 4096, 4096, 0)) == -1
     assert call(rows=0) == 0 and call(keep=0, rest=0) == 0
+    need = L.tq_evict_scratch(2, 40000)
+    assert need > 0 and L.tq_evict_scratch(2, 32768) == 0 and L.tq_evict_scratch(-1, 40000) == -5 and L.tq_evict_scratch(1, 1 << 31) == -5
+    long_rows = {"tokens": 40000, "ws": 50000}
+    assert call(**long_rows) == -1 and call(**long_rows, scratch=4096, words=need - 1) == -10 and call(**long_rows, scratch=4098, words=need) == -8
 
 
 def test_cpu_tensors_are_refused(pkg):

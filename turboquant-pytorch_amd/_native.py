@@ -23,7 +23,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libtqamd.so")
 FAST_NAME = "tqamd_fastcall"        # extension module: the eager calls from tensors to the library in one step each
 FAST_SOURCE = "tq_fastcall.cpp"
-FAST_INTERFACE = 4                  # INTERFACE there: what init and the functions take and answer
+FAST_INTERFACE = 5                  # INTERFACE there: what init and the functions take and answer
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
@@ -232,7 +232,7 @@ EXPORTS = (
     "tq_attend_prepare", "tq_attend_merge", "tq_append_token", "tq_attend_step",
     "tq_decode_supported", "tq_decode_scratch_floats", "tq_decode_attend", "tq_decode_attend_spread", "tq_decode_attend_cached", "tq_decode_streams", "tq_decode_append",
     "tq_compress_layer", "tq_restore_layer",
-    "tq_attend_many_scratch", "tq_attend_many", "tq_evict",
+    "tq_attend_many_scratch", "tq_attend_many", "tq_evict", "tq_evict_scratch",
 )
 
 _lib = None
@@ -298,9 +298,11 @@ def lib() -> ctypes.CDLL:
     L.tq_attend_many_scratch.restype = ll
     L.tq_attend_many_scratch.argtypes = [vp]
     L.tq_attend_many.argtypes = [vp, vp, ll, vp]
-    L.tq_evict.argtypes = [vp, vp, vp, ll, vp, ll, ll, ll, ll, ll, ci, ci, ci, vp, vp]
+    L.tq_evict.argtypes = [vp, vp, vp, ll, vp, ll, ll, ll, ll, ll, ci, ci, ci, vp, vp, ll, vp]
+    L.tq_evict_scratch.restype = ll
+    L.tq_evict_scratch.argtypes = [ll, ll]
     for name in EXPORTS:
-        if name not in ("tq_attend_many_scratch", "tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
+        if name not in ("tq_attend_many_scratch", "tq_evict_scratch", "tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
             getattr(L, name).restype = ci
     _lib = L
     return L
@@ -331,7 +333,7 @@ def fast():
         if getattr(module, "interface", None) != FAST_INTERFACE:       # (modules of before had none)
             raise TqError(f"{path} was built from another state of {FAST_SOURCE}: {how}")
         entries = ("tq_compress", "tq_decompress", "tq_compress_layer", "tq_restore_layer", "tq_decode_append", "tq_decode_attend_cached", "tq_qjl_compress", "tq_qjl_query_scores",
-                   "tq_attend_many_scratch", "tq_attend_many", "tq_evict")
+                   "tq_attend_many_scratch", "tq_attend_many", "tq_evict", "tq_evict_scratch")
         module.init(tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in entries), _workspace, _drop_workspace, _step_scratch, _arrived, _TABLE_TAG)
         _fast = module
     return _fast
@@ -912,8 +914,10 @@ def evict(packed, tokens: int, bits, D: int, weights: torch.Tensor, keep: int, i
         kept = torch.empty((B, H, keep), dtype=torch.int64, device=dev)
         store = lambda p, stride: TqPackedStore(p[0][0].data_ptr(), p[0][1].data_ptr(), p[1][0].data_ptr(), p[1][1].data_ptr(), stride)  # noqa: E731
         source, target = store(pairs, prs), store(into, into[0][0].shape[2])
+        words = int(lib().tq_evict_scratch(B * H, tokens))
+        scratch = torch.empty(words, dtype=torch.int32, device=dev) if words else None
         check(lib().tq_evict(ctypes.byref(source), ctypes.byref(target), weights.data_ptr(), sh if H > 1 else sb, weights_into.data_ptr(), weights_into.shape[2], rest,
-                             B * H, tokens, keep, D, *bits, kept.data_ptr(), _stream_handle(dev)), "tq_evict")
+                             B * H, tokens, keep, D, *bits, kept.data_ptr(), 0 if scratch is None else scratch.data_ptr(), words, _stream_handle(dev)), "tq_evict")
     return into, weights_into, kept
 
 

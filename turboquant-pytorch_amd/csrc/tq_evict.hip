@@ -1,5 +1,5 @@
 // Of every row of a packed store the `keep` tokens with the largest weights, in their order, into another store: tq_evict.
-// Two launches: which tokens stay (a block a row), and their bytes.
+// Two launches: which tokens stay (a block a row), and their bytes; of rows of more than 32768 tokens, five: a block a segment.
 #include "tq_device.h"
 
 namespace {
@@ -16,6 +16,8 @@ struct EvictArgs {
     uint16_t *norms_out[2];
     long long w_stride, w_out_stride, row_stride, out_stride;
     uint32_t rows, tokens, keep, rest, bytes[2], unit[2];
+    uint32_t *scratch;               // of rows of more than 32768 tokens: [rows][3 rounds][segments][2048] counts, [rows][segments] states
+    uint32_t segments, segment_tokens;
 };
 
 // Weights as whole numbers of the same order: NaN above everything, the two zeros equal.
@@ -47,9 +49,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
     return before + x - v;
 }
 
-// Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens; E = 0: of more, read again for every pass, 32 loads of a thread under way (the call,
-// 8 rows of 32768: 30 us with E = 32, 41 with 0; 128 of 8191: 45 with 16, 48 with 32, 58 with 0; 8 of 1152: 18 with 4, 24 with 32). Bound by its own steps one after the other: 10, 20 and
-// 13 us for 4 KB, 128 KB and 32 KB a row; E = 0 by the instructions of one compute unit a row: 8 rows of 131072 133 us, one of 2^20 794.
+// Block = row, its weights in registers (E a thread, token e * 1024 + thread), up to 32768 tokens (the call, 8 rows of 32768: 30 us; 128 of 8191: 45 with E = 16, 48 with 32;
+// 8 of 1152: 18 with 4, 24 with 32). Bound by its own steps one after the other: 10, 20 and 13 us for 4 KB, 128 KB and 32 KB a row.
 // The keep-th largest weight lies in a range of whole numbers, at first all there are.  While more than 256 tokens lie in it, it is cut into 2048 parts, the tokens of each are counted
 // in LDS, and the part with the keep-th one is the next range: a floating-point number's bits go with its logarithm, so that sums spread over the parts and few of the
 // counts' atomics meet (counting by the leading byte instead took 110 us for 8 x 32768 tokens; those at the lower end, zeros, are counted by ballots).
@@ -57,27 +58,17 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32
 // from counts per wave and register, in the tokens' order.
 template <int E>
 __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictArgs a) {
-    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048, FEW = 256, AHEAD = 32;        // AHEAD: loads of a thread under way
+    constexpr uint32_t WAVES = SELECT_THREADS / 64, PARTS = 2048, FEW = 256;
     __shared__ __attribute__((aligned(16))) uint32_t lds_few[FEW + 4];
-    __shared__ uint32_t lds_part[PARTS], lds_count[WAVES], lds_ends[2][WAVES], lds_place[E ? E * WAVES : 1], lds_found[3], lds_n;
+    __shared__ uint32_t lds_part[PARTS], lds_count[WAVES], lds_ends[2][WAVES], lds_place[E * WAVES], lds_found[3], lds_n;
     const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6);
     const TQ_GLOBAL float *w = (const TQ_GLOBAL float *)a.weights + (long long)row * a.w_stride;
-    uint32_t key[E ? E : 1], lo = 0xffffffffu, hi = 0u;           // a token that is none: 0, less than any number's
+    uint32_t key[E], lo = 0xffffffffu, hi = 0u;           // a token that is none: 0, less than any number's
     auto each = [&](auto f) __attribute__((always_inline)) {      // f(key) of all tokens, by all threads together
-        if constexpr (E) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) f(key[e]);
-        } else {
-            for (uint32_t i0 = 0; i0 < a.tokens; i0 += AHEAD * SELECT_THREADS) {
-                float v[AHEAD];
-#pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) v[k] = w[min(i0 + k * SELECT_THREADS + tid, a.tokens - 1u)];
-#pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) f(i0 + k * SELECT_THREADS + tid < a.tokens ? order_of(v[k]) : 0u);
-            }
-        }
+        for (int e = 0; e < E; ++e) f(key[e]);
     };
-    if constexpr (E) {
+    {
         constexpr int CH = E < 16 ? E : 16;
 #pragma unroll
         for (int e0 = 0; e0 < E; e0 += CH) {
@@ -158,40 +149,6 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
     // ---- places
     TQ_GLOBAL long long *kept = (TQ_GLOBAL long long *)a.kept + (long long)row * a.keep;
     auto before_lane = [&](unsigned long long m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
-    if constexpr (E == 0) {                                // a sixteenth of the tokens a wave: counted, then written
-        const uint32_t part = (a.tokens + WAVES * 64u - 1u) / (WAVES * 64u) * 64u, begin = min(a.tokens, wave * part), end = min(a.tokens, begin + part);
-        const uint32_t limit = left < agree ? left : 0xffffffffu;               // of those equal to the border
-        auto tokens = [&](auto f) __attribute__((always_inline)) {               // f(token of this lane, key) of 64 at a time, in order
-            for (uint32_t i0 = begin; i0 < end; i0 += AHEAD * 64u) {
-                float v[AHEAD];
-#pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) v[k] = w[min(i0 + k * 64u + lane, a.tokens - 1u)];
-#pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) f(i0 + k * 64u + lane, i0 + k * 64u + lane < end ? order_of(v[k]) : 0u);
-            }
-        };
-        uint32_t more = 0u, same = 0u;
-        tokens([&](uint32_t, uint32_t k) {
-            more += (uint32_t)__popcll(__ballot(k > border));
-            same += (uint32_t)__popcll(__ballot(k == border));
-        });
-        if (lane == 0u) { lds_ends[0][wave] = more; lds_ends[1][wave] = same; }
-        __syncthreads();
-        uint32_t out = 0u, equal = 0u;
-#pragma unroll
-        for (uint32_t k = 0; k < WAVES; ++k)
-            if (k < wave) { out += lds_ends[0][k]; equal += lds_ends[1][k]; }
-        out += min(equal, limit);
-        tokens([&](uint32_t i, uint32_t k) {
-            const unsigned long long equals = __ballot(k == border);
-            const bool stays = k > border || (k == border && equal + before_lane(equals) < limit);
-            const unsigned long long staying = __ballot(stays);
-            if (stays) kept[out + before_lane(staying)] = i;
-            equal += (uint32_t)__popcll(equals);
-            out += (uint32_t)__popcll(staying);
-        });
-        return;
-    } else {
     auto scan = [&]() {                                    // lds_place, [register][wave]: counts -> sums of those before
         __syncthreads();
         uint32_t all;
@@ -228,7 +185,145 @@ __global__ __launch_bounds__(SELECT_THREADS) void tq_evict_select_kernel(EvictAr
         const uint32_t at = lds_place[e * WAVES + wave] + before_lane(__ballot(stays));
         if (stays) kept[at] = e * SELECT_THREADS + tid;
     }
+}
+
+// ---- rows of more than 32768 tokens -----------------------------------------------------------------------------------------
+// Block (row, segment of its tokens); three launches that count the 2048 values of the next eleven bits (ten at last) among the segment's tokens that
+// agree with the border so far, and one that writes places. Each begins with what the counts before it say: the border's next digit, and how many tokens of the segments before
+// its own lie above it (a thread adds two digits over all segments). Counts are whole numbers and every block finds the same border: nothing depends on an order.
+// The call: 8 rows of 131072 tokens 63 us (a block a row, its weights read again for every pass: 133), one of 2^20 82 (794), 8 of 40000 42 (61); up to 32768 tokens the kernel above is
+// the faster one (8 of 32768 29 us).  Bound by the chain of five launches, and for many rows by the bytes that are moved.
+constexpr uint32_t LONG_DIGITS = 2048, LONG_SEGMENTS = 64, LONG_SEGMENT = 16384, LONG_AHEAD = 16;      // LONG_AHEAD: loads of a thread under way
+
+struct LongState { uint32_t prefix, left, agree, before; };        // border's bits so far, tokens that stay of the `agree` that have them, tokens above it in the segments before
+
+__device__ __forceinline__ uint32_t long_digit(uint32_t key, int round) { return round == 0 ? key >> 21 : round == 1 ? (key >> 10) & 2047u : key & 1023u; }
+
+// What round's counts say; equal: of the segments before, tokens that have the border's bits
+__device__ __forceinline__ LongState long_settle(const EvictArgs &a, int round, LongState was, uint32_t row, uint32_t segment, uint32_t *lds, uint32_t *lds_found, uint32_t &equal) {
+    const uint32_t tid = threadIdx.x, p1 = LONG_DIGITS - 1u - 2u * tid;
+    const TQ_GLOBAL uint32_t *counts = (const TQ_GLOBAL uint32_t *)a.scratch + ((size_t)row * 3u + round) * a.segments * LONG_DIGITS + (p1 - 1u);
+    uint32_t c0 = 0u, c1 = 0u, b0 = 0u, b1 = 0u;
+#pragma unroll 8
+    for (uint32_t s = 0; s < a.segments; ++s) {
+        const uint32_t x0 = counts[s * LONG_DIGITS], x1 = counts[s * LONG_DIGITS + 1u];
+        c0 += x0; c1 += x1;
+        b0 += s < segment ? x0 : 0u; b1 += s < segment ? x1 : 0u;
     }
+    uint32_t all;
+    const uint32_t above = block_scan(c1 + c0, lds, all), before = block_scan(b1 + b0, lds, all);
+    if (above < was.left && above + c1 + c0 >= was.left) {
+        const bool upper = above + c1 >= was.left;
+        lds_found[0] = upper ? p1 : p1 - 1u;
+        lds_found[1] = upper ? above : above + c1;
+        lds_found[2] = upper ? c1 : c0;
+        lds_found[3] = upper ? before : before + b1;
+        lds_found[4] = upper ? b1 : b0;
+    }
+    __syncthreads();
+    equal = lds_found[4];
+    return LongState{round == 0 ? lds_found[0] : (was.prefix << (round == 1 ? 11 : 10)) | lds_found[0], was.left - lds_found[1], lds_found[2], was.before + lds_found[3]};
+}
+
+__device__ __forceinline__ TQ_GLOBAL uint32_t *long_state(const EvictArgs &a, uint32_t row, uint32_t segment) {
+    return (TQ_GLOBAL uint32_t *)a.scratch + (size_t)a.rows * 3u * a.segments * LONG_DIGITS + ((size_t)row * a.segments + segment) * 4u;
+}
+
+template <int ROUND>
+__device__ __forceinline__ LongState long_now(const EvictArgs &a, uint32_t row, uint32_t segment, uint32_t *lds, uint32_t *lds_found, uint32_t &equal) {
+    LongState was = {0u, a.keep, a.tokens, 0u};
+    equal = 0u;
+    if constexpr (ROUND > 0) {
+        const TQ_GLOBAL uint32_t *state = long_state(a, row, segment);
+        if constexpr (ROUND > 1) was = LongState{state[0], state[1], state[2], state[3]};
+        was = long_settle(a, ROUND - 1, was, row, segment, lds, lds_found, equal);
+    }
+    return was;
+}
+
+template <int ROUND>
+__global__ __launch_bounds__(SELECT_THREADS) void tq_evict_count_kernel(EvictArgs a) {
+    __shared__ uint32_t lds_part[LONG_DIGITS], lds_scan[SELECT_THREADS / 64], lds_found[5];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, row = blockIdx.x / a.segments, segment = blockIdx.x - row * a.segments;
+    const uint32_t begin = segment * a.segment_tokens, end = min(a.tokens, begin + a.segment_tokens);
+    lds_part[tid] = lds_part[tid + SELECT_THREADS] = 0u;
+    uint32_t equal;
+    const LongState now = long_now<ROUND>(a, row, segment, lds_scan, lds_found, equal);
+    if (ROUND > 0 && tid == 0u) {
+        TQ_GLOBAL uint32_t *state = long_state(a, row, segment);
+        state[0] = now.prefix; state[1] = now.left; state[2] = now.agree; state[3] = now.before;
+    }
+    __syncthreads();
+    const TQ_GLOBAL float *w = (const TQ_GLOBAL float *)a.weights + (long long)row * a.w_stride;
+    for (uint32_t i0 = begin; i0 < end; i0 += LONG_AHEAD * SELECT_THREADS) {
+        float v[LONG_AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < LONG_AHEAD; ++k) v[k] = w[min(i0 + k * SELECT_THREADS + tid, a.tokens - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < LONG_AHEAD; ++k) {
+            const uint32_t key = order_of(v[k]), digit = long_digit(key, ROUND);
+            const bool counts = i0 + k * SELECT_THREADS + tid < end && (ROUND == 0 || key >> (ROUND == 1 ? 21 : 10) == now.prefix);
+            const unsigned long long who = __ballot(counts);
+            if (!who) continue;
+            const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)digit, (int)__builtin_ctzll(who));
+            if (__ballot(counts && digit == first) == who) {                       // (one value for all, as of tokens that have received nothing: no 64 additions to one place)
+                if (lane == 0u) atomicAdd(&lds_part[first], (uint32_t)__popcll(who));
+            } else if (counts) atomicAdd(&lds_part[digit], 1u);
+        }
+    }
+    __syncthreads();
+    TQ_GLOBAL uint32_t *out = (TQ_GLOBAL uint32_t *)a.scratch + (((size_t)row * 3u + ROUND) * a.segments + segment) * LONG_DIGITS;
+    out[tid] = lds_part[tid];
+    out[tid + SELECT_THREADS] = lds_part[tid + SELECT_THREADS];
+}
+
+// A sixteenth of the segment a wave: counted, then written
+__global__ __launch_bounds__(SELECT_THREADS) void tq_evict_place_kernel(EvictArgs a) {
+    constexpr uint32_t WAVES = SELECT_THREADS / 64;
+    __shared__ uint32_t lds_scan[WAVES], lds_found[5], lds_more[2][WAVES];
+    const uint32_t lane = threadIdx.x & 63u, wave = tq_uniform32(threadIdx.x >> 6), row = blockIdx.x / a.segments, segment = blockIdx.x - row * a.segments;
+    uint32_t equal;
+    const LongState now = long_now<3>(a, row, segment, lds_scan, lds_found, equal);
+    const uint32_t border = now.prefix;
+    const uint32_t first = segment * a.segment_tokens, last = min(a.tokens, first + a.segment_tokens), part = a.segment_tokens / WAVES;
+    const uint32_t begin = min(last, first + wave * part), end = min(last, begin + part);
+    const TQ_GLOBAL float *w = (const TQ_GLOBAL float *)a.weights + (long long)row * a.w_stride;
+    TQ_GLOBAL long long *kept = (TQ_GLOBAL long long *)a.kept + (long long)row * a.keep;
+    auto before_lane = [&](unsigned long long m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
+    auto tokens = [&](auto f) __attribute__((always_inline)) {               // f(token of this lane, key) of 64 at a time, in order
+        for (uint32_t i0 = begin; i0 < end; i0 += LONG_AHEAD * 64u) {
+            float v[LONG_AHEAD];
+#pragma unroll
+            for (uint32_t k = 0; k < LONG_AHEAD; ++k) v[k] = w[min(i0 + k * 64u + lane, a.tokens - 1u)];
+#pragma unroll
+            for (uint32_t k = 0; k < LONG_AHEAD; ++k) f(i0 + k * 64u + lane, i0 + k * 64u + lane < end ? order_of(v[k]) : 0u);
+        }
+    };
+    uint32_t more = 0u, same = 0u;
+    tokens([&](uint32_t, uint32_t k) {
+        more += (uint32_t)__popcll(__ballot(k > border));
+        same += (uint32_t)__popcll(__ballot(k == border));
+    });
+    if (lane == 0u) { lds_more[0][wave] = more; lds_more[1][wave] = same; }
+    __syncthreads();
+    uint32_t out = now.before;
+#pragma unroll
+    for (uint32_t k = 0; k < WAVES; ++k)
+        if (k < wave) { out += lds_more[0][k]; equal += lds_more[1][k]; }
+    out += min(equal, now.left);                            // (of those equal to the border the first `left` stay)
+    tokens([&](uint32_t i, uint32_t k) {
+        const unsigned long long equals = __ballot(k == border);
+        const bool stays = k > border || (k == border && equal + before_lane(equals) < now.left);
+        const unsigned long long staying = __ballot(stays);
+        if (stays) kept[out + before_lane(staying)] = i;
+        equal += (uint32_t)__popcll(equals);
+        out += (uint32_t)__popcll(staying);
+    });
+}
+
+long long long_segments(long long tokens) {
+    const long long n = (tokens + LONG_SEGMENT - 1) / LONG_SEGMENT;
+    return n < (long long)LONG_SEGMENTS ? n : (long long)LONG_SEGMENTS;
 }
 
 template <typename T>
@@ -262,8 +357,14 @@ __global__ __launch_bounds__(256) void tq_evict_move_kernel(EvictArgs a, uint32_
 
 }  // namespace
 
+extern "C" long long tq_evict_scratch(long long rows, long long tokens) {
+    if (rows < 0 || rows > 0x7fffffff || tokens < 0 || tokens > 0x7fffffff - 65536) return TQ_ERR_SIZE;
+    return tokens <= 32 * SELECT_THREADS ? 0 : rows * long_segments(tokens) * (3 * (long long)LONG_DIGITS + 4);
+}
+
 extern "C" int tq_evict(const tq_packed_store *from, const tq_packed_store *to, const float *weights, long long weights_stride, float *weights_out,
-                        long long weights_out_stride, long long rest, long long rows, long long tokens, long long keep, int head_dim, int bits_k, int bits_v, long long *kept, void *stream) {
+                        long long weights_out_stride, long long rest, long long rows, long long tokens, long long keep, int head_dim, int bits_k, int bits_v, long long *kept, uint32_t *scratch,
+                        long long scratch_words, void *stream) {
     if (!from || !to) return TQ_ERR_NULL;
     if (bits_k < 1 || bits_k > 8 || bits_v < 1 || bits_v > 8) return TQ_ERR_BITS;
     if (head_dim < TQ_ANYDIM_MIN || head_dim > TQ_ANYDIM_MAX) return TQ_ERR_HEAD_DIM;
@@ -280,6 +381,10 @@ extern "C" int tq_evict(const tq_packed_store *from, const tq_packed_store *to, 
     if (((uintptr_t)weights & 3u) || ((uintptr_t)weights_out & 3u) || ((uintptr_t)kept & 7u) ||
         (((uintptr_t)from->k_norms | (uintptr_t)from->v_norms | (uintptr_t)to->k_norms | (uintptr_t)to->v_norms) & 1u))
         return TQ_ERR_ALIGN;
+    const long long words = keep ? tq_evict_scratch(rows, tokens) : 0;
+    if (words && !scratch) return TQ_ERR_NULL;
+    if ((uintptr_t)scratch & 3u) return TQ_ERR_ALIGN;
+    if (scratch_words < words) return TQ_ERR_CAPACITY;
     EvictArgs a{};
     a.weights = weights; a.weights_out = weights_out; a.kept = kept;
     a.idx[0] = from->k_idx; a.idx[1] = from->v_idx; a.norms[0] = from->k_norms; a.norms[1] = from->v_norms;
@@ -298,7 +403,16 @@ extern "C" int tq_evict(const tq_packed_store *from, const tq_packed_store *to, 
         else if (tokens <= 4 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<4>), g, t, 0, st, a);
         else if (tokens <= 16 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<16>), g, t, 0, st, a);
         else if (tokens <= 32 * SELECT_THREADS) hipLaunchKernelGGL((tq_evict_select_kernel<32>), g, t, 0, st, a);
-        else hipLaunchKernelGGL((tq_evict_select_kernel<0>), g, t, 0, st, a);
+        else {
+            a.scratch = scratch;
+            a.segment_tokens = (uint32_t)(((tokens + long_segments(tokens) - 1) / long_segments(tokens) + SELECT_THREADS - 1) / SELECT_THREADS * SELECT_THREADS);
+            a.segments = (uint32_t)long_segments(tokens);
+            const dim3 blocks_of_segments((unsigned)(rows * a.segments));
+            hipLaunchKernelGGL((tq_evict_count_kernel<0>), blocks_of_segments, t, 0, st, a);
+            hipLaunchKernelGGL((tq_evict_count_kernel<1>), blocks_of_segments, t, 0, st, a);
+            hipLaunchKernelGGL((tq_evict_count_kernel<2>), blocks_of_segments, t, 0, st, a);
+            hipLaunchKernelGGL(tq_evict_place_kernel, blocks_of_segments, t, 0, st, a);
+        }
     }
     hipLaunchKernelGGL(tq_evict_move_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st, a, (uint32_t)blocks);
     return (int)hipGetLastError();

@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 4;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 5;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -39,6 +39,7 @@ struct Entries {
     decltype(&tq_attend_many_scratch) attend_many_scratch;
     decltype(&tq_attend_many) attend_many;
     decltype(&tq_evict) evict;
+    decltype(&tq_evict_scratch) evict_scratch;
 } lib{};
 
 struct Raised {};        // a Python exception is set
@@ -556,8 +557,12 @@ PyObject *evict(PyObject *const *a) {
     at::Tensor ko = empty({B, H, keep, packed_width(D, bk)}, at::kByte, ki), kno = empty({B, H, keep}, at::kHalf, ki), vo = empty({B, H, keep, packed_width(D, bv)}, at::kByte, ki);
     at::Tensor vno = empty({B, H, keep}, at::kHalf, ki), wo = empty({B, H, keep + rest}, at::kFloat, ki), kept = empty({B, H, keep}, at::kLong, ki);
     const tq_packed_store from{address(ki), (uint16_t *)address(kn), address(vi), (uint16_t *)address(vn), cap}, to{address(ko), (uint16_t *)address(kno), address(vo), (uint16_t *)address(vno), keep};
+    const long long words = lib.evict_scratch(B * H, tokens);
+    NEED(words >= 0);
+    at::Tensor scratch;
+    if (words) scratch = empty({words}, at::kInt, ki);
     const int rc = launch(lib.evict, (const tq_packed_store *)&from, (const tq_packed_store *)&to, (const float *)address(w), (long long)w.size(2), (float *)address(wo), keep + rest, rest, B * H, tokens, keep, (int)D, (int)bk, (int)bv,
-                          (long long *)address(kept), s.raw());
+                          (long long *)address(kept), words ? (uint32_t *)address(scratch) : (uint32_t *)nullptr, words, s.raw());
     if (rc > 0) return PyLong_FromLong(rc);
     NEED(rc == 0);
     return wrapped({ko, kno, vo, vno, wo, kept});
