@@ -109,6 +109,11 @@ TqManyPlain plain_of(const tq_plain_tokens &t) {
     return TqManyPlain{static_cast<const uint8_t *>(t.k), static_cast<const uint8_t *>(t.v), t.k_batch, t.k_head, t.k_token, t.v_batch, t.v_head, t.v_token, (uint32_t)t.tokens};
 }
 
+// Results where there is no token at all.  (Elements are two or four bytes.)
+__global__ __launch_bounds__(256) void tq_many_zero_kernel(uint16_t *out, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (size_t)gridDim.x * 256u) ((TQ_GLOBAL uint16_t *)out)[i] = 0u;
+}
+
 template <int DP>
 void launch_dim(const TqManyArgs &a, const Plan &plan, hipStream_t s) {
     const uint32_t at = a.rows * a.tiles;
@@ -221,6 +226,11 @@ extern "C" int tq_attend_many(const tq_attend_request *request, float *scratch, 
     a.aligned = !(r.head_dim & 7) && !((uintptr_t)r.queries & 15u) && !((r.q_batch * es) & 15) && !((r.q_head * es) & 15) && !((r.q_token * es) & 15) &&
                 (!r.window.tokens || aligned16(r.window, es)) && (!r.drafts.tokens || aligned16(r.drafts, es));
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (!r.tokens && !plain_tiles(request)) {          // (no kernel below has anything to do; sums of no key stay as they are)
+        const size_t n = (size_t)(p.rows * r.group * r.n_queries) * (size_t)r.head_dim * (size_t)(es / 2), blocks = (n + 255) / 256;
+        hipLaunchKernelGGL(tq_many_zero_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, static_cast<uint16_t *>(r.out), n);
+        return (int)hipGetLastError();
+    }
     a.plain_blocks = p.qt && p.plain_records ? (uint32_t)(p.rows * p.groups) : 0u;
     if (!p.qt) {
         const dim3 g((unsigned)(p.rows * ((p.tiles + 1) / 2))), t((p.tiles > 1 ? 4 : 2) * dp);
