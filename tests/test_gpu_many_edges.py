@@ -82,3 +82,21 @@ def test_nothing_to_attend_to(pkg, new_memory_is_nan, D, dtype):
     cache.append(k[:, :, :1], v[:, :, :1], 1)            # and on from there
     K, V = contents(cache)
     near(cache.attend(one, 1), one, K, V, torch.ones(1, dtype=torch.bool, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("D,n", [(128, 60), (128, 3000), (64, 100), (80, 100), (96, 2000), (256, 60), (33, 60)])
+def test_infinite_values_at_any_coordinate(pkg, D, n, dtype):
+    """One infinite element of a drafted value is found wherever it lies; the query that sees it has it there, and only there."""
+    B, H, T = 1, 1, 4
+    cache = make_cache(pkg, B, H, n, 5, D, dtype)
+    q, k, v = rand((B, H, T, D), 1, dtype), rand((B, H, T, D), 2, dtype), rand((B, H, T, D), 3, dtype)
+    tree = torch.eye(T, dtype=torch.bool, device=DEV)
+    want = cache.attend_tree(q, k, v, 1, tree)
+    for d in range(0, D, 5):
+        bad = v.clone()
+        bad[0, 0, d % T, d] = float("inf") if d % 2 else float("nan")
+        out = cache.attend_tree(q, k, bad, 1, tree)
+        assert not bool(torch.isfinite(out[0, 0, d % T, d]))
+        out[0, 0, d % T, d] = want[0, 0, d % T, d]
+        assert torch.equal(out, want), d

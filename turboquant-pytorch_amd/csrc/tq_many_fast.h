@@ -673,6 +673,7 @@ __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, f
             wild |= t.wild;
         }
         __syncthreads();             // (what the area held)
+        wild = __any(wild);          // (a lane knows of its own coordinates)
         if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
         float *const area = reinterpret_cast<float *>(lds);
         if (share) join_waves<DP, FAST_WAVES / 2>(area, lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, 1.f, m, l, acc, tid);
