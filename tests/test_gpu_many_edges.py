@@ -100,3 +100,61 @@ def test_infinite_values_at_any_coordinate(pkg, D, n, dtype):
         assert not bool(torch.isfinite(out[0, 0, d % T, d]))
         out[0, 0, d % T, d] = want[0, 0, d % T, d]
         assert torch.equal(out, want), d
+
+
+# (head dimension, tokens packed, window): one split of a row, several with the launch that joins them, and the kernel for all dimensions
+FORMS = [(128, 60, 5), (128, 3000, 0), (64, 1500, 40), (80, 700, 0), (96, 60, 20), (256, 900, 3), (33, 50, 0), (33, 700, 9)]
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("D,n,w", FORMS)
+def test_queries_that_are_no_numbers(pkg, D, n, w, dtype, bad):
+    """NaN for the query vector concerned, however its tokens are split; the others as ever. What keys receive is NaN in its rows and nowhere else."""
+    B, H, G, T = 2, 2, 2, 5
+    codec, ck, cv, K, V = states(pkg, B, H, n + w, w, D, dtype)
+    q = rand((B, H * G, T, D), 1, dtype)
+    q[1, 3, 2, 7] = bad
+    seen = torch.ones(n + w, dtype=torch.bool, device=DEV)
+    for track in (False, True):
+        sums = torch.zeros(B, H, n + w, device=DEV)
+        out = codec.attend_kv(q, ck, cv, **({"weights": sums} if track else {}))
+        assert bool(torch.isnan(out[1, 3, 2]).all())
+        fine, clean = out.clone(), q.clone()
+        fine[1, 3, 2], clean[1, 3, 2] = 0.0, 0.0
+        fine[1, 3, 2] = codec.attend_kv(clean, ck, cv)[1, 3, 2]
+        near(fine, clean, K, V, seen)
+        if track:
+            assert bool(torch.isnan(sums[1, 1]).all()) and bool(torch.isfinite(sums[0]).all()) and bool(torch.isfinite(sums[1, 0]).all())
+    hidden = torch.zeros(B, n + w, dtype=torch.bool, device=DEV)
+    assert not bool(codec.attend_kv(q, ck, cv, mask=hidden)[1, 3, 2].any())          # (it sees nothing)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("D,n,w", FORMS)
+def test_keys_that_are_no_numbers(pkg, D, n, w, dtype):
+    """A NaN key among those that a query sees is a NaN result, wherever it lies and whatever else there is; an infinite value is no finite result, however small its weight."""
+    B, H, G, T = 1, 2, 2, 4
+    cache = make_cache(pkg, B, H, n, w, D, dtype)
+    q, k, v = rand((B, H * G, T, D), 1, dtype), rand((B, H, T, D), 2, dtype), rand((B, H, T, D), 3, dtype)
+    tree = torch.eye(T, dtype=torch.bool, device=DEV)
+    want, lone = cache.attend_tree(q, k, v, 1, tree), make_cache(pkg, B, H, 0, w, D, dtype)
+    lone_want = lone.attend_tree(q, k, v, 1, tree)
+    bad_k = k.clone()
+    bad_k[0, 1, 2, 3] = float("nan")                  # kv head 1: query heads 2 and 3, token 2
+    for c, clean in ((cache, want), (lone, lone_want)):
+        out = c.attend_tree(q, bad_k, v, 1, tree)
+        assert bool(torch.isnan(out[0, 2:, 2]).all())
+        keep = torch.ones(H * G, T, dtype=torch.bool, device=DEV)
+        keep[2:, 2] = False
+        assert torch.equal(out[0, keep], clean[0, keep])
+    far_k, far_v = k.clone(), v.clone()
+    far_k[0, 0, 1], far_v[0, 0, 1, 5] = -300.0 * q[0, 0, 1], float("inf")           # a weight that underflows to zero, for query head 0
+    out = cache.attend_tree(q, far_k, far_v, 1, tree)
+    assert not bool(torch.isfinite(out[0, 0, 1, 5])) and not bool(torch.isfinite(out[0, 1, 1, 5]))
+    assert bool(torch.isfinite(out[0, 0, 1, :5]).all()) and torch.equal(out[0, 0, [0, 2, 3]], want[0, 0, [0, 2, 3]])
+    codec, ck, cv, _, _ = states(pkg, B, H, n + w, w, D, dtype)
+    ck["compressed"]["vec_norms"][0, 1, n // 2] = float("nan")
+    sums = torch.zeros(B, H, n + w, device=DEV)
+    out = codec.attend_kv(q, ck, cv, weights=sums)
+    assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isfinite(out[0, :2]).all()) and bool(torch.isnan(sums[0, 1]).all()) and bool(torch.isfinite(sums[0, 0]).all())
+    assert bool(torch.isnan(codec.attend_kv(q, ck, cv)[0, 2:]).all())

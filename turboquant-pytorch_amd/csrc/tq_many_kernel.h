@@ -155,19 +155,21 @@ __global__ __launch_bounds__(64 * PLAIN_WAVES) void tq_many_plain_kernel(TqManyA
             }
         }
         if (__any(wild)) {
-            // An infinite or NaN value must reach the queries that see its token and no other: a product would spread it as 0 * inf.
+            // An infinite or NaN value must reach the queries that see its token, be their weight too small for a number or not, and no other: a product would spread it as 0 * inf.
+            const uint32_t own = ManyQuery(a, min(tile * 32u + n, a.M - 1u)).t;
 #pragma unroll
             for (int r = 0; r < 16; ++r) lds_p[wave][acc_row(r, h)][n] = x[r];
             wave_sync();
 #pragma unroll 1
             for (uint32_t t = 0; t < min(32u, seg.n - t0); ++t) {
                 const float p = lds_p[wave][t][n];
+                const bool sees = plain_seen(a, which, b, own, t0 + t, length);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const uint32_t d = 32u * i + acc_row(r, h);
-                        if (d < a.D && p != 0.f) {
+                        if (d < a.D && sees) {
                             const float e = plain_element(v + ((long long)(t0 + t) * seg.v_token + d) * ES, DT);
                             if (!(fabsf(e) < __builtin_inff())) acc[i][r] = fmaf(p, e, acc[i][r]);
                         }
@@ -423,10 +425,12 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
 #pragma unroll 8
     for (uint32_t k = 0; k < PARTS; ++k) top = fmaxf(top, lds_red[0][k][c]);
     float sum = 0.f;
-    auto factor = [&](uint32_t i, float r, float t) {          // (a record of no token: zero, its sums need not have been written)
-        const float f = r == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(r - top);
+    // A record without a largest logit is one of no token, with sums of zero, or one whose logits are all NaN: its sum of weights tells.  Nothing is left out for a factor
+    // of zero: what is infinite or NaN in a record goes on into the result, however the tokens are split.
+    auto factor = [&](uint32_t i, float r, float t) {
+        const float f = r != MANY_NONE ? __builtin_amdgcn_exp2f(r - top) : t == 0.f ? 0.f : __builtin_nanf("");
         lds_f[i][c] = f;
-        sum = f == 0.f ? sum : fmaf(t, f, sum);
+        sum = fmaf(t, f, sum);
     };
 #pragma unroll
     for (uint32_t k = 0; k < 2; ++k)
@@ -448,9 +452,8 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
     }
     // ---- sums
     auto add = [&](tq_f4 &o, tq_f4 x, float f) __attribute__((always_inline)) {
-        if (f != 0.f)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
     };
 #pragma unroll
     for (uint32_t u0 = 0; u0 < UPT; ++u0) {
