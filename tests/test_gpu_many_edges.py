@@ -10,6 +10,8 @@ expm1(2 delta) + u_v of the longest value vector that the query sees, with
   float32           u_v = 2^-18: two fp16 terms each
 and (S / 8 + 100) 2^-24 more for float32 sums over S keys, of which a wave adds up an eighth at most and the others' sums are joined to its own
 (the way back out of the codec's space is in two terms throughout), plus half a step of the result's type."""
+import threading
+
 import pytest
 import torch
 
@@ -158,3 +160,69 @@ def test_keys_that_are_no_numbers(pkg, D, n, w, dtype):
     out = codec.attend_kv(q, ck, cv, weights=sums)
     assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isfinite(out[0, :2]).all()) and bool(torch.isnan(sums[0, 1]).all()) and bool(torch.isfinite(sums[0, 0]).all())
     assert bool(torch.isnan(codec.attend_kv(q, ck, cv)[0, 2:]).all())
+
+
+def test_nothing_is_handed_on_through_memory_that_others_use(pkg):
+    """The launches of a call hand their sums on through memory of the call's own: the scratch that decode steps of a stream share stays as it is."""
+    D, native = 128, pkg._native
+    plain, tracked = make_cache(pkg, 2, 2, 3000, 16, D, BF), make_cache(pkg, 2, 2, 3000, 16, D, BF, track_weights=True)
+    odd = make_cache(pkg, 1, 2, 300, 16, 33, BF)
+    codec, ck, cv, _, _ = states(pkg, 2, 2, 2000, 16, D, BF)
+    q, k, v, one = rand((2, 4, 6, D), 1, BF), rand((2, 2, 6, D), 2, BF), rand((2, 2, 6, D), 3, BF), rand((2, 4, 1, D), 4, BF)
+    plain.attend(one, 1)
+    assert native._step_scratch
+    for buf in native._step_scratch.values():
+        buf.fill_(12345.0)
+    for _ in range(2):
+        plain.attend_tree(q, k, v, 1)
+        tracked.attend(one, 1)
+        odd.attend_tree(q[:1, :, :, :33], k[:1, :, :, :33], v[:1, :, :, :33], 1)
+        codec.attend_kv(q, ck, cv, weights=torch.zeros(2, 2, 2000, device=DEV))
+    torch.cuda.synchronize()
+    assert all(bool((buf == 12345.0).all()) for buf in native._step_scratch.values())
+
+
+def run_threads(work):
+    """Every function of `work` in a thread of its own; the first exception is raised here."""
+    errors = []
+
+    def guarded(f):
+        try:
+            f()
+        except BaseException as e:          # noqa: B036
+            errors.append(e)
+    threads = [threading.Thread(target=guarded, args=(f,)) for f in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+def test_threads_on_one_stream(pkg):
+    """Calls of several threads whose launches meet on one stream answer as each does alone."""
+    caches = [make_cache(pkg, 1, 4, 3000 + 40 * i, 32, 128, BF, seed=i) for i in range(2)]
+    odd = make_cache(pkg, 1, 4, 400, 8, 33, BF)
+    sets = [(rand((1, 16, 9, 128), i, BF), rand((1, 4, 9, 128), 10 + i, BF), rand((1, 4, 9, 128), 20 + i, BF)) for i in range(2)]
+    small = tuple(t[..., :33].contiguous() for t in sets[0])
+    want = [c.attend_tree(*s, 1) for c, s in zip(caches, sets)]
+    want_odd, one = odd.attend_tree(*small, 1), rand((1, 16, 1, 128), 30, BF)
+    want_step = caches[0].attend(one, 1)
+    torch.cuda.synchronize()
+    got = [[] for _ in range(4)]
+
+    def tree(i):
+        for _ in range(50):
+            got[i].append(caches[i].attend_tree(*sets[i], 1))
+
+    def rest():
+        for _ in range(50):
+            got[2].append(odd.attend_tree(*small, 1))
+
+    def steps():
+        for _ in range(50):
+            got[3].append(caches[0].attend(one, 1))
+    run_threads([lambda: tree(0), lambda: tree(1), rest, steps])
+    torch.cuda.synchronize()
+    for outs, w in zip(got, (*want, want_odd, want_step)):
+        assert len(outs) == 50 and all(torch.equal(o, w) for o in outs)

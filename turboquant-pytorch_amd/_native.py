@@ -23,7 +23,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libtqamd.so")
 FAST_NAME = "tqamd_fastcall"        # extension module: the eager calls from tensors to the library in one step each
 FAST_SOURCE = "tq_fastcall.cpp"
-FAST_INTERFACE = 5                  # INTERFACE there: what init and the functions take and answer
+FAST_INTERFACE = 6                  # INTERFACE there: what init and the functions take and answer
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
@@ -760,7 +760,7 @@ def attend_many_store(queries: torch.Tensor, stores, tokens: int, tables, bits, 
     k_win, v_win = windows if windows is not None else (None, None)
     k_new, v_new = drafts if drafts is not None else (None, None)
     scale = queries.shape[-1] ** -0.5 if scale is None else float(scale)
-    out = fast().attend_many(queries, *stores, tokens, *tables, *bits, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale)
+    out = fast().attend_many(queries, *stores, tokens, *tables, *bits, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale, MANY_SCRATCH)
     if type(out) is int:
         check(out, "tq_attend_many")
     return out
@@ -851,7 +851,8 @@ def attend_many(queries: torch.Tensor, packed, tokens: int, tables, bits, window
     r.queries = queries.data_ptr()
     if tree is not None:
         r.tree, r.tree_batch = tree.data_ptr(), T * n_draft if tree.dim() == 3 else 0
-    floats = int(lib().tq_attend_many_scratch(ctypes.byref(r)))
+    with _on(dev):                               # (how a row is split goes by the device)
+        floats = int(lib().tq_attend_many_scratch(ctypes.byref(r)))
     if floats < 0:
         check(floats, "tq_attend_many_scratch")
     if floats > MANY_SCRATCH and T > 1:
@@ -867,11 +868,9 @@ def attend_many(queries: torch.Tensor, packed, tokens: int, tables, bits, window
         out = torch.empty((B, Hq, T, D), dtype=dtype, device=dev)
         r.out = out.data_ptr()
         if out.numel():
-            stream = _stream_handle(dev)
-            scratch = step_scratch(dev, stream, floats)
-            if scratch is None:
-                scratch = torch.empty(floats, dtype=torch.float32, device=dev)
-            check(lib().tq_attend_many(ctypes.byref(r), scratch.data_ptr(), scratch.numel(), stream), "tq_attend_many")
+            # the call's own: its launches hand their sums on through it, and those of another thread on the stream may come in between
+            scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+            check(lib().tq_attend_many(ctypes.byref(r), scratch.data_ptr(), floats, _stream_handle(dev)), "tq_attend_many")
     return out
 
 

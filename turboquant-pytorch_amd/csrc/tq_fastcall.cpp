@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 5;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 6;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -469,9 +469,10 @@ inline bool plain_tokens(PyObject *k_object, PyObject *v_object, long long first
     return true;
 }
 
-// attend_many(queries, k_idx, k_norms, v_idx, v_norms, tokens, table_k, table_v, bits_k, bits_v, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale)
+// attend_many(queries, k_idx, k_norms, v_idx, v_norms, tokens, table_k, table_v, bits_k, bits_v, k_win, v_win, win_first, n_win, k_new, v_new, lengths, mask, tree, weights, scale, most)
 // -> output: _native.attend_many where everything lies as the library takes it (packed stores dense, of which the first `tokens` slots count, window buffers of which
-// n_win tokens do; None where there is none).  Scratch of the stream as _native keeps it.
+// n_win tokens do; None where there is none) and no more than `most` float32 values of scratch are asked for.  Scratch is the call's own: its launches hand their sums on through it, and the launches of another thread
+// may come in between (the interpreter's lock is not held), or a decode step's, which uses the scratch that is kept for the stream.
 PyObject *attend_many(PyObject *const *a) {
     TENSOR(q, a[0]); TENSOR(ki, a[1]); TENSOR(kn, a[2]); TENSOR(vi, a[3]); TENSOR(vn, a[4]);
     NEED(q.dim() == 4 && ki.dim() == 4 && q.stride(3) == 1 && q.device() == ki.device());
@@ -524,19 +525,11 @@ PyObject *attend_many(PyObject *const *a) {
     r.scale = (float)scale;
     r.head_dim = (int)D; r.dtype = dt; r.bits_k = (int)bk; r.bits_v = (int)bv;
     const long long floats = lib.attend_many_scratch(&r);
-    NEED(floats >= 0);
-    PyObject *key = Py_BuildValue("(iK)", s.dev, s.handle);
-    if (!key) throw Raised{};
-    PyObject *scratch = PyDict_GetItem(g_scratch, key);      // borrowed; this frame keeps it through the call
-    Py_XINCREF(scratch);
-    Py_DECREF(key);
-    struct Held { PyObject *a; ~Held() { Py_XDECREF(a); } } held{scratch};
-    NEED(scratch);
-    TENSOR(buf, scratch);
-    NEED(buf.numel() >= floats);
+    NEED(floats >= 0 && floats <= integer(a[21]));
+    const at::Tensor scratch = empty({floats}, at::kFloat, q);
     at::Tensor out = empty({B, Hq, T, D}, q.scalar_type(), q);
     r.out = address(out);
-    const int rc = launch(lib.attend_many, (const tq_attend_request *)&r, (float *)address(buf), (long long)buf.numel(), s.raw());
+    const int rc = launch(lib.attend_many, (const tq_attend_request *)&r, (float *)address(scratch), floats, s.raw());
     if (rc > 0) return PyLong_FromLong(rc);
     NEED(rc == 0);           // (an argument the library refuses: nothing was launched)
     return THPVariable_Wrap(out);
@@ -613,7 +606,7 @@ PyObject *init(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
-    TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 21), TQ_ENTRY(evict, 10),
+    TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 22), TQ_ENTRY(evict, 10),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
