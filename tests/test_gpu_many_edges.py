@@ -162,6 +162,24 @@ def test_keys_that_are_no_numbers(pkg, D, n, w, dtype):
     assert bool(torch.isnan(codec.attend_kv(q, ck, cv)[0, 2:]).all())
 
 
+def run_threads(work):
+    """Every function of `work` in a thread of its own; the first exception is raised here."""
+    errors = []
+
+    def guarded(f):
+        try:
+            f()
+        except BaseException as e:          # noqa: B036
+            errors.append(e)
+    threads = [threading.Thread(target=guarded, args=(f,)) for f in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+
 def test_nothing_is_handed_on_through_memory_that_others_use(pkg):
     """The launches of a call hand their sums on through memory of the call's own: the scratch that decode steps of a stream share stays as it is."""
     D, native = 128, pkg._native
@@ -182,22 +200,32 @@ def test_nothing_is_handed_on_through_memory_that_others_use(pkg):
     assert all(bool((buf == 12345.0).all()) for buf in native._step_scratch.values())
 
 
-def run_threads(work):
-    """Every function of `work` in a thread of its own; the first exception is raised here."""
-    errors = []
+def test_decode_steps_of_several_launches_share_no_memory(pkg):
+    """The same for the decode step of float32 caches, which takes three launches."""
+    native = pkg._native
+    one_launch, three = make_cache(pkg, 1, 2, 900, 16, 128, BF), make_cache(pkg, 1, 2, 900, 16, 128, F32)
+    assert one_launch._stores[1].one_launch and not three._stores[1].one_launch
+    q = rand((1, 4, 1, 128), 1, F32)
+    one_launch.attend(q.to(BF), 1)
+    want = three.attend(q, 1)
+    assert native._step_scratch
+    for buf in native._step_scratch.values():
+        buf.fill_(12345.0)
+    got = three.attend(q, 1)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(bool((buf == 12345.0).all()) for buf in native._step_scratch.values())
+    other, other_q = make_cache(pkg, 2, 2, 700, 16, 128, F32, seed=3), rand((2, 4, 1, 128), 2, F32)
+    pairs = [(three, q, want), (other, other_q, other.attend(other_q, 1)), (one_launch, q.to(BF), one_launch.attend(q.to(BF), 1))]
+    got = [[] for _ in pairs]
 
-    def guarded(f):
-        try:
-            f()
-        except BaseException as e:          # noqa: B036
-            errors.append(e)
-    threads = [threading.Thread(target=guarded, args=(f,)) for f in work]
-    for t in threads:
-        t.start()
-    for t in threads:
-        t.join()
-    if errors:
-        raise errors[0]
+    def steps(i):
+        for _ in range(50):
+            got[i].append(pairs[i][0].attend(pairs[i][1], 1))
+    run_threads([lambda i=i: steps(i) for i in range(len(pairs))])
+    torch.cuda.synchronize()
+    for outs, (_, _, w) in zip(got, pairs):
+        assert len(outs) == 50 and all(torch.equal(o, w) for o in outs)
+
 
 def test_threads_on_one_stream(pkg):
     """Calls of several threads whose launches meet on one stream answer as each does alone."""

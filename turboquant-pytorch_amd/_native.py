@@ -561,7 +561,8 @@ SCRATCH_KEPT = 1 << 24          # float32 values a stream keeps at most: 64 MiB
 
 def step_scratch(device: torch.device, stream: int, floats: int) -> Optional[torch.Tensor]:
     """float32 scratch of a decode step (rotated queries, window records, split records), one buffer per
-    (device, stream), grown on demand: the steps of all layers on a stream run one after the other.  One entry per
+    (device, stream), grown on demand: the steps of all layers on a stream run one after the other.  Only for calls that are one launch: threads
+    share it, and between two launches of one call those of another may come.  One entry per
     stream that ever ran a decode step, kept for the life of the process: a few hundred KiB for a handful of sequences, 5 MiB for
     512 rows of 4 heads with a window of 128 tokens (a record per 32 window tokens and head), SCRATCH_KEPT at most.  What needs
     more gets a tensor of its own, which the caller holds until its launches have been queued on `stream`.

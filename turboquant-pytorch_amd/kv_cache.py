@@ -527,8 +527,9 @@ class V3Cache:
 
     @staticmethod
     def _attend_step(st: _LayerStore, query_states: torch.Tensor, G: int, scale: float) -> Optional[torch.Tensor]:
-        """The fused path of `attend` in one library call (rotate + window, packed history, merge), with the
-        scratch kept per stream.  None when the queries are not laid out for it."""
+        """The fused path of `attend` in one library call (rotate + window, packed history, merge): one launch with the
+        scratch kept per stream, or three with scratch of the call's own, since those of another thread on the stream may come
+        in between.  None when the queries are not laid out for it."""
         if st.one_launch and query_states.is_cuda:
             out = _native.fast().decode_attend(ctypes.addressof(st.record()), query_states, st.k_win, scale, st.w0, st.n_recent, st.n_compressed,
                                                st.cache_bytes())
@@ -553,10 +554,10 @@ class V3Cache:
         rec = D + 2
         n_q, n_pw, n_p = rows * G * D, rows * G * rec, rows * splits * G * rec
         with _native._on(dev):
-            stream = _native._stream_handle(dev)
-            scratch = _native.step_scratch(dev, stream, n_q + n_pw + n_p)
-            if scratch is None:
+            if torch.cuda.is_current_stream_capturing():
                 return None
+            stream = _native._stream_handle(dev)
+            scratch = torch.empty(n_q + n_pw + n_p, dtype=torch.float32, device=dev)
             base = scratch.data_ptr()
             out = torch.empty_like(query_states)
             code = _native.dtype_code(query_states.dtype)
