@@ -254,3 +254,17 @@ def test_threads_on_one_stream(pkg):
     torch.cuda.synchronize()
     for outs, w in zip(got, (*want, want_odd, want_step)):
         assert len(outs) == 50 and all(torch.equal(o, w) for o in outs)
+
+
+@pytest.mark.parametrize("S,w", [(200, 16), (200, 0)])
+def test_flat_dictionaries(pkg, S, w):
+    """Codes of all vectors one after the other, as decompress_kv takes them."""
+    codec, ck, cv, _, _ = states(pkg, 2, 2, S, w, 128, BF)
+    flat = [dict(c, compressed=dict(c["compressed"], idx_bytes=c["compressed"]["idx_bytes"].reshape(-1, c["compressed"]["idx_bytes"].shape[-1]),
+                                    vec_norms=c["compressed"]["vec_norms"].reshape(-1))) for c in (ck, cv)]
+    q = rand((2, 4, 3, 128), 1, BF)
+    for a, b in zip(codec.decompress_kv(*flat), codec.decompress_kv(ck, cv)):
+        assert torch.equal(a, b)
+    assert torch.equal(codec.attend_kv(q, *flat), codec.attend_kv(q, ck, cv))
+    sums = torch.rand(2, 2, S, device=DEV)
+    assert torch.equal(codec.evict_kv(*flat, sums, 50)[3], codec.evict_kv(ck, cv, sums, 50)[3])

@@ -369,7 +369,7 @@ class TurboQuantV3:
                 and shape[3] == kc.head_dim == vc.head_dim and (weights is None or weights.shape[-1] == shape[2])):
             tokens, windows = compressed_k["split_at"], (compressed_k["fp16"], compressed_v["fp16"])
             stores = (ck["idx_bytes"], ck["vec_norms"], cv["idx_bytes"], cv["vec_norms"])
-            if stores[0].shape[2] == tokens and windows[0].shape[2] == windows[1].shape[2] == shape[2] - tokens:
+            if stores[0].dim() == 4 and stores[0].shape[2] == tokens and windows[0].shape[2] == windows[1].shape[2] == shape[2] - tokens:
                 out = _native.attend_many_store(query_states, stores, tokens, (kc.table(device), vc.table(device)), (kc.bits, vc.bits), windows, 0, shape[2] - tokens,
                                                 None, lengths, mask, None, weights, scale)
                 if out is not None:
