@@ -268,3 +268,13 @@ def test_flat_dictionaries(pkg, S, w):
     assert torch.equal(codec.attend_kv(q, *flat), codec.attend_kv(q, ck, cv))
     sums = torch.rand(2, 2, S, device=DEV)
     assert torch.equal(codec.evict_kv(*flat, sums, 50)[3], codec.evict_kv(ck, cv, sums, 50)[3])
+
+
+def test_drafts_whose_values_are_more_than_their_keys(pkg):
+    """Refused, the first time and every other."""
+    cache = make_cache(pkg, 2, 2, 300, 16, 128, BF)
+    q, k, v = rand((2, 4, 6, 128), 1, BF), rand((2, 2, 6, 128), 2, BF), rand((2, 2, 9, 128), 3, BF)
+    for _ in range(3):
+        with pytest.raises(ValueError, match="do not go with"):
+            cache.attend_tree(q, k, v, 1)
+        cache.attend_tree(q, k, v[:, :, :6], 1)

@@ -485,8 +485,8 @@ PyObject *attend_many(PyObject *const *a) {
     const long long n_win = integer(a[13]), n_new = a[14] == Py_None ? 0 : T, total = tokens + n_win;
     NEED(plain_tokens(a[10], a[11], integer(a[12]), n_win, q, H, r.window));
     if (n_new) {
-        TENSOR(fresh, a[14]);
-        NEED(fresh.dim() == 4 && fresh.size(2) == T);
+        TENSOR(fresh_k, a[14]); TENSOR(fresh_v, a[15]);
+        NEED(fresh_k.dim() == 4 && fresh_v.dim() == 4 && fresh_k.size(2) == T && fresh_v.size(2) == T);
     }
     NEED(plain_tokens(a[14], a[15], 0, n_new, q, H, r.drafts));
     if (a[16] != Py_None) {
