@@ -278,3 +278,16 @@ def test_drafts_whose_values_are_more_than_their_keys(pkg):
         with pytest.raises(ValueError, match="do not go with"):
             cache.attend_tree(q, k, v, 1)
         cache.attend_tree(q, k, v[:, :, :6], 1)
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_lengths_of_any_whole_type(pkg, kind):
+    """More keys than the type can count, and lengths below zero where it has them."""
+    codec, ck, cv, K, V = states(pkg, 3, 2, 40000, 0, 64, BF, 2, 2)
+    q = rand((3, 2, 1, 64), 1, BF)
+    lengths = torch.tensor([100, 0, 7], dtype=kind, device=DEV)
+    if kind is not torch.uint8:
+        lengths[1] = -5
+    out = codec.attend_kv(q, ck, cv, lengths=lengths)
+    near(out, q, K, V, (torch.arange(40000, device=DEV) < lengths.view(-1, 1)).view(3, 1, 1, 1, -1))
+    assert not bool(out[1].any())

@@ -821,7 +821,7 @@ def attend_many(queries: torch.Tensor, packed, tokens: int, tables, bits, window
     if lengths is not None:
         if tuple(lengths.shape) != (B,) or lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
             raise ValueError(f"lengths must be one whole number per sequence, [{B}]; got {tuple(lengths.shape)} {lengths.dtype}")
-        lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, total).to(torch.int32)).contiguous()
+        lengths = (lengths if lengths.dtype == torch.int32 else lengths.long().clamp(0, total).to(torch.int32)).contiguous()
         r.lengths = lengths.data_ptr()
     if mask is not None:
         if tuple(mask.shape) != (B, total):
