@@ -291,3 +291,17 @@ def test_lengths_of_any_whole_type(pkg, kind):
     out = codec.attend_kv(q, ck, cv, lengths=lengths)
     near(out, q, K, V, (torch.arange(40000, device=DEV) < lengths.view(-1, 1)).view(3, 1, 1, 1, -1))
     assert not bool(out[1].any())
+
+
+def test_a_draft_over_nothing_settles_nothing(pkg):
+    """A cache that has seen a draft, and nothing else, takes states of any other head dimension."""
+    cache, fresh = pkg.V3Cache(n_layers=4), pkg.V3Cache(n_layers=4)
+    q, k = rand((1, 4, 3, 64), 1, BF), rand((1, 2, 3, 64), 2, BF)
+    cache.attend_tree(q, k, k, 1)
+    states_, one = outlier_kv((1, 2, 200, 128), seed=3, dtype=BF).to(DEV), rand((1, 4, 1, 128), 4, BF)
+    for c in (cache, fresh):
+        c.append(states_, states_, 1)
+    assert torch.equal(cache.attend(one, 1), fresh.attend(one, 1)) and cache._stores[1].comp.head_dim == 128
+    with pytest.raises(ValueError):                     # (what is cached has settled it)
+        cache.append(k, k, 1)
+    assert torch.equal(cache.attend(one, 1), fresh.attend(one, 1))

@@ -283,7 +283,9 @@ class V3Cache:
 
     def _get_compressor(self, layer_idx: int, head_dim: int, device) -> TurboQuantV3:
         # generation_test_v2.py:65-78: per-layer codec, residual_window=0 (the cache owns the window)
-        if layer_idx not in self._compressors:
+        comp = self._compressors.get(layer_idx)
+        # (what is cached for a layer settles its head dimension; a draft over nothing does not)
+        if comp is None or (comp.head_dim != head_dim and layer_idx not in self._stores):
             self._compressors[layer_idx] = TurboQuantV3(
                 head_dim=head_dim,
                 key_bits=self.key_bits,
