@@ -13,7 +13,8 @@ int padded(int D) { return TQ_PADDED_DIM(D); }
 long long plain_tiles(const tq_attend_request *r) { return (r->window.tokens + 31) / 32 + (r->drafts.tokens + 31) / 32; }
 
 struct Plan {
-    long long rows, tiles, groups, splits, records, plain_records, floats;
+    long long rows, tiles, groups, splits, records, plain_records;
+    long long operands, stats, scales, floats;          // float32 values of scratch: rotated queries, statistics, scales, and all with the records
     int qt, kt, vt;                  // tiles a block and fp16 terms of the kernels for one padded head dimension; qt = 0: the one for all
 };
 
@@ -80,7 +81,13 @@ int plan(const tq_attend_request *r, Plan &p) {
     p.records = whole || !r->tokens ? 0 : p.splits * (p.qt ? 1 : ANY_WAVES);
     p.plain_records = whole || !plain_tiles(r) ? 0 : (p.qt ? 1 : PLAIN_WAVES);
     const long long dp = padded(r->head_dim);
-    p.floats = at * ((long long)q_operand_bytes((uint32_t)dp) / 4 + (p.records + p.plain_records) * record_floats((uint32_t)dp) + 64) + (at + 3) / 4 * 4;
+    // Only what is written: kernels with tables rotate their queries themselves and write the operands out for the launch that adds up what keys receive, the only one that
+    // reads statistics.  (Four at least: a caller always has something to hand over.)
+    p.operands = p.qt && !r->weights ? 0 : at * ((long long)q_operand_bytes((uint32_t)dp) / 4);
+    p.stats = r->weights ? at * 64 : 0;
+    p.scales = p.qt && !r->weights ? 0 : (at + 3) / 4 * 4;
+    p.floats = p.operands + at * (p.records + p.plain_records) * record_floats((uint32_t)dp) + p.stats + p.scales;
+    if (p.floats < 4) p.floats = 4;
     return at * (p.splits + 1) * 4 > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;
 }
 
@@ -210,11 +217,11 @@ extern "C" int tq_attend_many(const tq_attend_request *request, float *scratch, 
     a.weights = r.weights; a.w_stride = r.weights_stride;
     // scratch: operands, records, uncompressed tokens' records, statistics, scales
     float *f = scratch;
-    a.q_op = reinterpret_cast<uint8_t *>(f); f += at * (q_operand_bytes(dp) / 4);
+    a.q_op = reinterpret_cast<uint8_t *>(f); f += p.operands;
     a.rec = f; f += at * p.records * record_floats(dp);
     a.plain_rec = f; f += at * p.plain_records * record_floats(dp);
     if (r.weights) a.stat = f;
-    f += at * 64;
+    f += p.stats;
     a.q_scale = f;
     a.scale = r.scale;
     a.rows = (uint32_t)p.rows; a.heads = (uint32_t)r.heads; a.group = (uint32_t)r.group; a.queries = (uint32_t)r.n_queries;
