@@ -104,6 +104,23 @@ def test_infinite_values_at_any_coordinate(pkg, D, n, dtype):
         assert torch.equal(out, want), d
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D,n", [(128, 40), (128, 1000), (64, 40), (80, 300), (256, 50), (33, 40)])
+def test_logits_far_below_zero(pkg, D, n, dtype):
+    """A query that points away from every key has the key with the largest logit all the same, below -1e30 as everywhere."""
+    codec = pkg.TurboQuantV3(D, key_bits=4, value_bits=4, residual_window=0, layer_idx=8, device=DEV)
+    along = rand((1, 1, 1, D), 1, F32)
+    ks, vs = (along * torch.arange(2, n + 2, device=DEV).view(1, 1, n, 1)).to(dtype), rand((1, 1, n, D), 2, dtype)
+    ck, cv = codec.compress_kv(ks.flip(2).contiguous(), vs)            # the shortest key is the last; the next is half as long again
+    V = dequantised(codec.val_compressor, (cv["compressed"]["idx_bytes"], cv["compressed"]["vec_norms"]))[:, :, -1:]
+    for size in (1.0, 1e25, 1e31, 1e33):
+        q = (-size * along).to(dtype)
+        got = codec.attend_kv(q, ck, cv)
+        # (its weight is one but for exp(-|along|^2 / sqrt(D)) at the least, logits being as far apart as that)
+        slack = HALF[dtype] + VALUE[dtype] + (n / 8 + 100) * 2.0 ** -24 + (0.0 if size > 1 else 4 * n * torch.exp(-0.9 * along.double().norm() ** 2 / D ** 0.5).item())
+        assert (got.double() - V).norm() <= slack * vs.double().norm(dim=-1).amax(), size
+
+
 # (head dimension, tokens packed, window): one split of a row, several with the launch that joins them, and the kernel for all dimensions
 FORMS = [(128, 60, 5), (128, 3000, 0), (64, 1500, 40), (80, 700, 0), (96, 60, 20), (256, 900, 3), (33, 50, 0), (33, 700, 9)]
 

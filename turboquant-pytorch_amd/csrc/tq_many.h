@@ -59,6 +59,13 @@ __host__ __device__ constexpr uint32_t record_floats(uint32_t dp) { return 64u +
 // blocks a compute unit)
 __host__ __device__ inline bool many_few(const TqManyArgs &a, uint32_t dp) { return a.M <= 16u && a.dtype != TQ_F32 && (dp == 64u || dp == 128u || dp == 256u); }
 
+// Base-2 logarithm of a weight times its query's sum, from a product and what it is to be multiplied by.  References lie at most 2^8 below the largest logit, but the attention's launch
+// had that from another order of sums, and of a logit in the millions the last bit is more than an exponent can be: kept sums stay finite.  (NaN stays NaN.)
+__device__ __forceinline__ float weight_exponent(float s, float f, float largest) {
+    const float x = fmaf(s, f, -largest);
+    return x > 16.f ? 16.f : x;
+}
+
 // Row of a result register r of a 32 x 32 product in lane half h
 __device__ __forceinline__ constexpr uint32_t acc_row(int r, uint32_t h) { return 8u * (uint32_t)(r / 4) + 4u * h + (uint32_t)(r % 4); }
 
@@ -267,7 +274,7 @@ __device__ __forceinline__ void plain_weights(const TqManyArgs &a, uint32_t item
         const float m = stat[n], inv = stat[32u + n];
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(x[r] - m), inv, w[r]);
+            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(x[r], 1.f, m)), inv, w[r]);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r)

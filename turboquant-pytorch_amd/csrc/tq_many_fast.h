@@ -13,7 +13,6 @@ constexpr int FAST_THREADS = 64 * FAST_WAVES;
 static_assert(FAST_THREADS == LUT_THREADS, "threads that stage the tables");
 constexpr int FAST_SLACK = 8;                // a column's reference moves when a logit exceeds it by more than this
 constexpr int FAST_P = 14 - FAST_SLACK;      // weights enter the products times 2^FAST_P, at most 2^14; value norms below 2 in their unit
-constexpr float FAST_START = -1.0e30f;
 
 // A head dimension as the kernels work on it: DP, the next multiple of 32.  64, 128 and 256 are taken as they are; for others (EVEN false, a.D below DP possible) packed
 // bytes go through LDS, where they may lie anywhere.  On the value side a lane has NC coordinates in a row, NC n ... NC n + NC - 1, of which the first LANES lanes' exist.
@@ -770,6 +769,8 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     using Values = ValueBytes<IPBV, NC>;
     constexpr int QW = KT * QT * STEPS * 4;                                        // registers of the queries' operands
     constexpr bool QREG = QW + QT * NC * 16 <= 136;
+    // a key's norm times the queries' scale from which on logits can pass 2^20: products are at most 2^14 sqrt(D) times the length of the levels, at most 4
+    constexpr float LARGE = (float)(1 << 20) / ((float)(1 << 16) * (DP <= 64 ? 8.f : 16.f) * (KT == 2 ? (float)(1 << LEVEL_SHIFT) : 1.f));
     constexpr int LUT_BYTES = 65536, Q_BYTES = KT * QT * STEPS * 1024;
     constexpr bool STAGE = !S::EVEN || GBV_MAX <= 128;
     constexpr int VPIECES = S::EVEN ? (GBV_MAX >= 32 ? GBV_MAX / 32 : 1) : (GBV_MAX + 31) / 32;        // 16 bytes of a run's values, that a lane stages
@@ -897,7 +898,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     tq_f16v acc[QT][NC];
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        m_ref[i] = FAST_START;
+        m_ref[i] = MANY_NONE;
         l[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[i][c] = tq_zero16();
@@ -929,6 +930,9 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 for (int c = 0; c < NC; ++c) acc[i][c] *= f;
         }
         norm *= h ? __uint_as_float((uint32_t)(127 - v_top) << 23) : q_scale;
+        // Where logits can be so large that what an unrounded product differs from the (rounded) reference by is no small part of one, up to more than an exponent can be, products
+        // are rounded first.
+        const bool large = __any(!h && norm >= LARGE);
         if (!h) lds_kn[wave][n] = norm;
         else if constexpr (VT == 2) lds_vn[wave][n] = norm;
         else lds_vn[wave][n] = __builtin_bit_cast(uint16_t, (_Float16)norm);
@@ -981,6 +985,18 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
             } else {
                 const tq_u2 v = *reinterpret_cast<const tq_u2 *>(&lds_vn[wave][8 * k + 4 * h]);
                 vn[2 * k] = v[0]; vn[2 * k + 1] = v[1];
+            }
+        }
+        if (large) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i) {
+                    float logit = s[i][r] * kn[r];
+                    asm volatile("" : "+v"(logit));
+                    s[i][r] = logit;
+                }
+                kn[r] = 1.f;
             }
         }
 #pragma unroll
@@ -1086,7 +1102,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     for (int i = 0; i < QT; ++i) {
         __syncthreads();
         join_waves<DP, FAST_WAVES>(reinterpret_cast<float *>(lds), lds_m, lds_l, J::sums(lds, 0u, i), J::largest(lds, 0u, i), J::total(lds, 0u, i), 0u, unit,
-                      m_ref[i] == FAST_START ? MANY_NONE : m_ref[i], l[i] * (1.0f / (float)(1 << FAST_P)), acc[i], tid);
+                      m_ref[i], l[i] * (1.0f / (float)(1 << FAST_P)), acc[i], tid);
     }
     __syncthreads();
     }
@@ -1142,7 +1158,7 @@ __device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t ite
                 const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (inv[r] != 0.f) w = fmaf(__builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.scale * LOG2E, -m[r])), inv[r], w);
+                    if (inv[r] != 0.f) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], a.scale * LOG2E, m[r])), inv[r], w);
             }
         }
         w = halves_add(w);
@@ -1219,7 +1235,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
                 if (8u * g >= queries) break;
                 const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(fmaf(s[4 * g + r], kn, -m[r])), inv[r], w);
+                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], kn, m[r])), inv[r], w);
             }
         };
         {
@@ -1347,7 +1363,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
             }
             w[i] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], kn[i], -m[r])), inv[r], w[i]);
+            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], kn[i], m[r])), inv[r], w[i]);
             w[i] = reduce_rows(w[i], OpAdd());
         }
         if (counts) *((TQ_GLOBAL float *)sums + t) = before + (lane & 16u ? w[1] : w[0]);

@@ -350,7 +350,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const uint32_t t = acc_row(r, h);
-            if (!((hidden >> t) & 1u) && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(s[r] * (lds_norm[wave][t] * q_scale) - m), inv, w[r]);
+            if (!((hidden >> t) & 1u) && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], lds_norm[wave][t] * q_scale, m)), inv, w[r]);
         }
     }
 #pragma unroll
