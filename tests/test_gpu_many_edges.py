@@ -121,6 +121,18 @@ def test_logits_far_below_zero(pkg, D, n, dtype):
         assert (got.double() - V).norm() <= slack * vs.double().norm(dim=-1).amax(), size
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("D,n,w", [(128, 60, 5), (128, 3000, 40), (64, 900, 0), (96, 500, 7), (256, 300, 3), (33, 200, 20)])
+def test_sums_of_large_logits(pkg, D, n, w, T, dtype):
+    """Logits of which the last bit is more than an exponent can be: no query gives a key more than its weight can be, and none gives less than nothing."""
+    codec, ck, cv, K, V = states(pkg, 2, 2, n + w, w, D, dtype)
+    for size in (1e3, 3e4) if dtype is F16 else (1e3, 1e6, 1e12, 1e20):
+        q, sums = (size * rand((2, 4, T, D), 1, F32)).clamp(-6e4, 6e4).to(dtype) if dtype is F16 else (size * rand((2, 4, T, D), 1, F32)).to(dtype), torch.zeros(2, 2, n + w, device=DEV)
+        out = codec.attend_kv(q, ck, cv, weights=sums, scale=1e3 if dtype is F16 else None)
+        assert bool(torch.isfinite(out).all()) and bool((sums >= 0).all()) and bool((sums <= 1.01 * 2 * T).all()), size
+
+
 # (head dimension, tokens packed, window): one split of a row, several with the launch that joins them, and the kernel for all dimensions
 FORMS = [(128, 60, 5), (128, 3000, 0), (64, 1500, 40), (80, 700, 0), (96, 60, 20), (256, 900, 3), (33, 50, 0), (33, 700, 9)]
 

@@ -31,7 +31,7 @@ struct TqManyArgs {
     float *q_scale;                  // [rows, tiles] what a tile's products are multiplied with
     float *rec;                      // [rows, tiles, records][32 largest logits, 32 sums, 32 x DP value sums]: packed tokens' (value space of the codec)
     float *plain_rec;                // the same of the uncompressed tokens (plain space)
-    float *stat;                     // [rows, tiles][32 largest logits, 32 reciprocal sums], written by the merge (only with weights)
+    float *stat;                     // [rows, tiles][32 largest logits, 32 reciprocal sums, 32 largest exponents], see put_stat (only with weights)
     float scale;
     uint32_t rows, heads, group, queries, M, tiles, tokens, packed_row_stride, D, bits_k, bits_v, dtype;
     uint32_t splits, chunk, records, plain_records;
@@ -59,12 +59,17 @@ __host__ __device__ constexpr uint32_t record_floats(uint32_t dp) { return 64u +
 // blocks a compute unit)
 __host__ __device__ inline bool many_few(const TqManyArgs &a, uint32_t dp) { return a.M <= 16u && a.dtype != TQ_F32 && (dp == 64u || dp == 128u || dp == 256u); }
 
-// Base-2 logarithm of a weight times its query's sum, from a product and what it is to be multiplied by.  References lie at most 2^8 below the largest logit, but the attention's launch
-// had that from another order of sums, and of a logit in the millions the last bit is more than an exponent can be: kept sums stay finite.  (NaN stays NaN.)
-__device__ __forceinline__ float weight_exponent(float s, float f, float largest) {
-    const float x = fmaf(s, f, -largest);
-    return x > 16.f ? 16.f : x;
+// What the launches that add up what keys receive know of a query: weight = 2^(logit - largest) / sum.  They have the logit from another order of sums than the attention's launch,
+// and of one in the millions the last bit is more than an exponent can be: no weight becomes larger than one (2^0.01 for rounding).  A query that is none, or sees nothing
+// (`some` false), gives nothing.
+constexpr uint32_t MANY_STATS = 96;
+__device__ __forceinline__ void put_stat(float *stat, uint32_t n, bool some, float largest, float sum, float inv) {
+    stat[n] = some ? largest : -MANY_NONE;
+    stat[32u + n] = some ? inv : 0.f;
+    stat[64u + n] = some ? __builtin_amdgcn_logf(sum) + 0.01f : 0.f;
 }
+// The exponent, from a product and what it is to be multiplied by.  (Where that is NaN the query's sum is, too.)
+__device__ __forceinline__ float weight_exponent(float s, float f, float largest, float most) { return fminf(fmaf(s, f, -largest), most); }
 
 // Row of a result register r of a 32 x 32 product in lane half h
 __device__ __forceinline__ constexpr uint32_t acc_row(int r, uint32_t h) { return 8u * (uint32_t)(r / 4) + 4u * h + (uint32_t)(r % 4); }
@@ -270,11 +275,11 @@ __device__ __forceinline__ void plain_weights(const TqManyArgs &a, uint32_t item
     for (uint32_t tile = 0; tile < a.tiles; ++tile) {
         float x[16];
         plain_logits<DT>(a, seg, 0u, row, b, kv, t0, tile * 32u + n, lane, length, steps, x);
-        const float *stat = a.stat + ((size_t)row * a.tiles + tile) * 64u;
-        const float m = stat[n], inv = stat[32u + n];
+        const float *stat = a.stat + ((size_t)row * a.tiles + tile) * MANY_STATS;
+        const float m = stat[n], inv = stat[32u + n], most = stat[64u + n];
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(x[r], 1.f, m)), inv, w[r]);
+            if (x[r] != MANY_NONE && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(x[r], 1.f, m, most)), inv, w[r]);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r)

@@ -703,12 +703,7 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
     const float f0 = m0 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m0 - m), f1 = m1 == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
     const float l = J::total(lds, 0u, i)[n] * f0 + (plain ? J::total(lds, 1u, i)[n] * f1 : 0.f), inv = l == 0.f ? 0.f : 1.0f / l;
     const uint32_t q = (tile0 + i) * 32u + n;
-    if (a.stat && w == 0u && h == 0u) {
-        float *stat = a.stat + ((size_t)row * a.tiles + tile0 + i) * 64u;
-        const bool some = q < a.M && inv != 0.f;
-        stat[n] = some ? m : -MANY_NONE;
-        stat[32u + n] = some ? inv : 0.f;
-    }
+    if (a.stat && w == 0u && h == 0u) put_stat(a.stat + ((size_t)row * a.tiles + tile0 + i) * MANY_STATS, n, q < a.M && inv != 0.f, m, l, inv);
     const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(DP) + ((size_t)w * STEPS * 64u + lane) * 16u;
     float largest = 0.f;
 #pragma unroll 8
@@ -1143,7 +1138,7 @@ __device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t ite
 #pragma unroll 1
         for (uint32_t tile = 0; tile < a.tiles; ++tile) {             // rows of the product: queries, columns: tokens
             const uint8_t *q = many_query(a, row, min(tile * 32u + n, a.M - 1u), 2u);
-            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + ((size_t)row * a.tiles + tile) * 64u + 4u * h;
+            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + ((size_t)row * a.tiles + tile) * MANY_STATS + 4u * h;
             tq_f16v s = tq_zero16();
 #pragma unroll 1
             for (int s0 = 0; s0 < STEPS; s0 += CH) {
@@ -1155,10 +1150,10 @@ __device__ __forceinline__ void window_weights(const TqManyArgs &a, uint32_t ite
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
+                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g), most = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 64 + 8 * g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (inv[r] != 0.f) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], a.scale * LOG2E, m[r])), inv[r], w);
+                    if (inv[r] != 0.f) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], a.scale * LOG2E, m[r], most[r])), inv[r], w);
             }
         }
         w = halves_add(w);
@@ -1229,13 +1224,13 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
         for (int i = 0; i < KW; ++i) kraw[i] = keys.raw[i];
         if (t_next < seen) issue(min(t_next, last));
         auto add = [&](const tq_f16v &s, uint32_t tile, float kn, uint32_t queries) __attribute__((always_inline)) {
-            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * 64u + 4u * h;
+            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * MANY_STATS + 4u * h;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 if (8u * g >= queries) break;
-                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g);
+                const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g), most = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 64 + 8 * g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], kn, m[r])), inv[r], w);
+                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], kn, m[r], most[r])), inv[r], w);
             }
         };
         {
@@ -1304,8 +1299,9 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
             q[t][s] = tq_gload16(a.q_op + (size_t)row * q_operand_bytes(DP) + ((t * (DP / 16) + (kg & 1u) * STEPS + s) * 64u + (kg >> 1) * 32u + n) * 16u);
-    const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (size_t)row * 64u + 4u * kg;
+    const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (size_t)row * MANY_STATS + 4u * kg;
     tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32);
+    const tq_f4 most = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 64);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
         if (4u * kg + r >= a.M) { m[r] = -MANY_NONE; inv[r] = 0.f; }
@@ -1363,7 +1359,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
             }
             w[i] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], kn[i], m[r])), inv[r], w[i]);
+            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], kn[i], m[r], most[r])), inv[r], w[i]);
             w[i] = reduce_rows(w[i], OpAdd());
         }
         if (counts) *((TQ_GLOBAL float *)sums + t) = before + (lane & 16u ? w[1] : w[0]);

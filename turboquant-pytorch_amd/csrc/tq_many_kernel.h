@@ -345,12 +345,12 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
     for (uint32_t tile = 0; tile < a.tiles; ++tile) {
         const size_t at = (size_t)row * a.tiles + tile;
         const tq_f16v s = any_products<DP>(lds_raw[wave], ks, lds_k, a.q_op + at * q_operand_bytes(DP), lane);
-        const float *stat = a.stat + at * 64u;
-        const float m = stat[n], inv = stat[32u + n], q_scale = a.q_scale[at];
+        const float *stat = a.stat + at * MANY_STATS;
+        const float m = stat[n], inv = stat[32u + n], most = stat[64u + n], q_scale = a.q_scale[at];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const uint32_t t = acc_row(r, h);
-            if (!((hidden >> t) & 1u) && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], lds_norm[wave][t] * q_scale, m)), inv, w[r]);
+            if (!((hidden >> t) & 1u) && inv != 0.f) w[r] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], lds_norm[wave][t] * q_scale, m, most)), inv, w[r]);
         }
     }
 #pragma unroll
@@ -444,11 +444,7 @@ __global__ __launch_bounds__(2 * DP) void tq_many_merge_kernel(TqManyArgs a) {
         for (uint32_t k = 0; k < PARTS; ++k) l += lds_red[1][k][tid];
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         lds_inv[tid] = inv;
-        if (a.stat) {          // (a query that is none, or sees nothing: weights of zero)
-            const bool some = tile * 32u + col0 + tid < a.M && inv != 0.f;
-            a.stat[(size_t)at * 64u + col0 + tid] = some ? top : -MANY_NONE;
-            a.stat[(size_t)at * 64u + 32u + col0 + tid] = some ? inv : 0.f;
-        }
+        if (a.stat) put_stat(a.stat + (size_t)at * MANY_STATS, col0 + tid, tile * 32u + col0 + tid < a.M && inv != 0.f, top, l, inv);
     }
     // ---- sums
     auto add = [&](tq_f4 &o, tq_f4 x, float f) __attribute__((always_inline)) {
