@@ -191,6 +191,37 @@ def test_keys_that_are_no_numbers(pkg, D, n, w, dtype):
     assert bool(torch.isnan(codec.attend_kv(q, ck, cv)[0, 2:]).all())
 
 
+@pytest.mark.parametrize("D,n,w,T,factor,dtype", [
+    (128, 60, 5, 9, 1e12, BF), (128, 3000, 16, 9, 1e25, BF), (128, 3000, 16, 40, 1e25, BF), (64, 700, 0, 3, 1e9, BF), (80, 700, 8, 9, 1e25, BF), (256, 900, 0, 9, 1e15, BF),
+    (33, 500, 4, 20, 1e25, BF), (128, 1000, 7, 9, 2e4, F16), (128, 60, 0, 70, 1e12, F32), (96, 900, 9, 9, 1e25, F32), (72, 300, 0, 1, 1e12, F32), (40, 90, 3, 33, 1e12, F32),
+])
+def test_a_query_far_larger_than_its_neighbours(pkg, D, n, w, T, factor, dtype):
+    """Queries that are worked on together do not have to be of one size: what a row of padding holds has no effect on the others."""
+    B, H, G = 2, 2, 3
+    codec, ck, cv, K, V = states(pkg, B, H, n + w, w, D, dtype)
+    q = rand((B, H * G, T, D), 1, dtype)
+    if dtype is F16:
+        q = q / 64
+    # along the longest key of its row, which then has all of its weight
+    longest = K.norm(dim=-1).argmax(-1)
+    for b in range(B):
+        for h in range(H):
+            along = K[b, h, longest[b, h]]
+            q[b, h * G + 1, T // 2] = (along / along.abs().max() * factor).to(dtype)
+    seen = torch.ones(n + w, dtype=torch.bool, device=DEV)
+    near(codec.attend_kv(q, ck, cv), q, K, V, seen)
+    sums = torch.zeros(B, H, n + w, device=DEV)
+    p = near(codec.attend_kv(q, ck, cv, weights=sums), q, K, V, seen)
+    p[:, :, 1, T // 2] = 0                               # (what the large one gives a key is some number from zero to one: its logits have no last bit that counts)
+    got = p.sum((2, 3))
+    delta = (2.0 ** -19 + D * 2.0 ** -22) * D ** -0.5 * q.double().norm(dim=-1).reshape(B, H, G, T, 1) * K.norm(dim=-1).amax(-1).view(B, H, 1, 1, 1)
+    delta[:, :, 1, T // 2] = 0
+    slack = (p * torch.expm1(2 * delta)).sum((2, 3)) + got * (T * G + 8 + (n + w) / 8 + 100) * 2.0 ** -23 + 1e-30
+    assert bool((sums.double() >= got - slack).all()) and bool((sums.double() <= got + slack + 1.01).all())
+    touched = (sums.double() > got + slack).sum(-1)
+    assert bool((touched <= (n + w) // 4).all())         # (it is one key's, or a few that lie as far in its direction)
+
+
 def run_threads(work):
     """Every function of `work` in a thread of its own; the first exception is raised here."""
     errors = []

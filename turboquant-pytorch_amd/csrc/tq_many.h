@@ -28,7 +28,7 @@ struct TqManyArgs {
     float *weights;                  // [rows, w_stride] what every key (packed, then window) receives is added here; or null
     long long w_stride;
     uint8_t *q_op;                   // rotated queries as operands, see q_operand_bytes
-    float *q_scale;                  // [rows, tiles] what a tile's products are multiplied with
+    float *q_scale;                  // [rows, tiles, 32] what a query's products are multiplied with
     float *rec;                      // [rows, tiles, records][32 largest logits, 32 sums, 32 x DP value sums]: packed tokens' (value space of the codec)
     float *plain_rec;                // the same of the uncompressed tokens (plain space)
     float *stat;                     // [rows, tiles][32 largest logits, 32 reciprocal sums, 32 largest exponents], see put_stat (only with weights)
@@ -45,7 +45,7 @@ typedef float tq_f4 __attribute__((ext_vector_type(4)));
 
 constexpr float MANY_NONE = -3.0e38f;        // largest logit of no token at all
 constexpr int LEVEL_SHIFT = 6;               // levels enter the products times 2^6: their second fp16 term stays above the subnormals' grid
-constexpr int Q_TOP = 13;                    // a tile's largest rotated query lies in [2^13, 2^14)
+constexpr int Q_TOP = 13;                    // the largest coordinate of rotated queries that are scaled together lies in [2^13, 2^14)
 constexpr int P_TOP = 14;                    // weight * value norm, at most 2^15
 constexpr int PLAIN_WAVES = 4;
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -90,6 +90,9 @@ __device__ __forceinline__ float halves_add(float x) {
     const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(two[0]) + __uint_as_float(two[1]);
 }
+
+// By which power of two a query whose largest coordinate is `top` is scaled to have it in [2^Q_TOP, 2^(Q_TOP + 1)).  (2^-114 does that for the largest float.)
+__device__ __forceinline__ int query_shift(float top) { return top > 0.f ? max(-114, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0; }
 
 // float -> two fp16 terms, packed (leading | rest << 16): 22 bits while neither term falls below 2^-14.  Infinities and NaN have no rest.
 __device__ __forceinline__ uint32_t fp16_terms(float x) {

@@ -85,7 +85,7 @@ int plan(const tq_attend_request *r, Plan &p) {
     // reads statistics.  (Four at least: a caller always has something to hand over.)
     p.operands = p.qt && !r->weights ? 0 : at * ((long long)q_operand_bytes((uint32_t)dp) / 4);
     p.stats = r->weights ? at * MANY_STATS : 0;
-    p.scales = p.qt && !r->weights ? 0 : (at + 3) / 4 * 4;
+    p.scales = p.qt && !r->weights ? 0 : at * 32;
     p.floats = p.operands + at * (p.records + p.plain_records) * record_floats((uint32_t)dp) + p.stats + p.scales;
     if (p.floats < 4) p.floats = 4;
     return at * (p.splits + 1) * 4 > 0x7fffffffLL ? TQ_ERR_SIZE : TQ_OK;

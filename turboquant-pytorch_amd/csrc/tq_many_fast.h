@@ -11,6 +11,7 @@ namespace {
 constexpr int FAST_WAVES = 8;                // one block per compute unit, two waves per SIMD, which share the tables
 constexpr int FAST_THREADS = 64 * FAST_WAVES;
 static_assert(FAST_THREADS == LUT_THREADS, "threads that stage the tables");
+constexpr int FAST_APART = 12;               // queries of a block are scaled together unless one is smaller than the largest by 2^12 or more
 constexpr int FAST_SLACK = 8;                // a column's reference moves when a logit exceeds it by more than this
 constexpr int FAST_P = 14 - FAST_SLACK;      // weights enter the products times 2^FAST_P, at most 2^14; value norms below 2 in their unit
 
@@ -207,8 +208,10 @@ __device__ __forceinline__ tq_u4 load_elements(const uint8_t *p, bool aligned) {
 }
 
 // Queries of QT tiles into the codec's space, q' = scale * log2(e) * Pi_k q, as fp16 operands in LDS ([tile][term][step][lane], as q_operand_bytes says): wave (tile i, w)
-// has coordinates 32 w ... + 31.  Pi as three bf16 terms, or for fp16 queries two fp16 ones (22 bits).  All tiles are scaled by the power of two
-// that puts their largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)); returns what products with them are to be multiplied by.  load() asks for everything, so that other loads
+// has coordinates 32 w ... + 31.  Pi as three bf16 terms, or for fp16 queries two fp16 ones (22 bits).  All queries are scaled by the power of two
+// that puts their largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)); finish() answers with what products with them are to be multiplied by.  Queries 2^FAST_APART times smaller
+// than the largest, and fp16 reaches no further than 2^14 below that for their smaller coordinates, make each query have a power of its own (`apart`): its products are then to be
+// multiplied by its entry of `own` first.  What a row of padding holds would otherwise take the bits of the others.  load() asks for everything, so that other loads
 // can be under way before finish() waits.
 template <int DP, int QT, int KT, int DT>
 struct Rotate {
@@ -255,7 +258,7 @@ struct Rotate {
         pi = a.table_k + (DT == TQ_F16 ? TQ_OFF_A_F16 : TQ_OFF_A_BF16(DP)) + ((size_t)w * STEPS * 64u + lane) * 16u;
         fetch(a, 0, lane >> 5);
     }
-    __device__ __forceinline__ float finish(const TqManyArgs &a, uint8_t *ops, float *lds_top, uint32_t wave, uint32_t lane) {
+    __device__ __forceinline__ float finish(const TqManyArgs &a, uint8_t *ops, float (*lds_top)[32], float (*own)[32], bool &apart, uint32_t wave, uint32_t lane) {
         const uint32_t n = lane & 31u, h = lane >> 5;
         float y[16], top = 0.f;
         if (i < (uint32_t)QT) {
@@ -280,14 +283,34 @@ struct Rotate {
                 const float v = fabsf(y[r]);
                 top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
             }
-            top = reduce_wave(top, OpMax());
+            top = halves_max(top);
         }
-        if (lane == 0u) lds_top[wave] = top;
+        if (h == 0u) lds_top[wave][n] = top;
         __syncthreads();
+        float of[QT];                            // largest coordinate of this column's query of each tile
+        top = 0.f;
 #pragma unroll
-        for (int k = 0; k < FAST_WAVES; ++k) top = fmaxf(top, lds_top[k]);
-        const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
-        const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+        for (int t = 0; t < QT; ++t) {
+            of[t] = 0.f;
+#pragma unroll
+            for (int k = 0; k < TILES; ++k) of[t] = fmaxf(of[t], lds_top[t * TILES + k][n]);
+            top = fmaxf(top, of[t]);
+        }
+        top = reduce_wave(top, OpMax());
+        bool far = false;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) far = far || (of[t] > 0.f && of[t] * (float)(1 << FAST_APART) <= top);
+        apart = __any(far);
+        const int up = query_shift(top);
+        float f = __uint_as_float((uint32_t)(up + 127) << 23);
+        if (apart) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const int mine = of[t] > 0.f ? min(query_shift(of[t]), up + 120) : up;        // (so that the entry is a normal number)
+                if (i == (uint32_t)t) f = __uint_as_float((uint32_t)(mine + 127) << 23);
+                if (wave == (uint32_t)t && h == 0u) own[t][n] = __uint_as_float((uint32_t)(127 + up - mine) << 23);
+            }
+        }
         if (i < (uint32_t)QT) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -776,7 +799,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[FAST_WAVES][32];
     __shared__ __attribute__((aligned(16))) std::conditional_t<VT == 2, float, uint16_t> lds_vn[FAST_WAVES][32];
-    __shared__ float lds_m[FAST_WAVES][32], lds_l[FAST_WAVES][32];
+    __shared__ float lds_m[FAST_WAVES][32], lds_l[FAST_WAVES][32], lds_own[QT][32];
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const uint32_t groups = (a.tiles + QT - 1u) / QT;
@@ -854,6 +877,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     if constexpr (VT == 1) table_v.load(a.table_v + TQ_OFF_LUT(DP), tid);
     else table_v.load(a.table_v, a.bits_v, DP, tid);
     float q_scale;
+    bool apart;
     auto start = [&](auto dt_tag) __attribute__((always_inline)) {
         Rotate<DP, QT, KT, decltype(dt_tag)::value> r;
         r.load(a, row, tile0, wave, lane);
@@ -864,7 +888,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
         __builtin_amdgcn_sched_barrier(0);
         table_k.store(lds, tid);
         table_v.store(lds + 128, tid);
-        q_scale = r.finish(a, ops, lds_kn[0], wave, lane);
+        q_scale = r.finish(a, ops, lds_kn, lds_own, apart, wave, lane);
     };
     if constexpr (VT == 2) start(std::integral_constant<int, TQ_F32>{});
     else if (a.dtype == TQ_BF16) start(std::integral_constant<int, TQ_BF16>{});
@@ -884,7 +908,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
     };
     if (a.weights && split == 0u) {          // (KT = 2: whole operands) for the launch that adds up what keys receive
         for (uint32_t i = tid; i < Q_BYTES / 16u; i += FAST_THREADS) tq_gstore16(a.q_op + first_tile * q_operand_bytes(DP) + i * 16u, *reinterpret_cast<const tq_u4 *>(ops + i * 16u));
-        if (tid == 0u) a.q_scale[first_tile] = q_scale;
+        if (tid < 32u) a.q_scale[first_tile * 32u + tid] = apart ? lds_own[0][tid] * q_scale : q_scale;
     }
     const uint32_t slot_k = KT == 1 ? RepLut<IPBK>::lane_offset(lane) : Lut2<IPBK>::lane_offset(lane);
     const uint32_t slot_v = 128u + (VT == 2 ? Lut2<IPBV>::lane_offset(lane) : IPBV == 4 && NC == 2 ? (lane & 30u) / 2u * 8u + 4u * (lane & 1u) : RepLut<IPBV>::lane_offset(lane));
@@ -982,12 +1006,15 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_ker
                 vn[2 * k] = v[0]; vn[2 * k + 1] = v[1];
             }
         }
-        if (large) {
+        if (large || apart) {
+            float own[QT];
+#pragma unroll
+            for (int i = 0; i < QT; ++i) own[i] = apart ? lds_own[i][n] : 1.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
 #pragma unroll
                 for (int i = 0; i < QT; ++i) {
-                    float logit = s[i][r] * kn[r];
+                    float logit = s[i][r] * own[i] * kn[r];
                     asm volatile("" : "+v"(logit));
                     s[i][r] = logit;
                 }
@@ -1188,7 +1215,6 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
     }
     tq_copy_to_lds(lds + LUT_BYTES, a.q_op + first_tile * q_operand_bytes(DP), 2 * STEPS * 1024, tid, FAST_THREADS);
     const uint32_t slot = (lane & (64u / IPBK - 1u)) * 4u * IPBK;
-    const float scale0 = a.q_scale[first_tile];
     __syncthreads();
     const size_t slot0 = (size_t)row * a.packed_row_stride;
     const uint32_t GBK = Shape<DP>::EVEN ? DP / IPBK : (a.D + IPBK - 1u) / IPBK;
@@ -1223,14 +1249,15 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
 #pragma unroll
         for (int i = 0; i < KW; ++i) kraw[i] = keys.raw[i];
         if (t_next < seen) issue(min(t_next, last));
-        auto add = [&](const tq_f16v &s, uint32_t tile, float kn, uint32_t queries) __attribute__((always_inline)) {
-            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * MANY_STATS + 4u * h;
+        auto add = [&](const tq_f16v &s, uint32_t tile, uint32_t queries) __attribute__((always_inline)) {
+            const TQ_GLOBAL float *stat = (const TQ_GLOBAL float *)a.stat + (first_tile + tile) * MANY_STATS + 4u * h, *scale = (const TQ_GLOBAL float *)a.q_scale + (first_tile + tile) * 32u + 4u * h;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 if (8u * g >= queries) break;
                 const tq_f4 m = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 8 * g), inv = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 32 + 8 * g), most = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(stat + 64 + 8 * g);
+                const tq_f4 qs = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(scale + 8 * g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], kn, m[r], most[r])), inv[r], w);
+                for (int r = 0; r < 4; ++r) w = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[4 * g + r], norm * qs[r], m[r], most[r])), inv[r], w);
             }
         };
         {
@@ -1244,7 +1271,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
                 s = mfma_f16(ql, hi, s);
                 s = mfma_f16(qh, lo, s);
             }
-            add(s, 0u, norm * scale0, a.M);
+            add(s, 0u, a.M);
         }
 #pragma unroll 1
         for (uint32_t tile = 1; tile < a.tiles; ++tile) {
@@ -1259,7 +1286,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_weights_
                 s = mfma_f16(ql, hi, s);
                 s = mfma_f16(qh, lo, s);
             }
-            add(s, tile, norm * a.q_scale[first_tile + tile], a.M - 32u * tile);
+            add(s, tile, a.M - 32u * tile);
         }
         w = halves_add(w);
         if (h == 0u && counts) *((TQ_GLOBAL float *)sums + t) = before + w;
@@ -1305,7 +1332,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
 #pragma unroll
     for (int r = 0; r < 4; ++r)
         if (4u * kg + r >= a.M) { m[r] = -MANY_NONE; inv[r] = 0.f; }
-    const float q_scale = a.q_scale[row];
+    const tq_f4 q_scale = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>((const TQ_GLOBAL float *)a.q_scale + (size_t)row * 32u + 4u * kg);
     const uint32_t slot = (lane & (64u / IPBK - 1u)) * 4u * IPBK;
     __syncthreads();
     const size_t slot0 = (size_t)row * a.packed_row_stride;
@@ -1338,7 +1365,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
         const uint32_t t_run = t_next, t0 = min(t_run, last), t = t0 + (lane & 31u);
         t_next += step;
         const bool counts = lane < 32u && t >= t_run && t < seen && (!a.mask || a.mask[(long long)b * a.mask_stride + t]);
-        const float before = before_raw, kn[2] = {(float)__builtin_bit_cast(_Float16, norm_raw[0]) * q_scale, (float)__builtin_bit_cast(_Float16, norm_raw[1]) * q_scale};
+        const float before = before_raw, kn[2] = {(float)__builtin_bit_cast(_Float16, norm_raw[0]), (float)__builtin_bit_cast(_Float16, norm_raw[1])};
         uint32_t now[2][KW];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -1359,7 +1386,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / (DP == 256 ? 4 : 2)) voi
             }
             w[i] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], kn[i], m[r], most[r])), inv[r], w[i]);
+            for (int r = 0; r < 4; ++r) w[i] = fmaf(__builtin_amdgcn_exp2f(weight_exponent(s[r], kn[i] * q_scale[r], m[r], most[r])), inv[r], w[i]);
             w[i] = reduce_rows(w[i], OpAdd());
         }
         if (counts) *((TQ_GLOBAL float *)sums + t) = before + (lane & 16u ? w[1] : w[0]);

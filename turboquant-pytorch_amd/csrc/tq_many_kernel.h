@@ -7,13 +7,13 @@ namespace {
 
 // ---- queries into the codec's space -----------------------------------------------------------------------------------------
 // Block (row, two tiles, one where a row has no more): a tile's wave w has coordinates 32 w ... + 31 of 32 queries, q' = scale * log2(e) * Pi_k q from the operands of the key codec's
-// table (Pi as three bf16 terms) and the queries' own bf16 terms, all products down to 2^-24 of the largest.  The tiles of a block are then scaled by
-// the power of two that puts its largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)), so that no query is too large or too small for the two fp16
-// terms it is stored as: 22 bits for queries down to 2^-16 of the largest.
+// table (Pi as three bf16 terms) and the queries' own bf16 terms, all products down to 2^-24 of the largest.  Every query is then scaled by
+// the power of two that puts its largest coordinate into [2^Q_TOP, 2^(Q_TOP + 1)), so that none is too large or too small for the two fp16
+// terms it is stored as, whatever the others are.
 template <int DT>
 __global__ __launch_bounds__(1024) void tq_many_prepare_kernel(TqManyArgs a, uint32_t waves) {
-    __shared__ float lds_top[16];
-    const uint32_t lane = threadIdx.x & 63u, all = blockDim.x >> 6, every = tq_uniform32(threadIdx.x >> 6), side = every / waves, wave = every - side * waves;
+    __shared__ float lds_top[16][32];
+    const uint32_t lane = threadIdx.x & 63u, every = tq_uniform32(threadIdx.x >> 6), side = every / waves, wave = every - side * waves;
     const uint32_t pairs = (a.tiles + 1u) / 2u, row = blockIdx.x / pairs, tile = 2u * (blockIdx.x - row * pairs) + side;
     const uint32_t DP = 32u * waves, steps = 2u * waves;
     const uint32_t n = lane & 31u, hk = lane >> 5, m = tile * 32u + n;
@@ -40,16 +40,15 @@ __global__ __launch_bounds__(1024) void tq_many_prepare_kernel(TqManyArgs a, uin
         const float v = fabsf(y[r]);
         top = fmaxf(top, v < __builtin_inff() ? v : 0.f);
     }
-#pragma unroll
-    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-    if (lane == 0u) lds_top[every] = top;
+    top = halves_max(top);
+    if (hk == 0u) lds_top[every][n] = top;
     __syncthreads();
-    for (uint32_t w = 0; w < all; ++w) top = fmaxf(top, lds_top[w]);
+    for (uint32_t w = 0; w < waves; ++w) top = fmaxf(top, lds_top[side * waves + w][n]);
     if (tile >= a.tiles) return;
     const size_t at = (size_t)row * a.tiles + tile;
-    const int up = top > 0.f ? max(-100, min(100, Q_TOP - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+    const int up = query_shift(top);
     const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-    if (wave == 0u && lane == 0u) a.q_scale[at] = __uint_as_float((uint32_t)(127 - up - LEVEL_SHIFT) << 23);
+    if (wave == 0u && hk == 0u) a.q_scale[at * 32u + n] = __uint_as_float((uint32_t)(127 - up - LEVEL_SHIFT) << 23);
     uint8_t *dst = a.q_op + at * q_operand_bytes(DP);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -253,7 +252,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_kernel(TqManyArgs 
     stage_levels(lds_k, a.table_k, a.bits_k);
     stage_levels(lds_v, a.table_v, a.bits_v);
     tq_copy_to_lds(lds_q, a.q_op + (size_t)at * q_operand_bytes(DP), q_operand_bytes(DP), threadIdx.x, blockDim.x);
-    const float q_scale = a.q_scale[at];
+    const float q_scale = a.q_scale[at * 32u + n];
     __syncthreads();
     const uint32_t seen = min(a.tokens, many_length(a, b));
     const uint32_t end = min(seen, split * a.chunk + a.chunk);
@@ -274,7 +273,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_kernel(TqManyArgs 
         const uint16_t *norms = h ? a.v_norms : a.k_norms;
         const float norm = own ? (float)__builtin_bit_cast(_Float16, tq_gload2(norms + slot0 + t0 + n)) : 0.f;
         const uint32_t hidden = ~(uint32_t)__ballot(own);                  // bit t: token t0 + t is not seen
-        (h ? vn : kn)[n] = h ? norm : norm * q_scale;
+        (h ? vn : kn)[n] = norm;
         // the largest value norm of the run: the sums are kept in units that go with the largest so far
         float top = h ? fabsf(norm) : 0.f;
 #pragma unroll
@@ -284,7 +283,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_kernel(TqManyArgs 
         const tq_f16v s = any_products<DP>(keys, ks, lds_k, lds_q, lane);
         float x[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = (hidden >> acc_row(r, h)) & 1u ? MANY_NONE : s[r] * kn[acc_row(r, h)];
+        for (int r = 0; r < 16; ++r) x[r] = (hidden >> acc_row(r, h)) & 1u ? MANY_NONE : s[r] * (kn[acc_row(r, h)] * q_scale);
         float shrink = softmax_tile(x, m, l);
         if (run_top > v_top) {
             shrink *= __uint_as_float((uint32_t)max(0, 127 + v_top - run_top) << 23);
@@ -346,7 +345,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
         const size_t at = (size_t)row * a.tiles + tile;
         const tq_f16v s = any_products<DP>(lds_raw[wave], ks, lds_k, a.q_op + at * q_operand_bytes(DP), lane);
         const float *stat = a.stat + at * MANY_STATS;
-        const float m = stat[n], inv = stat[32u + n], most = stat[64u + n], q_scale = a.q_scale[at];
+        const float m = stat[n], inv = stat[32u + n], most = stat[64u + n], q_scale = a.q_scale[at * 32u + n];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const uint32_t t = acc_row(r, h);
