@@ -365,3 +365,32 @@ def test_a_draft_over_nothing_settles_nothing(pkg):
     with pytest.raises(ValueError):                     # (what is cached has settled it)
         cache.append(k, k, 1)
     assert torch.equal(cache.attend(one, 1), fresh.attend(one, 1))
+
+
+@pytest.mark.parametrize("B,H,G,S,w,T,D,dtype", [
+    (8, 8, 4, 600, 40, 40, 128, BF), (8, 8, 4, 420, 0, 40, 64, BF), (8, 8, 4, 500, 300, 40, 96, BF),      # two tiles of queries a block, a row in one split
+    (16, 8, 4, 3000, 16, 8, 64, BF), (16, 8, 4, 3000, 0, 8, 128, F16), (16, 9, 2, 3100, 9, 16, 80, F32),  # 128 tiles and more, rows in several splits
+    (1, 2, 4, 70001, 16, 2, 64, BF), (1, 2, 4, 70001, 0, 2, 128, BF), (1, 1, 3, 50000, 5, 3, 96, F16), (1, 2, 2, 40000, 0, 5, 33, BF),      # 30 to 64 splits
+])
+def test_forms_of_large_calls(pkg, B, H, G, S, w, T, D, dtype):
+    codec, ck, cv, K, V = states(pkg, B, H, S, w, D, dtype)
+    q = rand((B, H * G, T, D), 1, dtype)
+    lengths = torch.full((B,), S, dtype=torch.int32, device=DEV)
+    lengths[::3] = S // 3
+    seen = (torch.arange(S, device=DEV) < lengths.view(-1, 1)).view(B, 1, 1, 1, S)
+    near(codec.attend_kv(q, ck, cv, lengths=lengths), q, K, V, seen)
+
+
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 12)])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, F16), (96, F32)])
+def test_sums_over_long_rows(pkg, D, dtype, G, T):
+    B, H, S, w = 2, 2, 20011, 30
+    codec, ck, cv, K, V = states(pkg, B, H, S, w, D, dtype)
+    q, sums = rand((B, H * G, T, D), 1, dtype), torch.zeros(B, H, S, device=DEV)
+    lengths = torch.tensor([S, 9000], dtype=torch.int32, device=DEV)
+    seen = (torch.arange(S, device=DEV) < lengths.view(-1, 1)).view(B, 1, 1, 1, S)
+    p = near(codec.attend_kv(q, ck, cv, lengths=lengths, weights=sums), q, K, V, seen)
+    delta = (2.0 ** -19 + D * 2.0 ** -22) * D ** -0.5 * q.double().norm(dim=-1).reshape(B, H, G, T, 1) * K.norm(dim=-1).amax(-1).view(B, H, 1, 1, 1)
+    got = p.sum((2, 3))
+    assert bool(((sums.double() - got).abs() <= (p * torch.expm1(2 * delta)).sum((2, 3)) + got * (T * G + 8 + S / 8 + 100) * 2.0 ** -23 + 1e-30).all())
+    assert not bool(sums[1, :, 9000:].any())
