@@ -265,7 +265,7 @@ __device__ __forceinline__ void plain_logits(const TqManyArgs &a, const TqManyPl
     }
 }
 
-// What the window's tokens receive: wave = 32 tokens, all query tiles of the row in order.
+// What the window's tokens receive is added to a.weights: wave = 32 tokens, all query tiles of the row in order, so that a token's sum is made by one wave in a fixed order.
 template <int DT>
 __device__ __forceinline__ void plain_weights(const TqManyArgs &a, uint32_t item, uint32_t steps, uint32_t lane) {
     const TqManyPlain &seg = a.plain[0];

@@ -101,8 +101,6 @@ __device__ __forceinline__ void put_sums(float *rec, uint32_t lane, float m, flo
 // ---- uncompressed tokens ---------------------------------------------------------------------------------------------------------
 // Block (row, tile), waves take 32 tokens at a time of the window, then of the drafted tokens.  Products in bf16 terms of the elements
 // and of the weights, down to 2^-24 of the largest: exact for 16-bit logits up to their summation.
-// WEIGHTS: instead of the sums, what every token of the window receives is added to a.weights; a.stat has the columns' statistics, and a block
-// goes through all tiles of its row, so that a token's sum is made by one wave in a fixed order.
 template <int DP, int DT>
 __global__ __launch_bounds__(64 * PLAIN_WAVES) void tq_many_plain_kernel(TqManyArgs a) {
     constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
