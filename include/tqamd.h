@@ -467,7 +467,8 @@ int tq_decode_append(const tq_decode_layer *layer, const void *k_new, const void
  *               tree_batch apart for each sequence (0: one for all)
  *   weights     NULL, or float32 [batch * heads, weights_stride]: to the value of every key (packed, then window) the weights that the
  *               row's queries give it are added, in an order that does not change
- * A query that sees no key gets zeros.  Infinities and NaN in masked or uncounted keys have no effect on the queries that do not see them.
+ * A query that sees no key gets zeros, also where there is none at all.  Infinities and NaN in masked or uncounted keys have no effect on the queries that do not see them;
+ * what a query does see of them, or holds, reaches its result and no other query's, and in its row the weights.  Queries may be of any size next to one another.
  * Element type dtype for queries, results, window and drafts; head_dim 8 ... 256; strides in elements, any alignment of the element type.
  * tq_attend_many_scratch: float32 values of scratch (16-byte aligned, not shared by launches that can overlap in time), or an error.
  */

@@ -30,9 +30,9 @@ bool fast(const tq_attend_request *r) {
 
 // Splits of the tokens among blocks of which one is resident per compute unit: rounds of blocks, each as long as a block's tokens and, in tokens, what its start and its
 // end cost (1500) and its uncompressed tokens (1000; `others`: blocks of those in the same launch), and for the merge 1000 and 30 a split.  A token with two terms of
-// everything (float32) counts three times.  Measured (us) against all other numbers of splits, 8 key/value heads of 128: 2048 tokens x 32 query vectors 19.1 with 8 (1: 32.3,
-// 4: 20.1), 8192 x 32 22.3 with 16 (8: 23.6, 32: 31.4), 131072 x 32 50.5 with 31 (24: 49.9, 16: 62.5, 64: 67.6), 16 sequences of 8192 x 64 as below, 32 of 8192 x 4 with kept
-// sums 139 with 1 (2: 152); float32 rows of 1003 tokens, 80 wide, 21.7 with 4 (1: 24.8).
+// everything (float32) counts three times.  Measured (us) against other numbers of splits, 8 key/value heads of 128: 2048 tokens x 32 query vectors 19.1 with 8 (1: 32.5,
+// 4: 20.2), 8192 x 32 21.5 with 16 (8: 24.0, 32: 31.1), 131072 x 32 47.4 with 31 (24: 50.9, 16: 61.7, 64: 66.2), 16 sequences of 8192 x 64 as below, 32 of 8192 x 4 with kept
+// sums 123 with 1 (2: 140); float32 rows of 1003 tokens, 80 wide, 22.0 with 4 (1: 25.1).
 long long fast_splits(int cus, long long blocks, long long others, long long tokens, int vt) {
     const long long weight = vt == 2 ? 3 : 1;
     long long most = (tokens + 255) / 256, best = 1, best_cost = 0;
@@ -57,7 +57,7 @@ int plan(const tq_attend_request *r, Plan &p) {
         p.kt = r->dtype == TQ_BF16 && !r->weights ? 1 : 2;
         p.vt = r->dtype == TQ_F32 ? 2 : 1;
         // Two tiles of queries a block share what is read and decoded.  One, where that fills no more than a round of blocks without splitting a row: 16 sequences
-        // of 8192 tokens, 64 query vectors a head, 72 us against 84, 2 of 1024 x 512 28 against 39; but 8 of 4096 x 2048 408 against 536, 1 of 32768 x 256 75 against 78.
+        // of 8192 tokens, 64 query vectors a head, 76 us against 91, 2 of 1024 x 512 29 against 40; but 8 of 4096 x 2048 541 against 419, 1 of 32768 x 256 78 against 68.
         int cus = 0;
         if (tq_device_cus(cus)) cus = 256;
         const long long others = plain_tiles(r) ? at : 0;

@@ -668,7 +668,7 @@ struct JoinArea {
 };
 
 // A row's uncompressed tokens against the block's tiles of queries, joined sums into LDS.  Two tiles share the waves where four of them hold all tokens (128 of a window,
-// 8 x 4096 x 2048: the call 418 us against 453).
+// 8 x 4096 x 2048: the call 435 us against 463).
 template <int DP, int QT, int DT>
 __device__ __forceinline__ void plain_phase(const TqManyArgs &a, uint8_t *lds, float (*lds_m)[32], float (*lds_l)[32], float *lds_wild, uint32_t row, uint32_t b, uint32_t tile0, uint32_t tiles,
                                             uint32_t length, uint32_t tid) {
@@ -773,12 +773,13 @@ __device__ __forceinline__ void finish_block(const TqManyArgs &a, uint8_t *lds, 
 // KT = 1: queries and levels as one fp16 value each, for bfloat16: the 2^-12 roundings move logits of some ten by 1e-3, where a bfloat16 result is rounded by up to 4e-3.
 // KT = 2: two terms each (three products, 22 bits), for float16, float32 and wherever sums of weights are kept; VT = 2: of weights and value levels as well, for float32.
 // Weights and value levels are otherwise one fp16 value each (the reference's own float32 levels are rounded to fp16 by the codec's decompress as well); with KT = 1 a query's
-// sum of weights is made of the rounded weights themselves, so that their rounding cancels in part.  KT = 2 for bfloat16 too would take 93 us instead of 77 (below), 628 instead of 426.
+// sum of weights is made of the rounded weights themselves, so that their rounding cancels in part.  KT = 2 for bfloat16 too would take 100 us instead of 76 (16 x 8192 x 64), 643 instead of
+// 419 (8 x 4096 x 2048).
 // What bounds it: vector instructions and products, which hardly overlap (16 x 8192 x 64: vector 52 % of the cycles, 280 a run of 32 tokens; matrix 24 %, LDS 40 %; 8 x 4096 x 2048: 51, 22
 // and 28 %). Waves are not what is missing: twelve with 168 registers took 84 us instead of 78 for the former, sixteen with 128 spill a hundred and took 178. 128 wide, 4 and 2 bits, 8 kv heads, us of this launch: 1 x 2048 tokens x 32 query vectors 12 (start 5, run 2, join 3);
-// 1 x 32768 x 256 65 (530 TFLOP/s); 16 x 8192 x 64 77 (450 TFLOP/s, 1.5 TB/s); 32 x 8192 x 4 for sums 84 (2.5 TB/s); with 4 and 4 bits 8 x 4096 x 2048 391 to 440 (400 TFLOP/s), a third
-// of it outside the loop (start, join, uncompressed tokens, way back).
-// Query operands stay in registers where they fit beside the sums (QREG): 131 us against 136 for the call with 32 x 8192 x 4, with two tiles of 128 wide queries they would spill.
+// 1 x 32768 x 256 65 (530 TFLOP/s); 16 x 8192 x 64 79 (440 TFLOP/s, 1.5 TB/s); 32 x 8192 x 4 for sums 87 (2.4 TB/s); with 4 and 4 bits 8 x 4096 x 2048 350 to 480, by card and its clock
+// (370 to 500 TFLOP/s), a third of it outside the loop (start, join, uncompressed tokens, way back).
+// Query operands stay in registers where they fit beside the sums (QREG): 132 to 134 us against 134 to 138 for the call with 32 x 8192 x 4, with two tiles of 128 wide queries they would spill.
 template <int DP, int IPBK, int IPBV, int QT, int KT, int VT>
 __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_many_fast_kernel(TqManyArgs a) {
     using S = Shape<DP>;

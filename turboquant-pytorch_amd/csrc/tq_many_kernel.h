@@ -236,7 +236,7 @@ __device__ __forceinline__ tq_f16v any_products(const uint8_t *keys, const CodeS
 }
 
 // The simplest form that is right for every head dimension and code width: a wave stages 32 tokens' bytes in LDS and looks every code up by itself, which is what it takes its time
-// for: 128 wide, 16 sequences of 8192 tokens x 64 query vectors a head 785 us (the kernel with tables 77), 1 x 2048 x 32 68 (19).  It is for what that one is not built for:
+// for: 128 wide, 16 sequences of 8192 tokens x 64 query vectors a head 785 us (the kernel with tables 76), 1 x 2048 x 32 69 (19).  It is for what that one is not built for:
 // 1 bit, head dimensions below 64, 72 ... 96 that are not whole words of packed bytes, above 96 but 128 and 256; fewer than 32 tokens; unaligned bytes.
 template <int DP>
 __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_kernel(TqManyArgs a) {
@@ -364,8 +364,8 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void tq_many_any_weights_kernel(TqM
 // ---- merge ------------------------------------------------------------------------------------------------------------------------
 // Block (row, tile, C of its 32 queries), DP / 32 waves: the records' sums with their factors, the packed ones turned back by Pi_v (two fp16 terms each of Pi_v^T,
 // from the value codec's table, and of the sums: 22 bits), the uncompressed ones added, everything divided by the sum of weights.
-// A query that sees nothing gets zeros.  C = 8 where tiles are fewer than 128: the records are then read by four times as many blocks (8 tiles x 31 records: the call 42 us instead of
-// 56; 96 x 5: 64.6 and 65.2; 256 x 2: 76.4 and, with C = 32, 73.2).  7 us for 8 tiles x 8 records of 128, 10.5 for 8 x 31.
+// A query that sees nothing gets zeros.  C = 8 where tiles are fewer than 128: the records are then read by four times as many blocks (8 tiles x 31 records: the call 47 us instead of
+// 60; 96 x 3: 52.0 and 53.5; but 256 x 2: 76.4 and, with C = 32, 73.2).  7 us for 8 tiles x 8 records of 128, 10.5 for 8 x 31.
 // A launch of few blocks lasts as long as its chain of loads: what does not depend on anything (references, sums, the first records, Pi_v) is asked for at once.
 constexpr uint32_t MERGE_RECORDS = 260;
 template <int DP, int C>

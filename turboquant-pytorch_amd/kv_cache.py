@@ -507,7 +507,8 @@ class V3Cache:
 
     def attention_weights(self, layer_idx: int = 0) -> torch.Tensor:
         """[B,H,n] float32: what every token held for the layer, packed tokens first, then the window, has received in the `attend` calls since
-        it came (summed over the query heads of its kv head).  The cache's own memory: it moves on with the next call."""
+        it came (summed over the query heads of its kv head).  `update` and `attend_tree` add nothing: after a prompt that went through `update`
+        alone all are zero.  The cache's own memory: it moves on with the next call."""
         st = self._stores.get(layer_idx)
         if st is None:
             raise ValueError(f"attention_weights: nothing is cached for layer {layer_idx}")
@@ -516,8 +517,8 @@ class V3Cache:
         return st.weights[:, :, :st.n_compressed + st.n_recent]
 
     def evict(self, keep: int, layer_idx: Optional[int] = None):
-        """Of the packed tokens of every (sequence, kv head) the `keep` that have received most attention stay, in their order (of equal ones the first);
-        the window stays whole.  Answers with the packed slots of what stayed, [B,H,min(keep, packed)] (int64); without a
+        """Of the packed tokens of every (sequence, kv head) the `keep` that have received most attention stay, in their order (of equal ones the first, so that
+        without any attention yet the oldest do); the window stays whole.  Heads keep tokens of their own: for unpadded batches.  Answers with the packed slots of what stayed, [B,H,min(keep, packed)] (int64); without a
         layer all layers are thinned out, and the answer is a dictionary of them.  `get_seq_length` still counts every token seen, so that
         positions go on; `update`, `append`, `attend` and `attend_tree` work on what is left."""
         if isinstance(keep, bool) or int(keep) != keep or keep < 0:
