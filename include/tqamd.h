@@ -518,6 +518,88 @@ int tq_evict(const tq_packed_store *from, const tq_packed_store *to, const float
              long long scratch_words, void *stream);
 long long tq_evict_scratch(long long rows, long long tokens);
 
+/*
+ * Beam search's choice: of the beams x vocab continuations of every sequence the `best` with the largest sums
+ *     sum(k, v) = scores[k] + logits[k][v] - log sum_v exp(logits[k][v])
+ * in falling order, equal ones by beam and then token (formed and compared in 64 bits, answered in 32).  No counterpart in the reference.
+ *   logits      element type dtype; token v of beam k of sequence b at element b * batch_stride + k * beam_stride + v
+ *   scores      float32, beam k of sequence b at b * score_stride + k
+ *   values, tokens, parents     dense [batch, best]
+ *   scratch     tq_beam_scratch bytes (8-byte aligned), not shared by launches that can overlap in time
+ * A beam whose sums are no numbers (a NaN or +infinity among its logits, nothing but -infinity, a score that is not finite) has sums of -infinity.  At most 1024 beams,
+ * beams * vocab < 2^31, best <= 64 and <= beams * vocab.
+ */
+long long tq_beam_scratch(long long batch, long long beams, long long vocab, long long best);
+int tq_beam_select(const void *logits, int dtype, long long batch, long long beams, long long vocab, long long batch_stride, long long beam_stride,
+                   const float *scores, long long score_stride, long long best, float *values, long long *tokens, long long *parents, void *scratch,
+                   long long scratch_bytes, void *stream);
+
+/*
+ * Rows of a cache follow others, in place: for every segment [batch][heads][bytes] (strides in bytes), sequence b becomes what sequence parents[b] (on the device) was.  A
+ * parent outside the batch leaves b as it is.  Segments must not overlap; at most 1024 sequences (TQ_ERR_CAPACITY).
+ */
+typedef struct tq_move_segment {
+    void *base;
+    long long batch_stride, head_stride, bytes;
+} tq_move_segment;
+int tq_reorder(const tq_move_segment *segments, int n_segments, long long batch, long long heads, const long long *parents, void *stream);
+
+/*
+ * Pages of a pool copied into pages of the same or another pool: a page is `rows` runs of row_bytes bytes, of which the first `bytes` are copied (multiples of 16, as addresses
+ * and strides).  `pairs` is host memory, read before the call returns; no page is both written and read or written twice.
+ */
+typedef struct tq_page_pair {
+    int32_t from, to, bytes;
+} tq_page_pair;
+int tq_copy_pages(const void *from, long long from_stride, void *to, long long to_stride, long long rows, long long row_bytes, const tq_page_pair *pairs, long long n_pairs,
+                  void *stream);
+
+/*
+ * New tokens into a pool of uncompressed pages: the key of token i and head h, vector_bytes bytes at i * k_token_stride + h * k_head_stride (bytes), goes to place
+ * slots[i] % page_tokens of page slots[i] / page_tokens, at page * page_stride + (h * page_tokens + place) * vector_bytes; the value side_stride further on.  page_tokens is a power of
+ * two; slots (int32, device) are not checked.
+ */
+int tq_put_tokens(const void *keys, const void *values, long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                  void *pool, long long page_stride, long long side_stride, const int32_t *slots, long long tokens, long long heads, long long vector_bytes,
+                  int page_tokens, void *stream);
+
+/*
+ * Attention of sequences' new tokens over pages: softmax(z) V with z = cap(scale q K^T) - slope * distance over the keys that a new token sees, all before it and itself, or the last
+ * sliding_window of those.  A page holds page_tokens tokens (a power of two, 32 or more) of all kv heads, head after head: packed ones as tq_compress leaves them with rows = heads,
+ * or plain ones in the queries' element type.
+ *   sequences   8 numbers each: first row of its queries, new tokens, all tokens (the new ones are the last), packed tokens (the first; no new ones), where in `tables` its packed and its
+ *               plain pages' numbers begin, two unused.  On the host for the plan, a copy on the device for the call, as items and merges
+ *   packed_pool, plain_pool     the layer's part of page 0 (key codes; keys), from which the other parts and the other pages are so many bytes on
+ *   queries     new token i, query head j at i * q_token + j * q_head elements; query head j reads kv head j / group.  out: dense [new tokens, heads * group, head_dim]
+ *   softcap     0: none; otherwise logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
+ * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, 4 a merge; counts also where they do not fit
+ * (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim and dtype.
+ * tq_paged_scratch: float32 values of scratch (16-byte aligned, not shared by calls that can overlap in time).
+ * tq_paged_supported: head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose packed vectors are words; 2 to 8 bits.
+ * Infinities and NaN reach the results of the queries that see them and no others.  Numbers of pages are not checked.  Pages are read whole runs of 32 tokens at a time.
+ */
+typedef struct tq_paged_counts {
+    long long items, merges, records;
+    int tiles, columns;
+} tq_paged_counts;
+typedef struct tq_paged_request {
+    const void *queries;
+    void *out;
+    const void *packed_pool, *plain_pool, *table_k, *table_v;
+    const int32_t *sequences, *tables, *items, *merges;
+    const float *slopes;
+    long long q_token, q_head;
+    long long packed_page_stride, k_norms, v_idx, v_norms, plain_page_stride, plain_values;
+    tq_paged_counts counts;
+    float scale, softcap;
+    int heads, group, sliding_window, page_tokens, head_dim, dtype, bits_k, bits_v;
+} tq_paged_request;
+int tq_paged_supported(int head_dim, int dtype, int bits_k, int bits_v);
+int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int32_t *items, long long max_items, int32_t *merges,
+                  long long max_merges, tq_paged_counts *counts);
+long long tq_paged_scratch(const tq_paged_counts *counts, int heads, int head_dim);
+int tq_paged_attend(const tq_paged_request *request, float *scratch, long long scratch_floats, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

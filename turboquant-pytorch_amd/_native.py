@@ -27,8 +27,10 @@ FAST_INTERFACE = 6                  # INTERFACE there: what init and the functio
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
-           "tq_qjl_scores.hip", "tq_decode.hip", "tq_wide.hip", "tq_many.hip", "tq_many_d64.hip", "tq_many_d96.hip", "tq_many_d128.hip", "tq_many_d256.hip", "tq_evict.hip", "tq_host.cpp")
-HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", "tq_many.h", "tq_many_kernel.h", "tq_many_fast.h", os.path.join("..", "..", "include", "tqamd.h"))
+           "tq_qjl_scores.hip", "tq_decode.hip", "tq_wide.hip", "tq_many.hip", "tq_many_d64.hip", "tq_many_d96.hip", "tq_many_d128.hip", "tq_many_d256.hip", "tq_evict.hip",
+           "tq_paged.hip", "tq_paged_d64.hip", "tq_paged_d96.hip", "tq_paged_d128.hip", "tq_paged_d256.hip", "tq_pages.hip", "tq_beam.hip", "tq_host.cpp")
+HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", "tq_many.h", "tq_many_kernel.h", "tq_many_fast.h", "tq_paged.h", "tq_paged_kernel.h",
+           os.path.join("..", "..", "include", "tqamd.h"))
 GPU_ARCH = "gfx950"
 
 TQ_F32, TQ_F16, TQ_BF16 = 0, 1, 2
@@ -222,6 +224,23 @@ class TqPackedStore(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("k_idx", "k_norms", "v_idx", "v_norms")] + [("packed_row_stride", ctypes.c_longlong)]
 
 
+class TqMoveSegment(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p)] + [(n, ctypes.c_longlong) for n in ("batch_stride", "head_stride", "bytes")]
+
+
+class TqPagedCounts(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_longlong) for n in ("items", "merges", "records")] + [("tiles", ctypes.c_int), ("columns", ctypes.c_int)]
+
+
+class TqPagedRequest(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("queries", "out", "packed_pool", "plain_pool", "table_k", "table_v", "sequences", "tables", "items", "merges", "slopes")]
+                + [(n, ctypes.c_longlong) for n in ("q_token", "q_head", "packed_page_stride", "k_norms", "v_idx", "v_norms", "plain_page_stride", "plain_values")]
+                + [("counts", TqPagedCounts), ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+                + [(n, ctypes.c_int) for n in ("heads", "group", "sliding_window", "page_tokens", "head_dim", "dtype", "bits_k", "bits_v")])
+
+
+PAGED_SEQ, PAGED_ITEM, PAGED_MERGE = 8, 8, 4       # numbers of a sequence, an item of the plan and a merge, as tq_paged.h has them
+
 EXPORTS = (
     "tq_abi_version", "tq_status_string", "tq_device_count", "tq_bytes_per_vector",
     "tq_decision_thresholds", "tq_table_bytes", "tq_table_build", "tq_table_check", "tq_table_quantize_host",
@@ -233,6 +252,7 @@ EXPORTS = (
     "tq_decode_supported", "tq_decode_scratch_floats", "tq_decode_attend", "tq_decode_attend_spread", "tq_decode_attend_cached", "tq_decode_streams", "tq_decode_append",
     "tq_compress_layer", "tq_restore_layer",
     "tq_attend_many_scratch", "tq_attend_many", "tq_evict", "tq_evict_scratch",
+    "tq_beam_scratch", "tq_beam_select", "tq_reorder", "tq_copy_pages", "tq_put_tokens", "tq_paged_supported", "tq_paged_plan", "tq_paged_scratch", "tq_paged_attend",
 )
 
 _lib = None
@@ -301,8 +321,19 @@ def lib() -> ctypes.CDLL:
     L.tq_evict.argtypes = [vp, vp, vp, ll, vp, ll, ll, ll, ll, ll, ci, ci, ci, vp, vp, ll, vp]
     L.tq_evict_scratch.restype = ll
     L.tq_evict_scratch.argtypes = [ll, ll]
+    L.tq_beam_scratch.restype = ll
+    L.tq_beam_scratch.argtypes = [ll, ll, ll, ll]
+    L.tq_beam_select.argtypes = [vp, ci, ll, ll, ll, ll, ll, vp, ll, ll, vp, vp, vp, vp, ll, vp]
+    L.tq_reorder.argtypes = [vp, ci, ll, ll, vp, vp]
+    L.tq_copy_pages.argtypes = [vp, ll, vp, ll, ll, ll, vp, ll, vp]
+    L.tq_put_tokens.argtypes = [vp, vp, ll, ll, ll, ll, vp, ll, ll, vp, ll, ll, ll, ci, vp]
+    L.tq_paged_supported.argtypes = [ci, ci, ci, ci]
+    L.tq_paged_plan.argtypes = [vp, ll, ci, ci, ci, ci, ci, vp, ll, vp, ll, vp]
+    L.tq_paged_scratch.restype = ll
+    L.tq_paged_scratch.argtypes = [vp, ci, ci]
+    L.tq_paged_attend.argtypes = [vp, vp, ll, vp]
     for name in EXPORTS:
-        if name not in ("tq_attend_many_scratch", "tq_evict_scratch", "tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
+        if name not in ("tq_beam_scratch", "tq_paged_scratch", "tq_attend_many_scratch", "tq_evict_scratch", "tq_status_string", "tq_table_bytes", "tq_workspace_bytes", "tq_qjl_table_bytes", "tq_decode_scratch_floats"):
             getattr(L, name).restype = ci
     _lib = L
     return L
@@ -919,6 +950,15 @@ def evict(packed, tokens: int, bits, D: int, weights: torch.Tensor, keep: int, i
         check(lib().tq_evict(ctypes.byref(source), ctypes.byref(target), weights.data_ptr(), sh if H > 1 else sb, weights_into.data_ptr(), weights_into.shape[2], rest,
                              B * H, tokens, keep, D, *bits, kept.data_ptr(), 0 if scratch is None else scratch.data_ptr(), words, _stream_handle(dev)), "tq_evict")
     return into, weights_into, kept
+
+
+def reorder(segments, parents: torch.Tensor, heads: int, device: torch.device) -> None:
+    """tq_reorder: segments (address, bytes between sequences, between heads, bytes) of a cache on `device`, in place."""
+    if parents.device != device or parents.dtype != torch.int64 or not parents.is_contiguous():
+        parents = parents.to(device=device, dtype=torch.int64).contiguous()
+    runs = (TqMoveSegment * len(segments))(*segments)
+    with _on(device):
+        check(lib().tq_reorder(runs, len(segments), parents.shape[0], heads, parents.data_ptr(), _stream_handle(device)), "tq_reorder")
 
 
 def compress_into(states: torch.Tensor, table: torch.Tensor, bits: int,

@@ -1,0 +1,290 @@
+// softmax(scale q K^T) V of sequences' new tokens over packed and plain pages, scores capped, biased by distance or within a window: tq_paged_attend, and the plan that its
+// blocks work by, tq_paged_plan (on the host, where the lengths are known; one plan serves all layers of a step).  Two launches: a block an item of the plan (tq_paged_kernel.h), and
+// where a tile's tokens are in several items, a merge.
+#include <algorithm>
+#include <vector>
+
+#include "tq_paged.h"
+
+namespace {
+
+constexpr int MAX_PIECES = 64;
+constexpr int MERGE_THREADS = 256;
+
+// Block = (merge, kv head, tile of the pair, share of a tile's results): results are the records' sums, each times 2^(its reference - the largest), over their sums of weights.
+template <int DP>
+__global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedArgs a, uint32_t qt, uint32_t shares) {
+    __shared__ float lds_m[MAX_PIECES * 32], lds_l[MAX_PIECES * 32];
+    uint32_t at = blockIdx.x;
+    const uint32_t share = at % shares;
+    at /= shares;
+    const uint32_t i = at % qt;
+    at /= qt;
+    const uint32_t kv = at % a.heads, merge = at / a.heads;
+    const int32_t *mg = a.merges + (size_t)merge * PAGED_MERGE;
+    const int32_t *sq = a.seqs + (size_t)mg[0] * PAGED_SEQ;
+    const uint32_t tile = (uint32_t)mg[1] + i, records = (uint32_t)mg[3], M = (uint32_t)sq[1] * a.group, tid = threadIdx.x;
+    if (tile * 32u >= M) return;
+    const size_t step = (size_t)a.heads * qt * paged_record(a.cols, DP);
+    const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + (((size_t)mg[2] * a.heads + kv) * qt + i) * paged_record(a.cols, DP);
+    for (uint32_t j = tid; j < records * a.cols; j += MERGE_THREADS) {
+        const uint32_t r = j / a.cols, c = j - r * a.cols;
+        lds_m[j] = rec[r * step + c];
+        lds_l[j] = rec[r * step + a.cols + c];
+    }
+    const uint32_t unit = share * MERGE_THREADS + tid, c = unit / (DP / 4u), d = (unit - c * (DP / 4u)) * 4u;
+    const uint32_t m = tile * 32u + c;
+    const bool some = c < a.cols && m < M && d < a.D;
+    __syncthreads();
+    if (!some) return;
+    float top = MANY_NONE;
+    for (uint32_t r = 0; r < records; ++r) top = fmaxf(top, lds_m[r * a.cols + c]);
+    float sum = 0.f;
+    tq_f4 o = {0.f, 0.f, 0.f, 0.f};
+    const TQ_GLOBAL float *p = rec + 2u * a.cols + c * DP + d;
+    for (uint32_t r0 = 0; r0 < records; r0 += 8u) {
+        tq_f4 x[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const TQ_GLOBAL tq_f4 *>(p + min(r0 + k, records - 1u) * step);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            if (r0 + k >= records) continue;
+            const float own = lds_m[(r0 + k) * a.cols + c], l = lds_l[(r0 + k) * a.cols + c];
+            const float f = own != MANY_NONE ? __builtin_amdgcn_exp2f(own - top) : l == 0.f ? 0.f : __builtin_nanf("");
+            sum = fmaf(l, f, sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[k][e], f, o[e]);
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const uint32_t token = m / a.group;
+    const size_t first = ((size_t)((uint32_t)sq[0] + token) * (a.heads * a.group) + kv * a.group + (m - token * a.group)) * a.D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = inv == 0.f ? 0.f : o[e] * inv;
+    if (a.dtype == TQ_F32) {
+        TQ_GLOBAL float *out = reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out) + first;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = o[e];
+    } else {
+        TQ_GLOBAL uint16_t *out = reinterpret_cast<TQ_GLOBAL uint16_t *>((TQ_GLOBAL uint8_t *)a.out) + first;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = a.dtype == TQ_F16 ? __builtin_bit_cast(uint16_t, (_Float16)o[e]) : __builtin_bit_cast(uint16_t, (__bf16)o[e]);
+    }
+}
+
+bool supported(int D, int dtype, int bits_k, int bits_v) {
+    if (dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16) return false;
+    if (bits_k < 2 || bits_k > 8 || bits_v < 2 || bits_v > 8) return false;
+    if (D == 64 || D == 128 || D == 256) return true;
+    const int ik = 8 / bits_k, iv = 8 / bits_v;       // 65 to 96: whole groups of eight elements, and words of packed bytes
+    return D > 64 && D <= 96 && !(D & 7) && !(D % ik) && !(D % iv) && !(D / ik & 3) && !(D / iv & 3);
+}
+
+// Times in tokens: what a block's packed tokens, its uncompressed ones and its start and end cost, for one tile of queries and for two, and what a merge does.
+struct Costs {
+    long long token, plain, block;
+};
+Costs costs(int qt, int dtype) {
+    // (quarters of a token)
+    if (dtype == TQ_F32) return {12, 24, 6000};
+    if (qt == 2) return {6, 14, 8000};
+    return {4, 8, 6000};
+}
+
+struct Reach {                       // what a group of tiles sees of its sequence, in runs of 32
+    long long packed_from, packed_to, plain_from, plain_to;
+    long long runs(const Costs &c) const { return (packed_to - packed_from + 31) / 32 * 32 * c.token + (plain_to - plain_from + 31) / 32 * 32 * c.plain; }
+};
+Reach reach(const int32_t *s, long long group, long long window, long long tile0, long long tiles) {
+    const long long fresh = s[1], total = s[2], packed = s[3], first_pos = total - fresh + tile0 * 32 / group;
+    long long last = ((tile0 + tiles) * 32 - 1) / group;
+    if (last > fresh - 1) last = fresh - 1;
+    const long long end = total - fresh + last + 1, lo = window && first_pos >= window ? first_pos - window + 1 : 0;
+    Reach r;
+    r.packed_from = (lo < packed ? lo : packed) / 32 * 32;
+    r.packed_to = packed;
+    if (lo >= packed) r.packed_from = r.packed_to = 0;
+    r.plain_from = lo > packed ? (lo - packed) / 32 * 32 : 0;
+    r.plain_to = end - packed;
+    return r;
+}
+
+struct Group {
+    int32_t seq, tile0;
+    Reach reach;
+    long long cost;
+};
+
+}  // namespace
+
+extern "C" int tq_paged_supported(int head_dim, int dtype, int bits_k, int bits_v) { return supported(head_dim, dtype, bits_k, bits_v) ? 1 : 0; }
+
+extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int32_t *items, long long max_items, int32_t *merges,
+                             long long max_merges, tq_paged_counts *counts) {
+    if (!counts || (n > 0 && !sequences)) return TQ_ERR_NULL;
+    if (n < 0 || heads < 1 || group < 1 || window < 0 || max_items < 0 || max_merges < 0) return TQ_ERR_SIZE;
+    long long tiles = 0, most = 0;
+    for (long long b = 0; b < n; ++b) {
+        const int32_t *s = sequences + b * PAGED_SEQ;
+        if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[3] < 0 || s[3] > s[2] - s[1] || s[4] < 0 || s[5] < 0) return TQ_ERR_SIZE;
+        if ((long long)s[1] * group > 0x7fffffff - 64) return TQ_ERR_SIZE;
+        const long long t = ((long long)s[1] * group + 31) / 32;
+        tiles += t;
+        if (t > most) most = t;
+    }
+    *counts = tq_paged_counts{};
+    counts->tiles = 1;
+    if (!tiles) return TQ_OK;
+    int cus = 0;
+    if (tq_device_cus(cus)) cus = 256;
+    try {
+        // Of one or two tiles a block and up to MAX_PIECES pieces of the longest, the pair with the shortest time by the costs above: as many rounds of blocks as the card takes, each
+        // as long as a block is on average, and no less than the longest block.
+        std::vector<Group> best;
+        long long best_time = -1, best_piece = 0;
+        int best_qt = 1;
+        const bool two = dtype == TQ_BF16 && head_dim != 256 && most > 1;
+        for (int qt = 1; qt <= (two ? 2 : 1); ++qt) {
+            const Costs c = costs(qt, dtype);
+            std::vector<Group> groups;
+            long long longest = 0;
+            for (long long b = 0; b < n; ++b) {
+                const int32_t *s = sequences + b * PAGED_SEQ;
+                const long long t = ((long long)s[1] * group + 31) / 32;
+                for (long long t0 = 0; t0 < t; t0 += qt) {
+                    Group g{(int32_t)b, (int32_t)t0, reach(s, group, window, t0, qt), 0};
+                    g.cost = g.reach.runs(c);
+                    if (g.cost > longest) longest = g.cost;
+                    groups.push_back(g);
+                }
+            }
+            for (long long k = 1; k <= MAX_PIECES; ++k) {
+                long long piece = (longest + k - 1) / k;
+                if (piece < 128 * c.token && k > 1) break;
+                long long blocks = 0, all = 0, pieces = 1;
+                for (const Group &g : groups) {
+                    const long long own = g.cost ? (g.cost + piece - 1) / piece : 1;
+                    blocks += own;
+                    all += g.cost + own * c.block;
+                    if (own > pieces) pieces = own;
+                }
+                blocks *= heads;
+                all *= heads;
+                const long long rounds = (blocks + cus - 1) / cus;
+                long long time = rounds * (all / blocks);
+                if (time < piece + c.block) time = piece + c.block;
+                if (pieces > 1) time += 6000 + 120 * pieces;
+                if (best_time < 0 || time < best_time) { best_time = time; best_piece = piece; best_qt = qt; best.clear(); }
+                if (rounds > 16 && k > 1) break;
+            }
+            if (best_qt == qt && best.empty()) best.swap(groups);
+        }
+        const Costs c = costs(best_qt, dtype);
+        struct Item { int32_t v[PAGED_ITEM]; long long cost; };
+        std::vector<Item> all;
+        std::vector<int32_t> joined;
+        long long records = 0, columns = 1;
+        for (const Group &g : best) {
+            const Reach &r = g.reach;
+            const long long k = g.cost ? (g.cost + best_piece - 1) / best_piece : 1, each = (g.cost + k - 1) / k;
+            const size_t first = all.size();
+            long long t = r.packed_from, u = r.plain_from;
+            do {
+                Item it{{g.seq, g.tile0, 0, 0, 0, 0, -1, 0}, 0};
+                it.v[2] = (int32_t)t;
+                while (t < r.packed_to && it.cost < each) { t += 32; it.cost += 32 * c.token; }
+                if (t > r.packed_to) t = r.packed_to;
+                it.v[3] = (int32_t)t;
+                it.v[4] = (int32_t)u;
+                while (t >= r.packed_to && u < r.plain_to && it.cost < each) { u += 32; it.cost += 32 * c.plain; }
+                if (u > r.plain_to) u = r.plain_to;
+                it.v[5] = (int32_t)u;
+                all.push_back(it);
+            } while (t < r.packed_to || u < r.plain_to);
+            const long long own = (long long)(all.size() - first);
+            if (own > 1) {
+                joined.insert(joined.end(), {g.seq, g.tile0, (int32_t)records, (int32_t)own});
+                for (size_t i = first; i < all.size(); ++i) all[i].v[6] = (int32_t)records++;
+                const long long m = (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group - 32LL * g.tile0;
+                columns = std::max(columns, std::min(32LL, m));
+            }
+        }
+        // the longest first: what is short fills the gaps at the end
+        std::stable_sort(all.begin(), all.end(), [](const Item &x, const Item &y) { return x.cost > y.cost; });
+        counts->items = (long long)all.size();
+        counts->merges = (long long)joined.size() / PAGED_MERGE;
+        counts->records = records;
+        counts->tiles = best_qt;
+        counts->columns = (int)columns;
+        if (counts->items > 0x7fffffff / heads || records > 0x7fffffff) return TQ_ERR_SIZE;
+        if (counts->items > max_items || counts->merges > max_merges) return TQ_ERR_CAPACITY;
+        if (!items || (counts->merges && !merges)) return TQ_ERR_NULL;
+        for (size_t i = 0; i < all.size(); ++i) std::copy(all[i].v, all[i].v + PAGED_ITEM, items + i * PAGED_ITEM);
+        std::copy(joined.begin(), joined.end(), merges);
+    } catch (...) {
+        return TQ_ERR_CAPACITY;              // (no memory)
+    }
+    return TQ_OK;
+}
+
+extern "C" long long tq_paged_scratch(const tq_paged_counts *counts, int heads, int head_dim) {
+    if (!counts) return TQ_ERR_NULL;
+    if (head_dim < TQ_ANYDIM_MIN || head_dim > TQ_ANYDIM_MAX) return TQ_ERR_HEAD_DIM;
+    if (heads < 1 || counts->records < 0 || counts->tiles < 1 || counts->tiles > 2 || counts->columns < 0 || counts->columns > 32) return TQ_ERR_SIZE;
+    return counts->records * heads * counts->tiles * (long long)paged_record((uint32_t)counts->columns, (uint32_t)TQ_PADDED_DIM(head_dim));
+}
+
+extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, long long scratch_floats, void *stream) {
+    if (!request) return TQ_ERR_NULL;
+    const tq_paged_request &r = *request;
+    const tq_paged_counts &n = r.counts;
+    if (r.dtype != TQ_F32 && r.dtype != TQ_F16 && r.dtype != TQ_BF16) return TQ_ERR_DTYPE;
+    if (r.bits_k < 1 || r.bits_k > 8 || r.bits_v < 1 || r.bits_v > 8) return TQ_ERR_BITS;
+    if (!supported(r.head_dim, r.dtype, r.bits_k, r.bits_v)) return TQ_ERR_HEAD_DIM;
+    if (r.heads < 1 || r.group < 1 || r.sliding_window < 0 || r.heads * (long long)r.group > 0x7fffffff) return TQ_ERR_SIZE;
+    if (r.page_tokens < 32 || (r.page_tokens & (r.page_tokens - 1)) || r.page_tokens > 65536) return TQ_ERR_SIZE;
+    if (r.page_tokens > 0x7fffffff / r.heads / (r.head_dim * 4)) return TQ_ERR_SIZE;
+    if (!(r.softcap >= 0.f) || !(r.softcap < __builtin_inff()) || n.items < 0 || n.merges < 0 || n.records < 0) return TQ_ERR_SIZE;
+    if (n.items == 0) return TQ_OK;
+    if (n.items > 0x7fffffff / r.heads || n.tiles < 1 || n.tiles > 2 || n.columns < 1 || n.columns > 32) return TQ_ERR_SIZE;
+    if (n.tiles == 2 && (r.dtype != TQ_BF16 || r.head_dim == 256)) return TQ_ERR_SIZE;
+    if (!r.queries || !r.out || !r.packed_pool || !r.plain_pool || !r.table_k || !r.table_v || !r.sequences || !r.tables || !r.items || (n.merges && (!r.merges || !scratch))) return TQ_ERR_NULL;
+    const long long es = r.dtype == TQ_F32 ? 4 : 2;
+    // vectors of a page as the kernels read them: runs of 32 tokens 16 bytes at a time (packed bytes of uneven dimensions: words)
+    if ((((uintptr_t)r.packed_pool | (uintptr_t)r.plain_pool | (uintptr_t)r.table_k | (uintptr_t)r.table_v) & 15u) ||
+        ((r.packed_page_stride | r.plain_page_stride | r.k_norms | r.v_idx | r.v_norms | r.plain_values) & 15) || ((uintptr_t)scratch & 15u) || ((uintptr_t)r.queries & (es - 1)) ||
+        ((uintptr_t)r.out & (es - 1)) || (((uintptr_t)r.sequences | (uintptr_t)r.tables | (uintptr_t)r.items | (uintptr_t)r.merges | (uintptr_t)r.slopes) & 3u))
+        return TQ_ERR_ALIGN;
+    if (scratch_floats < tq_paged_scratch(&n, r.heads, r.head_dim)) return TQ_ERR_CAPACITY;
+    TqPagedArgs a{};
+    a.q = static_cast<const uint8_t *>(r.queries); a.out = static_cast<uint8_t *>(r.out);
+    a.q_token = r.q_token; a.q_head = r.q_head;
+    a.pool = static_cast<const uint8_t *>(r.packed_pool); a.plain = static_cast<const uint8_t *>(r.plain_pool);
+    a.page_stride = r.packed_page_stride; a.plain_stride = r.plain_page_stride;
+    a.k_norms = r.k_norms; a.v_idx = r.v_idx; a.v_norms = r.v_norms; a.plain_v = r.plain_values;
+    a.table_k = static_cast<const uint8_t *>(r.table_k); a.table_v = static_cast<const uint8_t *>(r.table_v);
+    a.seqs = r.sequences; a.tables = r.tables; a.items = r.items; a.merges = r.merges; a.slopes = r.slopes;
+    a.rec = scratch;
+    a.scale = r.scale; a.cap = r.softcap;
+    a.heads = (uint32_t)r.heads; a.group = (uint32_t)r.group; a.D = (uint32_t)r.head_dim; a.dtype = (uint32_t)r.dtype;
+    a.bits_k = (uint32_t)r.bits_k; a.bits_v = (uint32_t)r.bits_v;
+    a.shift = (uint32_t)__builtin_ctz((unsigned)r.page_tokens);
+    a.cols = (uint32_t)n.columns; a.window = (uint32_t)r.sliding_window;
+    a.aligned = !((uintptr_t)r.queries & 15u) && !((r.q_token * es) & 15) && !((r.q_head * es) & 15);
+    const int kt = r.dtype == TQ_BF16 ? 1 : 2, vt = r.dtype == TQ_F32 ? 2 : 1, dp = TQ_PADDED_DIM(r.head_dim), ik = 8 / r.bits_k, iv = 8 / r.bits_v;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 g((unsigned)(n.items * r.heads));
+    if (dp == 64) tq_paged_launch_d64(ik, iv, g, s, a, n.tiles, kt, vt);
+    else if (dp == 96) tq_paged_launch_d96(ik, iv, g, s, a, n.tiles, kt, vt);
+    else if (dp == 128) tq_paged_launch_d128(ik, iv, g, s, a, n.tiles, kt, vt);
+    else tq_paged_launch_d256(ik, iv, g, s, a, n.tiles, kt, vt);
+    if (n.merges) {
+        const uint32_t qt = (uint32_t)n.tiles, shares = ((uint32_t)n.columns * (dp / 4u) + MERGE_THREADS - 1u) / MERGE_THREADS;
+        const dim3 gm((unsigned)(n.merges * r.heads * qt * shares)), t(MERGE_THREADS);
+        if (dp == 64) hipLaunchKernelGGL((tq_paged_merge_kernel<64>), gm, t, 0, s, a, qt, shares);
+        else if (dp == 96) hipLaunchKernelGGL((tq_paged_merge_kernel<96>), gm, t, 0, s, a, qt, shares);
+        else if (dp == 128) hipLaunchKernelGGL((tq_paged_merge_kernel<128>), gm, t, 0, s, a, qt, shares);
+        else hipLaunchKernelGGL((tq_paged_merge_kernel<256>), gm, t, 0, s, a, qt, shares);
+    }
+    return (int)hipGetLastError();
+}

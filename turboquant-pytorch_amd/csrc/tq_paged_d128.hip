@@ -1,0 +1,3 @@
+#include "tq_paged_kernel.h"
+
+int tq_paged_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt) { return launch_paged<128>(ipbk, ipbv, grid, s, a, qt, kt, vt); }

@@ -26,6 +26,7 @@ from typing import Dict, NamedTuple, Optional, Tuple
 import torch
 
 from . import _native
+from .beams import beam_select
 from .compressors_v3 import TurboQuantV3
 
 
@@ -239,6 +240,21 @@ class _LayerStore:
         self.weights, self.n_compressed = weights, keep
         self._consts = self._record = None
         return kept
+
+    def segments(self) -> list:
+        """What a sequence holds, as runs a kv head: (address, bytes between sequences, between heads, bytes).  Packed runs to a multiple of 16 bytes, which their capacity has room for."""
+        out = []
+        n = self.n_compressed
+        if n:
+            for t in (self.k_idx, self.k_nrm, self.v_idx, self.v_nrm):
+                token = t[0, 0, 0].numel() * t.element_size()
+                out.append((t, 0, min(-(-n * token // 16) * 16, self.capacity * token)))
+        if self.n_recent:
+            token = self.D * self.k_win.element_size()
+            out += [(t, self.w0 * token, self.n_recent * token) for t in (self.k_win, self.v_win)]
+        if self.weights is not None and n + self.n_recent:
+            out.append((self.weights, 0, 4 * (n + self.n_recent)))
+        return [(t.data_ptr() + first, t.stride(0) * t.element_size(), t.stride(1) * t.element_size(), size) for t, first, size in out]
 
     def window(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """Views [B,H,n_recent,D] of the uncompressed keys and values, oldest first."""
@@ -528,6 +544,37 @@ class V3Cache:
         self.attention_weights(layer_idx)          # (raises where there are none)
         return self._stores[layer_idx].evict(int(keep))
 
+    @torch.compiler.disable
+    @torch.no_grad()
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Sequence b of the batch goes on from what sequence parents[b] was, in every layer: packed tokens, window and kept sums, in place.  parents [B] (whole numbers, on the
+        cache's device: the host does not wait for them); one outside the batch leaves its sequence as it is.  At most 1024 sequences."""
+        stores = list(self._stores.values())
+        if not stores:
+            return
+        if not isinstance(parents, torch.Tensor) or parents.dim() != 1 or parents.dtype.is_floating_point or parents.dtype.is_complex or parents.dtype == torch.bool:
+            raise ValueError("reorder: parents must be a tensor of whole numbers, one for each sequence")
+        if any(parents.shape[0] != st.B for st in stores):
+            raise ValueError(f"reorder: {parents.shape[0]} parents for a batch of {stores[0].B}")
+        if parents.shape[0] > 1024:
+            raise ValueError(f"reorder: at most 1024 sequences, got {parents.shape[0]}")
+        _native._require_gpu(parents, "parents")
+        groups: Dict[Tuple[torch.device, int], list] = {}
+        for st in stores:
+            groups.setdefault((st.device, st.H), []).extend(st.segments())
+        for (device, heads), segments in groups.items():
+            _native.reorder(segments, parents, heads, device)
+
+    def beam_step(self, logits: torch.Tensor, scores: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One step of beam search over a cache whose batch is groups x beams: of every group (logits [groups, beams, vocabulary], scores [groups, beams]) the `beams` best
+        continuations, (scores, tokens, parents) [groups, beams] of `beam_select`, and the cache reordered by them."""
+        if logits.dim() != 3 or any(st.B != logits.shape[0] * logits.shape[1] for st in self._stores.values()):
+            raise ValueError(f"beam_step: logits must be [groups, beams, vocabulary] with groups x beams sequences as the cache has; got {tuple(logits.shape)}")
+        chosen = beam_select(logits, scores, logits.shape[1])
+        first = torch.arange(logits.shape[0], device=logits.device).unsqueeze(1) * logits.shape[1]
+        self.reorder((chosen[2] + first).flatten())
+        return chosen
+
     @staticmethod
     def _attend_step(st: _LayerStore, query_states: torch.Tensor, G: int, scale: float) -> Optional[torch.Tensor]:
         """The fused path of `attend` in one library call (rotate + window, packed history, merge): one launch with the
@@ -655,6 +702,11 @@ def hf_cache_class():
                 while len(layers) <= layer_idx:
                     layers.append(DynamicLayer())
             return out
+
+        def reorder_cache(self, beam_idx):
+            """Beam search: sequence b goes on from sequence beam_idx[b]."""
+            self._no_pending("reorder_cache")
+            V3Cache.reorder(self, beam_idx)
 
         def get_seq_length(self, layer_idx=0):
             self._no_pending("get_seq_length")

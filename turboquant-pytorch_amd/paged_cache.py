@@ -1,0 +1,610 @@
+"""
+Compressed KV cache in pages, for sequences of different lengths that are served together.
+
+`V3Cache` holds one batch whose sequences are equally long.  `PagedV3Cache` holds any number of sequences in two pools: whole pages of packed
+tokens, bit for bit what `V3Cache` packs, and uncompressed pages for the most recent `residual_window` tokens of a sequence and what fills up its next page.  A page is the
+same page of every layer, so that a sequence has one table of pages, and copying or sharing a page is one copy or none.
+
+A step gives sequences new tokens, one each (decoding) or many (chunks of prompts), mixed as they come:
+
+    step = cache.step(seqs, counts)
+    for layer in ...:
+        step.append(keys, values, layer)            # [new tokens, kv heads, D], sequence after sequence
+        out = step.attend(queries, layer)           # [new tokens, query heads, D], causal
+    step.commit()                                   # pages that have become old enough are packed
+
+The step's own tokens are attended to as they are; what is packed, and with which codec, is as in `V3Cache` (the reference's generation-time cache,
+turboquant/generation_test_v2.py:48-165), but a page at a time.  Lengths and tables live on the host.
+"""
+from __future__ import annotations
+
+import ctypes
+import heapq
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _native
+from .beams import beam_select
+from .compressors_v3 import TurboQuantV3
+
+_JOB = np.dtype([("states", np.uint64), ("idx_bytes", np.uint64), ("vec_norms", np.uint64), ("table", np.uint64), ("rows", np.int64), ("tokens", np.int64), ("row_stride", np.int64),
+                 ("token_stride", np.int64), ("bits", np.int32), ("dtype", np.int32), ("packed_row_stride", np.int64)])
+_PAIR = np.dtype([("from", np.int32), ("to", np.int32), ("bytes", np.int32)])
+assert _JOB.itemsize == ctypes.sizeof(_native.TqJob)
+MAX_JOBS = 4096                     # TQ_MAX_JOBS of include/tqamd.h
+
+
+class _Pages:
+    """Numbers of the pages of a pool: which are free, and how many sequences hold each of the others.  The lowest free one goes first."""
+
+    def __init__(self, count: int):
+        self.free = list(range(count))
+        self.held = [0] * count
+
+    def take(self) -> int:
+        page = heapq.heappop(self.free)
+        self.held[page] = 1
+        return page
+
+    def drop(self, page: int) -> bool:
+        self.held[page] -= 1
+        if self.held[page]:
+            return False
+        heapq.heappush(self.free, page)
+        return True
+
+
+class _Sequence:
+    __slots__ = ("pages", "plain", "total")
+
+    def __init__(self):
+        self.pages: List[int] = []
+        self.plain: List[int] = []
+        self.total = 0
+
+
+def _up(n: int) -> int:
+    return -(-n // 256) * 256
+
+
+class PagedV3Cache:
+    """head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose packed vectors are whole words; 2 to 8 bits.  pages, plain_pages: how many packed and uncompressed pages of
+    page_tokens tokens (a power of two, 32 to 1024) the pools have, over all layers at once; a sequence needs a packed page for every page_tokens tokens
+    and uncompressed ones for its window, a page that is being filled and the tokens of a step."""
+
+    def __init__(self, head_dim: int, kv_heads: int, key_bits: int = 4, value_bits: int = 2, residual_window: int = 128, protected_layers: int = 0, n_layers: int = 36, *,
+                 pages: int, plain_pages: int, page_tokens: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        for name, n, least in (("kv_heads", kv_heads, 1), ("n_layers", n_layers, 1), ("residual_window", residual_window, 0), ("pages", pages, 1), ("plain_pages", plain_pages, 1)):
+            if isinstance(n, bool) or int(n) != n or n < least:
+                raise ValueError(f"{name} must be a whole number, {least} or more; got {n!r}")
+        if page_tokens not in (32, 64, 128, 256, 512, 1024):
+            raise ValueError(f"page_tokens must be a power of two from 32 to 1024; got {page_tokens!r}")
+        code = _native.dtype_code(dtype)
+        self.head_dim, self.kv_heads, self.n_layers, self.residual_window, self.page_tokens = int(head_dim), int(kv_heads), int(n_layers), int(residual_window), page_tokens
+        self.dtype = dtype
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise _native.TqError(f"a paged cache lives on a HIP device (got {dev}); this package has no CPU path")
+        self._codecs = [TurboQuantV3(head_dim=head_dim, key_bits=key_bits, value_bits=value_bits, residual_window=0, layer_idx=i, n_layers=n_layers,
+                                     protected_layers=protected_layers, seed=42, device="cpu") for i in range(n_layers)]
+        for c in self._codecs:
+            if not _native.lib().tq_paged_supported(head_dim, code, c.key_bits, c.value_bits):
+                raise ValueError(f"no paged attention for head_dim {head_dim} at {c.key_bits} and {c.value_bits} bits: head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose "
+                                 "packed vectors are whole words, and 2 to 8 bits")
+        self.device = dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
+        # a packed page: of every layer key codes, key norms, value codes, value norms
+        H, P, at = self.kv_heads, page_tokens, 0
+        self._parts = []
+        for c in self._codecs:
+            widths = [-(-head_dim // (8 // b)) for b in (c.key_bits, c.value_bits)]
+            offsets = []
+            for size in (H * P * widths[0], 2 * H * P, H * P * widths[1], 2 * H * P):
+                offsets.append(at)
+                at += _up(size)
+            self._parts.append((*offsets, *widths))
+        self._page_bytes, self._plain_shape = at, (self.n_layers, 2, H, P, self.head_dim)
+        self._pool = torch.empty((pages, at), dtype=torch.uint8, device=self.device)
+        self._plain = torch.empty((plain_pages,) + self._plain_shape, dtype=dtype, device=self.device)
+        self._packed_pages, self._plain_pages = _Pages(pages), _Pages(plain_pages)
+        self._packed_of: Dict[int, int] = {}         # uncompressed pages still held by others -> the packed page one of their sequences made of them
+        self._seqs: Dict[int, _Sequence] = {}
+        self._next = 0
+        self._open: Optional[PagedStep] = None
+
+    # ---- what is there --------------------------------------------------------------------------------------------------------
+    def codec(self, layer_idx: int) -> TurboQuantV3:
+        """The layer's codec (the one `V3Cache` has for the same widths and layers)."""
+        return self._codecs[layer_idx]
+
+    def packed_pages(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The layer's part of every packed page, views of the pool: key codes [pages, H, page_tokens, width], key norms [pages, H, page_tokens], and the same of values."""
+        H, P, n = self.kv_heads, self.page_tokens, self._pool.shape[0]
+        k, kn, v, vn, wk, wv = self._parts[layer_idx]
+        halves = self._pool.view(torch.float16)
+        codes = lambda at, w: self._pool.as_strided((n, H, P, w), (self._page_bytes, P * w, w, 1), at)  # noqa: E731
+        norms = lambda at: halves.as_strided((n, H, P), (self._page_bytes // 2, P, 1), at // 2)  # noqa: E731
+        return codes(k, wk), norms(kn), codes(v, wv), norms(vn)
+
+    def plain_pages(self) -> torch.Tensor:
+        """The uncompressed pool, [pages, layers, keys and values, H, page_tokens, D]."""
+        return self._plain
+
+    def tables(self, seq: int) -> Tuple[List[int], List[int]]:
+        """Numbers of a sequence's packed and uncompressed pages, in the order of its tokens."""
+        s = self._sequence(seq)
+        return list(s.pages), list(s.plain)
+
+    def lengths(self, seqs: Sequence[int]) -> List[int]:
+        """Tokens of sequences, those of an open step among them."""
+        return [self._sequence(s).total for s in seqs]
+
+    def free_pages(self) -> Tuple[int, int]:
+        """How many packed and uncompressed pages no sequence holds."""
+        return len(self._packed_pages.free), len(self._plain_pages.free)
+
+    def stored_bytes(self) -> int:
+        """Bytes of the pages that are held, packed and uncompressed."""
+        used = [sum(map(bool, p.held)) for p in (self._packed_pages, self._plain_pages)]
+        return used[0] * self._page_bytes + used[1] * int(np.prod(self._plain_shape)) * self._plain.element_size()
+
+    def _sequence(self, seq: int) -> _Sequence:
+        s = self._seqs.get(seq)
+        if s is None:
+            raise ValueError(f"no sequence {seq!r} in this cache")
+        return s
+
+    def _eager(self, what: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} reads and changes tables on the host: it cannot be recorded into a graph (`append` and `attend` of a step made before can)")
+
+    # ---- sequences come, continue more than once, and go --------------------------------------------------------------------------
+    def add(self, count: int = 1) -> List[int]:
+        """New, empty sequences."""
+        if isinstance(count, bool) or int(count) != count or count < 0:
+            raise ValueError(f"count must be a whole number, 0 or more; got {count!r}")
+        new = list(range(self._next, self._next + int(count)))
+        self._next += int(count)
+        for s in new:
+            self._seqs[s] = _Sequence()
+        return new
+
+    def place(self, seqs: Sequence[int], packed: Sequence[int], plain: Sequence[int]) -> None:
+        """Pages for sequences that are empty so far, `packed` (whole pages) and `plain` tokens, whose contents the caller writes (`packed_pages`, `plain_pages`, `tables`): stores
+        that come from elsewhere."""
+        self._settle()
+        states = [self._sequence(s) for s in seqs]
+        if not len(states) == len(packed) == len(plain) or len(set(seqs)) != len(states):
+            raise ValueError("place: one number of packed and one of plain tokens for each of different sequences")
+        if any(s.total for s in states) or any(p < 0 or p % self.page_tokens for p in packed) or any(n < 0 for n in plain):
+            raise ValueError(f"place: sequences must be empty, packed tokens a multiple of {self.page_tokens}")
+        self._room("place", sum(p // self.page_tokens for p in packed), sum(-(-n // self.page_tokens) for n in plain))
+        for s, p, n in zip(states, packed, plain):
+            s.pages = [self._packed_pages.take() for _ in range(p // self.page_tokens)]
+            s.plain = [self._plain_pages.take() for _ in range(-(-n // self.page_tokens))]
+            s.total = int(p) + int(n)
+
+    def _room(self, what: str, packed: int, plain: int) -> None:
+        free = self.free_pages()
+        if packed > free[0] or plain > free[1]:
+            raise _native.TqError(f"{what} needs {packed} packed and {plain} uncompressed pages, {free[0]} and {free[1]} are free (free sequences, or `resize`)")
+
+    def _drop_plain(self, page: int) -> None:
+        if self._plain_pages.drop(page):
+            self._packed_of.pop(page, None)
+
+    def _drop_packed(self, page: int) -> None:
+        if self._packed_pages.drop(page):
+            for plain, packed in list(self._packed_of.items()):
+                if packed == page:
+                    del self._packed_of[plain]
+
+    def _settle(self) -> None:
+        """An open step is committed before tables change."""
+        if self._open is not None:
+            self._open.commit()
+
+    def free(self, seqs: Sequence[int]) -> None:
+        """Sequences end; pages that no other one holds are free."""
+        self._settle()
+        states = [self._sequence(s) for s in seqs]
+        if len(set(seqs)) != len(states):
+            raise ValueError("free: a sequence ends once")
+        for seq, s in zip(seqs, states):
+            for p in s.pages:
+                self._drop_packed(p)
+            for p in s.plain:
+                self._drop_plain(p)
+            del self._seqs[seq]
+
+    def _share(self, s: _Sequence, copies: List[Tuple[int, int, int]], own_last: bool) -> _Sequence:
+        """A sequence that continues as `s`: whole pages are held together, the one that is being filled is copied (own_last: taken over)."""
+        new = _Sequence()
+        new.pages, new.plain, new.total = list(s.pages), list(s.plain), s.total
+        for p in new.pages:
+            self._packed_pages.held[p] += 1
+        filled = s.total % self.page_tokens
+        for p in new.plain:
+            self._plain_pages.held[p] += 1
+        if filled and not own_last:
+            copies.append((new.plain[-1], -1, filled))
+        return new
+
+    def _copy_last(self, new: Sequence[_Sequence], copies: Sequence[Tuple[int, int, int]]) -> None:
+        """Pages of their own for the sequences of `new`, one for each of `copies`, whose last page is another's."""
+        if not copies:
+            return
+        pairs = np.empty(len(copies), dtype=_PAIR)
+        for i, (s, (source, _, filled)) in enumerate(zip(new, copies)):
+            target = self._plain_pages.take()
+            self._plain_pages.drop(source)           # (its owner still holds it)
+            s.plain[-1] = target
+            pairs[i] = (source, target, filled)
+        vector = self.head_dim * self._plain.element_size()
+        pairs["bytes"] *= vector
+        self._move(self._plain, self._plain, int(np.prod(self._plain_shape[:3])), self.page_tokens * vector, pairs)
+
+    def _move(self, source: torch.Tensor, target: torch.Tensor, rows: int, row_bytes: int, pairs: np.ndarray) -> None:
+        stride = lambda t: t.stride(0) * t.element_size()  # noqa: E731
+        with _native._on(self.device):
+            _native.check(_native.lib().tq_copy_pages(source.data_ptr(), stride(source), target.data_ptr(), stride(target), rows, row_bytes, pairs.ctypes.data, len(pairs),
+                                                      _native._stream_handle(self.device)), "tq_copy_pages")
+
+    def fork(self, seqs: Sequence[int]) -> List[int]:
+        """For each of `seqs` (one may be there more than once) a new sequence that begins as it is: whole pages are shared, one that is being filled is copied."""
+        self._eager("fork")
+        self._settle()
+        states = [self._sequence(s) for s in seqs]
+        self._room("fork", 0, sum(1 for s in states if s.total % self.page_tokens))
+        copies: List[Tuple[int, int, int]] = []
+        fresh = [self._share(s, copies, False) for s in states]
+        self._copy_last([f for f in fresh if f.total % self.page_tokens], copies)
+        new = self.add(len(states))
+        for seq, f in zip(new, fresh):
+            self._seqs[seq] = f
+        return new
+
+    def reorder(self, seqs: Sequence[int], parents) -> None:
+        """Sequence seqs[i] goes on from what seqs[parents[i]] is (beams that were chosen).  parents: whole numbers, a list or a tensor (which is waited for).
+        Pages are shared; of several that go on from one, all but one get a copy of the page that is being filled."""
+        self._eager("reorder")
+        self._settle()
+        states = [self._sequence(s) for s in seqs]
+        if isinstance(parents, torch.Tensor):
+            if parents.dtype.is_floating_point or parents.dtype == torch.bool:
+                raise ValueError(f"reorder: parents must be whole numbers, got {parents.dtype}")
+            parents = parents.flatten().tolist()
+        parents = list(parents)
+        if len(parents) != len(states) or len(set(seqs)) != len(states) or any(isinstance(p, bool) or int(p) != p or not 0 <= p < len(states) for p in parents):
+            raise ValueError(f"reorder: for each of {len(states)} different sequences the place of one among them")
+        # who takes over the page that is being filled: the sequence itself if it goes on, otherwise the first that goes on from it
+        heir: Dict[int, int] = {}
+        for i, p in enumerate(parents):
+            if p not in heir or i == p:
+                heir[p] = i
+        twice = sum(1 for i, p in enumerate(parents) if heir[p] != i and states[p].total % self.page_tokens)
+        # (pages of the ones that end become free first)
+        ends = sum(1 for p, s in enumerate(states) if p not in heir for page in s.plain if self._plain_pages.held[page] == 1)
+        self._room("reorder", 0, max(0, twice - ends))
+        copies: List[Tuple[int, int, int]] = []
+        fresh = [self._share(states[p], copies, heir[p] == i) for i, p in enumerate(parents)]
+        for s in states:
+            for page in s.pages:
+                self._drop_packed(page)
+            for page in s.plain:
+                self._drop_plain(page)
+        self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i and f.total % self.page_tokens], copies)
+        for seq, f in zip(seqs, fresh):
+            self._seqs[seq] = f
+
+    def beam_step(self, seqs: Sequence[int], logits: torch.Tensor, scores: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One step of beam search: of every group of beams (logits [groups, beams, vocabulary], scores [groups, beams]; seqs group after group) the `beams` best continuations,
+        (scores, tokens, parents) [groups, beams] of `beam_select`, and the sequences reordered by them.  Waits for the parents."""
+        if logits.dim() != 3 or len(seqs) != logits.shape[0] * logits.shape[1]:
+            raise ValueError(f"beam_step: logits [groups, beams, vocabulary] for {len(seqs)} sequences, got {tuple(logits.shape)}")
+        chosen = beam_select(logits, scores, logits.shape[1])
+        first = torch.arange(logits.shape[0], device=chosen[2].device).unsqueeze(1) * logits.shape[1]
+        self.reorder(seqs, chosen[2] + first)
+        return chosen
+
+    def resize(self, pages: Optional[int] = None, plain_pages: Optional[int] = None) -> None:
+        """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered, sequence after sequence."""
+        self._eager("resize")
+        self._settle()
+        orders = []
+        for name, get in (("pages", lambda s: s.pages), ("plain_pages", lambda s: s.plain)):
+            order: Dict[int, int] = {}
+            for seq in sorted(self._seqs):
+                for p in get(self._seqs[seq]):
+                    order.setdefault(p, len(order))
+            orders.append(order)
+        sizes = []
+        for name, asked, order in (("pages", pages, orders[0]), ("plain_pages", plain_pages, orders[1])):
+            n = max(1, len(order)) if asked is None else asked
+            if isinstance(n, bool) or int(n) != n or n < max(1, len(order)):
+                raise ValueError(f"resize: {name} must be a whole number, {max(1, len(order))} or more (as many are held); got {n!r}")
+            sizes.append(int(n))
+        pool = torch.empty((sizes[0], self._page_bytes), dtype=torch.uint8, device=self.device)
+        plain = torch.empty((sizes[1],) + self._plain_shape, dtype=self.dtype, device=self.device)
+        vector = self.head_dim * self._plain.element_size()
+        for source, target, order, rows, row_bytes in ((self._pool, pool, orders[0], 1, self._page_bytes),
+                                                       (self._plain, plain, orders[1], int(np.prod(self._plain_shape[:3])), self.page_tokens * vector)):
+            if order:
+                pairs = np.empty(len(order), dtype=_PAIR)
+                pairs["from"], pairs["to"], pairs["bytes"] = list(order), list(order.values()), row_bytes
+                self._move(source, target, rows, row_bytes, pairs)
+        self._pool, self._plain = pool, plain
+        for which, (order, size) in enumerate(zip(orders, sizes)):
+            old, new = (self._packed_pages, self._plain_pages)[which], _Pages(size)
+            for p, q in order.items():
+                new.held[q] = old.held[p]
+            new.free = list(range(len(order), size))
+            if which == 0:
+                self._packed_pages = new
+            else:
+                self._plain_pages = new
+        for s in self._seqs.values():
+            s.pages, s.plain = [orders[0][p] for p in s.pages], [orders[1][p] for p in s.plain]
+        self._packed_of = {orders[1][p]: orders[0][q] for p, q in self._packed_of.items()}
+
+    # ---- steps ----------------------------------------------------------------------------------------------------------------
+    def step(self, seqs: Sequence[int], counts) -> "PagedStep":
+        """Room for counts[i] new tokens (or `counts` each) of sequence seqs[i].  An open step is committed first."""
+        self._eager("step")
+        self._settle()
+        seqs = list(seqs)
+        states = [self._sequence(s) for s in seqs]
+        counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
+        if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(isinstance(c, bool) or int(c) != c or c < 0 for c in counts):
+            raise ValueError("step: for each of different sequences a whole number of new tokens, 0 or more")
+        counts = [int(c) for c in counts]
+        P = self.page_tokens
+        need = [max(0, -(-(s.total - len(s.pages) * P + c) // P) - len(s.plain)) for s, c in zip(states, counts)]
+        if any(s.total + c > 0x7fffffff - 65536 for s, c in zip(states, counts)):
+            raise ValueError("step: a sequence of more than 2^31 tokens")
+        self._room("step", 0, sum(need))
+        self._open = PagedStep(self, seqs, states, counts, need)
+        return self._open
+
+
+class PagedStep:
+    """New tokens of some sequences of a `PagedV3Cache`: `append` for every layer, `attend` where it is wanted, then `commit` (the next step or any other call that changes tables commits
+    what is open).  Where a graph is recorded, the step has to be made before, and `attend` called once with the same window before the recording; replays work on the step's tokens."""
+
+    def __init__(self, cache: PagedV3Cache, seqs, states, counts, need):
+        self.cache, self.seqs, self.counts = cache, seqs, counts
+        self._states = states
+        self.tokens = sum(counts)
+        P = cache.page_tokens
+        records = np.zeros((len(seqs), _native.PAGED_SEQ), dtype=np.int32)
+        tables, slots, at = [], [], 0
+        for i, (s, c, n) in enumerate(zip(states, counts, need)):
+            s.plain.extend(cache._plain_pages.take() for _ in range(n))
+            first = s.total - len(s.pages) * P
+            s.total += c
+            places = np.arange(first, first + c)
+            slots.append(np.asarray(s.plain, dtype=np.int64)[places // P] * P + places % P if c else places)
+            begin = sum(map(len, tables))
+            records[i, :6] = at, c, s.total, len(s.pages) * P, begin, begin + len(s.pages)
+            tables += [s.pages, s.plain]
+            at += c
+        self._records = records
+        self._sections = [records.ravel(), np.concatenate([np.asarray(t, dtype=np.int32) for t in tables] or [np.zeros(0, np.int32)]), np.concatenate(slots or [np.zeros(0)]).astype(np.int32)]
+        self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
+        self._plans: Dict[Tuple[int, int], tuple] = {}
+        self._ready: Dict[tuple, tuple] = {}
+        self._appended: set = set()
+        self._done = False
+
+    def _upload(self, sections: Sequence[np.ndarray]) -> Tuple[torch.Tensor, List[int]]:
+        """Whole numbers onto the card, in one copy; addresses of the sections."""
+        at, starts = 0, []
+        for s in sections:
+            starts.append(at)
+            at += -(-max(s.size, 1) // 4) * 4
+        host = torch.empty(at, dtype=torch.int32, pin_memory=True)
+        flat = host.numpy()
+        for s, lo in zip(sections, starts):
+            flat[lo:lo + s.size] = s
+        blob = host.to(self.cache.device, non_blocking=True)
+        event = torch.cuda.Event()
+        with torch.cuda.device(self.cache.device):
+            event.record()
+        stream = _native._stream_handle(self.cache.device)
+        return (blob, event, stream), [blob.data_ptr() + 4 * lo for lo in starts]
+
+    def _await(self, uploaded) -> None:
+        """The upload is done before this stream goes on, and its memory stays while the stream reads it."""
+        blob, event, stream = uploaded
+        if _native._stream_handle(self.cache.device) != stream and not torch.cuda.is_current_stream_capturing():
+            current = torch.cuda.current_stream(self.cache.device)
+            current.wait_event(event)
+            blob.record_stream(current)
+
+    def _live(self, what: str) -> None:
+        if self._done:
+            raise RuntimeError(f"{what}: the step is committed")
+
+    def _layer(self, layer_idx: int) -> int:
+        if isinstance(layer_idx, bool) or int(layer_idx) != layer_idx or not 0 <= layer_idx < self.cache.n_layers:
+            raise ValueError(f"layer_idx must be a whole number from 0 to {self.cache.n_layers - 1}, got {layer_idx!r}")
+        return int(layer_idx)
+
+    @torch.compiler.disable
+    @torch.no_grad()
+    def append(self, keys: torch.Tensor, values: torch.Tensor, layer_idx: int) -> None:
+        """The new tokens' keys and values of a layer, [new tokens, kv heads, D], sequence after sequence in the step's order."""
+        self._live("append")
+        c, layer = self.cache, self._layer(layer_idx)
+        shape = (self.tokens, c.kv_heads, c.head_dim)
+        for name, t in (("keys", keys), ("values", values)):
+            if tuple(t.shape) != shape or t.dtype != c.dtype:
+                raise ValueError(f"append: {name} must be {list(shape)} {c.dtype}, got {tuple(t.shape)} {t.dtype}")
+            if t.device != c.device:
+                raise _native.TqError(f"append: {name} on {t.device}, the cache on {c.device}")
+        self._appended.add(layer)
+        if not self.tokens:
+            return
+        keys, values = (t if t.stride(2) == 1 and min(t.stride()) >= 0 else t.contiguous() for t in (keys, values))
+        es = keys.element_size()
+        with _native._on(c.device):
+            self._await(self._blob)
+            pool = c._plain[:, layer]
+            _native.check(_native.lib().tq_put_tokens(keys.data_ptr(), values.data_ptr(), keys.stride(0) * es, keys.stride(1) * es, values.stride(0) * es, values.stride(1) * es,
+                                                      pool.data_ptr(), pool.stride(0) * es, pool.stride(1) * es, self._slot_at, self.tokens, c.kv_heads, c.head_dim * es, c.page_tokens,
+                                                      _native._stream_handle(c.device)), "tq_put_tokens")
+
+    def _plan(self, group: int, window: int) -> tuple:
+        """How the blocks of the attention share the step's work, on the card: (counts, items, merges, scratch)."""
+        key = (group, window)
+        plan = self._plans.get(key)
+        if plan is None:
+            self.cache._eager("the first attend of a step with this window")
+            c, counts = self.cache, _native.TqPagedCounts()
+            call = lambda items, merges: _native.lib().tq_paged_plan(  # noqa: E731
+                self._records.ctypes.data, len(self.seqs), c.kv_heads, group, window, c.head_dim, _native.dtype_code(c.dtype), items.ctypes.data, len(items), merges.ctypes.data,
+                len(merges), ctypes.byref(counts))
+            items, merges = np.empty((1024, _native.PAGED_ITEM), np.int32), np.empty((256, _native.PAGED_MERGE), np.int32)
+            with _native._on(c.device):
+                rc = call(items, merges)
+                if rc == _native.ERR_CAPACITY:
+                    items, merges = np.empty((counts.items, _native.PAGED_ITEM), np.int32), np.empty((max(1, counts.merges), _native.PAGED_MERGE), np.int32)
+                    rc = call(items, merges)
+            _native.check(rc, "tq_paged_plan")
+            floats = int(_native.lib().tq_paged_scratch(ctypes.byref(counts), c.kv_heads, c.head_dim))
+            uploaded, (items_at, merges_at) = self._upload([items[:counts.items].ravel(), merges[:counts.merges].ravel()])
+            plan = self._plans[key] = (counts, items_at, merges_at, floats, uploaded)
+        return plan
+
+    def _request(self, layer: int, group: int, window: int) -> tuple:
+        c = self.cache
+        key = (layer, group, window)
+        ready = self._ready.get(key)
+        if ready is not None and ready[0].packed_pool == c._pool.data_ptr() + c._parts[layer][0]:
+            return ready
+        counts, items_at, merges_at, floats, uploaded = self._plan(group, window)
+        codec, (k, kn, v, vn, _, _) = c._codecs[layer], c._parts[layer]
+        kc, vc = codec.key_compressor, codec.val_compressor
+        tables = kc.table(c.device), vc.table(c.device)
+        for t, comp in zip(tables, (kc, vc)):
+            _native.check_table(t, c.head_dim, comp.bits)
+        es = c._plain.element_size()
+        r = _native.TqPagedRequest()
+        r.packed_pool, r.plain_pool = c._pool.data_ptr() + k, c._plain.data_ptr() + layer * c._plain.stride(1) * es
+        r.table_k, r.table_v = (t.data_ptr() for t in tables)
+        r.sequences, r.tables, r.items, r.merges = self._seq_at, self._table_at, items_at, merges_at
+        r.packed_page_stride, r.k_norms, r.v_idx, r.v_norms = c._page_bytes, kn - k, v - k, vn - k
+        r.plain_page_stride, r.plain_values = c._plain.stride(0) * es, c._plain.stride(2) * es
+        r.counts = counts
+        r.heads, r.group, r.sliding_window, r.page_tokens, r.head_dim, r.dtype, r.bits_k, r.bits_v = (c.kv_heads, group, window, c.page_tokens, c.head_dim,
+                                                                                                      _native.dtype_code(c.dtype), kc.bits, vc.bits)
+        ready = self._ready[key] = (r, floats, uploaded, tables)
+        return ready
+
+    @torch.compiler.disable
+    @torch.no_grad()
+    def attend(self, queries: torch.Tensor, layer_idx: int, scale: Optional[float] = None, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+               sliding_window: Optional[int] = None) -> torch.Tensor:
+        """softmax(z) V of the new tokens' queries, [new tokens, query heads, D] -> the same shape and type: a new token sees everything its sequence holds before it and itself.
+        Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap is given, less
+        slopes[query head] * distance if slopes (float [query heads]) are; sliding_window: only the last so many tokens, the new one among them, are seen.
+        Every layer has to be appended to before (the step's own tokens are read from its pages).  Not differentiable."""
+        self._live("attend")
+        c, layer = self.cache, self._layer(layer_idx)
+        if queries.dim() != 3 or queries.shape[0] != self.tokens or queries.shape[2] != c.head_dim or queries.shape[1] == 0 or queries.shape[1] % c.kv_heads or queries.dtype != c.dtype:
+            raise ValueError(f"attend: queries must be [{self.tokens}, k * {c.kv_heads}, {c.head_dim}] {c.dtype}, got {tuple(queries.shape)} {queries.dtype}")
+        if queries.device != c.device:
+            raise _native.TqError(f"attend: queries on {queries.device}, the cache on {c.device}")
+        heads, cap, window = queries.shape[1], 0.0, 0
+        if softcap is not None:
+            cap = float(softcap)
+            if not 0.0 < cap < float("inf"):
+                raise ValueError(f"attend: softcap must be a number above zero, got {softcap!r}")
+        if sliding_window is not None:
+            if isinstance(sliding_window, bool) or int(sliding_window) != sliding_window or sliding_window < 1:
+                raise ValueError(f"attend: sliding_window must be a whole number, 1 or more; got {sliding_window!r}")
+            window = min(int(sliding_window), 0x7fffffff)
+        if slopes is not None:
+            if tuple(slopes.shape) != (heads,) or not slopes.dtype.is_floating_point:
+                raise ValueError(f"attend: slopes must be one float per query head, [{heads}]; got {tuple(slopes.shape)} {slopes.dtype}")
+            if slopes.device != c.device:
+                raise _native.TqError(f"attend: slopes on {slopes.device}, the cache on {c.device}")
+            slopes = slopes.float().contiguous()
+        with _native._on(c.device):
+            out = torch.empty(queries.shape, dtype=c.dtype, device=c.device)
+            if not self.tokens:
+                return out
+            if queries.stride(2) != 1:
+                queries = queries.contiguous()
+            r, floats, uploaded, _ = self._request(layer, heads // c.kv_heads, window)
+            self._await(self._blob)
+            self._await(uploaded)
+            r.queries, r.out = queries.data_ptr(), out.data_ptr()
+            r.q_token, r.q_head = queries.stride(0), queries.stride(1)
+            r.scale, r.softcap = c.head_dim ** -0.5 if scale is None else float(scale), cap
+            r.slopes = None if slopes is None else slopes.data_ptr()
+            # the call's own: its launches hand their sums on through it, and those of another thread on the stream may come in between
+            scratch = torch.empty(floats, dtype=torch.float32, device=c.device) if floats else None
+            _native.check(_native.lib().tq_paged_attend(ctypes.byref(r), None if scratch is None else scratch.data_ptr(), floats, _native._stream_handle(c.device)), "tq_paged_attend")
+        return out
+
+    @torch.no_grad()
+    def commit(self) -> None:
+        """The step is over: whole pages that lie before the last `residual_window` tokens are packed, all layers at once, and their uncompressed pages are free again.  Where packed pages
+        run out, pages stay uncompressed until a later commit of their sequences finds some."""
+        if self._done:
+            return
+        c = self.cache
+        c._eager("commit")
+        if self.tokens and len(self._appended) != c.n_layers:
+            missing = sorted(set(range(c.n_layers)) - self._appended)
+            raise RuntimeError(f"commit: layers {missing[:8]} have not been appended to in this step")
+        made: List[Tuple[int, int]] = []
+        for s in self._states:
+            for _ in range((s.total - c.residual_window) // c.page_tokens - len(s.pages)):
+                plain = s.plain[0]
+                packed = c._packed_of.get(plain)
+                if packed is None:
+                    if not c._packed_pages.free:
+                        break
+                    packed = c._packed_pages.take()
+                    made.append((plain, packed))
+                    if c._plain_pages.held[plain] > 1:
+                        c._packed_of[plain] = packed
+                else:
+                    c._packed_pages.held[packed] += 1
+                del s.plain[0]
+                s.pages.append(packed)
+                c._drop_plain(plain)
+        if made:
+            self._pack(np.asarray(made, dtype=np.uint64))
+        self._done = True
+        if c._open is self:
+            c._open = None
+
+    def _pack(self, made: np.ndarray) -> None:
+        """Uncompressed pages into packed ones, of all layers: a job a page, layer and side; a launch a code width."""
+        c = self.cache
+        H, P, D, es, code = c.kv_heads, c.page_tokens, c.head_dim, c._plain.element_size(), _native.dtype_code(c.dtype)
+        source = c._plain.data_ptr() + made[:, 0] * np.uint64(c._plain.stride(0) * es)
+        target = c._pool.data_ptr() + made[:, 1] * np.uint64(c._page_bytes)
+        by_bits: Dict[int, list] = {}
+        for layer, (codec, parts) in enumerate(zip(c._codecs, c._parts)):
+            for side, comp in enumerate((codec.key_compressor, codec.val_compressor)):
+                jobs = np.zeros(len(made), dtype=_JOB)
+                jobs["states"] = source + np.uint64((layer * 2 + side) * H * P * D * es)
+                jobs["idx_bytes"], jobs["vec_norms"] = target + np.uint64(parts[2 * side]), target + np.uint64(parts[2 * side + 1])
+                jobs["table"] = comp.table(c.device).data_ptr()
+                jobs["rows"], jobs["tokens"], jobs["row_stride"], jobs["token_stride"] = 1, H * P, 0, D          # (a page's vectors follow one another)
+                jobs["bits"], jobs["dtype"] = comp.bits, code
+                by_bits.setdefault(comp.bits, []).append(jobs)
+        with _native._on(c.device):
+            for jobs in by_bits.values():
+                jobs = np.concatenate(jobs)
+                for lo in range(0, len(jobs), MAX_JOBS):
+                    part = np.ascontiguousarray(jobs[lo:lo + MAX_JOBS])
+                    host = torch.empty(part.nbytes, dtype=torch.uint8, pin_memory=True)
+                    host.numpy()[:] = part.view(np.uint8)
+                    dev = host.to(c.device, non_blocking=True)
+                    _native.check(_native.lib().tq_compress_batched(part.ctypes.data, dev.data_ptr(), len(part), D, 0, _native._stream_handle(c.device)), "tq_compress_batched")
