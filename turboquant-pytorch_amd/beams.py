@@ -12,14 +12,26 @@ from . import _native
 MAX_BEST, MAX_BEAMS = 64, 1024
 
 
-@torch.compiler.disable
-@torch.no_grad()
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Of the continuations of every sequence's beams the `best` (default: as many as there are beams) with the largest sums scores + log_softmax(logits).
     logits [batch, beams, vocabulary] (float32, float16 or bfloat16), scores [batch, beams] -> sums (float32), tokens and beams they continue (int64),
     each [batch, best], in falling order, equal ones by beam and then token; sums are formed and compared in 64 bits.
     A beam whose sums are no numbers (a NaN or +infinity among its logits, nothing but -infinity, a score that is not finite: a beam that has ended or not begun) counts with sums of
     -infinity.  At most 64 are chosen, of at most 1024 beams.  Not differentiable."""
+    n = logits.shape[1] if best is None and logits.dim() > 1 else best
+    if logits.is_cuda and not torch.compiler.is_compiling():
+        chosen = _native.fast().beam_select(logits, scores, n)
+        if chosen is not None:
+            if type(chosen) is int:
+                _native.check(chosen, "tq_beam_select")
+            return chosen
+    return _select(logits, scores, n)
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def _select(logits: torch.Tensor, scores: torch.Tensor, best: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """beam_select for logits and scores of any layout, with every check."""
     _native._require_gpu(logits, "logits")
     if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
         raise ValueError(f"beam_select takes logits [batch, beams, vocabulary] and scores [batch, beams]; got {tuple(logits.shape)} and {tuple(scores.shape)}")
@@ -29,7 +41,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: Optional[int] 
     if not scores.dtype.is_floating_point:
         raise ValueError(f"scores must be floats, got {scores.dtype}")
     batch, beams, vocab = logits.shape
-    n = beams if best is None else best
+    n = best
     if isinstance(n, bool) or int(n) != n or not 0 <= n <= MAX_BEST or (batch and n > beams * vocab):
         raise ValueError(f"best must be a whole number from 0 to {min(MAX_BEST, beams * vocab)}, got {n!r}")
     n = int(n)

@@ -16,11 +16,13 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <vector>
+
 #include "../../include/tqamd.h"
 
 namespace {
 
-constexpr int INTERFACE = 6;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 7;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -40,6 +42,10 @@ struct Entries {
     decltype(&tq_attend_many) attend_many;
     decltype(&tq_evict) evict;
     decltype(&tq_evict_scratch) evict_scratch;
+    decltype(&tq_beam_scratch) beam_scratch;
+    decltype(&tq_beam_select) beam_select;
+    decltype(&tq_reorder) reorder;
+    decltype(&tq_paged_attend) paged_attend;
 } lib{};
 
 struct Raised {};        // a Python exception is set
@@ -561,6 +567,99 @@ PyObject *evict(PyObject *const *a) {
     return wrapped({ko, kno, vo, vno, wo, kept});
 }
 
+// beam_select(logits, scores, best) -> (sums, tokens, parents)
+PyObject *beam_select(PyObject *const *a) {
+    TENSOR(logits, a[0]); TENSOR(scores, a[1]);
+    NEED(logits.dim() == 3 && PyLong_CheckExact(a[2]) && scores.scalar_type() == at::kFloat && scores.device() == logits.device());
+    const int dt = dtype_code(logits);
+    const long long best = integer(a[2]), B = logits.size(0), K = logits.size(1), V = logits.size(2);
+    NEED(dt >= 0 && B > 0 && K > 0 && V > 0 && best > 0 && logits.stride(2) == 1 && shape_is(scores, {B, K}) && scores.is_contiguous());
+    const long long bytes = lib.beam_scratch(B, K, V, best);
+    NEED(bytes >= 0);
+    const Stream s(logits);
+    NEED(s.ok);
+    at::Tensor values = empty({B, best}, at::kFloat, logits), tokens = empty({B, best}, at::kLong, logits), parents = empty({B, best}, at::kLong, logits);
+    const at::Tensor scratch = empty({bytes}, at::kByte, logits);
+    const int rc = launch(lib.beam_select, (const void *)address(logits), dt, B, K, V, (long long)logits.stride(0), (long long)logits.stride(1), (const float *)address(scores), K, best,
+                          (float *)address(values), (long long *)address(tokens), (long long *)address(parents), (void *)address(scratch), bytes, s.raw());
+    if (rc > 0) return PyLong_FromLong(rc);
+    NEED(rc == 0);
+    return wrapped({values, tokens, parents});
+}
+
+// reorder(parents, batch, heads, layers) -> status; layers = ((address of the layer's tq_decode_layer, first window slot, window tokens, packed tokens, address of kept sums or 0, their
+// stride), ...): _LayerStore.segments of all of them in one call
+PyObject *reorder(PyObject *const *a) {
+    TENSOR(parents, a[0]);
+    const long long B = integer(a[1]), H = integer(a[2]);
+    NEED(parents.scalar_type() == at::kLong && parents.dim() == 1 && parents.size(0) == B && parents.is_contiguous() && PyTuple_CheckExact(a[3]) && B <= 1024);
+    const Stream s(parents);
+    NEED(s.ok);
+    std::vector<tq_move_segment> runs;
+    const Py_ssize_t n = PyTuple_GET_SIZE(a[3]);
+    runs.reserve((size_t)n * 7);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject *t = PyTuple_GET_ITEM(a[3], i);
+        NEED(PyTuple_CheckExact(t) && PyTuple_GET_SIZE(t) == 6);
+        long long v[6];
+        for (int j = 0; j < 6; ++j) v[j] = integer(PyTuple_GET_ITEM(t, j));
+        const tq_decode_layer &l = *reinterpret_cast<const tq_decode_layer *>(v[0]);
+        NEED(l.rows == B * H);
+        const long long tokens = v[3], cap = l.packed_row_stride, elem = l.dtype == TQ_F32 ? 4 : 2, vec = l.head_dim * elem;
+        // (packed runs to a multiple of 16 bytes, which their capacity has room for)
+        auto packed = [&](void *p, long long bytes) {
+            const long long up = (tokens * bytes + 15) / 16 * 16, most = cap * bytes;
+            runs.push_back({p, H * cap * bytes, cap * bytes, up < most ? up : most});
+        };
+        if (tokens) {
+            packed(l.k_idx, packed_width(l.head_dim, l.bits_k));
+            packed(l.k_norms, 2);
+            packed(l.v_idx, packed_width(l.head_dim, l.bits_v));
+            packed(l.v_norms, 2);
+        }
+        if (v[2])
+            for (void *w : {l.k_win, l.v_win}) runs.push_back({static_cast<uint8_t *>(w) + v[1] * vec, H * l.win_stride * elem, l.win_stride * elem, v[2] * vec});
+        if (v[4] && tokens + v[2]) runs.push_back({reinterpret_cast<void *>(v[4]), H * v[5] * 4, v[5] * 4, 4 * (tokens + v[2])});
+    }
+    return PyLong_FromLong(launch(lib.reorder, (const tq_move_segment *)runs.data(), (int)runs.size(), B, H, (const long long *)address(parents), s.raw()));
+}
+
+// paged_attend(address of the step's tq_paged_request, queries, tokens, scale, softcap or None, slopes or None, scratch values, like, stream) -> output; like: a tensor on the cache's
+// device; stream: the one the step's tables were uploaded on
+PyObject *paged_attend(PyObject *const *a) {
+    TENSOR(q, a[1]); TENSOR(like, a[7]);
+    tq_paged_request r = *reinterpret_cast<const tq_paged_request *>(integer(a[0]));
+    const long long tokens = integer(a[2]), floats = integer(a[6]);
+    NEED(q.dim() == 3 && dtype_code(q) == r.dtype && q.device() == like.device() && q.size(0) == tokens && q.size(1) == (long long)r.heads * r.group && q.size(2) == r.head_dim &&
+         q.stride(2) == 1 && tokens > 0);
+    r.scale = (float)PyFloat_AsDouble(a[3]);
+    r.softcap = 0.f;
+    if (a[4] != Py_None) {
+        const double cap = PyFloat_AsDouble(a[4]);
+        if (PyErr_Occurred()) throw Raised{};
+        NEED(cap > 0.0 && cap < 1e38 && (float)cap > 0.f);
+        r.softcap = (float)cap;
+    }
+    if (PyErr_Occurred()) throw Raised{};
+    r.slopes = nullptr;
+    if (a[5] != Py_None) {
+        TENSOR(slopes, a[5]);
+        NEED(slopes.scalar_type() == at::kFloat && shape_is(slopes, {q.size(1)}) && slopes.is_contiguous() && slopes.device() == q.device());
+        r.slopes = (const float *)address(slopes);
+    }
+    const Stream s(q);
+    NEED(s.ok && (long long)s.handle == integer(a[8]) && !s.capturing());
+    at::Tensor out = empty({tokens, q.size(1), q.size(2)}, q.scalar_type(), q), scratch;
+    if (floats) scratch = empty({floats}, at::kFloat, q);
+    r.queries = address(q);
+    r.out = address(out);
+    r.q_token = q.stride(0); r.q_head = q.stride(1);
+    const int rc = launch(lib.paged_attend, (const tq_paged_request *)&r, floats ? (float *)address(scratch) : (float *)nullptr, floats, s.raw());
+    if (rc > 0) return PyLong_FromLong(rc);
+    NEED(rc == 0);
+    return THPVariable_Wrap(out);
+}
+
 // No exception leaves a function, and none records gradients.  Errors of torch's (no memory, a device error) become the Python exceptions
 // that its own functions raise.
 template <PyObject *(*F)(PyObject *const *), int N>
@@ -607,6 +706,7 @@ PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
     TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 22), TQ_ENTRY(evict, 10),
+    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

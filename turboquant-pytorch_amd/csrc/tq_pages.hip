@@ -41,7 +41,7 @@ __global__ __launch_bounds__(THREADS) void tq_reorder_kernel(ReorderArgs a) {
     const bool some = at < (unsigned long long)s.pieces * a.heads;
     const uint32_t head = some ? (uint32_t)(at / s.pieces) : 0u, piece = some ? (uint32_t)(at - (unsigned long long)head * s.pieces) : 0u;
     uint8_t *p = s.base + (long long)head * s.head_stride + (long long)piece * (long long)sizeof(T);
-    const uint32_t first = threadIdx.x / COLUMNS;
+    const uint32_t first = COLUMNS == 64 ? tq_uniform32(threadIdx.x / COLUMNS) : threadIdx.x / COLUMNS;       // (a wave's: parents and addresses on the scalar unit)
     T v[K];
     uint32_t moved = 0u;
 #pragma unroll
@@ -79,25 +79,26 @@ struct CopyArgs {
     uint32_t used[PAIRS];                    // bytes of every run that are copied
 };
 
-// Block = a share of one page.  Four pieces a thread are under way at once.
+// Block = a share of one page.  Eight pieces a thread are under way at once; what is copied is not read again soon, so neither side asks the caches to keep it.
 __global__ __launch_bounds__(MOVE_THREADS) void tq_copy_pages_kernel(CopyArgs a, uint32_t blocks) {
+    constexpr int K = 8;
     const uint32_t pair = blockIdx.x / blocks, part = blockIdx.x - pair * blocks, pieces = a.used[pair] / 16u;
     const uint8_t *src = a.from + (long long)a.src[pair] * a.from_stride;
     uint8_t *dst = a.to + (long long)a.dst[pair] * a.to_stride;
     const unsigned long long all = (unsigned long long)pieces * a.rows;
-    for (unsigned long long i0 = (unsigned long long)part * (4u * MOVE_THREADS); i0 < all; i0 += (unsigned long long)blocks * (4u * MOVE_THREADS)) {
-        tq_u4 v[4];
-        unsigned long long off[4];
+    for (unsigned long long i0 = (unsigned long long)part * (K * MOVE_THREADS); i0 < all; i0 += (unsigned long long)blocks * (K * MOVE_THREADS)) {
+        tq_u4 v[K];
+        unsigned long long off[K];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < K; ++k) {
             const unsigned long long i = i0 + (uint32_t)k * MOVE_THREADS + threadIdx.x;
-            const unsigned long long row = i / pieces;
+            const unsigned long long row = a.rows == 1u ? 0ull : (unsigned long long)((uint32_t)i / pieces);      // (a page is less than 2^32 pieces)
             off[k] = row * a.row_bytes + (i - row * pieces) * 16u;
-            if (i < all) v[k] = get<tq_u4>(src + off[k]);
+            if (i < all) v[k] = tq_gload16_stream(src + off[k]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i0 + (uint32_t)k * MOVE_THREADS + threadIdx.x < all) put<tq_u4>(dst + off[k], v[k]);
+        for (int k = 0; k < K; ++k)
+            if (i0 + (uint32_t)k * MOVE_THREADS + threadIdx.x < all) tq_gstore16_stream(dst + off[k], v[k]);
     }
 }
 
@@ -192,6 +193,7 @@ extern "C" int tq_copy_pages(const void *from, long long from_stride, void *to, 
         if (pairs[i].bytes & 15) return TQ_ERR_ALIGN;
         if (pairs[i].bytes > largest) largest = pairs[i].bytes;
     }
+    if (row_bytes / 16 > 0xffffffffLL / rows) return TQ_ERR_SIZE;
     if (rows > 1 && (from_stride < rows * row_bytes || to_stride < rows * row_bytes)) return TQ_ERR_SIZE;
     int cus = 0;
     if (tq_device_cus(cus)) cus = 256;
@@ -207,8 +209,8 @@ extern "C" int tq_copy_pages(const void *from, long long from_stride, void *to, 
             a.dst[i] = pairs[i0 + i].to;
             a.used[i] = (uint32_t)pairs[i0 + i].bytes;
         }
-        // a block has 16 KiB under way; no more blocks a page than that, and sixteen a compute unit in all
-        long long blocks = (largest * rows + 64 * MOVE_THREADS - 1) / (64 * MOVE_THREADS), share = (16LL * cus + n - 1) / n;
+        // a block has 32 KiB under way; no more blocks a page than that, and sixteen a compute unit in all
+        long long blocks = (largest * rows + 128 * MOVE_THREADS - 1) / (128 * MOVE_THREADS), share = (16LL * cus + n - 1) / n;
         if (blocks > share) blocks = share;
         if (blocks < 1) blocks = 1;
         hipLaunchKernelGGL(tq_copy_pages_kernel, dim3((unsigned)(n * blocks)), dim3(MOVE_THREADS), 0, s, a, (uint32_t)blocks);

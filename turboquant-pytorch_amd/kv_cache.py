@@ -544,14 +544,28 @@ class V3Cache:
         self.attention_weights(layer_idx)          # (raises where there are none)
         return self._stores[layer_idx].evict(int(keep))
 
-    @torch.compiler.disable
-    @torch.no_grad()
     def reorder(self, parents: torch.Tensor) -> None:
         """Sequence b of the batch goes on from what sequence parents[b] was, in every layer: packed tokens, window and kept sums, in place.  parents [B] (whole numbers, on the
         cache's device: the host does not wait for them); one outside the batch leaves its sequence as it is.  At most 1024 sequences."""
         stores = list(self._stores.values())
         if not stores:
             return
+        one = stores[0]
+        # (something is packed: the codec's tables, which the records name, are on the card then)
+        alike = all(st.n_compressed and st.H == one.H and st.B == one.B and st.device == one.device for st in stores)
+        if alike and isinstance(parents, torch.Tensor) and parents.device == one.device and not torch.compiler.is_compiling():
+            layers = tuple([(ctypes.addressof(st.record()), st.w0, st.n_recent, st.n_compressed, *((0, 0) if st.weights is None else (st.weights.data_ptr(), st.weights.shape[2])))
+                            for st in stores])
+            rc = _native.fast().reorder(parents, one.B, one.H, layers)
+            if rc is not None:
+                _native.check(rc, "tq_reorder")
+                return
+        self._reorder(stores, parents)
+
+    @torch.compiler.disable
+    @torch.no_grad()
+    def _reorder(self, stores, parents: torch.Tensor) -> None:
+        """`reorder` for parents and layers of any kind, with every check."""
         if not isinstance(parents, torch.Tensor) or parents.dim() != 1 or parents.dtype.is_floating_point or parents.dtype.is_complex or parents.dtype == torch.bool:
             raise ValueError("reorder: parents must be a tensor of whole numbers, one for each sequence")
         if any(parents.shape[0] != st.B for st in stores):

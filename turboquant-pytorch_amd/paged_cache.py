@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+from itertools import chain
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -31,7 +32,6 @@ from .compressors_v3 import TurboQuantV3
 
 _JOB = np.dtype([("states", np.uint64), ("idx_bytes", np.uint64), ("vec_norms", np.uint64), ("table", np.uint64), ("rows", np.int64), ("tokens", np.int64), ("row_stride", np.int64),
                  ("token_stride", np.int64), ("bits", np.int32), ("dtype", np.int32), ("packed_row_stride", np.int64)])
-_PAIR = np.dtype([("from", np.int32), ("to", np.int32), ("bytes", np.int32)])
 assert _JOB.itemsize == ctypes.sizeof(_native.TqJob)
 MAX_JOBS = 4096                     # TQ_MAX_JOBS of include/tqamd.h
 
@@ -195,7 +195,7 @@ class PagedV3Cache:
             self._packed_of.pop(page, None)
 
     def _drop_packed(self, page: int) -> None:
-        if self._packed_pages.drop(page):
+        if self._packed_pages.drop(page) and self._packed_of:
             for plain, packed in list(self._packed_of.items()):
                 if packed == page:
                     del self._packed_of[plain]
@@ -211,44 +211,43 @@ class PagedV3Cache:
         states = [self._sequence(s) for s in seqs]
         if len(set(seqs)) != len(states):
             raise ValueError("free: a sequence ends once")
-        for seq, s in zip(seqs, states):
+        for seq in seqs:
+            s = self._seqs.pop(seq)
             for p in s.pages:
                 self._drop_packed(p)
             for p in s.plain:
                 self._drop_plain(p)
-            del self._seqs[seq]
 
-    def _share(self, s: _Sequence, copies: List[Tuple[int, int, int]], own_last: bool) -> _Sequence:
-        """A sequence that continues as `s`: whole pages are held together, the one that is being filled is copied (own_last: taken over)."""
+    def _share(self, s: _Sequence) -> _Sequence:
+        """A sequence that continues as `s`, with the same pages."""
         new = _Sequence()
-        new.pages, new.plain, new.total = list(s.pages), list(s.plain), s.total
-        for p in new.pages:
-            self._packed_pages.held[p] += 1
-        filled = s.total % self.page_tokens
-        for p in new.plain:
-            self._plain_pages.held[p] += 1
-        if filled and not own_last:
-            copies.append((new.plain[-1], -1, filled))
+        new.pages, new.plain, new.total = s.pages[:], s.plain[:], s.total
+        held = self._packed_pages.held
+        for p in s.pages:
+            held[p] += 1
+        held = self._plain_pages.held
+        for p in s.plain:
+            held[p] += 1
         return new
 
-    def _copy_last(self, new: Sequence[_Sequence], copies: Sequence[Tuple[int, int, int]]) -> None:
-        """Pages of their own for the sequences of `new`, one for each of `copies`, whose last page is another's."""
-        if not copies:
-            return
-        pairs = np.empty(len(copies), dtype=_PAIR)
-        for i, (s, (source, _, filled)) in enumerate(zip(new, copies)):
-            target = self._plain_pages.take()
-            self._plain_pages.drop(source)           # (its owner still holds it)
-            s.plain[-1] = target
-            pairs[i] = (source, target, filled)
-        vector = self.head_dim * self._plain.element_size()
-        pairs["bytes"] *= vector
-        self._move(self._plain, self._plain, int(np.prod(self._plain_shape[:3])), self.page_tokens * vector, pairs)
+    def _copy_last(self, sharing: Sequence[_Sequence]) -> None:
+        """The page that is being filled becomes a sequence's own, where it has been shared so far."""
+        pool, vector = self._plain_pages, self.head_dim * self._plain.element_size()
+        pairs: List[int] = []
+        for s in sharing:
+            filled = s.total % self.page_tokens
+            if filled:
+                target = pool.take()
+                pool.drop(s.plain[-1])           # (its owner still holds it)
+                pairs += (s.plain[-1], target, filled * vector)
+                s.plain[-1] = target
+        if pairs:
+            self._move(self._plain, self._plain, self.n_layers * 2 * self.kv_heads, self.page_tokens * vector, np.array(pairs, dtype=np.int32))
 
     def _move(self, source: torch.Tensor, target: torch.Tensor, rows: int, row_bytes: int, pairs: np.ndarray) -> None:
         stride = lambda t: t.stride(0) * t.element_size()  # noqa: E731
         with _native._on(self.device):
-            _native.check(_native.lib().tq_copy_pages(source.data_ptr(), stride(source), target.data_ptr(), stride(target), rows, row_bytes, pairs.ctypes.data, len(pairs),
+            _native.check(_native.lib().tq_copy_pages(source.data_ptr(), stride(source), target.data_ptr(), stride(target), rows, row_bytes, pairs.ctypes.data, pairs.size // 3,
                                                       _native._stream_handle(self.device)), "tq_copy_pages")
 
     def fork(self, seqs: Sequence[int]) -> List[int]:
@@ -257,12 +256,11 @@ class PagedV3Cache:
         self._settle()
         states = [self._sequence(s) for s in seqs]
         self._room("fork", 0, sum(1 for s in states if s.total % self.page_tokens))
-        copies: List[Tuple[int, int, int]] = []
-        fresh = [self._share(s, copies, False) for s in states]
-        self._copy_last([f for f in fresh if f.total % self.page_tokens], copies)
-        new = self.add(len(states))
-        for seq, f in zip(new, fresh):
-            self._seqs[seq] = f
+        fresh = [self._share(s) for s in states]
+        self._copy_last(fresh)
+        new = list(range(self._next, self._next + len(fresh)))
+        self._next += len(fresh)
+        self._seqs.update(zip(new, fresh))
         return new
 
     def reorder(self, seqs: Sequence[int], parents) -> None:
@@ -287,16 +285,14 @@ class PagedV3Cache:
         # (pages of the ones that end become free first)
         ends = sum(1 for p, s in enumerate(states) if p not in heir for page in s.plain if self._plain_pages.held[page] == 1)
         self._room("reorder", 0, max(0, twice - ends))
-        copies: List[Tuple[int, int, int]] = []
-        fresh = [self._share(states[p], copies, heir[p] == i) for i, p in enumerate(parents)]
+        fresh = [self._share(states[p]) for p in parents]
         for s in states:
             for page in s.pages:
                 self._drop_packed(page)
             for page in s.plain:
                 self._drop_plain(page)
-        self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i and f.total % self.page_tokens], copies)
-        for seq, f in zip(seqs, fresh):
-            self._seqs[seq] = f
+        self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i])
+        self._seqs.update(zip(seqs, fresh))
 
     def beam_step(self, seqs: Sequence[int], logits: torch.Tensor, scores: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """One step of beam search: of every group of beams (logits [groups, beams, vocabulary], scores [groups, beams]; seqs group after group) the `beams` best continuations,
@@ -312,13 +308,9 @@ class PagedV3Cache:
         """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered, sequence after sequence."""
         self._eager("resize")
         self._settle()
-        orders = []
-        for name, get in (("pages", lambda s: s.pages), ("plain_pages", lambda s: s.plain)):
-            order: Dict[int, int] = {}
-            for seq in sorted(self._seqs):
-                for p in get(self._seqs[seq]):
-                    order.setdefault(p, len(order))
-            orders.append(order)
+        states = [self._seqs[seq] for seq in sorted(self._seqs)]
+        # page -> its number in the new pool, as the sequences have them
+        orders = [{p: i for i, p in enumerate(dict.fromkeys(chain.from_iterable(lists)))} for lists in ([s.pages for s in states], [s.plain for s in states])]
         sizes = []
         for name, asked, order in (("pages", pages, orders[0]), ("plain_pages", plain_pages, orders[1])):
             n = max(1, len(order)) if asked is None else asked
@@ -331,21 +323,22 @@ class PagedV3Cache:
         for source, target, order, rows, row_bytes in ((self._pool, pool, orders[0], 1, self._page_bytes),
                                                        (self._plain, plain, orders[1], int(np.prod(self._plain_shape[:3])), self.page_tokens * vector)):
             if order:
-                pairs = np.empty(len(order), dtype=_PAIR)
-                pairs["from"], pairs["to"], pairs["bytes"] = list(order), list(order.values()), row_bytes
+                pairs = np.full((len(order), 3), row_bytes, dtype=np.int32)
+                pairs[:, 0], pairs[:, 1] = list(order), np.arange(len(order))
                 self._move(source, target, rows, row_bytes, pairs)
         self._pool, self._plain = pool, plain
-        for which, (order, size) in enumerate(zip(orders, sizes)):
-            old, new = (self._packed_pages, self._plain_pages)[which], _Pages(size)
-            for p, q in order.items():
-                new.held[q] = old.held[p]
+        pools = []
+        for old, order, size in zip((self._packed_pages, self._plain_pages), orders, sizes):
+            new = _Pages(0)
+            new.held = [old.held[p] for p in order] + [0] * (size - len(order))
             new.free = list(range(len(order), size))
-            if which == 0:
-                self._packed_pages = new
-            else:
-                self._plain_pages = new
-        for s in self._seqs.values():
-            s.pages, s.plain = [orders[0][p] for p in s.pages], [orders[1][p] for p in s.plain]
+            pools.append(new)
+        self._packed_pages, self._plain_pages = pools
+        for s in states:
+            if s.pages:
+                s.pages = [orders[0][p] for p in s.pages]
+            if s.plain:
+                s.plain = [orders[1][p] for p in s.plain]
         self._packed_of = {orders[1][p]: orders[0][q] for p, q in self._packed_of.items()}
 
     # ---- steps ----------------------------------------------------------------------------------------------------------------
@@ -394,6 +387,7 @@ class PagedStep:
         self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
         self._plans: Dict[Tuple[int, int], tuple] = {}
         self._ready: Dict[tuple, tuple] = {}
+        self._quick: Dict[tuple, tuple] = {}         # (layer, window) as they are asked for -> what the one-step call takes
         self._appended: set = set()
         self._done = False
 
@@ -481,7 +475,7 @@ class PagedStep:
         c = self.cache
         key = (layer, group, window)
         ready = self._ready.get(key)
-        if ready is not None and ready[0].packed_pool == c._pool.data_ptr() + c._parts[layer][0]:
+        if ready is not None:
             return ready
         counts, items_at, merges_at, floats, uploaded = self._plan(group, window)
         codec, (k, kn, v, vn, _, _) = c._codecs[layer], c._parts[layer]
@@ -502,14 +496,26 @@ class PagedStep:
         ready = self._ready[key] = (r, floats, uploaded, tables)
         return ready
 
-    @torch.compiler.disable
-    @torch.no_grad()
     def attend(self, queries: torch.Tensor, layer_idx: int, scale: Optional[float] = None, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
                sliding_window: Optional[int] = None) -> torch.Tensor:
         """softmax(z) V of the new tokens' queries, [new tokens, query heads, D] -> the same shape and type: a new token sees everything its sequence holds before it and itself.
         Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap is given, less
         slopes[query head] * distance if slopes (float [query heads]) are; sliding_window: only the last so many tokens, the new one among them, are seen.
         Every layer has to be appended to before (the step's own tokens are read from its pages).  Not differentiable."""
+        ready = self._quick.get((layer_idx, sliding_window))
+        if ready is not None and not self._done and not torch.compiler.is_compiling():
+            # as the call before with this layer and window, if the queries are laid out for it
+            out = _native.fast().paged_attend(ready[0], queries, self.tokens, self.cache.head_dim ** -0.5 if scale is None else scale, softcap, slopes, ready[1], ready[2], ready[3])
+            if out is not None:
+                if type(out) is int:
+                    _native.check(out, "tq_paged_attend")
+                return out
+        return self._attend(queries, layer_idx, scale, softcap, slopes, sliding_window)
+
+    @torch.compiler.disable
+    @torch.no_grad()
+    def _attend(self, queries, layer_idx, scale, softcap, slopes, sliding_window) -> torch.Tensor:
+        """`attend` with every check."""
         self._live("attend")
         c, layer = self.cache, self._layer(layer_idx)
         if queries.dim() != 3 or queries.shape[0] != self.tokens or queries.shape[2] != c.head_dim or queries.shape[1] == 0 or queries.shape[1] % c.kv_heads or queries.dtype != c.dtype:
@@ -537,9 +543,13 @@ class PagedStep:
                 return out
             if queries.stride(2) != 1:
                 queries = queries.contiguous()
-            r, floats, uploaded, _ = self._request(layer, heads // c.kv_heads, window)
+            ready = self._request(layer, heads // c.kv_heads, window)
+            floats, uploaded = ready[1:3]
+            if uploaded[2] == self._blob[2]:
+                self._quick[layer, sliding_window] = (ctypes.addressof(ready[0]), floats, self._blob[0], uploaded[2])
             self._await(self._blob)
             self._await(uploaded)
+            r = _native.TqPagedRequest.from_buffer_copy(ready[0])
             r.queries, r.out = queries.data_ptr(), out.data_ptr()
             r.q_token, r.q_head = queries.stride(0), queries.stride(1)
             r.scale, r.softcap = c.head_dim ** -0.5 if scale is None else float(scale), cap
