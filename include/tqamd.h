@@ -573,14 +573,14 @@ int tq_put_tokens(const void *keys, const void *values, long long k_token_stride
  *   queries     new token i, query head j at i * q_token + j * q_head elements; query head j reads kv head j / group.  out: dense [new tokens, heads * group, head_dim]
  *   softcap     0: none; otherwise logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
  * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, 4 a merge; counts also where they do not fit
- * (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim and dtype.
+ * (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim, dtype and page_tokens.
  * tq_paged_scratch: float32 values of scratch (16-byte aligned, not shared by calls that can overlap in time).
  * tq_paged_supported: head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose packed vectors are words; 2 to 8 bits.
  * Infinities and NaN reach the results of the queries that see them and no others.  Numbers of pages are not checked.  Pages are read whole runs of 32 tokens at a time.
  */
 typedef struct tq_paged_counts {
-    long long items, merges, records;
-    int tiles, columns;
+    long long items, few, merges, records;     /* few: the first items, those of sequences with few query vectors */
+    int tiles, columns, vectors;
 } tq_paged_counts;
 typedef struct tq_paged_request {
     const void *queries;
@@ -595,7 +595,7 @@ typedef struct tq_paged_request {
     int heads, group, sliding_window, page_tokens, head_dim, dtype, bits_k, bits_v;
 } tq_paged_request;
 int tq_paged_supported(int head_dim, int dtype, int bits_k, int bits_v);
-int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int32_t *items, long long max_items, int32_t *merges,
+int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int page_tokens, int32_t *items, long long max_items, int32_t *merges,
                   long long max_merges, tq_paged_counts *counts);
 long long tq_paged_scratch(const tq_paged_counts *counts, int heads, int head_dim);
 int tq_paged_attend(const tq_paged_request *request, float *scratch, long long scratch_floats, void *stream);

@@ -7,14 +7,14 @@ import pytest
 import torch
 
 
-def plan(pkg, sequences, heads=2, group=4, window=0, D=128, dtype=2, room=100000):
+def plan(pkg, sequences, heads=2, group=4, window=0, D=128, dtype=2, room=100000, page=64):
     native = pkg._native
     records = np.zeros((len(sequences), native.PAGED_SEQ), np.int32)
     for r, (fresh, total, packed) in zip(records, sequences):
         r[1:4] = fresh, total, packed
     counts = native.TqPagedCounts()
     items, merges = np.empty((room, native.PAGED_ITEM), np.int32), np.empty((room, native.PAGED_MERGE), np.int32)
-    rc = native.lib().tq_paged_plan(records.ctypes.data, len(records), heads, group, window, D, dtype, items.ctypes.data, room, merges.ctypes.data, room, ctypes.byref(counts))
+    rc = native.lib().tq_paged_plan(records.ctypes.data, len(records), heads, group, window, D, dtype, page, items.ctypes.data, room, merges.ctypes.data, room, ctypes.byref(counts))
     return rc, counts, items[:counts.items], merges[:counts.merges]
 
 
@@ -27,8 +27,12 @@ SEQUENCES = [
 @pytest.mark.parametrize("window", [0, 1, 33, 4096])
 @pytest.mark.parametrize("sequences", SEQUENCES)
 def test_a_plan_covers_what_is_seen_once(pkg, sequences, window):
-    for heads, group, D, dtype in ((8, 4, 128, 2), (1, 1, 64, 1), (2, 7, 256, 2), (8, 1, 80, 0)):
-        rc, counts, items, merges = plan(pkg, sequences, heads, group, window, D, dtype)
+    for heads, group, D, dtype, page in ((8, 4, 128, 2, 64), (8, 4, 128, 2, 32), (1, 1, 64, 1, 128), (2, 7, 256, 2, 64), (8, 1, 80, 0, 64)):
+        rc, counts, items, merges = plan(pkg, sequences, heads, group, window, D, dtype, page=page)
+        few = page >= 64 and dtype and D in (64, 96, 128, 256)
+        small = [bool(few and f * group <= 16) for f, _, _ in sequences]
+        assert all(small[b] == (i < counts.few) for i, b in enumerate(items[:, 0].tolist()))
+        assert counts.vectors == max([f * group for (f, _, _), s in zip(sequences, small) if s and f] or [0])
         assert rc == 0 and counts.tiles in ((1, 2) if dtype == 2 and D in (64, 128) else (1,)) and 1 <= counts.columns <= 32
         by_group = {}
         for it in items.tolist():
@@ -36,18 +40,19 @@ def test_a_plan_covers_what_is_seen_once(pkg, sequences, window):
         records, joined = [], {(m[0], m[1]): (m[2], m[3]) for m in merges.tolist()}
         for b, (fresh, total, packed) in enumerate(sequences):
             tiles = -(-fresh * group // 32)
-            for t0 in range(0, tiles, counts.tiles):
+            step, unit = (1, 64) if small[b] else (counts.tiles, 32)
+            for t0 in range(0, tiles, step):
                 parts = by_group.pop((b, t0))
-                first, last = total - fresh + t0 * 32 // group, total - fresh + min(fresh - 1, ((t0 + counts.tiles) * 32 - 1) // group)
+                first, last = total - fresh + t0 * 32 // group, total - fresh + min(fresh - 1, ((t0 + step) * 32 - 1) // group)
                 lo = max(0, first - window + 1) if window else 0
                 covered = set()
                 for a, z, u, w, _ in parts:
-                    assert a % 32 == 0 and u % 32 == 0 and 0 <= a <= z <= packed and 0 <= u <= w <= total - packed and (z > a or w > u)
-                    assert (z % 32 == 0 or z == packed)
+                    assert a % unit == 0 and u % 32 == 0 and 0 <= a <= z <= packed and 0 <= u <= w <= total - packed and (z > a or w > u)
+                    assert (z % unit == 0 or z == packed)
                     for x in itertools.chain(range(a // 32, -(-z // 32)), range(1 << 26 | u // 32, 1 << 26 | -(-w // 32))):
                         assert x not in covered
                         covered.add(x)
-                want = set(range(min(lo, packed) // 32, -(-packed // 32))) if lo < packed else set()
+                want = set(range(lo // unit * unit // 32, -(-packed // 32))) if lo < packed else set()
                 want |= set(range(1 << 26 | max(0, lo - packed) // 32, 1 << 26 | -(-(last + 1 - packed) // 32)))
                 assert covered == want
                 if len(parts) > 1:
@@ -68,8 +73,8 @@ def test_plans_are_refused_or_ask_for_room(pkg):
         assert plan(pkg, [(1, 5, 0)], **kw)[0] == -5
     rc, counts, _, _ = plan(pkg, SEQUENCES[7], room=3)
     assert rc == -10 and counts.items > 3
-    assert pkg._native.lib().tq_paged_plan(None, 1, 1, 1, 0, 128, 2, None, 0, None, 0, ctypes.byref(counts)) == -1
-    assert pkg._native.lib().tq_paged_plan(None, 0, 1, 1, 0, 128, 2, None, 0, None, 0, None) == -1
+    assert pkg._native.lib().tq_paged_plan(None, 1, 1, 1, 0, 128, 2, 64, None, 0, None, 0, ctypes.byref(counts)) == -1
+    assert pkg._native.lib().tq_paged_plan(None, 0, 1, 1, 0, 128, 2, 64, None, 0, None, 0, None) == -1
 
 
 def test_which_combinations_there_are(pkg):
@@ -122,6 +127,10 @@ def test_attention_checks_its_request(pkg):
     bad.counts.tiles = 2
     bad.dtype = 1
     assert L.tq_paged_attend(ctypes.byref(bad), 4096, 1 << 40, None) == -5
+    for field, value in (("few", -1), ("few", counts.items + 1), ("vectors", 0), ("vectors", 17)):
+        bad = copy()
+        setattr(bad.counts, field, value)
+        assert L.tq_paged_attend(ctypes.byref(bad), 4096, 1 << 40, None) == -5, field
     bad = copy()
     bad.counts.items = 0
     assert L.tq_paged_attend(ctypes.byref(bad), None, 0, None) == 0

@@ -28,8 +28,9 @@ FAST_INTERFACE = 7                  # INTERFACE there: what init and the functio
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
            "tq_qjl_scores.hip", "tq_decode.hip", "tq_wide.hip", "tq_many.hip", "tq_many_d64.hip", "tq_many_d96.hip", "tq_many_d128.hip", "tq_many_d256.hip", "tq_evict.hip",
-           "tq_paged.hip", "tq_paged_d64.hip", "tq_paged_d96.hip", "tq_paged_d128.hip", "tq_paged_d256.hip", "tq_pages.hip", "tq_beam.hip", "tq_host.cpp")
-HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", "tq_many.h", "tq_many_kernel.h", "tq_many_fast.h", "tq_paged.h", "tq_paged_kernel.h",
+           "tq_paged.hip", "tq_paged_d64.hip", "tq_paged_d96.hip", "tq_paged_d128.hip", "tq_paged_d256.hip", "tq_paged_few_d64.hip", "tq_paged_few_d96.hip",
+           "tq_paged_few_d128.hip", "tq_paged_few_d256.hip", "tq_pages.hip", "tq_beam.hip", "tq_host.cpp")
+HEADERS = ("tq_table.h", "tq_device.h", "tq_anydim.h", "tq_wide.h", "tq_wide_kernel.h", "tq_lut.h", "tq_decode.h", "tq_decode_kernel.h", "tq_many.h", "tq_many_kernel.h", "tq_many_fast.h", "tq_paged.h", "tq_paged_kernel.h", "tq_paged_few.h",
            os.path.join("..", "..", "include", "tqamd.h"))
 GPU_ARCH = "gfx950"
 
@@ -229,7 +230,7 @@ class TqMoveSegment(ctypes.Structure):
 
 
 class TqPagedCounts(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_longlong) for n in ("items", "merges", "records")] + [("tiles", ctypes.c_int), ("columns", ctypes.c_int)]
+    _fields_ = [(n, ctypes.c_longlong) for n in ("items", "few", "merges", "records")] + [(n, ctypes.c_int) for n in ("tiles", "columns", "vectors")]
 
 
 class TqPagedRequest(ctypes.Structure):
@@ -328,7 +329,7 @@ def lib() -> ctypes.CDLL:
     L.tq_copy_pages.argtypes = [vp, ll, vp, ll, ll, ll, vp, ll, vp]
     L.tq_put_tokens.argtypes = [vp, vp, ll, ll, ll, ll, vp, ll, ll, vp, ll, ll, ll, ci, vp]
     L.tq_paged_supported.argtypes = [ci, ci, ci, ci]
-    L.tq_paged_plan.argtypes = [vp, ll, ci, ci, ci, ci, ci, vp, ll, vp, ll, vp]
+    L.tq_paged_plan.argtypes = [vp, ll, ci, ci, ci, ci, ci, ci, vp, ll, vp, ll, vp]
     L.tq_paged_scratch.restype = ll
     L.tq_paged_scratch.argtypes = [vp, ci, ci]
     L.tq_paged_attend.argtypes = [vp, vp, ll, vp]

@@ -631,7 +631,7 @@ PyObject *paged_attend(PyObject *const *a) {
     tq_paged_request r = *reinterpret_cast<const tq_paged_request *>(integer(a[0]));
     const long long tokens = integer(a[2]), floats = integer(a[6]);
     NEED(q.dim() == 3 && dtype_code(q) == r.dtype && q.device() == like.device() && q.size(0) == tokens && q.size(1) == (long long)r.heads * r.group && q.size(2) == r.head_dim &&
-         q.stride(2) == 1 && tokens > 0);
+         q.stride(2) == 1 && tokens > 0 && aligned(address(q), 16) && (q.stride(0) * (long long)q.element_size()) % 16 == 0 && (q.stride(1) * (long long)q.element_size()) % 16 == 0);
     r.scale = (float)PyFloat_AsDouble(a[3]);
     r.softcap = 0.f;
     if (a[4] != Py_None) {

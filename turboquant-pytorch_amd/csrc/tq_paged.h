@@ -20,9 +20,9 @@ struct TqPagedArgs {
     const int32_t *items;            // {sequence, first tile, packed tokens from, to, plain ones from, to (multiples of 32, or the end), record or -1: all its tokens are here}
     const int32_t *merges;           // {sequence, first tile, first record, records}
     const float *slopes;             // [query heads], or null
-    float *rec;                      // [records][heads][QT][cols largest logits, cols sums, cols x DP value sums]
+    float *rec;                      // [records][heads][qt][cols largest logits, cols sums, cols x DP value sums]
     float scale, cap;                // cap: 0 for none
-    uint32_t heads, group, D, dtype, bits_k, bits_v, shift, cols, window, aligned;      // window: 0 for none
+    uint32_t heads, group, D, dtype, bits_k, bits_v, shift, cols, qt, window, aligned;      // qt: tiles of a record; window: 0 for none
 };
 
 namespace {
@@ -36,3 +36,8 @@ int tq_paged_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPa
 int tq_paged_launch_d96(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt);
 int tq_paged_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt);
 int tq_paged_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt);
+// Launches tq_paged_few_kernel for one head dimension; vectors: the most query vectors of a kv head of a sequence, at most 16
+int tq_paged_few_launch_d64(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, uint32_t vectors);
+int tq_paged_few_launch_d96(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, uint32_t vectors);
+int tq_paged_few_launch_d128(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, uint32_t vectors);
+int tq_paged_few_launch_d256(int ipbk, int ipbv, dim3 grid, hipStream_t s, const TqPagedArgs &a, uint32_t vectors);

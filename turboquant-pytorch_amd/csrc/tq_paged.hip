@@ -13,7 +13,8 @@ constexpr int MERGE_THREADS = 256;
 
 // Block = (merge, kv head, tile of the pair, share of a tile's results): results are the records' sums, each times 2^(its reference - the largest), over their sums of weights.
 template <int DP>
-__global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedArgs a, uint32_t qt, uint32_t shares) {
+__global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedArgs a, uint32_t shares) {
+    const uint32_t qt = a.qt;
     __shared__ float lds_m[MAX_PIECES * 32], lds_l[MAX_PIECES * 32];
     uint32_t at = blockIdx.x;
     const uint32_t share = at % shares;
@@ -80,28 +81,29 @@ bool supported(int D, int dtype, int bits_k, int bits_v) {
     return D > 64 && D <= 96 && !(D & 7) && !(D % ik) && !(D % iv) && !(D / ik & 3) && !(D / iv & 3);
 }
 
-// Times in tokens: what a block's packed tokens, its uncompressed ones and its start and end cost, for one tile of queries and for two, and what a merge does.
+// Times in quarters of a token of the kernel for one tile of 32 query vectors: what a block's packed tokens, its uncompressed ones and its start and end take.  qt: tiles a block, 0 for
+// the kernel for few query vectors.
 struct Costs {
     long long token, plain, block;
 };
 Costs costs(int qt, int dtype) {
-    // (quarters of a token)
+    if (qt == 0) return {2, 8, 4000};
     if (dtype == TQ_F32) return {12, 24, 6000};
     if (qt == 2) return {6, 14, 8000};
     return {4, 8, 6000};
 }
 
-struct Reach {                       // what a group of tiles sees of its sequence, in runs of 32
+struct Reach {                       // what a group of tiles sees of its sequence, in runs
     long long packed_from, packed_to, plain_from, plain_to;
     long long runs(const Costs &c) const { return (packed_to - packed_from + 31) / 32 * 32 * c.token + (plain_to - plain_from + 31) / 32 * 32 * c.plain; }
 };
-Reach reach(const int32_t *s, long long group, long long window, long long tile0, long long tiles) {
+Reach reach(const int32_t *s, long long group, long long window, long long tile0, long long tiles, long long run) {
     const long long fresh = s[1], total = s[2], packed = s[3], first_pos = total - fresh + tile0 * 32 / group;
     long long last = ((tile0 + tiles) * 32 - 1) / group;
     if (last > fresh - 1) last = fresh - 1;
     const long long end = total - fresh + last + 1, lo = window && first_pos >= window ? first_pos - window + 1 : 0;
     Reach r;
-    r.packed_from = (lo < packed ? lo : packed) / 32 * 32;
+    r.packed_from = lo / run * run;
     r.packed_to = packed;
     if (lo >= packed) r.packed_from = r.packed_to = 0;
     r.plain_from = lo > packed ? (lo - packed) / 32 * 32 : 0;
@@ -114,23 +116,67 @@ struct Group {
     Reach reach;
     long long cost;
 };
+struct Item {
+    int32_t v[PAGED_ITEM];
+    long long cost;
+};
+struct Shares {                      // how the blocks of a launch share its groups
+    std::vector<Group> groups;
+    long long piece = 0, time = -1;
+    int qt = 1;
+};
+
+// Pieces of the longest group from one to MAX_PIECES: the number with the shortest time by the costs above.  As many rounds of blocks as the card takes, each as long as a block
+// is on average, and no less than the longest block.
+void share(Shares &best, std::vector<Group> &groups, int qt, int dtype, int heads, int cus) {
+    const Costs c = costs(qt, dtype);
+    long long longest = 0;
+    for (Group &g : groups) {
+        g.cost = g.reach.runs(c);
+        if (g.cost > longest) longest = g.cost;
+    }
+    bool better = false;
+    for (long long k = 1; k <= MAX_PIECES; ++k) {
+        const long long piece = (longest + k - 1) / k;
+        if (piece < 128 * c.token && k > 1) break;
+        long long blocks = 0, all = 0, pieces = 1;
+        for (const Group &g : groups) {
+            const long long own = g.cost ? (g.cost + piece - 1) / piece : 1;
+            blocks += own;
+            all += g.cost + own * c.block;
+            if (own > pieces) pieces = own;
+        }
+        blocks *= heads;
+        all *= heads;
+        const long long rounds = (blocks + cus - 1) / cus;
+        long long time = rounds * (all / blocks);
+        if (time < piece + c.block) time = piece + c.block;
+        if (pieces > 1) time += 6000 + 120 * pieces;
+        if (best.time < 0 || time < best.time) { best.time = time; best.piece = piece; best.qt = qt; better = true; }
+        if (rounds > 16 && k > 1) break;
+    }
+    if (better) best.groups.swap(groups);
+}
 
 }  // namespace
 
 extern "C" int tq_paged_supported(int head_dim, int dtype, int bits_k, int bits_v) { return supported(head_dim, dtype, bits_k, bits_v) ? 1 : 0; }
 
-extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int32_t *items, long long max_items, int32_t *merges,
-                             long long max_merges, tq_paged_counts *counts) {
+extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, int group, int window, int head_dim, int dtype, int page_tokens, int32_t *items, long long max_items,
+                             int32_t *merges, long long max_merges, tq_paged_counts *counts) {
     if (!counts || (n > 0 && !sequences)) return TQ_ERR_NULL;
     if (n < 0 || heads < 1 || group < 1 || window < 0 || max_items < 0 || max_merges < 0) return TQ_ERR_SIZE;
-    long long tiles = 0, most = 0;
+    // Few query vectors a kv head: one token of up to 16 query heads, or some of fewer (16-bit elements; runs of 64 tokens, so pages of no less).
+    const bool has_few = dtype != TQ_F32 && page_tokens >= 64 && (head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256);
+    long long tiles = 0, most = 0, vectors = 0;
     for (long long b = 0; b < n; ++b) {
         const int32_t *s = sequences + b * PAGED_SEQ;
         if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[3] < 0 || s[3] > s[2] - s[1] || s[4] < 0 || s[5] < 0) return TQ_ERR_SIZE;
         if ((long long)s[1] * group > 0x7fffffff - 64) return TQ_ERR_SIZE;
-        const long long t = ((long long)s[1] * group + 31) / 32;
+        const long long m = (long long)s[1] * group, t = (m + 31) / 32;
         tiles += t;
-        if (t > most) most = t;
+        if (has_few && m <= 16) vectors = std::max(vectors, m);
+        else most = std::max(most, t);
     }
     *counts = tq_paged_counts{};
     counts->tiles = 1;
@@ -138,84 +184,61 @@ extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, i
     int cus = 0;
     if (tq_device_cus(cus)) cus = 256;
     try {
-        // Of one or two tiles a block and up to MAX_PIECES pieces of the longest, the pair with the shortest time by the costs above: as many rounds of blocks as the card takes, each
-        // as long as a block is on average, and no less than the longest block.
-        std::vector<Group> best;
-        long long best_time = -1, best_piece = 0;
-        int best_qt = 1;
-        const bool two = dtype == TQ_BF16 && head_dim != 256 && most > 1;
-        for (int qt = 1; qt <= (two ? 2 : 1); ++qt) {
-            const Costs c = costs(qt, dtype);
-            std::vector<Group> groups;
-            long long longest = 0;
-            for (long long b = 0; b < n; ++b) {
-                const int32_t *s = sequences + b * PAGED_SEQ;
-                const long long t = ((long long)s[1] * group + 31) / 32;
-                for (long long t0 = 0; t0 < t; t0 += qt) {
-                    Group g{(int32_t)b, (int32_t)t0, reach(s, group, window, t0, qt), 0};
-                    g.cost = g.reach.runs(c);
-                    if (g.cost > longest) longest = g.cost;
-                    groups.push_back(g);
-                }
-            }
-            for (long long k = 1; k <= MAX_PIECES; ++k) {
-                long long piece = (longest + k - 1) / k;
-                if (piece < 128 * c.token && k > 1) break;
-                long long blocks = 0, all = 0, pieces = 1;
-                for (const Group &g : groups) {
-                    const long long own = g.cost ? (g.cost + piece - 1) / piece : 1;
-                    blocks += own;
-                    all += g.cost + own * c.block;
-                    if (own > pieces) pieces = own;
-                }
-                blocks *= heads;
-                all *= heads;
-                const long long rounds = (blocks + cus - 1) / cus;
-                long long time = rounds * (all / blocks);
-                if (time < piece + c.block) time = piece + c.block;
-                if (pieces > 1) time += 6000 + 120 * pieces;
-                if (best_time < 0 || time < best_time) { best_time = time; best_piece = piece; best_qt = qt; best.clear(); }
-                if (rounds > 16 && k > 1) break;
-            }
-            if (best_qt == qt && best.empty()) best.swap(groups);
-        }
-        const Costs c = costs(best_qt, dtype);
-        struct Item { int32_t v[PAGED_ITEM]; long long cost; };
         std::vector<Item> all;
         std::vector<int32_t> joined;
         long long records = 0, columns = 1;
-        for (const Group &g : best) {
-            const Reach &r = g.reach;
-            const long long k = g.cost ? (g.cost + best_piece - 1) / best_piece : 1, each = (g.cost + k - 1) / k;
-            const size_t first = all.size();
-            long long t = r.packed_from, u = r.plain_from;
-            do {
-                Item it{{g.seq, g.tile0, 0, 0, 0, 0, -1, 0}, 0};
-                it.v[2] = (int32_t)t;
-                while (t < r.packed_to && it.cost < each) { t += 32; it.cost += 32 * c.token; }
-                if (t > r.packed_to) t = r.packed_to;
-                it.v[3] = (int32_t)t;
-                it.v[4] = (int32_t)u;
-                while (t >= r.packed_to && u < r.plain_to && it.cost < each) { u += 32; it.cost += 32 * c.plain; }
-                if (u > r.plain_to) u = r.plain_to;
-                it.v[5] = (int32_t)u;
-                all.push_back(it);
-            } while (t < r.packed_to || u < r.plain_to);
-            const long long own = (long long)(all.size() - first);
-            if (own > 1) {
-                joined.insert(joined.end(), {g.seq, g.tile0, (int32_t)records, (int32_t)own});
-                for (size_t i = first; i < all.size(); ++i) all[i].v[6] = (int32_t)records++;
-                const long long m = (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group - 32LL * g.tile0;
-                columns = std::max(columns, std::min(32LL, m));
+        for (int few = 1; few >= 0; --few) {
+            Shares best;
+            // (two tiles a block share what is read and decoded; 96 wide they would spill)
+            const bool two = !few && dtype == TQ_BF16 && (head_dim == 64 || head_dim == 128) && most > 1;
+            for (int qt = 1; qt <= (two ? 2 : 1); ++qt) {
+                std::vector<Group> groups;
+                for (long long b = 0; b < n; ++b) {
+                    const int32_t *s = sequences + b * PAGED_SEQ;
+                    const long long m = (long long)s[1] * group, t = (m + 31) / 32;
+                    if ((has_few && m <= 16) != (few == 1)) continue;
+                    for (long long t0 = 0; t0 < t; t0 += qt) groups.push_back(Group{(int32_t)b, (int32_t)t0, reach(s, group, window, t0, qt, few ? 64 : 32), 0});
+                }
+                if (!groups.empty()) share(best, groups, few ? 0 : qt, dtype, heads, cus);
             }
+            const Costs c = costs(best.qt, dtype);
+            const long long run = few ? 64 : 32;
+            const size_t begin = all.size();
+            for (const Group &g : best.groups) {
+                const Reach &r = g.reach;
+                const long long k = g.cost ? (g.cost + best.piece - 1) / best.piece : 1, each = (g.cost + k - 1) / k;
+                const size_t first = all.size();
+                long long t = r.packed_from, u = r.plain_from;
+                do {
+                    Item it{{g.seq, g.tile0, 0, 0, 0, 0, -1, 0}, 0};
+                    it.v[2] = (int32_t)t;
+                    while (t < r.packed_to && it.cost < each) { t += run; it.cost += run * c.token; }
+                    if (t > r.packed_to) t = r.packed_to;
+                    it.v[3] = (int32_t)t;
+                    it.v[4] = (int32_t)u;
+                    while (t >= r.packed_to && u < r.plain_to && it.cost < each) { u += 32; it.cost += 32 * c.plain; }
+                    if (u > r.plain_to) u = r.plain_to;
+                    it.v[5] = (int32_t)u;
+                    all.push_back(it);
+                } while (t < r.packed_to || u < r.plain_to);
+                const long long own = (long long)(all.size() - first);
+                if (own > 1) {
+                    joined.insert(joined.end(), {g.seq, g.tile0, (int32_t)records, (int32_t)own});
+                    for (size_t i = first; i < all.size(); ++i) all[i].v[6] = (int32_t)records++;
+                    const long long m = (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group - 32LL * g.tile0;
+                    columns = std::max(columns, std::min(32LL, m));
+                }
+            }
+            // the longest first: what is short fills the gaps at the end
+            std::stable_sort(all.begin() + (long)begin, all.end(), [](const Item &x, const Item &y) { return x.cost > y.cost; });
+            if (few) counts->few = (long long)all.size();
+            else if (best.qt == 2) counts->tiles = 2;
         }
-        // the longest first: what is short fills the gaps at the end
-        std::stable_sort(all.begin(), all.end(), [](const Item &x, const Item &y) { return x.cost > y.cost; });
         counts->items = (long long)all.size();
         counts->merges = (long long)joined.size() / PAGED_MERGE;
         counts->records = records;
-        counts->tiles = best_qt;
         counts->columns = (int)columns;
+        counts->vectors = (int)vectors;
         if (counts->items > 0x7fffffff / heads || records > 0x7fffffff) return TQ_ERR_SIZE;
         if (counts->items > max_items || counts->merges > max_merges) return TQ_ERR_CAPACITY;
         if (!items || (counts->merges && !merges)) return TQ_ERR_NULL;
@@ -246,8 +269,9 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     if (r.page_tokens > 0x7fffffff / r.heads / (r.head_dim * 4)) return TQ_ERR_SIZE;
     if (!(r.softcap >= 0.f) || !(r.softcap < __builtin_inff()) || n.items < 0 || n.merges < 0 || n.records < 0) return TQ_ERR_SIZE;
     if (n.items == 0) return TQ_OK;
+    if (n.few < 0 || n.few > n.items || (n.few && (n.vectors < 1 || n.vectors > 16 || r.dtype == TQ_F32 || r.page_tokens < 64 || (r.head_dim & 31)))) return TQ_ERR_SIZE;
     if (n.items > 0x7fffffff / r.heads || n.tiles < 1 || n.tiles > 2 || n.columns < 1 || n.columns > 32) return TQ_ERR_SIZE;
-    if (n.tiles == 2 && (r.dtype != TQ_BF16 || r.head_dim == 256)) return TQ_ERR_SIZE;
+    if (n.tiles == 2 && (r.dtype != TQ_BF16 || (r.head_dim != 64 && r.head_dim != 128))) return TQ_ERR_SIZE;
     if (!r.queries || !r.out || !r.packed_pool || !r.plain_pool || !r.table_k || !r.table_v || !r.sequences || !r.tables || !r.items || (n.merges && (!r.merges || !scratch))) return TQ_ERR_NULL;
     const long long es = r.dtype == TQ_F32 ? 4 : 2;
     // vectors of a page as the kernels read them: runs of 32 tokens 16 bytes at a time (packed bytes of uneven dimensions: words)
@@ -273,18 +297,32 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     a.aligned = !((uintptr_t)r.queries & 15u) && !((r.q_token * es) & 15) && !((r.q_head * es) & 15);
     const int kt = r.dtype == TQ_BF16 ? 1 : 2, vt = r.dtype == TQ_F32 ? 2 : 1, dp = TQ_PADDED_DIM(r.head_dim), ik = 8 / r.bits_k, iv = 8 / r.bits_v;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 g((unsigned)(n.items * r.heads));
-    if (dp == 64) tq_paged_launch_d64(ik, iv, g, s, a, n.tiles, kt, vt);
-    else if (dp == 96) tq_paged_launch_d96(ik, iv, g, s, a, n.tiles, kt, vt);
-    else if (dp == 128) tq_paged_launch_d128(ik, iv, g, s, a, n.tiles, kt, vt);
-    else tq_paged_launch_d256(ik, iv, g, s, a, n.tiles, kt, vt);
+    a.qt = (uint32_t)n.tiles;
+    // the plan's first items are those with few query vectors (whose kernel loads queries 16 bytes at a time; otherwise the other one does all)
+    const long long few = a.aligned ? n.few : 0;
+    if (few) {
+        const dim3 g((unsigned)(few * r.heads));
+        if (dp == 64) tq_paged_few_launch_d64(ik, iv, g, s, a, (uint32_t)n.vectors);
+        else if (dp == 96) tq_paged_few_launch_d96(ik, iv, g, s, a, (uint32_t)n.vectors);
+        else if (dp == 128) tq_paged_few_launch_d128(ik, iv, g, s, a, (uint32_t)n.vectors);
+        else tq_paged_few_launch_d256(ik, iv, g, s, a, (uint32_t)n.vectors);
+    }
+    if (n.items > few) {
+        const dim3 g((unsigned)((n.items - few) * r.heads));
+        TqPagedArgs rest = a;
+        rest.items += few * PAGED_ITEM;
+        if (dp == 64) tq_paged_launch_d64(ik, iv, g, s, rest, n.tiles, kt, vt);
+        else if (dp == 96) tq_paged_launch_d96(ik, iv, g, s, rest, n.tiles, kt, vt);
+        else if (dp == 128) tq_paged_launch_d128(ik, iv, g, s, rest, n.tiles, kt, vt);
+        else tq_paged_launch_d256(ik, iv, g, s, rest, n.tiles, kt, vt);
+    }
     if (n.merges) {
         const uint32_t qt = (uint32_t)n.tiles, shares = ((uint32_t)n.columns * (dp / 4u) + MERGE_THREADS - 1u) / MERGE_THREADS;
         const dim3 gm((unsigned)(n.merges * r.heads * qt * shares)), t(MERGE_THREADS);
-        if (dp == 64) hipLaunchKernelGGL((tq_paged_merge_kernel<64>), gm, t, 0, s, a, qt, shares);
-        else if (dp == 96) hipLaunchKernelGGL((tq_paged_merge_kernel<96>), gm, t, 0, s, a, qt, shares);
-        else if (dp == 128) hipLaunchKernelGGL((tq_paged_merge_kernel<128>), gm, t, 0, s, a, qt, shares);
-        else hipLaunchKernelGGL((tq_paged_merge_kernel<256>), gm, t, 0, s, a, qt, shares);
+        if (dp == 64) hipLaunchKernelGGL((tq_paged_merge_kernel<64>), gm, t, 0, s, a, shares);
+        else if (dp == 96) hipLaunchKernelGGL((tq_paged_merge_kernel<96>), gm, t, 0, s, a, shares);
+        else if (dp == 128) hipLaunchKernelGGL((tq_paged_merge_kernel<128>), gm, t, 0, s, a, shares);
+        else hipLaunchKernelGGL((tq_paged_merge_kernel<256>), gm, t, 0, s, a, shares);
     }
     return (int)hipGetLastError();
 }

@@ -397,7 +397,7 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, uint8_t *lds,
         return;
     }
     if (n >= a.cols) return;
-    TQ_GLOBAL float *rec = (TQ_GLOBAL float *)a.rec + (((size_t)record * a.heads + row.kv) * QT + i) * paged_record(a.cols, DP);
+    TQ_GLOBAL float *rec = (TQ_GLOBAL float *)a.rec + (((size_t)record * a.heads + row.kv) * a.qt + i) * paged_record(a.cols, DP);
     if (w == 0u && h == 0u) { rec[n] = m; rec[a.cols + n] = l; }
 #pragma unroll
     for (int r = 0; r < 16; r += 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(rec + 2u * a.cols + n * DP + d0 + r) = tq_f4{out[r], out[r + 1], out[r + 2], out[r + 3]};
@@ -777,8 +777,8 @@ template <int DP, int IPBK, int IPBV>
 int launch_paged(dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt) {
     if (vt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 2, 2>), grid, dim3(FAST_THREADS), 0, s, a);
     else if (kt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if (DP == 256 || qt == 1) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if constexpr (DP != 256) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 2, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if (DP == 96 || DP == 256 || qt == 1) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if constexpr (DP == 64 || DP == 128) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 2, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
     return 0;
 }
 template <int DP>

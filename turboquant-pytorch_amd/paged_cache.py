@@ -55,6 +55,14 @@ class _Pages:
         heapq.heappush(self.free, page)
         return True
 
+    def drop_all(self, pages: List[int]) -> None:
+        held, free = self.held, self.free
+        for p in pages:
+            n = held[p] - 1
+            held[p] = n
+            if not n:
+                heapq.heappush(free, p)
+
 
 class _Sequence:
     __slots__ = ("pages", "plain", "total")
@@ -190,15 +198,18 @@ class PagedV3Cache:
         if packed > free[0] or plain > free[1]:
             raise _native.TqError(f"{what} needs {packed} packed and {plain} uncompressed pages, {free[0]} and {free[1]} are free (free sequences, or `resize`)")
 
-    def _drop_plain(self, page: int) -> None:
-        if self._plain_pages.drop(page):
-            self._packed_of.pop(page, None)
+    def _drop(self, s: _Sequence) -> None:
+        """A sequence's pages are its no longer."""
+        if s.pages:
+            self._packed_pages.drop_all(s.pages)
+        if s.plain:
+            self._plain_pages.drop_all(s.plain)
 
-    def _drop_packed(self, page: int) -> None:
-        if self._packed_pages.drop(page) and self._packed_of:
-            for plain, packed in list(self._packed_of.items()):
-                if packed == page:
-                    del self._packed_of[plain]
+    def _forget(self) -> None:
+        """Of which pages it is known what they were packed into: those that are still held, as what they became is."""
+        if self._packed_of:
+            plain, packed = self._plain_pages.held, self._packed_pages.held
+            self._packed_of = {p: q for p, q in self._packed_of.items() if plain[p] and packed[q]}
 
     def _settle(self) -> None:
         """An open step is committed before tables change."""
@@ -208,15 +219,15 @@ class PagedV3Cache:
     def free(self, seqs: Sequence[int]) -> None:
         """Sequences end; pages that no other one holds are free."""
         self._settle()
-        states = [self._sequence(s) for s in seqs]
-        if len(set(seqs)) != len(states):
+        known = self._seqs
+        if len(set(seqs)) != len(seqs):
             raise ValueError("free: a sequence ends once")
         for seq in seqs:
-            s = self._seqs.pop(seq)
-            for p in s.pages:
-                self._drop_packed(p)
-            for p in s.plain:
-                self._drop_plain(p)
+            if seq not in known:
+                self._sequence(seq)
+        for seq in seqs:
+            self._drop(known.pop(seq))
+        self._forget()
 
     def _share(self, s: _Sequence) -> _Sequence:
         """A sequence that continues as `s`, with the same pages."""
@@ -287,10 +298,8 @@ class PagedV3Cache:
         self._room("reorder", 0, max(0, twice - ends))
         fresh = [self._share(states[p]) for p in parents]
         for s in states:
-            for page in s.pages:
-                self._drop_packed(page)
-            for page in s.plain:
-                self._drop_plain(page)
+            self._drop(s)
+        self._forget()               # (before a page that has become free is taken again)
         self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i])
         self._seqs.update(zip(seqs, fresh))
 
@@ -457,7 +466,7 @@ class PagedStep:
             self.cache._eager("the first attend of a step with this window")
             c, counts = self.cache, _native.TqPagedCounts()
             call = lambda items, merges: _native.lib().tq_paged_plan(  # noqa: E731
-                self._records.ctypes.data, len(self.seqs), c.kv_heads, group, window, c.head_dim, _native.dtype_code(c.dtype), items.ctypes.data, len(items), merges.ctypes.data,
+                self._records.ctypes.data, len(self.seqs), c.kv_heads, group, window, c.head_dim, _native.dtype_code(c.dtype), c.page_tokens, items.ctypes.data, len(items), merges.ctypes.data,
                 len(merges), ctypes.byref(counts))
             items, merges = np.empty((1024, _native.PAGED_ITEM), np.int32), np.empty((256, _native.PAGED_MERGE), np.int32)
             with _native._on(c.device):
@@ -541,8 +550,10 @@ class PagedStep:
             out = torch.empty(queries.shape, dtype=c.dtype, device=c.device)
             if not self.tokens:
                 return out
-            if queries.stride(2) != 1:
-                queries = queries.contiguous()
+            # (16 bytes at a time: with other loads other kernels would do some of the work, and results differ in their last bits)
+            es = queries.element_size()
+            if queries.stride(2) != 1 or queries.data_ptr() % 16 or queries.stride(0) * es % 16 or queries.stride(1) * es % 16:
+                queries = queries.clone(memory_format=torch.contiguous_format)
             ready = self._request(layer, heads // c.kv_heads, window)
             floats, uploaded = ready[1:3]
             if uploaded[2] == self._blob[2]:
@@ -570,25 +581,34 @@ class PagedStep:
         if self.tokens and len(self._appended) != c.n_layers:
             missing = sorted(set(range(c.n_layers)) - self._appended)
             raise RuntimeError(f"commit: layers {missing[:8]} have not been appended to in this step")
-        made: List[Tuple[int, int]] = []
+        becomes: Dict[int, int] = {}         # uncompressed page -> packed page, of those that are packed now
+        moves: List[Tuple[_Sequence, List[int]]] = []
         for s in self._states:
-            for _ in range((s.total - c.residual_window) // c.page_tokens - len(s.pages)):
-                plain = s.plain[0]
-                packed = c._packed_of.get(plain)
+            pages: List[int] = []
+            for plain in s.plain[:max(0, (s.total - c.residual_window) // c.page_tokens - len(s.pages))]:
+                packed = becomes.get(plain, c._packed_of.get(plain))
                 if packed is None:
                     if not c._packed_pages.free:
                         break
-                    packed = c._packed_pages.take()
-                    made.append((plain, packed))
-                    if c._plain_pages.held[plain] > 1:
-                        c._packed_of[plain] = packed
+                    packed = becomes[plain] = c._packed_pages.take()
                 else:
                     c._packed_pages.held[packed] += 1
-                del s.plain[0]
-                s.pages.append(packed)
-                c._drop_plain(plain)
-        if made:
-            self._pack(np.asarray(made, dtype=np.uint64))
+                pages.append(packed)
+            if pages:
+                moves.append((s, pages))
+        try:
+            if becomes:
+                self._pack(np.asarray(list(becomes.items()), dtype=np.uint64))
+        except BaseException:                # (tables stay as they were)
+            for _, pages in moves:
+                c._packed_pages.drop_all(pages)
+            raise
+        c._packed_of.update(becomes)
+        for s, pages in moves:
+            c._plain_pages.drop_all(s.plain[:len(pages)])
+            del s.plain[:len(pages)]
+            s.pages += pages
+        c._forget()
         self._done = True
         if c._open is self:
             c._open = None
