@@ -572,14 +572,15 @@ int tq_put_tokens(const void *keys, const void *values, long long k_token_stride
  *   packed_pool, plain_pool     the layer's part of page 0 (key codes; keys), from which the other parts and the other pages are so many bytes on
  *   queries     new token i, query head j at i * q_token + j * q_head elements; query head j reads kv head j / group.  out: dense [new tokens, heads * group, head_dim]
  *   softcap     0: none; otherwise logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
- * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, 4 a merge; counts also where they do not fit
- * (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim, dtype and page_tokens.
+ * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, then blocks + 1 (where each block's items
+ * begin), in room for 8 * max_items; 8 a merge; counts also where they do not fit (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim, dtype and page_tokens.
  * tq_paged_scratch: float32 values of scratch (16-byte aligned, not shared by calls that can overlap in time).
  * tq_paged_supported: head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose packed vectors are words; 2 to 8 bits.
- * Infinities and NaN reach the results of the queries that see them and no others.  Numbers of pages are not checked.  Pages are read whole runs of 32 tokens at a time.
+ * Infinities and NaN reach the results of the queries that see them and no others.  Numbers of pages are not checked.  Queries' vectors lie at multiples of 16 bytes where counts.few is not zero
+ * (TQ_ERR_ALIGN).  Pages are read whole runs of 32 tokens at a time.
  */
 typedef struct tq_paged_counts {
-    long long items, few, merges, records;     /* few: the first items, those of sequences with few query vectors */
+    long long items, few, blocks, merges, records;     /* few: the first items, those of sequences with few query vectors, by so many blocks */
     int tiles, columns, vectors;
 } tq_paged_counts;
 typedef struct tq_paged_request {

@@ -15,6 +15,8 @@ def plan(pkg, sequences, heads=2, group=4, window=0, D=128, dtype=2, room=100000
     counts = native.TqPagedCounts()
     items, merges = np.empty((room, native.PAGED_ITEM), np.int32), np.empty((room, native.PAGED_MERGE), np.int32)
     rc = native.lib().tq_paged_plan(records.ctypes.data, len(records), heads, group, window, D, dtype, page, items.ctypes.data, room, merges.ctypes.data, room, ctypes.byref(counts))
+    blocks = items.ravel()[counts.items * native.PAGED_ITEM:][:counts.blocks + 1 if counts.few else 0].tolist()
+    assert rc or (counts.few == 0) == (not blocks) and (not blocks or (blocks[0] == 0 and blocks[-1] == counts.few and blocks == sorted(blocks)))
     return rc, counts, items[:counts.items], merges[:counts.merges]
 
 
@@ -36,13 +38,16 @@ def test_a_plan_covers_what_is_seen_once(pkg, sequences, window):
         assert rc == 0 and counts.tiles in ((1, 2) if dtype == 2 and D in (64, 128) else (1,)) and 1 <= counts.columns <= 32
         by_group = {}
         for it in items.tolist():
-            by_group.setdefault((it[0], it[1]), []).append(it[2:7])
-        records, joined = [], {(m[0], m[1]): (m[2], m[3]) for m in merges.tolist()}
+            for h in range(heads) if it[7] < 0 else (it[7],):
+                by_group.setdefault((it[0], it[1], h), []).append(it[2:6] + [it[6] if it[6] < 0 or it[7] >= 0 else it[6] + h])
+        records, joined = [], {(m[0], m[1], m[2]): m[3:6] for m in merges.tolist()}
+        assert len(joined) == len(merges)
         for b, (fresh, total, packed) in enumerate(sequences):
             tiles = -(-fresh * group // 32)
             step, unit = (1, 64) if small[b] else (counts.tiles, 32)
             for t0 in range(0, tiles, step):
-                parts = by_group.pop((b, t0))
+              for head in range(heads):
+                parts = by_group.pop((b, t0, head))
                 first, last = total - fresh + t0 * 32 // group, total - fresh + min(fresh - 1, ((t0 + step) * 32 - 1) // group)
                 lo = max(0, first - window + 1) if window else 0
                 covered = set()
@@ -56,8 +61,8 @@ def test_a_plan_covers_what_is_seen_once(pkg, sequences, window):
                 want |= set(range(1 << 26 | max(0, lo - packed) // 32, 1 << 26 | -(-(last + 1 - packed) // 32)))
                 assert covered == want
                 if len(parts) > 1:
-                    start, n = joined.pop((b, t0))
-                    assert sorted(p[4] for p in parts) == list(range(start, start + n)) and n == len(parts) <= 64
+                    start, n, gap = joined.pop((b, t0, head))
+                    assert sorted(p[4] for p in parts) == list(range(start, start + n * gap, gap)) and n == len(parts) <= 64
                     assert counts.columns >= min(32, fresh * group - 32 * t0)
                     records += [p[4] for p in parts]
                 else:
@@ -103,7 +108,7 @@ def test_attention_checks_its_request(pkg):
     for name in ("queries", "out", "packed_pool", "plain_pool", "table_k", "table_v", "sequences", "tables", "items", "merges"):
         setattr(r, name, 4096)
     need = L.tq_paged_scratch(ctypes.byref(counts), 8, 128)
-    assert rc == 0 and counts.merges == 1 and need == counts.records * 8 * counts.columns * 130
+    assert rc == 0 and counts.merges == 8 and need == counts.records * counts.columns * 130
     assert L.tq_paged_attend(ctypes.byref(r), 4096, need - 1, None) == -10 and L.tq_paged_attend(None, None, 0, None) == -1
     assert L.tq_paged_scratch(None, 8, 128) == -1 and L.tq_paged_scratch(ctypes.byref(counts), 0, 128) == -5 and L.tq_paged_scratch(ctypes.byref(counts), 8, 7) == -3
     copy = lambda: native.TqPagedRequest.from_buffer_copy(r)  # noqa: E731

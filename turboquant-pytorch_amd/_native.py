@@ -230,7 +230,7 @@ class TqMoveSegment(ctypes.Structure):
 
 
 class TqPagedCounts(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_longlong) for n in ("items", "few", "merges", "records")] + [(n, ctypes.c_int) for n in ("tiles", "columns", "vectors")]
+    _fields_ = [(n, ctypes.c_longlong) for n in ("items", "few", "blocks", "merges", "records")] + [(n, ctypes.c_int) for n in ("tiles", "columns", "vectors")]
 
 
 class TqPagedRequest(ctypes.Structure):
@@ -240,7 +240,7 @@ class TqPagedRequest(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("heads", "group", "sliding_window", "page_tokens", "head_dim", "dtype", "bits_k", "bits_v")])
 
 
-PAGED_SEQ, PAGED_ITEM, PAGED_MERGE = 8, 8, 4       # numbers of a sequence, an item of the plan and a merge, as tq_paged.h has them
+PAGED_SEQ, PAGED_ITEM, PAGED_MERGE = 8, 8, 8       # numbers of a sequence, an item of the plan and a merge, as tq_paged.h has them
 
 EXPORTS = (
     "tq_abi_version", "tq_status_string", "tq_device_count", "tq_bytes_per_vector",

@@ -6,7 +6,7 @@
 #include "tq_many.h"
 
 // Six numbers a sequence, eight apart: first row of its queries, its new tokens, all its tokens, packed ones, and where in the tables its packed and its plain pages begin
-constexpr int PAGED_SEQ = 8, PAGED_ITEM = 8, PAGED_MERGE = 4;
+constexpr int PAGED_SEQ = 8, PAGED_ITEM = 8, PAGED_MERGE = 8;
 
 struct TqPagedArgs {
     const uint8_t *q;                // new token i, query head j at i * q_token + j * q_head elements
@@ -17,10 +17,12 @@ struct TqPagedArgs {
     long long k_norms, v_idx, v_norms, plain_v;      // bytes from the layer's key codes (plain: keys)
     const uint8_t *table_k, *table_v;
     const int32_t *seqs, *tables;
-    const int32_t *items;            // {sequence, first tile, packed tokens from, to, plain ones from, to (multiples of 32, or the end), record or -1: all its tokens are here}
-    const int32_t *merges;           // {sequence, first tile, first record, records}
+    const int32_t *items;            // {sequence, first tile, packed tokens from, to, plain ones from, to (multiples of 32, or the end), record or -1: all its tokens are here, kv head or -1: one block
+                                     // each, whose record is the item's and so many on}
+    const int32_t *blocks;           // items of sequences with few query vectors: block i has items [blocks[i], blocks[i + 1])
+    const int32_t *merges;           // {sequence, first tile, kv head, first record, records, from one of them to the next, two unused}
     const float *slopes;             // [query heads], or null
-    float *rec;                      // [records][heads][qt][cols largest logits, cols sums, cols x DP value sums]
+    float *rec;                      // [records][qt][cols largest logits, cols sums, cols x DP value sums]
     float scale, cap;                // cap: 0 for none
     uint32_t heads, group, D, dtype, bits_k, bits_v, shift, cols, qt, window, aligned;      // qt: tiles of a record; window: 0 for none
 };

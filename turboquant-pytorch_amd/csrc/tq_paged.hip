@@ -11,23 +11,17 @@ namespace {
 constexpr int MAX_PIECES = 64;
 constexpr int MERGE_THREADS = 256;
 
-// Block = (merge, kv head, tile of the pair, share of a tile's results): results are the records' sums, each times 2^(its reference - the largest), over their sums of weights.
+// Block = (merge, tile of the pair, share of a tile's results): results are the records' sums, each times 2^(its reference - the largest), over their sums of weights.
 template <int DP>
 __global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedArgs a, uint32_t shares) {
-    const uint32_t qt = a.qt;
     __shared__ float lds_m[MAX_PIECES * 32], lds_l[MAX_PIECES * 32];
-    uint32_t at = blockIdx.x;
-    const uint32_t share = at % shares;
-    at /= shares;
-    const uint32_t i = at % qt;
-    at /= qt;
-    const uint32_t kv = at % a.heads, merge = at / a.heads;
+    const uint32_t share = blockIdx.x % shares, at = blockIdx.x / shares, i = at % a.qt, merge = at / a.qt;
     const int32_t *mg = a.merges + (size_t)merge * PAGED_MERGE;
     const int32_t *sq = a.seqs + (size_t)mg[0] * PAGED_SEQ;
-    const uint32_t tile = (uint32_t)mg[1] + i, records = (uint32_t)mg[3], M = (uint32_t)sq[1] * a.group, tid = threadIdx.x;
+    const uint32_t tile = (uint32_t)mg[1] + i, kv = (uint32_t)mg[2], records = (uint32_t)mg[4], M = (uint32_t)sq[1] * a.group, tid = threadIdx.x;
     if (tile * 32u >= M) return;
-    const size_t step = (size_t)a.heads * qt * paged_record(a.cols, DP);
-    const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + (((size_t)mg[2] * a.heads + kv) * qt + i) * paged_record(a.cols, DP);
+    const size_t step = (size_t)mg[5] * a.qt * paged_record(a.cols, DP);
+    const TQ_GLOBAL float *rec = (const TQ_GLOBAL float *)a.rec + ((size_t)mg[3] * a.qt + i) * paged_record(a.cols, DP);
     for (uint32_t j = tid; j < records * a.cols; j += MERGE_THREADS) {
         const uint32_t r = j / a.cols, c = j - r * a.cols;
         lds_m[j] = rec[r * step + c];
@@ -81,13 +75,11 @@ bool supported(int D, int dtype, int bits_k, int bits_v) {
     return D > 64 && D <= 96 && !(D & 7) && !(D % ik) && !(D % iv) && !(D / ik & 3) && !(D / iv & 3);
 }
 
-// Times in quarters of a token of the kernel for one tile of 32 query vectors: what a block's packed tokens, its uncompressed ones and its start and end take.  qt: tiles a block, 0 for
-// the kernel for few query vectors.
+// Times in quarters of a token of the kernel for one tile of 32 query vectors: what a block's packed tokens, its uncompressed ones and its start and end take.
 struct Costs {
     long long token, plain, block;
 };
 Costs costs(int qt, int dtype) {
-    if (qt == 0) return {2, 8, 4000};
     if (dtype == TQ_F32) return {12, 24, 6000};
     if (qt == 2) return {6, 14, 8000};
     return {4, 8, 6000};
@@ -158,6 +150,133 @@ void share(Shares &best, std::vector<Group> &groups, int qt, int dtype, int head
     if (better) best.groups.swap(groups);
 }
 
+struct Plan {
+    std::vector<Item> items;
+    std::vector<int32_t> blocks, merges;
+    long long records = 0, columns = 1;
+    // pieces items[first] ... of one row, `step` from a record to the next
+    void join(size_t first, int32_t seq, int32_t tile0, int32_t head, long long vectors, long long step) {
+        const long long own = (long long)(items.size() - first);
+        merges.insert(merges.end(), {seq, tile0, head, (int32_t)records, (int32_t)own, (int32_t)step, 0, 0});
+        columns = std::max(columns, std::min(32LL, vectors));
+    }
+};
+
+// Sequences with few query vectors: the rows (sequence, kv head) of a launch laid end to end and cut into as many equal shares as there are blocks, one a compute unit; a row that is cut is
+// merged.  Or, where that takes less time, whole rows dealt out, the longest first to the block that has least.  Times in packed tokens of a block (4 ns; 64 ... 128 x 2048 x 8 heads: 25.0 us
+// without cuts, 21.0 with 64 blocks; 8 rows of 32768: 151 with 8 blocks, 30 with 128, 25 with 192): an uncompressed one three, an item 1100, a merge 1200 and 25 a piece.
+constexpr long long FEW_PLAIN = 3, FEW_ITEM = 1100, FEW_MERGE = 1200, FEW_PIECE = 25, FEW_LEAST = 512;
+void plan_few(Plan &p, std::vector<Group> &groups, int heads, int cus, const int32_t *sequences, int group) {
+    long long all = 0, longest = 0;
+    for (Group &g : groups) {
+        g.cost = g.reach.packed_to - g.reach.packed_from + FEW_PLAIN * ((g.reach.plain_to - g.reach.plain_from + 31) / 32 * 32);
+        all += g.cost * heads;
+        longest = std::max(longest, g.cost);
+    }
+    const long long rows = (long long)groups.size() * heads;
+    // whole rows
+    std::vector<std::pair<long long, std::vector<std::pair<int32_t, int32_t>>>> dealt((size_t)std::min<long long>(rows, cus));
+    {
+        std::vector<size_t> order(groups.size());
+        for (size_t i = 0; i < order.size(); ++i) order[i] = i;
+        std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return groups[x].cost > groups[y].cost; });
+        std::vector<std::pair<long long, size_t>> heap;          // (least first)
+        for (size_t i = 0; i < dealt.size(); ++i) heap.emplace_back(0, i);
+        const auto more = [](const std::pair<long long, size_t> &x, const std::pair<long long, size_t> &y) { return x > y; };
+        for (size_t i : order)
+            for (int h = 0; h < heads; ++h) {
+                std::pop_heap(heap.begin(), heap.end(), more);
+                heap.back().first += groups[i].cost + FEW_ITEM;
+                dealt[heap.back().second].second.emplace_back((int32_t)i, h);
+                dealt[heap.back().second].first = heap.back().first;
+                std::push_heap(heap.begin(), heap.end(), more);
+            }
+    }
+    long long best = 0, blocks = 0, room = 0;
+    for (const auto &d : dealt) best = std::max(best, d.first);
+    for (long long nb = cus; nb >= 1; nb /= 2) {
+        long long share = (all + FEW_ITEM * (rows + nb) + nb - 1) / nb;
+        share = std::max(share, std::max(longest / (MAX_PIECES - 4) + FEW_ITEM, FEW_LEAST + FEW_ITEM));
+        const long long time = share + FEW_MERGE + FEW_PIECE * (longest / (share - FEW_ITEM) + 1);
+        if (time < best) { best = time; blocks = nb; room = share; }
+    }
+    if (!blocks) {
+        for (const auto &d : dealt) {
+            p.blocks.push_back((int32_t)p.items.size());
+            for (const auto &[i, h] : d.second) {
+                const Group &g = groups[(size_t)i];
+                p.items.push_back(Item{{g.seq, 0, (int32_t)g.reach.packed_from, (int32_t)g.reach.packed_to, (int32_t)g.reach.plain_from, (int32_t)g.reach.plain_to, -1, h}, 0});
+            }
+        }
+        p.blocks.push_back((int32_t)p.items.size());
+        return;
+    }
+    long long left = room;
+    p.blocks.push_back((int32_t)p.items.size());
+    for (const Group &g : groups)
+        for (int h = 0; h < heads; ++h) {
+            const Reach &r = g.reach;
+            const size_t first = p.items.size();
+            long long t = r.packed_from, u = r.plain_from, cost = g.cost;
+            do {
+                long long can = left - FEW_ITEM;
+                if (can < FEW_LEAST && can < cost) {             // (the next block)
+                    p.blocks.push_back((int32_t)p.items.size());
+                    left = room;
+                    can = left - FEW_ITEM;
+                }
+                if (cost <= can + FEW_LEAST / 2) can = cost;
+                Item it{{g.seq, 0, (int32_t)t, 0, (int32_t)u, 0, -1, h}, 0};
+                while (t < r.packed_to && it.cost < can) { t += 64; it.cost += 64; }
+                if (t > r.packed_to) { it.cost -= t - r.packed_to; t = r.packed_to; }
+                while (t >= r.packed_to && u < r.plain_to && it.cost < can) { u += 32; it.cost += 32 * FEW_PLAIN; }
+                if (u > r.plain_to) u = r.plain_to;
+                it.v[3] = (int32_t)t;
+                it.v[5] = (int32_t)u;
+                cost -= it.cost;
+                left -= it.cost + FEW_ITEM;
+                p.items.push_back(it);
+            } while (t < r.packed_to || u < r.plain_to);
+            if (p.items.size() - first > 1) {
+                p.join(first, g.seq, 0, h, (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group, 1);
+                for (size_t i = first; i < p.items.size(); ++i) p.items[i].v[6] = (int32_t)p.records++;
+            }
+        }
+    p.blocks.push_back((int32_t)p.items.size());
+}
+
+// The others: a block an item and kv head.
+void plan_many(Plan &p, const Shares &best, int heads, int dtype, const int32_t *sequences, int group) {
+    const Costs c = costs(best.qt, dtype);
+    const size_t begin = p.items.size();
+    for (const Group &g : best.groups) {
+        const Reach &r = g.reach;
+        const long long k = g.cost ? (g.cost + best.piece - 1) / best.piece : 1, each = (g.cost + k - 1) / k;
+        const size_t first = p.items.size();
+        long long t = r.packed_from, u = r.plain_from;
+        do {
+            Item it{{g.seq, g.tile0, (int32_t)t, 0, (int32_t)u, 0, -1, -1}, 0};
+            while (t < r.packed_to && it.cost < each) { t += 32; it.cost += 32 * c.token; }
+            if (t > r.packed_to) t = r.packed_to;
+            while (t >= r.packed_to && u < r.plain_to && it.cost < each) { u += 32; it.cost += 32 * c.plain; }
+            if (u > r.plain_to) u = r.plain_to;
+            it.v[3] = (int32_t)t;
+            it.v[5] = (int32_t)u;
+            p.items.push_back(it);
+        } while (t < r.packed_to || u < r.plain_to);
+        if (p.items.size() - first > 1) {
+            const long long vectors = (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group - 32LL * g.tile0;
+            for (int h = 0; h < heads; ++h) {
+                p.join(first, g.seq, g.tile0, h, vectors, heads);
+                p.merges[p.merges.size() - PAGED_MERGE + 3] += h;
+            }
+            for (size_t i = first; i < p.items.size(); ++i, p.records += heads) p.items[i].v[6] = (int32_t)p.records;
+        }
+    }
+    // the longest first: what is short fills the gaps at the end
+    std::stable_sort(p.items.begin() + (long)begin, p.items.end(), [](const Item &x, const Item &y) { return x.cost > y.cost; });
+}
+
 }  // namespace
 
 extern "C" int tq_paged_supported(int head_dim, int dtype, int bits_k, int bits_v) { return supported(head_dim, dtype, bits_k, bits_v) ? 1 : 0; }
@@ -184,9 +303,7 @@ extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, i
     int cus = 0;
     if (tq_device_cus(cus)) cus = 256;
     try {
-        std::vector<Item> all;
-        std::vector<int32_t> joined;
-        long long records = 0, columns = 1;
+        Plan p;
         for (int few = 1; few >= 0; --few) {
             Shares best;
             // (two tiles a block share what is read and decoded; 96 wide they would spill)
@@ -199,51 +316,28 @@ extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, i
                     if ((has_few && m <= 16) != (few == 1)) continue;
                     for (long long t0 = 0; t0 < t; t0 += qt) groups.push_back(Group{(int32_t)b, (int32_t)t0, reach(s, group, window, t0, qt, few ? 64 : 32), 0});
                 }
-                if (!groups.empty()) share(best, groups, few ? 0 : qt, dtype, heads, cus);
+                if (groups.empty()) continue;
+                if (few) plan_few(p, groups, heads, cus, sequences, group);
+                else share(best, groups, qt, dtype, heads, cus);
             }
-            const Costs c = costs(best.qt, dtype);
-            const long long run = few ? 64 : 32;
-            const size_t begin = all.size();
-            for (const Group &g : best.groups) {
-                const Reach &r = g.reach;
-                const long long k = g.cost ? (g.cost + best.piece - 1) / best.piece : 1, each = (g.cost + k - 1) / k;
-                const size_t first = all.size();
-                long long t = r.packed_from, u = r.plain_from;
-                do {
-                    Item it{{g.seq, g.tile0, 0, 0, 0, 0, -1, 0}, 0};
-                    it.v[2] = (int32_t)t;
-                    while (t < r.packed_to && it.cost < each) { t += run; it.cost += run * c.token; }
-                    if (t > r.packed_to) t = r.packed_to;
-                    it.v[3] = (int32_t)t;
-                    it.v[4] = (int32_t)u;
-                    while (t >= r.packed_to && u < r.plain_to && it.cost < each) { u += 32; it.cost += 32 * c.plain; }
-                    if (u > r.plain_to) u = r.plain_to;
-                    it.v[5] = (int32_t)u;
-                    all.push_back(it);
-                } while (t < r.packed_to || u < r.plain_to);
-                const long long own = (long long)(all.size() - first);
-                if (own > 1) {
-                    joined.insert(joined.end(), {g.seq, g.tile0, (int32_t)records, (int32_t)own});
-                    for (size_t i = first; i < all.size(); ++i) all[i].v[6] = (int32_t)records++;
-                    const long long m = (long long)sequences[(size_t)g.seq * PAGED_SEQ + 1] * group - 32LL * g.tile0;
-                    columns = std::max(columns, std::min(32LL, m));
-                }
+            if (few) counts->few = (long long)p.items.size();
+            else if (!best.groups.empty()) {
+                plan_many(p, best, heads, dtype, sequences, group);
+                counts->tiles = best.qt;
             }
-            // the longest first: what is short fills the gaps at the end
-            std::stable_sort(all.begin() + (long)begin, all.end(), [](const Item &x, const Item &y) { return x.cost > y.cost; });
-            if (few) counts->few = (long long)all.size();
-            else if (best.qt == 2) counts->tiles = 2;
         }
-        counts->items = (long long)all.size();
-        counts->merges = (long long)joined.size() / PAGED_MERGE;
-        counts->records = records;
-        counts->columns = (int)columns;
+        counts->items = (long long)p.items.size();
+        counts->blocks = p.blocks.empty() ? 0 : (long long)p.blocks.size() - 1;
+        counts->merges = (long long)p.merges.size() / PAGED_MERGE;
+        counts->records = p.records;
+        counts->columns = (int)p.columns;
         counts->vectors = (int)vectors;
-        if (counts->items > 0x7fffffff / heads || records > 0x7fffffff) return TQ_ERR_SIZE;
-        if (counts->items > max_items || counts->merges > max_merges) return TQ_ERR_CAPACITY;
+        if (counts->items > 0x7fffffff / heads || p.records > 0x7fffffff || counts->merges > 0x7fffffff / 64) return TQ_ERR_SIZE;
+        if (counts->items * PAGED_ITEM + (long long)p.blocks.size() > max_items * PAGED_ITEM || counts->merges > max_merges) return TQ_ERR_CAPACITY;
         if (!items || (counts->merges && !merges)) return TQ_ERR_NULL;
-        for (size_t i = 0; i < all.size(); ++i) std::copy(all[i].v, all[i].v + PAGED_ITEM, items + i * PAGED_ITEM);
-        std::copy(joined.begin(), joined.end(), merges);
+        for (size_t i = 0; i < p.items.size(); ++i) std::copy(p.items[i].v, p.items[i].v + PAGED_ITEM, items + i * PAGED_ITEM);
+        std::copy(p.blocks.begin(), p.blocks.end(), items + p.items.size() * PAGED_ITEM);
+        std::copy(p.merges.begin(), p.merges.end(), merges);
     } catch (...) {
         return TQ_ERR_CAPACITY;              // (no memory)
     }
@@ -254,7 +348,7 @@ extern "C" long long tq_paged_scratch(const tq_paged_counts *counts, int heads, 
     if (!counts) return TQ_ERR_NULL;
     if (head_dim < TQ_ANYDIM_MIN || head_dim > TQ_ANYDIM_MAX) return TQ_ERR_HEAD_DIM;
     if (heads < 1 || counts->records < 0 || counts->tiles < 1 || counts->tiles > 2 || counts->columns < 0 || counts->columns > 32) return TQ_ERR_SIZE;
-    return counts->records * heads * counts->tiles * (long long)paged_record((uint32_t)counts->columns, (uint32_t)TQ_PADDED_DIM(head_dim));
+    return counts->records * counts->tiles * (long long)paged_record((uint32_t)counts->columns, (uint32_t)TQ_PADDED_DIM(head_dim));
 }
 
 extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, long long scratch_floats, void *stream) {
@@ -269,7 +363,7 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     if (r.page_tokens > 0x7fffffff / r.heads / (r.head_dim * 4)) return TQ_ERR_SIZE;
     if (!(r.softcap >= 0.f) || !(r.softcap < __builtin_inff()) || n.items < 0 || n.merges < 0 || n.records < 0) return TQ_ERR_SIZE;
     if (n.items == 0) return TQ_OK;
-    if (n.few < 0 || n.few > n.items || (n.few && (n.vectors < 1 || n.vectors > 16 || r.dtype == TQ_F32 || r.page_tokens < 64 || (r.head_dim & 31)))) return TQ_ERR_SIZE;
+    if (n.few < 0 || n.few > n.items || n.blocks < 0 || n.blocks > 0x7fffffff || (n.few && (n.blocks < 1 || n.vectors < 1 || n.vectors > 16 || r.dtype == TQ_F32 || r.page_tokens < 64 || (r.head_dim & 31)))) return TQ_ERR_SIZE;
     if (n.items > 0x7fffffff / r.heads || n.tiles < 1 || n.tiles > 2 || n.columns < 1 || n.columns > 32) return TQ_ERR_SIZE;
     if (n.tiles == 2 && (r.dtype != TQ_BF16 || (r.head_dim != 64 && r.head_dim != 128))) return TQ_ERR_SIZE;
     if (!r.queries || !r.out || !r.packed_pool || !r.plain_pool || !r.table_k || !r.table_v || !r.sequences || !r.tables || !r.items || (n.merges && (!r.merges || !scratch))) return TQ_ERR_NULL;
@@ -298,10 +392,12 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     const int kt = r.dtype == TQ_BF16 ? 1 : 2, vt = r.dtype == TQ_F32 ? 2 : 1, dp = TQ_PADDED_DIM(r.head_dim), ik = 8 / r.bits_k, iv = 8 / r.bits_v;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     a.qt = (uint32_t)n.tiles;
-    // the plan's first items are those with few query vectors (whose kernel loads queries 16 bytes at a time; otherwise the other one does all)
-    const long long few = a.aligned ? n.few : 0;
+    // the plan's first items are those with few query vectors
+    const long long few = n.few;
+    a.blocks = r.items + n.items * PAGED_ITEM;
+    if (few && !a.aligned) return TQ_ERR_ALIGN;
     if (few) {
-        const dim3 g((unsigned)(few * r.heads));
+        const dim3 g((unsigned)n.blocks);
         if (dp == 64) tq_paged_few_launch_d64(ik, iv, g, s, a, (uint32_t)n.vectors);
         else if (dp == 96) tq_paged_few_launch_d96(ik, iv, g, s, a, (uint32_t)n.vectors);
         else if (dp == 128) tq_paged_few_launch_d128(ik, iv, g, s, a, (uint32_t)n.vectors);
@@ -318,7 +414,7 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     }
     if (n.merges) {
         const uint32_t qt = (uint32_t)n.tiles, shares = ((uint32_t)n.columns * (dp / 4u) + MERGE_THREADS - 1u) / MERGE_THREADS;
-        const dim3 gm((unsigned)(n.merges * r.heads * qt * shares)), t(MERGE_THREADS);
+        const dim3 gm((unsigned)(n.merges * qt * shares)), t(MERGE_THREADS);
         if (dp == 64) hipLaunchKernelGGL((tq_paged_merge_kernel<64>), gm, t, 0, s, a, shares);
         else if (dp == 96) hipLaunchKernelGGL((tq_paged_merge_kernel<96>), gm, t, 0, s, a, shares);
         else if (dp == 128) hipLaunchKernelGGL((tq_paged_merge_kernel<128>), gm, t, 0, s, a, shares);

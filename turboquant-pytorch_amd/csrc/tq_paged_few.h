@@ -6,9 +6,104 @@
 
 namespace {
 
-// Block = (item of the plan, kv head).  Up to 16 / C query vectors are the columns of 16 x 16 x 32 products, C times over, so that C blocks of 16 tokens share a softmax: every block's
+// 32 uncompressed tokens of a page against up to 16 query vectors: scores as raw 16-bit products, softmax, weights in three bf16 terms (fp16: two of fp16) times the raw values.  Infinite
+// and NaN values count as zero here (`wild` says whether there are any, see paged_wild).
+template <int D, bool BF>
+struct FewPlain {
+    static constexpr int SK = D / 32, NC = D / 16, PT = BF ? 3 : 2;
+    static constexpr bool HELD = D <= 128;
+    static constexpr int VW = HELD ? NC / 2 : 4;         // words of a lane's coordinates that are held at a time
+    static constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
+    tq_u4 k[SK][2];
+    uint32_t v[8][VW];
+    const uint8_t *vw;
+    uint32_t valid;
+    static __device__ __forceinline__ uint32_t token(int j, uint32_t q4) { return 16u * (j / 4) + 4u * q4 + (uint32_t)(j % 4); }
+    // N coordinates from c0 on, into words w0 ...
+    template <int N> __device__ __forceinline__ void load_columns(uint32_t lane, int c0, int w0) {
+        const uint32_t first = value_coord<D>(lane & 15u, c0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t *src = vw + token(j, lane >> 4) * (2u * D) + 2u * first;
+            if constexpr (N == 8) { const tq_u4 x = tq_gload16(src); v[j][w0] = x[0]; v[j][w0 + 1] = x[1]; v[j][w0 + (VW > 2 ? 2 : 0)] = x[2]; v[j][w0 + (VW > 3 ? 3 : 0)] = x[3]; }
+            else if constexpr (N == 4) { const tq_u2 x = tq_gload8(src); v[j][w0] = x[0]; v[j][w0 + 1] = x[1]; }
+            else v[j][w0] = tq_gload4(src);
+        }
+    }
+    // keys, values: of the head's first of the 32 tokens (the page holds all of them; those from `valid` on are not used)
+    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint32_t valid_, uint32_t lane) {
+        valid = valid_;
+        vw = values;
+#pragma unroll
+        for (int s = 0; s < SK; ++s)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) k[s][b] = tq_gload16(keys + (16u * b + (lane & 15u)) * (2u * D) + 64 * s + 16u * (lane >> 4));
+        if constexpr (D == 64 || D == 128) load_columns<NC>(lane, 0, 0);
+        else if constexpr (D == 96) { load_columns<4>(lane, 0, 0); load_columns<2>(lane, 4, 2); }
+    }
+    __device__ __forceinline__ void scores(const tq_u4 (&q)[SK], float (&x)[8]) const {
+        tq_f4v sc[2] = {tq_f4v{0.f, 0.f, 0.f, 0.f}, tq_f4v{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int s = 0; s < SK; ++s)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sc[b] = BF ? mfma16_bf16(k[s][b], q[s], sc[b]) : mfma16_f16(k[s][b], q[s], sc[b]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = sc[j / 4][j % 4];
+    }
+    __device__ __forceinline__ void tame(uint32_t lane, bool &wild) {
+        uint32_t over = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < VW; ++c) {
+                if (token(j, lane >> 4) >= valid) v[j][c] = 0u;
+                over |= (v[j][c] & EXPO) + ONE;          // (an exponent of ones carries into the sign's place)
+            }
+        if (__any((over & 0x80008000u) != 0u)) {
+            wild = true;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < VW; ++c) v[j][c] &= ~(((((v[j][c] & EXPO) + ONE) >> 15) & 0x00010001u) * 0xffffu);
+        }
+    }
+    // acc[c]: register r = column 4 q4 + r, coordinate value_coord(n16, c)
+    __device__ __forceinline__ void values(const float (&p)[8], uint32_t lane, bool &wild, tq_f4v (&acc)[NC]) {
+        tq_u4 pa[3];
+        if constexpr (BF) bf16_terms(p, pa);
+        else {
+            uint32_t t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = fp16_terms(p[j]);
+            fp16_operands(t, pa[0], pa[1]);
+        }
+        auto column = [&](int c, int w) __attribute__((always_inline)) {
+            tq_u4 bt;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) bt[d] = __builtin_amdgcn_perm(v[2 * d + 1][w], v[2 * d][w], (c & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int t = 0; t < PT; ++t) acc[c] = BF ? mfma16_bf16(pa[t], bt, acc[c]) : mfma16_f16(pa[t], bt, acc[c]);
+        };
+        if constexpr (HELD) {
+            tame(lane, wild);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) column(c, c / 2);
+        } else {
+#pragma unroll
+            for (int c0 = 0; c0 < NC; c0 += 8) {
+                load_columns<8>(lane, c0, 0);
+                tame(lane, wild);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) column(c0 + c, c / 2);
+            }
+        }
+    }
+};
+
+// A block takes items of the plan in turn, each a share of what the queries of a (sequence, kv head) see; the tables stay in LDS.  Up to 16 / C query vectors are the columns of 16 x 16 x 32 products, C times over, so that C blocks of 16 tokens share a softmax: every block's
 // scores are made for all columns, a lane keeps those of its own column's block, and the weights of the others are zeros in its column of the value product (as in tq_decode_kernel, whose
-// loop this is, with runs found through the sequence's pages: a run lies within a page, whose number is fetched a run ahead).  QT: fp16 terms of a rotated query, one for bfloat16.
+// loop this is, with runs found through the sequence's pages: a run lies within a page, whose number is fetched a run ahead).  QT: fp16 terms of a rotated query, one for bfloat16 (two then, and two of the levels, for float16: with one the result of half a unit's
+// rounding, 2.1e-4, came out at 6e-4).
 // Base-2 logits are rounded before the reference is taken off, so that the largest ones stay exact against it however large they are.
 template <int D, int IPBK, int IPBV, int C, bool BF>
 __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedArgs a) {
@@ -20,41 +115,115 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     constexpr int VPB = GBV % 16 ? 8 : 16, VBYTES = RUN * GBV, VPIECES = VBYTES / VPB, NVP = (VPIECES + 63) / 64;
     constexpr float SLACK = 8.f;
     constexpr int P_SHIFT = 14 - 8;
-    constexpr int HR = HEADS < 8 ? HEADS : 8;            // columns a round of the join
+    constexpr int HR = D == 256 && C == 1 ? 4 : HEADS < 8 ? HEADS : 8;            // columns a round of the join
     constexpr int QROW = D + 4;
-    using J = JoinArea<D, 1>;
-    static_assert(DW * HR * PART * 4 <= (int)J::PACKED, "the waves' sums and the joined ones side by side");
-    constexpr uint32_t Q_AT = 65536u + DW * VBYTES, LOOP_BYTES = Q_AT + 16u * QROW * 4u, AREA = LOOP_BYTES > J::BYTES ? LOOP_BYTES : J::BYTES;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];           // tables, values of each wave, rotated queries; later the waves' sums and the joined ones
+    // LDS: tables; then values of each wave and rotated queries, later the waves' sums and the joined ones (packed tokens', plain ones')
+    constexpr uint32_t V_AT = 65536u, Q_AT = V_AT + DW * VBYTES, LOOP_END = Q_AT + 16u * QROW * 4u;
+    constexpr uint32_t JOIN_AT = V_AT, SUMS_AT = JOIN_AT + DW * HR * PART * 4u, SUMS = HEADS * QROW * 4u, STATS_AT = SUMS_AT + 2u * SUMS, JOIN_END = STATS_AT + 4u * HEADS * 4u;
+    constexpr uint32_t AREA = LOOP_END > JOIN_END ? LOOP_END : JOIN_END;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[DW][RUN];
     __shared__ __attribute__((aligned(16))) uint16_t lds_vn[DW][RUN];      // value norms / 2^ev_ref
     __shared__ __attribute__((aligned(16))) tq_u4 lds_q[QT > QREG ? (QT - QREG) * SK : 1][TQ_WAVE];
     __shared__ __attribute__((aligned(16))) float lds_corr[DW][16];
-    __shared__ float lds_m[FAST_WAVES][32], lds_l[FAST_WAVES][32];
     __shared__ uint32_t lds_trips[DW];
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n16 = lane & 15u, q4 = lane >> 4;
-    const uint32_t item = blockIdx.x / a.heads;
-    const int32_t *it = a.items + (size_t)item * PAGED_ITEM;
+    {
+        const uint32_t tid = threadIdx.x;
+        std::conditional_t<BF, Lut<IPBK>, Lut2<IPBK>> table_k;
+        Lut<IPBV> table_v;
+        if constexpr (BF) table_k.load(a.table_k + TQ_OFF_LUT(D), tid);
+        else table_k.load(a.table_k, a.bits_k, D, tid);
+        table_v.load(a.table_v + TQ_OFF_LUT(D), tid);
+        table_k.store(lds, tid);
+        table_v.store(lds + 128, tid);
+    }
+#pragma unroll 1
+    for (int32_t index = a.blocks[blockIdx.x]; index < a.blocks[blockIdx.x + 1]; ++index) {
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));        // (what lanes make of their number is made anew for every item: kept from one to the next it took a hundred registers that there are not)
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n16 = lane & 15u, q4 = lane >> 4, head = n16 % HEADS, cls = n16 / HEADS;
+    const bool shaped = a.cap != 0.f || a.slopes;
+    const Cap cap(a);
+    const int32_t *it = a.items + (size_t)index * PAGED_ITEM;
     const int32_t *sq = a.seqs + (size_t)it[0] * PAGED_SEQ;
     const uint32_t t_begin = (uint32_t)it[2], t_end = (uint32_t)it[3], plain_from = (uint32_t)it[4], plain_to = (uint32_t)it[5];
     const int record = it[6];
     PagedRow row;
     row.fresh = (uint32_t)sq[1]; row.total = (uint32_t)sq[2]; row.packed = (uint32_t)sq[3];
     row.pages = a.tables + sq[4]; row.plain_pages = a.tables + sq[5];
-    row.kv = blockIdx.x - item * a.heads;
+    row.kv = (uint32_t)it[7];
     const uint32_t q_first = (uint32_t)sq[0], M = row.fresh * a.group;
     const uint8_t *queries = a.q + ((long long)q_first * a.q_token + (long long)(row.kv * a.group) * a.q_head) * 2;
-    const uint32_t head = n16 % HEADS, cls = n16 / HEADS;
     const bool live = head < M;
+    const uint32_t vector = min(head, M - 1u), token = vector / a.group, pos = row.total - row.fresh + token;        // of this lane's column
+    const float slope = a.slopes ? a.slopes[row.kv * a.group + (vector - token * a.group)] * LOG2E : 0.f;
+    float *const sums = reinterpret_cast<float *>(lds + SUMS_AT), *const stats = reinterpret_cast<float *>(lds + STATS_AT);       // [packed, plain][HEADS][QROW]; [largest, total][HEADS] of each
+
+    // The waves' sums of HR columns at a time meet in LDS (which: 0 packed, 1 plain); unit: what this wave's value sums are multiplied by, l: all lanes' of a column
+    auto join = [&](uint32_t which, float m_ref, float l, float unit, const tq_f4v (&acc)[NC]) __attribute__((always_inline)) {
+        float *const mine = reinterpret_cast<float *>(lds + JOIN_AT) + wave * (HR * PART);
+        for (uint32_t h0 = 0; h0 < (uint32_t)HEADS && h0 < M; h0 += HR) {
+            __syncthreads();         // (values, queries, and the round before)
+            if (q4 == 0u && n16 < (uint32_t)HEADS && n16 >= h0 && n16 < h0 + HR) {
+                mine[(n16 - h0) * PART] = m_ref;
+                mine[(n16 - h0) * PART + 1u] = l;
+            }
+            if (C == 1 || which) {
+                if (4u * q4 >= h0 && 4u * q4 < min(h0 + HR, (uint32_t)HEADS)) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) mine[(4u * q4 + r - h0) * PART + 2u + value_coord<D>(n16, c)] = acc[c][r] * unit;
+                }
+            } else {
+                // The blocks of tokens lie in lanes 32 apart (C = 4: and 16 apart): two registers exchange halves and are added, which leaves the sum of one in each half (then quarters).
+                static_assert(C == 1 || HR >= HEADS, "one round");
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float half[NC / 2];
+#pragma unroll
+                    for (int c = 0; c < NC; c += 2) half[c / 2] = fold<32>(acc[c][r], acc[c + 1][r]);
+                    if constexpr (C == 2) {
+#pragma unroll
+                        for (int c = 0; c < NC; c += 2) mine[(4u * (q4 & 1u) + r) * PART + 2u + value_coord<D>(n16, c + (int)(q4 >> 1))] = half[c / 2] * unit;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < NC; c += 4) {
+                            const bool pair = c + 2 < NC;     // (96: the last two columns stand alone, both quarters hold them)
+                            const float sum = fold<16>(half[c / 2], half[pair ? c / 2 + 1 : c / 2]);
+                            mine[r * PART + 2u + value_coord<D>(n16, c + (int)((pair ? 2u * (q4 & 1u) : 0u) + (q4 >> 1)))] = sum * unit;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            const float *all = reinterpret_cast<const float *>(lds + JOIN_AT);
+            for (uint32_t i = tid; i < HR * D; i += DTHREADS) {
+                const uint32_t col = i / D, d = i - col * D;
+                float m = MANY_NONE, sum = 0.f, total = 0.f;
+#pragma unroll
+                for (int w = 0; w < DW; ++w) m = fmaxf(m, all[(w * HR + col) * PART]);
+#pragma unroll
+                for (int w = 0; w < DW; ++w) {
+                    const float own = all[(w * HR + col) * PART], lw = all[(w * HR + col) * PART + 1u];
+                    const float f = own != MANY_NONE ? __builtin_amdgcn_exp2f(own - m) : lw == 0.f ? 0.f : __builtin_nanf("");
+                    sum = fmaf(all[(w * HR + col) * PART + 2u + d], f, sum);
+                    total = fmaf(lw, f, total);
+                }
+                sums[which * (SUMS / 4u) + (h0 + col) * QROW + d] = sum;
+                if (d == 0u) {
+                    stats[(2u * which) * HEADS + h0 + col] = m;
+                    stats[(2u * which + 1u) * HEADS + h0 + col] = total;
+                }
+            }
+        }
+    };
 
     if (t_end > t_begin) {
-        const uint32_t token = min(head, M - 1u) / a.group, pos = row.total - row.fresh + token;
-        const float slope = a.slopes ? a.slopes[row.kv * a.group + (min(head, M - 1u) - token * a.group)] * LOG2E : 0.f;
         const uint32_t lo = a.window && pos >= a.window ? pos - a.window + 1u : 0u;              // first token that this lane's column sees
         const uint32_t last_pos = row.total - 1u, whole_from = a.window && last_pos >= a.window ? last_pos - a.window + 1u : 0u;
-        const bool shaped = a.cap != 0.f || a.slopes;
-        uint8_t *vcodes = lds + 65536 + wave * VBYTES;
+        uint8_t *vcodes = lds + V_AT + wave * VBYTES;
         // Runs of a wave: in every whole round of the block one of RUN tokens; what is left of the block's tokens is dealt out evenly, in blocks of 16, 32 or 64 tokens (which lie within a
         // page), so that no wave works on a whole run alone at the end.
         const uint32_t rounds = (t_end - t_begin) / (RUN * DW), rest0 = t_begin + rounds * (RUN * DW), rest = t_end - rest0;
@@ -119,21 +288,15 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             kn_raw = tq_gload2(reinterpret_cast<const uint16_t *>(base + a.k_norms) + own);
             vn_raw = tq_gload2(reinterpret_cast<const uint16_t *>(base + a.v_norms) + own);
         };
-        // ---- start: tables, then the operands of the query rotation (the first waves), then the first run
-        if (tid < (uint32_t)DW) lds_trips[tid] = 0u;
-        Lut<IPBK> table_k;
-        Lut<IPBV> table_v;
-        table_k.load(a.table_k + TQ_OFF_LUT(D), tid);
-        table_v.load(a.table_v + TQ_OFF_LUT(D), tid);
+        // ---- start: the operands of the query rotation (the first waves), then the first run
         Where now = where(0u), next = where(1u);
-        __builtin_amdgcn_sched_barrier(0);
         auto first_run = [&]() __attribute__((always_inline)) {
             __builtin_amdgcn_sched_barrier(0);
             issue_keys(now, max(run_tokens(0u), 1u));
             issue_values(now, max(run_tokens(0u), 1u));
             __builtin_amdgcn_sched_barrier(0);
-            table_k.store(lds, tid);
-            table_v.store(lds + 128, tid);
+            __syncthreads();         // (what the item before has left in LDS is read)
+            if (tid < (uint32_t)DW) lds_trips[tid] = 0u;
         };
         if (wave < (uint32_t)TILES) {
             Rotation<D, BF> r;
@@ -165,7 +328,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             if (big > 0.f && big < __builtin_inff()) (void)frexpf(big, &e);
             e = e < -100 ? -100 : e;
             const float up = ldexpf(1.f, TQ_F16_PI_SHIFT - e);
-            c1 = live ? ldexpf(LOG2E, e - TQ_F16_PI_SHIFT) : 0.f;
+            c1 = live ? ldexpf(LOG2E, e - TQ_F16_PI_SHIFT - (BF ? 0 : LEVEL_SHIFT)) : 0.f;
 #pragma unroll
             for (int s = 0; s < SK; ++s) {
                 tq_half8 term[QT];
@@ -184,7 +347,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
                 for (int k = QREG; k < QT; ++k) lds_q[(k - QREG) * SK + s][lane] = __builtin_bit_cast(tq_u4, term[k]);     // (the same in every wave, and each writes it)
             }
         }
-        const uint32_t slot_k = RepLut<IPBK>::lane_offset(lane), slot_v = 128u + RepLut<IPBV>::lane_offset(lane);
+        const uint32_t slot_k = BF ? RepLut<IPBK>::lane_offset(lane) : Lut2<IPBK>::lane_offset(lane), slot_v = 128u + RepLut<IPBV>::lane_offset(lane);
         tq_f4v acc[NC];          // register r = column 4 q4 + r, c = coordinate value_coord(n16, c)
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[c] = tq_f4v{0.f, 0.f, 0.f, 0.f};
@@ -200,9 +363,14 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
                 sc[u][0] = sc[u][1] = tq_f4v{0.f, 0.f, 0.f, 0.f};
                 if (!FULL && 32u * u >= n_tok) continue;       // uniform
                 auto step = [&](int b, int s, const tq_u4 (&q)[QT]) __attribute__((always_inline)) {
-                    const tq_u4 kd = decode_keys<IPBK, NWK>(kraw[u][b], s, lds, slot_k);
-#pragma unroll
-                    for (int k = 0; k < QT; ++k) sc[u][b] = mfma16_f16(kd, q[k], sc[u][b]);
+                    if constexpr (BF) sc[u][b] = mfma16_f16(decode_keys<IPBK, NWK>(kraw[u][b], s, lds, slot_k), q[0], sc[u][b]);
+                    else {
+                        tq_u4 hi, lo;
+                        decode_keys2<IPBK, NWK>(kraw[u][b], s, lds, slot_k, hi, lo);
+                        sc[u][b] = mfma16_f16(hi, q[0], sc[u][b]);
+                        sc[u][b] = mfma16_f16(hi, q[QT - 1], sc[u][b]);
+                        sc[u][b] = mfma16_f16(lo, q[0], sc[u][b]);
+                    }
                 };
                 auto terms = [&](int s, tq_u4 (&q)[QT]) __attribute__((always_inline)) {
 #pragma unroll
@@ -248,8 +416,13 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
 #pragma unroll
                 for (int j = 0; j < SPL; ++j) asm volatile("" : "+v"(z[j]));        // (rounded here, not fused with what is taken off)
                 if (shaped) {
+                    if (a.cap != 0.f) {
 #pragma unroll
-                    for (int j = 0; j < SPL; ++j) z[j] = shape_logit(a, z[j], slope, (float)((int)(t0 + tok + 16u * (j / 4) + (j % 4)) - (int)pos));
+                        for (int j = 0; j < SPL; ++j) z[j] = cap.template operator()<false>(z[j]);
+                    }
+                    const float first = (float)((int)(t0 + tok) - (int)pos);
+#pragma unroll
+                    for (int j = 0; j < SPL; ++j) z[j] = fmaf(slope, first + (float)(16 * (j / 4) + j % 4), z[j]);
                 }
                 auto gone = [&](int j) { const uint32_t i = tok + 16u * (j / 4) + (j % 4); return i >= n_tok || t0 + i < lo; };
                 if constexpr (!FULL) {
@@ -392,79 +565,89 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             if (lane == 0u) *(volatile __attribute__((address_space(3))) uint32_t *)&lds_trips[wave] = 0xffffffffu;
             __builtin_amdgcn_s_setprio(0);
         }
-        // ---- the waves' sums of HR columns at a time meet in LDS
         float l_all = l_run;
 #pragma unroll
         for (int d = HEADS; d < 64; d <<= 1) l_all += __shfl_xor(l_all, d);
-        l_all *= 1.0f / (float)(1 << P_SHIFT);
-        const float unit = ldexpf(1.f, ev_ref - P_SHIFT);
-        float *const mine = reinterpret_cast<float *>(lds) + wave * (HR * PART);
-        for (uint32_t h0 = 0; h0 < (uint32_t)HEADS && h0 < M; h0 += HR) {
-            __syncthreads();         // (tables, values, and the round before)
-            if (q4 == 0u && cls == 0u && n16 >= h0 && n16 < h0 + HR) {
-                mine[(n16 - h0) * PART] = m_ref;
-                mine[(n16 - h0) * PART + 1u] = l_all;
-            }
-            if constexpr (C == 1) {
-                if (4u * q4 >= h0 && 4u * q4 < h0 + HR) {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) mine[(4u * q4 + r - h0) * PART + 2u + value_coord<D>(n16, c)] = acc[c][r] * unit;
-                }
-            } else {
-                // The blocks of tokens lie in lanes 32 apart (C = 4: and 16 apart): two registers exchange halves and are added, which leaves the sum of one in each half (then quarters).
-                static_assert(HR >= HEADS, "one round");
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float half[NC / 2];
-#pragma unroll
-                    for (int c = 0; c < NC; c += 2) half[c / 2] = fold<32>(acc[c][r], acc[c + 1][r]);
-                    if constexpr (C == 2) {
-#pragma unroll
-                        for (int c = 0; c < NC; c += 2) mine[(4u * (q4 & 1u) + r) * PART + 2u + value_coord<D>(n16, c + (int)(q4 >> 1))] = half[c / 2] * unit;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < NC; c += 4) {
-                            const bool pair = c + 2 < NC;     // (96: the last two columns stand alone, both quarters hold them)
-                            const float sum = fold<16>(half[c / 2], half[pair ? c / 2 + 1 : c / 2]);
-                            mine[r * PART + 2u + value_coord<D>(n16, c + (int)((pair ? 2u * (q4 & 1u) : 0u) + (q4 >> 1)))] = sum * unit;
-                        }
-                    }
-                }
-            }
-            __syncthreads();
-            const float *all = reinterpret_cast<const float *>(lds);
-            for (uint32_t i = tid; i < HR * D; i += DTHREADS) {
-                const uint32_t col = i / D, d = i - col * D;
-                float m = MANY_NONE, sum = 0.f, total = 0.f;
-#pragma unroll
-                for (int w = 0; w < DW; ++w) m = fmaxf(m, all[(w * HR + col) * PART]);
-#pragma unroll
-                for (int w = 0; w < DW; ++w) {
-                    const float own = all[(w * HR + col) * PART], l = all[(w * HR + col) * PART + 1u];
-                    const float f = own != MANY_NONE ? __builtin_amdgcn_exp2f(own - m) : l == 0.f ? 0.f : __builtin_nanf("");
-                    sum = fmaf(all[(w * HR + col) * PART + 2u + d], f, sum);
-                    total = fmaf(l, f, total);
-                }
-                J::sums(lds, 0u, 0u)[(h0 + col) * (D + 4u) + d] = sum;
-                if (d == 0u) {
-                    J::largest(lds, 0u, 0u)[h0 + col] = m;
-                    J::total(lds, 0u, 0u)[h0 + col] = total;
-                }
-            }
-        }
-        __syncthreads();
+        join(0u, m_ref, l_all * (1.0f / (float)(1 << P_SHIFT)), ldexpf(1.f, ev_ref - P_SHIFT), acc);
     }
-    const bool plain = plain_to > plain_from;
+    const bool packed = t_end > t_begin, plain = plain_to > plain_from;
     if (plain) {
-        TqManyArgs v;            // (queries as the plain tokens' products take them: "heads" are the sequence's tokens)
-        v.q = queries;
-        v.q_batch = 0; v.q_head = a.q_token; v.q_token = a.q_head;
-        v.heads = 1u; v.queries = a.group; v.M = M; v.D = a.D; v.aligned = 1u;
-        paged_plain_phase<D, 1, BF ? TQ_BF16 : TQ_F16>(a, v, row, lds, lds_m, lds_l, &lds_corr[0][0], 0u, 1u, plain_from, plain_to, tid);
+        // ---- uncompressed tokens: a wave takes 32 at a time, columns as they are (not C times over)
+        const uint32_t runs = (plain_to - plain_from + 31u) / 32u, col = min(n16, M - 1u), ct = col / a.group, cpos = row.total - row.fresh + ct;
+        const float cslope = a.slopes ? a.slopes[row.kv * a.group + (col - ct * a.group)] * LOG2E : 0.f;
+        const uint8_t *cq = queries + ((long long)ct * a.q_token + (long long)(col - ct * a.group) * a.q_head) * 2;
+        tq_f4v acc[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c] = tq_f4v{0.f, 0.f, 0.f, 0.f};
+        float m_ref = MANY_NONE, l = 0.f;
+        bool wild = false;
+#pragma unroll 1
+        for (uint32_t w = wave; w < runs; w += DW) {
+            const uint32_t t0 = plain_from + 32u * w;
+            const uint8_t *page = a.plain + (long long)(int)tq_uniform32((uint32_t)row.plain_pages[t0 >> a.shift]) * a.plain_stride + (size_t)((row.kv << a.shift) + (t0 & ((1u << a.shift) - 1u))) * (2u * D);
+            FewPlain<D, BF> t;
+            tq_u4 q[SK];
+#pragma unroll
+            for (int s = 0; s < SK; ++s) q[s] = tq_gload16(cq + 64 * s + 16u * q4);
+            t.load(page, page + a.plain_v, min(32u, plain_to - t0), lane);
+            float x[8];
+            t.scores(q, x);
+            const uint32_t at = row.packed + t0, gone = unseen_bits(at, cpos, a.window);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= a.scale * LOG2E;
+            if (a.cap != 0.f) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = cap.template operator()<false>(x[j]);
+            }
+            float top = m_ref;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t i = FewPlain<D, BF>::token(j, q4);
+                x[j] = fmaf(cslope, (float)((int)(at + i) - (int)cpos), x[j]);
+                x[j] = i < t.valid && !((gone >> i) & 1u) ? x[j] : MANY_NONE;
+                top = fmaxf(top, x[j]);
+            }
+            top = reduce_rows(top, OpMax());
+            const float shrink = __builtin_amdgcn_exp2f(m_ref - top);
+            m_ref = top;
+            l *= shrink;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = x[j] == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(x[j] - top);
+                l += x[j];               // (this lane's tokens)
+            }
+            if (w != wave) {             // (sums so far: a lane has those of columns 4 q4 ...)
+                float4 c4;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) (&c4.x)[r] = __shfl(shrink, (int)(4u * q4 + r));
+#pragma unroll
+                for (int c = 0; c < NC; ++c) { acc[c][0] *= c4.x; acc[c][1] *= c4.y; acc[c][2] *= c4.z; acc[c][3] *= c4.w; }
+            }
+            t.values(x, lane, wild, acc);
+        }
+        l = reduce_rows(l, OpAdd());
+        wild = __any(wild);
+        join(1u, m_ref, l, 1.f, acc);
+        if (lane == 0u) lds_corr[wave][0] = wild ? 1.f : 0.f;
+        __syncthreads();
+        float any = 0.f;
+#pragma unroll
+        for (int w = 0; w < DW; ++w) any += lds_corr[w][0];
+        if (any != 0.f) paged_wild<D>(a, row, sums + SUMS / 4u, 0u, plain_from, plain_to, tid);
     }
-    paged_finish<D, 1>(a, lds, t_end > t_begin, plain, row, q_first, record, 0u, 1u, tid);
+    __syncthreads();
+    if (wave < (uint32_t)TILES) {
+        // (32 columns to an instruction: the sixteen twice)
+        const uint32_t col = lane & (uint32_t)(HEADS - 1);
+        JoinedColumn j;
+        j.packed = packed ? sums + col * QROW : nullptr;
+        j.plain = plain ? sums + SUMS / 4u + col * QROW : nullptr;
+        j.m0 = packed ? stats[col] : MANY_NONE; j.l0 = packed ? stats[HEADS + col] : 0.f;
+        j.m1 = plain ? stats[2 * HEADS + col] : MANY_NONE; j.l1 = plain ? stats[3 * HEADS + col] : 0.f;
+        TQ_GLOBAL float *rec = record < 0 ? nullptr : (TQ_GLOBAL float *)a.rec + (size_t)record * a.qt * paged_record(a.cols, D);
+        paged_finish<D>(a, j, row, q_first, rec, col, col, (lane & 31u) < M && (lane & 31u) < (uint32_t)HEADS, wave, lane);
+    }
+    }
 }
 
 template <int D, int IPBK, int IPBV>

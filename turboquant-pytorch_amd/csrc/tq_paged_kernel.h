@@ -12,17 +12,22 @@ struct PagedRow {
     uint32_t fresh, total, packed, kv;
 };
 
-// Base-2 logit z after the cap and the bias by distance.  tanh y = (1 - e) / (1 + e) with e = 2^(-2 |y| log2 e), near zero by its series (the difference would leave few bits).
-__device__ __forceinline__ float shape_logit(const TqPagedArgs &a, float z, float slope, float back) {
-    if (a.cap != 0.f) {
-        const float unit = a.cap * LOG2E, y = z * (1.f / unit), y2 = y * y;
-        const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * fabsf(y));
-        const float large = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), y);
-        const float small = y * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-        z = unit * (fabsf(y) < 0.3f ? small : large);
+// Base-2 logits after the cap: C tanh(z / C) = C - 2 C / (1 + 2^(2 z / cap)), C = cap log2 e.  The difference leaves some 2^-23 C of a logit; where products are as exact as float32 (EXACT) small
+// ones come from the series.  (Five instructions, two of them at a quarter of the rate; with series and selection for all, a chunk of 512 tokens over 32768 took 637 us instead of 374 without a cap.)
+struct Cap {
+    float rate, c;
+    __device__ __forceinline__ explicit Cap(const TqPagedArgs &a) : rate(a.cap != 0.f ? 2.f / a.cap : 0.f), c(a.cap * LOG2E) {}
+    template <bool EXACT>
+    __device__ __forceinline__ float operator()(float z) const {
+        const float large = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * rate)), c);
+        if constexpr (!EXACT) return large;
+        else {
+            const float y = z / c, y2 = y * y;
+            const float small = z * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+            return fabsf(y) < 0.3f ? small : large;
+        }
     }
-    return fmaf(slope, back, z);
-}
+};
 
 // Tokens t0 ... t0 + 31 that a query at `pos` does not see, as bits
 __device__ __forceinline__ uint32_t unseen_bits(uint32_t t0, uint32_t pos, uint32_t window) {
@@ -246,6 +251,7 @@ __device__ __forceinline__ void paged_plain_phase(const TqPagedArgs &a, const Tq
         const uint32_t mine = share ? side : i, m = min((tile0 + mine) * 32u + n, v.M - 1u), token = m / a.group, pos = r.total - r.fresh + token;
         const uint8_t *q = many_query(v, 0u, m, ES);
         const float slope = a.slopes ? a.slopes[r.kv * a.group + (m - token * a.group)] * LOG2E : 0.f;
+        const Cap cap(a);
         float m_ref = MANY_NONE, l = 0.f;
         tq_f16v acc[NC];
 #pragma unroll
@@ -263,10 +269,20 @@ __device__ __forceinline__ void paged_plain_phase(const TqPagedArgs &a, const Tq
             const uint32_t valid = t.valid;
             float x[16];
 #pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = s[j] * (a.scale * LOG2E);
+            if (a.cap != 0.f) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = cap.template operator()<DT == TQ_F32>(x[j]);
+            }
+            if (a.slopes) {
+                const float first = (float)((int)(at + 4u * h) - (int)pos);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = fmaf(slope, first + (float)acc_row(j, 0u), x[j]);
+            }
+#pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const uint32_t row = acc_row(j, 0u);
-                const float z = a.cap != 0.f || a.slopes ? shape_logit(a, s[j] * (a.scale * LOG2E), slope, (float)((int)(at + row + 4u * h) - (int)pos)) : s[j] * (a.scale * LOG2E);
-                x[j] = row + 4u * h < valid && !((gone >> row) & 1u) ? z : MANY_NONE;
+                x[j] = row + 4u * h < valid && !((gone >> row) & 1u) ? x[j] : MANY_NONE;
             }
             float top = x[0];
 #pragma unroll
@@ -337,24 +353,29 @@ __device__ __forceinline__ void paged_store(const TqPagedArgs &a, uint32_t q_fir
     }
 }
 
-// Joined sums in LDS: packed ones turned back by Pi_v (two fp16 terms each), the plain ones added; divided by the sum of weights into the result, or as they are into the record.
-template <int DP, int QT>
-__device__ __forceinline__ void paged_finish(const TqPagedArgs &a, uint8_t *lds, bool packed, bool plain, const PagedRow &row, uint32_t q_first, int record, uint32_t tile0, uint32_t tiles,
-                                             uint32_t tid) {
-    constexpr int TILES = Shape<DP>::TILES, STEPS = DP / 16, CH = STEPS < 8 ? STEPS : 8;
-    using J = JoinArea<DP, QT>;
-    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, i = wave / TILES, w = wave % TILES;
-    if (i >= tiles) return;
-    const float *o = J::sums(lds, 0u, i) + n * (DP + 4u), *p = J::sums(lds, 1u, i) + n * (DP + 4u);
-    const float m0 = packed ? J::largest(lds, 0u, i)[n] : MANY_NONE, m1 = plain ? J::largest(lds, 1u, i)[n] : MANY_NONE, m = fmaxf(m0, m1);
-    const float l0 = packed ? J::total(lds, 0u, i)[n] : 0.f, l1 = plain ? J::total(lds, 1u, i)[n] : 0.f;
+// Joined sums of a column as they lie in LDS: packed tokens' (value space of the codec; null: none) and plain ones', their largest logits and sums of weights
+struct JoinedColumn {
+    const float *packed, *plain;
+    float m0, l0, m1, l1;
+};
+
+// A wave's 32 coordinates of 32 columns' results: packed sums turned back by Pi_v (two fp16 terms each), the plain ones added; divided by the sum of weights into the result of query vector q, or as they are into
+// column `col` of the record.  `some`: whether the lane's column is one.
+template <int DP>
+__device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedColumn &j, const PagedRow &row, uint32_t q_first, TQ_GLOBAL float *rec, uint32_t q, uint32_t col, bool some,
+                                             uint32_t w, uint32_t lane) {
+    constexpr int STEPS = DP / 16, CH = STEPS < 8 ? STEPS : 8;
+    const uint32_t h = lane >> 5;
+    const bool packed = j.packed != nullptr, plain = j.plain != nullptr;
+    const float m = fmaxf(j.m0, j.m1);
     // (no largest logit: no token seen, or logits that are all NaN, which the sum of weights tells)
-    const float f0 = m0 != MANY_NONE ? __builtin_amdgcn_exp2f(m0 - m) : l0 == 0.f ? 0.f : __builtin_nanf("");
-    const float f1 = m1 != MANY_NONE ? __builtin_amdgcn_exp2f(m1 - m) : l1 == 0.f ? 0.f : __builtin_nanf("");
-    const float l = l0 * f0 + l1 * f1, inv = l == 0.f ? 0.f : 1.0f / l;
+    const float f0 = j.m0 != MANY_NONE ? __builtin_amdgcn_exp2f(j.m0 - m) : j.l0 == 0.f ? 0.f : __builtin_nanf("");
+    const float f1 = j.m1 != MANY_NONE ? __builtin_amdgcn_exp2f(j.m1 - m) : j.l1 == 0.f ? 0.f : __builtin_nanf("");
+    const float l = j.l0 * f0 + j.l1 * f1, inv = l == 0.f ? 0.f : 1.0f / l;
     tq_f16v acc = tq_zero16();
     float back = 0.f;
     if (packed) {
+        const float *o = j.packed;
         const uint8_t *pi = a.table_v + TQ_OFF_AT_F16(DP) + ((size_t)w * STEPS * 64u + lane) * 16u;
         float largest = 0.f;
 #pragma unroll 8
@@ -373,9 +394,9 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, uint8_t *lds,
             for (int s = 0; s < CH; ++s) { ph[s] = tq_gload16(pi + (size_t)(s0 + s) * 1024u); pl[s] = tq_gload16(pi + TQ_OPERAND_BYTES_FOR(DP) + (size_t)(s0 + s) * 1024u); }
 #pragma unroll
             for (int s = 0; s < CH; ++s) {
-                const uint32_t j = DP == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
-                tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + j), y = *reinterpret_cast<const tq_f4 *>(o + j + 4u);
-                if (!Shape<DP>::EVEN && j >= a.D) x = y = tq_f4{0.f, 0.f, 0.f, 0.f};        // (D a multiple of 8; what lies past it may be anything)
+                const uint32_t i = DP == TQ_HEAD_DIM ? 64u * h + 8u * (s0 + s) : 16u * (s0 + s) + 8u * h;       // (128 wide the table's operands have an order of their own, see tq_table.h)
+                tq_f4 x = *reinterpret_cast<const tq_f4 *>(o + i), y = *reinterpret_cast<const tq_f4 *>(o + i + 4u);
+                if (!Shape<DP>::EVEN && i >= a.D) x = y = tq_f4{0.f, 0.f, 0.f, 0.f};        // (D a multiple of 8; what lies past it may be anything)
                 tq_u4 oh, ol;
                 fp16_split8(x, y, f, oh, ol);
                 acc = mfma_f16(ph[s], oh, acc);
@@ -385,22 +406,20 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, uint8_t *lds,
         }
         back = __uint_as_float((uint32_t)(127 - up) << 23) * f0;
     }
-    const uint32_t q = (tile0 + i) * 32u + n, d0 = DP == TQ_HEAD_DIM ? 64u * h + 16u * w : 32u * w + 16u * h;
+    if (!some) return;
+    const uint32_t d0 = DP == TQ_HEAD_DIM ? 64u * h + 16u * w : 32u * w + 16u * h;
     float out[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) out[r] = (packed ? acc[r] * back : 0.f) + (plain ? p[d0 + r] * f1 : 0.f);
-    if (record < 0) {
-        if (q >= row.fresh * a.group) return;
+    for (int r = 0; r < 16; ++r) out[r] = (packed ? acc[r] * back : 0.f) + (plain ? j.plain[d0 + r] * f1 : 0.f);
+    if (!rec) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[r] = inv == 0.f ? 0.f : out[r] * inv;
         paged_store(a, q_first, row.kv, q, d0, out);
         return;
     }
-    if (n >= a.cols) return;
-    TQ_GLOBAL float *rec = (TQ_GLOBAL float *)a.rec + (((size_t)record * a.heads + row.kv) * a.qt + i) * paged_record(a.cols, DP);
-    if (w == 0u && h == 0u) { rec[n] = m; rec[a.cols + n] = l; }
+    if (w == 0u && h == 0u) { rec[col] = m; rec[a.cols + col] = l; }
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(rec + 2u * a.cols + n * DP + d0 + r) = tq_f4{out[r], out[r + 1], out[r + 2], out[r + 3]};
+    for (int r = 0; r < 16; r += 4) *reinterpret_cast<TQ_GLOBAL tq_f4 *>(rec + 2u * a.cols + col * DP + d0 + r) = tq_f4{out[r], out[r + 1], out[r + 2], out[r + 3]};
 }
 
 // Block = (item of the plan, kv head): QT tiles of 32 queries of a sequence against a share of what they see, packed tokens first, then plain ones.  The loop over packed tokens is the one of
@@ -551,6 +570,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
             for (int c = 0; c < NC; ++c) acc[i][c] = tq_zero16();
         }
         const bool shaped = a.cap != 0.f || a.slopes;
+        const Cap cap(a);
         // runs that begin before this are not seen whole by the last query of the block
         const uint32_t last_pos = row.total - row.fresh + min((tile0 + QT) * 32u - 1u, v.M - 1u) / a.group;
         const uint32_t whole_from = a.window && last_pos >= a.window ? last_pos - a.window + 1u : 0u;
@@ -650,10 +670,23 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
                     for (int i = 0; i < QT; ++i) {
                         float logit = s[i][r] * own[i] * kn[r];
                         asm volatile("" : "+v"(logit));
-                        if (shaped) logit = shape_logit(a, logit, slope[i], (float)((int)(t0 + acc_row(r, h)) - (int)pos[i]));
                         s[i][r] = logit;
                     }
                     kn[r] = 1.f;
+                }
+                if (a.cap != 0.f) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) s[i][r] = cap.template operator()<VT == 2>(s[i][r]);
+                }
+                if (a.slopes) {
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        const float first = (float)((int)(t0 + 4u * h) - (int)pos[i]);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = fmaf(slope[i], first + (float)acc_row(r, 0u), s[i][r]);
+                    }
                 }
             }
 #pragma unroll
@@ -770,7 +803,17 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
         else if (a.dtype == TQ_BF16) paged_plain_phase<DP, QT, TQ_BF16>(a, v, row, lds, lds_m, lds_l, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
         else if constexpr (KT == 2) paged_plain_phase<DP, QT, TQ_F16>(a, v, row, lds, lds_m, lds_l, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
     }
-    paged_finish<DP, QT>(a, lds, end > begin, plain, row, q_first, record, tile0, tiles, tid);
+    const uint32_t i = wave / S::TILES;
+    if (i >= tiles) return;
+    const bool packed = end > begin;
+    JoinedColumn j;
+    j.packed = packed ? J::sums(lds, 0u, i) + n * (DP + 4u) : nullptr;
+    j.plain = plain ? J::sums(lds, 1u, i) + n * (DP + 4u) : nullptr;
+    j.m0 = packed ? J::largest(lds, 0u, i)[n] : MANY_NONE; j.l0 = packed ? J::total(lds, 0u, i)[n] : 0.f;
+    j.m1 = plain ? J::largest(lds, 1u, i)[n] : MANY_NONE; j.l1 = plain ? J::total(lds, 1u, i)[n] : 0.f;
+    const uint32_t q = (tile0 + i) * 32u + n;
+    TQ_GLOBAL float *rec = record < 0 ? nullptr : (TQ_GLOBAL float *)a.rec + (((size_t)record + row.kv) * a.qt + i) * paged_record(a.cols, DP);
+    paged_finish<DP>(a, j, row, q_first, rec, q, n, record < 0 ? q < v.M : n < a.cols, wave % S::TILES, lane);
 }
 
 template <int DP, int IPBK, int IPBV>

@@ -472,11 +472,12 @@ class PagedStep:
             with _native._on(c.device):
                 rc = call(items, merges)
                 if rc == _native.ERR_CAPACITY:
-                    items, merges = np.empty((counts.items, _native.PAGED_ITEM), np.int32), np.empty((max(1, counts.merges), _native.PAGED_MERGE), np.int32)
+                    items = np.empty((counts.items + counts.blocks // _native.PAGED_ITEM + 1, _native.PAGED_ITEM), np.int32)
+                    merges = np.empty((max(1, counts.merges), _native.PAGED_MERGE), np.int32)
                     rc = call(items, merges)
             _native.check(rc, "tq_paged_plan")
             floats = int(_native.lib().tq_paged_scratch(ctypes.byref(counts), c.kv_heads, c.head_dim))
-            uploaded, (items_at, merges_at) = self._upload([items[:counts.items].ravel(), merges[:counts.merges].ravel()])
+            uploaded, (items_at, merges_at) = self._upload([items.ravel()[:counts.items * _native.PAGED_ITEM + (counts.blocks + 1 if counts.few else 0)], merges[:counts.merges].ravel()])
             plan = self._plans[key] = (counts, items_at, merges_at, floats, uploaded)
         return plan
 
