@@ -14,9 +14,10 @@ struct FewPlain {
     static constexpr bool HELD = D <= 128;
     static constexpr int VW = HELD ? NC / 2 : 4;         // words of a lane's coordinates that are held at a time
     static constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
-    tq_u4 k[SK][2];
+    static constexpr int KH = HELD ? SK : 1, CH = HELD ? SK : 2;      // 256 wide keys do not fit beside the sums: two steps at a time
+    tq_u4 k[KH][2];
     uint32_t v[8][VW];
-    const uint8_t *vw;
+    const uint8_t *kw, *vw;
     uint32_t valid;
     static __device__ __forceinline__ uint32_t token(int j, uint32_t q4) { return 16u * (j / 4) + 4u * q4 + (uint32_t)(j % 4); }
     // N coordinates from c0 on, into words w0 ...
@@ -33,20 +34,34 @@ struct FewPlain {
     // keys, values: of the head's first of the 32 tokens (the page holds all of them; those from `valid` on are not used)
     __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint32_t valid_, uint32_t lane) {
         valid = valid_;
+        kw = keys + (lane & 15u) * (2u * D) + 16u * (lane >> 4);
         vw = values;
+        if constexpr (HELD) {
 #pragma unroll
-        for (int s = 0; s < SK; ++s)
+            for (int s = 0; s < SK; ++s)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) k[s][b] = tq_gload16(keys + (16u * b + (lane & 15u)) * (2u * D) + 64 * s + 16u * (lane >> 4));
+                for (int b = 0; b < 2; ++b) k[s][b] = tq_gload16(kw + b * (32u * D) + 64 * s);
+        }
         if constexpr (D == 64 || D == 128) load_columns<NC>(lane, 0, 0);
         else if constexpr (D == 96) { load_columns<4>(lane, 0, 0); load_columns<2>(lane, 4, 2); }
     }
-    __device__ __forceinline__ void scores(const tq_u4 (&q)[SK], float (&x)[8]) const {
+    // q: this lane's column's vector, from element 8 q4 on
+    __device__ __forceinline__ void scores(const uint8_t *q, float (&x)[8]) const {
         tq_f4v sc[2] = {tq_f4v{0.f, 0.f, 0.f, 0.f}, tq_f4v{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 1
+        for (int s0 = 0; s0 < SK; s0 += CH) {
+            tq_u4 y[CH], z[CH][2];
 #pragma unroll
-        for (int s = 0; s < SK; ++s)
+            for (int s = 0; s < CH; ++s) {
+                y[s] = tq_gload16(q + 64 * (s0 + s));
 #pragma unroll
-            for (int b = 0; b < 2; ++b) sc[b] = BF ? mfma16_bf16(k[s][b], q[s], sc[b]) : mfma16_f16(k[s][b], q[s], sc[b]);
+                for (int b = 0; b < 2; ++b) z[s][b] = HELD ? k[HELD ? s : 0][b] : tq_gload16(kw + b * (32u * D) + 64 * (s0 + s));
+            }
+#pragma unroll
+            for (int s = 0; s < CH; ++s)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) sc[b] = BF ? mfma16_bf16(z[s][b], y[s], sc[b]) : mfma16_f16(z[s][b], y[s], sc[b]);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = sc[j / 4][j % 4];
     }
@@ -95,6 +110,7 @@ struct FewPlain {
                 tame(lane, wild);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) column(c0 + c, c / 2);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -117,9 +133,11 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     constexpr int P_SHIFT = 14 - 8;
     constexpr int HR = D == 256 && C == 1 ? 4 : HEADS < 8 ? HEADS : 8;            // columns a round of the join
     constexpr int QROW = D + 4;
-    // LDS: tables; then values of each wave and rotated queries, later the waves' sums and the joined ones (packed tokens', plain ones')
-    constexpr uint32_t V_AT = 65536u, Q_AT = V_AT + DW * VBYTES, LOOP_END = Q_AT + 16u * QROW * 4u;
-    constexpr uint32_t JOIN_AT = V_AT, SUMS_AT = JOIN_AT + DW * HR * PART * 4u, SUMS = HEADS * QROW * 4u, STATS_AT = SUMS_AT + 2u * SUMS, JOIN_END = STATS_AT + 4u * HEADS * 4u;
+    // LDS: tables; values of each wave, rotated queries; the waves' sums of packed tokens and of plain ones, and the joined ones.  Where that is more than there is, the waves' sums lie over values and
+    // queries, take turns, and cost barriers.
+    constexpr uint32_t V_AT = 65536u, Q_AT = V_AT + DW * VBYTES, LOOP_END = Q_AT + 16u * QROW * 4u, JOIN = DW * HR * PART * 4u, SUMS = HEADS * QROW * 4u, STATS = 4u * HEADS * 4u;
+    constexpr bool SIDE = HR >= HEADS && LOOP_END + 2u * JOIN + 2u * SUMS + STATS + DW * RUN * 6u + (QT > QREG ? (QT - QREG) * SK * 1024u : 0u) + 1024u <= 163840u;
+    constexpr uint32_t JOIN_AT = SIDE ? LOOP_END : V_AT, SUMS_AT = JOIN_AT + (SIDE ? 2u : 1u) * JOIN, STATS_AT = SUMS_AT + 2u * SUMS, JOIN_END = STATS_AT + STATS;
     constexpr uint32_t AREA = LOOP_END > JOIN_END ? LOOP_END : JOIN_END;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
     __shared__ __attribute__((aligned(16))) float lds_kn[DW][RUN];
@@ -127,6 +145,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     __shared__ __attribute__((aligned(16))) tq_u4 lds_q[QT > QREG ? (QT - QREG) * SK : 1][TQ_WAVE];
     __shared__ __attribute__((aligned(16))) float lds_corr[DW][16];
     __shared__ uint32_t lds_trips[DW];
+    __shared__ float lds_wild[DW];
 
     {
         const uint32_t tid = threadIdx.x;
@@ -137,9 +156,12 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         table_v.load(a.table_v + TQ_OFF_LUT(D), tid);
         table_k.store(lds, tid);
         table_v.store(lds + 128, tid);
+        if (tid < (uint32_t)DW) lds_trips[tid] = 0u;
     }
+    const int32_t first_item = a.blocks[blockIdx.x], end_item = a.blocks[blockIdx.x + 1];
+    uint32_t trips = 0u;
 #pragma unroll 1
-    for (int32_t index = a.blocks[blockIdx.x]; index < a.blocks[blockIdx.x + 1]; ++index) {
+    for (int32_t index = first_item; index < end_item; ++index) {
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));        // (what lanes make of their number is made anew for every item: kept from one to the next it took a hundred registers that there are not)
     const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n16 = lane & 15u, q4 = lane >> 4, head = n16 % HEADS, cls = n16 / HEADS;
@@ -160,65 +182,89 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     const float slope = a.slopes ? a.slopes[row.kv * a.group + (vector - token * a.group)] * LOG2E : 0.f;
     float *const sums = reinterpret_cast<float *>(lds + SUMS_AT), *const stats = reinterpret_cast<float *>(lds + STATS_AT);       // [packed, plain][HEADS][QROW]; [largest, total][HEADS] of each
 
-    // The waves' sums of HR columns at a time meet in LDS (which: 0 packed, 1 plain); unit: what this wave's value sums are multiplied by, l: all lanes' of a column
-    auto join = [&](uint32_t which, float m_ref, float l, float unit, const tq_f4v (&acc)[NC]) __attribute__((always_inline)) {
-        float *const mine = reinterpret_cast<float *>(lds + JOIN_AT) + wave * (HR * PART);
-        for (uint32_t h0 = 0; h0 < (uint32_t)HEADS && h0 < M; h0 += HR) {
-            __syncthreads();         // (values, queries, and the round before)
-            if (q4 == 0u && n16 < (uint32_t)HEADS && n16 >= h0 && n16 < h0 + HR) {
-                mine[(n16 - h0) * PART] = m_ref;
-                mine[(n16 - h0) * PART + 1u] = l;
+    // The waves' sums meet in LDS, HR columns from h0 on (which: 0 packed, 1 plain).  put(): unit: what this wave's value sums are multiplied by, l: all lanes' of a column
+    auto put = [&](uint32_t which, uint32_t h0, float m_ref, float l, float unit, const tq_f4v (&acc)[NC]) __attribute__((always_inline)) {
+        float *const mine = reinterpret_cast<float *>(lds + JOIN_AT + (SIDE ? which * JOIN : 0u)) + wave * (HR * PART);
+        if (q4 == 0u && n16 < (uint32_t)HEADS && n16 >= h0 && n16 < h0 + HR) {
+            mine[(n16 - h0) * PART] = m_ref;
+            mine[(n16 - h0) * PART + 1u] = l;
+        }
+        if (C == 1 || which) {
+            if (4u * q4 >= h0 && 4u * q4 < min(h0 + HR, (uint32_t)HEADS)) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mine[(4u * q4 + r - h0) * PART + 2u + value_coord<D>(n16, c)] = acc[c][r] * unit;
             }
-            if (C == 1 || which) {
-                if (4u * q4 >= h0 && 4u * q4 < min(h0 + HR, (uint32_t)HEADS)) {
+        } else {
+            // The blocks of tokens lie in lanes 32 apart (C = 4: and 16 apart): two registers exchange halves and are added, which leaves the sum of one in each half (then quarters).
+            static_assert(C == 1 || HR >= HEADS, "one round");
 #pragma unroll
-                    for (int c = 0; c < NC; ++c)
+            for (int r = 0; r < 4; ++r) {
+                float half[NC / 2];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) mine[(4u * q4 + r - h0) * PART + 2u + value_coord<D>(n16, c)] = acc[c][r] * unit;
-                }
-            } else {
-                // The blocks of tokens lie in lanes 32 apart (C = 4: and 16 apart): two registers exchange halves and are added, which leaves the sum of one in each half (then quarters).
-                static_assert(C == 1 || HR >= HEADS, "one round");
+                for (int c = 0; c < NC; c += 2) half[c / 2] = fold<32>(acc[c][r], acc[c + 1][r]);
+                if constexpr (C == 2) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float half[NC / 2];
+                    for (int c = 0; c < NC; c += 2) mine[(4u * (q4 & 1u) + r) * PART + 2u + value_coord<D>(n16, c + (int)(q4 >> 1))] = half[c / 2] * unit;
+                } else {
 #pragma unroll
-                    for (int c = 0; c < NC; c += 2) half[c / 2] = fold<32>(acc[c][r], acc[c + 1][r]);
-                    if constexpr (C == 2) {
-#pragma unroll
-                        for (int c = 0; c < NC; c += 2) mine[(4u * (q4 & 1u) + r) * PART + 2u + value_coord<D>(n16, c + (int)(q4 >> 1))] = half[c / 2] * unit;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < NC; c += 4) {
-                            const bool pair = c + 2 < NC;     // (96: the last two columns stand alone, both quarters hold them)
-                            const float sum = fold<16>(half[c / 2], half[pair ? c / 2 + 1 : c / 2]);
-                            mine[r * PART + 2u + value_coord<D>(n16, c + (int)((pair ? 2u * (q4 & 1u) : 0u) + (q4 >> 1)))] = sum * unit;
-                        }
+                    for (int c = 0; c < NC; c += 4) {
+                        const bool pair = c + 2 < NC;     // (96: the last two columns stand alone, both quarters hold them)
+                        const float sum = fold<16>(half[c / 2], half[pair ? c / 2 + 1 : c / 2]);
+                        mine[r * PART + 2u + value_coord<D>(n16, c + (int)((pair ? 2u * (q4 & 1u) : 0u) + (q4 >> 1)))] = sum * unit;
                     }
-                }
-            }
-            __syncthreads();
-            const float *all = reinterpret_cast<const float *>(lds + JOIN_AT);
-            for (uint32_t i = tid; i < HR * D; i += DTHREADS) {
-                const uint32_t col = i / D, d = i - col * D;
-                float m = MANY_NONE, sum = 0.f, total = 0.f;
-#pragma unroll
-                for (int w = 0; w < DW; ++w) m = fmaxf(m, all[(w * HR + col) * PART]);
-#pragma unroll
-                for (int w = 0; w < DW; ++w) {
-                    const float own = all[(w * HR + col) * PART], lw = all[(w * HR + col) * PART + 1u];
-                    const float f = own != MANY_NONE ? __builtin_amdgcn_exp2f(own - m) : lw == 0.f ? 0.f : __builtin_nanf("");
-                    sum = fmaf(all[(w * HR + col) * PART + 2u + d], f, sum);
-                    total = fmaf(lw, f, total);
-                }
-                sums[which * (SUMS / 4u) + (h0 + col) * QROW + d] = sum;
-                if (d == 0u) {
-                    stats[(2u * which) * HEADS + h0 + col] = m;
-                    stats[(2u * which + 1u) * HEADS + h0 + col] = total;
                 }
             }
         }
     };
+    // of the first `waves`
+    auto combine = [&](uint32_t which, uint32_t h0, uint32_t waves) __attribute__((always_inline)) {
+        const float *all = reinterpret_cast<const float *>(lds + JOIN_AT + (SIDE ? which * JOIN : 0u));
+        for (uint32_t i = tid; i < min((uint32_t)HR, M - h0) * D; i += DTHREADS) {
+            const uint32_t col = i / D, d = i - col * D;
+            float m = MANY_NONE, sum = 0.f, total = 0.f;
+#pragma unroll
+            for (uint32_t w = 0; w < DW; ++w) m = w < waves ? fmaxf(m, all[(w * HR + col) * PART]) : m;
+#pragma unroll
+            for (uint32_t w = 0; w < DW; ++w) {
+                if (w >= waves) continue;
+                const float own = all[(w * HR + col) * PART], lw = all[(w * HR + col) * PART + 1u];
+                const float f = own != MANY_NONE ? __builtin_amdgcn_exp2f(own - m) : lw == 0.f ? 0.f : __builtin_nanf("");
+                sum = fmaf(all[(w * HR + col) * PART + 2u + d], f, sum);
+                total = fmaf(lw, f, total);
+            }
+            sums[which * (SUMS / 4u) + (h0 + col) * QROW + d] = sum;
+            if (d == 0u) {
+                stats[(2u * which) * HEADS + h0 + col] = m;
+                stats[(2u * which + 1u) * HEADS + h0 + col] = total;
+            }
+        }
+    };
+    // where there is no room for both sides
+    auto join = [&](uint32_t which, float m_ref, float l, float unit, const tq_f4v (&acc)[NC]) __attribute__((always_inline)) {
+        for (uint32_t h0 = 0; h0 < (uint32_t)HEADS && h0 < M; h0 += HR) {
+            __syncthreads();         // (values, queries, and the round before)
+            put(which, h0, m_ref, l, unit, acc);
+            __syncthreads();
+            combine(which, h0, DW);
+        }
+    };
+    // Queries into the codec's space, of as many items as the columns hold (SIDE: what lies there has been read before the barrier that stood last)
+    if ((index - first_item) % C == 0) {
+        if (!SIDE) __syncthreads();
+        if (wave < (uint32_t)TILES) {
+            const int32_t *mine = a.items + (size_t)min(index + (int32_t)cls, end_item - 1) * PAGED_ITEM, *of = a.seqs + (size_t)mine[0] * PAGED_SEQ;
+            const uint32_t m = min(head, (uint32_t)of[1] * a.group - 1u), t = m / a.group;
+            Rotation<D, BF> r;
+            r.qsrc = a.q + ((long long)((uint32_t)of[0] + t) * a.q_token + (long long)((uint32_t)mine[7] * a.group + (m - t * a.group)) * a.q_head) * 2 + 16u * q4;
+            r.asrc = a.table_k + (BF ? TQ_OFF_A_BF16(D) : TQ_OFF_A_F16) + ((size_t)wave * (D / 16 * 64u) + q4 * 32u + n16) * 16u;
+            r.fetch(0);
+            r.finish(reinterpret_cast<float *>(lds + Q_AT), QROW, a.scale, wave, lane);
+        }
+        __syncthreads();
+    }
+    const uint32_t q_row = (uint32_t)((index - first_item) % C) * HEADS + head;
 
     if (t_end > t_begin) {
         const uint32_t lo = a.window && pos >= a.window ? pos - a.window + 1u : 0u;              // first token that this lane's column sees
@@ -288,26 +334,11 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             kn_raw = tq_gload2(reinterpret_cast<const uint16_t *>(base + a.k_norms) + own);
             vn_raw = tq_gload2(reinterpret_cast<const uint16_t *>(base + a.v_norms) + own);
         };
-        // ---- start: the operands of the query rotation (the first waves), then the first run
+        // ---- start: the first run's loads
         Where now = where(0u), next = where(1u);
-        auto first_run = [&]() __attribute__((always_inline)) {
-            __builtin_amdgcn_sched_barrier(0);
-            issue_keys(now, max(run_tokens(0u), 1u));
-            issue_values(now, max(run_tokens(0u), 1u));
-            __builtin_amdgcn_sched_barrier(0);
-            __syncthreads();         // (what the item before has left in LDS is read)
-            if (tid < (uint32_t)DW) lds_trips[tid] = 0u;
-        };
-        if (wave < (uint32_t)TILES) {
-            Rotation<D, BF> r;
-            const uint32_t m = n16 < M ? n16 : 0u, t = m / a.group;
-            r.qsrc = queries + ((long long)t * a.q_token + (long long)(m - t * a.group) * a.q_head) * 2 + 16u * q4;
-            r.asrc = a.table_k + (BF ? TQ_OFF_A_BF16(D) : TQ_OFF_A_F16) + ((size_t)wave * (D / 16 * 64u) + q4 * 32u + n16) * 16u;
-            r.fetch(0);
-            first_run();
-            r.finish(reinterpret_cast<float *>(lds + Q_AT), QROW, a.scale, wave, lane);
-        } else first_run();
-        __syncthreads();
+        issue_keys(now, max(run_tokens(0u), 1u));
+        issue_values(now, max(run_tokens(0u), 1u));
+        __builtin_amdgcn_sched_barrier(0);
 
         // ---- B operand of the score product: fp16 of q * 2^(10 - e), e = binary exponent of the column's largest magnitude
         tq_u4 qb[QREG][SK];
@@ -504,7 +535,6 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             }
         };
         // one trip: stage the run that has been loaded, start the loads of the next one, compute.  The two waves of a SIMD are kept level (see tq_decode_kernel).
-        uint32_t trips = 0u;
         auto trip = [&](auto full_tag, uint32_t i) __attribute__((always_inline)) {
             ++trips;
             volatile __attribute__((address_space(3))) uint32_t *begun = (__attribute__((address_space(3))) uint32_t *)lds_trips;
@@ -556,19 +586,20 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             // Whole runs in a loop of their own; those that the window's edge crosses and the partial one (a wave has one at most) by the careful form.
             uint32_t i = 0u;
 #pragma unroll 1
-            for (;;) {
+            while (run_tokens(i) && run_start(i) < whole_from) trip(std::false_type{}, i++);
 #pragma unroll 1
-                while (run_tokens(i) == (uint32_t)RUN && run_start(i) >= whole_from) trip(std::true_type{}, i++);
-                if (!run_tokens(i)) break;
-                trip(std::false_type{}, i++);
-            }
+            while (run_tokens(i) == (uint32_t)RUN) trip(std::true_type{}, i++);
+            if (run_tokens(i)) trip(std::false_type{}, i);
             if (lane == 0u) *(volatile __attribute__((address_space(3))) uint32_t *)&lds_trips[wave] = 0xffffffffu;
             __builtin_amdgcn_s_setprio(0);
         }
         float l_all = l_run;
 #pragma unroll
         for (int d = HEADS; d < 64; d <<= 1) l_all += __shfl_xor(l_all, d);
-        join(0u, m_ref, l_all * (1.0f / (float)(1 << P_SHIFT)), ldexpf(1.f, ev_ref - P_SHIFT), acc);
+        l_all *= 1.0f / (float)(1 << P_SHIFT);
+        const float unit = ldexpf(1.f, ev_ref - P_SHIFT);
+        if constexpr (SIDE) put(0u, 0u, m_ref, l_all, unit, acc);
+        else join(0u, m_ref, l_all, unit, acc);
     }
     const bool packed = t_end > t_begin, plain = plain_to > plain_from;
     if (plain) {
@@ -582,16 +613,13 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         float m_ref = MANY_NONE, l = 0.f;
         bool wild = false;
 #pragma unroll 1
-        for (uint32_t w = wave; w < runs; w += DW) {
+        for (uint32_t w = DW - 1u - wave; w < runs; w += DW) {
             const uint32_t t0 = plain_from + 32u * w;
             const uint8_t *page = a.plain + (long long)(int)tq_uniform32((uint32_t)row.plain_pages[t0 >> a.shift]) * a.plain_stride + (size_t)((row.kv << a.shift) + (t0 & ((1u << a.shift) - 1u))) * (2u * D);
             FewPlain<D, BF> t;
-            tq_u4 q[SK];
-#pragma unroll
-            for (int s = 0; s < SK; ++s) q[s] = tq_gload16(cq + 64 * s + 16u * q4);
             t.load(page, page + a.plain_v, min(32u, plain_to - t0), lane);
             float x[8];
-            t.scores(q, x);
+            t.scores(cq + 16u * q4, x);
             const uint32_t at = row.packed + t0, gone = unseen_bits(at, cpos, a.window);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= a.scale * LOG2E;
@@ -616,7 +644,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
                 x[j] = x[j] == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(x[j] - top);
                 l += x[j];               // (this lane's tokens)
             }
-            if (w != wave) {             // (sums so far: a lane has those of columns 4 q4 ...)
+            if (w >= DW) {             // (sums so far: a lane has those of columns 4 q4 ...)
                 float4 c4;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) (&c4.x)[r] = __shfl(shrink, (int)(4u * q4 + r));
@@ -627,13 +655,23 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         }
         l = reduce_rows(l, OpAdd());
         wild = __any(wild);
-        join(1u, m_ref, l, 1.f, acc);
-        if (lane == 0u) lds_corr[wave][0] = wild ? 1.f : 0.f;
-        __syncthreads();
+        if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
+        if constexpr (SIDE) put(1u, 0u, m_ref, l, 1.f, acc);
+        else join(1u, m_ref, l, 1.f, acc);
+    }
+    __syncthreads();
+    if constexpr (SIDE) {
+        if (packed) combine(0u, 0u, DW);
+        if (plain) combine(1u, 0u, DW);
+    }
+    if (plain) {
         float any = 0.f;
 #pragma unroll
-        for (int w = 0; w < DW; ++w) any += lds_corr[w][0];
-        if (any != 0.f) paged_wild<D>(a, row, sums + SUMS / 4u, 0u, plain_from, plain_to, tid);
+        for (int w = 0; w < DW; ++w) any += lds_wild[w];
+        if (any != 0.f) {
+            __syncthreads();
+            paged_wild<D>(a, row, sums + SUMS / 4u, 0u, plain_from, plain_to, tid);
+        }
     }
     __syncthreads();
     if (wave < (uint32_t)TILES) {
