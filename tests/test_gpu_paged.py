@@ -172,6 +172,20 @@ def test_splits_of_long_rows_meet(pkg):
             check(step.attend(q, 0, **kw), q, step, **kw)
 
 
+@pytest.mark.parametrize("D,H,G,dtype,kb,vb,n,new", [
+    (128, 8, 4, BF, 4, 2, 170, 1), (128, 8, 1, BF, 4, 2, 170, 1), (128, 4, 4, BF, 4, 2, 170, 2), (128, 8, 4, F16, 6, 4, 100, 4), (64, 8, 4, F16, 6, 4, 170, 1), (64, 8, 8, BF, 8, 8, 100, 1),
+    (96, 8, 2, BF, 4, 2, 170, 1), (96, 8, 16, F16, 3, 2, 70, 1), (256, 8, 4, BF, 4, 2, 100, 1), (256, 8, 8, BF, 4, 2, 100, 1), (256, 8, 16, F16, 8, 8, 70, 1), (80, 8, 4, BF, 4, 2, 100, 1)])
+def test_more_rows_than_the_device_takes_at_a_time(pkg, D, H, G, dtype, kb, vb, n, new):
+    lengths = [(0, 700, 64, 129, 1, 320, 63)[i % 7] + 3 * (i // 7) for i in range(n)]
+    cache = make(pkg, D, H, dtype, kb, vb, 20, pages=16 * n, plain=16 * n)
+    seqs = cache.add(n)
+    feed(cache, seqs, lengths, seed=1)
+    step = feed(cache, seqs, [new] * n, seed=2, commit=False)
+    q = rand((n * new, H * G, D), 3, dtype)
+    check(step.attend(q, 0), q, step)
+    check(step.attend(q, 0, sliding_window=90), q, step, sliding_window=90)
+
+
 def test_scale_and_layouts_of_queries(pkg):
     cache = make(pkg, H=2, layers=2, protected_layers=1)            # (8 bits in both)
     seqs = cache.add(2)

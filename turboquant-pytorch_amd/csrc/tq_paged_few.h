@@ -250,8 +250,8 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             combine(which, h0, DW);
         }
     };
-    // Queries into the codec's space, of as many items as the columns hold (SIDE: what lies there has been read before the barrier that stood last)
-    if ((index - first_item) % C == 0) {
+    // Queries into the codec's space, of as many items as the columns hold (SIDE: what lies there has been read before the barrier that stood last; else the sums have been written over it)
+    if (!SIDE || (index - first_item) % C == 0) {
         if (!SIDE) __syncthreads();
         if (wave < (uint32_t)TILES) {
             const int32_t *mine = a.items + (size_t)min(index + (int32_t)cls, end_item - 1) * PAGED_ITEM, *of = a.seqs + (size_t)mine[0] * PAGED_SEQ;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         }
         __syncthreads();
     }
-    const uint32_t q_row = (uint32_t)((index - first_item) % C) * HEADS + head;
+    const uint32_t q_row = (SIDE ? (uint32_t)((index - first_item) % C) * HEADS : 0u) + head;
 
     if (t_end > t_begin) {
         const uint32_t lo = a.window && pos >= a.window ? pos - a.window + 1u : 0u;              // first token that this lane's column sees
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         tq_u4 qb[QREG][SK];
         float c1;                // base-2 logit = accumulator * key norm * c1
         {
-            const float *q = reinterpret_cast<const float *>(lds + Q_AT) + head * QROW + (D / 4) * q4;
+            const float *q = reinterpret_cast<const float *>(lds + Q_AT) + q_row * QROW + (D / 4) * q4;
             float x[D / 4];
 #pragma unroll
             for (int i = 0; i < D / 4; i += 4) {
