@@ -23,7 +23,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libtqamd.so")
 FAST_NAME = "tqamd_fastcall"        # extension module: the eager calls from tensors to the library in one step each
 FAST_SOURCE = "tq_fastcall.cpp"
-FAST_INTERFACE = 7                  # INTERFACE there: what init and the functions take and answer
+FAST_INTERFACE = 8                  # INTERFACE there: what init and the functions take and answer
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
@@ -365,7 +365,7 @@ def fast():
         if getattr(module, "interface", None) != FAST_INTERFACE:       # (modules of before had none)
             raise TqError(f"{path} was built from another state of {FAST_SOURCE}: {how}")
         entries = ("tq_compress", "tq_decompress", "tq_compress_layer", "tq_restore_layer", "tq_decode_append", "tq_decode_attend_cached", "tq_qjl_compress", "tq_qjl_query_scores",
-                   "tq_attend_many_scratch", "tq_attend_many", "tq_evict", "tq_evict_scratch", "tq_beam_scratch", "tq_beam_select", "tq_reorder", "tq_paged_attend")
+                   "tq_attend_many_scratch", "tq_attend_many", "tq_evict", "tq_evict_scratch", "tq_beam_scratch", "tq_beam_select", "tq_reorder", "tq_paged_attend", "tq_copy_pages")
         module.init(tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in entries), _workspace, _drop_workspace, _step_scratch, _arrived, _TABLE_TAG)
         _fast = module
     return _fast
@@ -960,6 +960,19 @@ def reorder(segments, parents: torch.Tensor, heads: int, device: torch.device) -
     runs = (TqMoveSegment * len(segments))(*segments)
     with _on(device):
         check(lib().tq_reorder(runs, len(segments), parents.shape[0], heads, parents.data_ptr(), _stream_handle(device)), "tq_reorder")
+
+
+def copy_pages(source: torch.Tensor, target: torch.Tensor, rows: int, row_bytes: int, sources, targets=None, sizes=None) -> None:
+    """tq_copy_pages: pages `sources` of one pool ([pages, ...]) into pages `targets` (default 0, 1, ...) of another, or of the same one; sizes: bytes of each row that are copied (default all)."""
+    status = fast().copy_pages(source, target, rows, row_bytes, sources, targets, sizes)
+    if status is None:          # (another device is current)
+        n = len(sources)
+        pairs = np.empty((n, 3), dtype=np.int32)
+        pairs[:, 0], pairs[:, 1], pairs[:, 2] = sources, np.arange(n) if targets is None else targets, row_bytes if sizes is None else sizes
+        stride = lambda t: t.stride(0) * t.element_size()  # noqa: E731
+        with _on(source.device):
+            status = lib().tq_copy_pages(source.data_ptr(), stride(source), target.data_ptr(), stride(target), rows, row_bytes, pairs.ctypes.data, n, _stream_handle(source.device))
+    check(status, "tq_copy_pages")
 
 
 def compress_into(states: torch.Tensor, table: torch.Tensor, bits: int,

@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 7;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 8;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -46,6 +46,7 @@ struct Entries {
     decltype(&tq_beam_select) beam_select;
     decltype(&tq_reorder) reorder;
     decltype(&tq_paged_attend) paged_attend;
+    decltype(&tq_copy_pages) copy_pages;
 } lib{};
 
 struct Raised {};        // a Python exception is set
@@ -624,6 +625,27 @@ PyObject *reorder(PyObject *const *a) {
     return PyLong_FromLong(launch(lib.reorder, (const tq_move_segment *)runs.data(), (int)runs.size(), B, H, (const long long *)address(parents), s.raw()));
 }
 
+// copy_pages(source pool, target pool, rows, bytes between rows, source pages, target pages or None (0, 1, ...), bytes of a row that are copied or None (all)) -> status; lists of whole
+// numbers, which the caller answers for
+PyObject *copy_pages(PyObject *const *a) {
+    TENSOR(from, a[0]); TENSOR(to, a[1]);
+    const long long rows = integer(a[2]), row_bytes = integer(a[3]);
+    NEED(PyList_CheckExact(a[4]) && (a[5] == Py_None || PyList_CheckExact(a[5])) && (a[6] == Py_None || PyList_CheckExact(a[6])) && from.dim() > 0 && to.dim() > 0 && from.device() == to.device());
+    const Py_ssize_t n = PyList_GET_SIZE(a[4]);
+    NEED((a[5] == Py_None || PyList_GET_SIZE(a[5]) == n) && (a[6] == Py_None || PyList_GET_SIZE(a[6]) == n));
+    const Stream s(from);
+    NEED(s.ok);
+    std::vector<tq_page_pair> pairs((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const long long v[3] = {integer(PyList_GET_ITEM(a[4], i)), a[5] == Py_None ? (long long)i : integer(PyList_GET_ITEM(a[5], i)), a[6] == Py_None ? row_bytes : integer(PyList_GET_ITEM(a[6], i))};
+        for (long long x : v) NEED(x >= 0 && x <= 0x7fffffff);
+        NEED(v[0] < from.size(0) && v[1] < to.size(0));
+        pairs[(size_t)i] = {(int32_t)v[0], (int32_t)v[1], (int32_t)v[2]};
+    }
+    return PyLong_FromLong(launch(lib.copy_pages, (const void *)address(from), (long long)(from.stride(0) * from.element_size()), (void *)address(to),
+                                  (long long)(to.stride(0) * to.element_size()), rows, row_bytes, (const tq_page_pair *)pairs.data(), (long long)n, s.raw()));
+}
+
 // paged_attend(address of the step's tq_paged_request, queries, tokens, scale, softcap or None, slopes or None, scratch values, like, stream) -> output; like: a tensor on the cache's
 // device; stream: the one the step's tables were uploaded on
 PyObject *paged_attend(PyObject *const *a) {
@@ -706,7 +728,7 @@ PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
     TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 22), TQ_ENTRY(evict, 10),
-    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9),
+    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9), TQ_ENTRY(copy_pages, 7),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

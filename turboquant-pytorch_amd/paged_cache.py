@@ -20,8 +20,8 @@ from __future__ import annotations
 
 import ctypes
 import heapq
-from itertools import chain
-from typing import Dict, List, Optional, Sequence, Tuple
+from itertools import chain, groupby
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -55,7 +55,7 @@ class _Pages:
         heapq.heappush(self.free, page)
         return True
 
-    def drop_all(self, pages: List[int]) -> None:
+    def drop_all(self, pages: Iterable[int]) -> None:
         held, free = self.held, self.free
         for p in pages:
             n = held[p] - 1
@@ -67,10 +67,8 @@ class _Pages:
 class _Sequence:
     __slots__ = ("pages", "plain", "total")
 
-    def __init__(self):
-        self.pages: List[int] = []
-        self.plain: List[int] = []
-        self.total = 0
+    def __init__(self, pages: List[int], plain: List[int], total: int):
+        self.pages, self.plain, self.total = pages, plain, total
 
 
 def _up(n: int) -> int:
@@ -113,13 +111,17 @@ class PagedV3Cache:
                 at += _up(size)
             self._parts.append((*offsets, *widths))
         self._page_bytes, self._plain_shape = at, (self.n_layers, 2, H, P, self.head_dim)
-        self._pool = torch.empty((pages, at), dtype=torch.uint8, device=self.device)
-        self._plain = torch.empty((plain_pages,) + self._plain_shape, dtype=dtype, device=self.device)
+        self._pool, self._plain = self._pools(pages, plain_pages)
+        self._views = None
         self._packed_pages, self._plain_pages = _Pages(pages), _Pages(plain_pages)
         self._packed_of: Dict[int, int] = {}         # uncompressed pages still held by others -> the packed page one of their sequences made of them
         self._seqs: Dict[int, _Sequence] = {}
         self._next = 0
         self._open: Optional[PagedStep] = None
+
+    def _pools(self, pages: int, plain_pages: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        return (torch.empty((pages, self._page_bytes), dtype=torch.uint8, device=self.device),
+                torch.empty((plain_pages,) + self._plain_shape, dtype=self.dtype, device=self.device))
 
     # ---- what is there --------------------------------------------------------------------------------------------------------
     def codec(self, layer_idx: int) -> TurboQuantV3:
@@ -128,12 +130,19 @@ class PagedV3Cache:
 
     def packed_pages(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         """The layer's part of every packed page, views of the pool: key codes [pages, H, page_tokens, width], key norms [pages, H, page_tokens], and the same of values."""
-        H, P, n = self.kv_heads, self.page_tokens, self._pool.shape[0]
-        k, kn, v, vn, wk, wv = self._parts[layer_idx]
-        halves = self._pool.view(torch.float16)
-        codes = lambda at, w: self._pool.as_strided((n, H, P, w), (self._page_bytes, P * w, w, 1), at)  # noqa: E731
-        norms = lambda at: halves.as_strided((n, H, P), (self._page_bytes // 2, P, 1), at // 2)  # noqa: E731
-        return codes(k, wk), norms(kn), codes(v, wv), norms(vn)
+        if self._views is None:              # (of this pool: `resize` makes another)
+            H, P, n, row = self.kv_heads, self.page_tokens, self._pool.shape[0], self._page_bytes
+            halves, views = self._pool.view(torch.float16), []
+            # layers of equal widths follow one another at the same distance
+            for (wk, wv), group in groupby(self._parts, key=lambda part: part[4:]):
+                group = list(group)
+                (k, kn, v, vn), many = group[0][:4], len(group)
+                apart = group[1][0] - k if many > 1 else 0
+                codes = lambda at, w: self._pool.as_strided((many, n, H, P, w), (apart, row, P * w, w, 1), at).unbind(0)  # noqa: E731
+                norms = lambda at: halves.as_strided((many, n, H, P), (apart // 2, row // 2, P, 1), at // 2).unbind(0)  # noqa: E731
+                views += zip(codes(k, wk), norms(kn), codes(v, wv), norms(vn))
+            self._views = views
+        return self._views[layer_idx]
 
     def plain_pages(self) -> torch.Tensor:
         """The uncompressed pool, [pages, layers, keys and values, H, page_tokens, D]."""
@@ -163,6 +172,13 @@ class PagedV3Cache:
             raise ValueError(f"no sequence {seq!r} in this cache")
         return s
 
+    def _states(self, seqs: Iterable[int]) -> List[_Sequence]:
+        known = self._seqs
+        try:
+            return [known[s] for s in seqs]
+        except (KeyError, TypeError):
+            return [self._sequence(s) for s in seqs]         # (which says what is wrong)
+
     def _eager(self, what: str) -> None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what} reads and changes tables on the host: it cannot be recorded into a graph (`append` and `attend` of a step made before can)")
@@ -175,14 +191,14 @@ class PagedV3Cache:
         new = list(range(self._next, self._next + int(count)))
         self._next += int(count)
         for s in new:
-            self._seqs[s] = _Sequence()
+            self._seqs[s] = _Sequence([], [], 0)
         return new
 
     def place(self, seqs: Sequence[int], packed: Sequence[int], plain: Sequence[int]) -> None:
         """Pages for sequences that are empty so far, `packed` (whole pages) and `plain` tokens, whose contents the caller writes (`packed_pages`, `plain_pages`, `tables`): stores
         that come from elsewhere."""
         self._settle()
-        states = [self._sequence(s) for s in seqs]
+        states = self._states(seqs)
         if not len(states) == len(packed) == len(plain) or len(set(seqs)) != len(states):
             raise ValueError("place: one number of packed and one of plain tokens for each of different sequences")
         if any(s.total for s in states) or any(p < 0 or p % self.page_tokens for p in packed) or any(n < 0 for n in plain):
@@ -198,12 +214,10 @@ class PagedV3Cache:
         if packed > free[0] or plain > free[1]:
             raise _native.TqError(f"{what} needs {packed} packed and {plain} uncompressed pages, {free[0]} and {free[1]} are free (free sequences, or `resize`)")
 
-    def _drop(self, s: _Sequence) -> None:
-        """A sequence's pages are its no longer."""
-        if s.pages:
-            self._packed_pages.drop_all(s.pages)
-        if s.plain:
-            self._plain_pages.drop_all(s.plain)
+    def _drop(self, gone: Sequence[_Sequence]) -> None:
+        """Sequences' pages are theirs no longer."""
+        self._packed_pages.drop_all(chain.from_iterable([s.pages for s in gone]))
+        self._plain_pages.drop_all(chain.from_iterable([s.plain for s in gone]))
 
     def _forget(self) -> None:
         """Of which pages it is known what they were packed into: those that are still held, as what they became is."""
@@ -219,55 +233,47 @@ class PagedV3Cache:
     def free(self, seqs: Sequence[int]) -> None:
         """Sequences end; pages that no other one holds are free."""
         self._settle()
-        known = self._seqs
         if len(set(seqs)) != len(seqs):
             raise ValueError("free: a sequence ends once")
+        gone = self._states(seqs)
         for seq in seqs:
-            if seq not in known:
-                self._sequence(seq)
-        for seq in seqs:
-            self._drop(known.pop(seq))
+            del self._seqs[seq]
+        self._drop(gone)
         self._forget()
 
-    def _share(self, s: _Sequence) -> _Sequence:
-        """A sequence that continues as `s`, with the same pages."""
-        new = _Sequence()
-        new.pages, new.plain, new.total = s.pages[:], s.plain[:], s.total
-        held = self._packed_pages.held
-        for p in s.pages:
-            held[p] += 1
-        held = self._plain_pages.held
-        for p in s.plain:
-            held[p] += 1
-        return new
+    def _share(self, states: Sequence[_Sequence]) -> List[_Sequence]:
+        """Sequences that continue as `states` are, with the same pages."""
+        for pool, lists in ((self._packed_pages, [s.pages for s in states]), (self._plain_pages, [s.plain for s in states])):
+            held = pool.held
+            for p in chain.from_iterable(lists):
+                held[p] += 1
+        return [_Sequence(s.pages[:], s.plain[:], s.total) for s in states]
 
     def _copy_last(self, sharing: Sequence[_Sequence]) -> None:
         """The page that is being filled becomes a sequence's own, where it has been shared so far."""
-        pool, vector = self._plain_pages, self.head_dim * self._plain.element_size()
-        pairs: List[int] = []
+        P, vector, pool = self.page_tokens, self.head_dim * self._plain.element_size(), self._plain_pages
+        sources: List[int] = []
+        targets: List[int] = []
+        sizes: List[int] = []
         for s in sharing:
-            filled = s.total % self.page_tokens
+            filled = s.total % P
             if filled:
-                target = pool.take()
-                pool.drop(s.plain[-1])           # (its owner still holds it)
-                pairs += (s.plain[-1], target, filled * vector)
-                s.plain[-1] = target
-        if pairs:
-            self._move(self._plain, self._plain, self.n_layers * 2 * self.kv_heads, self.page_tokens * vector, np.array(pairs, dtype=np.int32))
-
-    def _move(self, source: torch.Tensor, target: torch.Tensor, rows: int, row_bytes: int, pairs: np.ndarray) -> None:
-        stride = lambda t: t.stride(0) * t.element_size()  # noqa: E731
-        with _native._on(self.device):
-            _native.check(_native.lib().tq_copy_pages(source.data_ptr(), stride(source), target.data_ptr(), stride(target), rows, row_bytes, pairs.ctypes.data, pairs.size // 3,
-                                                      _native._stream_handle(self.device)), "tq_copy_pages")
+                page = s.plain[-1]
+                s.plain[-1] = target = pool.take()
+                pool.drop(page)                  # (its owner still holds it)
+                sources.append(page)
+                targets.append(target)
+                sizes.append(filled * vector)
+        if sources:
+            _native.copy_pages(self._plain, self._plain, self.n_layers * 2 * self.kv_heads, P * vector, sources, targets, sizes)
 
     def fork(self, seqs: Sequence[int]) -> List[int]:
         """For each of `seqs` (one may be there more than once) a new sequence that begins as it is: whole pages are shared, one that is being filled is copied."""
         self._eager("fork")
         self._settle()
-        states = [self._sequence(s) for s in seqs]
-        self._room("fork", 0, sum(1 for s in states if s.total % self.page_tokens))
-        fresh = [self._share(s) for s in states]
+        states, P = self._states(seqs), self.page_tokens
+        self._room("fork", 0, len([s for s in states if s.total % P]))
+        fresh = self._share(states)
         self._copy_last(fresh)
         new = list(range(self._next, self._next + len(fresh)))
         self._next += len(fresh)
@@ -279,7 +285,7 @@ class PagedV3Cache:
         Pages are shared; of several that go on from one, all but one get a copy of the page that is being filled."""
         self._eager("reorder")
         self._settle()
-        states = [self._sequence(s) for s in seqs]
+        states = self._states(seqs)
         if isinstance(parents, torch.Tensor):
             if parents.dtype.is_floating_point or parents.dtype == torch.bool:
                 raise ValueError(f"reorder: parents must be whole numbers, got {parents.dtype}")
@@ -296,9 +302,8 @@ class PagedV3Cache:
         # (pages of the ones that end become free first)
         ends = sum(1 for p, s in enumerate(states) if p not in heir for page in s.plain if self._plain_pages.held[page] == 1)
         self._room("reorder", 0, max(0, twice - ends))
-        fresh = [self._share(states[p]) for p in parents]
-        for s in states:
-            self._drop(s)
+        fresh = self._share([states[p] for p in parents])
+        self._drop(states)
         self._forget()               # (before a page that has become free is taken again)
         self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i])
         self._seqs.update(zip(seqs, fresh))
@@ -317,38 +322,37 @@ class PagedV3Cache:
         """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered, sequence after sequence."""
         self._eager("resize")
         self._settle()
-        states = [self._seqs[seq] for seq in sorted(self._seqs)]
-        # page -> its number in the new pool, as the sequences have them
-        orders = [{p: i for i, p in enumerate(dict.fromkeys(chain.from_iterable(lists)))} for lists in ([s.pages for s in states], [s.plain for s in states])]
+        states = list(self._seqs.values())
+        # the pages that are held, as the sequences have them: a page's place here is its number in the new pool
+        lists = [[s.pages for s in states], [s.plain for s in states]]
+        orders = [list(dict.fromkeys(chain.from_iterable(of))) for of in lists]
         sizes = []
-        for name, asked, order in (("pages", pages, orders[0]), ("plain_pages", plain_pages, orders[1])):
+        for name, asked, order in zip(("pages", "plain_pages"), (pages, plain_pages), orders):
             n = max(1, len(order)) if asked is None else asked
             if isinstance(n, bool) or int(n) != n or n < max(1, len(order)):
                 raise ValueError(f"resize: {name} must be a whole number, {max(1, len(order))} or more (as many are held); got {n!r}")
             sizes.append(int(n))
-        pool = torch.empty((sizes[0], self._page_bytes), dtype=torch.uint8, device=self.device)
-        plain = torch.empty((sizes[1],) + self._plain_shape, dtype=self.dtype, device=self.device)
+        pool, plain = self._pools(*sizes)
         vector = self.head_dim * self._plain.element_size()
         for source, target, order, rows, row_bytes in ((self._pool, pool, orders[0], 1, self._page_bytes),
-                                                       (self._plain, plain, orders[1], int(np.prod(self._plain_shape[:3])), self.page_tokens * vector)):
+                                                       (self._plain, plain, orders[1], self.n_layers * 2 * self.kv_heads, self.page_tokens * vector)):
             if order:
-                pairs = np.full((len(order), 3), row_bytes, dtype=np.int32)
-                pairs[:, 0], pairs[:, 1] = list(order), np.arange(len(order))
-                self._move(source, target, rows, row_bytes, pairs)
-        self._pool, self._plain = pool, plain
+                _native.copy_pages(source, target, rows, row_bytes, order)
+            source.record_stream(torch.cuda.current_stream(self.device))         # (what it was allocated on may be another one)
+        self._pool, self._plain, self._views = pool, plain, None
+        # (the copies run while the tables are brought in line)
         pools = []
-        for old, order, size in zip((self._packed_pages, self._plain_pages), orders, sizes):
+        for old, of, order, size in zip((self._packed_pages, self._plain_pages), lists, orders, sizes):
             new = _Pages(0)
-            new.held = [old.held[p] for p in order] + [0] * (size - len(order))
+            new.held = list(map(old.held.__getitem__, order)) + [0] * (size - len(order))
             new.free = list(range(len(order), size))
             pools.append(new)
+            number = dict(zip(order, range(len(order))))
+            for pages_of in of:
+                if pages_of:
+                    pages_of[:] = map(number.__getitem__, pages_of)
+            self._packed_of = {(p if old is self._packed_pages else number[p]): (number[q] if old is self._packed_pages else q) for p, q in self._packed_of.items()}
         self._packed_pages, self._plain_pages = pools
-        for s in states:
-            if s.pages:
-                s.pages = [orders[0][p] for p in s.pages]
-            if s.plain:
-                s.plain = [orders[1][p] for p in s.plain]
-        self._packed_of = {orders[1][p]: orders[0][q] for p, q in self._packed_of.items()}
 
     # ---- steps ----------------------------------------------------------------------------------------------------------------
     def step(self, seqs: Sequence[int], counts) -> "PagedStep":
@@ -356,7 +360,7 @@ class PagedV3Cache:
         self._eager("step")
         self._settle()
         seqs = list(seqs)
-        states = [self._sequence(s) for s in seqs]
+        states = self._states(seqs)
         counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
         if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(isinstance(c, bool) or int(c) != c or c < 0 for c in counts):
             raise ValueError("step: for each of different sequences a whole number of new tokens, 0 or more")
