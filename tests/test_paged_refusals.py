@@ -35,7 +35,7 @@ def test_a_plan_covers_what_is_seen_once(pkg, sequences, window):
         small = [bool(few and f * group <= 16) for f, _, _ in sequences]
         assert all(small[b] == (i < counts.few) for i, b in enumerate(items[:, 0].tolist()))
         assert counts.vectors == max([f * group for (f, _, _), s in zip(sequences, small) if s and f] or [0])
-        assert rc == 0 and counts.tiles in ((1, 2) if dtype == 2 and D in (64, 128) else (1,)) and 1 <= counts.columns <= 32
+        assert rc == 0 and counts.tiles in ((1, 2) if dtype and D in (64, 128) else (1,)) and 1 <= counts.columns <= 32
         by_group = {}
         for it in items.tolist():
             for h in range(heads) if it[7] < 0 else (it[7],):
@@ -130,7 +130,7 @@ def test_attention_checks_its_request(pkg):
         assert L.tq_paged_attend(ctypes.byref(bad), 4096, need, None) == -8, name
     bad = copy()
     bad.counts.tiles = 2
-    bad.dtype = 1
+    bad.dtype = 0
     assert L.tq_paged_attend(ctypes.byref(bad), 4096, 1 << 40, None) == -5
     for field, value in (("few", -1), ("few", counts.items + 1), ("vectors", 0), ("vectors", 17)):
         bad = copy()

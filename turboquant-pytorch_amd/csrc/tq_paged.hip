@@ -307,7 +307,7 @@ extern "C" int tq_paged_plan(const int32_t *sequences, long long n, int heads, i
         for (int few = 1; few >= 0; --few) {
             Shares best;
             // (two tiles a block share what is read and decoded; 96 wide they would spill)
-            const bool two = !few && dtype == TQ_BF16 && (head_dim == 64 || head_dim == 128) && most > 1;
+            const bool two = !few && dtype != TQ_F32 && (head_dim == 64 || head_dim == 128) && most > 1;
             for (int qt = 1; qt <= (two ? 2 : 1); ++qt) {
                 std::vector<Group> groups;
                 for (long long b = 0; b < n; ++b) {
@@ -365,7 +365,7 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     if (n.items == 0) return TQ_OK;
     if (n.few < 0 || n.few > n.items || n.blocks < 0 || n.blocks > 0x7fffffff || (n.few && (n.blocks < 1 || n.vectors < 1 || n.vectors > 16 || r.dtype == TQ_F32 || r.page_tokens < 64 || (r.head_dim & 31)))) return TQ_ERR_SIZE;
     if (n.items > 0x7fffffff / r.heads || n.tiles < 1 || n.tiles > 2 || n.columns < 1 || n.columns > 32) return TQ_ERR_SIZE;
-    if (n.tiles == 2 && (r.dtype != TQ_BF16 || (r.head_dim != 64 && r.head_dim != 128))) return TQ_ERR_SIZE;
+    if (n.tiles == 2 && (r.dtype == TQ_F32 || (r.head_dim != 64 && r.head_dim != 128))) return TQ_ERR_SIZE;
     if (!r.queries || !r.out || !r.packed_pool || !r.plain_pool || !r.table_k || !r.table_v || !r.sequences || !r.tables || !r.items || (n.merges && (!r.merges || !scratch))) return TQ_ERR_NULL;
     const long long es = r.dtype == TQ_F32 ? 4 : 2;
     // vectors of a page as the kernels read them: runs of 32 tokens 16 bytes at a time (packed bytes of uneven dimensions: words)

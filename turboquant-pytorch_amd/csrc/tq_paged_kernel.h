@@ -819,9 +819,13 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
 template <int DP, int IPBK, int IPBV>
 int launch_paged(dim3 grid, hipStream_t s, const TqPagedArgs &a, int qt, int kt, int vt) {
     if (vt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 2, 2>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if (kt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if (DP == 96 || DP == 256 || qt == 1) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
-    else if constexpr (DP == 64 || DP == 128) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 2, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    else if (DP == 96 || DP == 256 || qt == 1) {
+        if (kt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+        else hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 1, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    } else if constexpr (DP == 64 || DP == 128) {
+        if (kt == 2) hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 2, 2, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+        else hipLaunchKernelGGL((tq_paged_kernel<DP, IPBK, IPBV, 2, 1, 1>), grid, dim3(FAST_THREADS), 0, s, a);
+    }
     return 0;
 }
 template <int DP>
