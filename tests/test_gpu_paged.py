@@ -186,6 +186,43 @@ def test_more_rows_than_the_device_takes_at_a_time(pkg, D, H, G, dtype, kb, vb, 
     check(step.attend(q, 0, sliding_window=90), q, step, sliding_window=90)
 
 
+@pytest.mark.parametrize("D,H,G,dtype,kb,vb,P", [(128, 2, 4, BF, 4, 2, 64), (128, 1, 7, F16, 4, 2, 32), (64, 2, 1, F16, 6, 4, 64), (64, 1, 4, BF, 4, 2, 128), (80, 2, 4, BF, 4, 2, 64), (96, 1, 2, F16, 4, 2, 64),
+                                                 (256, 1, 2, BF, 4, 2, 64), (256, 1, 1, F16, 8, 8, 256), (128, 1, 2, F32, 4, 2, 64), (72, 1, 1, F32, 4, 4, 64)])
+def test_prompts_that_nothing_is_packed_of_yet(pkg, D, H, G, dtype, kb, vb, P):
+    new = (600, 1, 257, 0, 32, 255)
+    cache = make(pkg, D, H, dtype, kb, vb, 64, P=P, pages=64, plain=128)
+    seqs = cache.add(len(new))
+    feed(cache, seqs, (0, 300, 31, 5, 0, 1), seed=1)
+    step = feed(cache, seqs, new, seed=2, commit=False)
+    q = rand((sum(new), H * G, D), 3, dtype)
+    check(step.attend(q, 0), q, step)
+    check(step.attend(q, 0, sliding_window=45, softcap=20.0), q, step, sliding_window=45, softcap=20.0)
+
+
+def test_values_that_are_no_numbers_in_a_long_prompt(pkg):
+    for dtype, D in ((BF, 128), (F16, 64), (BF, 80), (F32, 128)):
+        cache = make(pkg, D, 1, dtype, 4, 4, 64, plain=32)
+        (seq,) = cache.add(1)
+        step = cache.step([seq], 600)
+        k, v = states(600, 1, D, 1, dtype), states(600, 1, D, 2, dtype)
+        q = rand((600, 2, D), 3, dtype)
+        step.append(k, v, 0)
+        whole = step.attend(q, 0)
+        v[333, 0, 5], v[500, 0, 6], v[501, 0, 6], v[599, 0, 7] = float("inf"), float("inf"), float("-inf"), float("nan")
+        step.append(k, v, 0)
+        out = step.attend(q, 0)
+        rows = torch.arange(600, device=DEV)
+        want = whole.clone()
+        want[rows >= 333, :, 5] = float("inf")
+        want[rows == 500, :, 6] = float("inf")
+        want[rows >= 501, :, 6] = float("nan")
+        want[rows == 599, :, 7] = float("nan")
+        assert torch.equal(torch.isfinite(out), torch.isfinite(want)) and torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out[torch.isfinite(out)], whole[torch.isfinite(want)])
+        out = step.attend(q, 0, sliding_window=100)
+        assert bool(torch.isfinite(out[433:500]).all()) and bool(torch.isinf(out[333:433, :, 5]).all()) and bool(torch.isfinite(out[501:599, :, 5]).all())
+
+
 def test_scale_and_layouts_of_queries(pkg):
     cache = make(pkg, H=2, layers=2, protected_layers=1)            # (8 bits in both)
     seqs = cache.add(2)

@@ -40,181 +40,6 @@ __device__ __forceinline__ uint32_t unseen_bits(uint32_t t0, uint32_t pos, uint3
     return bits;
 }
 
-// 32 uncompressed tokens of a page against a tile of queries: raw 16-bit products are exact, weights enter the value product as three bf16 terms, or two fp16 ones.  Row r of
-// acc[c] is coordinate NC r + c.  Infinite and NaN values count as zero here (a product would spread them to queries that do not see their token as 0 * inf); `wild` says
-// whether there are any.  Up to 128 wide all loads are under way at once (HELD).
-template <int DP, int DT>
-struct PagedPlain {
-    static constexpr bool BF = DT == TQ_BF16, EVEN = Shape<DP>::EVEN, HELD = DP <= 128;
-    static constexpr int NC = Shape<DP>::NC, STEPS = DP / 16, PT = BF ? 3 : 2, VT = HELD ? 16 : 8, KH = HELD ? STEPS : 1;
-    static constexpr uint32_t EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
-    uint32_t vw[VT][NC / 2];
-    tq_u4 kx[KH];
-    const uint8_t *k, *v;
-    uint32_t valid;
-    bool wild;
-    // elements 16 st + 8 h ... + 7 of a vector, zeros from D on (a multiple of 8)
-    static __device__ __forceinline__ tq_u4 half_step(const uint8_t *vec, int st, uint32_t h, uint32_t D, bool aligned) {
-        const uint32_t d = 16u * st + 8u * h;
-        const tq_u4 x = load_elements(vec + 2u * (EVEN ? d : min(d, D - 8u)), aligned);
-        return EVEN || d < D ? x : tq_u4{0u, 0u, 0u, 0u};
-    }
-    __device__ __forceinline__ void load_values(uint32_t D, int j0, uint32_t h) {
-#pragma unroll
-        for (int j = 0; j < VT; ++j) {
-            const uint8_t *p = v + acc_row(j0 + j, h) * D * 2u;
-            if constexpr (NC == 2) vw[j][0] = tq_gload4(p);
-            else if constexpr (NC == 4) { const tq_u2 x = tq_gload8(p); vw[j][0] = x[0]; vw[j][1] = x[1]; }
-            else { const tq_u4 x = tq_gload16(p); vw[j][0] = x[0]; vw[j][1] = x[1]; vw[j][NC / 2 - 2] = x[2]; vw[j][NC / 2 - 1] = x[3]; }
-        }
-    }
-    __device__ __forceinline__ void tame_values(int j0, uint32_t h) {
-        uint32_t over = 0u;
-#pragma unroll
-        for (int j = 0; j < VT; ++j)
-#pragma unroll
-            for (int c = 0; c < NC / 2; ++c) {
-                if (acc_row(j0 + j, h) >= valid) vw[j][c] = 0u;
-                over |= (vw[j][c] & EXPO) + ONE;         // (an exponent of ones carries into the sign's place)
-            }
-        if (__any((over & 0x80008000u) != 0u)) {
-            wild = true;
-#pragma unroll
-            for (int j = 0; j < VT; ++j)
-#pragma unroll
-                for (int c = 0; c < NC / 2; ++c) vw[j][c] &= ~(((((vw[j][c] & EXPO) + ONE) >> 15) & 0x00010001u) * 0xffffu);
-        }
-    }
-    // keys, values: of the head's first of the 32 tokens, `valid` of which there are
-    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint32_t valid_, uint32_t D, uint32_t lane) {
-        const uint32_t n = lane & 31u, h = lane >> 5;
-        valid = valid_;
-        k = keys + n * D * 2u;
-        v = values + 2u * NC * (EVEN ? n : min(n, D / NC - 1u));
-        if constexpr (HELD) {
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) kx[st] = half_step(k, st, h, D, true);
-            load_values(D, 0, h);
-            tame_values(0, h);
-        }
-    }
-    __device__ __forceinline__ tq_f16v scores(const uint8_t *q, uint32_t D, bool aligned, uint32_t lane) {
-        const uint32_t h = lane >> 5;
-        tq_f16v s = tq_zero16();
-        constexpr int CH = HELD ? STEPS : 4;
-#pragma unroll 1
-        for (int s0 = 0; s0 < STEPS; s0 += CH) {
-            tq_u4 x[CH], y[CH];
-#pragma unroll
-            for (int st = 0; st < CH; ++st) x[st] = HELD ? kx[HELD ? st : 0] : half_step(k, s0 + st, h, D, true);
-            if (aligned) {
-#pragma unroll
-                for (int st = 0; st < CH; ++st) y[st] = half_step(q, s0 + st, h, D, true);
-            } else {
-#pragma unroll
-                for (int st = 0; st < CH; ++st) y[st] = half_step(q, s0 + st, h, D, false);
-            }
-#pragma unroll
-            for (int st = 0; st < CH; ++st) s = BF ? mfma_bf16(x[st], y[st], s) : mfma_f16(x[st], y[st], s);
-        }
-        return s;
-    }
-    __device__ __forceinline__ void values(uint32_t D, const float (&x)[16], uint32_t lane, tq_f16v (&acc)[NC]) {
-        const uint32_t h = lane >> 5;
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            if constexpr (!HELD) {
-                load_values(D, 8 * st, h);
-                tame_values(8 * st, h);
-            }
-            tq_u4 p[3];
-            float ps[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ps[j] = x[8 * st + j];
-            if constexpr (BF) bf16_terms(ps, p);
-            else {
-                uint32_t t[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = fp16_terms(ps[j]);
-                fp16_operands(t, p[0], p[1]);
-            }
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                tq_u4 o;
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    o[d] = __builtin_amdgcn_perm(vw[(HELD ? 8 * st : 0) + 2 * d + 1][c / 2], vw[(HELD ? 8 * st : 0) + 2 * d][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                for (int t = 0; t < PT; ++t) acc[c] = BF ? mfma_bf16(o, p[t], acc[c]) : mfma_f16(o, p[t], acc[c]);
-            }
-        }
-    }
-};
-
-// The same for float32 elements: three bf16 terms of everything, products down to 2^-24 of the largest.
-template <int DP>
-struct PagedPlain<DP, TQ_F32> {
-    static constexpr int NC = Shape<DP>::NC, STEPS = DP / 16;
-    const uint8_t *k, *v;
-    uint32_t valid;
-    bool wild;
-    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint32_t valid_, uint32_t D, uint32_t lane) {
-        const uint32_t n = lane & 31u;
-        valid = valid_;
-        k = keys + n * D * 4u;
-        v = values + 4u * NC * min(n, D / NC - 1u);
-    }
-    __device__ __forceinline__ tq_f16v scores(const uint8_t *q, uint32_t D, bool aligned, uint32_t lane) {
-        const uint32_t h = lane >> 5;
-        tq_f16v s = tq_zero16();
-#pragma unroll 1
-        for (int st = 0; st < STEPS; ++st) {
-            tq_u4 kt[3], qt[3];
-            load_plain8<TQ_F32>(k, 16u * st + 8u * h, D, true, kt);
-            load_plain8<TQ_F32>(q, 16u * st + 8u * h, D, aligned, qt);
-#pragma unroll
-            for (int i = 0; i < 3; ++i)
-#pragma unroll
-                for (int j = 0; j < 3 - i; ++j) s = mfma_bf16(kt[i], qt[j], s);
-        }
-        return s;
-    }
-    __device__ __forceinline__ void values(uint32_t D, const float (&x)[16], uint32_t lane, tq_f16v (&acc)[NC]) {
-        const uint32_t h = lane >> 5;
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            float ps[8], e[8][NC];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ps[j] = x[8 * st + j];
-                const uint32_t t = acc_row(8 * st + j, h);
-                const uint8_t *p = v + t * D * 4u;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const float value = t < valid ? plain_element(p + 4 * c, TQ_F32) : 0.f;
-                    const bool fine = fabsf(value) < __builtin_inff();
-                    wild = wild || !fine;
-                    e[j][c] = fine ? value : 0.f;
-                }
-            }
-            tq_u4 p[3];
-            bf16_terms(ps, p);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float own8[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) own8[j] = e[j][c];
-                tq_u4 vt[3];
-                bf16_terms(own8, vt);
-#pragma unroll
-                for (int i = 0; i < 3; ++i)
-#pragma unroll
-                    for (int j = 0; j < 3 - i; ++j) acc[c] = mfma_bf16(vt[i], p[j], acc[c]);
-            }
-        }
-    }
-};
-
 // Infinite and NaN values of plain tokens [from, to) into the joined sums of the queries that see them, whatever their weight (it is not zero).
 template <int DP>
 __device__ __forceinline__ void paged_wild(const TqPagedArgs &a, const PagedRow &r, float *out, uint32_t tile, uint32_t from, uint32_t to, uint32_t tid) {
@@ -236,90 +61,308 @@ __device__ __forceinline__ void paged_wild(const TqPagedArgs &a, const PagedRow 
     }
 }
 
-// A block's plain tokens against its tiles of queries, joined sums into LDS.
+// A block's plain tokens against its tiles of queries, sums into LDS.  Eight runs of 32 tokens at a time: a wave has the scores of one run, for all tiles; the waves agree on the largest logit
+// of every query, put their weights into LDS as operands, and then a wave has 32 coordinates of the value sums (of every second run, or fourth, where there are fewer than eight such
+// slices), so that what they hold need not be joined.  (Against a run a wave with all coordinates, joined at the end: 29000 cycles instead of 55000 for the 320 plain tokens of a block of 64
+// bfloat16 query vectors 128 wide, four chunks of 256 tokens over 8191: 138 us instead of 157 for the call.)
+// Raw 16-bit products are exact; weights are two terms (bfloat16: 16 bits, half a step of 2^-17 where a result has 2^-9; fp16: 22 bits); float32 elements are three bf16 terms of everything, products down
+// to 2^-24 of the largest.  Infinite and NaN values count as zero in the products (they would spread to queries that do not see their token as 0 * inf) and are added after.
 template <int DP, int QT, int DT>
-__device__ __forceinline__ void paged_plain_phase(const TqPagedArgs &a, const TqManyArgs &v, const PagedRow &r, uint8_t *lds, float (*lds_m)[32], float (*lds_l)[32], float *lds_wild,
-                                                  uint32_t tile0, uint32_t tiles, uint32_t from, uint32_t to, uint32_t tid) {
-    constexpr int NC = Shape<DP>::NC;
-    constexpr uint32_t ES = DT == TQ_F32 ? 4u : 2u;
+__device__ __forceinline__ void paged_plain_phase(const TqPagedArgs &a, const TqManyArgs &v, const PagedRow &r, uint8_t *lds, float *lds_wild, uint32_t tile0, uint32_t tiles, uint32_t from,
+                                                  uint32_t to, uint32_t tid) {
+    constexpr bool F32 = DT == TQ_F32, BF = DT == TQ_BF16, EVEN = Shape<DP>::EVEN;
+    constexpr int STEPS = DP / 16, SLICES = DP / 32, GROUPS = FAST_WAVES / SLICES, PT = F32 ? 3 : 2;
+    constexpr int RG = FAST_WAVES / GROUPS, VH = RG < 4 ? RG : 4;          // runs of a group, those whose values are under way at once
+    constexpr int CH = F32 ? 1 : EVEN ? 4 : STEPS;                         // steps of a score product that are staged at a time
+    constexpr uint32_t ES = F32 ? 4u : 2u, EXPO = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u, ROW = DP + 4u;
     using J = JoinArea<DP, QT>;
-    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, runs = (to - from + 31u) / 32u;
-    const bool share = QT == 2 && tiles == 2u && runs <= FAST_WAVES / 2u;
-    const uint32_t count = share ? FAST_WAVES / 2u : FAST_WAVES, side = wave / count, w0 = side * count, rounds = share ? 1u : tiles;
-#pragma unroll 1
-    for (uint32_t i = 0; i < rounds; ++i) {
-        const uint32_t mine = share ? side : i, m = min((tile0 + mine) * 32u + n, v.M - 1u), token = m / a.group, pos = r.total - r.fresh + token;
-        const uint8_t *q = many_query(v, 0u, m, ES);
-        const float slope = a.slopes ? a.slopes[r.kv * a.group + (m - token * a.group)] * LOG2E : 0.f;
-        const Cap cap(a);
-        float m_ref = MANY_NONE, l = 0.f;
-        tq_f16v acc[NC];
+    constexpr uint32_t PIECES = 2 * CH, TURN = PIECES % 8u ? 0u : 7u;        // sixteen bytes each of a staged vector; they lie in an order that is turned by the vector's number, so that lanes' reads spread over the banks
+    constexpr uint32_t OPERANDS = 2u * QT * PT * 1024u, STAGED = F32 ? 0u : 32u * 16u * PIECES, RUN_BYTES = OPERANDS > STAGED ? OPERANDS : STAGED, STATS = FAST_WAVES * RUN_BYTES;
+    static_assert(STATS + FAST_WAVES * QT * 128u <= J::PACKED && (GROUPS - 1u) * QT * 32u * ROW * 4u <= STATS, "beside the packed tokens' sums");
+    asm volatile("" : "+v"(tid));    // (what lanes make of their number is made here, not ahead of the loop over packed tokens, which has no register left)
+    const uint32_t lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5, runs = (to - from + 31u) / 32u, slice = wave % SLICES, g = wave / SLICES;
+    const bool adds = g < (uint32_t)GROUPS;          // (96 wide: two waves have no slice)
+    float *const stats = reinterpret_cast<float *>(lds + STATS) + n;       // [wave][tile][32]
+    uint8_t *const weights = lds + lane * 16u;       // [run][step][tile][term] operands; before that a wave's keys
+    uint8_t *const staged = lds + wave * RUN_BYTES, *const queries = reinterpret_cast<uint8_t *>(J::sums(lds, 1u, 0u));        // [step of CH][tile][32][pieces]
+    const Cap cap(a);
+    const uint8_t *q[QT];
+    uint32_t pos[QT];
+    float slope[QT], m_ref[QT], l[QT];
+    tq_f16v acc[QT];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) acc[c] = tq_zero16();
-        bool wild = false;
-#pragma unroll 1
-        for (uint32_t w = wave - w0; w < runs; w += count) {
-            const uint32_t t0 = from + 32u * w;
-            const uint8_t *page = a.plain + (long long)r.plain_pages[t0 >> a.shift] * a.plain_stride + (size_t)((r.kv << a.shift) + (t0 & ((1u << a.shift) - 1u))) * (a.D * ES);
-            PagedPlain<DP, DT> t;
-            t.wild = false;
-            t.load(page, page + a.plain_v, min(32u, to - t0), a.D, lane);
-            const tq_f16v s = t.scores(q, a.D, v.aligned, lane);
-            const uint32_t at = r.packed + t0, gone = unseen_bits(at, pos, a.window) >> (4u * h);
-            const uint32_t valid = t.valid;
-            float x[16];
+    for (int i = 0; i < QT; ++i) {
+        const uint32_t m = min((tile0 + i) * 32u + n, v.M - 1u), token = m / a.group;
+        q[i] = many_query(v, 0u, m, ES);
+        pos[i] = r.total - r.fresh + token;
+        slope[i] = a.slopes ? a.slopes[r.kv * a.group + (m - token * a.group)] * LOG2E : 0.f;
+        m_ref[i] = MANY_NONE;
+        l[i] = 0.f;
+        acc[i] = tq_zero16();
+    }
+    // pages of the eight runs from r0 on, a lane's each: asked for ahead of the runs before
+    auto lookup = [&](uint32_t r0) { return r.plain_pages[min(from + 32u * (r0 + (lane & 7u)), to - 1u) >> a.shift]; };
+    int pages = lookup(0u);
+    auto first_of = [&](uint32_t r0, uint32_t own) {         // of the head's keys: the first token of the run that is `own`'th of the eight
+        const uint32_t t0 = from + 32u * (r0 + own);
+        return a.plain + (long long)__builtin_amdgcn_readlane(pages, (int)own) * a.plain_stride + (size_t)((r.kv << a.shift) + (t0 & ((1u << a.shift) - 1u))) * ((EVEN ? (uint32_t)DP : a.D) * ES);
+    };
+    if constexpr (!F32) {
+        // queries into LDS, whole vectors by neighbouring lanes (as operands straight from memory every load touched a line a query)
+        auto copy = [&](bool aligned) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = s[j] * (a.scale * LOG2E);
-            if (a.cap != 0.f) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = cap.template operator()<DT == TQ_F32>(x[j]);
+            for (uint32_t at = tid; at < QT * 32u * (DP / 8u); at += FAST_THREADS) {
+                const uint32_t vec = at / (DP / 8u), piece = at % (DP / 8u);
+                const tq_u4 x = load_elements(many_query(v, 0u, min(tile0 * 32u + vec, v.M - 1u), ES) + 16u * (EVEN ? piece : min(piece, a.D / 8u - 1u)), aligned);
+                *reinterpret_cast<tq_u4 *>(queries + ((piece / PIECES * QT * 32u + vec) * PIECES + ((piece % PIECES) ^ (vec & TURN))) * 16u) = EVEN || 8u * piece < a.D ? x : tq_u4{0u, 0u, 0u, 0u};
             }
-            if (a.slopes) {
-                const float first = (float)((int)(at + 4u * h) - (int)pos);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = fmaf(slope, first + (float)acc_row(j, 0u), x[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uint32_t row = acc_row(j, 0u);
-                x[j] = row + 4u * h < valid && !((gone >> row) & 1u) ? x[j] : MANY_NONE;
-            }
-            float top = x[0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-            top = fmaxf(halves_max(top), m_ref);
-            const float shrink = __builtin_amdgcn_exp2f(m_ref - top);
-            m_ref = top;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] = x[j] == MANY_NONE ? 0.f : __builtin_amdgcn_exp2f(x[j] - top);
-                sum += x[j];
-            }
-            l = l * shrink + sum;          // (this lane's half)
-            if (__any(shrink != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) acc[c] *= shrink;
-            }
-            t.values(a.D, x, lane, acc);
-            wild |= t.wild;
-        }
-        __syncthreads();             // (what the area held)
-        wild = __any(wild);
-        if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
-        float *const area = reinterpret_cast<float *>(lds);
-        if (share) join_waves<DP, FAST_WAVES / 2>(area, lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), w0, 1.f, m_ref, l, acc, tid);
-        else join_waves<DP, FAST_WAVES>(area, lds_m, lds_l, J::sums(lds, 1u, mine), J::largest(lds, 1u, mine), J::total(lds, 1u, mine), 0u, 1.f, m_ref, l, acc, tid);
+        };
+        if (v.aligned) copy(true);
+        else copy(false);
         __syncthreads();
-        float any = 0.f;
+    }
+    uint32_t raw[VH][16];                            // values of coordinate 32 slice + n
+    const uint32_t vec_bytes = (EVEN ? (uint32_t)DP : a.D) * ES, v_at = (EVEN ? 32u * slice + n : min(32u * slice + n, a.D - 1u)) * ES + 4u * h * vec_bytes;
+    auto load_values = [&](uint32_t r0, int k0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int w = 0; w < FAST_WAVES; ++w) any += lds_wild[w];
-        if (any != 0.f) {
-            if (!share) paged_wild<DP>(a, r, J::sums(lds, 1u, i), tile0 + i, from, to, tid);
-            else
-                for (uint32_t k = 0; k < 2u; ++k) paged_wild<DP>(a, r, J::sums(lds, 1u, k), tile0 + k, from, to, tid);
-            __syncthreads();
+        for (int k = 0; k < VH; ++k) {
+            const uint32_t own = g + (uint32_t)((k0 + k) * GROUPS);
+            if (!adds || r0 + own >= runs) continue;
+            const uint8_t *p = first_of(r0, own) + a.plain_v;
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                const uint32_t lane_at = v_at + 16u * st * vec_bytes;        // (whole vectors up to 16 fit the instruction)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint8_t *e = p + lane_at + acc_row(j, 0u) * vec_bytes;
+                    if constexpr (F32) raw[k][8 * st + j] = tq_gload4(e);
+                    else raw[k][8 * st + j] = tq_gload2(reinterpret_cast<const uint16_t *>(e));
+                }
+            }
         }
+    };
+    bool wild = false;
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < runs; r0 += FAST_WAVES) {
+        const uint32_t run = r0 + wave, t0 = from + 32u * run;
+        const bool some = run < runs;
+        float x[QT][16];
+        const int pages_after = lookup(r0 + FAST_WAVES);
+        if (some) {
+            const uint8_t *k = first_of(r0, wave) + (F32 ? n * vec_bytes : 0u);
+            tq_u4 keys[F32 ? 1 : STEPS];
+            if constexpr (!F32) {
+#pragma unroll
+                for (int s0 = 0; s0 < STEPS; s0 += CH)
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        if constexpr (EVEN) keys[s0 + i] = tq_gload16(k + (lane / PIECES * vec_bytes + 16u * (lane % PIECES)) + (i * (64u / PIECES) * vec_bytes + 16u * (s0 / CH * PIECES)));
+                        else {
+                            const uint32_t at = i * 64u + lane, vec = at / PIECES, piece = at % PIECES;
+                            const tq_u4 x = tq_gload16(k + vec * vec_bytes + 16u * min(piece, a.D / 8u - 1u));
+                            keys[s0 + i] = 8u * piece < a.D ? x : tq_u4{0u, 0u, 0u, 0u};
+                        }
+                    }
+                load_values(r0, 0);
+            }
+            tq_f16v s[QT];
+#pragma unroll
+            for (int i = 0; i < QT; ++i) s[i] = tq_zero16();
+#pragma unroll(F32 ? 1 : 4)
+            for (int s0 = 0; s0 < STEPS; s0 += CH) {
+                if constexpr (F32) {
+                    tq_u4 kt[3];
+                    load_plain8<TQ_F32>(k, 16u * s0 + 8u * h, a.D, true, kt);
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        tq_u4 qt[3];
+                        load_plain8<TQ_F32>(q[i], 16u * s0 + 8u * h, a.D, v.aligned, qt);
+#pragma unroll
+                        for (int x0 = 0; x0 < 3; ++x0)
+#pragma unroll
+                            for (int x1 = 0; x1 < 3 - x0; ++x1) s[i] = mfma_bf16(kt[x0], qt[x1], s[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < CH; ++k) {
+                        const uint32_t at = k * 64u + lane, vec = at / PIECES, piece = at % PIECES;
+                        *reinterpret_cast<tq_u4 *>(staged + (vec * PIECES + (piece ^ (vec & TURN))) * 16u) = keys[s0 + k];
+                    }
+                    wave_sync();
+#pragma unroll
+                    for (int st = 0; st < CH; ++st) {
+                        const uint32_t piece = (2u * st + h) ^ (n & TURN);
+                        const tq_u4 y = *reinterpret_cast<const tq_u4 *>(staged + (n * PIECES + piece) * 16u);
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) {
+                            const tq_u4 z = *reinterpret_cast<const tq_u4 *>(queries + ((s0 / CH * QT * 32 + 32 * i + n) * PIECES + piece) * 16u);
+                            s[i] = BF ? mfma_bf16(y, z, s[i]) : mfma_f16(y, z, s[i]);
+                        }
+                    }
+                    wave_sync();
+                }
+            }
+            if (F32) load_values(r0, 0);
+            const uint32_t at = r.packed + t0, valid = min(32u, to - t0);
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                const uint32_t gone = (unseen_bits(at, pos[i], a.window) | (valid < 32u ? ~0u << valid : 0u)) >> (4u * h);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[i][j] = s[i][j] * (a.scale * LOG2E);
+                if (a.cap != 0.f) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[i][j] = cap.template operator()<F32>(x[i][j]);
+                }
+                if (a.slopes) {
+                    const float first = (float)((int)(at + 4u * h) - (int)pos[i]);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[i][j] = fmaf(slope[i], first + (float)acc_row(j, 0u), x[i][j]);
+                }
+                if (__any(gone != 0u)) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[i][j] = (gone >> acc_row(j, 0u)) & 1u ? MANY_NONE : x[i][j];
+                }
+                float top = x[i][0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) top = fmaxf(top, x[i][j]);
+                top = halves_max(fmaxf(top, MANY_NONE));
+                if (h == 0u) stats[(wave * QT + i) * 32u] = top;
+            }
+        } else {
+            load_values(r0, 0);
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+                if (h == 0u) stats[(wave * QT + i) * 32u] = MANY_NONE;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            float now = m_ref[i];
+#pragma unroll
+            for (int w = 0; w < FAST_WAVES; ++w) now = fmaxf(now, stats[(w * QT + i) * 32]);
+            const float shrink = __builtin_amdgcn_exp2f(m_ref[i] - now);
+            m_ref[i] = now;
+            l[i] *= shrink;              // (this lane's tokens)
+            acc[i] *= shrink;
+            if (!some) continue;
+            const float least = now == MANY_NONE ? 0.f : now;        // (no token seen so far: weights of zero)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[i][j] = __builtin_amdgcn_exp2f(x[i][j] - least);
+                l[i] += x[i][j];
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                tq_u4 p[3];
+                float ps[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ps[j] = x[i][8 * st + j];
+                if constexpr (BF || F32) bf16_terms(ps, p);
+                else fp16_split8(tq_f4{ps[0], ps[1], ps[2], ps[3]}, tq_f4{ps[4], ps[5], ps[6], ps[7]}, 1.f, p[0], p[1]);
+#pragma unroll
+                for (int t = 0; t < PT; ++t) *reinterpret_cast<tq_u4 *>(weights + (((wave * 2u + st) * QT + i) * PT + t) * 1024u) = p[t];
+            }
+        }
+        __syncthreads();
+        if (adds) {
+#pragma unroll
+        for (int k0 = 0; k0 < RG; k0 += VH) {
+            if (k0) load_values(r0, k0);
+#pragma unroll
+            for (int k = 0; k < VH; ++k) {
+                const uint32_t own = g + (uint32_t)((k0 + k) * GROUPS), left = to - min(to, from + 32u * (r0 + own));       // of the eight; its tokens and those behind them
+                if (!left) continue;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    tq_u4 o[3];
+                    if (left < 32u) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) raw[k][8 * st + j] = acc_row(8 * st + j, h) < left ? raw[k][8 * st + j] : 0u;
+                    }
+                    if constexpr (F32) {
+                        float e[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float value = __uint_as_float(raw[k][8 * st + j]);
+                            const bool fine = fabsf(value) < __builtin_inff();
+                            wild = wild || !fine;
+                            e[j] = fine ? value : 0.f;
+                        }
+                        bf16_terms(e, o);
+                    } else {
+                        uint32_t over = 0u;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            o[0][d] = raw[k][8 * st + 2 * d] | raw[k][8 * st + 2 * d + 1] << 16;
+                            over |= (o[0][d] & EXPO) + ONE;          // (an exponent of ones carries into the sign's place)
+                        }
+                        if (__any((over & 0x80008000u) != 0u)) {
+                            wild = true;
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) o[0][d] &= ~(((((o[0][d] & EXPO) + ONE) >> 15) & 0x00010001u) * 0xffffu);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        tq_u4 p[PT];
+#pragma unroll
+                        for (int t = 0; t < PT; ++t) p[t] = *reinterpret_cast<const tq_u4 *>(weights + (((own * 2u + st) * QT + i) * PT + t) * 1024u);
+#pragma unroll
+                        for (int t = 0; t < PT; ++t) {
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int x0 = 0; x0 < 3 - t; ++x0) acc[i] = mfma_bf16(o[x0], p[t], acc[i]);
+                            } else acc[i] = BF ? mfma_bf16(o[0], p[t], acc[i]) : mfma_f16(o[0], p[t], acc[i]);
+                        }
+                    }
+                }
+            }
+        }
+        }
+        pages = pages_after;
+        __syncthreads();             // (weights and stats have been read)
+    }
+    wild = __any(wild);
+    if (lane == 0u) lds_wild[wave] = wild ? 1.f : 0.f;
+    float *const others = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const float both = halves_add(l[i]);
+        if (h == 0u) stats[(wave * QT + i) * 32u] = both;
+        if (GROUPS > 1 && adds && g) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<tq_f4 *>(others + (((g - 1u) * QT + i) * 32u + n) * ROW + 32u * slice + 8u * k + 4u * h) = tq_f4{acc[i][4 * k], acc[i][4 * k + 1], acc[i][4 * k + 2], acc[i][4 * k + 3]};
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        if (g == 0u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                tq_f4 sum = tq_f4{acc[i][4 * k], acc[i][4 * k + 1], acc[i][4 * k + 2], acc[i][4 * k + 3]};
+#pragma unroll
+                for (int o = 0; o < GROUPS - 1; ++o) sum += *reinterpret_cast<const tq_f4 *>(others + ((o * QT + i) * 32u + n) * ROW + 32u * slice + 8u * k + 4u * h);
+                *reinterpret_cast<tq_f4 *>(J::sums(lds, 1u, i) + n * ROW + 32u * slice + 8u * k + 4u * h) = sum;
+            }
+        }
+        if (wave == (uint32_t)i && h == 0u) {
+            float total = 0.f;
+#pragma unroll
+            for (int w = 0; w < FAST_WAVES; ++w) total += stats[(w * QT + i) * 32];
+            J::largest(lds, 1u, i)[n] = m_ref[i];
+            J::total(lds, 1u, i)[n] = total;
+        }
+    }
+    __syncthreads();
+    float any = 0.f;
+#pragma unroll
+    for (int w = 0; w < FAST_WAVES; ++w) any += lds_wild[w];
+    if (any != 0.f) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < tiles; ++i) paged_wild<DP>(a, r, J::sums(lds, 1u, i), tile0 + i, from, to, tid);
+        __syncthreads();
     }
 }
 
@@ -799,9 +842,9 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
     }
     const bool plain = plain_to > plain_from;
     if (plain) {
-        if constexpr (VT == 2) paged_plain_phase<DP, QT, TQ_F32>(a, v, row, lds, lds_m, lds_l, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
-        else if (a.dtype == TQ_BF16) paged_plain_phase<DP, QT, TQ_BF16>(a, v, row, lds, lds_m, lds_l, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
-        else if constexpr (KT == 2) paged_plain_phase<DP, QT, TQ_F16>(a, v, row, lds, lds_m, lds_l, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
+        if constexpr (VT == 2) paged_plain_phase<DP, QT, TQ_F32>(a, v, row, lds, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
+        else if (a.dtype == TQ_BF16) paged_plain_phase<DP, QT, TQ_BF16>(a, v, row, lds, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
+        else if constexpr (KT == 2) paged_plain_phase<DP, QT, TQ_F16>(a, v, row, lds, lds_kn[0], tile0, tiles, plain_from, plain_to, tid);
     }
     const uint32_t i = wave / S::TILES;
     if (i >= tiles) return;
