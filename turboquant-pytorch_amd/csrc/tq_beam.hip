@@ -67,28 +67,57 @@ struct BeamList {
     uint32_t token[BEST_MAX + 64];
 };
 
-// The `best` of a list, in order, to its front; answers with the order of the last one.  Each in turn out of its lane's registers against all others.
+// The `best` of a list to its front, as they lie (in order they would fill every `best`'th place of the join's first groups alone: 32 of 16 beams x 262144 took 267 us instead of 56); answers
+// with the order of the last one.  Of few, each in turn out of its lane's registers against all others (24 cycles a candidate); of more, the n-th largest bit by bit, as above (60 cycles a bit; LOW: bits that the
+// logits' type leaves alike), and of those that equal it the ones of the lowest tokens, one by one: 16 x 8 x 128256 float32 logits 32.5 us by the first way alone, 28 with both; 4 x 32000 by the second alone 13.5 for 11.5.
+template <int LOW>
 __device__ __forceinline__ uint32_t keep_best(BeamList &list, uint32_t &count, uint32_t best, uint32_t lane) {
     wave_sync_lds();
     const uint32_t all = count;
     const float x0 = list.x[lane], x1 = list.x[64u + lane];
     const uint32_t t0 = list.token[lane], t1 = list.token[64u + lane];
-    uint32_t r0 = 0u, r1 = 0u;
-    const uint32_t k0 = beam_order(x0), k1 = beam_order(x1);
-    auto against = [&](uint32_t key, uint32_t token) __attribute__((always_inline)) {
-        r0 += key > k0 || (key == k0 && token < t0) ? 1u : 0u;
-        if (all > 64u) r1 += key > k1 || (key == k1 && token < t1) ? 1u : 0u;
-    };
-#pragma unroll 4
-    for (uint32_t j = 0; j < min(all, 64u); ++j) against((uint32_t)__builtin_amdgcn_readlane((int)k0, (int)j), (uint32_t)__builtin_amdgcn_readlane((int)t0, (int)j));
-#pragma unroll 4
-    for (uint32_t j = 64; j < all; ++j) against((uint32_t)__builtin_amdgcn_readlane((int)k1, (int)(j - 64u)), (uint32_t)__builtin_amdgcn_readlane((int)t1, (int)(j - 64u)));
-    wave_sync_lds();
-    if (lane < all && r0 < best) { list.x[r0] = x0; list.token[r0] = t0; }
-    if (64u + lane < all && r1 < best) { list.x[r1] = x1; list.token[r1] = t1; }
+    const uint32_t k0 = lane < all ? beam_order(x0) : 0u, k1 = 64u + lane < all ? beam_order(x1) : 0u;
     wave_sync_lds();
     count = min(all, best);
-    return count == best ? beam_order(list.x[best - 1u]) : 0u;
+    if (all <= best) return 0u;
+    bool in0, in1;
+    uint32_t last;
+    if (all <= 48u) {
+        uint32_t r0 = 0u;
+#pragma unroll 4
+        for (uint32_t j = 0; j < all; ++j) {
+            const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)k0, (int)j), token = (uint32_t)__builtin_amdgcn_readlane((int)t0, (int)j);
+            r0 += key > k0 || (key == k0 && token < t0) ? 1u : 0u;
+        }
+        in0 = lane < all && r0 < best;
+        in1 = false;
+        last = (uint32_t)__builtin_amdgcn_readlane((int)k0, __builtin_ctzll(__ballot(in0 && r0 + 1u == best)));
+    } else {
+        uint32_t left = all;             // at or above `last`
+        last = 0u;
+#pragma unroll 1
+        for (int bit = 31; bit >= LOW && left != best; --bit) {
+            const uint32_t with = last | (1u << bit), n = (uint32_t)__popcll(__ballot(k0 >= with)) + (uint32_t)__popcll(__ballot(k1 >= with));
+            if (n >= best) { last = with; left = n; }
+        }
+        in0 = k0 >= last;
+        in1 = k1 >= last;
+        if (left != best) {              // equal ones: those of them that come last are out
+            const uint32_t top = (LOW ? (1u << LOW) - 1u : 0u) | last;
+#pragma unroll 1
+            for (; left > best; --left) {
+                const uint32_t most = wave_max(max(in0 && k0 <= top ? t0 : 0u, in1 && k1 <= top ? t1 : 0u));
+                if (in0 && k0 <= top && t0 == most) in0 = false;
+                else if (in1 && k1 <= top && t1 == most) in1 = false;
+            }
+        }
+    }
+    const unsigned long long m0 = __ballot(in0), m1 = __ballot(in1);
+    const uint32_t to0 = lanes_before(m0), to1 = (uint32_t)__popcll(m0) + lanes_before(m1);
+    if (in0) { list.x[to0] = x0; list.token[to0] = t0; }
+    if (in1) { list.x[to1] = x1; list.token[to1] = t1; }
+    wave_sync_lds();
+    return last;
 }
 
 // Wave = part of a row, in chunks of 64 E logits that lie in registers, sixteen bytes a load, the next chunk's on their way meanwhile.  The n-th largest of the lanes' largest has n
@@ -96,7 +125,7 @@ __device__ __forceinline__ uint32_t keep_best(BeamList &list, uint32_t &count, u
 // Where ties leave more than fit (equal logits), the best of a chunk are taken one by one.
 template <int DT, int E>
 __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs a) {
-    constexpr int ES = DT == TQ_F32 ? 4 : 2, V = 16 / ES, LOADS = E / V;
+    constexpr int ES = DT == TQ_F32 ? 4 : 2, V = 16 / ES, LOADS = E / V, LOW = DT == TQ_F32 ? 0 : DT == TQ_F16 ? 13 : 16;
     constexpr uint32_t CHUNK = 64u * E;
     __shared__ BeamList lists[PART_WAVES];
     const uint32_t lane = threadIdx.x & 63u, wave = tq_uniform32(threadIdx.x >> 6), at = blockIdx.x * PART_WAVES + wave;
@@ -219,9 +248,9 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
             }
         }
         count += fresh;
-        if (count > 64u) bound = max(bound, keep_best(list, count, a.best, lane));
+        if (count > 64u) bound = max(bound, keep_best<LOW>(list, count, a.best, lane));
     }
-    if (count > a.best) keep_best(list, count, a.best, lane);
+    if (count > a.best) keep_best<LOW>(list, count, a.best, lane);
     wave_sync_lds();
     sum = reduce_wave(sum, OpAdd());
     if (lane == 0u) {
@@ -306,7 +335,6 @@ __global__ __launch_bounds__(JOIN_THREADS) void tq_beam_join_kernel(BeamArgs a) 
     each([&](const Choice &c) { most = max(most, beam_order((float)c.sum)); });
     lds_t[tid] = most;
     __syncthreads();
-    // (neighbours together: candidates lie best first, part after part, and the first ones of all parts are to be in groups of their own)
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) most = max(w ? most : 0u, lds_t[WAVES * lane + w]);
     const uint32_t least = max(nth_of_wave(most, a.best), 1u);
