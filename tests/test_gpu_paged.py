@@ -319,6 +319,69 @@ def test_large_logits(pkg):
         check(step.attend(q, 0, softcap=10.0), q, step, softcap=10.0) if dtype != BF else None
 
 
+def test_a_cap_far_above_the_logits(pkg):
+    # cap tanh(z / cap) is z (1 - (z / cap)^2 / 3): with |z| below 100 and a cap of 10^5 or more no different from z by 2^-21 of it, so weights by 2^-15 at most; what is left is which
+    # way a result is rounded (few, by 2^-7 or 2^-10 of themselves)
+    for dtype, most in ((BF, 1e-3), (F16, 2e-4), (F32, 2e-5)):
+        for new in (1, 20):
+            cache = make(pkg, 128, 2, dtype)
+            seqs = cache.add(2)
+            feed(cache, seqs, (500, 70), seed=1)
+            step = feed(cache, seqs, (new, new), seed=2, commit=False)
+            q = rand((2 * new, 8, 128), 3, dtype)
+            plain = step.attend(q, 0).double()
+            for cap in (1e5, 1e12, 2.0 ** 100):
+                assert (step.attend(q, 0, softcap=cap).double() - plain).norm() <= most * plain.norm()
+            for cap in (1025.0, 1024.0, 2000.0):
+                check(step.attend(q, 0, softcap=cap), q, step, softcap=cap)
+            small = step.attend(q, 0, softcap=2.0 ** -100).double()      # all logits are zero
+            assert bool(torch.isfinite(small).all())
+
+
+def test_a_step_that_is_taken_back(pkg):
+    cache, other = make(pkg), make(pkg)
+    kept = []
+    for c in (cache, other):
+        seqs = c.add(3)
+        feed(c, seqs, (100, 0, 63), seed=1)
+        if c is cache:
+            before = c.free_pages(), c.lengths(seqs), [c.tables(s) for s in seqs]
+            step = c.step(seqs, (200, 1, 65))
+            with pytest.raises(RuntimeError):
+                c.free(seqs)                     # (its commit lacks every layer)
+            step.cancel()
+            assert (c.free_pages(), c.lengths(seqs), [c.tables(s) for s in seqs]) == before
+            step.cancel()
+            with pytest.raises(RuntimeError):
+                step.append(states(266, 2, 128, 1, BF), states(266, 2, 128, 2, BF), 0)
+        step = feed(c, seqs, (1, 2, 130), seed=2, commit=False)
+        q = rand((133, 8, 128), 3, BF)
+        kept.append(step.attend(q, 0))
+        step.commit()
+        step.cancel()                            # (nothing: it is over)
+        assert c.lengths(seqs) == [101, 2, 193]
+    assert torch.equal(*kept)
+
+
+def test_a_recorded_step_outlives_its_name(pkg):
+    cache = make(pkg)
+    seqs = cache.add(2)
+    feed(cache, seqs, (300, 70), seed=1)
+    step = feed(cache, seqs, (1, 1), seed=2, commit=False)
+    q = rand((2, 8, 128), 3, BF)
+    want = step.attend(q, 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step.attend(q, 0)
+    step.commit()
+    del step
+    noise = [torch.full((1 << k,), 0x7fffffff, dtype=torch.int32, device=DEV) for k in range(4, 14) for _ in range(8)]       # (what has been given back is taken and overwritten)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and len(noise)
+
+
 def test_beams_fork_share_and_move(pkg):
     cache, kept = make(pkg, H=2, window=70, layers=2, plain=60), {}
     (a,) = cache.add(1)

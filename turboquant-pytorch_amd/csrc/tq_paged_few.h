@@ -448,8 +448,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
                 for (int j = 0; j < SPL; ++j) asm volatile("" : "+v"(z[j]));        // (rounded here, not fused with what is taken off)
                 if (shaped) {
                     if (a.cap != 0.f) {
-#pragma unroll
-                        for (int j = 0; j < SPL; ++j) z[j] = cap.template operator()<false>(z[j]);
+                        cap.template all<false>(z, SPL);
                     }
                     const float first = (float)((int)(t0 + tok) - (int)pos);
 #pragma unroll
@@ -624,8 +623,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= a.scale * LOG2E;
             if (a.cap != 0.f) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = cap.template operator()<false>(x[j]);
+                cap.template all<false>(x, 8);
             }
             float top = m_ref;
 #pragma unroll

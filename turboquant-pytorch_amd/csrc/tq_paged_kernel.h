@@ -12,19 +12,31 @@ struct PagedRow {
     uint32_t fresh, total, packed, kv;
 };
 
-// Base-2 logits after the cap: C tanh(z / C) = C - 2 C / (1 + 2^(2 z / cap)), C = cap log2 e.  The difference leaves some 2^-23 C of a logit; where products are as exact as float32 (EXACT) small
-// ones come from the series.  (Five instructions, two of them at a quarter of the rate; with series and selection for all, a chunk of 512 tokens over 32768 took 637 us instead of 374 without a cap.)
+// Base-2 logits after the cap: C tanh(z / C) = C - 2 C / (1 + 2^(2 z / cap)), C = cap log2 e.  The difference leaves some 2^-22 C of a logit; where that counts (products as exact as float32,
+// or a cap past 1024: `wide`) small ones come from the series.  (Five instructions, two of them at a quarter of the rate; with series and selection for all, a chunk of 512 tokens over 32768
+// took 637 us instead of 374 without a cap.)
 struct Cap {
     float rate, c;
-    __device__ __forceinline__ explicit Cap(const TqPagedArgs &a) : rate(a.cap != 0.f ? 2.f / a.cap : 0.f), c(a.cap * LOG2E) {}
+    bool wide;
+    __device__ __forceinline__ explicit Cap(const TqPagedArgs &a) : rate(a.cap != 0.f ? 2.f / a.cap : 0.f), c(a.cap * LOG2E), wide(a.cap > 1024.f) {}
     template <bool EXACT>
-    __device__ __forceinline__ float operator()(float z) const {
+    __device__ __forceinline__ float one(float z) const {
         const float large = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * rate)), c);
         if constexpr (!EXACT) return large;
         else {
-            const float y = z / c, y2 = y * y;
+            const float y = z * (0.34657359027997265f * rate), y2 = y * y;          // (z / c: half a log 2)
             const float small = z * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
             return fabsf(y) < 0.3f ? small : large;
+        }
+    }
+    template <bool EXACT, typename X>
+    __device__ __forceinline__ void all(X &x, int n) const {
+        if (EXACT || wide) {
+#pragma unroll
+            for (int j = 0; j < n; ++j) x[j] = one<true>(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < n; ++j) x[j] = one<false>(x[j]);
         }
     }
 };
@@ -209,10 +221,7 @@ __device__ __forceinline__ void paged_plain_phase(const TqPagedArgs &a, const Tq
                 const uint32_t gone = (unseen_bits(at, pos[i], a.window) | (valid < 32u ? ~0u << valid : 0u)) >> (4u * h);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) x[i][j] = s[i][j] * (a.scale * LOG2E);
-                if (a.cap != 0.f) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) x[i][j] = cap.template operator()<F32>(x[i][j]);
-                }
+                if (a.cap != 0.f) cap.template all<F32>(x[i], 16);
                 if (a.slopes) {
                     const float first = (float)((int)(at + 4u * h) - (int)pos[i]);
 #pragma unroll
@@ -719,9 +728,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
                 }
                 if (a.cap != 0.f) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-#pragma unroll
-                        for (int i = 0; i < QT; ++i) s[i][r] = cap.template operator()<VT == 2>(s[i][r]);
+                    for (int i = 0; i < QT; ++i) cap.template all<VT == 2>(s[i], 16);
                 }
                 if (a.slopes) {
 #pragma unroll

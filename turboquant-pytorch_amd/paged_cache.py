@@ -11,7 +11,7 @@ A step gives sequences new tokens, one each (decoding) or many (chunks of prompt
     for layer in ...:
         step.append(keys, values, layer)            # [new tokens, kv heads, D], sequence after sequence
         out = step.attend(queries, layer)           # [new tokens, query heads, D], causal
-    step.commit()                                   # pages that have become old enough are packed
+    step.commit()                                   # pages that have become old enough are packed (or step.cancel(): the tokens are taken back)
 
 The step's own tokens are attended to as they are; what is packed, and with which codec, is as in `V3Cache` (the reference's generation-time cache,
 turboquant/generation_test_v2.py:48-165), but a page at a time.  Lengths and tables live on the host.
@@ -118,6 +118,7 @@ class PagedV3Cache:
         self._seqs: Dict[int, _Sequence] = {}
         self._next = 0
         self._open: Optional[PagedStep] = None
+        self._recorded: List[PagedStep] = []         # into graphs
 
     def _pools(self, pages: int, plain_pages: int) -> Tuple[torch.Tensor, torch.Tensor]:
         return (torch.empty((pages, self._page_bytes), dtype=torch.uint8, device=self.device),
@@ -322,37 +323,38 @@ class PagedV3Cache:
         """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered, sequence after sequence."""
         self._eager("resize")
         self._settle()
-        states = list(self._seqs.values())
         # the pages that are held, as the sequences have them: a page's place here is its number in the new pool
-        lists = [[s.pages for s in states], [s.plain for s in states]]
+        lists = [[s.pages for s in self._seqs.values() if s.pages], [s.plain for s in self._seqs.values() if s.plain]]
         orders = [list(dict.fromkeys(chain.from_iterable(of))) for of in lists]
+        held = [len(order) for order in orders]
         sizes = []
-        for name, asked, order in zip(("pages", "plain_pages"), (pages, plain_pages), orders):
-            n = max(1, len(order)) if asked is None else asked
-            if isinstance(n, bool) or int(n) != n or n < max(1, len(order)):
-                raise ValueError(f"resize: {name} must be a whole number, {max(1, len(order))} or more (as many are held); got {n!r}")
-            sizes.append(int(n))
+        for name, asked, n in zip(("pages", "plain_pages"), (pages, plain_pages), held):
+            size = max(1, n) if asked is None else asked
+            if isinstance(size, bool) or int(size) != size or size < max(1, n):
+                raise ValueError(f"resize: {name} must be a whole number, {max(1, n)} or more (as many are held); got {size!r}")
+            sizes.append(int(size))
         pool, plain = self._pools(*sizes)
-        vector = self.head_dim * self._plain.element_size()
+        stream, vector = torch.cuda.current_stream(self.device), self.head_dim * self._plain.element_size()
         for source, target, order, rows, row_bytes in ((self._pool, pool, orders[0], 1, self._page_bytes),
                                                        (self._plain, plain, orders[1], self.n_layers * 2 * self.kv_heads, self.page_tokens * vector)):
             if order:
                 _native.copy_pages(source, target, rows, row_bytes, order)
-            source.record_stream(torch.cuda.current_stream(self.device))         # (what it was allocated on may be another one)
+            source.record_stream(stream)         # (what it was allocated on may be another one)
         self._pool, self._plain, self._views = pool, plain, None
         # (the copies run while the tables are brought in line)
-        pools = []
-        for old, of, order, size in zip((self._packed_pages, self._plain_pages), lists, orders, sizes):
+        pools, numbers = [], []
+        for old, of, order, n, size in zip((self._packed_pages, self._plain_pages), lists, orders, held, sizes):
             new = _Pages(0)
-            new.held = list(map(old.held.__getitem__, order)) + [0] * (size - len(order))
-            new.free = list(range(len(order), size))
+            new.held = [old.held[p] for p in order] + [0] * (size - n)
+            new.free = list(range(n, size))
             pools.append(new)
-            number = dict(zip(order, range(len(order))))
+            number = dict(zip(order, range(n)))
+            numbers.append(number)
             for pages_of in of:
-                if pages_of:
-                    pages_of[:] = map(number.__getitem__, pages_of)
-            self._packed_of = {(p if old is self._packed_pages else number[p]): (number[q] if old is self._packed_pages else q) for p, q in self._packed_of.items()}
+                pages_of[:] = [number[p] for p in pages_of]
         self._packed_pages, self._plain_pages = pools
+        if self._packed_of:
+            self._packed_of = {numbers[1][p]: numbers[0][q] for p, q in self._packed_of.items()}
 
     # ---- steps ----------------------------------------------------------------------------------------------------------------
     def step(self, seqs: Sequence[int], counts) -> "PagedStep":
@@ -376,11 +378,12 @@ class PagedV3Cache:
 
 class PagedStep:
     """New tokens of some sequences of a `PagedV3Cache`: `append` for every layer, `attend` where it is wanted, then `commit` (the next step or any other call that changes tables commits
-    what is open).  Where a graph is recorded, the step has to be made before, and `attend` called once with the same window before the recording; replays work on the step's tokens."""
+    what is open).  Where a graph is recorded, the step has to be made before, and `attend` called once with the same window before the recording; replays work on the step's tokens, until `resize` gives the
+    cache other pools."""
 
     def __init__(self, cache: PagedV3Cache, seqs, states, counts, need):
         self.cache, self.seqs, self.counts = cache, seqs, counts
-        self._states = states
+        self._states, self._pages_taken = states, need
         self.tokens = sum(counts)
         P = cache.page_tokens
         records = np.zeros((len(seqs), _native.PAGED_SEQ), dtype=np.int32)
@@ -424,7 +427,11 @@ class PagedStep:
     def _await(self, uploaded) -> None:
         """The upload is done before this stream goes on, and its memory stays while the stream reads it."""
         blob, event, stream = uploaded
-        if _native._stream_handle(self.cache.device) != stream and not torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing():
+            if self not in self.cache._recorded:
+                self.cache._recorded.append(self)        # (replays read its tables, whether the caller keeps it or not)
+            return
+        if _native._stream_handle(self.cache.device) != stream:
             current = torch.cuda.current_stream(self.cache.device)
             current.wait_event(event)
             blob.record_stream(current)
@@ -539,8 +546,8 @@ class PagedStep:
         heads, cap, window = queries.shape[1], 0.0, 0
         if softcap is not None:
             cap = float(softcap)
-            if not 0.0 < cap < float("inf"):
-                raise ValueError(f"attend: softcap must be a number above zero, got {softcap!r}")
+            if not 2.0 ** -100 <= cap <= 2.0 ** 100:
+                raise ValueError(f"attend: softcap must be a number above zero (2^-100 to 2^100), got {softcap!r}")
         if sliding_window is not None:
             if isinstance(sliding_window, bool) or int(sliding_window) != sliding_window or sliding_window < 1:
                 raise ValueError(f"attend: sliding_window must be a whole number, 1 or more; got {sliding_window!r}")
@@ -614,6 +621,21 @@ class PagedStep:
             del s.plain[:len(pages)]
             s.pages += pages
         c._forget()
+        self._done = True
+        if c._open is self:
+            c._open = None
+
+    def cancel(self) -> None:
+        """The step has not been: its tokens are taken back (what came in between, an error in a forward pass, leaves the sequences as they were)."""
+        if self._done:
+            return
+        c = self.cache
+        c._eager("cancel")
+        for s, count, pages in zip(self._states, self.counts, self._pages_taken):
+            s.total -= count
+            if pages:
+                c._plain_pages.drop_all(s.plain[-pages:])
+                del s.plain[-pages:]
         self._done = True
         if c._open is self:
             c._open = None
