@@ -571,7 +571,7 @@ int tq_put_tokens(const void *keys, const void *values, long long k_token_stride
  *               plain pages' numbers begin, two unused.  On the host for the plan, a copy on the device for the call, as items and merges
  *   packed_pool, plain_pool     the layer's part of page 0 (key codes; keys), from which the other parts and the other pages are so many bytes on
  *   queries     new token i, query head j at i * q_token + j * q_head elements; query head j reads kv head j / group.  out: dense [new tokens, heads * group, head_dim]
- *   softcap     0: none; otherwise, from 2^-100 to 2^100, logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
+ *   softcap     0: none; otherwise, from 2^-100 to 1024 (float32: 2^100), logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
  * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, then blocks + 1 (where each block's items
  * begin), in room for 8 * max_items; 8 a merge; counts also where they do not fit (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim, dtype and page_tokens.
  * tq_paged_scratch: float32 values of scratch (16-byte aligned, not shared by calls that can overlap in time).

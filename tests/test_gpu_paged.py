@@ -322,7 +322,7 @@ def test_large_logits(pkg):
 def test_a_cap_far_above_the_logits(pkg):
     # cap tanh(z / cap) is z (1 - (z / cap)^2 / 3): with |z| below 100 and a cap of 10^5 or more no different from z by 2^-21 of it, so weights by 2^-15 at most; what is left is which
     # way a result is rounded (few, by 2^-7 or 2^-10 of themselves)
-    for dtype, most in ((BF, 1e-3), (F16, 2e-4), (F32, 2e-5)):
+    for dtype, most in ((BF, 0.0), (F16, 0.0), (F32, 2e-5)):
         for new in (1, 20):
             cache = make(pkg, 128, 2, dtype)
             seqs = cache.add(2)
@@ -331,8 +331,12 @@ def test_a_cap_far_above_the_logits(pkg):
             q = rand((2 * new, 8, 128), 3, dtype)
             plain = step.attend(q, 0).double()
             for cap in (1e5, 1e12, 2.0 ** 100):
+                if dtype != F32:
+                    with pytest.raises(ValueError):
+                        step.attend(q, 0, softcap=cap)
+                    continue
                 assert (step.attend(q, 0, softcap=cap).double() - plain).norm() <= most * plain.norm()
-            for cap in (1025.0, 1024.0, 2000.0):
+            for cap in (1024.0, 700.0):
                 check(step.attend(q, 0, softcap=cap), q, step, softcap=cap)
             small = step.attend(q, 0, softcap=2.0 ** -100).double()      # all logits are zero
             assert bool(torch.isfinite(small).all())

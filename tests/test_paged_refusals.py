@@ -113,7 +113,7 @@ def test_attention_checks_its_request(pkg):
     assert L.tq_paged_scratch(None, 8, 128) == -1 and L.tq_paged_scratch(ctypes.byref(counts), 0, 128) == -5 and L.tq_paged_scratch(ctypes.byref(counts), 8, 7) == -3
     copy = lambda: native.TqPagedRequest.from_buffer_copy(r)  # noqa: E731
     for field, value, status in (("dtype", 3, -4), ("bits_k", 0, -2), ("bits_v", 9, -2), ("bits_k", 1, -3), ("head_dim", 100, -3), ("heads", 0, -5), ("group", 0, -5), ("page_tokens", 48, -5),
-                                 ("page_tokens", 16, -5), ("sliding_window", -1, -5), ("softcap", -1.0, -5), ("softcap", float("nan"), -5), ("softcap", float("inf"), -5), ("softcap", 1e-38, -5), ("softcap", 2e30, -5)):
+                                 ("page_tokens", 16, -5), ("sliding_window", -1, -5), ("softcap", -1.0, -5), ("softcap", float("nan"), -5), ("softcap", float("inf"), -5), ("softcap", 1e-38, -5), ("softcap", 1025.0, -5)):
         bad = copy()
         setattr(bad, field, value)
         assert L.tq_paged_attend(ctypes.byref(bad), 4096, 1 << 40, None) == status, field

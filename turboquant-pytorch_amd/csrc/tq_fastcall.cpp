@@ -659,7 +659,7 @@ PyObject *paged_attend(PyObject *const *a) {
     if (a[4] != Py_None) {
         const double cap = PyFloat_AsDouble(a[4]);
         if (PyErr_Occurred()) throw Raised{};
-        NEED(cap >= 0x1p-100 && cap <= 0x1p100);
+        NEED(cap >= 0x1p-100 && cap <= 1024.0);
         r.softcap = (float)cap;
     }
     if (PyErr_Occurred()) throw Raised{};

@@ -361,7 +361,7 @@ extern "C" int tq_paged_attend(const tq_paged_request *request, float *scratch, 
     if (r.heads < 1 || r.group < 1 || r.sliding_window < 0 || r.heads * (long long)r.group > 0x7fffffff) return TQ_ERR_SIZE;
     if (r.page_tokens < 32 || (r.page_tokens & (r.page_tokens - 1)) || r.page_tokens > 65536) return TQ_ERR_SIZE;
     if (r.page_tokens > 0x7fffffff / r.heads / (r.head_dim * 4)) return TQ_ERR_SIZE;
-    if (!(r.softcap == 0.f || (r.softcap >= 0x1p-100f && r.softcap <= 0x1p100f)) || n.items < 0 || n.merges < 0 || n.records < 0) return TQ_ERR_SIZE;
+    if (!(r.softcap == 0.f || (r.softcap >= 0x1p-100f && r.softcap <= (r.dtype == TQ_F32 ? 0x1p100f : 1024.f))) || n.items < 0 || n.merges < 0 || n.records < 0) return TQ_ERR_SIZE;
     if (n.items == 0) return TQ_OK;
     if (n.few < 0 || n.few > n.items || n.blocks < 0 || n.blocks > 0x7fffffff || (n.few && (n.blocks < 1 || n.vectors < 1 || n.vectors > 16 || r.dtype == TQ_F32 || r.page_tokens < 64 || (r.head_dim & 31)))) return TQ_ERR_SIZE;
     if (n.items > 0x7fffffff / r.heads || n.tiles < 1 || n.tiles > 2 || n.columns < 1 || n.columns > 32) return TQ_ERR_SIZE;

@@ -12,13 +12,12 @@ struct PagedRow {
     uint32_t fresh, total, packed, kv;
 };
 
-// Base-2 logits after the cap: C tanh(z / C) = C - 2 C / (1 + 2^(2 z / cap)), C = cap log2 e.  The difference leaves some 2^-22 C of a logit; where that counts (products as exact as float32,
-// or a cap past 1024: `wide`) small ones come from the series.  (Five instructions, two of them at a quarter of the rate; with series and selection for all, a chunk of 512 tokens over 32768
+// Base-2 logits after the cap: C tanh(z / C) = C - 2 C / (1 + 2^(2 z / cap)), C = cap log2 e.  The difference leaves some 2^-22 C of a logit (so that caps of 16-bit elements end at 1024); where products
+// are as exact as float32 (EXACT) small ones come from the series.  (Five instructions, two of them at a quarter of the rate; with series and selection for all, a chunk of 512 tokens over 32768
 // took 637 us instead of 374 without a cap.)
 struct Cap {
     float rate, c;
-    bool wide;
-    __device__ __forceinline__ explicit Cap(const TqPagedArgs &a) : rate(a.cap != 0.f ? 2.f / a.cap : 0.f), c(a.cap * LOG2E), wide(a.cap > 1024.f) {}
+    __device__ __forceinline__ explicit Cap(const TqPagedArgs &a) : rate(a.cap != 0.f ? 2.f / a.cap : 0.f), c(a.cap * LOG2E) {}
     template <bool EXACT>
     __device__ __forceinline__ float one(float z) const {
         const float large = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * rate)), c);
@@ -31,13 +30,8 @@ struct Cap {
     }
     template <bool EXACT, typename X>
     __device__ __forceinline__ void all(X &x, int n) const {
-        if (EXACT || wide) {
 #pragma unroll
-            for (int j = 0; j < n; ++j) x[j] = one<true>(x[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < n; ++j) x[j] = one<false>(x[j]);
-        }
+        for (int j = 0; j < n; ++j) x[j] = one<EXACT>(x[j]);
     }
 };
 

@@ -520,7 +520,7 @@ class PagedStep:
     def attend(self, queries: torch.Tensor, layer_idx: int, scale: Optional[float] = None, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
                sliding_window: Optional[int] = None) -> torch.Tensor:
         """softmax(z) V of the new tokens' queries, [new tokens, query heads, D] -> the same shape and type: a new token sees everything its sequence holds before it and itself.
-        Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap is given, less
+        Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap (up to 1024 for 16-bit elements) is given, less
         slopes[query head] * distance if slopes (float [query heads]) are; sliding_window: only the last so many tokens, the new one among them, are seen.
         Every layer has to be appended to before (the step's own tokens are read from its pages).  Not differentiable."""
         ready = self._quick.get((layer_idx, sliding_window))
@@ -546,8 +546,8 @@ class PagedStep:
         heads, cap, window = queries.shape[1], 0.0, 0
         if softcap is not None:
             cap = float(softcap)
-            if not 2.0 ** -100 <= cap <= 2.0 ** 100:
-                raise ValueError(f"attend: softcap must be a number above zero (2^-100 to 2^100), got {softcap!r}")
+            if not 2.0 ** -100 <= cap <= (2.0 ** 100 if c.dtype == torch.float32 else 1024.0):         # (what a cap far above the logits leaves of them has too few bits there)
+                raise ValueError(f"attend: softcap must be a number above zero, up to 1024 for 16-bit elements; got {softcap!r}")
         if sliding_window is not None:
             if isinstance(sliding_window, bool) or int(sliding_window) != sliding_window or sliding_window < 1:
                 raise ValueError(f"attend: sliding_window must be a whole number, 1 or more; got {sliding_window!r}")
