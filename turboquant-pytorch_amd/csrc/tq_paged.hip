@@ -75,14 +75,15 @@ bool supported(int D, int dtype, int bits_k, int bits_v) {
     return D > 64 && D <= 96 && !(D & 7) && !(D % ik) && !(D % iv) && !(D / ik & 3) && !(D / iv & 3);
 }
 
-// Times in quarters of a token of the kernel for one tile of 32 query vectors: what a block's packed tokens, its uncompressed ones and its start and end take.
+// Times in quarters of a token of the kernel for one tile of 32 query vectors (14 cycles): what a block's packed tokens, its uncompressed ones and its start and end take.  (Clocked 128 wide: two tiles
+// 22 cycles a packed token, 45 an uncompressed one, 50 thousand for start, joins and end.)
 struct Costs {
     long long token, plain, block;
 };
 Costs costs(int qt, int dtype) {
-    if (dtype == TQ_F32) return {12, 24, 6000};
-    if (qt == 2) return {6, 14, 8000};
-    return {4, 8, 6000};
+    if (dtype == TQ_F32) return {12, 24, 10000};
+    if (qt == 2) return {6, 14, 14000};
+    return {4, 10, 10000};
 }
 
 struct Reach {                       // what a group of tiles sees of its sequence, in runs
@@ -143,7 +144,7 @@ void share(Shares &best, std::vector<Group> &groups, int qt, int dtype, int head
         const long long rounds = (blocks + cus - 1) / cus;
         long long time = rounds * (all / blocks);
         if (time < piece + c.block) time = piece + c.block;
-        if (pieces > 1) time += 6000 + 120 * pieces;
+        if (pieces > 1) time += 4000 + 120 * pieces;
         if (best.time < 0 || time < best.time) { best.time = time; best.piece = piece; best.qt = qt; better = true; }
         if (rounds > 16 && k > 1) break;
     }
@@ -163,9 +164,9 @@ struct Plan {
 };
 
 // Sequences with few query vectors: the rows (sequence, kv head) of a launch laid end to end and cut into as many equal shares as there are blocks, one a compute unit; a row that is cut is
-// merged.  Or, where that takes less time, whole rows dealt out, the longest first to the block that has least.  Times in packed tokens of a block (4 ns; 64 ... 128 x 2048 x 8 heads: 25.0 us
-// without cuts, 21.0 with 64 blocks; 8 rows of 32768: 151 with 8 blocks, 30 with 128, 25 with 192): an uncompressed one three, an item 1100, a merge 1200 and 25 a piece.
-constexpr long long FEW_PLAIN = 3, FEW_ITEM = 1100, FEW_MERGE = 1200, FEW_PIECE = 25, FEW_LEAST = 512;
+// merged.  Or, where that takes less time, whole rows dealt out, the longest first to the block that has least.  Times in packed tokens of a block (4.6 ns: 64 x 16384 x 8 heads of 128 186 us, 64 x 8192
+// 110): an uncompressed one three, an item's start and end 2000 (33 sequences of 500 to 16384 tokens 66 us; with 1100, 77), a merge 1200 and 25 a piece.  One sequence of 32768: 25 us in 256 shares, 151 uncut.
+constexpr long long FEW_PLAIN = 3, FEW_ITEM = 2000, FEW_MERGE = 1200, FEW_PIECE = 25, FEW_LEAST = 512;
 void plan_few(Plan &p, std::vector<Group> &groups, int heads, int cus, const int32_t *sequences, int group) {
     long long all = 0, longest = 0;
     for (Group &g : groups) {

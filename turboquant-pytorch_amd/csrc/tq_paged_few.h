@@ -116,6 +116,8 @@ struct FewPlain {
     }
 };
 
+// Bound by reading (64 x 16384 tokens x 8 heads of 128, 4- and 2-bit codes: 839 MB in 186 us, 4.5 TB/s; 32 x 16384 x 8 of 256: 198 us), in short rows by an item's start and end (128 x 2048: 87 us), where one
+// block a compute unit has nothing to overlap them with.
 // A block takes items of the plan in turn, each a share of what the queries of a (sequence, kv head) see; the tables stay in LDS.  Up to 16 / C query vectors are the columns of 16 x 16 x 32 products, C times over, so that C blocks of 16 tokens share a softmax: every block's
 // scores are made for all columns, a lane keeps those of its own column's block, and the weights of the others are zeros in its column of the value product (as in tq_decode_kernel, whose
 // loop this is, with runs found through the sequence's pages: a run lies within a page, whose number is fetched a run ahead).  QT: fp16 terms of a rotated query, one for bfloat16 (two then, and two of the levels, for float16: with one the result of half a unit's
