@@ -116,7 +116,7 @@ struct FewPlain {
     }
 };
 
-// Bound by reading (64 x 16384 tokens x 8 heads of 128, 4- and 2-bit codes: 839 MB in 186 us, 4.5 TB/s; 32 x 16384 x 8 of 256: 198 us), in short rows by an item's start and end (128 x 2048: 87 us), where one
+// Bound by reading (64 x 16384 tokens x 8 heads of 128, 4- and 2-bit codes: 839 MB in 186 us, 4.5 TB/s; 32 x 16384 x 8 of 256: 198 us), in short rows by an item's start and end (128 x 2048: 79 us, and 86 with a way back for every item by itself), where one
 // block a compute unit has nothing to overlap them with.
 // A block takes items of the plan in turn, each a share of what the queries of a (sequence, kv head) see; the tables stay in LDS.  Up to 16 / C query vectors are the columns of 16 x 16 x 32 products, C times over, so that C blocks of 16 tokens share a softmax: every block's
 // scores are made for all columns, a lane keeps those of its own column's block, and the weights of the others are zeros in its column of the value product (as in tq_decode_kernel, whose
@@ -137,8 +137,9 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     constexpr int QROW = D + 4;
     // LDS: tables; values of each wave, rotated queries; the waves' sums of packed tokens and of plain ones, and the joined ones.  Where that is more than there is, the waves' sums lie over values and
     // queries, take turns, and cost barriers.
-    constexpr uint32_t V_AT = 65536u, Q_AT = V_AT + DW * VBYTES, LOOP_END = Q_AT + 16u * QROW * 4u, JOIN = DW * HR * PART * 4u, SUMS = HEADS * QROW * 4u, STATS = 4u * HEADS * 4u;
-    constexpr bool SIDE = HR >= HEADS && LOOP_END + 2u * JOIN + 2u * SUMS + STATS + DW * RUN * 6u + (QT > QREG ? (QT - QREG) * SK * 1024u : 0u) + 1024u <= 163840u;
+    constexpr uint32_t V_AT = 65536u, Q_AT = V_AT + DW * VBYTES, LOOP_END = Q_AT + 16u * QROW * 4u, JOIN = DW * HR * PART * 4u;
+    constexpr bool SIDE = HR >= HEADS && LOOP_END + 2u * JOIN + 2u * 16u * QROW * 4u + 4u * 16u * 4u + DW * RUN * 6u + (QT > QREG ? (QT - QREG) * SK * 1024u : 0u) + 1280u <= 163840u;
+    constexpr uint32_t COLS = SIDE ? 16u : HEADS, SUMS = COLS * QROW * 4u, STATS = 4u * COLS * 4u;          // columns that joined sums are held of
     constexpr uint32_t JOIN_AT = SIDE ? LOOP_END : V_AT, SUMS_AT = JOIN_AT + (SIDE ? 2u : 1u) * JOIN, STATS_AT = SUMS_AT + 2u * SUMS, JOIN_END = STATS_AT + STATS;
     constexpr uint32_t AREA = LOOP_END > JOIN_END ? LOOP_END : JOIN_END;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[AREA];
@@ -148,6 +149,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     __shared__ __attribute__((aligned(16))) float lds_corr[DW][16];
     __shared__ uint32_t lds_trips[DW];
     __shared__ float lds_wild[DW];
+    __shared__ uint32_t lds_item[C][4];              // of the items whose sums are held: first query token, kv head, query vectors, record
 
     {
         const uint32_t tid = threadIdx.x;
@@ -162,6 +164,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     }
     const int32_t first_item = a.blocks[blockIdx.x], end_item = a.blocks[blockIdx.x + 1];
     uint32_t trips = 0u;
+    bool turned = false;                     // whether any of the items whose sums are held has packed tokens
 #pragma unroll 1
     for (int32_t index = first_item; index < end_item; ++index) {
     uint32_t tid = threadIdx.x;
@@ -182,7 +185,9 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
     const bool live = head < M;
     const uint32_t vector = min(head, M - 1u), token = vector / a.group, pos = row.total - row.fresh + token;        // of this lane's column
     const float slope = a.slopes ? a.slopes[row.kv * a.group + (vector - token * a.group)] * LOG2E : 0.f;
-    float *const sums = reinterpret_cast<float *>(lds + SUMS_AT), *const stats = reinterpret_cast<float *>(lds + STATS_AT);       // [packed, plain][HEADS][QROW]; [largest, total][HEADS] of each
+    // [packed, plain][COLS][QROW]; [largest, total of packed, of plain][COLS]: HEADS columns an item, of as many items as there is a way back for at a time (SIDE)
+    const uint32_t slot = SIDE ? (uint32_t)((index - first_item) % C) : 0u;
+    float *const sums = reinterpret_cast<float *>(lds + SUMS_AT) + slot * (HEADS * QROW), *const stats = reinterpret_cast<float *>(lds + STATS_AT) + slot * HEADS;
 
     // The waves' sums meet in LDS, HR columns from h0 on (which: 0 packed, 1 plain).  put(): unit: what this wave's value sums are multiplied by, l: all lanes' of a column
     auto put = [&](uint32_t which, uint32_t h0, float m_ref, float l, float unit, const tq_f4v (&acc)[NC]) __attribute__((always_inline)) {
@@ -220,7 +225,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             }
         }
     };
-    // of the first `waves`
+    // of the first `waves` (none: zeros)
     auto combine = [&](uint32_t which, uint32_t h0, uint32_t waves) __attribute__((always_inline)) {
         const float *all = reinterpret_cast<const float *>(lds + JOIN_AT + (SIDE ? which * JOIN : 0u));
         for (uint32_t i = tid; i < min((uint32_t)HR, M - h0) * D; i += DTHREADS) {
@@ -238,8 +243,8 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
             }
             sums[which * (SUMS / 4u) + (h0 + col) * QROW + d] = sum;
             if (d == 0u) {
-                stats[(2u * which) * HEADS + h0 + col] = m;
-                stats[(2u * which + 1u) * HEADS + h0 + col] = total;
+                stats[(2u * which) * COLS + h0 + col] = m;
+                stats[(2u * which + 1u) * COLS + h0 + col] = total;
             }
         }
     };
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         }
         __syncthreads();
     }
-    const uint32_t q_row = (SIDE ? (uint32_t)((index - first_item) % C) * HEADS : 0u) + head;
+    const uint32_t q_row = slot * HEADS + head;
 
     if (t_end > t_begin) {
         const uint32_t lo = a.window && pos >= a.window ? pos - a.window + 1u : 0u;              // first token that this lane's column sees
@@ -660,9 +665,18 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         else join(1u, m_ref, l, 1.f, acc);
     }
     __syncthreads();
+    turned = packed || (slot && turned);
     if constexpr (SIDE) {
-        if (packed) combine(0u, 0u, DW);
-        if (plain) combine(1u, 0u, DW);
+        combine(0u, 0u, packed ? DW : 0u);
+        combine(1u, 0u, plain ? DW : 0u);
+    } else {
+        for (uint32_t h0 = 0; h0 < (uint32_t)HEADS && h0 < M; h0 += HR) {
+            if (!packed) combine(0u, h0, 0u);
+            if (!plain) combine(1u, h0, 0u);
+        }
+    }
+    if (tid == 0u) {
+        lds_item[slot][0] = q_first; lds_item[slot][1] = row.kv; lds_item[slot][2] = M; lds_item[slot][3] = (uint32_t)record;
     }
     if (plain) {
         float any = 0.f;
@@ -674,16 +688,16 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
         }
     }
     __syncthreads();
-    if (wave < (uint32_t)TILES) {
+    // The way back, of up to C items at a time (9000 cycles of four waves, whose operands come from memory)
+    if (wave < (uint32_t)TILES && (!SIDE || slot == C - 1u || index + 1 == end_item)) {
         // (32 columns to an instruction: the sixteen twice)
-        const uint32_t col = lane & (uint32_t)(HEADS - 1);
-        JoinedColumn j;
-        j.packed = packed ? sums + col * QROW : nullptr;
-        j.plain = plain ? sums + SUMS / 4u + col * QROW : nullptr;
-        j.m0 = packed ? stats[col] : MANY_NONE; j.l0 = packed ? stats[HEADS + col] : 0.f;
-        j.m1 = plain ? stats[2 * HEADS + col] : MANY_NONE; j.l1 = plain ? stats[3 * HEADS + col] : 0.f;
-        TQ_GLOBAL float *rec = record < 0 ? nullptr : (TQ_GLOBAL float *)a.rec + (size_t)record * a.qt * paged_record(a.cols, D);
-        paged_finish<D>(a, j, row, q_first, rec, col, col, (lane & 31u) < M && (lane & 31u) < (uint32_t)HEADS, wave, lane);
+        const uint32_t col = lane % COLS, its = col / HEADS, vec = col % HEADS;
+        const float *const s0 = sums - slot * (HEADS * QROW) + col * QROW, *const t0 = stats - slot * HEADS + col;
+        const JoinedColumn j{turned ? s0 : nullptr, s0 + SUMS / 4u, t0[0], t0[COLS], t0[2u * COLS], t0[3u * COLS]};
+        const bool some = (lane & 31u) < COLS && its <= slot && vec < lds_item[its][2];
+        const int to = (int)lds_item[its][3];
+        TQ_GLOBAL float *rec = to < 0 ? nullptr : (TQ_GLOBAL float *)a.rec + (size_t)to * a.qt * paged_record(a.cols, D);
+        paged_finish<D>(a, j, lds_item[its][1], lds_item[its][0], rec, vec, vec, some, wave, lane);
     }
     }
 }

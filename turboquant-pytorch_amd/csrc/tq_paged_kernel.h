@@ -408,7 +408,7 @@ struct JoinedColumn {
 // A wave's 32 coordinates of 32 columns' results: packed sums turned back by Pi_v (two fp16 terms each), the plain ones added; divided by the sum of weights into the result of query vector q, or as they are into
 // column `col` of the record.  `some`: whether the lane's column is one.
 template <int DP>
-__device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedColumn &j, const PagedRow &row, uint32_t q_first, TQ_GLOBAL float *rec, uint32_t q, uint32_t col, bool some,
+__device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedColumn &j, uint32_t kv, uint32_t q_first, TQ_GLOBAL float *rec, uint32_t q, uint32_t col, bool some,
                                              uint32_t w, uint32_t lane) {
     constexpr int STEPS = DP / 16, CH = STEPS < 8 ? STEPS : 8;
     const uint32_t h = lane >> 5;
@@ -460,7 +460,7 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedC
     if (!rec) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[r] = inv == 0.f ? 0.f : out[r] * inv;
-        paged_store(a, q_first, row.kv, q, d0, out);
+        paged_store(a, q_first, kv, q, d0, out);
         return;
     }
     if (w == 0u && h == 0u) { rec[col] = m; rec[a.cols + col] = l; }
@@ -857,7 +857,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
     j.m1 = plain ? J::largest(lds, 1u, i)[n] : MANY_NONE; j.l1 = plain ? J::total(lds, 1u, i)[n] : 0.f;
     const uint32_t q = (tile0 + i) * 32u + n;
     TQ_GLOBAL float *rec = record < 0 ? nullptr : (TQ_GLOBAL float *)a.rec + (((size_t)record + row.kv) * a.qt + i) * paged_record(a.cols, DP);
-    paged_finish<DP>(a, j, row, q_first, rec, q, n, record < 0 ? q < v.M : n < a.cols, wave % S::TILES, lane);
+    paged_finish<DP>(a, j, row.kv, q_first, rec, q, n, record < 0 ? q < v.M : n < a.cols, wave % S::TILES, lane);
 }
 
 template <int DP, int IPBK, int IPBV>
