@@ -223,6 +223,44 @@ def test_values_that_are_no_numbers_in_a_long_prompt(pkg):
         assert bool(torch.isfinite(out[433:500]).all()) and bool(torch.isinf(out[333:433, :, 5]).all()) and bool(torch.isfinite(out[501:599, :, 5]).all())
 
 
+@pytest.mark.parametrize("D,G,dtype,kb,vb,new", [(64, 71, BF, 4, 2, (1, 3, 1)), (128, 40, F16, 4, 2, (1, 1, 2)), (256, 33, BF, 4, 2, (1, 2, 1)), (80, 64, F32, 4, 4, (2, 1, 1)), (128, 128, BF, 8, 8, (1, 1, 1)),
+                                                 (96, 17, F16, 4, 4, (1, 1, 1))])
+def test_many_query_heads_of_one_kv_head(pkg, D, G, dtype, kb, vb, new):
+    cache = make(pkg, D, 1, dtype, kb, vb, 30, pages=64, plain=40)
+    seqs = cache.add(3)
+    feed(cache, seqs, (2000, 0, 95), seed=1)
+    step = feed(cache, seqs, new, seed=2, commit=False)
+    q = rand((sum(new), G, D), 3, dtype)
+    check(step.attend(q, 0), q, step)
+    check(step.attend(q, 0, sliding_window=1000), q, step, sliding_window=1000)
+
+
+def test_threads_and_steps_at_once(pkg):
+    import threading
+    caches, steps, qs, wants = [], [], [], []
+    for k in range(4):
+        cache = make(pkg, 128, 4, BF if k % 2 else F16, pages=80, plain=80)
+        seqs = cache.add(5)
+        feed(cache, seqs, (900, 3, 64, 2500, 0), seed=k)
+        step = feed(cache, seqs, (1, 1, 20, 1, 70), seed=10 + k, commit=False)
+        q = rand((93, 16, 128), k, cache.dtype)
+        caches.append(cache); steps.append(step); qs.append(q); wants.append(step.attend(q, 0))
+    got = [[] for _ in range(4)]
+
+    def work(k):
+        stream = torch.cuda.Stream(DEV) if k % 2 else torch.cuda.current_stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[k].append(steps[k].attend(qs[k], 0))
+            stream.synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert all(len(g) == 20 and all(torch.equal(x, w) for x in g) for g, w in zip(got, wants))
+
+
 def test_scale_and_layouts_of_queries(pkg):
     cache = make(pkg, H=2, layers=2, protected_layers=1)            # (8 bits in both)
     seqs = cache.add(2)
