@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 8;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 9;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -47,6 +47,7 @@ struct Entries {
     decltype(&tq_reorder) reorder;
     decltype(&tq_paged_attend) paged_attend;
     decltype(&tq_copy_pages) copy_pages;
+    decltype(&tq_put_tokens) put_tokens;
 } lib{};
 
 struct Raised {};        // a Python exception is set
@@ -625,6 +626,22 @@ PyObject *reorder(PyObject *const *a) {
     return PyLong_FromLong(launch(lib.reorder, (const tq_move_segment *)runs.data(), (int)runs.size(), B, H, (const long long *)address(parents), s.raw()));
 }
 
+// put_tokens(keys, values, uncompressed pool, layer, address of the slots, tokens, stream) -> status; pool: [pages, layers, keys and values, heads, page tokens, head dimension]; stream: the one
+// the slots were uploaded on
+PyObject *put_tokens(PyObject *const *a) {
+    TENSOR(k, a[0]); TENSOR(v, a[1]); TENSOR(pool, a[2]);
+    const long long layer = integer(a[3]), slots = integer(a[4]), tokens = integer(a[5]);
+    NEED(pool.dim() == 6 && layer >= 0 && layer < pool.size(1) && tokens > 0);
+    const long long es = (long long)pool.element_size(), heads = pool.size(3), dim = pool.size(5);
+    for (const at::Tensor *t : {&k, &v})
+        NEED(t->scalar_type() == pool.scalar_type() && t->device() == pool.device() && shape_is(*t, {tokens, heads, dim}) && t->stride(2) == 1 && t->stride(0) >= 0 && t->stride(1) >= 0);
+    const Stream s(pool);
+    NEED(s.ok && (long long)s.handle == integer(a[6]) && !s.capturing());
+    return PyLong_FromLong(launch(lib.put_tokens, (const void *)address(k), (const void *)address(v), (long long)k.stride(0) * es, (long long)k.stride(1) * es, (long long)v.stride(0) * es,
+                                  (long long)v.stride(1) * es, (void *)(address(pool) + layer * pool.stride(1) * es), (long long)pool.stride(0) * es, (long long)pool.stride(2) * es,
+                                  reinterpret_cast<const int32_t *>(slots), tokens, heads, dim * es, (int)pool.size(4), s.raw()));
+}
+
 // copy_pages(source pool, target pool, rows, bytes between rows, source pages, target pages or None (0, 1, ...), bytes of a row that are copied or None (all)) -> status; lists of whole
 // numbers, which the caller answers for
 PyObject *copy_pages(PyObject *const *a) {
@@ -728,7 +745,7 @@ PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
     TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 22), TQ_ENTRY(evict, 10),
-    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9), TQ_ENTRY(copy_pages, 7),
+    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9), TQ_ENTRY(copy_pages, 7), TQ_ENTRY(put_tokens, 7),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

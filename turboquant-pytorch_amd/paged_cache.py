@@ -445,10 +445,20 @@ class PagedStep:
             raise ValueError(f"layer_idx must be a whole number from 0 to {self.cache.n_layers - 1}, got {layer_idx!r}")
         return int(layer_idx)
 
-    @torch.compiler.disable
-    @torch.no_grad()
     def append(self, keys: torch.Tensor, values: torch.Tensor, layer_idx: int) -> None:
         """The new tokens' keys and values of a layer, [new tokens, kv heads, D], sequence after sequence in the step's order."""
+        if not self._done and type(layer_idx) is int and self.tokens and not torch.compiler.is_compiling():
+            status = _native.fast().put_tokens(keys, values, self.cache._plain, layer_idx, self._slot_at, self.tokens, self._blob[2])
+            if status is not None:
+                _native.check(status, "tq_put_tokens")
+                self._appended.add(layer_idx)
+                return
+        self._append(keys, values, layer_idx)
+
+    @torch.compiler.disable
+    @torch.no_grad()
+    def _append(self, keys: torch.Tensor, values: torch.Tensor, layer_idx: int) -> None:
+        """`append` with every check."""
         self._live("append")
         c, layer = self.cache, self._layer(layer_idx)
         shape = (self.tokens, c.kv_heads, c.head_dim)
