@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+from array import array
 from itertools import chain, groupby
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -65,9 +66,10 @@ class _Pages:
 
 
 class _Sequence:
+    """Its pages, as int32 (a step joins the tables of all its sequences), and tokens."""
     __slots__ = ("pages", "plain", "total")
 
-    def __init__(self, pages: List[int], plain: List[int], total: int):
+    def __init__(self, pages: array, plain: array, total: int):
         self.pages, self.plain, self.total = pages, plain, total
 
 
@@ -192,7 +194,7 @@ class PagedV3Cache:
         new = list(range(self._next, self._next + int(count)))
         self._next += int(count)
         for s in new:
-            self._seqs[s] = _Sequence([], [], 0)
+            self._seqs[s] = _Sequence(array("i"), array("i"), 0)
         return new
 
     def place(self, seqs: Sequence[int], packed: Sequence[int], plain: Sequence[int]) -> None:
@@ -206,8 +208,8 @@ class PagedV3Cache:
             raise ValueError(f"place: sequences must be empty, packed tokens a multiple of {self.page_tokens}")
         self._room("place", sum(p // self.page_tokens for p in packed), sum(-(-n // self.page_tokens) for n in plain))
         for s, p, n in zip(states, packed, plain):
-            s.pages = [self._packed_pages.take() for _ in range(p // self.page_tokens)]
-            s.plain = [self._plain_pages.take() for _ in range(-(-n // self.page_tokens))]
+            s.pages.extend(self._packed_pages.take() for _ in range(p // self.page_tokens))
+            s.plain.extend(self._plain_pages.take() for _ in range(-(-n // self.page_tokens)))
             s.total = int(p) + int(n)
 
     def _room(self, what: str, packed: int, plain: int) -> None:
@@ -351,7 +353,7 @@ class PagedV3Cache:
             number = dict(zip(order, range(n)))
             numbers.append(number)
             for pages_of in of:
-                pages_of[:] = [number[p] for p in pages_of]
+                pages_of[:] = array("i", [number[p] for p in pages_of])
         self._packed_pages, self._plain_pages = pools
         if self._packed_of:
             self._packed_of = {numbers[1][p]: numbers[0][q] for p, q in self._packed_of.items()}
@@ -386,20 +388,27 @@ class PagedStep:
         self._states, self._pages_taken = states, need
         self.tokens = sum(counts)
         P = cache.page_tokens
-        records = np.zeros((len(seqs), _native.PAGED_SEQ), dtype=np.int32)
-        tables, slots, at = [], [], 0
-        for i, (s, c, n) in enumerate(zip(states, counts, need)):
-            s.plain.extend(cache._plain_pages.take() for _ in range(n))
-            first = s.total - len(s.pages) * P
+        records, tables, singles, slots, at, begin = [], [], [], [], 0, 0
+        rest = (0,) * (_native.PAGED_SEQ - 6)
+        for s, c, n in zip(states, counts, need):
+            if n:
+                s.plain.extend(cache._plain_pages.take() for _ in range(n))
+            held = len(s.pages)
+            first = s.total - held * P
             s.total += c
-            places = np.arange(first, first + c)
-            slots.append(np.asarray(s.plain, dtype=np.int64)[places // P] * P + places % P if c else places)
-            begin = sum(map(len, tables))
-            records[i, :6] = at, c, s.total, len(s.pages) * P, begin, begin + len(s.pages)
+            if c == 1:
+                singles.append(s.plain[first // P] * P + first % P)
+            elif c:
+                places = np.arange(first, first + c)
+                slots += [np.array(singles, dtype=np.int64), np.array(s.plain, dtype=np.int64)[places // P] * P + places % P]
+                singles = []
+            records += (at, c, s.total, held * P, begin, begin + held, *rest)
             tables += [s.pages, s.plain]
+            begin += held + len(s.plain)
             at += c
-        self._records = records
-        self._sections = [records.ravel(), np.concatenate([np.asarray(t, dtype=np.int32) for t in tables] or [np.zeros(0, np.int32)]), np.concatenate(slots or [np.zeros(0)]).astype(np.int32)]
+        slots.append(np.array(singles, dtype=np.int64))
+        self._records = np.array(records, dtype=np.int32).reshape(len(seqs), _native.PAGED_SEQ)
+        self._sections = [self._records.ravel(), np.frombuffer(b"".join(tables), dtype=np.int32), np.concatenate(slots).astype(np.int32)]
         self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
         self._plans: Dict[Tuple[int, int], tuple] = {}
         self._ready: Dict[tuple, tuple] = {}
@@ -629,7 +638,7 @@ class PagedStep:
         for s, pages in moves:
             c._plain_pages.drop_all(s.plain[:len(pages)])
             del s.plain[:len(pages)]
-            s.pages += pages
+            s.pages.extend(pages)
         c._forget()
         self._done = True
         if c._open is self:
