@@ -326,8 +326,9 @@ class PagedV3Cache:
         self._eager("resize")
         self._settle()
         # the pages that are held, as the sequences have them: a page's place here is its number in the new pool
-        lists = [[s.pages for s in self._seqs.values() if s.pages], [s.plain for s in self._seqs.values() if s.plain]]
-        orders = [list(dict.fromkeys(chain.from_iterable(of))) for of in lists]
+        states = list(self._seqs.values())
+        flat = [np.frombuffer(b"".join([getattr(s, side) for s in states]), dtype=np.int32) for side in ("pages", "plain")]
+        orders = [list(dict.fromkeys(of.tolist())) for of in flat]
         held = [len(order) for order in orders]
         sizes = []
         for name, asked, n in zip(("pages", "plain_pages"), (pages, plain_pages), held):
@@ -344,19 +345,28 @@ class PagedV3Cache:
             source.record_stream(stream)         # (what it was allocated on may be another one)
         self._pool, self._plain, self._views = pool, plain, None
         # (the copies run while the tables are brought in line)
-        pools, numbers = [], []
-        for old, of, order, n, size in zip((self._packed_pages, self._plain_pages), lists, orders, held, sizes):
+        pools, numbers, tables = [], [], []
+        for old, of, order, n, size in zip((self._packed_pages, self._plain_pages), flat, orders, held, sizes):
             new = _Pages(0)
             new.held = [old.held[p] for p in order] + [0] * (size - n)
             new.free = list(range(n, size))
             pools.append(new)
-            number = dict(zip(order, range(n)))
+            number = np.zeros(len(old.held), dtype=np.int32)
+            number[order] = np.arange(n, dtype=np.int32)
             numbers.append(number)
-            for pages_of in of:
-                pages_of[:] = array("i", [number[p] for p in pages_of])
+            tables.append(array("i", number[of].tobytes()))
+        packed_at = plain_at = 0
+        for s in states:
+            k, n = len(s.pages), len(s.plain)
+            if k:
+                s.pages = tables[0][packed_at:packed_at + k]
+                packed_at += k
+            if n:
+                s.plain = tables[1][plain_at:plain_at + n]
+                plain_at += n
         self._packed_pages, self._plain_pages = pools
         if self._packed_of:
-            self._packed_of = {numbers[1][p]: numbers[0][q] for p, q in self._packed_of.items()}
+            self._packed_of = {int(numbers[1][p]): int(numbers[0][q]) for p, q in self._packed_of.items()}
 
     # ---- steps ----------------------------------------------------------------------------------------------------------------
     def step(self, seqs: Sequence[int], counts) -> "PagedStep":
