@@ -261,6 +261,30 @@ def test_threads_and_steps_at_once(pkg):
     assert all(len(g) == 20 and all(torch.equal(x, w) for x in g) for g, w in zip(got, wants))
 
 
+def test_layers_of_their_own_widths_and_codecs(pkg):
+    cache = make(pkg, 128, 2, BF, 4, 2, 20, layers=4, protected_layers=1, pages=40, plain=40)
+    assert len({(cache.codec(i).key_bits, cache.codec(i).value_bits) for i in range(4)}) > 1
+    seqs = cache.add(3)
+    feed(cache, seqs, (300, 0, 70), seed=1)
+    q = rand((5, 8, 128), 3, BF)
+
+    def every_layer(step):
+        for _ in range(2):
+            for layer in range(4):
+                check(step.attend(q, layer), q, step, layer)
+                check(step.attend(q, layer, sliding_window=33), q, step, layer, sliding_window=33)
+    every_layer(feed(cache, seqs, (1, 3, 1), seed=2, commit=False))
+    every_layer(feed(cache, seqs, (1, 3, 1), seed=3, commit=False))
+    cache.resize(pages=50, plain_pages=50)
+    step = feed(cache, seqs, (1, 3, 1), seed=4, commit=False)
+    every_layer(step)
+    other = pkg.PagedV3Cache(128, 2, 4, 2, 20, n_layers=4, pages=1, plain_pages=1, dtype=BF, device=DEV)
+    before = step.attend(q, 1)
+    cache.codec(1).key_compressor = pkg.MSECompressor(128, cache.codec(1).key_bits, seed=77, device="cpu")       # (what is packed means something else now)
+    assert other.codec(1).key_bits == cache.codec(1).key_bits and not torch.equal(before, step.attend(q, 1))
+    check(step.attend(q, 1), q, step, 1)
+
+
 def test_scale_and_layouts_of_queries(pkg):
     cache = make(pkg, H=2, layers=2, protected_layers=1)            # (8 bits in both)
     seqs = cache.add(2)

@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int INTERFACE = 9;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 10;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -663,31 +663,35 @@ PyObject *copy_pages(PyObject *const *a) {
                                   (long long)(to.stride(0) * to.element_size()), rows, row_bytes, (const tq_page_pair *)pairs.data(), (long long)n, s.raw()));
 }
 
-// paged_attend(address of the step's tq_paged_request, queries, tokens, scale, softcap or None, slopes or None, scratch values, like, stream) -> output; like: a tensor on the cache's
-// device; stream: the one the step's tables were uploaded on
+// paged_attend(address of the step's tq_paged_request, address of one with what the layer has of its own, queries, tokens, scale, softcap or None, slopes or None, scratch values, like, stream)
+// -> output; like: a tensor on the cache's device; stream: the one the step's tables were uploaded on
 PyObject *paged_attend(PyObject *const *a) {
-    TENSOR(q, a[1]); TENSOR(like, a[7]);
+    TENSOR(q, a[2]); TENSOR(like, a[8]);
     tq_paged_request r = *reinterpret_cast<const tq_paged_request *>(integer(a[0]));
-    const long long tokens = integer(a[2]), floats = integer(a[6]);
+    const tq_paged_request &l = *reinterpret_cast<const tq_paged_request *>(integer(a[1]));
+    r.packed_pool = l.packed_pool; r.plain_pool = l.plain_pool; r.table_k = l.table_k; r.table_v = l.table_v;
+    r.packed_page_stride = l.packed_page_stride; r.k_norms = l.k_norms; r.v_idx = l.v_idx; r.v_norms = l.v_norms;
+    r.plain_page_stride = l.plain_page_stride; r.plain_values = l.plain_values; r.bits_k = l.bits_k; r.bits_v = l.bits_v;
+    const long long tokens = integer(a[3]), floats = integer(a[7]);
     NEED(q.dim() == 3 && dtype_code(q) == r.dtype && q.device() == like.device() && q.size(0) == tokens && q.size(1) == (long long)r.heads * r.group && q.size(2) == r.head_dim &&
          q.stride(2) == 1 && tokens > 0 && aligned(address(q), 16) && (q.stride(0) * (long long)q.element_size()) % 16 == 0 && (q.stride(1) * (long long)q.element_size()) % 16 == 0);
-    r.scale = (float)PyFloat_AsDouble(a[3]);
+    r.scale = (float)PyFloat_AsDouble(a[4]);
     r.softcap = 0.f;
-    if (a[4] != Py_None) {
-        const double cap = PyFloat_AsDouble(a[4]);
+    if (a[5] != Py_None) {
+        const double cap = PyFloat_AsDouble(a[5]);
         if (PyErr_Occurred()) throw Raised{};
         NEED(cap >= 0x1p-100 && cap <= 1024.0);
         r.softcap = (float)cap;
     }
     if (PyErr_Occurred()) throw Raised{};
     r.slopes = nullptr;
-    if (a[5] != Py_None) {
-        TENSOR(slopes, a[5]);
+    if (a[6] != Py_None) {
+        TENSOR(slopes, a[6]);
         NEED(slopes.scalar_type() == at::kFloat && shape_is(slopes, {q.size(1)}) && slopes.is_contiguous() && slopes.device() == q.device());
         r.slopes = (const float *)address(slopes);
     }
     const Stream s(q);
-    NEED(s.ok && (long long)s.handle == integer(a[8]) && !s.capturing());
+    NEED(s.ok && (long long)s.handle == integer(a[9]) && !s.capturing());
     at::Tensor out = empty({tokens, q.size(1), q.size(2)}, q.scalar_type(), q), scratch;
     if (floats) scratch = empty({floats}, at::kFloat, q);
     r.queries = address(q);
@@ -745,7 +749,7 @@ PyMethodDef methods[] = {
     {"init", &init, METH_VARARGS, nullptr},
     TQ_ENTRY(compress, 3), TQ_ENTRY(decompress, 5), TQ_ENTRY(compress_layer, 7), TQ_ENTRY(restore_layer, 11), TQ_ENTRY(restore_dicts, 13), TQ_ENTRY(restore_store, 13),
     TQ_ENTRY(decode_append, 7), TQ_ENTRY(decode_attend, 8), TQ_ENTRY(qjl_compress, 4), TQ_ENTRY(qjl_scores, 8), TQ_ENTRY(attend_many, 22), TQ_ENTRY(evict, 10),
-    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 9), TQ_ENTRY(copy_pages, 7), TQ_ENTRY(put_tokens, 7),
+    TQ_ENTRY(beam_select, 3), TQ_ENTRY(reorder, 4), TQ_ENTRY(paged_attend, 10), TQ_ENTRY(copy_pages, 7), TQ_ENTRY(put_tokens, 7),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "tqamd_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

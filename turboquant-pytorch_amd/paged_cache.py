@@ -115,6 +115,7 @@ class PagedV3Cache:
         self._page_bytes, self._plain_shape = at, (self.n_layers, 2, H, P, self.head_dim)
         self._pool, self._plain = self._pools(pages, plain_pages)
         self._views = None
+        self._layers: List[Optional[tuple]] = [None] * self.n_layers
         self._packed_pages, self._plain_pages = _Pages(pages), _Pages(plain_pages)
         self._packed_of: Dict[int, int] = {}         # uncompressed pages still held by others -> the packed page one of their sequences made of them
         self._seqs: Dict[int, _Sequence] = {}
@@ -168,6 +169,22 @@ class PagedV3Cache:
         """Bytes of the pages that are held, packed and uncompressed."""
         used = [sum(map(bool, p.held)) for p in (self._packed_pages, self._plain_pages)]
         return used[0] * self._page_bytes + used[1] * int(np.prod(self._plain_shape)) * self._plain.element_size()
+
+    def _layer(self, layer: int) -> tuple:
+        """What an attention call needs of a layer, whatever the step: (address of a request with it, the codec's compressors, the request, their tables)."""
+        kept, codec = self._layers[layer], self._codecs[layer]
+        kc, vc = codec.key_compressor, codec.val_compressor
+        if kept is not None and kept[1] is kc and kept[2] is vc:
+            return kept
+        tables = kc.table(self.device), vc.table(self.device)
+        for t, comp in zip(tables, (kc, vc)):
+            _native.check_table(t, self.head_dim, comp.bits)
+        (k, kn, v, vn, _, _), plain, es = self._parts[layer], self._plain, self._plain.element_size()
+        r = _native.TqPagedRequest(packed_pool=self._pool.data_ptr() + k, plain_pool=plain.data_ptr() + layer * plain.stride(1) * es, table_k=tables[0].data_ptr(), table_v=tables[1].data_ptr(),
+                                   packed_page_stride=self._page_bytes, k_norms=kn - k, v_idx=v - k, v_norms=vn - k, plain_page_stride=plain.stride(0) * es, plain_values=plain.stride(2) * es,
+                                   bits_k=kc.bits, bits_v=vc.bits)
+        kept = self._layers[layer] = (ctypes.addressof(r), kc, vc, r, tables)
+        return kept
 
     def _sequence(self, seq: int) -> _Sequence:
         s = self._seqs.get(seq)
@@ -343,7 +360,7 @@ class PagedV3Cache:
             if order:
                 _native.copy_pages(source, target, rows, row_bytes, order)
             source.record_stream(stream)         # (what it was allocated on may be another one)
-        self._pool, self._plain, self._views = pool, plain, None
+        self._pool, self._plain, self._views, self._layers = pool, plain, None, [None] * self.n_layers
         # (the copies run while the tables are brought in line)
         pools, numbers, tables = [], [], []
         for old, of, order, n, size in zip((self._packed_pages, self._plain_pages), flat, orders, held, sizes):
@@ -422,7 +439,7 @@ class PagedStep:
         self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
         self._plans: Dict[Tuple[int, int], tuple] = {}
         self._ready: Dict[tuple, tuple] = {}
-        self._quick: Dict[tuple, tuple] = {}         # (layer, window) as they are asked for -> what the one-step call takes
+        self._quick: Dict[Optional[int], tuple] = {}         # window as it is asked for -> what the one-step call takes
         self._appended: set = set()
         self._done = False
 
@@ -505,6 +522,9 @@ class PagedStep:
         if plan is None:
             self.cache._eager("the first attend of a step with this window")
             c, counts = self.cache, _native.TqPagedCounts()
+            if None in c._layers:            # (all tables are on the card before a graph may be recorded)
+                for i in range(c.n_layers):
+                    c._layer(i)
             call = lambda items, merges: _native.lib().tq_paged_plan(  # noqa: E731
                 self._records.ctypes.data, len(self.seqs), c.kv_heads, group, window, c.head_dim, _native.dtype_code(c.dtype), c.page_tokens, items.ctypes.data, len(items), merges.ctypes.data,
                 len(merges), ctypes.byref(counts))
@@ -521,29 +541,15 @@ class PagedStep:
             plan = self._plans[key] = (counts, items_at, merges_at, floats, uploaded)
         return plan
 
-    def _request(self, layer: int, group: int, window: int) -> tuple:
-        c = self.cache
-        key = (layer, group, window)
-        ready = self._ready.get(key)
-        if ready is not None:
-            return ready
-        counts, items_at, merges_at, floats, uploaded = self._plan(group, window)
-        codec, (k, kn, v, vn, _, _) = c._codecs[layer], c._parts[layer]
-        kc, vc = codec.key_compressor, codec.val_compressor
-        tables = kc.table(c.device), vc.table(c.device)
-        for t, comp in zip(tables, (kc, vc)):
-            _native.check_table(t, c.head_dim, comp.bits)
-        es = c._plain.element_size()
-        r = _native.TqPagedRequest()
-        r.packed_pool, r.plain_pool = c._pool.data_ptr() + k, c._plain.data_ptr() + layer * c._plain.stride(1) * es
-        r.table_k, r.table_v = (t.data_ptr() for t in tables)
-        r.sequences, r.tables, r.items, r.merges = self._seq_at, self._table_at, items_at, merges_at
-        r.packed_page_stride, r.k_norms, r.v_idx, r.v_norms = c._page_bytes, kn - k, v - k, vn - k
-        r.plain_page_stride, r.plain_values = c._plain.stride(0) * es, c._plain.stride(2) * es
-        r.counts = counts
-        r.heads, r.group, r.sliding_window, r.page_tokens, r.head_dim, r.dtype, r.bits_k, r.bits_v = (c.kv_heads, group, window, c.page_tokens, c.head_dim,
-                                                                                                      _native.dtype_code(c.dtype), kc.bits, vc.bits)
-        ready = self._ready[key] = (r, floats, uploaded, tables)
+    def _request(self, group: int, window: int) -> tuple:
+        """What is the same in all layers: (request, scratch values, what its plan was uploaded as)."""
+        ready = self._ready.get((group, window))
+        if ready is None:
+            counts, items_at, merges_at, floats, uploaded = self._plan(group, window)
+            c = self.cache
+            r = _native.TqPagedRequest(sequences=self._seq_at, tables=self._table_at, items=items_at, merges=merges_at, counts=counts, heads=c.kv_heads, group=group, sliding_window=window,
+                                       page_tokens=c.page_tokens, head_dim=c.head_dim, dtype=_native.dtype_code(c.dtype))
+            ready = self._ready[group, window] = (r, floats, uploaded)
         return ready
 
     def attend(self, queries: torch.Tensor, layer_idx: int, scale: Optional[float] = None, softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
@@ -552,10 +558,10 @@ class PagedStep:
         Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap (up to 1024 for 16-bit elements) is given, less
         slopes[query head] * distance if slopes (float [query heads]) are; sliding_window: only the last so many tokens, the new one among them, are seen.
         Every layer has to be appended to before (the step's own tokens are read from its pages).  Not differentiable."""
-        ready = self._quick.get((layer_idx, sliding_window))
-        if ready is not None and not self._done and not torch.compiler.is_compiling():
-            # as the call before with this layer and window, if the queries are laid out for it
-            out = _native.fast().paged_attend(ready[0], queries, self.tokens, self.cache.head_dim ** -0.5 if scale is None else scale, softcap, slopes, ready[1], ready[2], ready[3])
+        ready = self._quick.get(sliding_window)
+        if ready is not None and not self._done and type(layer_idx) is int and 0 <= layer_idx < self.cache.n_layers and not torch.compiler.is_compiling():
+            # as the call before with this window, if the queries are laid out for it
+            out = _native.fast().paged_attend(ready[0], self.cache._layer(layer_idx)[0], queries, self.tokens, self.cache.head_dim ** -0.5 if scale is None else scale, softcap, slopes, ready[1], ready[2], ready[3])
             if out is not None:
                 if type(out) is int:
                     _native.check(out, "tq_paged_attend")
@@ -595,13 +601,14 @@ class PagedStep:
             es = queries.element_size()
             if queries.stride(2) != 1 or queries.data_ptr() % 16 or queries.stride(0) * es % 16 or queries.stride(1) * es % 16:
                 queries = queries.clone(memory_format=torch.contiguous_format)
-            ready = self._request(layer, heads // c.kv_heads, window)
-            floats, uploaded = ready[1:3]
+            request, floats, uploaded = self._request(heads // c.kv_heads, window)
             if uploaded[2] == self._blob[2]:
-                self._quick[layer, sliding_window] = (ctypes.addressof(ready[0]), floats, self._blob[0], uploaded[2])
+                self._quick[sliding_window] = (ctypes.addressof(request), floats, self._blob[0], uploaded[2])
             self._await(self._blob)
             self._await(uploaded)
-            r = _native.TqPagedRequest.from_buffer_copy(ready[0])
+            r, own = _native.TqPagedRequest.from_buffer_copy(request), c._layer(layer)[3]
+            for name in ("packed_pool", "plain_pool", "table_k", "table_v", "packed_page_stride", "k_norms", "v_idx", "v_norms", "plain_page_stride", "plain_values", "bits_k", "bits_v"):
+                setattr(r, name, getattr(own, name))
             r.queries, r.out = queries.data_ptr(), out.data_ptr()
             r.q_token, r.q_head = queries.stride(0), queries.stride(1)
             r.scale, r.softcap = c.head_dim ** -0.5 if scale is None else float(scale), cap
