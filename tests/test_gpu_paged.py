@@ -285,6 +285,19 @@ def test_layers_of_their_own_widths_and_codecs(pkg):
     check(step.attend(q, 1), q, step, 1)
 
 
+@pytest.mark.parametrize("D,H,G,dtype,kb,vb,most", [(128, 8, 1, BF, 4, 2, 4), (64, 4, 2, F16, 6, 4, 2), (128, 4, 1, F16, 8, 8, 8), (96, 4, 4, BF, 4, 2, 4), (256, 4, 1, BF, 4, 2, 8), (256, 2, 2, F16, 4, 2, 8)])
+def test_rows_of_different_numbers_of_query_vectors(pkg, D, H, G, dtype, kb, vb, most):
+    n = 150
+    cache = make(pkg, D, H, dtype, kb, vb, 30, pages=12 * n, plain=12 * n)
+    seqs = cache.add(n)
+    feed(cache, seqs, [(0, 200, 64, 450, 31, 130)[i % 6] for i in range(n)], seed=1)
+    new = [(i * 7) % (most + 1) for i in range(n)]
+    step = feed(cache, seqs, new, seed=2, commit=False)
+    q = rand((sum(new), H * G, D), 3, dtype)
+    check(step.attend(q, 0), q, step)
+    check(step.attend(q, 0, sliding_window=40, softcap=30.0), q, step, sliding_window=40, softcap=30.0)
+
+
 def test_scale_and_layouts_of_queries(pkg):
     cache = make(pkg, H=2, layers=2, protected_layers=1)            # (8 bits in both)
     seqs = cache.add(2)
