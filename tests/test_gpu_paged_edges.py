@@ -1,0 +1,64 @@
+"""GPU tests of the paged cache where something has gone wrong: packed vectors that are no numbers behind a window's edge.  Tolerances are those of
+test_gpu_paged."""
+import pytest
+import torch
+
+from test_gpu_paged import BF, F16, F32, check, feed, make, rand
+from test_gpu_parity import DEV
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("these tests need a HIP device; there is no CPU fallback to test")
+
+
+@pytest.mark.parametrize("side", [1, 3], ids=["keys", "values"])
+@pytest.mark.parametrize("D,G,dtype,kb,vb,new,P", [
+    (128, 4, BF, 4, 2, 1, 64), (128, 4, BF, 4, 2, 4, 64), (128, 8, F16, 6, 4, 1, 64), (64, 4, F16, 6, 4, 1, 128), (64, 2, BF, 8, 8, 3, 64), (96, 2, BF, 4, 2, 1, 64), (256, 4, BF, 4, 2, 1, 64), (256, 2, F16, 8, 4, 2, 64),
+    (128, 4, BF, 4, 2, 40, 64), (128, 4, F16, 6, 4, 40, 64), (64, 4, BF, 8, 8, 33, 64), (80, 2, BF, 4, 4, 20, 64), (96, 4, F16, 4, 4, 30, 64), (256, 2, BF, 4, 2, 20, 64), (128, 1, BF, 4, 2, 40, 32),
+    (128, 2, F32, 4, 2, 1, 64), (128, 2, F32, 4, 4, 40, 64), (256, 1, F32, 2, 8, 9, 32)])
+def test_packed_vectors_that_are_no_numbers_stay_with_those_who_see_them(pkg, D, G, dtype, kb, vb, new, P, side):
+    W, n = 150, 700
+    cache = make(pkg, D, 2, dtype, kb, vb, 16, P=P)
+    seqs = cache.add(2)
+    feed(cache, seqs, (n, 390), seed=1)
+    step = feed(cache, seqs, (new, new), seed=2, commit=False)
+    q = rand((2 * new, 2 * G, D), 3, dtype)
+    want = step.attend(q, 0, sliding_window=W)
+    check(want, q, step, sliding_window=W)
+    norms = cache.packed_pages(0)[side]
+    # a norm of its first kv head that the first `seen` of the new tokens see: none, the token just outside the window or further out; some
+    for seen in sorted({-45, -20, 0, new // 2}):
+        t = n - W + seen
+        at = cache.tables(seqs[0])[0][t // P], 0, t % P
+        for value in (float("inf"), float("nan")):
+            kept = norms[at].clone()
+            norms[at] = value
+            got = step.attend(q, 0, sliding_window=W)
+            norms[at] = kept
+            if seen > 0:
+                if side == 3 or value != value:          # (an infinite key may be one that nobody likes)
+                    assert not bool(torch.isfinite(got[:seen, :G]).any())
+                got[:seen, :G] = want[:seen, :G]
+            check(got, q, step, sliding_window=W)
+
+
+def test_queries_that_are_no_numbers_stay_by_themselves(pkg):
+    for dtype, D, G, new in ((BF, 128, 4, 1), (F16, 64, 4, 2), (BF, 128, 4, 33), (F16, 128, 4, 33), (BF, 80, 2, 17), (F32, 128, 2, 9), (BF, 256, 4, 1), (F16, 256, 2, 20)):
+        cache = make(pkg, D, 2, dtype, 4, 2 if D != 80 else 4, 30)
+        seqs = cache.add(2)
+        feed(cache, seqs, (500, 90), seed=1)
+        step = feed(cache, seqs, (new, new), seed=2, commit=False)
+        q = rand((2 * new, 2 * G, D), 3, dtype)
+        want = step.attend(q, 0)
+        for value in (float("inf"), float("nan")):
+            wild = q.clone()
+            wild[0, 0, 3] = value
+            wild[new, G, 5] = -value
+            got = step.attend(wild, 0)
+            assert bool(torch.isnan(got[0, 0]).all()) and bool(torch.isnan(got[new, G]).all())
+            got[0, 0], got[new, G] = want[0, 0], want[new, G]
+            check(got, q, step)

@@ -557,10 +557,13 @@ __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedA
                 }
             }
             {
-                const _Float16 kh = __builtin_bit_cast(_Float16, kn_raw);
+                // Where not all columns need see a token, an infinite norm of its values times a weight of 0 would make NaN of those that do not: it is zero there, and the keys' norm NaN (see
+                // tq_paged_kernel)
+                const bool wild = !FULL && (vn_raw & 0x7c00u) == 0x7c00u;
+                const _Float16 kh = __builtin_bit_cast(_Float16, wild ? (uint16_t)0x7e00u : kn_raw);
                 if (RUN == 64 || lane < (uint32_t)RUN) lds_kn[wave][lane] = (float)kh;     // one token per lane
                 // does a value norm of this run exceed the reference exponent?  (a vote; a handful of times per wave)
-                const uint16_t vn = lane < n_tok ? vn_raw : (uint16_t)0;   // tokens past the end weigh nothing
+                const uint16_t vn = lane < n_tok && !wild ? vn_raw : (uint16_t)0;   // tokens past the end weigh nothing
                 uint32_t e = ((uint32_t)vn >> 10) & 31u;
                 if (__any((int)max(e, 1u) - 15 > ev_ref)) {
                     e = max(e, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)e, 0x111, 0xf, 0xf, true));

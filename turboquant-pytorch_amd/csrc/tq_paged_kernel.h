@@ -635,6 +635,12 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
             // ---- norms: keys' times the queries' scale, values' in the unit of the largest so far
             float norm = (float)__builtin_bit_cast(_Float16, h ? vn_raw : kn_raw);
             if (hidden) norm = (hidden >> n) & 1u ? 0.f : norm;
+            if (cut) {
+                // Where not all queries see a token, an infinite norm of its values times a weight of 0 would make NaN of those that do not: it is zero there, and the keys' norm NaN, which
+                // makes NaN of the logits of those that do.  (Logits are masked by selection.  Masking products or norms by tile: 5 to 10 registers more are spilled in the loop.)
+                const uint32_t wild = (uint32_t)(__ballot(!(norm < __builtin_inff())) >> 32);
+                if ((wild >> n) & 1u) norm = h ? 0.f : __builtin_nanf("");
+            }
             const int top = (int)((__float_as_uint(norm) >> 23) & 255u) - 127;
             if (__any(h && top > v_top)) {
                 int new_top = h ? top : -100;
