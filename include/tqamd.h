@@ -521,7 +521,8 @@ long long tq_evict_scratch(long long rows, long long tokens);
 /*
  * Beam search's choice: of the beams x vocab continuations of every sequence the `best` with the largest sums
  *     sum(k, v) = scores[k] + logits[k][v] - log sum_v exp(logits[k][v])
- * in falling order, equal ones by beam and then token (formed and compared in 64 bits, answered in 32).  No counterpart in the reference.
+ * in falling order, equal ones by beam and then token (formed and compared in 64 bits, from sums of exponentials in 32; answered in 32).  Beams of equal logits and scores have equal
+ * sums, wherever in memory they lie.  No counterpart in the reference.
  *   logits      element type dtype; token v of beam k of sequence b at element b * batch_stride + k * beam_stride + v
  *   scores      float32, beam k of sequence b at b * score_stride + k
  *   values, tokens, parents     dense [batch, best]

@@ -15,7 +15,8 @@ MAX_BEST, MAX_BEAMS = 64, 1024
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Of the continuations of every sequence's beams the `best` (default: as many as there are beams) with the largest sums scores + log_softmax(logits).
     logits [batch, beams, vocabulary] (float32, float16 or bfloat16), scores [batch, beams] -> sums (float32), tokens and beams they continue (int64),
-    each [batch, best], in falling order, equal ones by beam and then token; sums are formed and compared in 64 bits.
+    each [batch, best], in falling order, equal ones by beam and then token.  Sums are formed and compared in 64 bits, from sums of exponentials in 32 (a beam's sums can be off by some 2^-22,
+    all by the same); beams of equal logits and scores have equal sums, wherever in memory they lie.
     A beam whose sums are no numbers (a NaN or +infinity among its logits, nothing but -infinity, a score that is not finite: a beam that has ended or not begun) counts with sums of
     -infinity.  At most 64 are chosen, of at most 1024 beams.  Not differentiable."""
     n = logits.shape[1] if best is None and logits.dim() > 1 else best

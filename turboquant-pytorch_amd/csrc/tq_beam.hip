@@ -2,7 +2,7 @@
 //
 // sum(k, v) = score_k + logit_kv - log sum_v exp(logit_kv).  Within a beam sums have the order of the logits, so that a part of a row can name its `best` largest logits
 // before the row's sum of exponentials is known.  Two launches: parts of rows (their largest logits, and largest and sum of exponentials), each logit read once and held in
-// registers; then a block a sequence joins the sums in 64 bits and chooses.
+// registers; then a block a sequence joins the sums in 64 bits and chooses.  (The sums of exponentials are of 32 bits, from lane to row: terms of one sign, so that some 2^-22 of a logarithm is lost.)
 #include <type_traits>
 
 #include "tq_lut.h"
@@ -26,6 +26,15 @@ struct BeamArgs {
 };
 constexpr uint32_t NO_TOKEN = 0xffffffffu;
 constexpr float LOG2E_F = 1.44269504088896340736f;
+
+// Sixteen bytes at the address of any element
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t Halves __attribute__((ext_vector_type(4), aligned(2)));
+template <int ES>
+__device__ __forceinline__ tq_u4 load_piece(const uint8_t *p) {
+    if constexpr (ES == 4) return *reinterpret_cast<const TQ_GLOBAL Words *>((const TQ_GLOBAL uint8_t *)p);
+    else return *reinterpret_cast<const TQ_GLOBAL Halves *>((const TQ_GLOBAL uint8_t *)p);
+}
 
 // Order of this wave's LDS accesses among its lanes
 __device__ __forceinline__ void wave_sync_lds() {
@@ -132,19 +141,17 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
     if (at >= a.rows * a.parts) return;
     const uint32_t row = at / a.parts, part = at - row * a.parts, b = row / a.beams, k = row - b * a.beams;
     const uint8_t *src = a.logits + ((long long)b * a.batch_stride + (long long)k * a.beam_stride) * ES;
-    // Positions count from the aligned address at or before the row's first logit, so that every chunk but the row's first and last one is whole pieces of 16 bytes; those two go
-    // element by element, neighbours in neighbouring lanes.
-    const uint32_t ahead = (uint32_t)((uintptr_t)src & 15u) / ES, stop = a.vocab + ahead;
-    const uint32_t begin = part * (a.chunks * CHUNK), end = min(stop, begin + a.chunks * CHUNK);
-    src -= ahead * ES;
+    // Every chunk but the row's last one is whole pieces of 16 bytes, wherever in memory the row begins: which lane adds an exponential depends on its token alone, so that equal logits have
+    // equal sums, bit for bit.  The last chunk goes element by element, neighbours in neighbouring lanes.
+    const uint32_t stop = a.vocab, begin = part * (a.chunks * CHUNK), end = min(stop, begin + a.chunks * CHUNK);
     BeamList &list = lists[wave];
     const float none = -__builtin_inff();
     tq_u4 raw[LOADS];
-    auto is_whole = [&](uint32_t first) { return first >= ahead && first + CHUNK <= stop; };
+    auto is_whole = [&](uint32_t first) { return first + CHUNK <= stop; };
     auto load = [&](uint32_t first) __attribute__((always_inline)) {
         if (is_whole(first)) {
 #pragma unroll
-            for (int l = 0; l < LOADS; ++l) raw[l] = tq_gload16(src + (size_t)(first + (l * 64u + lane) * V) * ES);
+            for (int l = 0; l < LOADS; ++l) raw[l] = load_piece<ES>(src + (size_t)(first + (l * 64u + lane) * V) * ES);
             return;
         }
 #pragma unroll
@@ -153,11 +160,11 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
             for (int d = 0; d < 4; ++d) {
                 if constexpr (DT == TQ_F32) {
                     const uint32_t p = first + (4 * l + d) * 64u + lane;
-                    raw[l][d] = p >= ahead && p < stop ? tq_gload4(src + (size_t)p * 4u) : 0xff800000u;
+                    raw[l][d] = p < stop ? tq_gload4(src + (size_t)p * 4u) : 0xff800000u;
                 } else {
                     const uint32_t none16 = DT == TQ_F16 ? 0xfc00u : 0xff80u, p = first + (8 * l + 2 * d) * 64u + lane, q = p + 64u;
                     const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
-                    raw[l][d] = (p >= ahead && p < stop ? (uint32_t)tq_gload2(h + p) : none16) | ((q >= ahead && q < stop ? (uint32_t)tq_gload2(h + q) : none16) << 16);
+                    raw[l][d] = (p < stop ? (uint32_t)tq_gload2(h + p) : none16) | ((q < stop ? (uint32_t)tq_gload2(h + q) : none16) << 16);
                 }
             }
         }
@@ -181,8 +188,7 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
         if (first + CHUNK < end) load(first + CHUNK);
         const bool whole = is_whole(first);
         auto place_of = [&](int i) { return first + (whole ? ((i / V) * 64u + lane) * V + i % V : 64u * i + lane); };
-        auto is_token = [&](int i) { return whole || (place_of(i) >= ahead && place_of(i) < stop); };
-        const uint32_t lowest = first + lane < ahead ? first + lane + 64u : first + lane;        // this lane's first logit, of a chunk that is not whole
+        auto is_token = [&](int i) { return whole || place_of(i) < stop; };
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < E; ++i) top = fmaxf(top, x[i]);
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
                 const uint32_t to = fresh + lanes_before(mask);
                 if (in && to < 64u) {
                     list.x[count + to] = x[i];
-                    list.token[count + to] = place_of(i) - ahead;
+                    list.token[count + to] = place_of(i);
                 }
                 fresh += (uint32_t)__popcll(mask);
             }
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
 #pragma unroll 1
         for (bool known = bound != 0u;; known = false) {
             if (!known) {
-                const uint32_t t = nth_of_wave(whole || lowest < stop ? beam_order(top) : 0u, a.best);
+                const uint32_t t = nth_of_wave(first + lane < stop ? beam_order(top) : 0u, a.best);
                 need = max(need, t);
                 if (t > bound) bound = t;
             }
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(64 * PART_WAVES) void tq_beam_part_kernel(BeamArgs 
                 unsigned long long mine = 0ull;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const unsigned long long u = is_token(i) && x[i] >= need_x ? ((unsigned long long)beam_order(x[i]) << 32) | (uint32_t)~(place_of(i) - ahead) : 0ull;
+                    const unsigned long long u = is_token(i) && x[i] >= need_x ? ((unsigned long long)beam_order(x[i]) << 32) | (uint32_t)~place_of(i) : 0ull;
                     if (u < last && u > mine) mine = u;
                 }
                 last = wave_max(mine);
@@ -414,7 +420,7 @@ int beam_plan(long long batch, long long beams, long long vocab, long long best,
     p.rows = batch * beams;
     const long long waves = 8LL * cus;
     p.per_lane = p.rows * ((vocab + 2047) / 2048) >= waves ? 32 : 8;
-    const long long chunk = 64LL * p.per_lane, all = (vocab + 7 + chunk - 1) / chunk;       // (up to seven logits ahead of an aligned address)
+    const long long chunk = 64LL * p.per_lane, all = (vocab + chunk - 1) / chunk;
     p.chunks = 1;
     while (p.chunks < 4 && p.rows * ((all + 2 * p.chunks - 1) / (2 * p.chunks)) >= waves) p.chunks *= 2;
     // (a row's sums are joined by one block: no more than 64 parts, unless chunks get many)
