@@ -558,7 +558,7 @@ int tq_copy_pages(const void *from, long long from_stride, void *to, long long t
 /*
  * New tokens into a pool of uncompressed pages: the key of token i and head h, vector_bytes bytes at i * k_token_stride + h * k_head_stride (bytes), goes to place
  * slots[i] % page_tokens of page slots[i] / page_tokens, at page * page_stride + (h * page_tokens + place) * vector_bytes; the value side_stride further on.  page_tokens is a power of
- * two; slots (int32, device) are not checked.
+ * two; slots (int32, device) are not checked, but that a token of slot -1 is passed over.
  */
 int tq_put_tokens(const void *keys, const void *values, long long k_token_stride, long long k_head_stride, long long v_token_stride, long long v_head_stride,
                   void *pool, long long page_stride, long long side_stride, const int32_t *slots, long long tokens, long long heads, long long vector_bytes,
@@ -575,6 +575,7 @@ int tq_put_tokens(const void *keys, const void *values, long long k_token_stride
  *   softcap     0: none; otherwise, from 2^-100 to 1024 (float32: 2^100), logits become softcap * tanh(logit / softcap).  slopes: NULL, or float32 of every query head.  sliding_window: 0: none
  * tq_paged_plan: how the call's blocks share the work, by lengths and window, for the current device: 8 numbers an item, then blocks + 1 (where each block's items
  * begin), in room for 8 * max_items; 8 a merge; counts also where they do not fit (TQ_ERR_CAPACITY: call again with room).  One plan serves calls of any layer for the same sequences, window, heads, group, head_dim, dtype and page_tokens.
+ * A plan on the device that is overwritten with -1, its items, the numbers behind them and its merges, makes the call do nothing: calls that a graph has recorded are ended so.
  * tq_paged_scratch: float32 values of scratch (16-byte aligned, not shared by calls that can overlap in time).
  * tq_paged_supported: head_dim 64, 128, 256, or a multiple of 8 from 72 to 96 whose packed vectors are words; 2 to 8 bits.
  * Infinities and NaN reach the results of the queries that see them and no others.  Numbers of pages are not checked.  Queries' vectors lie at multiples of 16 bytes where counts.few is not zero

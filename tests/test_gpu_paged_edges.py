@@ -1,9 +1,9 @@
-"""GPU tests of the paged cache where something has gone wrong: packed vectors that are no numbers behind a window's edge.  Tolerances are those of
-test_gpu_paged."""
+"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end.
+Tolerances are those of test_gpu_paged."""
 import pytest
 import torch
 
-from test_gpu_paged import BF, F16, F32, check, feed, make, rand
+from test_gpu_paged import BF, F16, F32, check, feed, make, rand, states
 from test_gpu_parity import DEV
 
 pytestmark = pytest.mark.gpu
@@ -44,6 +44,63 @@ def test_packed_vectors_that_are_no_numbers_stay_with_those_who_see_them(pkg, D,
                     assert not bool(torch.isfinite(got[:seen, :G]).any())
                 got[:seen, :G] = want[:seen, :G]
             check(got, q, step, sliding_window=W)
+
+
+def recorded(pkg):
+    """A cache with an open step that a graph has recorded: (cache, its sequences, step, graph, result)."""
+    cache = make(pkg, H=2, window=20, pages=40, plain=40)
+    seqs = cache.add(2)
+    feed(cache, seqs, (300, 63), seed=1)
+    step = cache.step(seqs, (9, 1))
+    k, v, q = states(10, 2, 128, 1, BF), states(10, 2, 128, 2, BF), rand((10, 8, 128), 3, BF)
+    step.append(k, v, 0)
+    step.attend(q, 0)
+    step.attend(q[:, :2], 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.append(k, v, 0)
+        outs = [step.attend(q, 0), step.attend(q[:, :2], 0)]
+    graph.replay()
+    torch.cuda.synchronize()
+    check(outs[0], q, step)
+    k.fill_(7.0), v.fill_(7.0)
+    return cache, seqs, step, graph, outs
+
+
+@pytest.mark.parametrize("change", ["step", "free", "fork", "reorder", "place", "cancel", "resize"])
+def test_replays_of_a_step_that_is_over_do_nothing(pkg, change):
+    cache, seqs, step, graph, outs = recorded(pkg)
+    if change == "cancel":
+        step.cancel()
+    else:
+        step.commit()
+    others = cache.add(2)
+    if change == "free":
+        cache.free(seqs)
+    elif change == "fork":
+        others += cache.fork(seqs)
+    elif change == "reorder":
+        cache.reorder(seqs, [0, 0])
+    elif change == "place":
+        cache.place(others, [0, 64], [70, 1])
+    elif change == "resize":
+        cache.resize(pages=41, plain_pages=42)
+    if change != "place":
+        feed(cache, others, [100] * len(others), seed=5)
+    for out in outs:
+        out.fill_(5.0)
+    torch.cuda.synchronize()
+    before = cache._plain.view(torch.int16).clone(), cache._pool.clone()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache._plain.view(torch.int16), before[0]) and torch.equal(cache._pool, before[1])
+        assert all(bool((out == 5.0).all()) for out in outs)
+    step = feed(cache, others, [3] * len(others), seed=6, commit=False)
+    q = rand((3 * len(others), 8, 128), 4, BF)
+    if change != "place":
+        check(step.attend(q, 0), q, step)
 
 
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):

@@ -17,7 +17,7 @@ struct TqPagedArgs {
     long long k_norms, v_idx, v_norms, plain_v;      // bytes from the layer's key codes (plain: keys)
     const uint8_t *table_k, *table_v;
     const int32_t *seqs, *tables;
-    const int32_t *items;            // {sequence, first tile, packed tokens from, to, plain ones from, to (multiples of 32, or the end), record or -1: all its tokens are here, kv head or -1: one block
+    const int32_t *items;            // {sequence (-1, here as in the merges: nothing is done; blocks from -1 to -1 have no items), first tile, packed tokens from, to, plain ones from, to (multiples of 32, or the end), record or -1: all its tokens are here, kv head or -1: one block
                                      // each, whose record is the item's and so many on}
     const int32_t *blocks;           // items of sequences with few query vectors: block i has items [blocks[i], blocks[i + 1])
     const int32_t *merges;           // {sequence, first tile, kv head, first record, records, from one of them to the next, two unused}

@@ -17,6 +17,7 @@ __global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedAr
     __shared__ float lds_m[MAX_PIECES * 32], lds_l[MAX_PIECES * 32];
     const uint32_t share = blockIdx.x % shares, at = blockIdx.x / shares, i = at % a.qt, merge = at / a.qt;
     const int32_t *mg = a.merges + (size_t)merge * PAGED_MERGE;
+    if (mg[0] < 0) return;                   // (a plan that is over)
     const int32_t *sq = a.seqs + (size_t)mg[0] * PAGED_SEQ;
     const uint32_t tile = (uint32_t)mg[1] + i, kv = (uint32_t)mg[2], records = (uint32_t)mg[4], M = (uint32_t)sq[1] * a.group, tid = threadIdx.x;
     if (tile * 32u >= M) return;

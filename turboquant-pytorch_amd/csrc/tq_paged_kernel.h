@@ -495,6 +495,7 @@ __global__ __launch_bounds__(FAST_THREADS, FAST_WAVES / 4) void tq_paged_kernel(
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tq_uniform32(tid >> 6), n = lane & 31u, h = lane >> 5;
     const uint32_t item = blockIdx.x / a.heads;
     const int32_t *it = a.items + (size_t)item * PAGED_ITEM;
+    if (it[0] < 0) return;                   // (a plan that is over)
     const int32_t *sq = a.seqs + (size_t)it[0] * PAGED_SEQ;
     const uint32_t tile0 = (uint32_t)it[1], begin = (uint32_t)it[2], end = (uint32_t)it[3], plain_from = (uint32_t)it[4], plain_to = (uint32_t)it[5];
     const int record = it[6];

@@ -107,7 +107,7 @@ struct PutArgs {
     const uint8_t *src[2];                   // keys, values: token i, head h at i * token_stride + h * head_stride bytes
     long long token_stride[2], head_stride[2];
     uint8_t *pool;                           // page p, keys or values s, head h, place t at p * page_stride + s * side_stride + (h * page_tokens + t) * vector
-    const int32_t *slots;                    // [tokens] page * page_tokens + place
+    const int32_t *slots;                    // [tokens] page * page_tokens + place, or -1: the token is passed over
     long long page_stride, side_stride;
     uint32_t tokens, heads, vector, page_tokens, shift;
 };
@@ -122,6 +122,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void tq_put_tokens_kernel(PutArgs a) 
         const unsigned long long two = vec / a.heads;
         const uint32_t s = two >= a.tokens ? 1u : 0u, token = (uint32_t)(two - (s ? a.tokens : 0u));
         const uint32_t slot = (uint32_t)a.slots[token], page = slot >> a.shift, place = slot & (a.page_tokens - 1u);
+        if (slot == 0xffffffffu) continue;       // (-1: of a step that is over)
         const T v = get<T>((s ? a.src[1] : a.src[0]) + (long long)token * (s ? a.token_stride[1] : a.token_stride[0]) +
                            (long long)h * (s ? a.head_stride[1] : a.head_stride[0]) + (size_t)piece * sizeof(T));
         put<T>(a.pool + (long long)page * a.page_stride + (long long)s * a.side_stride + ((long long)h * a.page_tokens + place) * (long long)a.vector + (size_t)piece * sizeof(T), v);

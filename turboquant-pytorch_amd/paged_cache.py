@@ -121,7 +121,8 @@ class PagedV3Cache:
         self._seqs: Dict[int, _Sequence] = {}
         self._next = 0
         self._open: Optional[PagedStep] = None
-        self._recorded: List[PagedStep] = []         # into graphs
+        self._recorded: List[PagedStep] = []         # into graphs, and not over yet
+        self._kept: List[torch.Tensor] = []          # tables of recorded steps that are over, which replays read
 
     def _pools(self, pages: int, plain_pages: int) -> Tuple[torch.Tensor, torch.Tensor]:
         return (torch.empty((pages, self._page_bytes), dtype=torch.uint8, device=self.device),
@@ -246,9 +247,14 @@ class PagedV3Cache:
             self._packed_of = {p: q for p, q in self._packed_of.items() if plain[p] and packed[q]}
 
     def _settle(self) -> None:
-        """An open step is committed before tables change."""
+        """An open step is committed before tables change, and what graphs have recorded of steps works on the pages no longer."""
         if self._open is not None:
             self._open.commit()
+        if self._recorded:
+            self._eager("a call that changes tables")
+            for step in self._recorded:
+                step._end()
+            self._recorded.clear()
 
     def free(self, seqs: Sequence[int]) -> None:
         """Sequences end; pages that no other one holds are free."""
@@ -407,8 +413,9 @@ class PagedV3Cache:
 
 class PagedStep:
     """New tokens of some sequences of a `PagedV3Cache`: `append` for every layer, `attend` where it is wanted, then `commit` (the next step or any other call that changes tables commits
-    what is open).  Where a graph is recorded, the step has to be made before, and `attend` called once with the same window before the recording; replays work on the step's tokens, until `resize` gives the
-    cache other pools."""
+    what is open).  Where a graph is recorded, the step has to be made before, and `attend` called once with the same window before the recording.  Replays work on the step's tokens until the step is taken
+    back, or is committed and the cache's tables then change (the next step, place, fork, reorder, free, resize): from then on a replay does nothing, as the step's pages may be others'.  The tables
+    that a graph reads, some numbers a page, are kept as long as the cache."""
 
     def __init__(self, cache: PagedV3Cache, seqs, states, counts, need):
         self.cache, self.seqs, self.counts = cache, seqs, counts
@@ -471,6 +478,14 @@ class PagedStep:
             current = torch.cuda.current_stream(self.cache.device)
             current.wait_event(event)
             blob.record_stream(current)
+
+    def _end(self) -> None:
+        """Replays of what was recorded of this step do nothing from here on: no token has a place, no item a sequence."""
+        with _native._on(self.cache.device):
+            for uploaded in (self._blob, *(plan[4] for plan in self._plans.values())):
+                self._await(uploaded)
+                uploaded[0].fill_(-1)
+                self.cache._kept.append(uploaded[0])
 
     def _live(self, what: str) -> None:
         if self._done:
@@ -675,6 +690,9 @@ class PagedStep:
         self._done = True
         if c._open is self:
             c._open = None
+        if self in c._recorded:
+            c._recorded.remove(self)
+            self._end()
 
     def _pack(self, made: np.ndarray) -> None:
         """Uncompressed pages into packed ones, of all layers: a job a page, layer and side; a launch a code width."""
