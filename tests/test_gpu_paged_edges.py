@@ -1,5 +1,7 @@
-"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end.
+"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end, failures halfway.
 Tolerances are those of test_gpu_paged."""
+from importlib import import_module
+
 import pytest
 import torch
 
@@ -101,6 +103,51 @@ def test_replays_of_a_step_that_is_over_do_nothing(pkg, change):
     q = rand((3 * len(others), 8, 128), 4, BF)
     if change != "place":
         check(step.attend(q, 0), q, step)
+
+
+def tables(cache):
+    """All that says which pages are whose."""
+    return (cache.free_pages(), sorted(cache._packed_pages.free), sorted(cache._plain_pages.free), list(cache._packed_pages.held), list(cache._plain_pages.held),
+            {s: (cache.lengths([s]), cache.tables(s)) for s in cache._seqs}, dict(cache._packed_of))
+
+
+@pytest.mark.parametrize("what", ["step", "fork", "reorder", "reorder in a full pool"])
+def test_a_failure_halfway_leaves_the_tables_as_they_were(pkg, monkeypatch, what):
+    module = import_module("turboquant-pytorch_amd.paged_cache")
+    cache = make(pkg, H=2, window=64, plain=40)
+    a, b, c = cache.add(3)
+    feed(cache, [a, b, c], (200, 130, 70), seed=1)
+    shared = cache.fork([a, b, b])
+    feed(cache, [a], (64,), seed=2)          # (packs a page that the fork still holds uncompressed)
+    assert cache._packed_of
+    seqs = [a, b, c] + shared
+    if "full" in what:
+        (d,) = cache.add(1)
+        cache.place([d], [0], [64 * cache.free_pages()[1]])
+    before = tables(cache)
+
+    def fail(*args, **kw):
+        raise MemoryError("no room for this")
+    with monkeypatch.context() as m:
+        m.setattr(module.PagedStep, "_upload", fail)
+        m.setattr(module._native, "copy_pages", fail)
+        with pytest.raises(MemoryError):
+            if what == "step":
+                cache.step(seqs, 70)
+            elif what == "fork":
+                cache.fork([a, b, b])
+            else:
+                cache.reorder(seqs, [2, 2, 2, 5, 5, 4] if "full" in what else [0, 0, 1, 2, 2, 2])
+    assert tables(cache) == before and cache._open is None
+    if "full" in what:
+        cache.free([d])
+    cache.reorder(seqs, [0, 0, 1, 2, 2, 2])
+    step = feed(cache, seqs, 3, seed=3, commit=False)
+    q = rand((18, 8, 128), 3, BF)
+    check(step.attend(q, 0), q, step)
+    step.commit()
+    cache.free(seqs)
+    assert cache.free_pages() == (64, 40) and not cache._packed_of
 
 
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):

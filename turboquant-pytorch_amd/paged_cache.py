@@ -64,6 +64,14 @@ class _Pages:
             if not n:
                 heapq.heappush(free, p)
 
+    def hold_again(self, pages: Iterable[int]) -> None:
+        """The reverse of drop_all, of pages that nobody has taken meanwhile."""
+        held = self.held
+        for p in pages:
+            held[p] += 1
+        self.free = [p for p in self.free if not held[p]]
+        heapq.heapify(self.free)
+
 
 class _Sequence:
     """Its pages, as int32 (a step joins the tables of all its sequences), and tokens."""
@@ -240,6 +248,10 @@ class PagedV3Cache:
         self._packed_pages.drop_all(chain.from_iterable([s.pages for s in gone]))
         self._plain_pages.drop_all(chain.from_iterable([s.plain for s in gone]))
 
+    def _undrop(self, states: Sequence[_Sequence]) -> None:
+        self._packed_pages.hold_again(chain.from_iterable([s.pages for s in states]))
+        self._plain_pages.hold_again(chain.from_iterable([s.plain for s in states]))
+
     def _forget(self) -> None:
         """Of which pages it is known what they were packed into: those that are still held, as what they became is."""
         if self._packed_of:
@@ -300,7 +312,11 @@ class PagedV3Cache:
         states, P = self._states(seqs), self.page_tokens
         self._room("fork", 0, len([s for s in states if s.total % P]))
         fresh = self._share(states)
-        self._copy_last(fresh)
+        try:
+            self._copy_last(fresh)
+        except BaseException:                # (tables stay as they were)
+            self._drop(fresh)
+            raise
         new = list(range(self._next, self._next + len(fresh)))
         self._next += len(fresh)
         self._seqs.update(zip(new, fresh))
@@ -328,10 +344,16 @@ class PagedV3Cache:
         # (pages of the ones that end become free first)
         ends = sum(1 for p, s in enumerate(states) if p not in heir for page in s.plain if self._plain_pages.held[page] == 1)
         self._room("reorder", 0, max(0, twice - ends))
-        fresh = self._share([states[p] for p in parents])
+        fresh, known = self._share([states[p] for p in parents]), self._packed_of
         self._drop(states)
         self._forget()               # (before a page that has become free is taken again)
-        self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i])
+        try:
+            self._copy_last([f for i, (f, p) in enumerate(zip(fresh, parents)) if heir[p] != i])
+        except BaseException:                # (tables stay as they were; a copy that is refused has written nothing)
+            self._drop(fresh)
+            self._undrop(states)
+            self._packed_of = known
+            raise
         self._seqs.update(zip(seqs, fresh))
 
     def beam_step(self, seqs: Sequence[int], logits: torch.Tensor, scores: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -419,17 +441,31 @@ class PagedStep:
 
     def __init__(self, cache: PagedV3Cache, seqs, states, counts, need):
         self.cache, self.seqs, self.counts = cache, seqs, counts
-        self._states, self._pages_taken = states, need
+        self._states, self._pages_taken, self._begun = states, need, 0
         self.tokens = sum(counts)
-        P = cache.page_tokens
+        try:
+            self._begin()
+        except BaseException:                # (no memory for the tables: the sequences stay as they were)
+            self._take_back()
+            raise
+        self._plans: Dict[Tuple[int, int], tuple] = {}
+        self._ready: Dict[tuple, tuple] = {}
+        self._quick: Dict[Optional[int], tuple] = {}         # window as it is asked for -> what the one-step call takes
+        self._appended: set = set()
+        self._done = False
+
+    def _begin(self) -> None:
+        """Pages for the new tokens, and the tables of all sequences onto the card."""
+        cache, P = self.cache, self.cache.page_tokens
         records, tables, singles, slots, at, begin = [], [], [], [], 0, 0
         rest = (0,) * (_native.PAGED_SEQ - 6)
-        for s, c, n in zip(states, counts, need):
-            if n:
-                s.plain.extend(cache._plain_pages.take() for _ in range(n))
+        for s, c, n in zip(self._states, self.counts, self._pages_taken):
             held = len(s.pages)
             first = s.total - held * P
+            if n:
+                s.plain.extend([cache._plain_pages.take() for _ in range(n)])
             s.total += c
+            self._begun += 1
             if c == 1:
                 singles.append(s.plain[first // P] * P + first % P)
             elif c:
@@ -441,14 +477,16 @@ class PagedStep:
             begin += held + len(s.plain)
             at += c
         slots.append(np.array(singles, dtype=np.int64))
-        self._records = np.array(records, dtype=np.int32).reshape(len(seqs), _native.PAGED_SEQ)
+        self._records = np.array(records, dtype=np.int32).reshape(len(self.seqs), _native.PAGED_SEQ)
         self._sections = [self._records.ravel(), np.frombuffer(b"".join(tables), dtype=np.int32), np.concatenate(slots).astype(np.int32)]
         self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
-        self._plans: Dict[Tuple[int, int], tuple] = {}
-        self._ready: Dict[tuple, tuple] = {}
-        self._quick: Dict[Optional[int], tuple] = {}         # window as it is asked for -> what the one-step call takes
-        self._appended: set = set()
-        self._done = False
+
+    def _take_back(self) -> None:
+        for s, count, pages in zip(self._states[:self._begun], self.counts, self._pages_taken):
+            s.total -= count
+            if pages:
+                self.cache._plain_pages.drop_all(s.plain[-pages:])
+                del s.plain[-pages:]
 
     def _upload(self, sections: Sequence[np.ndarray]) -> Tuple[torch.Tensor, List[int]]:
         """Whole numbers onto the card, in one copy; addresses of the sections."""
@@ -682,11 +720,7 @@ class PagedStep:
             return
         c = self.cache
         c._eager("cancel")
-        for s, count, pages in zip(self._states, self.counts, self._pages_taken):
-            s.total -= count
-            if pages:
-                c._plain_pages.drop_all(s.plain[-pages:])
-                del s.plain[-pages:]
+        self._take_back()
         self._done = True
         if c._open is self:
             c._open = None
