@@ -1,4 +1,4 @@
-"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end, failures halfway.
+"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end, failures halfway, pools that are nearly full.
 Tolerances are those of test_gpu_paged."""
 from importlib import import_module
 
@@ -148,6 +148,32 @@ def test_a_failure_halfway_leaves_the_tables_as_they_were(pkg, monkeypatch, what
     step.commit()
     cache.free(seqs)
     assert cache.free_pages() == (64, 40) and not cache._packed_of
+
+
+def test_pages_that_only_ending_sequences_share_have_room_for_others(pkg):
+    cache = make(pkg, H=1, window=128, pages=4, plain=3)
+    (a,) = cache.add(1)
+    feed(cache, [a], 64, seed=1)
+    (b,) = cache.fork([a])                   # (a whole page, shared)
+    (c,) = cache.add(1)
+    feed(cache, [c], 10, seed=2)
+    assert cache.free_pages()[1] == 1
+    cache.reorder([a, b, c], [2, 2, 2])      # two copies of a page: into the free one and the one that a and b end with
+    assert cache.free_pages()[1] == 0 and cache.lengths([a, b, c]) == [10, 10, 10] and len({cache.tables(s)[1][0] for s in (a, b, c)}) == 3
+    step = feed(cache, [a, b, c], 1, seed=3, commit=False)
+    q = rand((3, 2, 128), 3, BF)
+    check(step.attend(q, 0), q, step)
+    # one of them goes on: its page stays, and there is room for one copy less than it takes
+    cache = make(pkg, H=1, window=128, pages=4, plain=3)
+    (a,) = cache.add(1)
+    feed(cache, [a], 64, seed=1)
+    b, d = cache.fork([a, a])
+    (c,) = cache.add(1)
+    feed(cache, [c], 10, seed=2)
+    before = tables(cache)
+    with pytest.raises(pkg._native.TqError, match="uncompressed pages"):
+        cache.reorder([a, b, c, d], [2, 2, 2, 0])
+    assert tables(cache) == before
 
 
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):

@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 from array import array
+from collections import Counter
 from itertools import chain, groupby
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -341,9 +342,11 @@ class PagedV3Cache:
             if p not in heir or i == p:
                 heir[p] = i
         twice = sum(1 for i, p in enumerate(parents) if heir[p] != i and states[p].total % self.page_tokens)
-        # (pages of the ones that end become free first)
-        ends = sum(1 for p, s in enumerate(states) if p not in heir for page in s.plain if self._plain_pages.held[page] == 1)
-        self._room("reorder", 0, max(0, twice - ends))
+        if twice > len(self._plain_pages.free):
+            # (pages that only sequences hold that end become free first)
+            held = self._plain_pages.held
+            ending = Counter(chain.from_iterable(s.plain for p, s in enumerate(states) if p not in heir))
+            self._room("reorder", 0, twice - sum(1 for page, n in ending.items() if n == held[page]))
         fresh, known = self._share([states[p] for p in parents]), self._packed_of
         self._drop(states)
         self._forget()               # (before a page that has become free is taken again)
