@@ -1,9 +1,9 @@
-"""GPU tests of beam search: equal sums, however the logits lie in memory."""
+"""GPU tests of beam search: equal sums however the logits lie in memory, and caches whose answer is still due."""
 import pytest
 import torch
 
 from test_gpu_beams import check
-from test_gpu_parity import DEV
+from test_gpu_parity import DEV, outlier_kv
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,20 @@ def test_a_choice_does_not_depend_on_where_logits_lie(pkg, dtype, B, K, V):
             view = wide[ahead:].view(B, K, row)[:, :, :V]
             view.copy_(logits)
             assert all(torch.equal(x, y) for x, y in zip(pkg.beam_select(view, scores, best), want))
+
+
+def test_a_pending_step_is_answered_before_beams_move(pkg):
+    pytest.importorskip("transformers")
+    for call in (lambda c: c.reorder(torch.tensor([1, 0], device=DEV)), lambda c: c.reorder_cache(torch.tensor([1, 0], device=DEV)),
+                 lambda c: c.beam_step(torch.randn((1, 2, 50), device=DEV), torch.zeros((1, 2), device=DEV))):
+        cache = pkg.hf_cache_class()(residual_window=8, n_layers=1, packed_attention=True)
+        k, v = (outlier_kv((2, 2, 50, 128), seed=i, dtype=torch.bfloat16).to(DEV) for i in (0, 1))
+        t = outlier_kv((2, 2, 1, 128), seed=5, dtype=torch.bfloat16).to(DEV)
+        cache.update(k, v, 0)
+        call(cache)                          # (nothing is due)
+        before = [x.clone() for x in cache._stores[0].window()]
+        cache.update(t, t, 0)
+        held = [x.clone() for x in cache._stores[0].window()]
+        with pytest.raises(RuntimeError, match="never answered"):
+            call(cache)
+        assert all(torch.equal(x, y) for x, y in zip(cache._stores[0].window(), held)) and len(before) == 2

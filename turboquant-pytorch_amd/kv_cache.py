@@ -722,6 +722,14 @@ def hf_cache_class():
             self._no_pending("reorder_cache")
             V3Cache.reorder(self, beam_idx)
 
+        def reorder(self, parents):
+            self._no_pending("reorder")
+            V3Cache.reorder(self, parents)
+
+        def beam_step(self, logits, scores):
+            self._no_pending("beam_step")
+            return V3Cache.beam_step(self, logits, scores)
+
         def get_seq_length(self, layer_idx=0):
             self._no_pending("get_seq_length")
             return V3Cache.get_seq_length(self, layer_idx)
