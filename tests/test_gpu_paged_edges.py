@@ -1,5 +1,7 @@
-"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end, failures halfway, pools that are nearly full.
+"""GPU tests of the paged cache where something has gone wrong or is over: packed vectors that are no numbers behind a window's edge, recorded steps after their end, failures halfway, pools that are nearly full or have been
+gathered.
 Tolerances are those of test_gpu_paged."""
+import random
 from importlib import import_module
 
 import pytest
@@ -174,6 +176,63 @@ def test_pages_that_only_ending_sequences_share_have_room_for_others(pkg):
     with pytest.raises(pkg._native.TqError, match="uncompressed pages"):
         cache.reorder([a, b, c, d], [2, 2, 2, 0])
     assert tables(cache) == before
+
+@pytest.mark.parametrize("seed", range(6))
+def test_gathers_between_all_other_calls(pkg, seed):
+    rng = random.Random(seed)
+    cache, kept, seqs, at = make(pkg, H=1, window=rng.choice((0, 50, 128)), layers=2, pages=30, plain=60), {}, [], 0
+    for turn in range(60):
+        what = rng.choice(("add", "step", "step", "step", "fork", "reorder", "free", "resize", "resize"))
+        if what == "add" and len(seqs) < 6:
+            seqs += cache.add(1)
+            for layer in range(2):
+                kept[seqs[-1], layer] = []
+        elif what == "step" and seqs:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            counts = [rng.choice((0, 1, 1, 2, 60, 130)) for _ in some]
+            if sum(-(-c // 64) + 1 for c in counts) > cache.free_pages()[1]:
+                cache.resize(plain_pages=400, pages=100)
+            step = feed(cache, some, counts, seed=100 + turn, kept=kept, commit=False)
+            if sum(counts):
+                q = rand((sum(counts), 2, 128), turn, BF)
+                check(step.attend(q, turn % 2), q, step, turn % 2)
+        elif what == "fork" and 0 < len(seqs) < 5:
+            if cache.free_pages()[1] < 1:
+                cache.resize(plain_pages=400, pages=100)
+            s = rng.choice(seqs)
+            seqs += cache.fork([s])
+            for layer in range(2):
+                kept[seqs[-1], layer] = list(kept[s, layer])
+        elif what == "reorder" and seqs:
+            if cache.free_pages()[1] < len(seqs):
+                cache.resize(plain_pages=400, pages=100)
+            parents = [rng.randrange(len(seqs)) for _ in seqs]
+            cache.reorder(seqs, parents)
+            kept = {(s, layer): list(kept[seqs[p], layer]) for s, p in zip(seqs, parents) for layer in range(2)}
+        elif what == "free" and len(seqs) > 1:
+            s = seqs.pop(rng.randrange(len(seqs)))
+            cache.free([s])
+            kept = {k: v for k, v in kept.items() if k[0] != s}
+        elif what == "resize":
+            cache.resize(*((None, None) if rng.random() < 0.5 else (100, 200)))
+        for s in seqs if turn % 5 == 4 else ():
+            pages, plain = cache.tables(s)
+            assert max(pages + [0]) < cache.packed_pages(0)[0].shape[0] and max(plain + [0]) < cache.plain_pages().shape[0]
+            for layer in range(2):
+                if not kept[s, layer]:
+                    continue
+                k, v = (torch.cat([t[i] for t in kept[s, layer]]).transpose(0, 1) for i in (0, 1))
+                n = 64 * len(pages)
+                assert cache.lengths([s]) == [k.shape[1]]
+                for side, comp in enumerate((cache.codec(layer).key_compressor, cache.codec(layer).val_compressor)):
+                    if n:
+                        want, views = comp.compress((k, v)[side][:, :n].unsqueeze(0)), cache.packed_pages(layer)
+                        assert torch.equal(views[2 * side][torch.tensor(pages, device=DEV)].transpose(0, 1).flatten(1, 2), want["idx_bytes"][0])
+                    held = cache.plain_pages()[plain, layer, side].transpose(0, 1).flatten(1, 2)[:, :k.shape[1] - n]
+                    assert torch.equal(held, (k, v)[side][:, n:])
+    cache.free(seqs)
+    cache.resize()
+    assert cache.free_pages() == (1, 1) and not cache._packed_of
 
 
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):

@@ -23,7 +23,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libtqamd.so")
 FAST_NAME = "tqamd_fastcall"        # extension module: the eager calls from tensors to the library in one step each
 FAST_SOURCE = "tq_fastcall.cpp"
-FAST_INTERFACE = 10                  # INTERFACE there: what init and the functions take and answer
+FAST_INTERFACE = 11                  # INTERFACE there: what init and the functions take and answer
 # (the ones that take longest to compile first)
 SOURCES = ("tq_decode_d256.hip", "tq_decode_d96.hip", "tq_decode_d64.hip", "tq_decode_d128_narrow.hip", "tq_decode_d128_wide.hip", "tq_compress.hip", "tq_decompress.hip",
            "tq_wide_d224.hip", "tq_wide_d192.hip", "tq_wide_d160.hip", "tq_wide_d96.hip", "tq_anydim.hip", "tq_attend.hip", "tq_qjl.hip",
@@ -963,8 +963,8 @@ def reorder(segments, parents: torch.Tensor, heads: int, device: torch.device) -
 
 
 def copy_pages(source: torch.Tensor, target: torch.Tensor, rows: int, row_bytes: int, sources, targets=None, sizes=None) -> None:
-    """tq_copy_pages: pages `sources` of one pool ([pages, ...]) into pages `targets` (default 0, 1, ...) of another, or of the same one; sizes: bytes of each row that are copied (default all)."""
-    status = fast().copy_pages(source, target, rows, row_bytes, sources, targets, sizes)
+    """tq_copy_pages: pages `sources` (a list, or an array of int32) of one pool ([pages, ...]) into pages `targets` (default 0, 1, ...) of another, or of the same one; sizes: bytes of each row that are copied (default all)."""
+    status = fast().copy_pages(source, target, rows, row_bytes, sources.tobytes() if isinstance(sources, np.ndarray) else sources, targets, sizes)
     if status is None:          # (another device is current)
         n = len(sources)
         pairs = np.empty((n, 3), dtype=np.int32)

@@ -16,13 +16,14 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <cstring>
 #include <vector>
 
 #include "../../include/tqamd.h"
 
 namespace {
 
-constexpr int INTERFACE = 10;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
+constexpr int INTERFACE = 11;      // of this module to _native.py (FAST_INTERFACE there): raised with any change of what init or a function takes or answers
 
 PyObject *g_workspace = nullptr, *g_drop_workspace = nullptr;      // _native's: ticket counters of (device, stream)
 PyObject *g_scratch = nullptr, *g_arrived = nullptr;               // _native's: (device index, stream) -> tensor
@@ -643,18 +644,21 @@ PyObject *put_tokens(PyObject *const *a) {
 }
 
 // copy_pages(source pool, target pool, rows, bytes between rows, source pages, target pages or None (0, 1, ...), bytes of a row that are copied or None (all)) -> status; lists of whole
-// numbers, which the caller answers for
+// numbers, which the caller answers for; source pages may be int32 in bytes
 PyObject *copy_pages(PyObject *const *a) {
     TENSOR(from, a[0]); TENSOR(to, a[1]);
     const long long rows = integer(a[2]), row_bytes = integer(a[3]);
-    NEED(PyList_CheckExact(a[4]) && (a[5] == Py_None || PyList_CheckExact(a[5])) && (a[6] == Py_None || PyList_CheckExact(a[6])) && from.dim() > 0 && to.dim() > 0 && from.device() == to.device());
-    const Py_ssize_t n = PyList_GET_SIZE(a[4]);
+    const bool raw = PyBytes_CheckExact(a[4]);
+    NEED((raw || PyList_CheckExact(a[4])) && (a[5] == Py_None || PyList_CheckExact(a[5])) && (a[6] == Py_None || PyList_CheckExact(a[6])) && from.dim() > 0 && to.dim() > 0 && from.device() == to.device());
+    const Py_ssize_t n = raw ? PyBytes_GET_SIZE(a[4]) / (Py_ssize_t)sizeof(int32_t) : PyList_GET_SIZE(a[4]);
     NEED((a[5] == Py_None || PyList_GET_SIZE(a[5]) == n) && (a[6] == Py_None || PyList_GET_SIZE(a[6]) == n));
     const Stream s(from);
     NEED(s.ok);
     std::vector<tq_page_pair> pairs((size_t)n);
     for (Py_ssize_t i = 0; i < n; ++i) {
-        const long long v[3] = {integer(PyList_GET_ITEM(a[4], i)), a[5] == Py_None ? (long long)i : integer(PyList_GET_ITEM(a[5], i)), a[6] == Py_None ? row_bytes : integer(PyList_GET_ITEM(a[6], i))};
+        int32_t own = 0;
+        if (raw) std::memcpy(&own, PyBytes_AS_STRING(a[4]) + i * (Py_ssize_t)sizeof(int32_t), sizeof(int32_t));
+        const long long v[3] = {raw ? own : integer(PyList_GET_ITEM(a[4], i)), a[5] == Py_None ? (long long)i : integer(PyList_GET_ITEM(a[5], i)), a[6] == Py_None ? row_bytes : integer(PyList_GET_ITEM(a[6], i))};
         for (long long x : v) NEED(x >= 0 && x <= 0x7fffffff);
         NEED(v[0] < from.size(0) && v[1] < to.size(0));
         pairs[(size_t)i] = {(int32_t)v[0], (int32_t)v[1], (int32_t)v[2]};

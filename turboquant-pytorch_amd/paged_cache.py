@@ -39,11 +39,36 @@ MAX_JOBS = 4096                     # TQ_MAX_JOBS of include/tqamd.h
 
 
 class _Pages:
-    """Numbers of the pages of a pool: which are free, and how many sequences hold each of the others.  The lowest free one goes first."""
+    """Numbers of the pages of a pool: which are free, and how many sequences hold each of the others.  The lowest free one goes first.  A page keeps its number when it is moved into
+    another pool: `places` has where it lies there (None: every page lies at its number)."""
 
     def __init__(self, count: int):
         self.free = list(range(count))
-        self.held = [0] * count
+        self.held = array("i", bytes(4 * count))
+        self.places: Optional[np.ndarray] = None
+
+    def numbers(self) -> np.ndarray:
+        """Of the pages that are held."""
+        return np.flatnonzero(np.frombuffer(self.held, dtype=np.int32))
+
+    def lie(self, pages: np.ndarray) -> np.ndarray:
+        """Where pages lie."""
+        return pages if self.places is None else self.places[pages]
+
+    def gathered(self, numbers: np.ndarray, size: int) -> "_Pages":
+        """What becomes of these pages in a pool of `size` that has the held ones (`numbers`) at its beginning."""
+        new, n, known = _Pages(0), len(numbers), len(self.held)
+        free = np.flatnonzero(np.frombuffer(self.held, dtype=np.int32) == 0)[:size - n]
+        if len(free) < size - n:
+            free = np.concatenate((free, np.arange(known, known + size - n - len(free))))
+        new.free = free.tolist()
+        new.held = self.held[:]
+        new.held.extend([0] * (1 + max(numbers[-1] if n else 0, free[-1] if len(free) else 0) - known))
+        if n and numbers[-1] != n - 1:
+            new.places = np.zeros(len(new.held), dtype=np.int32)
+            new.places[numbers] = np.arange(n, dtype=np.int32)
+            new.places[free] = np.arange(n, size, dtype=np.int32)
+        return new
 
     def take(self) -> int:
         page = heapq.heappop(self.free)
@@ -165,7 +190,7 @@ class PagedV3Cache:
     def tables(self, seq: int) -> Tuple[List[int], List[int]]:
         """Numbers of a sequence's packed and uncompressed pages, in the order of its tokens."""
         s = self._sequence(seq)
-        return list(s.pages), list(s.plain)
+        return tuple(pool.lie(np.array(of, dtype=np.int32)).tolist() for pool, of in ((self._packed_pages, s.pages), (self._plain_pages, s.plain)))
 
     def lengths(self, seqs: Sequence[int]) -> List[int]:
         """Tokens of sequences, those of an open step among them."""
@@ -294,16 +319,20 @@ class PagedV3Cache:
         sources: List[int] = []
         targets: List[int] = []
         sizes: List[int] = []
+        held, free, take = pool.held, pool.free, heapq.heappop
         for s in sharing:
             filled = s.total % P
             if filled:
                 page = s.plain[-1]
-                s.plain[-1] = target = pool.take()
-                pool.drop(page)                  # (its owner still holds it)
+                s.plain[-1] = target = take(free)
+                held[target] = 1
+                held[page] -= 1                  # (its owner still holds it)
                 sources.append(page)
                 targets.append(target)
                 sizes.append(filled * vector)
         if sources:
+            if pool.places is not None:
+                sources, targets = (pool.places[pages].tolist() for pages in (sources, targets))
             _native.copy_pages(self._plain, self._plain, self.n_layers * 2 * self.kv_heads, P * vector, sources, targets, sizes)
 
     def fork(self, seqs: Sequence[int]) -> List[int]:
@@ -370,51 +399,26 @@ class PagedV3Cache:
         return chosen
 
     def resize(self, pages: Optional[int] = None, plain_pages: Optional[int] = None) -> None:
-        """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered, sequence after sequence."""
+        """Pools of other sizes (default: just what is held, one page at least), into which the pages that are held are gathered (`tables` says where they lie then)."""
         self._eager("resize")
         self._settle()
-        # the pages that are held, as the sequences have them: a page's place here is its number in the new pool
-        states = list(self._seqs.values())
-        flat = [np.frombuffer(b"".join([getattr(s, side) for s in states]), dtype=np.int32) for side in ("pages", "plain")]
-        orders = [list(dict.fromkeys(of.tolist())) for of in flat]
-        held = [len(order) for order in orders]
+        # (sequences' tables have numbers, which stay: what a gather costs the host does not depend on how many sequences there are)
+        kept = self._packed_pages.numbers(), self._plain_pages.numbers()
         sizes = []
-        for name, asked, n in zip(("pages", "plain_pages"), (pages, plain_pages), held):
+        for name, asked, n in zip(("pages", "plain_pages"), (pages, plain_pages), map(len, kept)):
             size = max(1, n) if asked is None else asked
             if isinstance(size, bool) or int(size) != size or size < max(1, n):
                 raise ValueError(f"resize: {name} must be a whole number, {max(1, n)} or more (as many are held); got {size!r}")
             sizes.append(int(size))
         pool, plain = self._pools(*sizes)
         stream, vector = torch.cuda.current_stream(self.device), self.head_dim * self._plain.element_size()
-        for source, target, order, rows, row_bytes in ((self._pool, pool, orders[0], 1, self._page_bytes),
-                                                       (self._plain, plain, orders[1], self.n_layers * 2 * self.kv_heads, self.page_tokens * vector)):
-            if order:
-                _native.copy_pages(source, target, rows, row_bytes, order)
+        for source, target, of, numbers, rows, row_bytes in ((self._pool, pool, self._packed_pages, kept[0], 1, self._page_bytes),
+                                                             (self._plain, plain, self._plain_pages, kept[1], self.n_layers * 2 * self.kv_heads, self.page_tokens * vector)):
+            if len(numbers):
+                _native.copy_pages(source, target, rows, row_bytes, of.lie(numbers).astype(np.int32))
             source.record_stream(stream)         # (what it was allocated on may be another one)
         self._pool, self._plain, self._views, self._layers = pool, plain, None, [None] * self.n_layers
-        # (the copies run while the tables are brought in line)
-        pools, numbers, tables = [], [], []
-        for old, of, order, n, size in zip((self._packed_pages, self._plain_pages), flat, orders, held, sizes):
-            new = _Pages(0)
-            new.held = [old.held[p] for p in order] + [0] * (size - n)
-            new.free = list(range(n, size))
-            pools.append(new)
-            number = np.zeros(len(old.held), dtype=np.int32)
-            number[order] = np.arange(n, dtype=np.int32)
-            numbers.append(number)
-            tables.append(array("i", number[of].tobytes()))
-        packed_at = plain_at = 0
-        for s in states:
-            k, n = len(s.pages), len(s.plain)
-            if k:
-                s.pages = tables[0][packed_at:packed_at + k]
-                packed_at += k
-            if n:
-                s.plain = tables[1][plain_at:plain_at + n]
-                plain_at += n
-        self._packed_pages, self._plain_pages = pools
-        if self._packed_of:
-            self._packed_of = {int(numbers[1][p]): int(numbers[0][q]) for p, q in self._packed_of.items()}
+        self._packed_pages, self._plain_pages = (of.gathered(numbers, size) for of, numbers, size in zip((self._packed_pages, self._plain_pages), kept, sizes))
 
     # ---- steps ----------------------------------------------------------------------------------------------------------------
     def step(self, seqs: Sequence[int], counts) -> "PagedStep":
@@ -460,7 +464,7 @@ class PagedStep:
     def _begin(self) -> None:
         """Pages for the new tokens, and the tables of all sequences onto the card."""
         cache, P = self.cache, self.cache.page_tokens
-        records, tables, singles, slots, at, begin = [], [], [], [], 0, 0
+        records, packed, plain, singles, slots, at, packed_at, plain_at = [], [], [], [], [], 0, 0, 0
         rest = (0,) * (_native.PAGED_SEQ - 6)
         for s, c, n in zip(self._states, self.counts, self._pages_taken):
             held = len(s.pages)
@@ -475,13 +479,20 @@ class PagedStep:
                 places = np.arange(first, first + c)
                 slots += [np.array(singles, dtype=np.int64), np.array(s.plain, dtype=np.int64)[places // P] * P + places % P]
                 singles = []
-            records += (at, c, s.total, held * P, begin, begin + held, *rest)
-            tables += [s.pages, s.plain]
-            begin += held + len(s.plain)
+            records += (at, c, s.total, held * P, packed_at, plain_at, *rest)
+            packed.append(s.pages)
+            plain.append(s.plain)
+            packed_at += held
+            plain_at += len(s.plain)
             at += c
         slots.append(np.array(singles, dtype=np.int64))
         self._records = np.array(records, dtype=np.int32).reshape(len(self.seqs), _native.PAGED_SEQ)
-        self._sections = [self._records.ravel(), np.frombuffer(b"".join(tables), dtype=np.int32), np.concatenate(slots).astype(np.int32)]
+        self._records[:, 5] += packed_at     # (plain pages' numbers lie behind those of all packed ones)
+        tables, slots = np.frombuffer(b"".join(packed + plain), dtype=np.int32), np.concatenate(slots)
+        if cache._packed_pages.places is not None or cache._plain_pages.places is not None:
+            tables = np.concatenate((cache._packed_pages.lie(tables[:packed_at]), cache._plain_pages.lie(tables[packed_at:])))
+            slots = cache._plain_pages.lie(slots // P) * np.int64(P) + slots % P
+        self._sections = [self._records.ravel(), tables, slots.astype(np.int32)]
         self._blob, (self._seq_at, self._table_at, self._slot_at) = self._upload(self._sections)
 
     def _take_back(self) -> None:
@@ -702,7 +713,8 @@ class PagedStep:
                 moves.append((s, pages))
         try:
             if becomes:
-                self._pack(np.asarray(list(becomes.items()), dtype=np.uint64))
+                made = np.array(list(becomes.items()))
+                self._pack(np.stack((c._plain_pages.lie(made[:, 0]), c._packed_pages.lie(made[:, 1])), 1).astype(np.uint64))
         except BaseException:                # (tables stay as they were)
             for _, pages in moves:
                 c._packed_pages.drop_all(pages)
