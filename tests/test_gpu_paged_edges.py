@@ -235,6 +235,28 @@ def test_gathers_between_all_other_calls(pkg, seed):
     assert cache.free_pages() == (1, 1) and not cache._packed_of
 
 
+def test_a_layer_that_was_not_appended_to_is_not_attended_to(pkg):
+    cache = make(pkg, H=2, layers=3)
+    seqs = cache.add(2)
+    feed(cache, seqs, (100, 7), seed=1)
+    step = cache.step(seqs, (1, 3))
+    k, v, q = states(4, 2, 128, 1, BF), states(4, 2, 128, 2, BF), rand((4, 8, 128), 3, BF)
+    # tokens that the caller puts into the pages himself
+    at = [(cache.tables(s)[1][p // 64], p % 64) for s, places in zip(seqs, ((100 - 64 * len(cache.tables(seqs[0])[0]),), (7, 8, 9))) for p in places]
+    for i, (page, place) in enumerate(at):
+        cache.plain_pages()[page, 0, 0, :, place], cache.plain_pages()[page, 0, 1, :, place] = k[i], v[i]
+    want = step.attend(q, 0)
+    check(want, q, step)
+    step.append(k, v, 0)
+    assert torch.equal(step.attend(q, 0), want)
+    for layer in (1, 2):
+        with pytest.raises(RuntimeError, match="appended"):
+            step.attend(q, layer)
+        step.append(k, v, layer)
+        check(step.attend(q, layer), q, step, layer)
+    step.commit()
+
+
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):
     for dtype, D, G, new in ((BF, 128, 4, 1), (F16, 64, 4, 2), (BF, 128, 4, 33), (F16, 128, 4, 33), (BF, 80, 2, 17), (F32, 128, 2, 9), (BF, 256, 4, 1), (F16, 256, 2, 20)):
         cache = make(pkg, D, 2, dtype, 4, 2 if D != 80 else 4, 30)

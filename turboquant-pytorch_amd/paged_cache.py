@@ -570,8 +570,8 @@ class PagedStep:
                 raise ValueError(f"append: {name} must be {list(shape)} {c.dtype}, got {tuple(t.shape)} {t.dtype}")
             if t.device != c.device:
                 raise _native.TqError(f"append: {name} on {t.device}, the cache on {c.device}")
-        self._appended.add(layer)
         if not self.tokens:
+            self._appended.add(layer)
             return
         keys, values = (t if t.stride(2) == 1 and min(t.stride()) >= 0 else t.contiguous() for t in (keys, values))
         es = keys.element_size()
@@ -581,6 +581,7 @@ class PagedStep:
             _native.check(_native.lib().tq_put_tokens(keys.data_ptr(), values.data_ptr(), keys.stride(0) * es, keys.stride(1) * es, values.stride(0) * es, values.stride(1) * es,
                                                       pool.data_ptr(), pool.stride(0) * es, pool.stride(1) * es, self._slot_at, self.tokens, c.kv_heads, c.head_dim * es, c.page_tokens,
                                                       _native._stream_handle(c.device)), "tq_put_tokens")
+        self._appended.add(layer)
 
     def _plan(self, group: int, window: int) -> tuple:
         """How the blocks of the attention share the step's work, on the card: (counts, items, merges, scratch)."""
@@ -624,9 +625,10 @@ class PagedStep:
         """softmax(z) V of the new tokens' queries, [new tokens, query heads, D] -> the same shape and type: a new token sees everything its sequence holds before it and itself.
         Query head j uses kv head j // (query heads / kv heads).  z = scale * q . k (scale: D ** -0.5 by default), as softcap * tanh(z / softcap) if softcap (up to 1024 for 16-bit elements) is given, less
         slopes[query head] * distance if slopes (float [query heads]) are; sliding_window: only the last so many tokens, the new one among them, are seen.
-        Every layer has to be appended to before (the step's own tokens are read from its pages).  Not differentiable."""
-        ready = self._quick.get(sliding_window)
-        if ready is not None and not self._done and type(layer_idx) is int and 0 <= layer_idx < self.cache.n_layers and not torch.compiler.is_compiling():
+        The layer has to be appended to before (the step's own tokens are read from its pages); of a step that no layer has been appended to, it is what the caller has written there itself.
+        Not differentiable."""
+        ready, appended = self._quick.get(sliding_window), self._appended
+        if ready is not None and not self._done and type(layer_idx) is int and 0 <= layer_idx < self.cache.n_layers and (layer_idx in appended or not appended) and not torch.compiler.is_compiling():
             # as the call before with this window, if the queries are laid out for it
             out = _native.fast().paged_attend(ready[0], self.cache._layer(layer_idx)[0], queries, self.tokens, self.cache.head_dim ** -0.5 if scale is None else scale, softcap, slopes, ready[1], ready[2], ready[3])
             if out is not None:
@@ -641,6 +643,8 @@ class PagedStep:
         """`attend` with every check."""
         self._live("attend")
         c, layer = self.cache, self._layer(layer_idx)
+        if self._appended and layer not in self._appended and self.tokens:
+            raise RuntimeError(f"attend: layer {layer} has not been appended to in this step")
         if queries.dim() != 3 or queries.shape[0] != self.tokens or queries.shape[2] != c.head_dim or queries.shape[1] == 0 or queries.shape[1] % c.kv_heads or queries.dtype != c.dtype:
             raise ValueError(f"attend: queries must be [{self.tokens}, k * {c.kv_heads}, {c.head_dim}] {c.dtype}, got {tuple(queries.shape)} {queries.dtype}")
         if queries.device != c.device:
