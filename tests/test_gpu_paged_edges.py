@@ -7,7 +7,8 @@ from importlib import import_module
 import pytest
 import torch
 
-from test_gpu_paged import BF, F16, F32, check, feed, make, rand, states
+from test_gpu_many import HALF
+from test_gpu_paged import BF, F16, F32, check, contents, feed, make, rand, states
 from test_gpu_parity import DEV
 
 pytestmark = pytest.mark.gpu
@@ -31,23 +32,24 @@ def test_packed_vectors_that_are_no_numbers_stay_with_those_who_see_them(pkg, D,
     feed(cache, seqs, (n, 390), seed=1)
     step = feed(cache, seqs, (new, new), seed=2, commit=False)
     q = rand((2 * new, 2 * G, D), 3, dtype)
-    want = step.attend(q, 0, sliding_window=W)
-    check(want, q, step, sliding_window=W)
     norms = cache.packed_pages(0)[side]
-    # a norm of its first kv head that the first `seen` of the new tokens see: none, the token just outside the window or further out; some
-    for seen in sorted({-45, -20, 0, new // 2}):
-        t = n - W + seen
-        at = cache.tables(seqs[0])[0][t // P], 0, t % P
-        for value in (float("inf"), float("nan")):
-            kept = norms[at].clone()
-            norms[at] = value
-            got = step.attend(q, 0, sliding_window=W)
-            norms[at] = kept
-            if seen > 0:
-                if side == 3 or value != value:          # (an infinite key may be one that nobody likes)
-                    assert not bool(torch.isfinite(got[:seen, :G]).any())
-                got[:seen, :G] = want[:seen, :G]
-            check(got, q, step, sliding_window=W)
+    for kw in ({"sliding_window": W}, {"sliding_window": W, "softcap": 20.0, "slopes": torch.linspace(0.01, 0.1, 2 * G, device=DEV)}):
+        want = step.attend(q, 0, **kw)
+        check(want, q, step, **kw)
+        # a norm of its first kv head that the first `seen` of the new tokens see: none, the token just outside the window or further out; some
+        for seen in sorted({-45, -20, 0, new // 2}):
+            t = n - W + seen
+            at = cache.tables(seqs[0])[0][t // P], 0, t % P
+            for value in (float("inf"), float("nan")):
+                kept = norms[at].clone()
+                norms[at] = value
+                got = step.attend(q, 0, **kw)
+                norms[at] = kept
+                if seen > 0:
+                    if side == 3 or value != value:          # (an infinite key may be one that nobody likes)
+                        assert not bool(torch.isfinite(got[:seen, :G]).any())
+                    got[:seen, :G] = want[:seen, :G]
+                check(got, q, step, **kw)
 
 
 def recorded(pkg):
@@ -255,6 +257,33 @@ def test_a_layer_that_was_not_appended_to_is_not_attended_to(pkg):
         step.append(k, v, layer)
         check(step.attend(q, layer), q, step, layer)
     step.commit()
+
+
+@pytest.mark.parametrize("dtype,size", [(BF, 1e2), (BF, 1e4), (BF, 1e18), (F16, 1e2), (F16, 2e3), (F32, 1e3), (F32, 1e6), (F32, 1e18)])
+@pytest.mark.parametrize("D,new", [(128, 1), (128, 5), (64, 40), (256, 1), (80, 7)])
+def test_a_query_far_along_one_key_has_its_value(pkg, dtype, size, D, new):
+    """Logits so large that one token has all of the weight: what the others are behind by is more than both are off by (the delta of test_gpu_paged, twice), and 40 more, so that their weights are below
+    2^-57 together with how many there are."""
+    kb, vb = (4, 4) if D == 80 else (4, 2)
+    cache = make(pkg, D, 1, dtype, kb, vb, 20)
+    (seq,) = cache.add(1)
+    feed(cache, [seq], (500,), seed=1)
+    step = feed(cache, [seq], (new,), seed=3, commit=False)
+    k, v = (t[0] for t in contents(cache, seq))
+    u, u_v = (2.0 ** -11 if dtype == BF else 2.0 ** -20) + D * 2.0 ** -24, 2.0 ** -10 if dtype != F32 else 2.0 ** -18
+    unit = k / k.norm(dim=-1, keepdim=True)
+    gap = (unit @ k.T).clone()
+    gap = gap.diagonal() - gap.masked_fill(torch.eye(len(k), dtype=torch.bool, device=DEV), float("-inf")).amax(-1)
+    # the packed token and the uncompressed one that stand out most
+    old = 64 * len(cache.tables(seq)[0])
+    for t in (int(gap[:old].argmax()), old + int(gap[old:500].argmax())):
+        q = (size * unit[t]).to(dtype)
+        z = (k @ q.double()) * D ** -0.5
+        delta = u * D ** -0.5 * q.double().norm() * k.norm(dim=-1).amax()
+        others = torch.cat((z[:t], z[t + 1:])).amax()
+        assert float(z[t] - others - 2 * delta) >= 40.0
+        out = step.attend(q.expand(new, 2, D).contiguous(), 0).double()
+        assert float(((out - v[t]).norm(dim=-1) / v[t].norm()).max()) <= HALF[dtype] + u_v
 
 
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):
