@@ -243,7 +243,7 @@ def test_a_layer_that_was_not_appended_to_is_not_attended_to(pkg):
     feed(cache, seqs, (100, 7), seed=1)
     step = cache.step(seqs, (1, 3))
     k, v, q = states(4, 2, 128, 1, BF), states(4, 2, 128, 2, BF), rand((4, 8, 128), 3, BF)
-    # tokens that the caller puts into the pages himself
+    # tokens that go into the pages without append
     at = [(cache.tables(s)[1][p // 64], p % 64) for s, places in zip(seqs, ((100 - 64 * len(cache.tables(seqs[0])[0]),), (7, 8, 9))) for p in places]
     for i, (page, place) in enumerate(at):
         cache.plain_pages()[page, 0, 0, :, place], cache.plain_pages()[page, 0, 1, :, place] = k[i], v[i]

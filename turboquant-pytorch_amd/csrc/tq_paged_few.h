@@ -121,7 +121,7 @@ struct FewPlain {
 // A block takes items of the plan in turn, each a share of what the queries of a (sequence, kv head) see; the tables stay in LDS.  Up to 16 / C query vectors are the columns of 16 x 16 x 32 products, C times over, so that C blocks of 16 tokens share a softmax: every block's
 // scores are made for all columns, a lane keeps those of its own column's block, and the weights of the others are zeros in its column of the value product (as in tq_decode_kernel, whose
 // loop this is, with runs found through the sequence's pages: a run lies within a page, whose number is fetched a run ahead).  QT: fp16 terms of a rotated query, one for bfloat16 (two then, and two of the levels, for float16: with one the result of half a unit's
-// rounding, 2.1e-4, came out at 6e-4).
+// rounding, 2.1e-4, came out at 6e-4.  Weights, their products with norms and value levels keep one: 3.0e-4; second ones would be two more value products and tables of two words).
 // Base-2 logits are rounded before the reference is taken off, so that the largest ones stay exact against it however large they are.
 template <int D, int IPBK, int IPBV, int C, bool BF>
 __global__ __launch_bounds__(DTHREADS, DW / 4) void tq_paged_few_kernel(TqPagedArgs a) {
