@@ -286,6 +286,28 @@ def test_a_query_far_along_one_key_has_its_value(pkg, dtype, size, D, new):
         assert float(((out - v[t]).norm(dim=-1) / v[t].norm()).max()) <= HALF[dtype] + u_v
 
 
+@pytest.mark.parametrize("D,G,dtype,P", [(128, 4, BF, 64), (64, 2, F16, 64), (256, 4, BF, 64), (80, 2, BF, 64), (128, 2, F32, 64), (128, 4, F16, 32)])
+def test_logits_that_are_all_minus_infinity_make_no_number(pkg, D, G, dtype, P):
+    cache = make(pkg, D, 1, dtype, 4, 4, 64, P=P)
+    seqs = cache.add(3)
+    feed(cache, seqs, (300, 0, 0), seed=1)
+    for counts in ((1, 1, 1), (1, 20, 1)):
+        step = cache.step(seqs, counts)
+        k, v, q = states(sum(counts), 1, D, 2, dtype), states(sum(counts), 1, D, 3, dtype), rand((sum(counts), G, D), 4, dtype)
+        q[..., 3] = q[..., 3].abs() + 1
+        k[1], k[2] = 0.0, 0.0
+        k[1, 0, 3] = k[2, 0, 3] = float("-inf")          # (its queries' logits: -infinity; of the second sequence the first token alone or the first two, of the first one none)
+        step.append(k, v, 0)
+        for kw in ({}, {"sliding_window": 1}):
+            out = step.attend(q, 0, **kw)
+            nothing = torch.zeros(sum(counts), dtype=torch.bool, device=DEV)
+            nothing[1:3 if sum(counts) > 3 else 2] = True
+            if sum(counts) == 3:
+                nothing[2] = True                        # (the third sequence's only token is the other one)
+            assert bool(torch.isnan(out[nothing]).all()) and bool(torch.isfinite(out[~nothing]).all())
+        step.cancel()
+
+
 def test_queries_that_are_no_numbers_stay_by_themselves(pkg):
     for dtype, D, G, new in ((BF, 128, 4, 1), (F16, 64, 4, 2), (BF, 128, 4, 33), (F16, 128, 4, 33), (BF, 80, 2, 17), (F32, 128, 2, 9), (BF, 256, 4, 1), (F16, 256, 2, 20)):
         cache = make(pkg, D, 2, dtype, 4, 2 if D != 80 else 4, 30)

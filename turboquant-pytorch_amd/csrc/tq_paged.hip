@@ -52,11 +52,11 @@ __global__ __launch_bounds__(MERGE_THREADS) void tq_paged_merge_kernel(TqPagedAr
             for (int e = 0; e < 4; ++e) o[e] = fmaf(x[k][e], f, o[e]);
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = 1.0f / sum;            // (a query sees its own token: a sum of zero is that of logits which are all -infinity, and 0 / 0 the result)
     const uint32_t token = m / a.group;
     const size_t first = ((size_t)((uint32_t)sq[0] + token) * (a.heads * a.group) + kv * a.group + (m - token * a.group)) * a.D + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = inv == 0.f ? 0.f : o[e] * inv;
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
     if (a.dtype == TQ_F32) {
         TQ_GLOBAL float *out = reinterpret_cast<TQ_GLOBAL float *>((TQ_GLOBAL uint8_t *)a.out) + first;
 #pragma unroll

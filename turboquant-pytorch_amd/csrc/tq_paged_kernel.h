@@ -417,7 +417,7 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedC
     // (no largest logit: no token seen, or logits that are all NaN, which the sum of weights tells)
     const float f0 = j.m0 != MANY_NONE ? __builtin_amdgcn_exp2f(j.m0 - m) : j.l0 == 0.f ? 0.f : __builtin_nanf("");
     const float f1 = j.m1 != MANY_NONE ? __builtin_amdgcn_exp2f(j.m1 - m) : j.l1 == 0.f ? 0.f : __builtin_nanf("");
-    const float l = j.l0 * f0 + j.l1 * f1, inv = l == 0.f ? 0.f : 1.0f / l;
+    const float l = j.l0 * f0 + j.l1 * f1, inv = 1.0f / l;         // (of a result a query's own token is part: a sum of zero is that of logits which are all -infinity, and 0 / 0 what comes of it)
     tq_f16v acc = tq_zero16();
     float back = 0.f;
     if (packed) {
@@ -459,7 +459,7 @@ __device__ __forceinline__ void paged_finish(const TqPagedArgs &a, const JoinedC
     for (int r = 0; r < 16; ++r) out[r] = (packed ? acc[r] * back : 0.f) + (plain ? j.plain[d0 + r] * f1 : 0.f);
     if (!rec) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) out[r] = inv == 0.f ? 0.f : out[r] * inv;
+        for (int r = 0; r < 16; ++r) out[r] *= inv;
         paged_store(a, q_first, kv, q, d0, out);
         return;
     }
